@@ -84,9 +84,9 @@ def draw(rng):
     return dict(c, group=group, page=page)
 
 
-#: base, and what the scaling takes: factor, original length, and the two limits of a blend
+#: base, and what the scaling takes: factor, original length, and how often a plane turns within that to be kept, or at most to be stretched
 BASE, FACTOR, ORIGINAL = 10000.0, 8.0, 4096
-LIMITS = {"yarn": (32.0, 1.0), "wavelength": (1.0, 4.0)}
+LIMITS = {"yarn": (32.0, 1.0), "wavelength": (4.0, 1.0)}
 
 
 def _lengths(case):
@@ -131,16 +131,16 @@ def _frequencies(case):
         ramp = ((i - lo) / max(hi - lo, 0.001)).clamp(0, 1)
         f = f * (1 - ramp) + f / FACTOR * ramp
     elif scaling == "wavelength":
-        low, high = LIMITS["wavelength"]
-        keep = ((ORIGINAL * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        most, least = LIMITS["wavelength"]
+        keep = ((ORIGINAL * f / (2 * math.pi) - least) / (most - least)).clamp(0, 1)
         f = f * keep + f / FACTOR * (1 - keep)
     return f, (0.1 * math.log(FACTOR) + 1.0 if scaling == "yarn" else 1.0)
 
 
 def _rotary_table(lib, case):
     s = case["scaling"]
-    low, high = LIMITS.get(s, (0.0, 0.0))
-    return lib.RotaryTable(case["rd"], base=BASE, scaling=s, factor=FACTOR, original_length=ORIGINAL, low=low, high=high)
+    keep, stretch = LIMITS.get(s, (0.0, 0.0))
+    return lib.RotaryTable(case["rd"], base=BASE, scaling=s, factor=FACTOR, original_length=ORIGINAL, keep_turns=keep, stretch_turns=stretch)
 
 
 def _empty_cache(pages, heads, page, d, group):
@@ -325,8 +325,8 @@ def _exact_rotary(case, x, positions):
             f = f + part * (f / FACTOR - f)
         elif s == "wavelength":
             turns = ORIGINAL * f / (2 * math.pi)
-            low, high = LIMITS[s]
-            part = 0.0 if turns <= low else 1.0 if turns >= high else (turns - low) / (high - low)
+            most, least = LIMITS[s]
+            part = 0.0 if turns <= least else 1.0 if turns >= most else (turns - least) / (most - least)
             f = f / FACTOR + part * (f - f / FACTOR)
         planes.append(f)
     angle = positions.double().unsqueeze(1) * torch.tensor(planes, dtype=torch.float64, device="cuda")
