@@ -219,10 +219,12 @@ def prepare(case, seed):
 # ---- the plain forms ---------------------------------------------------------------------------------------------
 
 def _quantize(x, group):
-    """int8 values and fp16 scales: the largest magnitude of a group is 127 steps."""
+    """int8 values and fp16 scales: a group's largest magnitude is 127 steps, or barely less, since the scale is rounded up."""
     x = x.float().unflatten(-1, (-1, group))
-    scale = (x.abs().amax(-1, keepdim=True) / 127).to(torch.float16).clamp_min(2.0 ** -24)
-    q = torch.round(x / scale.float()).clamp(-127, 127).to(torch.int8)
+    step = x.abs().amax(-1, keepdim=True) / 127
+    scale = step.to(torch.float16)
+    scale = (scale.view(torch.int16) + (scale.float() < step)).view(torch.float16).clamp_min(2.0 ** -24)
+    q = torch.round(x / scale.float()).to(torch.int8)
     return q.flatten(-2), scale.squeeze(-1)
 
 
@@ -339,10 +341,13 @@ def _exact_rotary(case, x, positions):
 
 
 def _exact_stored(x, group):
-    """What is read back for x (fp16): whole multiples of a group's scale, which is held in fp16."""
+    """What is read back for x (fp16): whole multiples of a group's scale, the smallest fp16 that puts the group within 127 of them."""
     y = x.double().reshape(*x.shape[:-1], -1, group)
-    scale = torch.clamp((y.abs().amax(-1, keepdim=True) / 127).half().double(), min=2.0 ** -24)
-    return (torch.clamp(torch.round(y / scale), -127, 127) * scale).reshape(x.shape)
+    least = y.abs().amax(-1, keepdim=True).cpu().numpy() / 127
+    scale = least.astype(np.float16)
+    scale = np.where(scale < least, np.nextafter(scale, np.float16(np.inf)), scale).astype(np.float64)
+    scale = torch.from_numpy(np.maximum(scale, 2.0 ** -24)).cuda()
+    return (torch.round(y / scale) * scale).reshape(x.shape)
 
 
 def exact(case, seed):
