@@ -676,3 +676,7 @@ def stream_read_probe(sizes=(16 << 20, 48 << 20, 384 << 20), pool_bytes=1536 << 
         med = times[len(times) // 2]
         out["%d MiB" % (size >> 20)] = {"us": round(med, 2), "gb_per_s": round(size / (med * 1e-6) / 1e9, 1)}
     return out
+
+
+from .attention import (PagedDecodeAttention, PagedKVCache, RotaryTable, kv_cache_read, kv_cache_write,  # noqa: E402,F401
+                        rotary_fp16, rotary_kv_cache_write)
