@@ -249,8 +249,15 @@ def test_read_takes_a_slot_several_times(cuda, pplb200):
 
 # ---- attention -------------------------------------------------------------------------------------------------------
 
-def _attention(cuda, q, k, v, seen, scale):
-    """One sequence in 64 bits: q [hq, d], k, v [tokens, hk, d] as they are read back, seen [tokens] -> out, lse and the bounds of both."""
+def _stored(cuda, cache, slots):
+    """(k, v) [tokens, heads, d] in 64 bits, what is stored at the slots: fp16, or whole numbers times scales."""
+    rows = [None if t is None else _rows(t, slots, cache.page_size).double() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    return [x if s is None else x * s.repeat_interleave(cache.quant_group, -1) for x, s in (rows[::2], rows[1::2])]
+
+
+def _attention(cuda, q, k, v, seen, scale, values_rounded=False):
+    """One sequence in 64 bits: q [hq, d], k, v [tokens, hk, d], seen [tokens] -> out, lse and the bounds of both.  values_rounded: whole
+    numbers times scales of groups of eight dimensions are rounded to fp16 before they are weighted."""
     hq, d = q.shape
     shared = hq // k.shape[1]
     out, lse = cuda.zeros((hq, d), dtype=cuda.float64, device="cuda"), cuda.full((hq,), -math.inf, dtype=cuda.float64, device="cuda")
@@ -267,6 +274,9 @@ def _attention(cuda, q, k, v, seen, scale):
     off = size * (d + 8) * 2.0 ** -24 + 2.0 ** -20
     # a weight: that as a relative error (twice: the sum of the weights has it too), its rounding to fp16, sums over tokens in 32 bits
     weight = 2 * off + HALF + 2.0 ** -14
+    if values_rounded:
+        weight += HALF
+        bound += TINY
     bound += out.abs() * HALF + weight[:, None] * cuda.einsum("ht,thd->hd", p, v.abs()) * (1 + HALF)
     return out, lse, bound, off + 2.0 ** -14 + lse.abs() * 2.0 ** -22
 
@@ -295,7 +305,7 @@ def _run_attention(cuda, pplb200, lengths, hq, hk, d, page, group, order="heads"
         k, v = _randn(cuda, g, n, hk, d), _randn(cuda, g, n, hk, d)
         if n:
             pplb200.kv_cache_write(cache, k, v, slots)
-        written.append(pplb200.kv_cache_read(cache, slots) if n else (k, v))
+        written.append(_stored(cuda, cache, slots) if n else (k, v))
     for b, i, value in holes:
         table[b, i] = value
     lens = cuda.tensor(lengths, dtype=cuda.int32, device="cuda")
@@ -308,7 +318,7 @@ def _run_attention(cuda, pplb200, lengths, hq, hk, d, page, group, order="heads"
         at = cuda.arange(n, device="cuda")
         page_of = table[b].long()[at // page] if n else at
         seen = (page_of >= 0) & (page_of < pages) & ((at >= n - window) if window else (at >= 0))
-        want.append(_attention(cuda, q[b], *written[b], seen, att.scale))
+        want.append(_attention(cuda, q[b], *written[b], seen, att.scale, group == 8))
     return out, got_lse, want, (att, q, table, lens, cache)
 
 
@@ -391,7 +401,7 @@ def test_attention_scores_that_rise_or_fall(cuda, pplb200, rising, group):
     ramp = cuda.linspace(0, 60, n, device="cuda")
     k[:, 0, 0] = (ramp if rising else ramp.flip(0)).to(cuda.float16)
     pplb200.kv_cache_write(cache, k, v, cuda.arange(n, device="cuda"))
-    kr, vr = pplb200.kv_cache_read(cache, cuda.arange(n, device="cuda"))
+    kr, vr = _stored(cuda, cache, cuda.arange(n, device="cuda"))
     q = cuda.zeros((1, 4, d), dtype=cuda.float16, device="cuda")
     q[0, :, 0] = cuda.tensor([1.0, 4.0, -4.0, 0.0])
     table = cuda.arange(125, dtype=cuda.int32, device="cuda")[None]
@@ -561,7 +571,7 @@ def test_a_layers_decode_step(cuda, pplb200):
     _check_rotated(cuda, qr, q, pos, table, False)
     at = cuda.arange(n + 1, device="cuda")
     for b in range(M):
-        kr, vr = pplb200.kv_cache_read(cache, pages.long()[b, at // page] * page + at % page)
-        _check_attention(out[b:b + 1], None, [_attention(cuda, qr[b], kr, vr, at >= 0, att.scale)])
+        kr, vr = _stored(cuda, cache, pages.long()[b, at // page] * page + at % page)
+        _check_attention(out[b:b + 1], None, [_attention(cuda, qr[b], kr, vr, at >= 0, att.scale, True)])
     oq, os_ = pplb200.minmax_quantize_fp16(out.view(M, hq * d))
     assert cuda.equal(y, pplb200.gemm_i8i8(oq, wo, pplb200.EPI_DEQUANT_F16, os_, sno)) and bool(cuda.isfinite(y).all()) and pplb200.gemm_status() == 0
