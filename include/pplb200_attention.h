@@ -113,7 +113,7 @@ int32_t pplb200_kv_cache_read_fp16(pplb200_stream_t stream, const pplb200_kv_cac
  * hole: its tokens take no part.  window > 0: only the last `window` tokens do.  What lies in the cache beyond a sequence's
  * tokens has no influence, whatever it is.  A sequence of which nothing is seen has zeros for its output and -inf for its lse.
  * optional_lse fp32 [batch, q_heads], contiguous: log(sum_t exp(scale q . k_t)), for joining results over parts of a context.
- * head_dim 64, 96, 128 or 256; q_heads a multiple of kv_heads; strides multiples of 8; q and out 16-byte aligned; out may be q.
+ * head_dim 64, 96, 128 or 256 (with quant_group 8: scales 4-byte aligned, their strides even); q_heads a multiple of kv_heads; strides multiples of 8; q and out 16-byte aligned; out may be q.
  * ws: pplb200_paged_decode_attention_workspace_bytes(), 256-byte aligned, not initialised, not shared by calls that may run at the
  * same time (two captured graphs that are replayed at once need one each).
  * The result does not depend on what else is in the batch's other rows beyond the order in which a sequence's parts are summed,

@@ -3,11 +3,11 @@
 // What bounds it is the cache: every key and value is read once, for a few multiply-adds per element.  So the work is laid out for
 // loads: tiles of CT tokens of one head, numbered over all sequences and heads, are dealt out evenly to as many CTAs as the device holds
 // at once, whatever the sequences' lengths; a CTA whose share begins or ends inside a sequence leaves its sums in the workspace
-// and a second kernel joins them.  A warp takes 16 tokens at a time and brings them into a ring of its own: every lane copies exactly the
-// bytes it will use (the dimensions of a product may be taken in any order), so that the ring needs no barrier, no swizzle and no
-// second look at an address.  Scores are computed transposed, keys [16 tokens x dimensions] x queries [dimensions x 8 heads]: the eight
-// columns hold the query heads that share the key head, and the weights turn into the operand of the second product, values^T x
-// weights^T, by transposing 8 x 8 blocks between registers.
+// and a second kernel joins them.  A warp takes 16 tokens at a time, and while it works on these the next ones are on their way into
+// its registers: a lane loads exactly the bytes that it will use (the dimensions of a product may be taken in any order), so that
+// nothing passes through shared memory.  Scores are computed transposed, keys [16 tokens x dimensions] x queries [dimensions x 8
+// heads]: the eight columns hold the query heads that share the key head, and the weights turn into the operand of the second
+// product, values^T x weights^T, by transposing 8 x 8 blocks between registers.
 #include "kv_cache.cuh"
 
 #include <algorithm>
@@ -17,7 +17,7 @@ namespace pplb200 {
 namespace paged {
 
 constexpr int WARPS = 4, ATPB = 32 * WARPS, WT = 16, CT = WARPS * WT;
-constexpr int kSms = 148;
+constexpr int kSms = 148, kMostCtas = 4 * kSms;
 enum : int { CACHE_F16 = 0, CACHE_I8_GROUPS = 1, CACHE_I8_ROWS = 2 };
 
 constexpr int piece(int bytes) { return bytes % 16 == 0 ? 16 : bytes % 8 == 0 ? 8 : 4; }
@@ -30,16 +30,12 @@ struct Shape {
     // a quad's lane holds a quarter of the dimensions of two keys, an eighth of those of four values
     static constexpr int KB = D * ES / 4, KP = piece(KB), KN = KB / KP;
     static constexpr int VB = D * ES / 8, VP = piece(VB), VN = VB / VP;
-    static constexpr int SB = D / 4, SP = piece(SB), SN = SB / SP; // CACHE_I8_GROUPS: a row's scales
-    static constexpr int K_BYTES = WT * D * ES, V_BYTES = K_BYTES;
-    static constexpr int SCALE_BYTES = KIND == CACHE_I8_GROUPS ? 2 * WT * SB : KIND == CACHE_I8_ROWS ? WT * 8 : 0;
-    static constexpr int STAGE = K_BYTES + V_BYTES + SCALE_BYTES + 16;
-    static constexpr int BUDGET = 17408; // of shared memory per warp, for three CTAs of four warps on an SM
-    static constexpr int STAGES = STAGE * 4 <= BUDGET ? 4 : STAGE * 3 <= BUDGET ? 3 : 2;
-    static constexpr int CTAS = STAGES * STAGE * WARPS * 3 <= 225 * 1024 ? 3 : STAGES * STAGE * WARPS * 2 <= 225 * 1024 ? 2 : 1;
+    static constexpr int KG = KP >= 8 ? KP / 8 : 1, VG = VP >= 8 ? VP / 8 : 1; // CACHE_I8_GROUPS: scales of a piece
+    // CTAs on an SM, by the registers a thread needs: sums, queries and a tile on its way
+    static constexpr int REGS = NT * D / 4 + NT * D / 8 + D * ES / 4;
+    static constexpr int CTAS = REGS <= 80 ? 4 : REGS <= 128 ? 3 : 2;
     static constexpr int ROW = D + 4; // of the sums that the warps exchange
     static constexpr int EXCHANGE = WARPS * HEADS * (ROW + 2) * 4;
-    static constexpr int SMEM = STAGES * STAGE * WARPS > EXCHANGE ? STAGES * STAGE * WARPS : EXCHANGE;
     static constexpr int STEPS = D / 16; // of 16 dimensions in the first product, and blocks of 16 in the second
 };
 
@@ -58,7 +54,10 @@ struct AttentionParams {
     int32_t q_heads, shared, tiles; // query heads per key-value head, and how many blocks of HEADS these make
     int32_t window;
     float scale_log2;
-    int32_t unit; // log2 of the bytes in which offsets of rows are counted
+    int32_t num_pages;
+    // Offsets of rows and scales within a head, which travel between lanes, are 32-bit numbers of `unit` and `scale_unit` bytes.
+    uint32_t unit, page_units, token_units, scale_unit, scale_page_units, scale_token_units;
+    uint32_t page_magic, page_shift; // token / page_size = token * page_magic >> page_shift
     pplb200_kv_cache cache;
     // workspace
     float* sums;       // [2 * CTAs][HEADS][D]
@@ -67,22 +66,25 @@ struct AttentionParams {
 };
 enum : int { TAIL_NONE = 0, TAIL_MORE = 1, TAIL_END = 2 };
 
-__device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// A piece of a row, read once: kept out of L1.  volatile: loads stay where they are put, ahead of the work on the tile before.
 template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool valid) {
-    const int n = valid ? BYTES : 0; // the rest of the destination is filled with zeros
-    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+__device__ __forceinline__ void load_piece(uint32_t (&w)[BYTES / 4], const char* p) {
+    if constexpr (BYTES == 16) asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+    else if constexpr (BYTES == 8) asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+    else asm volatile("ld.global.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// N neighbouring scales of two bytes, in one word
 template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-template <int BYTES>
-__device__ __forceinline__ void load_words(uint32_t (&w)[BYTES / 4], uint32_t at) {
-    if constexpr (BYTES == 16) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
-    else if constexpr (BYTES == 8) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
-    else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
+__device__ __forceinline__ uint32_t load_scales(const char* p) {
+    uint32_t w;
+    if constexpr (N == 2) {
+        asm volatile("ld.global.u32 %0, [%1];" : "=r"(w) : "l"(p));
+    } else {
+        uint16_t x;
+        asm volatile("ld.global.u16 %0, [%1];" : "=h"(x) : "l"(p));
+        w = x;
+    }
+    return w;
 }
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -147,7 +149,7 @@ __device__ __forceinline__ void snap(Share& s, int32_t quantum) {
 
 template <class S>
 __global__ void __launch_bounds__(ATPB, S::CTAS) paged_attention_kernel(const __grid_constant__ AttentionParams p) {
-    extern __shared__ __align__(128) char smem[];
+    __shared__ __align__(16) float part[WARPS * S::HEADS * S::ROW], tops[WARPS * S::HEADS * 2];
     __shared__ int64_t scan[WARPS], ends[2][2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int heads_per_sequence = p.cache.kv_heads * p.tiles;
@@ -217,7 +219,6 @@ __global__ void __launch_bounds__(ATPB, S::CTAS) paged_attention_kernel(const __
     int32_t begun = -1, began_with = TAIL_NONE;
     int64_t b = from.b;
     int32_t hh = from.head, tile0 = from.tile;
-    const uint32_t ring = smem_of(smem) + warp * S::STAGES * S::STAGE;
 
     for (; b < p.batch; tile0 = 0) {
         const int64_t item = b * heads_per_sequence + hh;
@@ -231,8 +232,8 @@ __global__ void __launch_bounds__(ATPB, S::CTAS) paged_attention_kernel(const __
             const int q_count = min(S::HEADS, p.shared - q_first);
             const char* const kbase = (const char*)p.cache.k + (int64_t)kvh * p.cache.head_stride * S::ES;
             const char* const vbase = (const char*)p.cache.v + (int64_t)kvh * p.cache.head_stride * S::ES;
-            const half* const ksbase = (const half*)p.cache.k_scale + (int64_t)kvh * p.cache.scale_head_stride;
-            const half* const vsbase = (const half*)p.cache.v_scale + (int64_t)kvh * p.cache.scale_head_stride;
+            const char* const ksbase = (const char*)p.cache.k_scale + (int64_t)kvh * p.cache.scale_head_stride * 2;
+            const char* const vsbase = (const char*)p.cache.v_scale + (int64_t)kvh * p.cache.scale_head_stride * 2;
             const int32_t* const row_pages = p.pages + b * p.pages_stride;
 
             // ---- queries: column g of block nt, the dimensions of quad lane t --------------------------------------------
@@ -257,150 +258,146 @@ __global__ void __launch_bounds__(ATPB, S::CTAS) paged_attention_kernel(const __
 #pragma unroll
             for (int nt = 0; nt < S::NT; ++nt) top[nt][0] = top[nt][1] = -1e30f;
 
-            // ---- the ring --------------------------------------------------------------------------------------------------
-            // Lane l looks after token l % 16 of a tile: its page, then the offset of its row.
-            auto token_of = [&](int32_t tile) { return first + tile * CT + warp * WT + (lane & 15); };
-            auto page_of = [&](int32_t tile) {
-                const int32_t token = token_of(tile);
-                return tile < tile1 && token < n ? row_pages[token / p.cache.page_size] : -1;
+            // ---- tiles on their way ----------------------------------------------------------------------------------------
+            // Lane l looks after token l % 16 of a tile: its page, two tiles ahead, then where its row lies, one tile ahead.
+            struct Place {
+                int32_t page;
+                uint32_t in_page;
             };
-            // CACHE_I8_ROWS: the key's scale (lanes 0 to 15) or the value's of the lane's token.  Two bytes are too few for the copy engine:
-            // they come through a register, and are put into their stage when the next one is requested.
-            auto request = [&](int32_t tile, int32_t page, uint32_t stage, float& scale_ahead) {
-                const int32_t token = token_of(tile);
-                const bool ok = page >= 0 && page < p.cache.num_pages;
-                const int32_t in_page = token - token / p.cache.page_size * p.cache.page_size;
-                const uint32_t seen = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-                const uint32_t off = ok ? (uint32_t)((((int64_t)page * p.cache.page_stride + (int64_t)in_page * p.cache.token_stride) * S::ES) >> p.unit) : 0u;
+            auto find = [&](int32_t tile) {
+                const int32_t token = first + tile * CT + warp * WT + (lane & 15);
+                const uint32_t index = (uint32_t)((uint64_t)(uint32_t)token * p.page_magic >> p.page_shift);
+                Place at;
+                at.page = tile < tile1 && token < n ? row_pages[index] : -1;
+                at.in_page = token - index * p.cache.page_size;
+                return at;
+            };
+            uint32_t row = 0, scale_row = 0, coming = 0; // of the tile that is loaded next: offsets, and which tokens there are
+            auto locate = [&](const Place& at) {
+                const bool ok = (uint32_t)at.page < (uint32_t)p.num_pages;
+                coming = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+                row = ok ? at.page * p.page_units + at.in_page * p.token_units : 0u;
+                if constexpr (S::KIND != CACHE_F16) scale_row = ok ? at.page * p.scale_page_units + at.in_page * p.scale_token_units : 0u;
+            };
+            uint32_t kw[2][S::KN][S::KP / 4] = {}, vw[4][S::VN][S::VP / 4] = {};
+            uint32_t ks[2][S::KN] = {}, vs[4][S::VN] = {}; // CACHE_I8_GROUPS
+            uint32_t scale_bits = 0;                       // CACHE_I8_ROWS: key scale of a token in lanes 0 to 15, value scale in the others
+            auto load_keys = [&](bool all) {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const int row = g + 8 * r;
-                    const char* src = kbase + ((uint64_t)__shfl_sync(0xffffffffu, off, row) << p.unit) + t * S::KP;
+                    const int token = g + 8 * r;
+                    const char* src = kbase + (uint64_t)__shfl_sync(0xffffffffu, row, token) * p.unit + t * S::KP;
+                    const char* scales = ksbase;
+                    if constexpr (S::KIND == CACHE_I8_GROUPS) scales += (uint64_t)__shfl_sync(0xffffffffu, scale_row, token) * p.scale_unit + t * S::KG * 2;
+                    const bool there = all || (coming >> token & 1);
 #pragma unroll
-                    for (int i = 0; i < S::KN; ++i)
-                        copy_async<S::KP>(stage + ((r * S::KN + i) * 32 + lane) * S::KP, src + i * 4 * S::KP, seen >> row & 1);
-                }
+                    for (int i = 0; i < S::KN; ++i) {
+                        if (there) {
+                            load_piece<S::KP>(kw[r][i], src + i * 4 * S::KP);
+                            if constexpr (S::KIND == CACHE_I8_GROUPS) ks[r][i] = load_scales<S::KG>(scales + i * 4 * S::KG * 2);
+                        } else { // zeros: what lies there may be anything
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int row = 2 * t + (j & 1) + 8 * (j >> 1);
-                    const char* src = vbase + ((uint64_t)__shfl_sync(0xffffffffu, off, row) << p.unit) + g * S::VP;
-#pragma unroll
-                    for (int i = 0; i < S::VN; ++i)
-                        copy_async<S::VP>(stage + S::K_BYTES + ((j * S::VN + i) * 32 + lane) * S::VP, src + i * 8 * S::VP, seen >> row & 1);
-                }
-                if constexpr (S::KIND != CACHE_F16) {
-                    const int64_t at = ok ? (int64_t)page * p.cache.scale_page_stride + (int64_t)in_page * p.cache.scale_token_stride : 0;
-                    if constexpr (S::KIND == CACHE_I8_ROWS) {
-                        scale_ahead = ok ? __half2float(ld_global_half((lane < 16 ? ksbase : vsbase) + at)) : 0.0f;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < WT * S::SN; i += 32) {
-                            const int row = (i + lane) / S::SN, part = (i + lane) - row * S::SN;
-                            const int64_t from_row = __shfl_sync(0xffffffffu, at, row & 15);
-                            if (i + lane < WT * S::SN) {
-                                const bool there = seen >> row & 1;
-                                const uint32_t dst = stage + S::K_BYTES + S::V_BYTES + (i + lane) * S::SP;
-                                copy_async<S::SP>(dst, ksbase + from_row + part * (S::SP / 2), there);
-                                copy_async<S::SP>(dst + WT * S::SB, vsbase + from_row + part * (S::SP / 2), there);
-                            }
+                            for (int x = 0; x < S::KP / 4; ++x) kw[r][i][x] = 0;
+                            ks[r][i] = 0;
                         }
                     }
                 }
-                if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(stage + S::STAGE - 16), "r"(seen) : "memory");
-                copy_commit();
             };
-            auto put_scale = [&](uint32_t stage, float scale) {
+            auto load_values = [&](bool all) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int token = 2 * t + (j & 1) + 8 * (j >> 1);
+                    const char* src = vbase + (uint64_t)__shfl_sync(0xffffffffu, row, token) * p.unit + g * S::VP;
+                    const char* scales = vsbase;
+                    if constexpr (S::KIND == CACHE_I8_GROUPS) scales += (uint64_t)__shfl_sync(0xffffffffu, scale_row, token) * p.scale_unit;
+                    const bool there = all || (coming >> token & 1);
+#pragma unroll
+                    for (int i = 0; i < S::VN; ++i) {
+                        constexpr int EP = S::VP / S::ES;
+                        if (there) {
+                            load_piece<S::VP>(vw[j][i], src + i * 8 * S::VP);
+                            if constexpr (S::KIND == CACHE_I8_GROUPS) vs[j][i] = load_scales<S::VG>(scales + (i * 8 + g) * EP / 8 * 2);
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < S::VP / 4; ++x) vw[j][i][x] = 0;
+                            vs[j][i] = 0;
+                        }
+                    }
+                }
                 if constexpr (S::KIND == CACHE_I8_ROWS)
-                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(stage + S::K_BYTES + S::V_BYTES + (lane & 15) * 8 + (lane >> 4) * 4), "f"(scale) : "memory");
+                    scale_bits = (coming >> (lane & 15) & 1) ? load_scales<1>((lane < 16 ? ksbase : vsbase) + (uint64_t)scale_row * p.scale_unit) : 0u;
             };
 
-            float scale_ahead = 0.0f;
-            uint32_t scale_stage = ring;
+            Place ahead = find(tile0);
             {
-                int32_t pages[S::STAGES];
-                float scales[S::STAGES] = {};
-#pragma unroll
-                for (int s = 0; s < S::STAGES; ++s) pages[s] = page_of(tile0 + s);
-#pragma unroll
-                for (int s = 0; s < S::STAGES; ++s) request(tile0 + s, pages[s], ring + s * S::STAGE, scales[s]);
-#pragma unroll
-                for (int s = 0; s < S::STAGES; ++s) put_scale(ring + s * S::STAGE, scales[s]);
-                scale_ahead = scales[0];
+                const Place second = find(tile0 + 1);
+                locate(ahead);
+                ahead = second;
             }
-            int32_t page_ahead = page_of(tile0 + S::STAGES);
-            uint32_t stage = ring;
+            uint32_t seen = coming;
+            if (seen == 0xffffu) load_keys(true), load_values(true);
+            else if (seen) load_keys(false), load_values(false);
+            locate(ahead);
+            ahead = find(tile0 + 2);
+
             for (int32_t tile = tile0; tile < tile1; ++tile) {
-                put_scale(scale_stage, scale_ahead);
-                copy_wait<S::STAGES - 1>();
-                __syncwarp();
-                uint32_t seen;
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(seen) : "r"(stage + S::STAGE - 16) : "memory");
+                float c[S::NT][4] = {};
                 if (seen != 0) {
-                    // ---- scores [16 tokens x 8 heads] ----------------------------------------------------------------------
-                    float c[S::NT][4] = {};
+                    // ---- scores [16 tokens x 8 heads], in two chains -----------------------------------------------------------
+                    float c2[S::NT][4] = {};
                     constexpr int KW = S::KP / 4;
 #pragma unroll
                     for (int i = 0; i < S::KN; ++i) {
-                        uint32_t w0[KW], w1[KW];
-                        load_words<S::KP>(w0, stage + (i * 32 + lane) * S::KP);
-                        load_words<S::KP>(w1, stage + ((S::KN + i) * 32 + lane) * S::KP);
                         if constexpr (S::ES == 2) {
 #pragma unroll
                             for (int s = 0; s < KW / 2; ++s)
 #pragma unroll
                                 for (int nt = 0; nt < S::NT; ++nt) {
-                                    const auto& b = q[nt][i * (KW / 2) + s];
-                                    mma(c[nt], w0[2 * s], w1[2 * s], w0[2 * s + 1], w1[2 * s + 1], b[0], b[1]);
+                                    const auto& qs = q[nt][i * (KW / 2) + s];
+                                    mma(s & 1 ? c2[nt] : c[nt], kw[0][i][2 * s], kw[1][i][2 * s], kw[0][i][2 * s + 1], kw[1][i][2 * s + 1], qs[0], qs[1]);
                                 }
                         } else {
-                            // scales of this piece's dimensions for keys g and g + 8
-                            constexpr int GROUPS = S::KP >= 8 ? S::KP / 8 : 1;
-                            uint32_t s0[GROUPS], s1[GROUPS];
-                            if constexpr (S::KIND == CACHE_I8_GROUPS) {
-#pragma unroll
-                                for (int j = 0; j < GROUPS; ++j) {
-                                    const uint32_t at = stage + S::K_BYTES + S::V_BYTES + ((i * 4 + t) * GROUPS + j) * 2;
-                                    uint16_t x, y;
-                                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(at + g * S::SB) : "memory");
-                                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(y) : "r"(at + (g + 8) * S::SB) : "memory");
-                                    s0[j] = x * 0x10001u;
-                                    s1[j] = y * 0x10001u;
-                                }
-                            }
 #pragma unroll
                             for (int s = 0; s < KW; ++s) {
                                 uint32_t a0, a1, a2, a3;
-                                widen(w0[s], a0, a2);
-                                widen(w1[s], a1, a3);
+                                widen(kw[0][i][s], a0, a2);
+                                widen(kw[1][i][s], a1, a3);
                                 if constexpr (S::KIND == CACHE_I8_GROUPS) {
                                     // value x scale has up to 18 bits: its rounding to fp16, and what that left, as a second operand
-                                    const __half2 f0 = as_h2(s0[s / 2]), f1 = as_h2(s1[s / 2]);
+                                    const __half2 f0 = as_h2(__byte_perm(ks[0][i], 0, s < 2 ? 0x1010 : 0x3232)), f1 = as_h2(__byte_perm(ks[1][i], 0, s < 2 ? 0x1010 : 0x3232));
                                     const __half2 h0 = __hmul2(as_h2(a0), f0), h1 = __hmul2(as_h2(a1), f1), h2_ = __hmul2(as_h2(a2), f0), h3 = __hmul2(as_h2(a3), f1);
                                     const uint32_t r0 = h2(__hfma2(as_h2(a0), f0, __hneg2(h0))), r1 = h2(__hfma2(as_h2(a1), f1, __hneg2(h1)));
                                     const uint32_t r2 = h2(__hfma2(as_h2(a2), f0, __hneg2(h2_))), r3 = h2(__hfma2(as_h2(a3), f1, __hneg2(h3)));
 #pragma unroll
                                     for (int nt = 0; nt < S::NT; ++nt) {
-                                        const auto& b = q[nt][i * KW + s];
-                                        mma(c[nt], h2(h0), h2(h1), h2(h2_), h2(h3), b[0], b[1]);
-                                        mma(c[nt], r0, r1, r2, r3, b[0], b[1]);
+                                        const auto& qs = q[nt][i * KW + s];
+                                        mma(c[nt], h2(h0), h2(h1), h2(h2_), h2(h3), qs[0], qs[1]);
+                                        mma(c2[nt], r0, r1, r2, r3, qs[0], qs[1]);
                                     }
                                 } else {
 #pragma unroll
-                                    for (int nt = 0; nt < S::NT; ++nt) mma(c[nt], a0, a1, a2, a3, q[nt][i * KW + s][0], q[nt][i * KW + s][1]);
+                                    for (int nt = 0; nt < S::NT; ++nt) mma(s & 1 ? c2[nt] : c[nt], a0, a1, a2, a3, q[nt][i * KW + s][0], q[nt][i * KW + s][1]);
                                 }
                             }
                         }
                     }
+#pragma unroll
+                    for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) c[nt][x] += c2[nt][x];
+                }
+                if (coming == 0xffffu) load_keys(true);
+                else if (coming) load_keys(false);
 
+                if (seen != 0) {
                     // ---- weights: 2^(score - top + 8) ----------------------------------------------------------------------
                     float f0 = p.scale_log2, f1 = p.scale_log2, v0 = 1.0f, v1 = 1.0f, e0 = 0.0f, e1 = 0.0f;
                     if constexpr (S::KIND == CACHE_I8_ROWS) {
-                        const uint32_t at = stage + S::K_BYTES + S::V_BYTES;
-                        float k0, k1;
-                        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(k0), "=f"(v0) : "r"(at + g * 8) : "memory");
-                        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(k1), "=f"(v1) : "r"(at + (g + 8) * 8) : "memory");
-                        f0 *= k0;
-                        f1 *= k1;
+                        const float mine = __half2float(__ushort_as_half((unsigned short)scale_bits));
+                        f0 *= __shfl_sync(0xffffffffu, mine, g);
+                        f1 *= __shfl_sync(0xffffffffu, mine, g + 8);
+                        v0 = __shfl_sync(0xffffffffu, mine, g + 16);
+                        v1 = __shfl_sync(0xffffffffu, mine, g + 24);
                         // the value's scale goes into the weight; 2^e is above it
                         e0 = (float)max((int)(__float_as_uint(v0) >> 23) - 126, -24);
                         e1 = (float)max((int)(__float_as_uint(v1) >> 23) - 126, -24);
@@ -462,14 +459,11 @@ __global__ void __launch_bounds__(ATPB, S::CTAS) paged_attention_kernel(const __
                     constexpr int VW = S::VP / 4, EP = S::VP / S::ES; // words and dimensions of a piece
 #pragma unroll
                     for (int i = 0; i < S::VN; ++i) {
-                        uint32_t w[4][VW];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) load_words<S::VP>(w[j], stage + S::K_BYTES + ((j * S::VN + i) * 32 + lane) * S::VP);
                         if constexpr (S::ES == 2) {
 #pragma unroll
                             for (int x = 0; x < VW; ++x) {
-                                const uint32_t a0 = __byte_perm(w[0][x], w[1][x], 0x5410), a1 = __byte_perm(w[0][x], w[1][x], 0x7632);
-                                const uint32_t a2 = __byte_perm(w[2][x], w[3][x], 0x5410), a3 = __byte_perm(w[2][x], w[3][x], 0x7632);
+                                const uint32_t a0 = __byte_perm(vw[0][i][x], vw[1][i][x], 0x5410), a1 = __byte_perm(vw[0][i][x], vw[1][i][x], 0x7632);
+                                const uint32_t a2 = __byte_perm(vw[2][i][x], vw[3][i][x], 0x5410), a3 = __byte_perm(vw[2][i][x], vw[3][i][x], 0x7632);
 #pragma unroll
                                 for (int nt = 0; nt < S::NT; ++nt) {
                                     mma(o[nt][i * EP / 2 + x], a0, a1, a2, a3, wh[nt][0], wh[nt][1]);
@@ -480,17 +474,12 @@ __global__ void __launch_bounds__(ATPB, S::CTAS) paged_attention_kernel(const __
 #pragma unroll
                             for (int x = 0; x < VW; ++x) {
                                 uint32_t u[4], v[4];
-                                widen_pairs(w[0][x], w[1][x], u);
-                                widen_pairs(w[2][x], w[3][x], v);
+                                widen_pairs(vw[0][i][x], vw[1][i][x], u);
+                                widen_pairs(vw[2][i][x], vw[3][i][x], v);
                                 if constexpr (S::KIND == CACHE_I8_GROUPS) {
-                                    // the group of these four dimensions; value x scale is rounded to fp16, as it is when it is read back
-                                    const int group = ((i * 8 + g) * EP + x * 4) / 8;
-                                    const uint32_t at = stage + S::K_BYTES + S::V_BYTES + WT * S::SB + group * 2;
-                                    uint16_t s[4];
-#pragma unroll
-                                    for (int j = 0; j < 4; ++j)
-                                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(s[j]) : "r"(at + (2 * t + (j & 1) + 8 * (j >> 1)) * S::SB) : "memory");
-                                    const __half2 fu = as_h2(s[0] | (uint32_t)s[1] << 16), fv = as_h2(s[2] | (uint32_t)s[3] << 16);
+                                    // these four dimensions are of one group; value x scale is rounded to fp16, as it is when it is read back
+                                    const __half2 fu = as_h2(__byte_perm(vs[0][i], vs[1][i], x < 2 ? 0x5410 : 0x7632));
+                                    const __half2 fv = as_h2(__byte_perm(vs[2][i], vs[3][i], x < 2 ? 0x5410 : 0x7632));
 #pragma unroll
                                     for (int y = 0; y < 4; ++y) {
                                         u[y] = h2(__hmul2(as_h2(u[y]), fu));
@@ -508,18 +497,14 @@ __global__ void __launch_bounds__(ATPB, S::CTAS) paged_attention_kernel(const __
                         }
                     }
                 }
-                __syncwarp();
-                request(tile + S::STAGES, page_ahead, stage, scale_ahead);
-                scale_stage = stage;
-                page_ahead = page_of(tile + S::STAGES + 1);
-                stage = stage == ring + (S::STAGES - 1) * S::STAGE ? ring : stage + S::STAGE;
+                if (coming == 0xffffu) load_values(true);
+                else if (coming) load_values(false);
+                seen = coming;
+                locate(ahead);
+                ahead = find(tile + 3);
             }
-            copy_wait<0>();
-            __syncthreads();
 
             // ---- the four warps' sums --------------------------------------------------------------------------------------
-            float* const part = reinterpret_cast<float*>(smem);                 // [warp][head][ROW]
-            float* const tops = part + WARPS * S::HEADS * S::ROW;               // [warp][head][2]
 #pragma unroll
             for (int nt = 0; nt < S::NT; ++nt) {
 #pragma unroll
@@ -577,83 +562,125 @@ __global__ void __launch_bounds__(ATPB, S::CTAS) paged_attention_kernel(const __
     if (threadIdx.x == 0 && p.items) *reinterpret_cast<int2*>(p.items + 2 * blockIdx.x) = make_int2(begun, began_with);
 }
 
-// Joins the pieces of the item that CTA blockIdx.x began and others went on with, in the order of the tokens: a warp per query head.
+// Joins the pieces of the item that CTA blockIdx.x began and others went on with: four warps for each of two query heads, every fourth
+// piece to a warp, in an order that does not change.
+constexpr int JTPB = 256, JWARPS = 4;
 template <int D, int HEADS>
-__global__ void __launch_bounds__(ATPB) paged_attention_join_kernel(const __grid_constant__ AttentionParams p, int32_t ctas) {
+__global__ void __launch_bounds__(JTPB) paged_attention_join_kernel(const __grid_constant__ AttentionParams p, int32_t ctas) {
     constexpr int V = D / 32;
+    __shared__ int32_t slots[kMostCtas];
+    __shared__ float weights[2][kMostCtas], part[2][JWARPS][D], total[2];
+    __shared__ int32_t count;
     pdl_wait_prior_grid();
-    const int lane = threadIdx.x & 31, h = blockIdx.y * WARPS + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, side = warp / JWARPS, w = warp - side * JWARPS;
     const int32_t item = p.items[2 * blockIdx.x];
     if (item < 0) return;
     const int heads_per_sequence = p.cache.kv_heads * p.tiles;
     const int64_t b = item / heads_per_sequence;
     const int hh = (int)(item - b * heads_per_sequence), kvh = hh / p.tiles, q_first = (hh - kvh * p.tiles) * HEADS;
-    if (h >= min(HEADS, p.shared - q_first)) return;
-    float m = -1e30f, l = 0.0f, o[V] = {};
-    auto add = [&](int64_t slot, float w) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] += w * p.sums[(slot * HEADS + h) * D + i * 32 + lane];
-    };
-    {
-        const int64_t slot = 2 * (int64_t)blockIdx.x + 1;
-        const float2 s = p.tops[slot * HEADS + h];
-        m = s.x;
-        l = s.y;
-        add(slot, 1.0f);
-    }
-    for (int32_t c0 = blockIdx.x + 1; c0 < ctas; c0 += 32) {
-        const int32_t c = c0 + lane;
-        int32_t kind = c < ctas ? p.items[2 * c + 1] : TAIL_NONE;
-        const uint32_t end = __ballot_sync(0xffffffffu, kind == TAIL_END);
-        const uint32_t upto = end ? (end & (0u - end)) * 2u - 1u : 0xffffffffu; // lanes up to the one that ends the item
-        if (!(upto >> lane & 1)) kind = TAIL_NONE;
-        const float2 s = kind != TAIL_NONE ? p.tops[2 * (int64_t)c * HEADS + h] : make_float2(-1e30f, 0.0f);
-        float top = s.x;
-#pragma unroll
-        for (int x = 16; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        top = fmaxf(top, m);
-        const float keep = exp2_fast(m - top), w = kind != TAIL_NONE ? exp2_fast(s.x - top) : 0.0f;
-        m = top;
-        float part = w * s.y;
-#pragma unroll
-        for (int x = 16; x >= 1; x >>= 1) part += __shfl_xor_sync(0xffffffffu, part, x);
-        l = l * keep + part;
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] *= keep;
-        uint32_t todo = __ballot_sync(0xffffffffu, kind != TAIL_NONE);
-        while (todo) {
-            const int x = __ffs(todo) - 1;
-            todo &= todo - 1;
-            add(2 * (int64_t)(c0 + x), __shfl_sync(0xffffffffu, w, x));
+    const int heads = min(HEADS, p.shared - q_first), h = blockIdx.y * 2 + side;
+    if ((int)blockIdx.y * 2 >= heads) return;
+
+    // the pieces: this CTA's own, then those with which the next CTAs' shares begin, up to the one that ends the item
+    if (warp == 0) {
+        int32_t found = 1;
+        if (lane == 0) slots[0] = 2 * blockIdx.x + 1;
+        for (int32_t c0 = blockIdx.x + 1; c0 < ctas; c0 += 32) {
+            const int32_t c = c0 + lane, kind = c < ctas ? p.items[2 * c + 1] : TAIL_NONE;
+            const uint32_t end = __ballot_sync(0xffffffffu, kind == TAIL_END);
+            const uint32_t upto = end ? (end & (0u - end)) * 2u - 1u : 0xffffffffu;
+            const uint32_t has = __ballot_sync(0xffffffffu, kind != TAIL_NONE) & upto;
+            if (has >> lane & 1) slots[found + __popc(has & ((1u << lane) - 1))] = 2 * c;
+            found += __popc(has);
+            if (end) break;
         }
-        if (end) break;
+        if (lane == 0) count = found;
     }
-    const int head = kvh * p.shared + q_first + h;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    __syncthreads();
+    const int32_t pieces = count;
+    // their factors, by the first warp of each head
+    float m = -1e30f;
+    if (w == 0 && h < heads) {
+        for (int i = lane; i < pieces; i += 32) m = fmaxf(m, p.tops[(int64_t)slots[i] * HEADS + h].x);
 #pragma unroll
-    for (int i = 0; i < V; ++i) p.out[b * p.out_stride + (int64_t)head * D + i * 32 + lane] = __float2half_rn(o[i] * inv);
-    if (p.lse && lane == 0) p.lse[b * p.q_heads + head] = l == 0.0f ? -INFINITY : (m - 8.0f + log2f(l)) * 0.69314718055994531f;
+        for (int x = 16; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+        float l = 0.0f;
+        for (int i = lane; i < pieces; i += 32) {
+            const float2 s = p.tops[(int64_t)slots[i] * HEADS + h];
+            const float f = exp2_fast(s.x - m);
+            weights[side][i] = f;
+            l += f * s.y;
+        }
+#pragma unroll
+        for (int x = 16; x >= 1; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+        if (lane == 0) total[side] = l;
+    }
+    __syncthreads();
+    float o[V] = {};
+    if (h < heads) {
+        for (int i0 = w; i0 < pieces; i0 += 4 * JWARPS) {
+            float v[4][V];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int x = 0; x < V; ++x) v[u][x] = i0 + u * JWARPS < pieces ? p.sums[((int64_t)slots[i0 + u * JWARPS] * HEADS + h) * D + x * 32 + lane] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int x = 0; x < V; ++x)
+                    if (i0 + u * JWARPS < pieces) o[x] += weights[side][i0 + u * JWARPS] * v[u][x];
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < V; ++x) part[side][w][x * 32 + lane] = o[x];
+    __syncthreads();
+    if (h >= heads) return;
+    const int head = kvh * p.shared + q_first + h;
+    const float l = total[side], inv = l == 0.0f ? 0.0f : 1.0f / l;
+    for (int d = w * 32 + lane; d < D; d += JWARPS * 32) {
+        float v = 0.0f;
+#pragma unroll
+        for (int x = 0; x < JWARPS; ++x) v += part[side][x][d];
+        p.out[b * p.out_stride + (int64_t)head * D + d] = __float2half_rn(v * inv);
+    }
+    if (p.lse && w == 0 && lane == 0) p.lse[b * p.q_heads + head] = l == 0.0f ? -INFINITY : (m - 8.0f + log2f(l)) * 0.69314718055994531f;
+}
+
+// Strides in bytes -> in units of the largest power of two that divides them; false where an offset would not fit 32 bits.
+bool row_units(int64_t pages, int64_t page_size, int64_t page_bytes, int64_t token_bytes, uint32_t& unit, uint32_t& page_units, uint32_t& token_units) {
+    const int64_t strides = (pages > 1 ? page_bytes : 0) | (page_size > 1 ? token_bytes : 0);
+    const int shift = strides ? std::min(__builtin_ctzll((uint64_t)strides), 30) : 0;
+    const __int128 last = pages > 0 ? (__int128)(pages - 1) * page_bytes + (__int128)(page_size - 1) * token_bytes : 0;
+    unit = 1u << shift;
+    page_units = (uint32_t)(pages > 1 ? page_bytes >> shift : 0);
+    token_units = (uint32_t)(page_size > 1 ? token_bytes >> shift : 0);
+    return (last >> shift) < ((__int128)1 << 32);
+}
+
+// token / d = token * magic >> shift for all tokens below 2^31: with 2^(s - 1) < d <= 2^s and magic = ceil(2^(31 + s) / d), magic * d
+// exceeds 2^(31 + s) by less than d <= 2^s, which token < 2^31 keeps below 1 / d of the quotient.
+void page_division(uint32_t d, uint32_t& magic, uint32_t& shift) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) ++s;
+    shift = 31 + s;
+    magic = (uint32_t)(((1ull << shift) + d - 1) / d);
 }
 
 // Query heads that a CTA takes at once: two blocks of eight where that many share a key-value head and registers allow.
 int heads_at_once(int32_t head_dim, int32_t shared) { return shared > 8 && head_dim <= 128 ? 16 : 8; }
-constexpr int kMostCtas = 3 * kSms;
-
 template <class S>
 int32_t launch(cudaStream_t stream, AttentionParams& p, int64_t tokens) {
     static_assert(S::CTAS * kSms <= kMostCtas, "workspace");
-    if (cudaFuncSetAttribute(paged_attention_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess)
-        return fail(RC_DEVICE_RUNTIME_ERROR, "shared memory of the attention kernel: %s", cudaGetErrorString(cudaGetLastError()));
     const int64_t tiles = (tokens + CT - 1) / CT;
     const int64_t items = p.batch * p.cache.kv_heads * p.tiles;
     const int64_t most = S::CTAS * kSms;
     const int64_t ctas = tiles > most || items > most ? most : std::min(most, items * std::max<int64_t>(1, tiles));
-    launch_ex(paged_attention_kernel<S>, dim3((unsigned)ctas), dim3(ATPB), (size_t)S::SMEM, stream, true, p);
+    launch_ex(paged_attention_kernel<S>, dim3((unsigned)ctas), dim3(ATPB), stream, true, p);
     int32_t rc = check_launch("paged attention");
     if (rc != RC_SUCCESS) return rc;
     // no cut falls inside an item of one tile, nor, where cuts are moved by four tiles (see `quantum`), of six
     if (tiles <= 1 || (tiles <= 6 && items * tiles < 16 * ctas)) return RC_SUCCESS;
-    launch_ex(paged_attention_join_kernel<S::D, S::HEADS>, dim3((unsigned)ctas, S::HEADS / WARPS), dim3(ATPB), stream, true, p, (int32_t)ctas);
+    launch_ex(paged_attention_join_kernel<S::D, S::HEADS>, dim3((unsigned)ctas, S::HEADS / 2), dim3(JTPB), stream, true, p, (int32_t)ctas);
     return check_launch("joining of attention");
 }
 
@@ -710,19 +737,16 @@ int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb2
     if (!a->ws || a->ws_bytes < need || ((uintptr_t)a->ws & 255))
         return fail(RC_INVALID_VALUE, "workspace of %lld bytes (256-byte aligned) needed, got %lld", (long long)need, (long long)a->ws_bytes);
     AttentionParams p = {};
-    if (cache->quant_group == 8) {
-        const int64_t unit = D == 96 ? 4 : 8;
-        if ((((uintptr_t)cache->k_scale | (uintptr_t)cache->v_scale) & (2 * unit - 1)) || cache->scale_page_stride % unit || cache->scale_head_stride % unit || cache->scale_token_stride % unit)
-            return fail(RC_INVALID_VALUE, "attention: scales of groups of 8 must be aligned to, and their strides multiples of, %lld bytes", (long long)(2 * unit));
-    }
-    // Offsets of rows travel between lanes as 32-bit numbers of the largest power of two of bytes that divides the strides.
-    const int64_t es = cache->quant_group ? 1 : 2;
-    const uint64_t strides = (uint64_t)(cache->page_stride | cache->token_stride) * es;
-    p.unit = strides ? __builtin_ctzll(strides) : 4;
-    if (cache->num_pages > 0) {
-        const __int128 last = ((__int128)(cache->num_pages - 1) * cache->page_stride + (__int128)(cache->page_size - 1) * cache->token_stride) * es;
-        if ((last >> p.unit) >= ((__int128)1 << 32)) return fail(RC_UNSUPPORTED, "attention: a cache whose rows lie further apart than 2^32 times their alignment");
-    }
+    if (cache->quant_group == 8 && ((((uintptr_t)cache->k_scale | (uintptr_t)cache->v_scale) & 3) ||
+                                    ((cache->scale_page_stride | cache->scale_head_stride | cache->scale_token_stride) & 1)))
+        return fail(RC_INVALID_VALUE, "attention: scales of groups of 8 must be 4-byte aligned, and their strides even");
+    if (!row_units(cache->num_pages, cache->page_size, cache->page_stride * (cache->quant_group ? 1 : 2), cache->token_stride * (cache->quant_group ? 1 : 2),
+                   p.unit, p.page_units, p.token_units) ||
+        (cache->quant_group && !row_units(cache->num_pages, cache->page_size, cache->scale_page_stride * 2, cache->scale_token_stride * 2, p.scale_unit,
+                                          p.scale_page_units, p.scale_token_units)))
+        return fail(RC_UNSUPPORTED, "attention: the rows of a head lie further apart than 2^32 times their alignment");
+    page_division(cache->page_size, p.page_magic, p.page_shift);
+    p.num_pages = (int32_t)std::min<int64_t>(cache->num_pages, 0x7fffffff); // a table's entry is no larger
     p.q = (const half*)a->q; p.out = (half*)a->out; p.lse = a->optional_lse;
     p.pages = a->pages; p.lengths = a->lengths;
     p.q_stride = a->q_stride; p.out_stride = a->out_stride;
