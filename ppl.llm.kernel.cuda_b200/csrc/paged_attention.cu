@@ -3,7 +3,7 @@
 // What bounds it is the cache: every key and value is read once, for a few multiply-adds per element.  So the work is laid out for
 // loads: tiles of CT tokens of one head, numbered over all sequences and heads, are dealt out evenly to as many CTAs as the device holds
 // at once, whatever the sequences' lengths; a CTA whose share begins or ends inside a sequence leaves its sums in the workspace
-// and a second kernel joins them.  A warp takes 16 tokens at a time, and while it works on these the next ones are on their way into
+// and the CTA that is last to do so joins them.  A warp takes 16 tokens at a time, and while it works on these the next ones are on their way into
 // its registers: a lane loads exactly the bytes that it will use (the dimensions of a product may be taken in any order), so that
 // nothing passes through shared memory.  Scores are computed transposed, keys [16 tokens x dimensions] x queries [dimensions x 8
 // heads]: the eight columns hold the query heads that share the key head, and the weights turn into the operand of the second
@@ -16,8 +16,7 @@
 namespace pplb200 {
 namespace paged {
 
-constexpr int WARPS = 4, ATPB = 32 * WARPS, WT = 16, CT = WARPS * WT;
-constexpr int kSms = 148, kMostCtas = 4 * kSms;
+constexpr int kSms = 148, kCtas = 4 * kSms;
 enum : int { CACHE_F16 = 0, CACHE_I8_GROUPS = 1, CACHE_I8_ROWS = 2 };
 
 constexpr int piece(int bytes) { return bytes % 16 == 0 ? 16 : bytes % 8 == 0 ? 8 : 4; }
@@ -27,16 +26,18 @@ template <int D_, int KIND_, int NT_>
 struct Shape {
     static constexpr int D = D_, KIND = KIND_, NT = NT_, HEADS = 8 * NT;
     static constexpr int ES = KIND == CACHE_F16 ? 2 : 1;
-    // a quad's lane holds a quarter of the dimensions of two keys, an eighth of those of four values
+    // Tokens of a step: 32 where that leaves room for twelve warps on an SM (64 x 8192, int8 rows: 123 us with 32, 129 with 16; groups,
+    // whose scales take registers too: 16 x 4096 71 us with 32, 67 with 16).
+    static constexpr int SUBS = D * ES <= 64 || (D * ES <= 128 && KIND == CACHE_I8_ROWS) ? 2 : 1, TOKENS = 16 * SUBS;
+    // of 16 tokens a quad's lane holds a quarter of the dimensions of two keys, an eighth of those of four values
     static constexpr int KB = D * ES / 4, KP = piece(KB), KN = KB / KP;
     static constexpr int VB = D * ES / 8, VP = piece(VB), VN = VB / VP;
     static constexpr int KG = KP >= 8 ? KP / 8 : 1, VG = VP >= 8 ? VP / 8 : 1; // CACHE_I8_GROUPS: scales of a piece
-    // CTAs on an SM, by the registers a thread needs: sums, queries and a tile on its way
-    static constexpr int REGS = NT * D / 4 + NT * D / 8 + D * ES / 4;
-    static constexpr int CTAS = REGS <= 80 ? 4 : REGS <= 128 ? 3 : 2;
-    static constexpr int ROW = D + 4; // of the sums that the warps exchange
-    static constexpr int EXCHANGE = WARPS * HEADS * (ROW + 2) * 4;
     static constexpr int STEPS = D / 16; // of 16 dimensions in the first product, and blocks of 16 in the second
+    // Registers for the sums, the queries and the tokens on their way decide how many CTAs share an SM.
+    static constexpr int WORDS = NT * D / 4 + NT * D / 8 + SUBS * (D * ES / 4 + (KIND == CACHE_I8_GROUPS ? 2 * KN + 4 * VN : 0));
+    static constexpr int ROW = D + 4; // of the sums that the warps exchange
+    static constexpr int WARPS = 4, THREADS = 32 * WARPS, CTAS = WORDS <= 88 ? 4 : WORDS <= 128 ? 3 : 2;
 };
 
 } // namespace paged
@@ -59,12 +60,13 @@ struct AttentionParams {
     uint32_t unit, page_units, token_units, scale_unit, scale_page_units, scale_token_units;
     uint32_t page_magic, page_shift; // token / page_size = token * page_magic >> page_shift
     pplb200_kv_cache cache;
+    // what spread() flips: in registers, since an instruction holds one constant
+    uint32_t flip, flip_1024;
     // workspace
-    float* sums;       // [2 * CTAs][HEADS][D]
+    uint32_t* arrived; // [CTAs]: pieces of the item that the CTA began; zero between calls
     float2* tops;      // [2 * CTAs][HEADS]: reference exponent and sum of weights
-    int32_t* items;    // [CTAs][2]: the item that the CTA began and did not end (or -1), and what its share began with
+    float* sums;       // [2 * CTAs][HEADS][D]
 };
-enum : int { TAIL_NONE = 0, TAIL_MORE = 1, TAIL_END = 2 };
 
 // A piece of a row, read once: kept out of L1.  volatile: loads stay where they are put, ahead of the work on the tile before.
 template <int BYTES>
@@ -101,27 +103,32 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+__device__ __forceinline__ float log2_fast(float x) {
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 __device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
 __device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 
-// A half whose bits are 0x6400 + u is 1024 + u: with the byte's sign bit flipped, u = value + 128, and 1152 taken off leaves the value.
-constexpr uint32_t k1152 = 0x64806480u;
-__device__ __forceinline__ uint32_t less_1152(uint32_t v) { return h2(__hsub2(as_h2(v), as_h2(k1152))); }
+// Bytes 0, 2 or (of w >> 8) bytes 1, 3 of a word as two halves' bits: u = value + 128, a byte with its sign bit flipped, beneath the
+// exponent that `flip` brings.  With none, the half is u * 2^-24, a subnormal number; with 0x64 above it, 1024 + u.
+__device__ __forceinline__ uint32_t spread(uint32_t w, uint32_t flip) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, 0x00ff00ff, %2, 0x6a;" : "=r"(r) : "r"(w), "r"(flip)); // (w & 0x00ff00ff) ^ flip
+    return r;
+}
+__device__ __forceinline__ uint32_t less_1152(uint32_t v) { return h2(__hsub2(as_h2(v), as_h2(0x64806480u))); }
 
-// Bytes 0, 2 and bytes 1, 3 of a word as pairs of halves (the first product takes dimensions in any order).
-__device__ __forceinline__ void widen(uint32_t w, uint32_t& even, uint32_t& odd) {
-    even = less_1152((w & 0x00ff00ffu) ^ k1152);
-    odd = less_1152(((w >> 8) & 0x00ff00ffu) ^ k1152);
+// The four bytes of a word as halves, 0, 2 and 1, 3 (a product's dimensions may come in any order).
+__device__ __forceinline__ void widen(const AttentionParams& p, uint32_t w, uint32_t& even, uint32_t& odd) {
+    even = less_1152(spread(w, p.flip_1024));
+    odd = less_1152(spread(w >> 8, p.flip_1024));
 }
 // The four bytes of the words of two tokens as pairs (token a, token b).
-__device__ __forceinline__ void widen_pairs(uint32_t a, uint32_t b, uint32_t (&o)[4]) {
-    a ^= 0x80808080u;
-    b ^= 0x80808080u;
-    const uint32_t lo = __byte_perm(a, b, 0x5140), hi = __byte_perm(a, b, 0x7362);
-    o[0] = less_1152(__byte_perm(lo, 0x64646464u, 0x4140));
-    o[1] = less_1152(__byte_perm(lo, 0x64646464u, 0x4342));
-    o[2] = less_1152(__byte_perm(hi, 0x64646464u, 0x4140));
-    o[3] = less_1152(__byte_perm(hi, 0x64646464u, 0x4342));
+__device__ __forceinline__ void widen_pairs(const AttentionParams& p, uint32_t a, uint32_t b, uint32_t (&o)[4]) {
+    widen(p, __byte_perm(a, b, 0x5410), o[0], o[1]);
+    widen(p, __byte_perm(a, b, 0x7632), o[2], o[3]);
 }
 
 // Tokens of a sequence that are looked at: [first, n).
@@ -129,357 +136,453 @@ __device__ __forceinline__ void visible(const AttentionParams& p, int64_t b, int
     n = (int32_t)min((int64_t)max(p.lengths[b], 0), p.tokens_in_table);
     first = p.window > 0 ? max(0, n - p.window) : 0;
 }
-// Tiles of a sequence and head; an empty sequence has one too, so that its output is written.
-__device__ __forceinline__ int32_t tiles_of(const AttentionParams& p, int64_t b) {
+// Steps of a sequence and head; an empty sequence has one too, so that its output is written.
+template <int TOKENS>
+__device__ __forceinline__ int32_t steps_of(const AttentionParams& p, int64_t b) {
     int32_t first, n;
     visible(p, b, first, n);
-    return max(1, (n - first + CT - 1) / CT);
+    return max(1, (n - first + TOKENS - 1) / TOKENS);
 }
 
-struct Share { // where a CTA's share begins or ends
+// What beginning a head of a sequence costs, in steps: a chain of look-ups before the first step, the joining of the warps' sums behind
+// the last, while the other CTAs of the SM go on.
+template <class S>
+constexpr int32_t kBeginning = 2 * S::WARPS;
+
+struct Share { // where a CTA's share begins or ends: a step of a head of a sequence
     int64_t b;
-    int32_t head, tile, tiles; // item of sequence b, tile of it, tiles it has
+    int32_t head, step;
 };
 
-// Moves a cut to a multiple of `quantum` tiles from its item's beginning (or to its end), so that no piece is shorter than half of that.
-__device__ __forceinline__ void snap(Share& s, int32_t quantum) {
-    const int32_t t = (s.tile + quantum / 2) / quantum * quantum;
-    s.tile = t > 0 && s.tiles - t <= quantum / 2 ? s.tiles : t;
+// Output of one query head, dimensions d to d + 3, from sums in units of 2^top.
+__device__ __forceinline__ void finish(const AttentionParams& p, int64_t b, int32_t head, int32_t dims, int32_t d, const float4& v, float top, float sum) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const uint2 r = make_uint2(h2(__floats2half2_rn(v.x * inv, v.y * inv)), h2(__floats2half2_rn(v.z * inv, v.w * inv)));
+    *reinterpret_cast<uint2*>(p.out + b * p.out_stride + (int64_t)head * dims + d) = r;
+    if (p.lse && d == 0) p.lse[b * p.q_heads + head] = sum == 0.0f ? -INFINITY : (top - 8.0f + log2f(sum)) * 0.69314718055994531f;
 }
 
 template <class S>
-__global__ void __launch_bounds__(ATPB, S::CTAS) paged_attention_kernel(const __grid_constant__ AttentionParams p) {
-    __shared__ __align__(16) float part[WARPS * S::HEADS * S::ROW], tops[WARPS * S::HEADS * 2];
+__global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(const __grid_constant__ AttentionParams p) {
+    constexpr int WARPS = S::WARPS, PAD = kBeginning<S>;
+    __shared__ __align__(16) float part[WARPS * S::HEADS * S::ROW];
+    __shared__ float2 tops[WARPS * S::HEADS];
     __shared__ int64_t scan[WARPS], ends[2][2];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    __shared__ volatile struct { int64_t all, last_item; int32_t ctas, to_step; } share; // kept out of the registers
+    __shared__ int32_t longest[WARPS], is_last;
+    // the warp's number from a shuffle, so that the compiler knows that it is the same in all lanes
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, t = lane & 3;
     const int heads_per_sequence = p.cache.kv_heads * p.tiles;
     pdl_wait_prior_grid();
     pdl_launch_dependents();
 
-    // ---- this CTA's share: tiles [c, c + 1) * total / CTAs, in the order sequence, head, tile --------------------------
+    // ---- this CTA's share -----------------------------------------------------------------------------------------------
+    // Steps are numbered in the order sequence, head, step, PAD numbers ahead of every head's first step standing for what its
+    // beginning costs.  CTA c takes the steps from c * all / ctas to (c + 1) * all / ctas; or, where no sequence is so long that splitting
+    // it would pay for the joining, item c and no other.
     Share from, to;
+    int64_t all;
+    int32_t ctas;
     {
-        const int64_t per_thread = (p.batch + ATPB - 1) / ATPB, b0 = min(p.batch, threadIdx.x * per_thread), b1 = min(p.batch, b0 + per_thread);
+        const int64_t per_thread = (p.batch + S::THREADS - 1) / S::THREADS, b0 = min(p.batch, threadIdx.x * per_thread), b1 = min(p.batch, b0 + per_thread);
         int64_t mine = 0;
-        for (int64_t b = b0; b < b1; ++b) mine += tiles_of(p, b);
+        int32_t most = 0;
+        for (int64_t b = b0; b < b1; ++b) {
+            const int32_t n = steps_of<S::TOKENS>(p, b) + PAD;
+            mine += n;
+            most = max(most, n);
+        }
         int64_t before = mine;
 #pragma unroll
         for (int m = 1; m < 32; m <<= 1) {
             const int64_t v = __shfl_up_sync(0xffffffffu, before, m);
             if (lane >= m) before += v;
         }
-        if (lane == 31) scan[warp] = before;
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 31) scan[warp] = before, longest[warp] = most;
         __syncthreads();
         int64_t total = 0;
         before -= mine;
         for (int w = 0; w < WARPS; ++w) {
             if (w < warp) before += scan[w];
             total += scan[w];
+            most = max(most, longest[w]);
         }
-        // a cut at tile x lies in sequence b where the tiles of one head up to b are at most x / heads
-        const int64_t all = total * heads_per_sequence;
-        int64_t cut[2];
+        all = total * heads_per_sequence;
+        const int64_t items = p.batch * heads_per_sequence;
+        ctas = (int32_t)min((int64_t)gridDim.x, max((int64_t)1, all / (2 * WARPS)));
+        // Joining takes about as long as three rounds of steps.
+        const bool whole_items = items <= gridDim.x && most <= all / ctas + 3 * WARPS;
+        if (whole_items) ctas = (int32_t)items;
+        if (blockIdx.x >= ctas) return;
+        if (whole_items) {
+            from.b = blockIdx.x / heads_per_sequence;
+            from.head = blockIdx.x - (int32_t)from.b * heads_per_sequence;
+            to.b = (blockIdx.x + 1) / heads_per_sequence;
+            to.head = blockIdx.x + 1 - (int32_t)to.b * heads_per_sequence;
+            from.step = to.step = 0;
+        } else {
+            // a cut at step x lies in sequence b where the steps of one head up to b are at most x / heads
+            int64_t cut[2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            cut[e] = (int64_t)(blockIdx.x + e) * all / gridDim.x;
-            const int64_t y = cut[e] / heads_per_sequence;
-            if (y >= before && y < before + mine) {
-                int64_t b = b0, at = before;
-                for (;; ++b) {
-                    const int32_t n = tiles_of(p, b);
-                    if (y < at + n) break;
-                    at += n;
+            for (int e = 0; e < 2; ++e) {
+                cut[e] = (int64_t)(blockIdx.x + e) * all / ctas;
+                const int64_t y = cut[e] / heads_per_sequence;
+                if (y >= before && y < before + mine) {
+                    int64_t b = b0, at = before;
+                    for (;; ++b) {
+                        const int32_t n = steps_of<S::TOKENS>(p, b) + PAD;
+                        if (y < at + n) break;
+                        at += n;
+                    }
+                    ends[e][0] = b;
+                    ends[e][1] = at;
                 }
-                ends[e][0] = b;
-                ends[e][1] = at;
+                if (threadIdx.x == 0 && cut[e] == all) ends[e][0] = p.batch, ends[e][1] = total;
             }
-            if (threadIdx.x == 0 && cut[e] == all) ends[e][0] = p.batch, ends[e][1] = total;
-        }
-        __syncthreads();
-        // With few tiles a CTA, pieces of a tile or two cost more to join than they spare.
-        const int32_t quantum = all >= 16 * (int64_t)gridDim.x ? 1 : 4;
-        Share* const end[2] = {&from, &to};
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            Share& s = *end[e];
-            s.b = ends[e][0];
-            s.head = s.tile = s.tiles = 0;
-            if (s.b < p.batch) {
-                s.tiles = tiles_of(p, s.b);
-                const int64_t in = cut[e] - ends[e][1] * heads_per_sequence;
-                s.head = (int32_t)(in / s.tiles);
-                s.tile = (int32_t)(in - (int64_t)s.head * s.tiles);
-                snap(s, quantum);
-            }
+            __syncthreads();
+            auto place = [&](int e, Share& s) {
+                s.b = ends[e][0];
+                s.head = s.step = 0;
+                if (s.b < p.batch) {
+                    const int32_t n = steps_of<S::TOKENS>(p, s.b) + PAD;
+                    const int64_t in = cut[e] - ends[e][1] * heads_per_sequence;
+                    s.head = (int32_t)(in / n);
+                    s.step = max(0, (int32_t)(in - (int64_t)s.head * n) - PAD);
+                }
+            };
+            place(0, from);
+            place(1, to);
         }
     }
-    auto item_of = [&](const Share& s) { return s.b * heads_per_sequence + s.head; };
-    const int64_t last_item = item_of(to); // nothing of it if to.tile == 0
-
-    int32_t begun = -1, began_with = TAIL_NONE;
+    if (threadIdx.x == 0) {
+        share.all = all;
+        share.ctas = ctas;
+        share.last_item = to.b * heads_per_sequence + to.head; // nothing of it if to_step == 0
+        share.to_step = to.step;
+    }
+    __syncthreads();
     int64_t b = from.b;
-    int32_t hh = from.head, tile0 = from.tile;
+    int32_t hh = from.head, step0 = from.step;
 
-    for (; b < p.batch; tile0 = 0) {
+    for (; b < p.batch; step0 = 0) {
         const int64_t item = b * heads_per_sequence + hh;
+        if (item > share.last_item || (item == share.last_item && share.to_step <= step0)) break;
         int32_t first, n;
         visible(p, b, first, n);
-        const int32_t tiles = max(1, (n - first + CT - 1) / CT);
-        if (item > last_item || (item == last_item && to.tile <= tile0)) break;
-        const int32_t tile1 = item == last_item ? to.tile : tiles;
-        if (tile0 < tile1) {
-            const int kvh = hh / p.tiles, q_first = (hh - kvh * p.tiles) * S::HEADS;
-            const int q_count = min(S::HEADS, p.shared - q_first);
-            const char* const kbase = (const char*)p.cache.k + (int64_t)kvh * p.cache.head_stride * S::ES;
-            const char* const vbase = (const char*)p.cache.v + (int64_t)kvh * p.cache.head_stride * S::ES;
-            const char* const ksbase = (const char*)p.cache.k_scale + (int64_t)kvh * p.cache.scale_head_stride * 2;
-            const char* const vsbase = (const char*)p.cache.v_scale + (int64_t)kvh * p.cache.scale_head_stride * 2;
-            const int32_t* const row_pages = p.pages + b * p.pages_stride;
+        const int32_t steps = max(1, (n - first + S::TOKENS - 1) / S::TOKENS);
+        const int32_t step1 = item == share.last_item ? share.to_step : steps;
+        const int kvh = hh / p.tiles, q_first = (hh - kvh * p.tiles) * S::HEADS;
+        const int q_count = min(S::HEADS, p.shared - q_first);
+        const char* const kbase = (const char*)p.cache.k + (int64_t)kvh * p.cache.head_stride * S::ES + t * S::KP;
+        const char* const vbase = (const char*)p.cache.v + (int64_t)kvh * p.cache.head_stride * S::ES + g * S::VP;
+        const char* const ksbase = (const char*)p.cache.k_scale + (int64_t)kvh * p.cache.scale_head_stride * 2 + (S::KIND == CACHE_I8_GROUPS ? t * S::KG * 2 : 0);
+        const char* const vsbase = (const char*)p.cache.v_scale + (int64_t)kvh * p.cache.scale_head_stride * 2 + (S::KIND == CACHE_I8_GROUPS ? g * (S::VP / S::ES) / 8 * 2 : 0);
+        const int32_t* const row_pages = p.pages + b * p.pages_stride;
 
-            // ---- queries: column g of block nt, the dimensions of quad lane t --------------------------------------------
-            uint32_t q[S::NT][S::STEPS][2];
+        // ---- tokens on their way -----------------------------------------------------------------------------------------
+        // Lane l looks after token l of a step (of l % 16): its page, two steps ahead, then where its row lies, one step ahead.
+        struct Place {
+            int32_t page;
+            uint32_t in_page;
+        };
+        auto find = [&](int32_t step) {
+            const int32_t token = first + step * S::TOKENS + (lane & (S::TOKENS - 1));
+            const uint32_t index = (uint32_t)((uint64_t)(uint32_t)token * p.page_magic >> p.page_shift);
+            Place at;
+            at.page = step < step1 && token < n ? row_pages[index] : -1;
+            at.in_page = token - index * p.cache.page_size;
+            return at;
+        };
+        constexpr uint32_t EVERY = S::SUBS == 2 ? 0xffffffffu : 0xffffu;
+        uint32_t row = 0, scale_row = 0, coming = 0; // of the step that is loaded next: offsets, and which tokens there are
+        auto locate = [&](const Place& at) {
+            const bool ok = (uint32_t)at.page < (uint32_t)p.num_pages;
+            coming = __ballot_sync(0xffffffffu, ok) & EVERY;
+            row = ok ? at.page * p.page_units + at.in_page * p.token_units : 0u;
+            if constexpr (S::KIND != CACHE_F16) scale_row = ok ? at.page * p.scale_page_units + at.in_page * p.scale_token_units : 0u;
+        };
+        uint32_t kw[S::SUBS][2][S::KN][S::KP / 4] = {}, vw[S::SUBS][4][S::VN][S::VP / 4] = {};
+        uint32_t ks[S::SUBS][2][S::KN] = {}, vs[S::SUBS][4][S::VN] = {}; // CACHE_I8_GROUPS
+        uint32_t k_scale = 0, v_scale = 0;                               // CACHE_I8_ROWS: of the lane's token
+        auto load_keys = [&](bool every) {
 #pragma unroll
-            for (int nt = 0; nt < S::NT; ++nt) {
-                const int h = nt * 8 + g;
-                const half* src = p.q + b * p.q_stride + (int64_t)(kvh * p.shared + q_first + h) * S::D;
-                constexpr int EP = S::KP / S::ES; // dimensions of a piece, EP / 4 steps
-#pragma unroll
-                for (int i = 0; i < S::KN; ++i)
-#pragma unroll
-                    for (int s = 0; s < EP / 4; ++s) {
-                        uint2 w = make_uint2(0, 0);
-                        if (h < q_count) w = *reinterpret_cast<const uint2*>(src + (i * 4 + t) * EP + s * 4);
-                        q[nt][i * (EP / 4) + s][0] = S::ES == 2 ? w.x : __byte_perm(w.x, w.y, 0x5410);
-                        q[nt][i * (EP / 4) + s][1] = S::ES == 2 ? w.y : __byte_perm(w.x, w.y, 0x7632);
-                    }
-            }
-
-            float o[S::NT][S::STEPS][4] = {}, top[S::NT][2], sum[S::NT][2] = {};
-#pragma unroll
-            for (int nt = 0; nt < S::NT; ++nt) top[nt][0] = top[nt][1] = -1e30f;
-
-            // ---- tiles on their way ----------------------------------------------------------------------------------------
-            // Lane l looks after token l % 16 of a tile: its page, two tiles ahead, then where its row lies, one tile ahead.
-            struct Place {
-                int32_t page;
-                uint32_t in_page;
-            };
-            auto find = [&](int32_t tile) {
-                const int32_t token = first + tile * CT + warp * WT + (lane & 15);
-                const uint32_t index = (uint32_t)((uint64_t)(uint32_t)token * p.page_magic >> p.page_shift);
-                Place at;
-                at.page = tile < tile1 && token < n ? row_pages[index] : -1;
-                at.in_page = token - index * p.cache.page_size;
-                return at;
-            };
-            uint32_t row = 0, scale_row = 0, coming = 0; // of the tile that is loaded next: offsets, and which tokens there are
-            auto locate = [&](const Place& at) {
-                const bool ok = (uint32_t)at.page < (uint32_t)p.num_pages;
-                coming = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-                row = ok ? at.page * p.page_units + at.in_page * p.token_units : 0u;
-                if constexpr (S::KIND != CACHE_F16) scale_row = ok ? at.page * p.scale_page_units + at.in_page * p.scale_token_units : 0u;
-            };
-            uint32_t kw[2][S::KN][S::KP / 4] = {}, vw[4][S::VN][S::VP / 4] = {};
-            uint32_t ks[2][S::KN] = {}, vs[4][S::VN] = {}; // CACHE_I8_GROUPS
-            uint32_t scale_bits = 0;                       // CACHE_I8_ROWS: key scale of a token in lanes 0 to 15, value scale in the others
-            auto load_keys = [&](bool all) {
+            for (int sub = 0; sub < S::SUBS; ++sub)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const int token = g + 8 * r;
-                    const char* src = kbase + (uint64_t)__shfl_sync(0xffffffffu, row, token) * p.unit + t * S::KP;
+                    const int token = 16 * sub + g + 8 * r;
+                    const char* src = kbase + (uint64_t)__shfl_sync(0xffffffffu, row, token) * p.unit;
                     const char* scales = ksbase;
-                    if constexpr (S::KIND == CACHE_I8_GROUPS) scales += (uint64_t)__shfl_sync(0xffffffffu, scale_row, token) * p.scale_unit + t * S::KG * 2;
-                    const bool there = all || (coming >> token & 1);
+                    if constexpr (S::KIND == CACHE_I8_GROUPS) scales += (uint64_t)__shfl_sync(0xffffffffu, scale_row, token) * p.scale_unit;
+                    const bool there = every || (coming >> token & 1);
 #pragma unroll
                     for (int i = 0; i < S::KN; ++i) {
                         if (there) {
-                            load_piece<S::KP>(kw[r][i], src + i * 4 * S::KP);
-                            if constexpr (S::KIND == CACHE_I8_GROUPS) ks[r][i] = load_scales<S::KG>(scales + i * 4 * S::KG * 2);
+                            load_piece<S::KP>(kw[sub][r][i], src + i * 4 * S::KP);
+                            if constexpr (S::KIND == CACHE_I8_GROUPS) ks[sub][r][i] = load_scales<S::KG>(scales + i * 4 * S::KG * 2);
                         } else { // zeros: what lies there may be anything
 #pragma unroll
-                            for (int x = 0; x < S::KP / 4; ++x) kw[r][i][x] = 0;
-                            ks[r][i] = 0;
+                            for (int x = 0; x < S::KP / 4; ++x) kw[sub][r][i][x] = 0;
+                            ks[sub][r][i] = 0;
                         }
                     }
                 }
-            };
-            auto load_values = [&](bool all) {
+            if constexpr (S::KIND == CACHE_I8_ROWS)
+                k_scale = (every || (coming >> (lane & (S::TOKENS - 1)) & 1)) ? load_scales<1>(ksbase + (uint64_t)scale_row * p.scale_unit) : 0u;
+        };
+        auto load_values = [&](bool every) {
+#pragma unroll
+            for (int sub = 0; sub < S::SUBS; ++sub)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int token = 2 * t + (j & 1) + 8 * (j >> 1);
-                    const char* src = vbase + (uint64_t)__shfl_sync(0xffffffffu, row, token) * p.unit + g * S::VP;
+                    const int token = 16 * sub + 2 * t + (j & 1) + 8 * (j >> 1);
+                    const char* src = vbase + (uint64_t)__shfl_sync(0xffffffffu, row, token) * p.unit;
                     const char* scales = vsbase;
                     if constexpr (S::KIND == CACHE_I8_GROUPS) scales += (uint64_t)__shfl_sync(0xffffffffu, scale_row, token) * p.scale_unit;
-                    const bool there = all || (coming >> token & 1);
+                    const bool there = every || (coming >> token & 1);
 #pragma unroll
                     for (int i = 0; i < S::VN; ++i) {
                         constexpr int EP = S::VP / S::ES;
                         if (there) {
-                            load_piece<S::VP>(vw[j][i], src + i * 8 * S::VP);
-                            if constexpr (S::KIND == CACHE_I8_GROUPS) vs[j][i] = load_scales<S::VG>(scales + (i * 8 + g) * EP / 8 * 2);
+                            load_piece<S::VP>(vw[sub][j][i], src + i * 8 * S::VP);
+                            if constexpr (S::KIND == CACHE_I8_GROUPS) vs[sub][j][i] = load_scales<S::VG>(scales + i * 8 * EP / 8 * 2);
                         } else {
 #pragma unroll
-                            for (int x = 0; x < S::VP / 4; ++x) vw[j][i][x] = 0;
-                            vs[j][i] = 0;
+                            for (int x = 0; x < S::VP / 4; ++x) vw[sub][j][i][x] = 0;
+                            vs[sub][j][i] = 0;
                         }
                     }
                 }
-                if constexpr (S::KIND == CACHE_I8_ROWS)
-                    scale_bits = (coming >> (lane & 15) & 1) ? load_scales<1>((lane < 16 ? ksbase : vsbase) + (uint64_t)scale_row * p.scale_unit) : 0u;
-            };
+            if constexpr (S::KIND == CACHE_I8_ROWS)
+                v_scale = (every || (coming >> (lane & (S::TOKENS - 1)) & 1)) ? load_scales<1>(vsbase + (uint64_t)scale_row * p.scale_unit) : 0u;
+        };
 
-            Place ahead = find(tile0);
-            {
-                const Place second = find(tile0 + 1);
-                locate(ahead);
-                ahead = second;
+        Place ahead = find(step0 + warp);
+        const Place second = find(step0 + warp + WARPS);
+        // the queries, while the pages are looked up: column g of block nt, the dimensions of quad lane t
+        uint32_t q[S::NT][S::STEPS][2];
+#pragma unroll
+        for (int nt = 0; nt < S::NT; ++nt) {
+            const int h = nt * 8 + g;
+            const half* src = p.q + b * p.q_stride + (int64_t)(kvh * p.shared + q_first + h) * S::D;
+            constexpr int EP = S::KP / S::ES; // dimensions of a piece
+#pragma unroll
+            for (int i = 0; i < S::KN; ++i)
+#pragma unroll
+                for (int s = 0; s < EP / 4; ++s) {
+                    uint2 w = make_uint2(0, 0);
+                    if (h < q_count) w = *reinterpret_cast<const uint2*>(src + (i * 4 + t) * EP + s * 4);
+                    const bool apart = S::ES == 1; // dimensions 0, 2 and 1, 3, as they come out of a word of bytes
+                    q[nt][i * (EP / 4) + s][0] = apart ? __byte_perm(w.x, w.y, 0x5410) : w.x;
+                    q[nt][i * (EP / 4) + s][1] = apart ? __byte_perm(w.x, w.y, 0x7632) : w.y;
+                }
+        }
+        locate(ahead);
+        ahead = second;
+        uint32_t seen = coming;
+        if (seen == EVERY) load_keys(true), load_values(true);
+        else if (seen) load_keys(false), load_values(false);
+        locate(ahead);
+        ahead = find(step0 + warp + 2 * WARPS);
+
+        // CACHE_I8_ROWS: keys enter the product as (value + 128) * 2^-24, exactly; 128 * 2^-24 times the sum of a query's elements is taken
+        // off its scores, here for the lane's two heads.
+        float off[S::NT][2] = {};
+        if constexpr (S::KIND == CACHE_I8_ROWS) {
+#pragma unroll
+            for (int nt = 0; nt < S::NT; ++nt) {
+                float all_dims = 0.0f;
+#pragma unroll
+                for (int s = 0; s < S::STEPS; ++s)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float2 f = __half22float2(as_h2(q[nt][s][x]));
+                        all_dims += f.x + f.y;
+                    }
+                all_dims += __shfl_xor_sync(0xffffffffu, all_dims, 1);
+                all_dims += __shfl_xor_sync(0xffffffffu, all_dims, 2);
+                off[nt][0] = __shfl_sync(0xffffffffu, all_dims, 8 * t) * 0x1p-17f;
+                off[nt][1] = __shfl_sync(0xffffffffu, all_dims, 8 * t + 4) * 0x1p-17f;
             }
-            uint32_t seen = coming;
-            if (seen == 0xffffu) load_keys(true), load_values(true);
-            else if (seen) load_keys(false), load_values(false);
-            locate(ahead);
-            ahead = find(tile0 + 2);
+        }
 
-            for (int32_t tile = tile0; tile < tile1; ++tile) {
-                float c[S::NT][4] = {};
-                if (seen != 0) {
-                    // ---- scores [16 tokens x 8 heads], in two chains -----------------------------------------------------------
-                    float c2[S::NT][4] = {};
-                    constexpr int KW = S::KP / 4;
+        float o[S::NT][S::STEPS][4] = {}, top[S::NT][2], sum[S::NT][2] = {};
 #pragma unroll
-                    for (int i = 0; i < S::KN; ++i) {
-                        if constexpr (S::ES == 2) {
+        for (int nt = 0; nt < S::NT; ++nt) top[nt][0] = top[nt][1] = -1e30f;
+
+        for (int32_t step = step0 + warp; step < step1; step += WARPS) {
+            float c[S::SUBS][S::NT][4];
+            if (seen != 0) {
+                // ---- scores [16 tokens x 8 heads] ------------------------------------------------------------------------
+                constexpr int KW = S::KP / 4;
 #pragma unroll
-                            for (int s = 0; s < KW / 2; ++s)
+                for (int sub = 0; sub < S::SUBS; ++sub) {
+                    {
+                        float c2[S::NT][4] = {}; // a second chain
 #pragma unroll
-                                for (int nt = 0; nt < S::NT; ++nt) {
-                                    const auto& qs = q[nt][i * (KW / 2) + s];
-                                    mma(s & 1 ? c2[nt] : c[nt], kw[0][i][2 * s], kw[1][i][2 * s], kw[0][i][2 * s + 1], kw[1][i][2 * s + 1], qs[0], qs[1]);
+                        for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) c[sub][nt][x] = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < S::KN; ++i) {
+                            if constexpr (S::KIND == CACHE_F16) {
+#pragma unroll
+                                for (int s = 0; s < KW / 2; ++s)
+#pragma unroll
+                                    for (int nt = 0; nt < S::NT; ++nt) {
+                                        const auto& qs = q[nt][i * (KW / 2) + s];
+                                        mma(s & 1 ? c2[nt] : c[sub][nt], kw[sub][0][i][2 * s], kw[sub][1][i][2 * s], kw[sub][0][i][2 * s + 1], kw[sub][1][i][2 * s + 1], qs[0], qs[1]);
+                                    }
+                            } else if constexpr (S::KIND == CACHE_I8_ROWS) {
+#pragma unroll
+                                for (int s = 0; s < KW; ++s) {
+                                    const uint32_t w0 = kw[sub][0][i][s], w1 = kw[sub][1][i][s];
+                                    const uint32_t a0 = spread(w0, p.flip), a1 = spread(w1, p.flip), a2 = spread(w0 >> 8, p.flip), a3 = spread(w1 >> 8, p.flip);
+#pragma unroll
+                                    for (int nt = 0; nt < S::NT; ++nt) mma(s & 1 ? c2[nt] : c[sub][nt], a0, a1, a2, a3, q[nt][i * KW + s][0], q[nt][i * KW + s][1]);
                                 }
-                        } else {
+                            } else {
 #pragma unroll
-                            for (int s = 0; s < KW; ++s) {
-                                uint32_t a0, a1, a2, a3;
-                                widen(kw[0][i][s], a0, a2);
-                                widen(kw[1][i][s], a1, a3);
-                                if constexpr (S::KIND == CACHE_I8_GROUPS) {
+                                for (int s = 0; s < KW; ++s) {
+                                    uint32_t a0, a1, a2, a3;
+                                    widen(p, kw[sub][0][i][s], a0, a2);
+                                    widen(p, kw[sub][1][i][s], a1, a3);
                                     // value x scale has up to 18 bits: its rounding to fp16, and what that left, as a second operand
-                                    const __half2 f0 = as_h2(__byte_perm(ks[0][i], 0, s < 2 ? 0x1010 : 0x3232)), f1 = as_h2(__byte_perm(ks[1][i], 0, s < 2 ? 0x1010 : 0x3232));
+                                    const __half2 f0 = as_h2(__byte_perm(ks[sub][0][i], 0, s < 2 ? 0x1010 : 0x3232)), f1 = as_h2(__byte_perm(ks[sub][1][i], 0, s < 2 ? 0x1010 : 0x3232));
                                     const __half2 h0 = __hmul2(as_h2(a0), f0), h1 = __hmul2(as_h2(a1), f1), h2_ = __hmul2(as_h2(a2), f0), h3 = __hmul2(as_h2(a3), f1);
                                     const uint32_t r0 = h2(__hfma2(as_h2(a0), f0, __hneg2(h0))), r1 = h2(__hfma2(as_h2(a1), f1, __hneg2(h1)));
                                     const uint32_t r2 = h2(__hfma2(as_h2(a2), f0, __hneg2(h2_))), r3 = h2(__hfma2(as_h2(a3), f1, __hneg2(h3)));
 #pragma unroll
                                     for (int nt = 0; nt < S::NT; ++nt) {
                                         const auto& qs = q[nt][i * KW + s];
-                                        mma(c[nt], h2(h0), h2(h1), h2(h2_), h2(h3), qs[0], qs[1]);
+                                        mma(c[sub][nt], h2(h0), h2(h1), h2(h2_), h2(h3), qs[0], qs[1]);
                                         mma(c2[nt], r0, r1, r2, r3, qs[0], qs[1]);
                                     }
-                                } else {
-#pragma unroll
-                                    for (int nt = 0; nt < S::NT; ++nt) mma(s & 1 ? c2[nt] : c[nt], a0, a1, a2, a3, q[nt][i * KW + s][0], q[nt][i * KW + s][1]);
                                 }
                             }
                         }
-                    }
-#pragma unroll
-                    for (int nt = 0; nt < S::NT; ++nt)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) c[nt][x] += c2[nt][x];
-                }
-                if (coming == 0xffffu) load_keys(true);
-                else if (coming) load_keys(false);
-
-                if (seen != 0) {
-                    // ---- weights: 2^(score - top + 8) ----------------------------------------------------------------------
-                    float f0 = p.scale_log2, f1 = p.scale_log2, v0 = 1.0f, v1 = 1.0f, e0 = 0.0f, e1 = 0.0f;
-                    if constexpr (S::KIND == CACHE_I8_ROWS) {
-                        const float mine = __half2float(__ushort_as_half((unsigned short)scale_bits));
-                        f0 *= __shfl_sync(0xffffffffu, mine, g);
-                        f1 *= __shfl_sync(0xffffffffu, mine, g + 8);
-                        v0 = __shfl_sync(0xffffffffu, mine, g + 16);
-                        v1 = __shfl_sync(0xffffffffu, mine, g + 24);
-                        // the value's scale goes into the weight; 2^e is above it
-                        e0 = (float)max((int)(__float_as_uint(v0) >> 23) - 126, -24);
-                        e1 = (float)max((int)(__float_as_uint(v1) >> 23) - 126, -24);
-                    }
-                    bool higher = false;
-#pragma unroll
-                    for (int nt = 0; nt < S::NT; ++nt) {
-                        c[nt][0] *= f0; c[nt][1] *= f0;
-                        c[nt][2] *= f1; c[nt][3] *= f1;
-                    }
-                    if (seen != 0xffffu) {
-#pragma unroll
-                        for (int nt = 0; nt < S::NT; ++nt) {
-                            if (!(seen >> g & 1)) c[nt][0] = c[nt][1] = -INFINITY;
-                            if (!(seen >> (g + 8) & 1)) c[nt][2] = c[nt][3] = -INFINITY;
-                        }
-                    }
-#pragma unroll
-                    for (int nt = 0; nt < S::NT; ++nt) {
-                        higher |= fmaxf(c[nt][0] + e0, c[nt][2] + e1) > top[nt][0] + 6.0f;
-                        higher |= fmaxf(c[nt][1] + e0, c[nt][3] + e1) > top[nt][1] + 6.0f;
-                    }
-                    // The reference exponent need not be the maximum: it moves when a weight would pass 2^14, which after the first tiles is rare.
-                    if (__any_sync(0xffffffffu, higher)) {
 #pragma unroll
                         for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
-                            for (int k = 0; k < 2; ++k) {
-                                float m = fmaxf(c[nt][k] + e0, c[nt][2 + k] + e1);
+                            for (int x = 0; x < 4; ++x) c[sub][nt][x] += c2[nt][x];
+                        if constexpr (S::KIND == CACHE_I8_ROWS) {
+                            const float mine = __half2float(__ushort_as_half((unsigned short)k_scale)) * (p.scale_log2 * 0x1p24f);
+                            const float k0 = __shfl_sync(0xffffffffu, mine, 16 * sub + g), k1 = __shfl_sync(0xffffffffu, mine, 16 * sub + g + 8);
 #pragma unroll
-                                for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-                                m = fmaxf(m, top[nt][k]);
-                                const float keep = exp2_fast(top[nt][k] - m);
-                                top[nt][k] = m;
-                                sum[nt][k] *= keep;
+                            for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
-                                for (int j = 0; j < S::STEPS; ++j) {
-                                    o[nt][j][k] *= keep;
-                                    o[nt][j][2 + k] *= keep;
-                                }
-                            }
+                                for (int x = 0; x < 4; ++x) c[sub][nt][x] = (c[sub][nt][x] - off[nt][x & 1]) * (x < 2 ? k0 : k1);
+                        } else {
+#pragma unroll
+                            for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) c[sub][nt][x] *= p.scale_log2;
+                        }
                     }
+                }
+            }
+            if (coming == EVERY) load_keys(true);
+            else if (coming) load_keys(false);
+
+            if (seen != 0) {
+                // ---- weights: 2^(score - top + 8) --------------------------------------------------------------------------
+                float v0[S::SUBS], v1[S::SUBS], e0[S::SUBS] = {}, e1[S::SUBS] = {};
+                if constexpr (S::KIND == CACHE_I8_ROWS) {
+                    // a value's scale goes into its weight, the scale's logarithm into what decides about the reference exponent
+                    const float mine = __half2float(__ushort_as_half((unsigned short)v_scale)), size = fmaxf(log2_fast(mine), -24.0f);
+#pragma unroll
+                    for (int sub = 0; sub < S::SUBS; ++sub) {
+                        v0[sub] = __shfl_sync(0xffffffffu, mine, 16 * sub + g);
+                        v1[sub] = __shfl_sync(0xffffffffu, mine, 16 * sub + g + 8);
+                        e0[sub] = __shfl_sync(0xffffffffu, size, 16 * sub + g);
+                        e1[sub] = __shfl_sync(0xffffffffu, size, 16 * sub + g + 8);
+                    }
+                }
+                if (seen != EVERY) {
+#pragma unroll
+                    for (int sub = 0; sub < S::SUBS; ++sub)
+#pragma unroll
+                        for (int nt = 0; nt < S::NT; ++nt) {
+                            if (!(seen >> (16 * sub + g) & 1)) c[sub][nt][0] = c[sub][nt][1] = -INFINITY;
+                            if (!(seen >> (16 * sub + g + 8) & 1)) c[sub][nt][2] = c[sub][nt][3] = -INFINITY;
+                        }
+                }
+                float high[S::NT][2];
+                bool higher = false;
+#pragma unroll
+                for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        high[nt][k] = fmaxf(c[0][nt][k] + e0[0], c[0][nt][2 + k] + e1[0]);
+                        if constexpr (S::SUBS == 2) high[nt][k] = fmaxf(high[nt][k], fmaxf(c[S::SUBS - 1][nt][k] + e0[S::SUBS - 1], c[S::SUBS - 1][nt][2 + k] + e1[S::SUBS - 1]));
+                        higher |= high[nt][k] > top[nt][k] + 6.0f;
+                    }
+                // The reference exponent need not be the maximum: it moves when a weight would pass 2^14, which after the first steps is rare.
+                if (__any_sync(0xffffffffu, higher)) {
+#pragma unroll
+                    for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            float m = high[nt][k];
+#pragma unroll
+                            for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+                            m = fmaxf(m, top[nt][k]);
+                            const float keep = exp2_fast(top[nt][k] - m);
+                            top[nt][k] = m;
+                            sum[nt][k] *= keep;
+#pragma unroll
+                            for (int j = 0; j < S::STEPS; ++j) {
+                                o[nt][j][k] *= keep;
+                                o[nt][j][2 + k] *= keep;
+                            }
+                        }
+                }
+#pragma unroll
+                for (int sub = 0; sub < S::SUBS; ++sub) {
                     uint32_t wh[S::NT][2], wl[S::NT][2]; // weights in fp16, and what the rounding left: together 22 bits
 #pragma unroll
                     for (int nt = 0; nt < S::NT; ++nt) {
-                        const float a = exp2_fast(c[nt][0] - (top[nt][0] - 8.0f)), b2 = exp2_fast(c[nt][1] - (top[nt][1] - 8.0f));
-                        const float a1 = exp2_fast(c[nt][2] - (top[nt][0] - 8.0f)), b1 = exp2_fast(c[nt][3] - (top[nt][1] - 8.0f));
-                        sum[nt][0] += a + a1;
-                        sum[nt][1] += b2 + b1;
-                        const __half2 x = __floats2half2_rn(a * v0, b2 * v0), y = __floats2half2_rn(a1 * v1, b1 * v1);
-                        const float2 xf = __half22float2(x), yf = __half22float2(y);
-                        wh[nt][0] = transpose8x8(h2(x));
-                        wh[nt][1] = transpose8x8(h2(y));
-                        wl[nt][0] = transpose8x8(h2(__floats2half2_rn(a * v0 - xf.x, b2 * v0 - xf.y)));
-                        wl[nt][1] = transpose8x8(h2(__floats2half2_rn(a1 * v1 - yf.x, b1 * v1 - yf.y)));
+                        float w[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) w[x] = exp2_fast(c[sub][nt][x] - (top[nt][x & 1] - 8.0f));
+                        sum[nt][0] += w[0] + w[2];
+                        sum[nt][1] += w[1] + w[3];
+                        if constexpr (S::KIND == CACHE_I8_ROWS) {
+                            w[0] *= v0[sub]; w[1] *= v0[sub];
+                            w[2] *= v1[sub]; w[3] *= v1[sub];
+                        }
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const __half2 x = __floats2half2_rn(w[2 * r], w[2 * r + 1]);
+                            const float2 f = __half22float2(x);
+                            wh[nt][r] = transpose8x8(h2(x));
+                            wl[nt][r] = transpose8x8(h2(__floats2half2_rn(w[2 * r] - f.x, w[2 * r + 1] - f.y)));
+                        }
                     }
 
-                    // ---- values^T x weights^T ------------------------------------------------------------------------------
+                    // ---- values^T x weights^T ----------------------------------------------------------------------------------
                     constexpr int VW = S::VP / 4, EP = S::VP / S::ES; // words and dimensions of a piece
 #pragma unroll
                     for (int i = 0; i < S::VN; ++i) {
-                        if constexpr (S::ES == 2) {
+                        const auto& w = vw[sub];
 #pragma unroll
-                            for (int x = 0; x < VW; ++x) {
-                                const uint32_t a0 = __byte_perm(vw[0][i][x], vw[1][i][x], 0x5410), a1 = __byte_perm(vw[0][i][x], vw[1][i][x], 0x7632);
-                                const uint32_t a2 = __byte_perm(vw[2][i][x], vw[3][i][x], 0x5410), a3 = __byte_perm(vw[2][i][x], vw[3][i][x], 0x7632);
+                        for (int x = 0; x < VW; ++x) {
+                            if constexpr (S::ES == 2) {
+                                const uint32_t a0 = __byte_perm(w[0][i][x], w[1][i][x], 0x5410), a1 = __byte_perm(w[0][i][x], w[1][i][x], 0x7632);
+                                const uint32_t a2 = __byte_perm(w[2][i][x], w[3][i][x], 0x5410), a3 = __byte_perm(w[2][i][x], w[3][i][x], 0x7632);
 #pragma unroll
                                 for (int nt = 0; nt < S::NT; ++nt) {
                                     mma(o[nt][i * EP / 2 + x], a0, a1, a2, a3, wh[nt][0], wh[nt][1]);
                                     mma(o[nt][i * EP / 2 + x], a0, a1, a2, a3, wl[nt][0], wl[nt][1]);
                                 }
-                            }
-                        } else {
-#pragma unroll
-                            for (int x = 0; x < VW; ++x) {
+                            } else {
                                 uint32_t u[4], v[4];
-                                widen_pairs(vw[0][i][x], vw[1][i][x], u);
-                                widen_pairs(vw[2][i][x], vw[3][i][x], v);
+                                widen_pairs(p, w[0][i][x], w[1][i][x], u);
+                                widen_pairs(p, w[2][i][x], w[3][i][x], v);
                                 if constexpr (S::KIND == CACHE_I8_GROUPS) {
                                     // these four dimensions are of one group; value x scale is rounded to fp16, as it is when it is read back
-                                    const __half2 fu = as_h2(__byte_perm(vs[0][i], vs[1][i], x < 2 ? 0x5410 : 0x7632));
-                                    const __half2 fv = as_h2(__byte_perm(vs[2][i], vs[3][i], x < 2 ? 0x5410 : 0x7632));
+                                    const __half2 fu = as_h2(__byte_perm(vs[sub][0][i], vs[sub][1][i], x < 2 ? 0x5410 : 0x7632));
+                                    const __half2 fv = as_h2(__byte_perm(vs[sub][2][i], vs[sub][3][i], x < 2 ? 0x5410 : 0x7632));
 #pragma unroll
                                     for (int y = 0; y < 4; ++y) {
                                         u[y] = h2(__hmul2(as_h2(u[y]), fu));
@@ -497,153 +600,113 @@ __global__ void __launch_bounds__(ATPB, S::CTAS) paged_attention_kernel(const __
                         }
                     }
                 }
-                if (coming == 0xffffu) load_values(true);
-                else if (coming) load_values(false);
-                seen = coming;
-                locate(ahead);
-                ahead = find(tile + 3);
             }
-
-            // ---- the four warps' sums --------------------------------------------------------------------------------------
-#pragma unroll
-            for (int nt = 0; nt < S::NT; ++nt) {
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    float s = sum[nt][k];
-#pragma unroll
-                    for (int x = 4; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-                    const int h = nt * 8 + 2 * t + k;
-                    if (g == 0) {
-                        tops[(warp * S::HEADS + h) * 2] = top[nt][k];
-                        tops[(warp * S::HEADS + h) * 2 + 1] = s;
-                    }
-                    constexpr int EP = S::VP / S::ES;
-#pragma unroll
-                    for (int i = 0; i < S::VN; ++i)
-#pragma unroll
-                        for (int x = 0; x < EP; x += 4)
-                            *reinterpret_cast<float4*>(&part[(warp * S::HEADS + h) * S::ROW + (i * 8 + g) * EP + x]) =
-                                make_float4(o[nt][(i * EP + x) / 2][k], o[nt][(i * EP + x) / 2][2 + k], o[nt][(i * EP + x) / 2 + 1][k], o[nt][(i * EP + x) / 2 + 1][2 + k]);
-                }
-            }
-            __syncthreads();
-            const bool whole = tile0 == 0 && tile1 == tiles;
-            const int64_t slot = 2 * (int64_t)blockIdx.x + (tile0 == 0 ? 1 : 0);
-            for (int x = threadIdx.x; x < q_count * (S::D / 4); x += ATPB) {
-                const int h = x / (S::D / 4), d = (x - h * (S::D / 4)) * 4;
-                float m = -1e30f, l = 0.0f;
-                float4 v = make_float4(0, 0, 0, 0);
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) m = fmaxf(m, tops[(w * S::HEADS + h) * 2]);
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) {
-                    const float f = exp2_fast(tops[(w * S::HEADS + h) * 2] - m);
-                    const float4 a = *reinterpret_cast<const float4*>(&part[(w * S::HEADS + h) * S::ROW + d]);
-                    l += f * tops[(w * S::HEADS + h) * 2 + 1];
-                    v.x += f * a.x; v.y += f * a.y; v.z += f * a.z; v.w += f * a.w;
-                }
-                if (whole) {
-                    const int head = kvh * p.shared + q_first + h;
-                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                    const uint2 r = make_uint2(h2(__floats2half2_rn(v.x * inv, v.y * inv)), h2(__floats2half2_rn(v.z * inv, v.w * inv)));
-                    *reinterpret_cast<uint2*>(p.out + b * p.out_stride + (int64_t)head * S::D + d) = r;
-                    if (p.lse && d == 0) p.lse[b * p.q_heads + head] = l == 0.0f ? -INFINITY : (m - 8.0f + log2f(l)) * 0.69314718055994531f;
-                } else {
-                    *reinterpret_cast<float4*>(p.sums + (slot * S::HEADS + h) * S::D + d) = v;
-                    if (d == 0) p.tops[slot * S::HEADS + h] = make_float2(m, l);
-                }
-            }
-            __syncthreads();
-            if (tile0 != 0) began_with = tile1 == tiles ? TAIL_END : TAIL_MORE;
-            else if (!whole) begun = (int32_t)item;
+            if (coming == EVERY) load_values(true);
+            else if (coming) load_values(false);
+            seen = coming;
+            locate(ahead);
+            ahead = find(step + 3 * WARPS);
         }
+
+        // ---- the warps' sums -------------------------------------------------------------------------------------------------
+#pragma unroll
+        for (int nt = 0; nt < S::NT; ++nt) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float s = sum[nt][k];
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+                const int h = nt * 8 + 2 * t + k;
+                if (g == 0) tops[warp * S::HEADS + h] = make_float2(top[nt][k], s);
+                constexpr int EP = S::VP / S::ES;
+#pragma unroll
+                for (int i = 0; i < S::VN; ++i)
+#pragma unroll
+                    for (int x = 0; x < EP; x += 4)
+                        *reinterpret_cast<float4*>(&part[(warp * S::HEADS + h) * S::ROW + (i * 8 + g) * EP + x]) =
+                            make_float4(o[nt][(i * EP + x) / 2][k], o[nt][(i * EP + x) / 2][2 + k], o[nt][(i * EP + x) / 2 + 1][k], o[nt][(i * EP + x) / 2 + 1][2 + k]);
+            }
+        }
+        __syncthreads();
+        const bool whole = step0 == 0 && step1 == steps;
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (step0 == 0 ? 1 : 0);
+        const int head0 = kvh * p.shared + q_first;
+        for (int x = threadIdx.x; x < q_count * (S::D / 4); x += S::THREADS) {
+            const int h = x / (S::D / 4), d = (x - h * (S::D / 4)) * 4;
+            float m = -1e30f, l = 0.0f;
+            float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) m = fmaxf(m, tops[w * S::HEADS + h].x);
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float2 s = tops[w * S::HEADS + h];
+                const float f = exp2_fast(s.x - m);
+                const float4 a = *reinterpret_cast<const float4*>(&part[(w * S::HEADS + h) * S::ROW + d]);
+                l += f * s.y;
+                v.x += f * a.x; v.y += f * a.y; v.z += f * a.z; v.w += f * a.w;
+            }
+            if (whole) {
+                finish(p, b, head0 + h, S::D, d, v, m, l);
+            } else {
+                __stcg(reinterpret_cast<float4*>(p.sums + (slot * S::HEADS + h) * S::D + d), v);
+                if (d == 0) __stcg(&p.tops[slot * S::HEADS + h], make_float2(m, l));
+            }
+        }
+
+        // ---- an item in pieces: the CTA that is last to have its sums in the workspace joins them, in the order of the tokens ----
+        if (!whole) {
+            // CTAs whose shares begin inside the item: c with begin < c * all / ctas < end, rounded down
+            const int64_t all = share.all, ctas = share.ctas;
+            const int64_t begin = step1 < steps ? (int64_t)(blockIdx.x + 1) * all / ctas - step1 : (int64_t)blockIdx.x * all / ctas - step0;
+            const int64_t end = begin + steps;
+            const int32_t c0 = (int32_t)(((begin + 1) * ctas + all - 1) / all), c1 = (int32_t)((end * ctas + all - 1) / all);
+            const int32_t pieces = c1 - c0 + 1; // the first is the one of CTA c0 - 1, which began the item
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                is_last = atomicAdd(&p.arrived[c0 - 1], 1u) == (uint32_t)(pieces - 1);
+                if (is_last) p.arrived[c0 - 1] = 0; // for the next call
+            }
+            __syncthreads();
+            if (is_last) {
+                __threadfence();
+                constexpr int BATCH = 8;
+                auto slot_of = [&](int32_t i) { return i == 0 ? 2 * (int64_t)(c0 - 1) + 1 : 2 * (int64_t)(c0 - 1 + i); };
+                for (int x = threadIdx.x; x < q_count * (S::D / 4); x += S::THREADS) {
+                    const int h = x / (S::D / 4), d = (x - h * (S::D / 4)) * 4;
+                    float m = -1e30f, l = 0.0f;
+                    float4 v = make_float4(0, 0, 0, 0);
+                    for (int32_t i = 0; i < pieces; i += BATCH) {
+                        float2 s[BATCH];
+                        float4 a[BATCH];
+#pragma unroll
+                        for (int j = 0; j < BATCH; ++j) {
+                            const int64_t at = slot_of(min(i + j, pieces - 1)) * S::HEADS + h;
+                            s[j] = __ldcg(&p.tops[at]);
+                            a[j] = __ldcg(reinterpret_cast<const float4*>(p.sums + at * S::D + d));
+                            if (i + j >= pieces) s[j] = make_float2(-1e30f, 0.0f);
+                        }
+                        float up = m;
+#pragma unroll
+                        for (int j = 0; j < BATCH; ++j) up = fmaxf(up, s[j].x);
+                        const float keep = exp2_fast(m - up);
+                        m = up;
+                        l *= keep;
+                        v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
+#pragma unroll
+                        for (int j = 0; j < BATCH; ++j) {
+                            const float f = i + j < pieces ? exp2_fast(s[j].x - m) : 0.0f;
+                            l += f * s[j].y;
+                            if (i + j < pieces) v.x += f * a[j].x, v.y += f * a[j].y, v.z += f * a[j].z, v.w += f * a[j].w;
+                        }
+                    }
+                    finish(p, b, head0 + h, S::D, d, v, m, l);
+                }
+            }
+        }
+        __syncthreads();
         if (++hh == heads_per_sequence) hh = 0, ++b;
     }
-    if (threadIdx.x == 0 && p.items) *reinterpret_cast<int2*>(p.items + 2 * blockIdx.x) = make_int2(begun, began_with);
-}
-
-// Joins the pieces of the item that CTA blockIdx.x began and others went on with: four warps for each of two query heads, every fourth
-// piece to a warp, in an order that does not change.
-constexpr int JTPB = 256, JWARPS = 4;
-template <int D, int HEADS>
-__global__ void __launch_bounds__(JTPB) paged_attention_join_kernel(const __grid_constant__ AttentionParams p, int32_t ctas) {
-    constexpr int V = D / 32;
-    __shared__ int32_t slots[kMostCtas];
-    __shared__ float weights[2][kMostCtas], part[2][JWARPS][D], total[2];
-    __shared__ int32_t count;
-    pdl_wait_prior_grid();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, side = warp / JWARPS, w = warp - side * JWARPS;
-    const int32_t item = p.items[2 * blockIdx.x];
-    if (item < 0) return;
-    const int heads_per_sequence = p.cache.kv_heads * p.tiles;
-    const int64_t b = item / heads_per_sequence;
-    const int hh = (int)(item - b * heads_per_sequence), kvh = hh / p.tiles, q_first = (hh - kvh * p.tiles) * HEADS;
-    const int heads = min(HEADS, p.shared - q_first), h = blockIdx.y * 2 + side;
-    if ((int)blockIdx.y * 2 >= heads) return;
-
-    // the pieces: this CTA's own, then those with which the next CTAs' shares begin, up to the one that ends the item
-    if (warp == 0) {
-        int32_t found = 1;
-        if (lane == 0) slots[0] = 2 * blockIdx.x + 1;
-        for (int32_t c0 = blockIdx.x + 1; c0 < ctas; c0 += 32) {
-            const int32_t c = c0 + lane, kind = c < ctas ? p.items[2 * c + 1] : TAIL_NONE;
-            const uint32_t end = __ballot_sync(0xffffffffu, kind == TAIL_END);
-            const uint32_t upto = end ? (end & (0u - end)) * 2u - 1u : 0xffffffffu;
-            const uint32_t has = __ballot_sync(0xffffffffu, kind != TAIL_NONE) & upto;
-            if (has >> lane & 1) slots[found + __popc(has & ((1u << lane) - 1))] = 2 * c;
-            found += __popc(has);
-            if (end) break;
-        }
-        if (lane == 0) count = found;
-    }
-    __syncthreads();
-    const int32_t pieces = count;
-    // their factors, by the first warp of each head
-    float m = -1e30f;
-    if (w == 0 && h < heads) {
-        for (int i = lane; i < pieces; i += 32) m = fmaxf(m, p.tops[(int64_t)slots[i] * HEADS + h].x);
-#pragma unroll
-        for (int x = 16; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-        float l = 0.0f;
-        for (int i = lane; i < pieces; i += 32) {
-            const float2 s = p.tops[(int64_t)slots[i] * HEADS + h];
-            const float f = exp2_fast(s.x - m);
-            weights[side][i] = f;
-            l += f * s.y;
-        }
-#pragma unroll
-        for (int x = 16; x >= 1; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-        if (lane == 0) total[side] = l;
-    }
-    __syncthreads();
-    float o[V] = {};
-    if (h < heads) {
-        for (int i0 = w; i0 < pieces; i0 += 4 * JWARPS) {
-            float v[4][V];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int x = 0; x < V; ++x) v[u][x] = i0 + u * JWARPS < pieces ? p.sums[((int64_t)slots[i0 + u * JWARPS] * HEADS + h) * D + x * 32 + lane] : 0.0f;
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int x = 0; x < V; ++x)
-                    if (i0 + u * JWARPS < pieces) o[x] += weights[side][i0 + u * JWARPS] * v[u][x];
-        }
-    }
-#pragma unroll
-    for (int x = 0; x < V; ++x) part[side][w][x * 32 + lane] = o[x];
-    __syncthreads();
-    if (h >= heads) return;
-    const int head = kvh * p.shared + q_first + h;
-    const float l = total[side], inv = l == 0.0f ? 0.0f : 1.0f / l;
-    for (int d = w * 32 + lane; d < D; d += JWARPS * 32) {
-        float v = 0.0f;
-#pragma unroll
-        for (int x = 0; x < JWARPS; ++x) v += part[side][x][d];
-        p.out[b * p.out_stride + (int64_t)head * D + d] = __float2half_rn(v * inv);
-    }
-    if (p.lse && w == 0 && lane == 0) p.lse[b * p.q_heads + head] = l == 0.0f ? -INFINITY : (m - 8.0f + log2f(l)) * 0.69314718055994531f;
 }
 
 // Strides in bytes -> in units of the largest power of two that divides them; false where an offset would not fit 32 bits.
@@ -670,18 +733,11 @@ void page_division(uint32_t d, uint32_t& magic, uint32_t& shift) {
 int heads_at_once(int32_t head_dim, int32_t shared) { return shared > 8 && head_dim <= 128 ? 16 : 8; }
 template <class S>
 int32_t launch(cudaStream_t stream, AttentionParams& p, int64_t tokens) {
-    static_assert(S::CTAS * kSms <= kMostCtas, "workspace");
-    const int64_t tiles = (tokens + CT - 1) / CT;
-    const int64_t items = p.batch * p.cache.kv_heads * p.tiles;
-    const int64_t most = S::CTAS * kSms;
-    const int64_t ctas = tiles > most || items > most ? most : std::min(most, items * std::max<int64_t>(1, tiles));
-    launch_ex(paged_attention_kernel<S>, dim3((unsigned)ctas), dim3(ATPB), stream, true, p);
-    int32_t rc = check_launch("paged attention");
-    if (rc != RC_SUCCESS) return rc;
-    // no cut falls inside an item of one tile, nor, where cuts are moved by four tiles (see `quantum`), of six
-    if (tiles <= 1 || (tiles <= 6 && items * tiles < 16 * ctas)) return RC_SUCCESS;
-    launch_ex(paged_attention_join_kernel<S::D, S::HEADS>, dim3((unsigned)ctas, S::HEADS / 2), dim3(JTPB), stream, true, p, (int32_t)ctas);
-    return check_launch("joining of attention");
+    // No more CTAs than there can be work for: the lengths are known on the device only.
+    const int64_t steps = std::max<int64_t>(1, (tokens + S::TOKENS - 1) / S::TOKENS), items = p.batch * p.cache.kv_heads * p.tiles;
+    const int64_t most = S::CTAS * kSms, ctas = items >= most ? most : std::min(most, std::max(items, items * (steps + kBeginning<S>) / S::WARPS));
+    launch_ex(paged_attention_kernel<S>, dim3((unsigned)ctas), dim3(S::THREADS), stream, true, p);
+    return check_launch("paged attention");
 }
 
 template <int D>
@@ -708,9 +764,9 @@ extern "C" {
 
 int64_t pplb200_paged_decode_attention_workspace_bytes(int64_t batch, int64_t max_tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
     if (batch < 0 || max_tokens < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0) return -1;
-    // two pieces a CTA at most
+    // a counter and two pieces a CTA at most
     const int heads = heads_at_once(head_dim, q_heads / kv_heads);
-    return round_up(kMostCtas * 8, 256) + round_up(2 * kMostCtas * heads * 8, 256) + 2LL * kMostCtas * heads * head_dim * 4;
+    return round_up(kCtas * 4, 256) + round_up(2 * kCtas * heads * 8, 256) + 2LL * kCtas * heads * head_dim * 4;
 }
 
 int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_paged_attention_args* a) {
@@ -756,10 +812,11 @@ int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb2
     p.tiles = (p.shared + heads - 1) / heads;
     p.window = a->window; p.scale_log2 = a->scale * 1.4426950408889634f;
     p.cache = *cache;
-    p.items = (int32_t*)a->ws;
-    p.tops = (float2*)((char*)a->ws + round_up(kMostCtas * 8, 256));
-    p.sums = (float*)((char*)p.tops + round_up(2 * kMostCtas * heads * 8, 256));
-    if (a->batch * (int64_t)cache->kv_heads * p.tiles > 0x7fffffffLL) return fail(RC_UNSUPPORTED, "too many sequences and heads");
+    p.flip = 0x00800080u;
+    p.flip_1024 = 0x64806480u;
+    p.arrived = (uint32_t*)a->ws;
+    p.tops = (float2*)((char*)a->ws + round_up(kCtas * 4, 256));
+    p.sums = (float*)((char*)p.tops + round_up(2 * kCtas * heads * 8, 256));
     const cudaStream_t s = (cudaStream_t)stream;
     if (D == 64) return launch_kind<64>(s, p, p.tokens_in_table);
     if (D == 96) return launch_kind<96>(s, p, p.tokens_in_table);

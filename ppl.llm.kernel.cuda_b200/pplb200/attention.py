@@ -222,7 +222,7 @@ class PagedDecodeAttention:
         self.max_pages = -(-max_length // cache.page_size)
         self.scale = cache.head_dim ** -0.5 if scale is None else scale
         need = lib.pplb200_paged_decode_attention_workspace_bytes(max_batch, self.max_pages * cache.page_size, q_heads, cache.kv_heads, cache.head_dim)
-        self.ws = torch.empty((need,), dtype=torch.uint8, device=cache.k.device)
+        self.ws = torch.zeros((need,), dtype=torch.uint8, device=cache.k.device)
 
     def __call__(self, q, pages, lengths, out=None, lse=None):
         """q fp16 [batch, q_heads, head_dim], pages int32 [batch, pages a sequence] (negative: a hole), lengths int32 [batch] -> out as q;
