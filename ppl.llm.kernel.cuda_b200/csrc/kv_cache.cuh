@@ -27,6 +27,15 @@ __host__ __device__ inline bool kv_find(int64_t slot, int64_t num_pages, int32_t
     return page < num_pages;
 }
 
+// n / d = n * magic >> shift for all n below 2^31: with 2^(s - 1) < d <= 2^s and magic = ceil(2^(31 + s) / d), magic * d exceeds 2^(31 + s)
+// by less than d <= 2^s, which n < 2^31 keeps below 1 / d of the quotient.
+inline void small_division(uint32_t d, uint32_t& magic, uint32_t& shift) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) ++s;
+    shift = 31 + s;
+    magic = (uint32_t)(((1ull << shift) + d - 1) / d);
+}
+
 // RC_SUCCESS, or the first thing wrong with the description (the text goes to pplb200_last_error()).
 int32_t check_kv_cache(const pplb200_kv_cache* c);
 

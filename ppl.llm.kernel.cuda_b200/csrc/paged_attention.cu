@@ -720,15 +720,6 @@ bool row_units(int64_t pages, int64_t page_size, int64_t page_bytes, int64_t tok
     return (last >> shift) < ((__int128)1 << 32);
 }
 
-// token / d = token * magic >> shift for all tokens below 2^31: with 2^(s - 1) < d <= 2^s and magic = ceil(2^(31 + s) / d), magic * d
-// exceeds 2^(31 + s) by less than d <= 2^s, which token < 2^31 keeps below 1 / d of the quotient.
-void page_division(uint32_t d, uint32_t& magic, uint32_t& shift) {
-    uint32_t s = 0;
-    while ((1ull << s) < d) ++s;
-    shift = 31 + s;
-    magic = (uint32_t)(((1ull << shift) + d - 1) / d);
-}
-
 // Query heads that a CTA takes at once: two blocks of eight where that many share a key-value head and registers allow.
 int heads_at_once(int32_t head_dim, int32_t shared) { return shared > 8 && head_dim <= 128 ? 16 : 8; }
 template <class S>
@@ -801,7 +792,7 @@ int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb2
         (cache->quant_group && !row_units(cache->num_pages, cache->page_size, cache->scale_page_stride * 2, cache->scale_token_stride * 2, p.scale_unit,
                                           p.scale_page_units, p.scale_token_units)))
         return fail(RC_UNSUPPORTED, "attention: the rows of a head lie further apart than 2^32 times their alignment");
-    page_division(cache->page_size, p.page_magic, p.page_shift);
+    small_division(cache->page_size, p.page_magic, p.page_shift);
     p.num_pages = (int32_t)std::min<int64_t>(cache->num_pages, 0x7fffffff); // a table's entry is no larger
     p.q = (const half*)a->q; p.out = (half*)a->out; p.lse = a->optional_lse;
     p.pages = a->pages; p.lengths = a->lengths;

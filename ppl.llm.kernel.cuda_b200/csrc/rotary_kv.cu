@@ -1,6 +1,7 @@
 // Rotary positions, and the paged key-value cache written and read back.
 #include "kv_cache.cuh"
 
+#include <algorithm>
 #include <cmath>
 
 namespace pplb200 {
@@ -30,17 +31,23 @@ int32_t check_kv_cache(const pplb200_kv_cache* c) {
 
 namespace {
 
-constexpr int TPB = 256;
+constexpr int TPB = 256; // reading back
+
+enum : int { Q = 0, K = 1, V = 2 };
 
 struct RotaryKvParams {
-    const half *q, *k, *v;
-    half *q_out, *k_out;
+    const half* src[3];
+    half* dst[2];
+    int64_t src_stride[3], dst_stride[2];
+    int32_t heads[3], turns_of[3]; // rows of a token, and how many of them a thread takes at most
     const int64_t *positions, *slots;
     const uint64_t* turns;
-    int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
-    int32_t q_heads, k_heads, v_heads, head_dim, rotary_dim, interleaved;
+    int64_t tokens;
+    int32_t head_dim, rotary_dim, interleaved;
     float magnitude;
-    int32_t store; // keys go to the cache instead of k_out, values too
+    int32_t store; // keys go to the cache instead of dst[K], values too
+    int32_t groups;                    // threads that share a token's rows, for each 16 dimensions
+    uint32_t group_magic, group_shift; // n / groups = n * group_magic >> group_shift
     pplb200_kv_cache cache;
 };
 
@@ -58,118 +65,147 @@ __device__ __forceinline__ uint32_t absmax_bits(const uint4& a) {
 // The scale of a group: amax / 127 rounded up to fp16 -- fp16 so that what is divided by is what is stored, up so that no quotient is
 // beyond 127 steps, among the subnormal scales of very small groups too -- at least the smallest fp16 above zero, and for finite
 // groups at most 515.5: with 516, 127 steps would read back as infinity.
+// The quotient: a product with the reciprocal, corrected by what it leaves of amax.  That is exact where amax / 127 is an fp16, and
+// off by less than 2^-22 otherwise, when amax / 127 lies 2^-18 or more of its size from any fp16 (amax has 11 bits, 127 times an fp16 18).
 __device__ __forceinline__ half group_scale(uint32_t amax) {
-    const uint32_t s = __half_as_ushort(__float2half_ru(__fdiv_rn(__half2float(__ushort_as_half((unsigned short)amax)), 127.0f)));
-    return __ushort_as_half((unsigned short)(amax < 0x7c00u ? min(max(s, 1u), 0x6007u) : s));
+    const float a = __half2float(__ushort_as_half((unsigned short)amax)), guess = a * (1.0f / 127.0f);
+    const float step = __fmaf_rn(__fmaf_rn(-127.0f, guess, a), 1.0f / 127.0f, guess);
+    const uint32_t s = __half_as_ushort(__float2half_ru(step));
+    return __ushort_as_half((unsigned short)(amax < 0x7c00u ? min(max(s, 1u), 0x6007u) : amax));
 }
 
-// The quotient in 32 bits, rounded to nearest even.  Its magnitude is at most 127.07 (65504 / 515.5); NaN, in a group with an infinity
-// or a NaN in it, becomes 0, and is NaN again when it is multiplied by that group's scale.
-__device__ __forceinline__ uint32_t quantize_one(float v, float scale) {
-    return (uint32_t)__float2int_rn(__fdiv_rn(v, scale)) & 0xffu;
-}
-__device__ __forceinline__ uint2 quantize_eight(const Eight& e, float scale) {
-    uint32_t b[8];
+// Eight quotients rounded to nearest even, as bytes.  Their magnitude is at most 127.07 (65504 / 515.5).  The product with the scale's
+// reciprocal, moved by 2^-21 to either side, brackets the quotient in 32 bits (the reciprocal is off by 2^-23 at most, its moving, the
+// product and the quotient by 2^-24 each); 1.5 * 2^23 added, the low byte is the rounded number.  Where the two sides differ, and in a
+// group with an infinity or a NaN, the division decides; there NaN becomes 0, and is NaN again when it is multiplied by that group's scale.
+__device__ __forceinline__ uint2 quantize_eight(const Eight& e, half scale) {
+    const float s = __half2float(scale);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    const float hi = inv * (1.0f + 0x1p-21f), lo = inv * (1.0f - 0x1p-21f);
+    constexpr float kMagic = 12582912.0f;
+    uint32_t b[8], differ = __half_as_ushort(scale) < 0x7c00u ? 0u : 1u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(e.h[i]);
-        b[2 * i] = quantize_one(f.x, scale);
-        b[2 * i + 1] = quantize_one(f.y, scale);
+        const float2 v = __half22float2(e.h[i]);
+        b[2 * i] = __float_as_uint(__fmaf_rn(v.x, hi, kMagic));
+        b[2 * i + 1] = __float_as_uint(__fmaf_rn(v.y, hi, kMagic));
+        differ |= b[2 * i] ^ __float_as_uint(__fmaf_rn(v.x, lo, kMagic));
+        differ |= b[2 * i + 1] ^ __float_as_uint(__fmaf_rn(v.y, lo, kMagic));
     }
-    return make_uint2(b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24, b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24);
+    if (differ != 0u) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 v = __half22float2(e.h[i]);
+            b[2 * i] = (uint32_t)__float2int_rn(__fdiv_rn(v.x, s));
+            b[2 * i + 1] = (uint32_t)__float2int_rn(__fdiv_rn(v.y, s));
+        }
+    }
+    return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
 }
 
-// One CTA turns the rows (heads of q, k and v) of one token, LANES threads a row, 16 dimensions a thread: two runs of eight that
-// are rotated against each other (half layout: rotary_dim / 2 apart), so that nothing crosses threads but the scale of a whole head.
-template <int LANES>
-__global__ void __launch_bounds__(TPB) rotary_kv_kernel(const RotaryKvParams p) {
-    __shared__ float2 turn[kMaxHeadDim / 2];
-    pdl_wait_prior_grid();
-    const int64_t token = blockIdx.x;
-    const int planes = p.rotary_dim >> 1;
-    if (planes > 0) {
-        const uint64_t at = (uint64_t)p.positions[token];
-        for (int i = threadIdx.x; i < planes; i += TPB) {
-            // the angle modulo one turn, exactly, as a signed fraction; half turns for sincospi
-            const float half_turns = (float)(int64_t)(at * p.turns[i]) * 0x1p-63f;
-            float s, c;
-            sincospif(half_turns, &s, &c);
-            turn[i] = make_float2(c * p.magnitude, s * p.magnitude);
-        }
-        __syncthreads();
+// Cosines and sines (times the magnitude) of eight planes: the angle modulo one turn, exactly, as a signed fraction, in half turns.
+struct Turns {
+    float c[8], s[8];
+};
+__device__ __forceinline__ void turns_at(Turns& t, uint64_t position, const uint64_t* turns, float magnitude) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        sincospif((float)(int64_t)(position * turns[i]) * 0x1p-63f, &t.s[i], &t.c[i]);
+        t.c[i] *= magnitude;
+        t.s[i] *= magnitude;
     }
-    int64_t page = 0;
-    int32_t in_page = 0;
-    const bool stored = p.store && kv_find(p.slots[token], p.cache.num_pages, p.cache.page_size, page, in_page);
+}
+// a and b against each other, or (interleaved) neighbours within a and within b.
+__device__ __forceinline__ void rotate(Eight& a, Eight& b, const Turns& t, bool interleaved) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = __half22float2(a.h[i]), y = __half22float2(b.h[i]);
+        if (!interleaved) {
+            a.h[i] = __floats2half2_rn(x.x * t.c[2 * i] - y.x * t.s[2 * i], x.y * t.c[2 * i + 1] - y.y * t.s[2 * i + 1]);
+            b.h[i] = __floats2half2_rn(y.x * t.c[2 * i] + x.x * t.s[2 * i], y.y * t.c[2 * i + 1] + x.y * t.s[2 * i + 1]);
+        } else {
+            a.h[i] = __floats2half2_rn(x.x * t.c[i] - x.y * t.s[i], x.y * t.c[i] + x.x * t.s[i]);
+            b.h[i] = __floats2half2_rn(y.x * t.c[4 + i] - y.y * t.s[4 + i], y.y * t.c[4 + i] + y.x * t.s[4 + i]);
+        }
+    }
+}
 
-    const int u = threadIdx.x & (LANES - 1);
-    const int rows = p.q_heads + p.k_heads + p.v_heads;
-    const int per_cta = TPB / LANES;
-    for (int row = blockIdx.y * per_cta + threadIdx.x / LANES; row < rows; row += gridDim.y * per_cta) {
-        const bool is_q = row < p.q_heads, is_v = row >= p.q_heads + p.k_heads;
-        const int head = is_q ? row : is_v ? row - p.q_heads - p.k_heads : row - p.q_heads;
-        const half* src = is_q ? p.q + token * p.q_stride : is_v ? p.v + token * p.v_stride : p.k + token * p.k_stride;
-        src += (int64_t)head * p.head_dim;
-        const bool turned = !is_v && 16 * u < p.rotary_dim;
-        const int da = turned && !p.interleaved ? 8 * u : 16 * u;
-        const int db = turned && !p.interleaved ? planes + 8 * u : 16 * u + 8;
-        const bool active = 16 * u < p.head_dim;
-        Eight a = {}, b = {};
-        if (active) {
-            a.raw = ld_global_16(src + da);
-            b.raw = ld_global_16(src + db);
+// A thread has 16 dimensions of a token: two runs of eight that are rotated against each other (half layout: rotary_dim / 2
+// apart), so that nothing crosses threads but the scale of a whole head.  It computes their eight sines and cosines once, while its
+// first rows are on their way, and takes every groups-th head of q, k and v with them; LANES threads side by side make a row.
+constexpr int RTPB = 128;
+template <int LANES, bool INTERLEAVED, bool STORE>
+struct RotaryKv {
+    struct Row {
+        Eight a, b; // zeros where there is nothing
+    };
+    const RotaryKvParams& p;
+    int64_t token;
+    int u;
+    bool active, turned; // whether the thread has dimensions, and whether they are rotated
+    Turns turns;
+    int64_t at, scale_at; // in the cache; at < 0: not stored
+
+    template <int KIND>
+    __device__ __forceinline__ void places(int& da, int& db) const {
+        const bool apart = !INTERLEAVED && KIND != V && turned;
+        da = apart ? 8 * u : 16 * u;
+        db = apart ? (p.rotary_dim >> 1) + 8 * u : 16 * u + 8;
+    }
+    template <int KIND>
+    __device__ __forceinline__ void fetch(int head, Row& x) const {
+        int da, db;
+        places<KIND>(da, db);
+        x.a.raw = x.b.raw = make_uint4(0, 0, 0, 0);
+        if (active && head < p.heads[KIND]) {
+            const half* src = p.src[KIND] + token * p.src_stride[KIND] + (int64_t)head * p.head_dim;
+            x.a.raw = ld_global_16(src + da);
+            x.b.raw = ld_global_16(src + db);
         }
-        if (turned) {
-            if (!p.interleaved) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 x = __half22float2(a.h[i]), y = __half22float2(b.h[i]);
-                    const float2 r0 = turn[8 * u + 2 * i], r1 = turn[8 * u + 2 * i + 1];
-                    a.h[i] = __floats2half2_rn(x.x * r0.x - y.x * r0.y, x.y * r1.x - y.y * r1.y);
-                    b.h[i] = __floats2half2_rn(y.x * r0.x + x.x * r0.y, y.y * r1.x + x.y * r1.y);
+    }
+    // Called by all threads of a warp.
+    template <int KIND>
+    __device__ __forceinline__ void finish(int head, Row& x) const {
+        int da, db;
+        places<KIND>(da, db);
+        if (KIND != V && turned) rotate(x.a, x.b, turns, INTERLEAVED);
+        const bool there = active && head < p.heads[KIND];
+        if constexpr (!STORE || KIND == Q) {
+            half* dst = p.dst[KIND] + token * p.dst_stride[KIND] + (int64_t)head * p.head_dim;
+            if (there) {
+                *reinterpret_cast<uint4*>(dst + da) = x.a.raw;
+                *reinterpret_cast<uint4*>(dst + db) = x.b.raw;
+            }
+        } else {
+            const int64_t row = at + (int64_t)head * p.cache.head_stride;
+            void* const data = KIND == V ? p.cache.v : p.cache.k;
+            const bool stored = there && at >= 0;
+            if (p.cache.quant_group == 0) {
+                if (stored) {
+                    *reinterpret_cast<uint4*>((half*)data + row + da) = x.a.raw;
+                    *reinterpret_cast<uint4*>((half*)data + row + db) = x.b.raw;
                 }
+                return;
+            }
+            uint32_t ma = absmax_bits(x.a.raw), mb = absmax_bits(x.b.raw);
+            if (p.cache.quant_group != 8) {
+                ma = max(ma, mb);
+#pragma unroll
+                for (int m = LANES / 2; m >= 1; m >>= 1) ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, m));
+            }
+            if (!stored) return;
+            const half sa = group_scale(ma), sb = p.cache.quant_group == 8 ? group_scale(mb) : sa;
+            const uint2 qa = quantize_eight(x.a, sa), qb = quantize_eight(x.b, sb);
+            int8_t* dst = (int8_t*)data + row;
+            if (KIND == V || INTERLEAVED || !turned) {
+                *reinterpret_cast<uint4*>(dst + da) = make_uint4(qa.x, qa.y, qb.x, qb.y);
             } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 x = __half22float2(a.h[i]), y = __half22float2(b.h[i]);
-                    const float2 r0 = turn[8 * u + i], r1 = turn[8 * u + 4 + i];
-                    a.h[i] = __floats2half2_rn(x.x * r0.x - x.y * r0.y, x.y * r0.x + x.x * r0.y);
-                    b.h[i] = __floats2half2_rn(y.x * r1.x - y.y * r1.y, y.y * r1.x + y.x * r1.y);
-                }
+                *reinterpret_cast<uint2*>(dst + da) = qa;
+                *reinterpret_cast<uint2*>(dst + db) = qb;
             }
-        }
-        if (is_q || !p.store) {
-            half* dst = (is_q ? p.q_out + token * p.q_out_stride : p.k_out + token * p.k_out_stride) + (int64_t)head * p.head_dim;
-            if (active) {
-                *reinterpret_cast<uint4*>(dst + da) = a.raw;
-                *reinterpret_cast<uint4*>(dst + db) = b.raw;
-            }
-            continue;
-        }
-        const int64_t at = kv_row(page, in_page, head, p.cache.page_stride, p.cache.head_stride, p.cache.token_stride);
-        if (p.cache.quant_group == 0) {
-            half* dst = (half*)(is_v ? p.cache.v : p.cache.k) + at;
-            if (active && stored) {
-                *reinterpret_cast<uint4*>(dst + da) = a.raw;
-                *reinterpret_cast<uint4*>(dst + db) = b.raw;
-            }
-            continue;
-        }
-        uint32_t ma = absmax_bits(a.raw), mb = absmax_bits(b.raw);
-        if (p.cache.quant_group != 8) {
-            ma = max(ma, mb);
-            const uint32_t row_mask = (LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1)) << (threadIdx.x & 31 & ~(LANES - 1));
-#pragma unroll
-            for (int m = LANES / 2; m >= 1; m >>= 1) ma = max(ma, __shfl_xor_sync(row_mask, ma, m));
-            mb = ma;
-        }
-        if (active && stored) {
-            const half sa = group_scale(ma), sb = group_scale(mb);
-            int8_t* dst = (int8_t*)(is_v ? p.cache.v : p.cache.k) + at;
-            *reinterpret_cast<uint2*>(dst + da) = quantize_eight(a, __half2float(sa));
-            *reinterpret_cast<uint2*>(dst + db) = quantize_eight(b, __half2float(sb));
-            half* scale = (half*)(is_v ? p.cache.v_scale : p.cache.k_scale) +
-                          kv_row(page, in_page, head, p.cache.scale_page_stride, p.cache.scale_head_stride, p.cache.scale_token_stride);
+            half* scale = (half*)(KIND == V ? p.cache.v_scale : p.cache.k_scale) + scale_at + (int64_t)head * p.cache.scale_head_stride;
             if (p.cache.quant_group == 8) {
                 scale[da >> 3] = sa;
                 scale[db >> 3] = sb;
@@ -178,51 +214,151 @@ __global__ void __launch_bounds__(TPB) rotary_kv_kernel(const RotaryKvParams p) 
             }
         }
     }
+    // Rows behind the first, two at a time.
+    template <int KIND>
+    __device__ __forceinline__ void others(int group) const {
+        for (int i = 1; i < p.turns_of[KIND]; i += 2) {
+            Row x, y;
+            fetch<KIND>(group + i * p.groups, x);
+            fetch<KIND>(group + (i + 1) * p.groups, y);
+            finish<KIND>(group + i * p.groups, x);
+            if (i + 1 < p.turns_of[KIND]) finish<KIND>(group + (i + 1) * p.groups, y);
+        }
+    }
+};
+
+template <int LANES, bool INTERLEAVED, bool STORE>
+__global__ void __launch_bounds__(RTPB, 7) rotary_kv_kernel(const __grid_constant__ RotaryKvParams p) {
+    pdl_wait_prior_grid();
+    const uint32_t n = blockIdx.x * (RTPB / LANES) + threadIdx.x / LANES;
+    RotaryKv<LANES, INTERLEAVED, STORE> r{p};
+    r.token = (uint32_t)((uint64_t)n * p.group_magic >> p.group_shift);
+    const int group = n - (uint32_t)r.token * p.groups;
+    const bool valid = r.token < p.tokens;
+    r.u = threadIdx.x & (LANES - 1);
+    r.active = valid && 16 * r.u < p.head_dim;
+    r.turned = valid && 16 * r.u < p.rotary_dim;
+    typename RotaryKv<LANES, INTERLEAVED, STORE>::Row q, k, v;
+    r.template fetch<Q>(group, q);
+    r.template fetch<K>(group, k);
+    if (STORE) r.template fetch<V>(group, v);
+    if (r.turned) turns_at(r.turns, (uint64_t)p.positions[r.token], p.turns + 8 * r.u, p.magnitude);
+    r.at = -1;
+    r.scale_at = 0;
+    if (STORE && valid) {
+        int64_t page;
+        int32_t in_page;
+        if (kv_find(p.slots[r.token], p.cache.num_pages, p.cache.page_size, page, in_page)) {
+            r.at = kv_row(page, in_page, 0, p.cache.page_stride, 0, p.cache.token_stride);
+            r.scale_at = kv_row(page, in_page, 0, p.cache.scale_page_stride, 0, p.cache.scale_token_stride);
+        }
+    }
+    if (p.turns_of[Q] > 0) r.template finish<Q>(group, q);
+    if (p.turns_of[K] > 0) r.template finish<K>(group, k);
+    if (STORE) r.template finish<V>(group, v);
+    r.template others<Q>(group);
+    r.template others<K>(group);
+    if (STORE) r.template others<V>(group);
 }
 
-int32_t launch_rotary_kv(cudaStream_t stream, int64_t tokens, const RotaryKvParams& p) {
-    const int rows = p.q_heads + p.k_heads + p.v_heads;
-    if (tokens == 0 || rows == 0) return RC_SUCCESS;
-    const int lanes = p.head_dim <= 64 ? 4 : p.head_dim <= 128 ? 8 : 16;
-    const int passes = (rows * lanes + TPB - 1) / TPB;
-    // few tokens: every CTA makes one pass, so that the rows spread over more SMs
-    const dim3 grid((unsigned)tokens, (unsigned)(tokens < 1024 ? passes : 1));
-    if (lanes == 4) launch_ex(rotary_kv_kernel<4>, grid, dim3(TPB), stream, true, p);
-    else if (lanes == 8) launch_ex(rotary_kv_kernel<8>, grid, dim3(TPB), stream, true, p);
-    else launch_ex(rotary_kv_kernel<16>, grid, dim3(TPB), stream, true, p);
+template <int LANES>
+int32_t launch_lanes(cudaStream_t stream, RotaryKvParams& p) {
+    // Heads a thread: as many as spread the sines over enough of them, while the device stays full.
+    const int32_t most = std::max(p.heads[Q], std::max(p.heads[K], p.heads[V]));
+    const int64_t heads = std::min<int64_t>(4, std::max<int64_t>(1, p.tokens * most * LANES / (148LL * 1024 * 2)));
+    p.groups = (int32_t)std::min<int64_t>((most + heads - 1) / heads, std::max<int64_t>(1, 0x7fff0000LL / p.tokens));
+    for (int k = 0; k < 3; ++k) p.turns_of[k] = (p.heads[k] + p.groups - 1) / p.groups;
+    small_division(p.groups, p.group_magic, p.group_shift);
+    const dim3 grid((unsigned)((p.tokens * p.groups + RTPB / LANES - 1) / (RTPB / LANES)));
+    if (p.store) {
+        if (p.interleaved) launch_ex(rotary_kv_kernel<LANES, true, true>, grid, dim3(RTPB), stream, true, p);
+        else launch_ex(rotary_kv_kernel<LANES, false, true>, grid, dim3(RTPB), stream, true, p);
+    } else {
+        if (p.interleaved) launch_ex(rotary_kv_kernel<LANES, true, false>, grid, dim3(RTPB), stream, true, p);
+        else launch_ex(rotary_kv_kernel<LANES, false, false>, grid, dim3(RTPB), stream, true, p);
+    }
     return check_launch("rotary / cache write");
 }
+int32_t launch_rotary_kv(cudaStream_t stream, RotaryKvParams& p) {
+    if (p.tokens == 0 || p.heads[Q] + p.heads[K] + p.heads[V] == 0) return RC_SUCCESS;
+    return p.head_dim <= 64 ? launch_lanes<4>(stream, p) : p.head_dim <= 128 ? launch_lanes<8>(stream, p) : launch_lanes<16>(stream, p);
+}
 
-// One thread per eight dimensions of a key or value row.
-__global__ void __launch_bounds__(TPB) kv_read_kernel(const pplb200_kv_cache c, const int64_t* slots, int64_t units, half* k_out, half* v_out) {
+// 16 dimensions of a key and of the value beside it a thread; where a token lies is looked up once a CTA.
+struct KvReadParams {
+    pplb200_kv_cache cache;
+    const int64_t* slots;
+    int64_t tokens;
+    half *k_out, *v_out;
+    int32_t tokens_per_cta, units; // 16 dimensions each, of a token
+    uint32_t units_magic, units_shift, head_magic, head_shift;
+};
+__global__ void __launch_bounds__(TPB) kv_read_kernel(const __grid_constant__ KvReadParams p) {
+    struct Row {
+        int64_t at, scale_at;
+    };
+    __shared__ Row where[TPB];
+    const pplb200_kv_cache& c = p.cache;
     pdl_wait_prior_grid();
-    const int per_head = c.head_dim >> 3;
-    const int64_t n = (int64_t)blockIdx.x * TPB + threadIdx.x;
-    if (n >= units) return;
-    const int64_t row = n / per_head;
-    const int d = (int)(n - row * per_head) * 8;
-    const int64_t token = row / c.kv_heads;
-    const int head = (int)(row - token * c.kv_heads);
-    int64_t page = 0;
-    int32_t in_page = 0;
-    const bool found = kv_find(slots[token], c.num_pages, c.page_size, page, in_page);
-    const int64_t at = kv_row(page, in_page, head, c.page_stride, c.head_stride, c.token_stride) + d;
-    const int64_t sat = kv_row(page, in_page, head, c.scale_page_stride, c.scale_head_stride, c.scale_token_stride) + (c.quant_group == 8 ? d >> 3 : 0);
+    const int64_t token0 = (int64_t)blockIdx.x * p.tokens_per_cta;
+    const int tokens = (int)min((int64_t)p.tokens_per_cta, p.tokens - token0);
+    if (threadIdx.x < tokens) {
+        Row w = {-1, 0};
+        int64_t page;
+        int32_t in_page;
+        if (kv_find(p.slots[token0 + threadIdx.x], c.num_pages, c.page_size, page, in_page)) {
+            w.at = kv_row(page, in_page, 0, c.page_stride, 0, c.token_stride);
+            w.scale_at = kv_row(page, in_page, 0, c.scale_page_stride, 0, c.scale_token_stride);
+        }
+        where[threadIdx.x] = w;
+    }
+    __syncthreads();
+    const int per_head = c.head_dim >> 4;
+    for (int i = blockIdx.y * TPB + threadIdx.x; i < tokens * p.units; i += gridDim.y * TPB) {
+        const int local = (int)((uint64_t)(uint32_t)i * p.units_magic >> p.units_shift), unit = i - local * p.units;
+        const int head = (int)((uint64_t)(uint32_t)unit * p.head_magic >> p.head_shift), d = (unit - head * per_head) * 16;
+        const Row w = where[local];
+        const int64_t at = w.at + (int64_t)head * c.head_stride + d;
+        const int64_t scale_at = w.scale_at + (int64_t)head * c.scale_head_stride + (c.quant_group == 8 ? d >> 3 : 0);
+        Eight o[2][2];
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-        Eight e = {};
-        if (found) {
+        for (int n = 0; n < 4; ++n) o[n >> 1][n & 1].raw = make_uint4(0, 0, 0, 0);
+        if (w.at >= 0) {
             if (c.quant_group == 0) {
-                e.raw = ld_global_16((const half*)(kv ? c.v : c.k) + at);
-            } else {
-                const uint2 w = *reinterpret_cast<const uint2*>((const int8_t*)(kv ? c.v : c.k) + at);
-                const float s = __half2float(ld_global_half((const half*)(kv ? c.v_scale : c.k_scale) + sat));
-                const int8_t* b = reinterpret_cast<const int8_t*>(&w);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) e.h[i] = __floats2half2_rn((float)b[2 * i] * s, (float)b[2 * i + 1] * s);
+                for (int n = 0; n < 4; ++n) o[n >> 1][n & 1].raw = ld_global_16((const half*)(n >> 1 ? c.v : c.k) + at + 8 * (n & 1));
+            } else {
+                uint4 q[2];
+                half s[2][2];
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    q[n] = ld_global_16((const int8_t*)(n ? c.v : c.k) + at);
+                    const half* scale = (const half*)(n ? c.v_scale : c.k_scale) + scale_at;
+                    s[n][0] = ld_global_half(scale);
+                    s[n][1] = c.quant_group == 8 ? ld_global_half(scale + 1) : s[n][0];
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const uint32_t words[4] = {q[n].x, q[n].y, q[n].z, q[n].w};
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        // a byte with its sign flipped beneath 0x64 is 1152 + value, as a half: whole numbers, then one rounding
+                        const uint32_t w4 = words[x] ^ 0x80808080u;
+                        const __half2 s2 = __half2half2(s[n][x >> 1]), offset = __float2half2_rn(1152.0f);
+                        uint32_t lo = __byte_perm(w4, 0x64646464u, 0x4140), hi = __byte_perm(w4, 0x64646464u, 0x4342);
+                        o[n][x >> 1].h[2 * (x & 1)] = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&lo), offset), s2);
+                        o[n][x >> 1].h[2 * (x & 1) + 1] = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&hi), offset), s2);
+                    }
+                }
             }
         }
-        *reinterpret_cast<uint4*>((kv ? v_out : k_out) + n * 8) = e.raw;
+        const int64_t out = ((token0 * p.units) + i) * 16;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            half* dst = (n ? p.v_out : p.k_out) + out;
+            *reinterpret_cast<uint4*>(dst) = o[n][0].raw;
+            *reinterpret_cast<uint4*>(dst + 8) = o[n][1].raw;
+        }
     }
 }
 
@@ -300,15 +436,15 @@ int32_t pplb200_rotary_fp16(pplb200_stream_t stream, const pplb200_rotary_args* 
     if (rc == RC_SUCCESS) rc = check_rows("k_out", a->k_out, a->k_out_stride, a->k_heads, a->head_dim, a->tokens);
     if (rc != RC_SUCCESS) return rc;
     RotaryKvParams p = {};
-    p.q = (const half*)a->q; p.k = (const half*)a->k;
-    p.q_out = (half*)a->q_out; p.k_out = (half*)a->k_out;
-    p.positions = a->positions; p.turns = a->turns;
-    p.q_stride = a->q_stride; p.k_stride = a->k_stride;
-    p.q_out_stride = a->q_out_stride; p.k_out_stride = a->k_out_stride;
-    p.q_heads = a->q_heads; p.k_heads = a->k_heads;
+    p.src[0] = (const half*)a->q; p.src[1] = (const half*)a->k;
+    p.dst[0] = (half*)a->q_out; p.dst[1] = (half*)a->k_out;
+    p.src_stride[0] = a->q_stride; p.src_stride[1] = a->k_stride;
+    p.dst_stride[0] = a->q_out_stride; p.dst_stride[1] = a->k_out_stride;
+    p.heads[Q] = a->q_heads; p.heads[K] = a->k_heads;
+    p.tokens = a->tokens; p.positions = a->positions; p.turns = a->turns;
     p.head_dim = a->head_dim; p.rotary_dim = a->rotary_dim; p.interleaved = a->interleaved;
     p.magnitude = a->magnitude;
-    return launch_rotary_kv((cudaStream_t)stream, a->tokens, p);
+    return launch_rotary_kv((cudaStream_t)stream, p);
 }
 
 int32_t pplb200_kv_cache_write_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_kv_write_args* a) {
@@ -327,16 +463,17 @@ int32_t pplb200_kv_cache_write_fp16(pplb200_stream_t stream, const pplb200_kv_ca
     if (rc == RC_SUCCESS) rc = check_rows("v", a->v, a->v_stride, cache->kv_heads, cache->head_dim, a->tokens);
     if (rc != RC_SUCCESS) return rc;
     RotaryKvParams p = {};
-    p.q = (const half*)a->q; p.k = (const half*)a->k; p.v = (const half*)a->v;
-    p.q_out = (half*)a->q_out;
-    p.positions = a->positions; p.slots = a->slots; p.turns = a->turns;
-    p.q_stride = a->q_stride; p.k_stride = a->k_stride; p.v_stride = a->v_stride; p.q_out_stride = a->q_out_stride;
-    p.q_heads = q_heads; p.k_heads = p.v_heads = cache->kv_heads;
+    p.src[0] = (const half*)a->q; p.src[1] = (const half*)a->k; p.src[2] = (const half*)a->v;
+    p.dst[0] = (half*)a->q_out;
+    p.src_stride[0] = a->q_stride; p.src_stride[1] = a->k_stride; p.src_stride[2] = a->v_stride;
+    p.dst_stride[0] = a->q_out_stride;
+    p.heads[Q] = q_heads; p.heads[K] = p.heads[V] = cache->kv_heads;
+    p.tokens = a->tokens; p.positions = a->positions; p.slots = a->slots; p.turns = a->turns;
     p.head_dim = cache->head_dim; p.rotary_dim = a->rotary_dim; p.interleaved = a->interleaved;
     p.magnitude = a->magnitude;
     p.store = 1;
     p.cache = *cache;
-    return launch_rotary_kv((cudaStream_t)stream, a->tokens, p);
+    return launch_rotary_kv((cudaStream_t)stream, p);
 }
 
 int32_t pplb200_kv_cache_read_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache, const int64_t* slots, int64_t tokens,
@@ -348,8 +485,18 @@ int32_t pplb200_kv_cache_read_fp16(pplb200_stream_t stream, const pplb200_kv_cac
     if (!slots || ((uintptr_t)slots & 7)) return fail(RC_INVALID_VALUE, "slots must be an 8-byte aligned pointer");
     if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out)) return fail(RC_INVALID_VALUE, "k_out and v_out must be 16-byte aligned pointers");
     if (tokens > (1LL << 38) / (cache->kv_heads * (int64_t)cache->head_dim)) return fail(RC_UNSUPPORTED, "too many elements");
-    const int64_t units = tokens * cache->kv_heads * (cache->head_dim / 8);
-    launch_ex(kv_read_kernel, dim3((unsigned)((units + TPB - 1) / TPB)), dim3(TPB), (cudaStream_t)stream, true, *cache, slots, units, (half*)k_out, (half*)v_out);
+    KvReadParams p = {};
+    p.cache = *cache;
+    p.slots = slots; p.tokens = tokens;
+    p.k_out = (half*)k_out; p.v_out = (half*)v_out;
+    p.units = cache->kv_heads * (cache->head_dim / 16);
+    // about two units a thread; a token of very many heads is shared by CTAs
+    p.tokens_per_cta = (int32_t)std::min<int64_t>(TPB, std::max<int64_t>(1, 2 * TPB / p.units));
+    const int64_t blocks = (tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
+    const unsigned shares = (unsigned)std::max<int64_t>(1, std::min<int64_t>(p.units / (2 * TPB), 65535));
+    small_division(p.units, p.units_magic, p.units_shift);
+    small_division(cache->head_dim / 16, p.head_magic, p.head_shift);
+    launch_ex(kv_read_kernel, dim3((unsigned)blocks, shares), dim3(TPB), (cudaStream_t)stream, true, p);
     return check_launch("cache read");
 }
 

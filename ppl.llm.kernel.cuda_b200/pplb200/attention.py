@@ -6,7 +6,9 @@ Tensors are checked for type, shape and device here; sizes, alignment and stride
 import ctypes
 import struct
 
-from . import RC_SUCCESS, PplError, _check, lib
+import torch
+
+from . import PplError, _check, lib
 
 EXPORTS = [
     "pplb200_rotary_frequencies", "pplb200_rotary_fp16", "pplb200_kv_cache_write_fp16", "pplb200_kv_cache_read_fp16",
@@ -39,22 +41,22 @@ def _need(ok, what):
         raise ValueError(what)
 
 
+_F16, _I64, _I32 = torch.float16, torch.int64, torch.int32
+
+
+# These run on every call, and a small call's kernel takes two microseconds: one look at each property, the text only where it is needed.
 def _heads(t, name, tokens, head_dim, device):
     """(heads, elements between tokens) of an fp16 [tokens, heads, head_dim] tensor whose heads are contiguous."""
-    import torch
-    if t.dtype is not torch.float16 or t.get_device() != device:
-        raise ValueError("%s must be fp16 on device %d" % (name, device))
     shape, stride = t.shape, t.stride()
-    if len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim:
-        raise ValueError("%s must be [%d, heads, %d], got %s" % (name, tokens, head_dim, tuple(shape)))
-    if stride[2] != 1 or (shape[1] > 1 and stride[1] != head_dim):
-        raise ValueError("%s: the heads of a token must be contiguous" % name)
+    if (len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim or stride[2] != 1 or (stride[1] != head_dim and shape[1] > 1)
+            or t.dtype is not _F16 or t.get_device() != device):
+        raise ValueError("%s must be fp16 [%d, heads, %d] on device %d, the heads of a token contiguous; got %s %s, strides %s, on device %d"
+                         % (name, tokens, head_dim, device, t.dtype, tuple(shape), stride, t.get_device()))
     return shape[1], stride[0]
 
 
 def _indices(t, name, tokens, device):
-    import torch
-    if t.dtype is not torch.int64 or t.dim() != 1 or t.shape[0] != tokens or t.get_device() != device or (tokens > 1 and t.stride(0) != 1):
+    if t.shape != (tokens,) or t.dtype is not _I64 or (t.stride(0) != 1 and tokens > 1) or t.get_device() != device:
         raise ValueError("%s must be a contiguous int64 [%d] tensor on device %d" % (name, tokens, device))
     return t.data_ptr()
 
@@ -62,7 +64,6 @@ def _indices(t, name, tokens, device):
 def _here():
     """(current device, handle of its current stream): tensors have to be on that device.  The first call puts the look-up in its place."""
     global _here
-    import torch
     torch.cuda.init()
     device, raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
@@ -77,40 +78,44 @@ class RotaryTable:
 
     def __init__(self, rotary_dim, base=10000.0, scaling="none", factor=1.0, original_length=0, keep_turns=0.0, stretch_turns=0.0,
                  device="cuda"):
-        import torch
         _need(scaling in ROTARY_SCALINGS, "unknown scaling %r" % (scaling,))
         words, magnitude = (ctypes.c_uint64 * max(1, rotary_dim // 2))(), ctypes.c_float()
         _check(lib.pplb200_rotary_frequencies(rotary_dim, base, ROTARY_SCALINGS[scaling], factor, original_length, keep_turns,
                                               stretch_turns, words, ctypes.byref(magnitude)))
         self.rotary_dim, self.magnitude = rotary_dim, magnitude.value
-        self.turns = torch.frombuffer(words, dtype=torch.int64).to(device, copy=True)
+        self.turns = torch.frombuffer(words, dtype=_I64).to(device, copy=True)
+        self.device_index, self.address = self.turns.get_device(), self.turns.data_ptr()
 
 
 def rotary_fp16(q, k, positions, table, interleaved=False, q_out=None, k_out=None):
     """q [tokens, q_heads, head_dim], k [tokens, k_heads, head_dim] fp16 (either may be None) -> both rotated by `positions` (int64
     [tokens]).  q_out=q and k_out=k rotate in place."""
-    import torch
     dev, stream = _here()
-    first = q if q is not None else k
-    tokens, head_dim = first.shape[0], first.shape[-1]
-    ends = []
-    for name, x, y in (("q", q, q_out), ("k", k, k_out)):
-        if x is None:
-            ends.append((0, 0, 0, 0, 0, None))
-            continue
-        heads, stride = _heads(x, name, tokens, head_dim, dev)
-        if y is None:
-            y = torch.empty((tokens, heads, head_dim), dtype=torch.float16, device=x.device)
-        out_heads, out_stride = _heads(y, name + "_out", tokens, head_dim, dev)
-        _need(out_heads == heads, "%s_out must have the heads of %s" % (name, name))
-        ends.append((x.data_ptr(), y.data_ptr(), heads, stride, out_stride, y))
-    (qp, qo, qh, qs, qos, q_out), (kp, ko, kh, ks, kos, k_out) = ends
-    _need(table.turns.get_device() == dev, "the rotary table is on another device")
-    rc = _rotary(stream, _pack_rotary(qp, kp, qo, ko, _indices(positions, "positions", tokens, dev), table.turns.data_ptr(), tokens,
-                                         qs, ks, qos, kos, qh, kh, head_dim, table.rotary_dim, 1 if interleaved else 0, table.magnitude))
-    if rc != RC_SUCCESS:
+    tokens, _, head_dim = (k if q is None else q).shape
+    qp = qo = qh = qs = qos = kp = ko = kh = ks = kos = 0
+    if q is not None:
+        qh, qs = _heads(q, "q", tokens, head_dim, dev)
+        if q_out is None:
+            q_out = torch.empty((tokens, qh, head_dim), dtype=_F16, device=q.device)
+        heads, qos = _heads(q_out, "q_out", tokens, head_dim, dev)
+        qp, qo = q.data_ptr(), q_out.data_ptr()
+        if heads != qh:
+            raise ValueError("q_out must have the heads of q")
+    if k is not None:
+        kh, ks = _heads(k, "k", tokens, head_dim, dev)
+        if k_out is None:
+            k_out = torch.empty((tokens, kh, head_dim), dtype=_F16, device=k.device)
+        heads, kos = _heads(k_out, "k_out", tokens, head_dim, dev)
+        kp, ko = k.data_ptr(), k_out.data_ptr()
+        if heads != kh:
+            raise ValueError("k_out must have the heads of k")
+    if table.device_index != dev:
+        raise ValueError("the rotary table is on another device")
+    rc = _rotary(stream, _pack_rotary(qp, kp, qo, ko, _indices(positions, "positions", tokens, dev), table.address, tokens,
+                                      qs, ks, qos, kos, qh, kh, head_dim, table.rotary_dim, 1 if interleaved else 0, table.magnitude))
+    if rc:
         raise PplError(rc)
-    return q_out, k_out
+    return (None if q is None else q_out), (None if k is None else k_out)
 
 
 class PagedKVCache:
@@ -119,7 +124,6 @@ class PagedKVCache:
     dimensions: a cache that is stored token by token is passed as its transpose(1, 2)."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
-        import torch
         _need(k.dim() == 4 and v.shape == k.shape and v.stride() == k.stride(), "k and v must be [pages, heads, tokens, dimensions], laid out alike")
         _need(k.dtype == v.dtype and k.dtype in (torch.float16, torch.int8), "k and v must be fp16 or int8")
         _need((k.dtype == torch.int8) == (k_scale is not None) == (v_scale is not None), "an int8 cache has scales, an fp16 cache none")
@@ -143,7 +147,6 @@ class PagedKVCache:
     @classmethod
     def allocate(cls, num_pages, page_size, kv_heads, head_dim, quant_group=0, device="cuda"):
         """A zeroed cache; quant_group 0 (fp16), 8 or head_dim (int8)."""
-        import torch
         _need(quant_group in (0, 8, head_dim), "quant_group must be 0, 8 or head_dim")
         k, v = (torch.zeros((num_pages, kv_heads, page_size, head_dim), dtype=torch.int8 if quant_group else torch.float16, device=device)
                 for _ in range(2))
@@ -155,25 +158,26 @@ class PagedKVCache:
 
 def _store(cache, q, k, v, positions, slots, table, interleaved, q_out):
     dev, stream = _here()
-    _need(cache.device_index == dev, "the cache is not on the current device")
     tokens, dim = k.shape[0], cache.head_dim
     kh, ks = _heads(k, "k", tokens, dim, dev)
     vh, vs = _heads(v, "v", tokens, dim, dev)
-    _need(kh == vh == cache.kv_heads, "k and v must have the cache's heads")
+    if kh != cache.kv_heads or vh != kh or cache.device_index != dev:
+        raise ValueError("k and v must have the cache's %d heads, and the cache be on device %d" % (cache.kv_heads, dev))
     qp = qo = qh = qs = qos = pos = turns = rotary_dim = 0
     magnitude = 1.0
     if table is not None:
         if q is not None:
             qh, qs = _heads(q, "q", tokens, dim, dev)
-            out_heads, qos = _heads(q_out, "q_out", tokens, dim, dev)
-            _need(out_heads == qh, "q_out must have the heads of q")
+            heads, qos = _heads(q_out, "q_out", tokens, dim, dev)
             qp, qo = q.data_ptr(), q_out.data_ptr()
-        _need(table.turns.get_device() == dev, "the rotary table is on another device")
-        pos, turns = _indices(positions, "positions", tokens, dev), table.turns.data_ptr()
-        rotary_dim, magnitude = table.rotary_dim, table.magnitude
+            if heads != qh:
+                raise ValueError("q_out must have the heads of q")
+        if table.device_index != dev:
+            raise ValueError("the rotary table is on another device")
+        pos, turns, rotary_dim, magnitude = _indices(positions, "positions", tokens, dev), table.address, table.rotary_dim, table.magnitude
     rc = _write(stream, cache._block, _pack_write(qp, k.data_ptr(), v.data_ptr(), qo, pos, _indices(slots, "slots", tokens, dev), turns,
-                                                     tokens, qs, ks, vs, qos, qh, rotary_dim, 1 if interleaved else 0, magnitude))
-    if rc != RC_SUCCESS:
+                                                  tokens, qs, ks, vs, qos, qh, rotary_dim, 1 if interleaved else 0, magnitude))
+    if rc:
         raise PplError(rc)
 
 
@@ -184,7 +188,6 @@ def kv_cache_write(cache, k, v, slots):
 
 def rotary_kv_cache_write(cache, q, k, v, positions, slots, table, interleaved=False, q_out=None):
     """rotary_fp16 of q and k and kv_cache_write of the rotated k and of v, in one pass.  Returns the rotated q."""
-    import torch
     if q is not None and q_out is None:
         q_out = torch.empty(q.shape, dtype=torch.float16, device=q.device)
     _store(cache, q, k, v, positions, slots, table, interleaved, q_out)
@@ -193,21 +196,21 @@ def rotary_kv_cache_write(cache, q, k, v, positions, slots, table, interleaved=F
 
 def kv_cache_read(cache, slots, k_out=None, v_out=None):
     """-> (k, v) fp16 [tokens, kv_heads, head_dim], what is stored at `slots` (int64 [tokens]; negative: zeros)."""
-    import torch
     dev, stream = _here()
-    _need(cache.device_index == dev, "the cache is not on the current device")
-    tokens = slots.shape[0]
-    shape = (tokens, cache.kv_heads, cache.head_dim)
-    outs = []
+    tokens, heads, dim = slots.shape[0], cache.kv_heads, cache.head_dim
+    if cache.device_index != dev:
+        raise ValueError("the cache is not on the current device")
+    if k_out is None:
+        k_out = torch.empty((tokens, heads, dim), dtype=_F16, device=cache.k.device)
+    if v_out is None:
+        v_out = torch.empty((tokens, heads, dim), dtype=_F16, device=cache.k.device)
     for name, t in (("k_out", k_out), ("v_out", v_out)):
-        if t is None:
-            t = torch.empty(shape, dtype=torch.float16, device=cache.k.device)
-        _need(t.dtype is torch.float16 and t.shape == shape and t.is_contiguous() and t.get_device() == dev, "%s must be a contiguous fp16 %s" % (name, shape))
-        outs.append(t)
-    rc = _read(stream, cache._block, _indices(slots, "slots", tokens, dev), tokens, outs[0].data_ptr(), outs[1].data_ptr())
-    if rc != RC_SUCCESS:
+        if t.shape != (tokens, heads, dim) or t.dtype is not _F16 or not t.is_contiguous() or t.get_device() != dev:
+            raise ValueError("%s must be a contiguous fp16 [%d, %d, %d] on device %d" % (name, tokens, heads, dim, dev))
+    rc = _read(stream, cache._block, _indices(slots, "slots", tokens, dev), tokens, k_out.data_ptr(), v_out.data_ptr())
+    if rc:
         raise PplError(rc)
-    return outs[0], outs[1]
+    return k_out, v_out
 
 
 class PagedDecodeAttention:
@@ -215,7 +218,6 @@ class PagedDecodeAttention:
     one object serves one stream at a time.  scale: 1 / sqrt(head_dim) unless given; window: how many of the last tokens are seen (0: all)."""
 
     def __init__(self, cache, q_heads, max_batch, max_length, scale=None, window=0):
-        import torch
         _need(q_heads > 0 and q_heads % cache.kv_heads == 0, "q_heads must be a multiple of the cache's heads")
         _need(max_batch >= 0 and max_length >= 0 and window >= 0, "negative extent")
         self.cache, self.q_heads, self.max_batch, self.window = cache, q_heads, max_batch, window
@@ -223,32 +225,32 @@ class PagedDecodeAttention:
         self.scale = cache.head_dim ** -0.5 if scale is None else scale
         need = lib.pplb200_paged_decode_attention_workspace_bytes(max_batch, self.max_pages * cache.page_size, q_heads, cache.kv_heads, cache.head_dim)
         self.ws = torch.zeros((need,), dtype=torch.uint8, device=cache.k.device)
+        self._ws, self._ws_bytes = self.ws.data_ptr(), need
 
     def __call__(self, q, pages, lengths, out=None, lse=None):
         """q fp16 [batch, q_heads, head_dim], pages int32 [batch, pages a sequence] (negative: a hole), lengths int32 [batch] -> out as q;
         lse fp32 [batch, q_heads], where given, receives log(sum exp(scores))."""
-        import torch
         (dev, stream), cache = _here(), self.cache
-        batch = q.shape[0]
-        heads, qs = _heads(q, "q", batch, cache.head_dim, dev)
+        batch, heads, dim = q.shape[0], self.q_heads, cache.head_dim
         if out is None:
-            out = torch.empty((batch, heads, cache.head_dim), dtype=torch.float16, device=q.device)
-        out_heads, os_ = _heads(out, "out", batch, cache.head_dim, dev)
-        if cache.device_index != dev or heads != self.q_heads or out_heads != heads or batch > self.max_batch:
-            raise ValueError("expected at most %d sequences of %d heads on the cache's device %d" % (self.max_batch, self.q_heads, cache.device_index))
-        if (pages.dtype is not torch.int32 or lengths.dtype is not torch.int32 or pages.dim() != 2 or pages.shape[0] != batch or lengths.shape != (batch,)
-                or pages.get_device() != dev or lengths.get_device() != dev):
-            raise ValueError("pages must be int32 [%d, pages] and lengths int32 [%d] on device %d" % (batch, batch, dev))
-        width = pages.shape[1]
-        _need(width <= self.max_pages, "the page table is wider than max_length tokens")
-        _need((width <= 1 or pages.stride(1) == 1) and (batch <= 1 or lengths.stride(0) == 1), "rows of pages and lengths must be contiguous")
+            out = torch.empty((batch, heads, dim), dtype=_F16, device=q.device)
+        qh, qs = _heads(q, "q", batch, dim, dev)
+        oh, os_ = _heads(out, "out", batch, dim, dev)
+        if qh != heads or oh != heads or batch > self.max_batch or cache.device_index != dev:
+            raise ValueError("expected at most %d sequences of %d heads on the cache's device %d" % (self.max_batch, heads, cache.device_index))
+        shape, stride = pages.shape, pages.stride()
+        if (len(shape) != 2 or shape[0] != batch or shape[1] > self.max_pages or (stride[1] != 1 and shape[1] > 1) or pages.dtype is not _I32
+                or pages.get_device() != dev):
+            raise ValueError("pages must be int32 [%d, at most %d] with contiguous rows on device %d" % (batch, self.max_pages, dev))
+        if lengths.shape != (batch,) or lengths.dtype is not _I32 or (lengths.stride(0) != 1 and batch > 1) or lengths.get_device() != dev:
+            raise ValueError("lengths must be a contiguous int32 [%d] tensor on device %d" % (batch, dev))
         lse_ptr = 0
         if lse is not None:
-            _need(lse.dtype is torch.float32 and lse.shape == (batch, heads) and lse.is_contiguous() and lse.get_device() == dev, "lse must be a contiguous fp32 [batch, heads]")
+            if lse.shape != (batch, heads) or lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.get_device() != dev:
+                raise ValueError("lse must be a contiguous fp32 [%d, %d] tensor on device %d" % (batch, heads, dev))
             lse_ptr = lse.data_ptr()
-        ws = self.ws
-        rc = _attend(stream, cache._block, _pack_attention(q.data_ptr(), out.data_ptr(), lse_ptr, pages.data_ptr(), lengths.data_ptr(), ws.data_ptr(),
-                                                              ws.numel(), batch, width, pages.stride(0), qs, os_, heads, self.window, self.scale, 0))
-        if rc != RC_SUCCESS:
+        rc = _attend(stream, cache._block, _pack_attention(q.data_ptr(), out.data_ptr(), lse_ptr, pages.data_ptr(), lengths.data_ptr(), self._ws, self._ws_bytes,
+                                                           batch, shape[1], stride[0], qs, os_, heads, self.window, self.scale, 0))
+        if rc:
             raise PplError(rc)
         return out
