@@ -31,7 +31,13 @@ int32_t check_kv_cache(const pplb200_kv_cache* c) {
 
 namespace {
 
-constexpr int TPB = 256; // reading back
+#ifndef NU
+#define NU 2
+#endif
+#ifndef NT
+#define NT 256
+#endif
+constexpr int TPB = NT; // reading back
 
 enum : int { Q = 0, K = 1, V = 2 };
 
@@ -105,14 +111,14 @@ __device__ __forceinline__ uint2 quantize_eight(const Eight& e, half scale) {
                       __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
 }
 
-// Cosines and sines (times the magnitude) of eight planes: the angle modulo one turn, exactly, as a signed fraction, in half turns.
+// Cosines and sines (times the magnitude) of four and four planes: the angle modulo one turn, exactly, as a signed fraction, in half turns.
 struct Turns {
     float c[8], s[8];
 };
-__device__ __forceinline__ void turns_at(Turns& t, uint64_t position, const uint64_t* turns, float magnitude) {
+__device__ __forceinline__ void turns_at(Turns& t, uint64_t position, const uint64_t* first, const uint64_t* second, float magnitude) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        sincospif((float)(int64_t)(position * turns[i]) * 0x1p-63f, &t.s[i], &t.c[i]);
+        sincospif((float)(int64_t)(position * (i < 4 ? first[i] : second[i - 4])) * 0x1p-63f, &t.s[i], &t.c[i]);
         t.c[i] *= magnitude;
         t.s[i] *= magnitude;
     }
@@ -132,8 +138,8 @@ __device__ __forceinline__ void rotate(Eight& a, Eight& b, const Turns& t, bool 
     }
 }
 
-// A thread has 16 dimensions of a token: two runs of eight that are rotated against each other (half layout: rotary_dim / 2
-// apart), so that nothing crosses threads but the scale of a whole head.  It computes their eight sines and cosines once, while its
+// A thread has 16 dimensions of a token: two runs of eight that are rotated against each other (half layout) or each in itself, so that
+// nothing crosses threads but the scale of a whole head; neighbouring threads have neighbouring runs, so that loads and stores fill lines.  It computes their eight sines and cosines once, while its
 // first rows are on their way, and takes every groups-th head of q, k and v with them; LANES threads side by side make a row.
 constexpr int RTPB = 128;
 template <int LANES, bool INTERLEAVED, bool STORE>
@@ -143,21 +149,13 @@ struct RotaryKv {
     };
     const RotaryKvParams& p;
     int64_t token;
-    int u;
+    int u, da, db; // the thread's number in its row, and where its runs begin
     bool active, turned; // whether the thread has dimensions, and whether they are rotated
     Turns turns;
     int64_t at, scale_at; // in the cache; at < 0: not stored
 
     template <int KIND>
-    __device__ __forceinline__ void places(int& da, int& db) const {
-        const bool apart = !INTERLEAVED && KIND != V && turned;
-        da = apart ? 8 * u : 16 * u;
-        db = apart ? (p.rotary_dim >> 1) + 8 * u : 16 * u + 8;
-    }
-    template <int KIND>
     __device__ __forceinline__ void fetch(int head, Row& x) const {
-        int da, db;
-        places<KIND>(da, db);
         x.a.raw = x.b.raw = make_uint4(0, 0, 0, 0);
         if (active && head < p.heads[KIND]) {
             const half* src = p.src[KIND] + token * p.src_stride[KIND] + (int64_t)head * p.head_dim;
@@ -168,8 +166,6 @@ struct RotaryKv {
     // Called by all threads of a warp.
     template <int KIND>
     __device__ __forceinline__ void finish(int head, Row& x) const {
-        int da, db;
-        places<KIND>(da, db);
         if (KIND != V && turned) rotate(x.a, x.b, turns, INTERLEAVED);
         const bool there = active && head < p.heads[KIND];
         if constexpr (!STORE || KIND == Q) {
@@ -199,12 +195,8 @@ struct RotaryKv {
             const half sa = group_scale(ma), sb = p.cache.quant_group == 8 ? group_scale(mb) : sa;
             const uint2 qa = quantize_eight(x.a, sa), qb = quantize_eight(x.b, sb);
             int8_t* dst = (int8_t*)data + row;
-            if (KIND == V || INTERLEAVED || !turned) {
-                *reinterpret_cast<uint4*>(dst + da) = make_uint4(qa.x, qa.y, qb.x, qb.y);
-            } else {
-                *reinterpret_cast<uint2*>(dst + da) = qa;
-                *reinterpret_cast<uint2*>(dst + db) = qb;
-            }
+            *reinterpret_cast<uint2*>(dst + da) = qa;
+            *reinterpret_cast<uint2*>(dst + db) = qb;
             half* scale = (half*)(KIND == V ? p.cache.v_scale : p.cache.k_scale) + scale_at + (int64_t)head * p.cache.scale_head_stride;
             if (p.cache.quant_group == 8) {
                 scale[da >> 3] = sa;
@@ -238,11 +230,18 @@ __global__ void __launch_bounds__(RTPB, 7) rotary_kv_kernel(const __grid_constan
     r.u = threadIdx.x & (LANES - 1);
     r.active = valid && 16 * r.u < p.head_dim;
     r.turned = valid && 16 * r.u < p.rotary_dim;
+    // runs of the rotated part lie half of it apart, those behind it half of the rest
+    const int behind = r.u - (p.rotary_dim >> 4);
+    r.da = behind < 0 ? 8 * r.u : p.rotary_dim + 8 * behind;
+    r.db = r.da + ((behind < 0 ? p.rotary_dim : p.head_dim - p.rotary_dim) >> 1);
     typename RotaryKv<LANES, INTERLEAVED, STORE>::Row q, k, v;
     r.template fetch<Q>(group, q);
     r.template fetch<K>(group, k);
     if (STORE) r.template fetch<V>(group, v);
-    if (r.turned) turns_at(r.turns, (uint64_t)p.positions[r.token], p.turns + 8 * r.u, p.magnitude);
+    if (r.turned) {
+        const uint64_t* first = p.turns + (INTERLEAVED ? 4 : 8) * r.u; // planes of the runs: eight of both, or four of each
+        turns_at(r.turns, (uint64_t)p.positions[r.token], first, first + (INTERLEAVED ? p.rotary_dim >> 2 : 4), p.magnitude);
+    }
     r.at = -1;
     r.scale_at = 0;
     if (STORE && valid) {
@@ -284,80 +283,74 @@ int32_t launch_rotary_kv(cudaStream_t stream, RotaryKvParams& p) {
     return p.head_dim <= 64 ? launch_lanes<4>(stream, p) : p.head_dim <= 128 ? launch_lanes<8>(stream, p) : launch_lanes<16>(stream, p);
 }
 
-// 16 dimensions of a key and of the value beside it a thread; where a token lies is looked up once a CTA.
+// Eight dimensions of a key and of the value beside it are a unit, so that a warp's stores fill whole lines (16 dimensions a thread, in two
+// stores of every other 16 bytes: 32768 tokens 41 us); a thread takes UNITS of them, a block apart.
+constexpr int UNITS = NU;
 struct KvReadParams {
     pplb200_kv_cache cache;
     const int64_t* slots;
-    int64_t tokens;
     half *k_out, *v_out;
-    int32_t tokens_per_cta, units; // 16 dimensions each, of a token
+    int64_t tokens;
+    int32_t units; // of a token
     uint32_t units_magic, units_shift, head_magic, head_shift;
 };
+// Bytes 0 to 3 of a word times a scale: whole numbers as halves (a byte with its sign flipped beneath 0x64 is 1152 + value), one rounding.
+__device__ __forceinline__ void scaled(uint32_t w, __half2 s, __half2& lo, __half2& hi) {
+    w ^= 0x80808080u;
+    const __half2 offset = __float2half2_rn(1152.0f);
+    uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+    lo = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&a), offset), s);
+    hi = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&b), offset), s);
+}
+__device__ __forceinline__ uint2 ld_global_8(const void* p) {
+    uint2 v;
+    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+template <bool INT8>
 __global__ void __launch_bounds__(TPB) kv_read_kernel(const __grid_constant__ KvReadParams p) {
-    struct Row {
-        int64_t at, scale_at;
-    };
-    __shared__ Row where[TPB];
     const pplb200_kv_cache& c = p.cache;
     pdl_wait_prior_grid();
-    const int64_t token0 = (int64_t)blockIdx.x * p.tokens_per_cta;
-    const int tokens = (int)min((int64_t)p.tokens_per_cta, p.tokens - token0);
-    if (threadIdx.x < tokens) {
-        Row w = {-1, 0};
-        int64_t page;
-        int32_t in_page;
-        if (kv_find(p.slots[token0 + threadIdx.x], c.num_pages, c.page_size, page, in_page)) {
-            w.at = kv_row(page, in_page, 0, c.page_stride, 0, c.token_stride);
-            w.scale_at = kv_row(page, in_page, 0, c.scale_page_stride, 0, c.scale_token_stride);
-        }
-        where[threadIdx.x] = w;
-    }
-    __syncthreads();
-    const int per_head = c.head_dim >> 4;
-    for (int i = blockIdx.y * TPB + threadIdx.x; i < tokens * p.units; i += gridDim.y * TPB) {
-        const int local = (int)((uint64_t)(uint32_t)i * p.units_magic >> p.units_shift), unit = i - local * p.units;
-        const int head = (int)((uint64_t)(uint32_t)unit * p.head_magic >> p.head_shift), d = (unit - head * per_head) * 16;
-        const Row w = where[local];
-        const int64_t at = w.at + (int64_t)head * c.head_stride + d;
-        const int64_t scale_at = w.scale_at + (int64_t)head * c.scale_head_stride + (c.quant_group == 8 ? d >> 3 : 0);
-        Eight o[2][2];
+    // a block's units: of whole tokens where a token has fewer than a block, else part of one
+    const int per_head = c.head_dim >> 3, tokens_here = max(1, TPB * UNITS / p.units);
+    const int64_t token0 = (int64_t)blockIdx.x * tokens_here;
+    const int all = (int)min((int64_t)tokens_here, p.tokens - token0) * p.units;
+    for (int first = blockIdx.y * TPB * UNITS + threadIdx.x; first < all; first += gridDim.y * TPB * UNITS) {
+        Eight o[UNITS][2];
+        uint2 q[UNITS][2];
+        half s[UNITS][2];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) o[n >> 1][n & 1].raw = make_uint4(0, 0, 0, 0);
-        if (w.at >= 0) {
-            if (c.quant_group == 0) {
+        for (int i = 0; i < UNITS; ++i) {
+            const uint32_t n = min(first + i * TPB, all - 1), local = (uint32_t)((uint64_t)n * p.units_magic >> p.units_shift), unit = n - local * p.units;
+            const uint32_t head = (uint32_t)((uint64_t)unit * p.head_magic >> p.head_shift), d = (unit - head * per_head) * 8;
+            int64_t page = 0;
+            int32_t in_page = 0;
+            const bool found = kv_find(p.slots[token0 + local], c.num_pages, c.page_size, page, in_page);
+            const int64_t at = kv_row(page, in_page, head, c.page_stride, c.head_stride, c.token_stride) + d;
+            const int64_t scale_at = kv_row(page, in_page, head, c.scale_page_stride, c.scale_head_stride, c.scale_token_stride) + (c.quant_group == 8 ? d >> 3 : 0);
 #pragma unroll
-                for (int n = 0; n < 4; ++n) o[n >> 1][n & 1].raw = ld_global_16((const half*)(n >> 1 ? c.v : c.k) + at + 8 * (n & 1));
-            } else {
-                uint4 q[2];
-                half s[2][2];
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    q[n] = ld_global_16((const int8_t*)(n ? c.v : c.k) + at);
-                    const half* scale = (const half*)(n ? c.v_scale : c.k_scale) + scale_at;
-                    s[n][0] = ld_global_half(scale);
-                    s[n][1] = c.quant_group == 8 ? ld_global_half(scale + 1) : s[n][0];
-                }
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const uint32_t words[4] = {q[n].x, q[n].y, q[n].z, q[n].w};
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        // a byte with its sign flipped beneath 0x64 is 1152 + value, as a half: whole numbers, then one rounding
-                        const uint32_t w4 = words[x] ^ 0x80808080u;
-                        const __half2 s2 = __half2half2(s[n][x >> 1]), offset = __float2half2_rn(1152.0f);
-                        uint32_t lo = __byte_perm(w4, 0x64646464u, 0x4140), hi = __byte_perm(w4, 0x64646464u, 0x4342);
-                        o[n][x >> 1].h[2 * (x & 1)] = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&lo), offset), s2);
-                        o[n][x >> 1].h[2 * (x & 1) + 1] = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&hi), offset), s2);
-                    }
+            for (int x = 0; x < 2; ++x) {
+                if constexpr (INT8) {
+                    q[i][x] = found ? ld_global_8((const int8_t*)(x ? c.v : c.k) + at) : make_uint2(0, 0);
+                    s[i][x] = found ? ld_global_half((const half*)(x ? c.v_scale : c.k_scale) + scale_at) : __ushort_as_half(0);
+                } else {
+                    o[i][x].raw = found ? ld_global_16((const half*)(x ? c.v : c.k) + at) : make_uint4(0, 0, 0, 0);
                 }
             }
         }
-        const int64_t out = ((token0 * p.units) + i) * 16;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            half* dst = (n ? p.v_out : p.k_out) + out;
-            *reinterpret_cast<uint4*>(dst) = o[n][0].raw;
-            *reinterpret_cast<uint4*>(dst + 8) = o[n][1].raw;
+        for (int i = 0; i < UNITS; ++i) {
+            if (first + i * TPB >= all) break;
+            const int64_t out = (token0 * p.units + first + i * TPB) * 8;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                if constexpr (INT8) {
+                    const __half2 s2 = __half2half2(s[i][x]);
+                    scaled(q[i][x].x, s2, o[i][x].h[0], o[i][x].h[1]);
+                    scaled(q[i][x].y, s2, o[i][x].h[2], o[i][x].h[3]);
+                }
+                *reinterpret_cast<uint4*>((x ? p.v_out : p.k_out) + out) = o[i][x].raw;
+            }
         }
     }
 }
@@ -489,14 +482,13 @@ int32_t pplb200_kv_cache_read_fp16(pplb200_stream_t stream, const pplb200_kv_cac
     p.cache = *cache;
     p.slots = slots; p.tokens = tokens;
     p.k_out = (half*)k_out; p.v_out = (half*)v_out;
-    p.units = cache->kv_heads * (cache->head_dim / 16);
-    // about two units a thread; a token of very many heads is shared by CTAs
-    p.tokens_per_cta = (int32_t)std::min<int64_t>(TPB, std::max<int64_t>(1, 2 * TPB / p.units));
-    const int64_t blocks = (tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
-    const unsigned shares = (unsigned)std::max<int64_t>(1, std::min<int64_t>(p.units / (2 * TPB), 65535));
+    p.units = cache->kv_heads * (cache->head_dim / 8);
+    const int64_t tokens_here = std::max<int64_t>(1, TPB * UNITS / p.units), shares = std::min<int64_t>((p.units + TPB * UNITS - 1) / (TPB * UNITS), 65535);
     small_division(p.units, p.units_magic, p.units_shift);
-    small_division(cache->head_dim / 16, p.head_magic, p.head_shift);
-    launch_ex(kv_read_kernel, dim3((unsigned)blocks, shares), dim3(TPB), (cudaStream_t)stream, true, p);
+    small_division(cache->head_dim / 8, p.head_magic, p.head_shift);
+    const dim3 grid((unsigned)((tokens + tokens_here - 1) / tokens_here), (unsigned)shares);
+    if (cache->quant_group) launch_ex(kv_read_kernel<true>, grid, dim3(TPB), (cudaStream_t)stream, true, p);
+    else launch_ex(kv_read_kernel<false>, grid, dim3(TPB), (cudaStream_t)stream, true, p);
     return check_launch("cache read");
 }
 
