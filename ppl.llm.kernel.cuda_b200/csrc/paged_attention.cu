@@ -146,8 +146,17 @@ __device__ __forceinline__ int32_t steps_of(const AttentionParams& p, int64_t b)
 
 // What beginning a head of a sequence costs, in steps: a chain of look-ups before the first step, the joining of the warps' sums behind
 // the last, while the other CTAs of the SM go on.
+#ifndef MINR
+#define MINR 2
+#endif
+#ifndef JOINR
+#define JOINR 3
+#endif
+#ifndef PADR
+#define PADR 2
+#endif
 template <class S>
-constexpr int32_t kBeginning = 2 * S::WARPS;
+constexpr int32_t kBeginning = PADR * S::WARPS;
 
 struct Share { // where a CTA's share begins or ends: a step of a head of a sequence
     int64_t b;
@@ -210,9 +219,9 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
         }
         all = total * heads_per_sequence;
         const int64_t items = p.batch * heads_per_sequence;
-        ctas = (int32_t)min((int64_t)gridDim.x, max((int64_t)1, all / (2 * WARPS)));
+        ctas = (int32_t)min((int64_t)gridDim.x, max((int64_t)1, all / (MINR * WARPS)));
         // Joining takes about as long as three rounds of steps.
-        const bool whole_items = items <= gridDim.x && most <= all / ctas + 3 * WARPS;
+        const bool whole_items = items <= gridDim.x && most <= all / ctas + JOINR * WARPS;
         if (whole_items) ctas = (int32_t)items;
         if (blockIdx.x >= ctas) return;
         if (whole_items) {

@@ -31,13 +31,7 @@ int32_t check_kv_cache(const pplb200_kv_cache* c) {
 
 namespace {
 
-#ifndef NU
-#define NU 2
-#endif
-#ifndef NT
-#define NT 256
-#endif
-constexpr int TPB = NT; // reading back
+constexpr int TPB = 256; // reading back
 
 enum : int { Q = 0, K = 1, V = 2 };
 
@@ -283,15 +277,15 @@ int32_t launch_rotary_kv(cudaStream_t stream, RotaryKvParams& p) {
     return p.head_dim <= 64 ? launch_lanes<4>(stream, p) : p.head_dim <= 128 ? launch_lanes<8>(stream, p) : launch_lanes<16>(stream, p);
 }
 
-// Eight dimensions of a key and of the value beside it are a unit, so that a warp's stores fill whole lines (16 dimensions a thread, in two
-// stores of every other 16 bytes: 32768 tokens 41 us); a thread takes UNITS of them, a block apart.
-constexpr int UNITS = NU;
+// Eight dimensions of a key and of the value beside it are a unit, so that a warp's stores fill whole lines.  A block looks up once
+// where its tokens lie (look-ups by every thread: 207 instructions a unit, 32768 tokens 42 us) and then goes through their units.
+constexpr int UNITS = 4; // a thread
 struct KvReadParams {
     pplb200_kv_cache cache;
     const int64_t* slots;
     half *k_out, *v_out;
     int64_t tokens;
-    int32_t units; // of a token
+    int32_t units, tokens_here; // units of a token, tokens of a block
     uint32_t units_magic, units_shift, head_magic, head_shift;
 };
 // Bytes 0 to 3 of a word times a scale: whole numbers as halves (a byte with its sign flipped beneath 0x64 is 1152 + value), one rounding.
@@ -309,48 +303,53 @@ __device__ __forceinline__ uint2 ld_global_8(const void* p) {
 }
 template <bool INT8>
 __global__ void __launch_bounds__(TPB) kv_read_kernel(const __grid_constant__ KvReadParams p) {
+    struct Row {
+        int64_t at, scale_at; // at < 0: not in the cache
+    };
+    __shared__ Row where[TPB];
     const pplb200_kv_cache& c = p.cache;
     pdl_wait_prior_grid();
-    // a block's units: of whole tokens where a token has fewer than a block, else part of one
-    const int per_head = c.head_dim >> 3, tokens_here = max(1, TPB * UNITS / p.units);
-    const int64_t token0 = (int64_t)blockIdx.x * tokens_here;
-    const int all = (int)min((int64_t)tokens_here, p.tokens - token0) * p.units;
-    for (int first = blockIdx.y * TPB * UNITS + threadIdx.x; first < all; first += gridDim.y * TPB * UNITS) {
-        Eight o[UNITS][2];
-        uint2 q[UNITS][2];
-        half s[UNITS][2];
+    const int64_t token0 = (int64_t)blockIdx.x * p.tokens_here;
+    const int tokens = (int)min((int64_t)p.tokens_here, p.tokens - token0), all = tokens * p.units, per_head = c.head_dim >> 3;
+    if (threadIdx.x < tokens) {
+        Row w = {-1, 0};
+        int64_t page;
+        int32_t in_page;
+        if (kv_find(p.slots[token0 + threadIdx.x], c.num_pages, c.page_size, page, in_page)) {
+            w.at = kv_row(page, in_page, 0, c.page_stride, 0, c.token_stride);
+            w.scale_at = kv_row(page, in_page, 0, c.scale_page_stride, 0, c.scale_token_stride);
+        }
+        where[threadIdx.x] = w;
+    }
+    __syncthreads();
+#pragma unroll 2
+    for (int n = blockIdx.y * TPB + threadIdx.x; n < all; n += gridDim.y * TPB) {
+        const uint32_t local = (uint32_t)((uint64_t)(uint32_t)n * p.units_magic >> p.units_shift), unit = n - local * p.units;
+        const uint32_t head = (uint32_t)((uint64_t)unit * p.head_magic >> p.head_shift), d = (unit - head * per_head) * 8;
+        const Row w = where[local];
+        const bool found = w.at >= 0;
+        const int64_t at = w.at + head * c.head_stride + d, scale_at = w.scale_at + head * c.scale_head_stride + (c.quant_group == 8 ? d >> 3 : 0);
+        Eight o[2];
+        uint2 q[2];
+        half s[2];
 #pragma unroll
-        for (int i = 0; i < UNITS; ++i) {
-            const uint32_t n = min(first + i * TPB, all - 1), local = (uint32_t)((uint64_t)n * p.units_magic >> p.units_shift), unit = n - local * p.units;
-            const uint32_t head = (uint32_t)((uint64_t)unit * p.head_magic >> p.head_shift), d = (unit - head * per_head) * 8;
-            int64_t page = 0;
-            int32_t in_page = 0;
-            const bool found = kv_find(p.slots[token0 + local], c.num_pages, c.page_size, page, in_page);
-            const int64_t at = kv_row(page, in_page, head, c.page_stride, c.head_stride, c.token_stride) + d;
-            const int64_t scale_at = kv_row(page, in_page, head, c.scale_page_stride, c.scale_head_stride, c.scale_token_stride) + (c.quant_group == 8 ? d >> 3 : 0);
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                if constexpr (INT8) {
-                    q[i][x] = found ? ld_global_8((const int8_t*)(x ? c.v : c.k) + at) : make_uint2(0, 0);
-                    s[i][x] = found ? ld_global_half((const half*)(x ? c.v_scale : c.k_scale) + scale_at) : __ushort_as_half(0);
-                } else {
-                    o[i][x].raw = found ? ld_global_16((const half*)(x ? c.v : c.k) + at) : make_uint4(0, 0, 0, 0);
-                }
+        for (int x = 0; x < 2; ++x) {
+            if constexpr (INT8) {
+                q[x] = found ? ld_global_8((const int8_t*)(x ? c.v : c.k) + at) : make_uint2(0, 0);
+                s[x] = found ? ld_global_half((const half*)(x ? c.v_scale : c.k_scale) + scale_at) : __ushort_as_half(0);
+            } else {
+                o[x].raw = found ? ld_global_16((const half*)(x ? c.v : c.k) + at) : make_uint4(0, 0, 0, 0);
             }
         }
+        const int64_t out = (token0 * p.units + n) * 8;
 #pragma unroll
-        for (int i = 0; i < UNITS; ++i) {
-            if (first + i * TPB >= all) break;
-            const int64_t out = (token0 * p.units + first + i * TPB) * 8;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                if constexpr (INT8) {
-                    const __half2 s2 = __half2half2(s[i][x]);
-                    scaled(q[i][x].x, s2, o[i][x].h[0], o[i][x].h[1]);
-                    scaled(q[i][x].y, s2, o[i][x].h[2], o[i][x].h[3]);
-                }
-                *reinterpret_cast<uint4*>((x ? p.v_out : p.k_out) + out) = o[i][x].raw;
+        for (int x = 0; x < 2; ++x) {
+            if constexpr (INT8) {
+                const __half2 s2 = __half2half2(s[x]);
+                scaled(q[x].x, s2, o[x].h[0], o[x].h[1]);
+                scaled(q[x].y, s2, o[x].h[2], o[x].h[3]);
             }
+            *reinterpret_cast<uint4*>((x ? p.v_out : p.k_out) + out) = o[x].raw;
         }
     }
 }
@@ -483,10 +482,13 @@ int32_t pplb200_kv_cache_read_fp16(pplb200_stream_t stream, const pplb200_kv_cac
     p.slots = slots; p.tokens = tokens;
     p.k_out = (half*)k_out; p.v_out = (half*)v_out;
     p.units = cache->kv_heads * (cache->head_dim / 8);
-    const int64_t tokens_here = std::max<int64_t>(1, TPB * UNITS / p.units), shares = std::min<int64_t>((p.units + TPB * UNITS - 1) / (TPB * UNITS), 65535);
+    // few tokens: fewer units a thread, so that there are blocks for all SMs
+    const int64_t each = std::min<int64_t>(UNITS, std::max<int64_t>(1, tokens * p.units / (TPB * 1184LL)));
+    p.tokens_here = (int32_t)std::min<int64_t>(TPB, std::max<int64_t>(1, TPB * each / p.units));
+    const int64_t shares = std::min<int64_t>((p.units + TPB * each - 1) / (TPB * each), 65535);
     small_division(p.units, p.units_magic, p.units_shift);
     small_division(cache->head_dim / 8, p.head_magic, p.head_shift);
-    const dim3 grid((unsigned)((tokens + tokens_here - 1) / tokens_here), (unsigned)shares);
+    const dim3 grid((unsigned)((tokens + p.tokens_here - 1) / p.tokens_here), (unsigned)shares);
     if (cache->quant_group) launch_ex(kv_read_kernel<true>, grid, dim3(TPB), (cudaStream_t)stream, true, p);
     else launch_ex(kv_read_kernel<false>, grid, dim3(TPB), (cudaStream_t)stream, true, p);
     return check_launch("cache read");
