@@ -146,17 +146,8 @@ __device__ __forceinline__ int32_t steps_of(const AttentionParams& p, int64_t b)
 
 // What beginning a head of a sequence costs, in steps: a chain of look-ups before the first step, the joining of the warps' sums behind
 // the last, while the other CTAs of the SM go on.
-#ifndef MINR
-#define MINR 2
-#endif
-#ifndef JOINR
-#define JOINR 3
-#endif
-#ifndef PADR
-#define PADR 2
-#endif
 template <class S>
-constexpr int32_t kBeginning = PADR * S::WARPS;
+constexpr int32_t kBeginning = 2 * S::WARPS;
 
 struct Share { // where a CTA's share begins or ends: a step of a head of a sequence
     int64_t b;
@@ -219,9 +210,9 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
         }
         all = total * heads_per_sequence;
         const int64_t items = p.batch * heads_per_sequence;
-        ctas = (int32_t)min((int64_t)gridDim.x, max((int64_t)1, all / (MINR * WARPS)));
+        ctas = (int32_t)min((int64_t)gridDim.x, max((int64_t)1, all / WARPS)); // a step a warp at least
         // Joining takes about as long as three rounds of steps.
-        const bool whole_items = items <= gridDim.x && most <= all / ctas + JOINR * WARPS;
+        const bool whole_items = items <= gridDim.x && most <= all / ctas + 3 * WARPS;
         if (whole_items) ctas = (int32_t)items;
         if (blockIdx.x >= ctas) return;
         if (whole_items) {
@@ -314,9 +305,8 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
         uint32_t kw[S::SUBS][2][S::KN][S::KP / 4] = {}, vw[S::SUBS][4][S::VN][S::VP / 4] = {};
         uint32_t ks[S::SUBS][2][S::KN] = {}, vs[S::SUBS][4][S::VN] = {}; // CACHE_I8_GROUPS
         uint32_t k_scale = 0, v_scale = 0;                               // CACHE_I8_ROWS: of the lane's token
-        auto load_keys = [&](bool every) {
-#pragma unroll
-            for (int sub = 0; sub < S::SUBS; ++sub)
+        auto load_keys = [&](int sub) {
+            auto load = [&](bool every) {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     const int token = 16 * sub + g + 8 * r;
@@ -336,12 +326,12 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                         }
                     }
                 }
-            if constexpr (S::KIND == CACHE_I8_ROWS)
-                k_scale = (every || (coming >> (lane & (S::TOKENS - 1)) & 1)) ? load_scales<1>(ksbase + (uint64_t)scale_row * p.scale_unit) : 0u;
+            };
+            if (coming == EVERY) load(true);
+            else if (coming) load(false);
         };
-        auto load_values = [&](bool every) {
-#pragma unroll
-            for (int sub = 0; sub < S::SUBS; ++sub)
+        auto load_values = [&](int sub) {
+            auto load = [&](bool every) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int token = 16 * sub + 2 * t + (j & 1) + 8 * (j >> 1);
@@ -362,8 +352,14 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                         }
                     }
                 }
+            };
+            if (coming == EVERY) load(true);
+            else if (coming) load(false);
+        };
+        // CACHE_I8_ROWS: the scales of the lane's token
+        auto load_scale = [&](uint32_t& scale, const char* base) {
             if constexpr (S::KIND == CACHE_I8_ROWS)
-                v_scale = (every || (coming >> (lane & (S::TOKENS - 1)) & 1)) ? load_scales<1>(vsbase + (uint64_t)scale_row * p.scale_unit) : 0u;
+                scale = (coming >> (lane & (S::TOKENS - 1)) & 1) ? load_scales<1>(base + (uint64_t)scale_row * p.scale_unit) : 0u;
         };
 
         Place ahead = find(step0 + warp);
@@ -389,8 +385,12 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
         locate(ahead);
         ahead = second;
         uint32_t seen = coming;
-        if (seen == EVERY) load_keys(true), load_values(true);
-        else if (seen) load_keys(false), load_values(false);
+#pragma unroll
+        for (int sub = 0; sub < S::SUBS; ++sub) load_keys(sub);
+        load_scale(k_scale, ksbase);
+#pragma unroll
+        for (int sub = 0; sub < S::SUBS; ++sub) load_values(sub);
+        load_scale(v_scale, vsbase);
         locate(ahead);
         ahead = find(step0 + warp + 2 * WARPS);
 
@@ -421,6 +421,8 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
 
         for (int32_t step = step0 + warp; step < step1; step += WARPS) {
             float c[S::SUBS][S::NT][4];
+            // Each part of the next step is requested as soon as its registers are free.
+            const uint32_t k_scale_now = k_scale;
             if (seen != 0) {
                 // ---- scores [16 tokens x 8 heads] ------------------------------------------------------------------------
                 constexpr int KW = S::KP / 4;
@@ -475,7 +477,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
 #pragma unroll
                             for (int x = 0; x < 4; ++x) c[sub][nt][x] += c2[nt][x];
                         if constexpr (S::KIND == CACHE_I8_ROWS) {
-                            const float mine = __half2float(__ushort_as_half((unsigned short)k_scale)) * (p.scale_log2 * 0x1p24f);
+                            const float mine = __half2float(__ushort_as_half((unsigned short)k_scale_now)) * (p.scale_log2 * 0x1p24f);
                             const float k0 = __shfl_sync(0xffffffffu, mine, 16 * sub + g), k1 = __shfl_sync(0xffffffffu, mine, 16 * sub + g + 8);
 #pragma unroll
                             for (int nt = 0; nt < S::NT; ++nt)
@@ -488,12 +490,11 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                                 for (int x = 0; x < 4; ++x) c[sub][nt][x] *= p.scale_log2;
                         }
                     }
+                    load_keys(sub);
                 }
-            }
-            if (coming == EVERY) load_keys(true);
-            else if (coming) load_keys(false);
+                load_scale(k_scale, ksbase);
 
-            if (seen != 0) {
+
                 // ---- weights: 2^(score - top + 8) --------------------------------------------------------------------------
                 float v0[S::SUBS], v1[S::SUBS], e0[S::SUBS] = {}, e1[S::SUBS] = {};
                 if constexpr (S::KIND == CACHE_I8_ROWS) {
@@ -608,10 +609,15 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                             }
                         }
                     }
+                    load_values(sub);
                 }
+                load_scale(v_scale, vsbase);
+            } else { // nothing of this step was there
+#pragma unroll
+                for (int sub = 0; sub < S::SUBS; ++sub) load_keys(sub), load_values(sub);
+                load_scale(k_scale, ksbase);
+                load_scale(v_scale, vsbase);
             }
-            if (coming == EVERY) load_values(true);
-            else if (coming) load_values(false);
             seen = coming;
             locate(ahead);
             ahead = find(step + 3 * WARPS);
@@ -679,38 +685,54 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
             __syncthreads();
             if (is_last) {
                 __threadfence();
-                constexpr int BATCH = 8;
-                auto slot_of = [&](int32_t i) { return i == 0 ? 2 * (int64_t)(c0 - 1) + 1 : 2 * (int64_t)(c0 - 1 + i); };
-                for (int x = threadIdx.x; x < q_count * (S::D / 4); x += S::THREADS) {
-                    const int h = x / (S::D / 4), d = (x - h * (S::D / 4)) * 4;
-                    float m = -1e30f, l = 0.0f;
-                    float4 v = make_float4(0, 0, 0, 0);
-                    for (int32_t i = 0; i < pieces; i += BATCH) {
-                        float2 s[BATCH];
-                        float4 a[BATCH];
+                // 16 loads a thread at once: ITEMS places of the output times BATCH pieces
+                constexpr int ITEMS = (S::HEADS * S::D / 4 + S::THREADS - 1) / S::THREADS, BATCH = ITEMS >= 4 ? 4 : 16 / ITEMS;
+                float4 v[ITEMS];
+                float m[ITEMS], l[ITEMS];
+                int h[ITEMS], d[ITEMS];
 #pragma unroll
-                        for (int j = 0; j < BATCH; ++j) {
-                            const int64_t at = slot_of(min(i + j, pieces - 1)) * S::HEADS + h;
-                            s[j] = __ldcg(&p.tops[at]);
-                            a[j] = __ldcg(reinterpret_cast<const float4*>(p.sums + at * S::D + d));
-                            if (i + j >= pieces) s[j] = make_float2(-1e30f, 0.0f);
-                        }
-                        float up = m;
+                for (int x = 0; x < ITEMS; ++x) {
+                    const int at = min((int)threadIdx.x + x * S::THREADS, q_count * (S::D / 4) - 1); // some do the last one again
+                    h[x] = at / (S::D / 4);
+                    d[x] = (at - h[x] * (S::D / 4)) * 4;
+                    v[x] = make_float4(0, 0, 0, 0);
+                    m[x] = -1e30f;
+                    l[x] = 0.0f;
+                }
+                for (int32_t i = 0; i < pieces; i += BATCH) {
+                    float2 s[BATCH][ITEMS];
+                    float4 a[BATCH][ITEMS];
 #pragma unroll
-                        for (int j = 0; j < BATCH; ++j) up = fmaxf(up, s[j].x);
-                        const float keep = exp2_fast(m - up);
-                        m = up;
-                        l *= keep;
-                        v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
+                    for (int j = 0; j < BATCH; ++j) {
+                        const int32_t n = min(i + j, pieces - 1);
+                        const int64_t slot = (n == 0 ? 2 * (int64_t)(c0 - 1) + 1 : 2 * (int64_t)(c0 - 1 + n)) * S::HEADS;
 #pragma unroll
-                        for (int j = 0; j < BATCH; ++j) {
-                            const float f = i + j < pieces ? exp2_fast(s[j].x - m) : 0.0f;
-                            l += f * s[j].y;
-                            if (i + j < pieces) v.x += f * a[j].x, v.y += f * a[j].y, v.z += f * a[j].z, v.w += f * a[j].w;
+                        for (int x = 0; x < ITEMS; ++x) {
+                            s[j][x] = __ldcg(&p.tops[slot + h[x]]);
+                            a[j][x] = __ldcg(reinterpret_cast<const float4*>(p.sums + (slot + h[x]) * S::D + d[x]));
+                            if (i + j >= pieces) s[j][x].x = -INFINITY; // the last piece once more, without weight
                         }
                     }
-                    finish(p, b, head0 + h, S::D, d, v, m, l);
+#pragma unroll
+                    for (int x = 0; x < ITEMS; ++x) {
+                        float up = m[x];
+#pragma unroll
+                        for (int j = 0; j < BATCH; ++j) up = fmaxf(up, s[j][x].x);
+                        const float keep = exp2_fast(m[x] - up);
+                        m[x] = up;
+                        l[x] *= keep;
+                        v[x].x *= keep; v[x].y *= keep; v[x].z *= keep; v[x].w *= keep;
+#pragma unroll
+                        for (int j = 0; j < BATCH; ++j)
+                            if (i + j < pieces) {
+                                const float f = exp2_fast(s[j][x].x - up);
+                                l[x] += f * s[j][x].y;
+                                v[x].x += f * a[j][x].x; v[x].y += f * a[j][x].y; v[x].z += f * a[j][x].z; v[x].w += f * a[j][x].w;
+                            }
+                    }
                 }
+#pragma unroll
+                for (int x = 0; x < ITEMS; ++x) finish(p, b, head0 + h[x], S::D, d[x], v[x], m[x], l[x]);
             }
         }
         __syncthreads();
