@@ -21,14 +21,22 @@ enum : int { CACHE_F16 = 0, CACHE_I8_GROUPS = 1, CACHE_I8_ROWS = 2 };
 
 constexpr int piece(int bytes) { return bytes % 16 == 0 ? 16 : bytes % 8 == 0 ? 8 : 4; }
 
-// Sizes of one variant: D dimensions, KIND of cache, NT blocks of eight query heads.
-template <int D_, int KIND_, int NT_>
+// Sizes of one variant: D dimensions, KIND of cache, NT blocks of eight query heads.  PACKED: a page has a multiple of 16 tokens, whose
+// rows follow each other, so that 16 tokens are one address and offsets that the instructions hold.
+template <int D_, int KIND_, int NT_, bool PACKED_>
 struct Shape {
     static constexpr int D = D_, KIND = KIND_, NT = NT_, HEADS = 8 * NT;
+    static constexpr bool PACKED = PACKED_;
     static constexpr int ES = KIND == CACHE_F16 ? 2 : 1;
     // Tokens of a step: 32 where that leaves room for twelve warps on an SM (64 x 8192, int8 rows: 123 us with 32, 129 with 16; groups,
     // whose scales take registers too: 16 x 4096 71 us with 32, 67 with 16).
-    static constexpr int SUBS = D * ES <= 64 || (D * ES <= 128 && KIND == CACHE_I8_ROWS) ? 2 : 1, TOKENS = 16 * SUBS;
+#ifndef PSUB
+#define PSUB 2
+#endif
+#ifndef PL4
+#define PL4 88
+#endif
+    static constexpr int SUBS = D * ES <= 64 ? 2 : D * ES <= 128 && KIND == CACHE_I8_ROWS ? (PACKED ? PSUB : 2) : 1, TOKENS = 16 * SUBS;
     // of 16 tokens a quad's lane holds a quarter of the dimensions of two keys, an eighth of those of four values
     static constexpr int KB = D * ES / 4, KP = piece(KB), KN = KB / KP;
     static constexpr int VB = D * ES / 8, VP = piece(VB), VN = VB / VP;
@@ -37,7 +45,7 @@ struct Shape {
     // Registers for the sums, the queries and the tokens on their way decide how many CTAs share an SM.
     static constexpr int WORDS = NT * D / 4 + NT * D / 8 + SUBS * (D * ES / 4 + (KIND == CACHE_I8_GROUPS ? 2 * KN + 4 * VN : 0));
     static constexpr int ROW = D + 4; // of the sums that the warps exchange
-    static constexpr int WARPS = 4, THREADS = 32 * WARPS, CTAS = WORDS <= 88 ? 4 : WORDS <= 128 ? 3 : 2;
+    static constexpr int WARPS = 4, THREADS = 32 * WARPS, CTAS = WORDS <= (PACKED ? PL4 : 88) ? 4 : WORDS <= 128 ? 3 : 2;
 };
 
 } // namespace paged
@@ -131,7 +139,7 @@ __device__ __forceinline__ void widen_pairs(const AttentionParams& p, uint32_t a
     widen(p, __byte_perm(a, b, 0x7632), o[2], o[3]);
 }
 
-// Tokens of a sequence that are looked at: [first, n).
+// Tokens of a sequence that are looked at: [first, n).  Steps begin at a multiple of 16.
 __device__ __forceinline__ void visible(const AttentionParams& p, int64_t b, int32_t& first, int32_t& n) {
     n = (int32_t)min((int64_t)max(p.lengths[b], 0), p.tokens_in_table);
     first = p.window > 0 ? max(0, n - p.window) : 0;
@@ -141,7 +149,7 @@ template <int TOKENS>
 __device__ __forceinline__ int32_t steps_of(const AttentionParams& p, int64_t b) {
     int32_t first, n;
     visible(p, b, first, n);
-    return max(1, (n - first + TOKENS - 1) / TOKENS);
+    return max(1, (n - (first & ~15) + TOKENS - 1) / TOKENS);
 }
 
 // What beginning a head of a sequence costs, in steps: a chain of look-ups before the first step, the joining of the warps' sums behind
@@ -270,38 +278,64 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
         if (item > share.last_item || (item == share.last_item && share.to_step <= step0)) break;
         int32_t first, n;
         visible(p, b, first, n);
-        const int32_t steps = max(1, (n - first + S::TOKENS - 1) / S::TOKENS);
+        const int32_t start = first & ~15, steps = max(1, (n - start + S::TOKENS - 1) / S::TOKENS);
         const int32_t step1 = item == share.last_item ? share.to_step : steps;
         const int kvh = hh / p.tiles, q_first = (hh - kvh * p.tiles) * S::HEADS;
         const int q_count = min(S::HEADS, p.shared - q_first);
-        const char* const kbase = (const char*)p.cache.k + (int64_t)kvh * p.cache.head_stride * S::ES + t * S::KP;
-        const char* const vbase = (const char*)p.cache.v + (int64_t)kvh * p.cache.head_stride * S::ES + g * S::VP;
-        const char* const ksbase = (const char*)p.cache.k_scale + (int64_t)kvh * p.cache.scale_head_stride * 2 + (S::KIND == CACHE_I8_GROUPS ? t * S::KG * 2 : 0);
-        const char* const vsbase = (const char*)p.cache.v_scale + (int64_t)kvh * p.cache.scale_head_stride * 2 + (S::KIND == CACHE_I8_GROUPS ? g * (S::VP / S::ES) / 8 * 2 : 0);
+        const char* const kbase = (const char*)p.cache.k + (int64_t)kvh * p.cache.head_stride * S::ES + t * S::KP + (S::PACKED ? g * (S::D * S::ES) : 0);
+        const char* const vbase = (const char*)p.cache.v + (int64_t)kvh * p.cache.head_stride * S::ES + g * S::VP + (S::PACKED ? 2 * t * (S::D * S::ES) : 0);
+        // scales: of the lane's groups, or of the lane's token
+        const int64_t scale_bytes = S::KIND == CACHE_I8_ROWS && S::PACKED ? (lane & 15) * p.cache.scale_token_stride * 2 : 0;
+        const char* const ksbase = (const char*)p.cache.k_scale + (int64_t)kvh * p.cache.scale_head_stride * 2 + scale_bytes +
+                                   (S::KIND == CACHE_I8_GROUPS ? t * S::KG * 2 + (S::PACKED ? g * (S::D / 4) : 0) : 0);
+        const char* const vsbase = (const char*)p.cache.v_scale + (int64_t)kvh * p.cache.scale_head_stride * 2 + scale_bytes +
+                                   (S::KIND == CACHE_I8_GROUPS ? g * (S::VP / S::ES) / 8 * 2 + (S::PACKED ? 2 * t * (S::D / 4) : 0) : 0);
         const int32_t* const row_pages = p.pages + b * p.pages_stride;
 
         // ---- tokens on their way -----------------------------------------------------------------------------------------
-        // Lane l looks after token l of a step (of l % 16): its page, two steps ahead, then where its row lies, one step ahead.
+        // Of the step that is loaded next: which tokens there are, and where their rows lie.  Lane l looks after token l of a step (of l %
+        // 16): its page, two steps ahead, then its row, one step ahead; PACKED: all lanes look after the first of every 16.
+        constexpr uint32_t EVERY = S::SUBS == 2 ? 0xffffffffu : 0xffffu;
+        constexpr int PLACES = S::PACKED ? S::SUBS : 1;
         struct Place {
-            int32_t page;
-            uint32_t in_page;
+            int32_t page[PLACES];
+            uint32_t in_page[PLACES];
         };
+        uint32_t row[PLACES] = {}, scale_row[PLACES] = {}, coming = 0;
+        const char *k_at[PLACES], *v_at[PLACES], *ks_at[PLACES], *vs_at[PLACES]; // PACKED: the lane's first bytes of every 16 tokens
         auto find = [&](int32_t step) {
-            const int32_t token = first + step * S::TOKENS + (lane & (S::TOKENS - 1));
-            const uint32_t index = (uint32_t)((uint64_t)(uint32_t)token * p.page_magic >> p.page_shift);
             Place at;
-            at.page = step < step1 && token < n ? row_pages[index] : -1;
-            at.in_page = token - index * p.cache.page_size;
+#pragma unroll
+            for (int i = 0; i < PLACES; ++i) {
+                const int32_t token = start + step * S::TOKENS + (S::PACKED ? 16 * i : lane & (S::TOKENS - 1));
+                const uint32_t index = (uint32_t)((uint64_t)(uint32_t)token * p.page_magic >> p.page_shift);
+                at.page[i] = step < step1 && token < n && (S::PACKED || token >= first) ? row_pages[index] : -1;
+                at.in_page[i] = token - index * p.cache.page_size;
+            }
             return at;
         };
-        constexpr uint32_t EVERY = S::SUBS == 2 ? 0xffffffffu : 0xffffu;
-        uint32_t row = 0, scale_row = 0, coming = 0; // of the step that is loaded next: offsets, and which tokens there are
-        auto locate = [&](const Place& at) {
-            const bool ok = (uint32_t)at.page < (uint32_t)p.num_pages;
-            coming = __ballot_sync(0xffffffffu, ok) & EVERY;
-            row = ok ? at.page * p.page_units + at.in_page * p.token_units : 0u;
-            if constexpr (S::KIND != CACHE_F16) scale_row = ok ? at.page * p.scale_page_units + at.in_page * p.scale_token_units : 0u;
+        auto locate = [&](const Place& at, int32_t step) {
+            if constexpr (S::PACKED) coming = 0;
+#pragma unroll
+            for (int i = 0; i < PLACES; ++i) {
+                const bool ok = (uint32_t)at.page[i] < (uint32_t)p.num_pages;
+                row[i] = ok ? at.page[i] * p.page_units + at.in_page[i] * p.token_units : 0u;
+                if constexpr (S::KIND != CACHE_F16) scale_row[i] = ok ? at.page[i] * p.scale_page_units + at.in_page[i] * p.scale_token_units : 0u;
+                if constexpr (S::PACKED) {
+                    const uint64_t off = (uint64_t)row[i] * p.unit, scale_off = (uint64_t)scale_row[i] * p.scale_unit;
+                    k_at[i] = kbase + off;
+                    v_at[i] = vbase + off;
+                    ks_at[i] = ksbase + scale_off;
+                    vs_at[i] = vsbase + scale_off;
+                    const int32_t token = start + step * S::TOKENS + 16 * i; // bits of tokens from `first` and below n
+                    if (ok) coming |= ((0xffffu >> max(0, 16 - (n - token))) & (0xffffu << max(0, first - token)) & 0xffffu) << (16 * i);
+                } else {
+                    coming = __ballot_sync(0xffffffffu, ok) & EVERY;
+                }
+            }
         };
+        auto offset_of = [&](int token) { return (uint64_t)__shfl_sync(0xffffffffu, row[0], token) * p.unit; };
+        auto scale_offset_of = [&](int token) { return (uint64_t)__shfl_sync(0xffffffffu, scale_row[0], token) * p.scale_unit; };
         uint32_t kw[S::SUBS][2][S::KN][S::KP / 4] = {}, vw[S::SUBS][4][S::VN][S::VP / 4] = {};
         uint32_t ks[S::SUBS][2][S::KN] = {}, vs[S::SUBS][4][S::VN] = {}; // CACHE_I8_GROUPS
         uint32_t k_scale = 0, v_scale = 0;                               // CACHE_I8_ROWS: of the lane's token
@@ -310,9 +344,14 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     const int token = 16 * sub + g + 8 * r;
-                    const char* src = kbase + (uint64_t)__shfl_sync(0xffffffffu, row, token) * p.unit;
-                    const char* scales = ksbase;
-                    if constexpr (S::KIND == CACHE_I8_GROUPS) scales += (uint64_t)__shfl_sync(0xffffffffu, scale_row, token) * p.scale_unit;
+                    const char *src, *scales = nullptr;
+                    if constexpr (S::PACKED) {
+                        src = k_at[sub] + 8 * r * (S::D * S::ES);
+                        scales = ks_at[sub] + 8 * r * (S::D / 4);
+                    } else {
+                        src = kbase + offset_of(token);
+                        if constexpr (S::KIND == CACHE_I8_GROUPS) scales = ksbase + scale_offset_of(token);
+                    }
                     const bool there = every || (coming >> token & 1);
 #pragma unroll
                     for (int i = 0; i < S::KN; ++i) {
@@ -335,9 +374,15 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int token = 16 * sub + 2 * t + (j & 1) + 8 * (j >> 1);
-                    const char* src = vbase + (uint64_t)__shfl_sync(0xffffffffu, row, token) * p.unit;
-                    const char* scales = vsbase;
-                    if constexpr (S::KIND == CACHE_I8_GROUPS) scales += (uint64_t)__shfl_sync(0xffffffffu, scale_row, token) * p.scale_unit;
+                    const int in_lane = (j & 1) + 8 * (j >> 1); // tokens behind the lane's first
+                    const char *src, *scales = nullptr;
+                    if constexpr (S::PACKED) {
+                        src = v_at[sub] + in_lane * (S::D * S::ES);
+                        scales = vs_at[sub] + in_lane * (S::D / 4);
+                    } else {
+                        src = vbase + offset_of(token);
+                        if constexpr (S::KIND == CACHE_I8_GROUPS) scales = vsbase + scale_offset_of(token);
+                    }
                     const bool there = every || (coming >> token & 1);
 #pragma unroll
                     for (int i = 0; i < S::VN; ++i) {
@@ -357,9 +402,13 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
             else if (coming) load(false);
         };
         // CACHE_I8_ROWS: the scales of the lane's token
-        auto load_scale = [&](uint32_t& scale, const char* base) {
-            if constexpr (S::KIND == CACHE_I8_ROWS)
-                scale = (coming >> (lane & (S::TOKENS - 1)) & 1) ? load_scales<1>(base + (uint64_t)scale_row * p.scale_unit) : 0u;
+        auto load_scale = [&](uint32_t& scale, bool values) {
+            if constexpr (S::KIND == CACHE_I8_ROWS) {
+                const char* at;
+                if constexpr (S::PACKED) at = lane >= 16 ? (values ? vs_at : ks_at)[PLACES - 1] : (values ? vs_at : ks_at)[0];
+                else at = (values ? vsbase : ksbase) + (uint64_t)scale_row[0] * p.scale_unit;
+                scale = (coming >> (lane & (S::TOKENS - 1)) & 1) ? load_scales<1>(at) : 0u;
+            }
         };
 
         Place ahead = find(step0 + warp);
@@ -382,16 +431,16 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                     q[nt][i * (EP / 4) + s][1] = apart ? __byte_perm(w.x, w.y, 0x7632) : w.y;
                 }
         }
-        locate(ahead);
+        locate(ahead, step0 + warp);
         ahead = second;
         uint32_t seen = coming;
 #pragma unroll
         for (int sub = 0; sub < S::SUBS; ++sub) load_keys(sub);
-        load_scale(k_scale, ksbase);
+        load_scale(k_scale, false);
 #pragma unroll
         for (int sub = 0; sub < S::SUBS; ++sub) load_values(sub);
-        load_scale(v_scale, vsbase);
-        locate(ahead);
+        load_scale(v_scale, true);
+        locate(ahead, step0 + warp + WARPS);
         ahead = find(step0 + warp + 2 * WARPS);
 
         // CACHE_I8_ROWS: keys enter the product as (value + 128) * 2^-24, exactly; 128 * 2^-24 times the sum of a query's elements is taken
@@ -492,7 +541,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                     }
                     load_keys(sub);
                 }
-                load_scale(k_scale, ksbase);
+                load_scale(k_scale, false);
 
 
                 // ---- weights: 2^(score - top + 8) --------------------------------------------------------------------------
@@ -611,15 +660,15 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                     }
                     load_values(sub);
                 }
-                load_scale(v_scale, vsbase);
+                load_scale(v_scale, true);
             } else { // nothing of this step was there
 #pragma unroll
                 for (int sub = 0; sub < S::SUBS; ++sub) load_keys(sub), load_values(sub);
-                load_scale(k_scale, ksbase);
-                load_scale(v_scale, vsbase);
+                load_scale(k_scale, false);
+                load_scale(v_scale, true);
             }
             seen = coming;
-            locate(ahead);
+            locate(ahead, step + 2 * WARPS);
             ahead = find(step + 3 * WARPS);
         }
 
@@ -762,19 +811,21 @@ int32_t launch(cudaStream_t stream, AttentionParams& p, int64_t tokens) {
     return check_launch("paged attention");
 }
 
-template <int D>
+template <int D, int NT, bool PACKED>
 int32_t launch_kind(cudaStream_t stream, AttentionParams& p, int64_t tokens) {
-    const int kind = p.cache.quant_group == 0 ? CACHE_F16 : p.cache.quant_group == 8 ? CACHE_I8_GROUPS : CACHE_I8_ROWS;
-    if constexpr (D <= 128) {
-        if (heads_at_once(D, p.shared) == 16) {
-            if (kind == CACHE_F16) return launch<Shape<D, CACHE_F16, 2>>(stream, p, tokens);
-            if (kind == CACHE_I8_GROUPS) return launch<Shape<D, CACHE_I8_GROUPS, 2>>(stream, p, tokens);
-            return launch<Shape<D, CACHE_I8_ROWS, 2>>(stream, p, tokens);
-        }
-    }
-    if (kind == CACHE_F16) return launch<Shape<D, CACHE_F16, 1>>(stream, p, tokens);
-    if (kind == CACHE_I8_GROUPS) return launch<Shape<D, CACHE_I8_GROUPS, 1>>(stream, p, tokens);
-    return launch<Shape<D, CACHE_I8_ROWS, 1>>(stream, p, tokens);
+    if (p.cache.quant_group == 0) return launch<Shape<D, CACHE_F16, NT, PACKED>>(stream, p, tokens);
+    if (p.cache.quant_group == 8) return launch<Shape<D, CACHE_I8_GROUPS, NT, PACKED>>(stream, p, tokens);
+    return launch<Shape<D, CACHE_I8_ROWS, NT, PACKED>>(stream, p, tokens);
+}
+template <int D, bool PACKED>
+int32_t launch_heads(cudaStream_t stream, AttentionParams& p, int64_t tokens) {
+    if constexpr (D <= 128)
+        if (heads_at_once(D, p.shared) == 16) return launch_kind<D, 2, PACKED>(stream, p, tokens);
+    return launch_kind<D, 1, PACKED>(stream, p, tokens);
+}
+template <int D>
+int32_t launch_dim(cudaStream_t stream, AttentionParams& p, int64_t tokens, bool packed) {
+    return packed ? launch_heads<D, true>(stream, p, tokens) : launch_heads<D, false>(stream, p, tokens);
 }
 
 } // namespace
@@ -839,11 +890,12 @@ int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb2
     p.arrived = (uint32_t*)a->ws;
     p.tops = (float2*)((char*)a->ws + round_up(kCtas * 4, 256));
     p.sums = (float*)((char*)p.tops + round_up(2 * kCtas * heads * 8, 256));
+    const bool packed = cache->page_size % 16 == 0 && cache->token_stride == D && (cache->quant_group != 8 || cache->scale_token_stride == D / 8);
     const cudaStream_t s = (cudaStream_t)stream;
-    if (D == 64) return launch_kind<64>(s, p, p.tokens_in_table);
-    if (D == 96) return launch_kind<96>(s, p, p.tokens_in_table);
-    if (D == 128) return launch_kind<128>(s, p, p.tokens_in_table);
-    return launch_kind<256>(s, p, p.tokens_in_table);
+    if (D == 64) return launch_dim<64>(s, p, p.tokens_in_table, packed);
+    if (D == 96) return launch_dim<96>(s, p, p.tokens_in_table, packed);
+    if (D == 128) return launch_dim<128>(s, p, p.tokens_in_table, packed);
+    return launch_dim<256>(s, p, p.tokens_in_table, packed);
 }
 
 } // extern "C"
