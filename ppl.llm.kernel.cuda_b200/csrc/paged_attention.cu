@@ -11,6 +11,7 @@
 #include "kv_cache.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 namespace pplb200 {
@@ -30,13 +31,7 @@ struct Shape {
     static constexpr int ES = KIND == CACHE_F16 ? 2 : 1;
     // Tokens of a step: 32 where that leaves room for twelve warps on an SM (64 x 8192, int8 rows: 123 us with 32, 129 with 16; groups,
     // whose scales take registers too: 16 x 4096 71 us with 32, 67 with 16).
-#ifndef PSUB
-#define PSUB 2
-#endif
-#ifndef PL4
-#define PL4 88
-#endif
-    static constexpr int SUBS = D * ES <= 64 ? 2 : D * ES <= 128 && KIND == CACHE_I8_ROWS ? (PACKED ? PSUB : 2) : 1, TOKENS = 16 * SUBS;
+    static constexpr int SUBS = D * ES <= 64 || (D * ES <= 128 && KIND == CACHE_I8_ROWS) ? 2 : 1, TOKENS = 16 * SUBS;
     // of 16 tokens a quad's lane holds a quarter of the dimensions of two keys, an eighth of those of four values
     static constexpr int KB = D * ES / 4, KP = piece(KB), KN = KB / KP;
     static constexpr int VB = D * ES / 8, VP = piece(VB), VN = VB / VP;
@@ -45,7 +40,7 @@ struct Shape {
     // Registers for the sums, the queries and the tokens on their way decide how many CTAs share an SM.
     static constexpr int WORDS = NT * D / 4 + NT * D / 8 + SUBS * (D * ES / 4 + (KIND == CACHE_I8_GROUPS ? 2 * KN + 4 * VN : 0));
     static constexpr int ROW = D + 4; // of the sums that the warps exchange
-    static constexpr int WARPS = 4, THREADS = 32 * WARPS, CTAS = WORDS <= (PACKED ? PL4 : 88) ? 4 : WORDS <= 128 ? 3 : 2;
+    static constexpr int WARPS = 4, THREADS = 32 * WARPS, CTAS = WORDS <= 88 ? 4 : WORDS <= 128 ? 3 : 2;
 };
 
 } // namespace paged
@@ -71,7 +66,8 @@ struct AttentionParams {
     // what spread() flips: in registers, since an instruction holds one constant
     uint32_t flip, flip_1024;
     // workspace
-    uint32_t* arrived; // [CTAs]: pieces of the item that the CTA began; zero between calls
+    uint64_t call;     // number of the call, counted by the process
+    uint64_t* arrived; // [CTAs]: pieces of the item that the CTA began
     float2* tops;      // [2 * CTAs][HEADS]: reference exponent and sum of weights
     float* sums;       // [2 * CTAs][HEADS][D]
 };
@@ -302,7 +298,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
             uint32_t in_page[PLACES];
         };
         uint32_t row[PLACES] = {}, scale_row[PLACES] = {}, coming = 0;
-        const char *k_at[PLACES], *v_at[PLACES], *ks_at[PLACES], *vs_at[PLACES]; // PACKED: the lane's first bytes of every 16 tokens
+        uint64_t off[PLACES], scale_off[PLACES]; // PACKED: of every 16 tokens, in bytes
         auto find = [&](int32_t step) {
             Place at;
 #pragma unroll
@@ -322,11 +318,8 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                 row[i] = ok ? at.page[i] * p.page_units + at.in_page[i] * p.token_units : 0u;
                 if constexpr (S::KIND != CACHE_F16) scale_row[i] = ok ? at.page[i] * p.scale_page_units + at.in_page[i] * p.scale_token_units : 0u;
                 if constexpr (S::PACKED) {
-                    const uint64_t off = (uint64_t)row[i] * p.unit, scale_off = (uint64_t)scale_row[i] * p.scale_unit;
-                    k_at[i] = kbase + off;
-                    v_at[i] = vbase + off;
-                    ks_at[i] = ksbase + scale_off;
-                    vs_at[i] = vsbase + scale_off;
+                    off[i] = (uint64_t)row[i] * p.unit;
+                    scale_off[i] = (uint64_t)scale_row[i] * p.scale_unit;
                     const int32_t token = start + step * S::TOKENS + 16 * i; // bits of tokens from `first` and below n
                     if (ok) coming |= ((0xffffu >> max(0, 16 - (n - token))) & (0xffffu << max(0, first - token)) & 0xffffu) << (16 * i);
                 } else {
@@ -346,8 +339,8 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                     const int token = 16 * sub + g + 8 * r;
                     const char *src, *scales = nullptr;
                     if constexpr (S::PACKED) {
-                        src = k_at[sub] + 8 * r * (S::D * S::ES);
-                        scales = ks_at[sub] + 8 * r * (S::D / 4);
+                        src = kbase + off[sub] + 8 * r * (S::D * S::ES);
+                        scales = ksbase + scale_off[sub] + 8 * r * (S::D / 4);
                     } else {
                         src = kbase + offset_of(token);
                         if constexpr (S::KIND == CACHE_I8_GROUPS) scales = ksbase + scale_offset_of(token);
@@ -377,8 +370,8 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                     const int in_lane = (j & 1) + 8 * (j >> 1); // tokens behind the lane's first
                     const char *src, *scales = nullptr;
                     if constexpr (S::PACKED) {
-                        src = v_at[sub] + in_lane * (S::D * S::ES);
-                        scales = vs_at[sub] + in_lane * (S::D / 4);
+                        src = vbase + off[sub] + in_lane * (S::D * S::ES);
+                        scales = vsbase + scale_off[sub] + in_lane * (S::D / 4);
                     } else {
                         src = vbase + offset_of(token);
                         if constexpr (S::KIND == CACHE_I8_GROUPS) scales = vsbase + scale_offset_of(token);
@@ -404,9 +397,9 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
         // CACHE_I8_ROWS: the scales of the lane's token
         auto load_scale = [&](uint32_t& scale, bool values) {
             if constexpr (S::KIND == CACHE_I8_ROWS) {
-                const char* at;
-                if constexpr (S::PACKED) at = lane >= 16 ? (values ? vs_at : ks_at)[PLACES - 1] : (values ? vs_at : ks_at)[0];
-                else at = (values ? vsbase : ksbase) + (uint64_t)scale_row[0] * p.scale_unit;
+                const char* at = values ? vsbase : ksbase;
+                if constexpr (S::PACKED) at += lane >= 16 ? scale_off[PLACES - 1] : scale_off[0];
+                else at += (uint64_t)scale_row[0] * p.scale_unit;
                 scale = (coming >> (lane & (S::TOKENS - 1)) & 1) ? load_scales<1>(at) : 0u;
             }
         };
@@ -445,7 +438,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
 
         // CACHE_I8_ROWS: keys enter the product as (value + 128) * 2^-24, exactly; 128 * 2^-24 times the sum of a query's elements is taken
         // off its scores, here for the lane's two heads.
-        float off[S::NT][2] = {};
+        float bias[S::NT][2] = {};
         if constexpr (S::KIND == CACHE_I8_ROWS) {
 #pragma unroll
             for (int nt = 0; nt < S::NT; ++nt) {
@@ -459,8 +452,8 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                     }
                 all_dims += __shfl_xor_sync(0xffffffffu, all_dims, 1);
                 all_dims += __shfl_xor_sync(0xffffffffu, all_dims, 2);
-                off[nt][0] = __shfl_sync(0xffffffffu, all_dims, 8 * t) * 0x1p-17f;
-                off[nt][1] = __shfl_sync(0xffffffffu, all_dims, 8 * t + 4) * 0x1p-17f;
+                bias[nt][0] = __shfl_sync(0xffffffffu, all_dims, 8 * t) * 0x1p-17f;
+                bias[nt][1] = __shfl_sync(0xffffffffu, all_dims, 8 * t + 4) * 0x1p-17f;
             }
         }
 
@@ -531,7 +524,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
 #pragma unroll
                             for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
-                                for (int x = 0; x < 4; ++x) c[sub][nt][x] = (c[sub][nt][x] - off[nt][x & 1]) * (x < 2 ? k0 : k1);
+                                for (int x = 0; x < 4; ++x) c[sub][nt][x] = (c[sub][nt][x] - bias[nt][x & 1]) * (x < 2 ? k0 : k1);
                         } else {
 #pragma unroll
                             for (int nt = 0; nt < S::NT; ++nt)
@@ -725,15 +718,20 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
             const int64_t end = begin + steps;
             const int32_t c0 = (int32_t)(((begin + 1) * ctas + all - 1) / all), c1 = (int32_t)((end * ctas + all - 1) / all);
             const int32_t pieces = c1 - c0 + 1; // the first is the one of CTA c0 - 1, which began the item
-            __threadfence();
+            // The barrier puts the other threads' sums ahead of this thread's release, and its acquire ahead of their reads.  A counter is
+            // the call's number above 16 bits of arrivals, none between calls; the maximum throws out what calls that ran at the same time
+            // on this workspace, against the rules, have left.
             __syncthreads();
             if (threadIdx.x == 0) {
-                is_last = atomicAdd(&p.arrived[c0 - 1], 1u) == (uint32_t)(pieces - 1);
-                if (is_last) p.arrived[c0 - 1] = 0; // for the next call
+                uint64_t before;
+                uint64_t* const counter = p.arrived + (c0 - 1);
+                asm volatile("red.relaxed.gpu.global.max.u64 [%0], %1;" ::"l"(counter), "l"(p.call << 16) : "memory");
+                asm volatile("atom.add.acq_rel.gpu.global.u64 %0, [%1], 1;" : "=l"(before) : "l"(counter) : "memory");
+                is_last = (before & 0xffffu) == (uint32_t)(pieces - 1);
+                if (is_last) *counter = before & ~0xffffull;
             }
             __syncthreads();
             if (is_last) {
-                __threadfence();
                 // 16 loads a thread at once: ITEMS places of the output times BATCH pieces
                 constexpr int ITEMS = (S::HEADS * S::D / 4 + S::THREADS - 1) / S::THREADS, BATCH = ITEMS >= 4 ? 4 : 16 / ITEMS;
                 float4 v[ITEMS];
@@ -839,7 +837,7 @@ int64_t pplb200_paged_decode_attention_workspace_bytes(int64_t batch, int64_t ma
     if (batch < 0 || max_tokens < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0) return -1;
     // a counter and two pieces a CTA at most
     const int heads = heads_at_once(head_dim, q_heads / kv_heads);
-    return round_up(kCtas * 4, 256) + round_up(2 * kCtas * heads * 8, 256) + 2LL * kCtas * heads * head_dim * 4;
+    return round_up(kCtas * 8, 256) + round_up(2 * kCtas * heads * 8, 256) + 2LL * kCtas * heads * head_dim * 4;
 }
 
 int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_paged_attention_args* a) {
@@ -887,8 +885,10 @@ int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb2
     p.cache = *cache;
     p.flip = 0x00800080u;
     p.flip_1024 = 0x64806480u;
-    p.arrived = (uint32_t*)a->ws;
-    p.tops = (float2*)((char*)a->ws + round_up(kCtas * 4, 256));
+    static std::atomic<uint64_t> calls{0};
+    p.call = ++calls;
+    p.arrived = (uint64_t*)a->ws;
+    p.tops = (float2*)((char*)a->ws + round_up(kCtas * 8, 256));
     p.sums = (float*)((char*)p.tops + round_up(2 * kCtas * heads * 8, 256));
     const bool packed = cache->page_size % 16 == 0 && cache->token_stride == D && (cache->quant_group != 8 || cache->scale_token_stride == D / 8);
     const cudaStream_t s = (cudaStream_t)stream;

@@ -73,6 +73,12 @@ def _here():
     return _here()
 
 
+def _settle(device):
+    """What an object has just laid out on the device is there before the object is: its calls may come on any stream."""
+    if device.type == "cuda":
+        torch.cuda.current_stream(device).synchronize()
+
+
 class RotaryTable:
     """Frequencies of the rotated planes, laid out once on `device`.  scaling: "none", "linear", "ntk", "yarn" or "wavelength"."""
 
@@ -85,6 +91,7 @@ class RotaryTable:
         self.rotary_dim, self.magnitude = rotary_dim, magnitude.value
         self.turns = torch.frombuffer(words, dtype=_I64).to(device, copy=True)
         self.device_index, self.address = self.turns.get_device(), self.turns.data_ptr()
+        _settle(self.turns.device)
 
 
 def rotary_fp16(q, k, positions, table, interleaved=False, q_out=None, k_out=None):
@@ -226,6 +233,7 @@ class PagedDecodeAttention:
         need = lib.pplb200_paged_decode_attention_workspace_bytes(max_batch, self.max_pages * cache.page_size, q_heads, cache.kv_heads, cache.head_dim)
         self.ws = torch.zeros((need,), dtype=torch.uint8, device=cache.k.device)
         self._ws, self._ws_bytes = self.ws.data_ptr(), need
+        _settle(cache.k.device)
 
     def __call__(self, q, pages, lengths, out=None, lse=None):
         """q fp16 [batch, q_heads, head_dim], pages int32 [batch, pages a sequence] (negative: a hole), lengths int32 [batch] -> out as q;

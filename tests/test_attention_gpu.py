@@ -369,9 +369,10 @@ def test_attention_all_empty(cuda, pplb200):
 
 
 @pytest.mark.parametrize("window", [1, 2, 16, 100, 129, 100000])
-@pytest.mark.parametrize("group", [0, 128])
-def test_attention_window(cuda, pplb200, window, group):
-    _check_attention(*_run_attention(cuda, pplb200, [1, 2, 15, 100, 101, 700, 0, 3001], 8, 2, 128, 24, group, window=window)[:3])
+@pytest.mark.parametrize("group", [0, 8, 128])
+@pytest.mark.parametrize("page", [16, 24])
+def test_attention_window(cuda, pplb200, window, group, page):
+    _check_attention(*_run_attention(cuda, pplb200, [1, 2, 15, 100, 101, 700, 0, 3001], 8, 2, 128, page, group, window=window)[:3])
 
 
 @pytest.mark.parametrize("group", [0, 8, 128])
@@ -475,9 +476,79 @@ def test_attention_fewer_sequences_leave_the_rest_alone(cuda, pplb200):
 def test_attention_is_the_same_run_after_run(cuda, pplb200, group):
     out, lse, _, (att, q, table, lens, cache) = _run_attention(cuda, pplb200, [9000, 3, 500, 1234], 16, 2, 128, 16, group)
     for fill in (0, 255, 127):
-        att.ws[4096:].fill_(fill)  # whatever an earlier call's sums were
+        att.ws[8192:].fill_(fill)  # whatever an earlier call's sums were; the counters of arrivals lie in front of them
         again = cuda.empty_like(lse)
         assert cuda.equal(att(q, table, lens, lse=again), out) and cuda.equal(again, lse)
+
+
+def test_attention_recovers_from_counters_that_were_left(cuda, pplb200):
+    """Calls that overlapped on one workspace, against the rules, may leave counters of arrivals behind: the next call is right again."""
+    out, _, _, (att, q, table, lens, cache) = _run_attention(cuda, pplb200, [9000, 3, 500, 1234], 16, 2, 128, 16, 128)
+    for left in (1, 5, (1 << 16) + 3):
+        att.ws[:592 * 8].view(cuda.int64).fill_(left)
+        assert cuda.equal(att(q, table, lens), out)
+
+
+@pytest.mark.parametrize("group", [0, 8, 128])
+def test_attention_shared_pages(cuda, pplb200, group):
+    """Sequences that share the pages of a common beginning, and one in which a page stands twice."""
+    out, _, _, (att, q, table, lens, cache) = _run_attention(cuda, pplb200, [64, 64, 64], 8, 2, 128, 16, group)
+    table[1, :2], table[2, 1] = table[0, :2], table[2, 0]
+    got = att(q, table, lens)
+    at = cuda.arange(64, device="cuda")
+    for b in range(3):
+        k, v = _stored(cuda, cache, table[b].long()[at // 16] * 16 + at % 16)
+        _check_attention(got[b:b + 1], None, [_attention(cuda, q[b], k, v, at >= 0, att.scale, group == 8)])
+
+
+@pytest.mark.parametrize("group,d,pages", [(0, 128, 36000), (8, 128, 70000), (128, 128, 70000)])
+@pytest.mark.parametrize("order", ["heads", "tokens"])
+def test_offsets_beyond_32_bits(cuda, pplb200, group, d, pages, order):
+    """Keys and values of more than 2^32 bytes each: the last pages are written, read back and attended to."""
+    page, heads, n = 64, 8, 200
+    shape = (pages, heads, page) if order == "heads" else (pages, page, heads)
+    make = lambda w, t: cuda.empty(shape + (w,), dtype=t, device="cuda")  # noqa: E731
+    tensors = [make(d, cuda.int8 if group else cuda.float16) for _ in range(2)] + ([make(d // group, cuda.float16) for _ in range(2)] if group else [])
+    assert tensors[0].numel() * tensors[0].element_size() > 1 << 32
+    cache = pplb200.PagedKVCache(*(t if order == "heads" else t.transpose(1, 2) for t in tensors))
+    g = _gen(cuda, 4)
+    table = cuda.tensor([[pages - 1, 0, pages - 2, pages // 2]], dtype=cuda.int32, device="cuda")
+    at = cuda.arange(n, device="cuda")
+    slots = table[0].long()[at // page] * page + at % page
+    k, v = _randn(cuda, g, n, heads, d), _randn(cuda, g, n, heads, d)
+    pplb200.kv_cache_write(cache, k, v, slots)
+    for x, back in zip((k, v), pplb200.kv_cache_read(cache, slots)):
+        if group:
+            q, s = _quantized(x.cpu().numpy(), group)
+            x = cuda.from_numpy((q.astype(np.float64) * np.repeat(s.astype(np.float64), group, -1)).astype(np.float16)).cuda()
+        assert cuda.equal(back, x)
+    q = _randn(cuda, g, 1, 16, d)
+    att = pplb200.PagedDecodeAttention(cache, 16, 1, 4 * page)
+    out = att(q, table, cuda.tensor([n], dtype=cuda.int32, device="cuda"))
+    _check_attention(out, None, [_attention(cuda, q[0], *_stored(cuda, cache, slots), at >= 0, att.scale, group == 8)])
+
+
+def test_two_streams_at_once(cuda, pplb200):
+    """Two objects on the same cache, each on its own stream, and rotations and stores beside them: no call disturbs another."""
+    out, _, _, (att, q, table, lens, cache) = _run_attention(cuda, pplb200, [5000, 17, 900], 16, 2, 128, 16, 8, lse=False)
+    other = pplb200.PagedDecodeAttention(cache, 16, 3, 5008)
+    mine = pplb200.PagedKVCache.allocate(40, 16, 2, 128, 128)
+    g = _gen(cuda, 12)
+    k, v, pos, turns = _randn(cuda, g, 600, 2, 128), _randn(cuda, g, 600, 2, 128), cuda.arange(600, device="cuda"), pplb200.RotaryTable(128)
+    plain = pplb200.PagedKVCache.allocate(40, 16, 2, 128, 128)
+    pplb200.rotary_kv_cache_write(plain, None, k, v, pos, pos, turns)
+    cuda.cuda.synchronize()
+    streams = [cuda.cuda.Stream() for _ in range(3)]
+    results = []
+    for _ in range(20):
+        for s, a in zip(streams, (att, other)):
+            with cuda.cuda.stream(s):
+                results.append(a(q, table, lens))
+        with cuda.cuda.stream(streams[2]):
+            pplb200.rotary_kv_cache_write(mine, None, k, v, pos, pos, turns)
+    cuda.cuda.synchronize()
+    assert all(cuda.equal(r, out) for r in results)
+    assert cuda.equal(mine.k, plain.k) and cuda.equal(mine.v_scale, plain.v_scale)
 
 
 def test_attention_parts_join_by_their_lse(cuda, pplb200):
