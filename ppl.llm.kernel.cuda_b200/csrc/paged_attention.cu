@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                 float v0[S::SUBS], v1[S::SUBS], e0[S::SUBS] = {}, e1[S::SUBS] = {};
                 if constexpr (S::KIND == CACHE_I8_ROWS) {
                     // a value's scale goes into its weight, the scale's logarithm into what decides about the reference exponent
-                    const float mine = __half2float(__ushort_as_half((unsigned short)v_scale)), size = fmaxf(log2_fast(mine), -24.0f);
+                    const float mine = __half2float(__ushort_as_half((unsigned short)v_scale)), size = fmaxf(log2_fast(fabsf(mine)), -24.0f);
 #pragma unroll
                     for (int sub = 0; sub < S::SUBS; ++sub) {
                         v0[sub] = __shfl_sync(0xffffffffu, mine, 16 * sub + g);
@@ -850,7 +850,8 @@ int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb2
     if (a->batch > 65535) return fail(RC_UNSUPPORTED, "more than 65535 sequences");
     if (a->q_heads <= 0 || a->q_heads > 65535 || a->q_heads % cache->kv_heads)
         return fail(RC_INVALID_VALUE, "q_heads (%d) must be a multiple of the cache's heads (%d)", a->q_heads, cache->kv_heads);
-    if (!std::isfinite(a->scale)) return fail(RC_INVALID_VALUE, "the scale must be finite");
+    // up to here no score is as low as -1e30, the reference exponent of a sequence before its first token
+    if (!(std::fabs(a->scale) <= 0x1p50f)) return fail(RC_INVALID_VALUE, "the scale must be within 2^50 of zero");
     if (a->batch == 0) return RC_SUCCESS;
     if (!a->q || !a->out || !aligned16(a->q) || !aligned16(a->out)) return fail(RC_INVALID_VALUE, "q and out must be 16-byte aligned pointers");
     if (a->q_stride % 8 || a->out_stride % 8 || (a->batch > 1 && (a->q_stride < a->q_heads * D || a->out_stride < a->q_heads * D)))

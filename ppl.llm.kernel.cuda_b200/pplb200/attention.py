@@ -98,6 +98,8 @@ def rotary_fp16(q, k, positions, table, interleaved=False, q_out=None, k_out=Non
     """q [tokens, q_heads, head_dim], k [tokens, k_heads, head_dim] fp16 (either may be None) -> both rotated by `positions` (int64
     [tokens]).  q_out=q and k_out=k rotate in place."""
     dev, stream = _here()
+    if q is None and k is None:
+        raise ValueError("neither q nor k is given")
     tokens, _, head_dim = (k if q is None else q).shape
     qp = qo = qh = qs = qos = kp = ko = kh = ks = kos = 0
     if q is not None:
@@ -195,6 +197,8 @@ def kv_cache_write(cache, k, v, slots):
 
 def rotary_kv_cache_write(cache, q, k, v, positions, slots, table, interleaved=False, q_out=None):
     """rotary_fp16 of q and k and kv_cache_write of the rotated k and of v, in one pass.  Returns the rotated q."""
+    if table is None:
+        raise ValueError("a rotary table is needed")
     if q is not None and q_out is None:
         q_out = torch.empty(q.shape, dtype=torch.float16, device=q.device)
     _store(cache, q, k, v, positions, slots, table, interleaved, q_out)

@@ -198,7 +198,7 @@ def test_read_refusals():
 
 @pytest.mark.parametrize("bad,rc", [
     (dict(batch=-1), 4), (dict(batch=70000), 2), (dict(width=-1), 4), (dict(width=1 << 40, pages_stride=1 << 40), 2), (dict(q_heads=0), 4), (dict(q_heads=12), 4), (dict(q_heads=-8), 4), (dict(scale=float("nan")), 4),
-    (dict(scale=float("inf")), 4), (dict(q=0), 4), (dict(out=0), 4), (dict(q=AT + 8), 4), (dict(out=AT + 2), 4), (dict(q_stride=1020), 4), (dict(q_stride=512), 4),
+    (dict(scale=float("inf")), 4), (dict(scale=1.2e15), 4), (dict(scale=-2.0 ** 51), 4), (dict(q=0), 4), (dict(out=0), 4), (dict(q=AT + 8), 4), (dict(out=AT + 2), 4), (dict(q_stride=1020), 4), (dict(q_stride=512), 4),
     (dict(out_stride=1016), 4), (dict(pages=0), 4), (dict(lengths=0), 4), (dict(pages=AT + 2), 4), (dict(lengths=AT + 1), 4), (dict(lse=AT + 2), 4), (dict(pages_stride=9), 4),
     (dict(ws=0), 4), (dict(ws=AT + 16), 4), (dict(ws_bytes=16), 4)])
 def test_attention_refusals(bad, rc):
@@ -283,6 +283,7 @@ def test_binding_refuses_other_types_shapes_and_devices(here, monkeypatch):
             lambda: pplb200.rotary_fp16(z(4, 8, 64), None, z(3, t=i64), table), lambda: pplb200.rotary_fp16(z(4, 8, 64), None, z(4, t=i32), table),
             lambda: pplb200.rotary_fp16(z(4, 8, 128)[..., ::2], None, pos, table), lambda: pplb200.rotary_fp16(z(4, 16, 64)[:, ::2], None, pos, table),
             lambda: pplb200.rotary_fp16(z(4, 8, 64), None, pos, table, q_out=z(4, 7, 64)), lambda: pplb200.rotary_fp16(z(4, 512), None, pos, table),
+            lambda: pplb200.rotary_fp16(None, None, pos, table), lambda: pplb200.rotary_kv_cache_write(cache, z(4, 8, 64), kv, kv, pos, pos, None),
             lambda: pplb200.kv_cache_write(cache, z(4, 3, 64), kv, pos), lambda: pplb200.kv_cache_write(cache, kv, z(4, 2, 32), pos),
             lambda: pplb200.kv_cache_write(cache, kv, kv, z(8, t=i64)[::2]), lambda: pplb200.kv_cache_write(cache, kv, kv.float(), pos),
             lambda: pplb200.rotary_kv_cache_write(cache, z(4, 8, 64), kv, kv, pos, pos, table, q_out=z(4, 6, 64)),

@@ -425,6 +425,41 @@ def test_attention_values_of_all_sizes(cuda, pplb200):
         _check_attention(out, None, [_attention(cuda, q[0], k, v, cuda.ones(300, dtype=cuda.bool, device="cuda"), att.scale)])
 
 
+@pytest.mark.parametrize("group", [0, 8, 128])
+@pytest.mark.parametrize("scale", [2.0 ** 50, -(2.0 ** 50)])
+def test_attention_scores_at_the_largest_scale(cuda, pplb200, group, scale):
+    """Scores of 1e20: one token has all the weight, and the reference exponent follows it far from where it begins."""
+    d, n = 128, 300
+    cache = _cache(cuda, pplb200, 20, 16, 1, d, group, "heads", 0)
+    k = ((cuda.randperm(n, generator=_gen(cuda, 3), device="cuda") - 150.5) * 2).to(cuda.float16)[:, None, None].expand(n, 1, d).contiguous()
+    pplb200.kv_cache_write(cache, k, _randn(cuda, _gen(cuda, 4), n, 1, d), cuda.arange(n, device="cuda"))
+    kr, vr = _stored(cuda, cache, cuda.arange(n, device="cuda"))
+    q = cuda.tensor([500.0, -500.0, 0.001], device="cuda").to(cuda.float16)[None, :, None].expand(1, 3, d).contiguous()
+    att = pplb200.PagedDecodeAttention(cache, 3, 1, 320, scale=scale)
+    out = att(q, cuda.arange(20, dtype=cuda.int32, device="cuda")[None], cuda.tensor([n], dtype=cuda.int32, device="cuda"))
+    # neighbouring keys are 1 / 300 of the largest apart, 2^14 roundings to 32 bits: the same token wins.  Its value is rounded when it is
+    # read with groups of 8, and rounded on output; the weights' sum is a power of two, and the quotient off by 2^-20 at most.
+    score = cuda.einsum("hd,td->ht", q[0].double(), kr[:, 0]) * scale
+    want = vr[score.argmax(-1), 0]
+    assert bool(((out[0].double() - want).abs() <= want.abs() * (2 * HALF + 2.0 ** -20) + 2 * TINY).all())
+
+
+@pytest.mark.parametrize("group", [8, 128])
+def test_attention_scales_of_either_sign(cuda, pplb200, group):
+    """Scales that another program stored may be negative."""
+    n, d = 300, 128
+    cache = _cache(cuda, pplb200, 20, 16, 1, d, group, "heads", 0)
+    g = _gen(cuda, 5)
+    pplb200.kv_cache_write(cache, _randn(cuda, g, n, 1, d), _randn(cuda, g, n, 1, d, scale=1000.0), cuda.arange(n, device="cuda"))
+    for t in (cache.k_scale, cache.v_scale):
+        t.mul_((cuda.rand(t.shape, generator=g, device="cuda") < 0.5) * 2 - 1)
+    q = _randn(cuda, g, 1, 4, d)
+    att = pplb200.PagedDecodeAttention(cache, 4, 1, 320)
+    out = att(q, cuda.arange(20, dtype=cuda.int32, device="cuda")[None], cuda.tensor([n], dtype=cuda.int32, device="cuda"))
+    kr, vr = _stored(cuda, cache, cuda.arange(n, device="cuda"))
+    _check_attention(out, None, [_attention(cuda, q[0], kr, vr, cuda.ones(n, dtype=cuda.bool, device="cuda"), att.scale, group == 8)])
+
+
 def test_attention_lengths_beyond_the_table_and_negative(cuda, pplb200):
     """No more is looked at than the table has pages for; a negative length is an empty sequence."""
     out, lse, want, (att, q, table, lens, cache) = _run_attention(cuda, pplb200, [64, 64, 33], 8, 2, 128, 16, 0)
