@@ -67,7 +67,7 @@ struct AttentionParams {
     uint32_t flip, flip_1024;
     // workspace
     uint64_t call;     // number of the call, counted by the process
-    uint64_t* arrived; // [CTAs]: pieces of the item that the CTA began
+    uint64_t* arrived; // [CTAs]: pieces, or groups of them, of the item that the CTA began; then [2 * CTAs]: pieces of a group
     float2* tops;      // [2 * CTAs][HEADS]: reference exponent and sum of weights
     float* sums;       // [2 * CTAs][HEADS][D]
 };
@@ -716,48 +716,53 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
             const int64_t all = share.all, ctas = share.ctas;
             const int64_t begin = step1 < steps ? (int64_t)(blockIdx.x + 1) * all / ctas - step1 : (int64_t)blockIdx.x * all / ctas - step0;
             const int64_t end = begin + steps;
-            const int32_t c0 = (int32_t)(((begin + 1) * ctas + all - 1) / all), c1 = (int32_t)((end * ctas + all - 1) / all);
-            const int32_t pieces = c1 - c0 + 1; // the first is the one of CTA c0 - 1, which began the item
+            const int32_t c0 = (int32_t)(((begin + 1) * ctas + all - 1) / all) - 1; // began the item
+            const int32_t pieces = (int32_t)((end * ctas + all - 1) / all) - c0;
             // The barrier puts the other threads' sums ahead of this thread's release, and its acquire ahead of their reads.  A counter is
             // the call's number above 16 bits of arrivals, none between calls; the maximum throws out what calls that ran at the same time
             // on this workspace, against the rules, have left.
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                uint64_t before;
-                uint64_t* const counter = p.arrived + (c0 - 1);
-                asm volatile("red.relaxed.gpu.global.max.u64 [%0], %1;" ::"l"(counter), "l"(p.call << 16) : "memory");
-                asm volatile("atom.add.acq_rel.gpu.global.u64 %0, [%1], 1;" : "=l"(before) : "l"(counter) : "memory");
-                is_last = (before & 0xffffu) == (uint32_t)(pieces - 1);
-                if (is_last) *counter = before & ~0xffffull;
+            auto last_of = [&](uint64_t* counter, int32_t number) {
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    uint64_t before;
+                    asm volatile("red.relaxed.gpu.global.max.u64 [%0], %1;" ::"l"(counter), "l"(p.call << 16) : "memory");
+                    asm volatile("atom.add.acq_rel.gpu.global.u64 %0, [%1], 1;" : "=l"(before) : "l"(counter) : "memory");
+                    is_last = (before & 0xffffu) == (uint32_t)(number - 1);
+                    if (is_last) *counter = before & ~0xffffull;
+                }
+                __syncthreads();
+                return is_last;
+            };
+            auto slot_of = [&](int32_t piece) { return 2 * (int64_t)(c0 + piece) + (piece == 0 ? 1 : 0); };
+            // 16 loads a thread at once: ITEMS places of the output times BATCH pieces
+            constexpr int ITEMS = (S::HEADS * S::D / 4 + S::THREADS - 1) / S::THREADS, BATCH = ITEMS >= 4 ? 4 : 16 / ITEMS;
+            float4 v[ITEMS];
+            float m[ITEMS], l[ITEMS];
+            int h[ITEMS], d[ITEMS];
+#pragma unroll
+            for (int x = 0; x < ITEMS; ++x) {
+                const int at = min((int)threadIdx.x + x * S::THREADS, q_count * (S::D / 4) - 1); // some do the last one again
+                h[x] = at / (S::D / 4);
+                d[x] = (at - h[x] * (S::D / 4)) * 4;
             }
-            __syncthreads();
-            if (is_last) {
-                // 16 loads a thread at once: ITEMS places of the output times BATCH pieces
-                constexpr int ITEMS = (S::HEADS * S::D / 4 + S::THREADS - 1) / S::THREADS, BATCH = ITEMS >= 4 ? 4 : 16 / ITEMS;
-                float4 v[ITEMS];
-                float m[ITEMS], l[ITEMS];
-                int h[ITEMS], d[ITEMS];
+            auto join = [&](int32_t piece, int32_t number, int32_t apart) {
 #pragma unroll
                 for (int x = 0; x < ITEMS; ++x) {
-                    const int at = min((int)threadIdx.x + x * S::THREADS, q_count * (S::D / 4) - 1); // some do the last one again
-                    h[x] = at / (S::D / 4);
-                    d[x] = (at - h[x] * (S::D / 4)) * 4;
                     v[x] = make_float4(0, 0, 0, 0);
                     m[x] = -1e30f;
                     l[x] = 0.0f;
                 }
-                for (int32_t i = 0; i < pieces; i += BATCH) {
+                for (int32_t i = 0; i < number; i += BATCH) {
                     float2 s[BATCH][ITEMS];
                     float4 a[BATCH][ITEMS];
 #pragma unroll
                     for (int j = 0; j < BATCH; ++j) {
-                        const int32_t n = min(i + j, pieces - 1);
-                        const int64_t slot = (n == 0 ? 2 * (int64_t)(c0 - 1) + 1 : 2 * (int64_t)(c0 - 1 + n)) * S::HEADS;
+                        const int64_t slot = slot_of(piece + min(i + j, number - 1) * apart) * S::HEADS;
 #pragma unroll
                         for (int x = 0; x < ITEMS; ++x) {
                             s[j][x] = __ldcg(&p.tops[slot + h[x]]);
                             a[j][x] = __ldcg(reinterpret_cast<const float4*>(p.sums + (slot + h[x]) * S::D + d[x]));
-                            if (i + j >= pieces) s[j][x].x = -INFINITY; // the last piece once more, without weight
+                            if (i + j >= number) s[j][x].x = -INFINITY; // the last piece once more, without weight
                         }
                     }
 #pragma unroll
@@ -771,13 +776,37 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                         v[x].x *= keep; v[x].y *= keep; v[x].z *= keep; v[x].w *= keep;
 #pragma unroll
                         for (int j = 0; j < BATCH; ++j)
-                            if (i + j < pieces) {
+                            if (i + j < number) {
                                 const float f = exp2_fast(s[j][x].x - up);
                                 l[x] += f * s[j][x].y;
                                 v[x].x += f * a[j][x].x; v[x].y += f * a[j][x].y; v[x].z += f * a[j][x].z; v[x].w += f * a[j][x].w;
                             }
                     }
                 }
+            };
+            // Many pieces are joined in groups, whose sums take the place of their first piece's, and then the groups: one CTA alone reads
+            // its 4 kB a piece at 100 GB/s.
+            const int32_t first_of_mine = (int32_t)blockIdx.x - c0;
+            int32_t per_group = 1;
+            bool ends = true;
+            if (pieces > 2 * BATCH) {
+                for (per_group = BATCH; per_group * per_group < pieces;) per_group += BATCH;
+                const int32_t piece = first_of_mine / per_group * per_group, number = min(per_group, pieces - piece);
+                const int64_t at = slot_of(piece);
+                ends = last_of(p.arrived + kCtas + at, number);
+                if (ends) {
+                    join(piece, number, 1);
+                    __syncthreads(); // all have read what is now replaced
+#pragma unroll
+                    for (int x = 0; x < ITEMS; ++x) {
+                        __stcg(reinterpret_cast<float4*>(p.sums + (at * S::HEADS + h[x]) * S::D + d[x]), v[x]);
+                        if (d[x] == 0) __stcg(&p.tops[at * S::HEADS + h[x]], make_float2(m[x], l[x]));
+                    }
+                }
+            }
+            const int32_t groups = (pieces + per_group - 1) / per_group;
+            if (ends && last_of(p.arrived + c0, groups)) {
+                join(0, groups, per_group);
 #pragma unroll
                 for (int x = 0; x < ITEMS; ++x) finish(p, b, head0 + h[x], S::D, d[x], v[x], m[x], l[x]);
             }
@@ -835,9 +864,9 @@ extern "C" {
 
 int64_t pplb200_paged_decode_attention_workspace_bytes(int64_t batch, int64_t max_tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
     if (batch < 0 || max_tokens < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0) return -1;
-    // a counter and two pieces a CTA at most
+    // three counters and two pieces a CTA at most
     const int heads = heads_at_once(head_dim, q_heads / kv_heads);
-    return round_up(kCtas * 8, 256) + round_up(2 * kCtas * heads * 8, 256) + 2LL * kCtas * heads * head_dim * 4;
+    return round_up(3 * kCtas * 8, 256) + round_up(2 * kCtas * heads * 8, 256) + 2LL * kCtas * heads * head_dim * 4;
 }
 
 int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_paged_attention_args* a) {
@@ -889,7 +918,7 @@ int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb2
     static std::atomic<uint64_t> calls{0};
     p.call = ++calls;
     p.arrived = (uint64_t*)a->ws;
-    p.tops = (float2*)((char*)a->ws + round_up(kCtas * 8, 256));
+    p.tops = (float2*)((char*)a->ws + round_up(3 * kCtas * 8, 256));
     p.sums = (float*)((char*)p.tops + round_up(2 * kCtas * heads * 8, 256));
     const bool packed = cache->page_size % 16 == 0 && cache->token_stride == D && (cache->quant_group != 8 || cache->scale_token_stride == D / 8);
     const cudaStream_t s = (cudaStream_t)stream;

@@ -511,7 +511,7 @@ def test_attention_fewer_sequences_leave_the_rest_alone(cuda, pplb200):
 def test_attention_is_the_same_run_after_run(cuda, pplb200, group):
     out, lse, _, (att, q, table, lens, cache) = _run_attention(cuda, pplb200, [9000, 3, 500, 1234], 16, 2, 128, 16, group)
     for fill in (0, 255, 127):
-        att.ws[8192:].fill_(fill)  # whatever an earlier call's sums were; the counters of arrivals lie in front of them
+        att.ws[14336:].fill_(fill)  # whatever an earlier call's sums were; the counters of arrivals lie in front of them
         again = cuda.empty_like(lse)
         assert cuda.equal(att(q, table, lens, lse=again), out) and cuda.equal(again, lse)
 
@@ -520,8 +520,16 @@ def test_attention_recovers_from_counters_that_were_left(cuda, pplb200):
     """Calls that overlapped on one workspace, against the rules, may leave counters of arrivals behind: the next call is right again."""
     out, _, _, (att, q, table, lens, cache) = _run_attention(cuda, pplb200, [9000, 3, 500, 1234], 16, 2, 128, 16, 128)
     for left in (1, 5, (1 << 16) + 3):
-        att.ws[:592 * 8].view(cuda.int64).fill_(left)
+        att.ws[:3 * 592 * 8].view(cuda.int64).fill_(left)
         assert cuda.equal(att(q, table, lens), out)
+
+
+@pytest.mark.parametrize("hq,hk,d", [(8, 1, 64), (4, 1, 128), (16, 1, 128), (3, 1, 256), (8, 4, 96)])
+@pytest.mark.parametrize("group", [0, 8, -1])
+def test_attention_of_few_heads_is_joined_from_many_parts(cuda, pplb200, hq, hk, d, group):
+    """One or two sequences over the whole device: hundreds of parts of one item, beside items of one part."""
+    for lengths in ([40000], [30001, 0, 5], [700, 20000], [2500]):
+        _check_attention(*_run_attention(cuda, pplb200, lengths, hq, hk, d, 48, d if group < 0 else group)[:3])
 
 
 @pytest.mark.parametrize("group", [0, 8, 128])
