@@ -1,4 +1,5 @@
-"""Builds the sm_100a shared library in-tree: lib/libpplb200_i8i8.so.
+"""Builds the sm_100a shared library in-tree, lib/libpplb200_i8i8.so, and (where torch is installed, whose tensors it reads) the
+compiled part of the Python binding, lib/pplb200_attention_binding.so.
 
     python build.py [--force] [--verbose]
 
@@ -6,9 +7,11 @@ nvcc cross-compiles without a GPU.  The explicit -gencode form matters: tcgen05 
 accepted for the arch-specific target sm_100a, and plain -arch=sm_100a would also emit a
 generic compute_100 PTX image in which it is rejected.
 """
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -16,6 +19,8 @@ LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libpplb200_i8i8.so")
 SOURCES = ["capi.cu", "quantize.cu", "rmsnorm_quantize.cu", "activation_requant.cu", "gemm_i8_tcgen05.cu", "gemm_i8_decode.cu", "gemm_i8_token_pair.cu", "tensor_parallel.cu", "p2p_row_parallel.cu", "no_alloc.cu", "rotary_kv.cu", "paged_attention.cu", "probes.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+BINDING = os.path.join(LIBDIR, "pplb200_attention_binding.so")
+BINDING_SOURCE = os.path.join(CSRC, "attention_binding.cpp")
 FLAGS = [
     "-std=c++17", "-O3", "-lineinfo",
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -47,6 +52,15 @@ def build(force=False, verbose=False):
             subprocess.run(cmd, check=True)
     if force or _stale(LIB, objs):
         cmd = [NVCC, "-shared", "-o", LIB] + objs + ["-ldl"]
+        if verbose:
+            print(" ".join(cmd))
+        subprocess.run(cmd, check=True)
+    torch = importlib.util.find_spec("torch")
+    if torch is not None and (force or _stale(BINDING, [BINDING_SOURCE] + headers)):
+        home = torch.submodule_search_locations[0]
+        cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-Wall", "-shared", "-fPIC", "-fvisibility=hidden", "-I" + sysconfig.get_paths()["include"],
+               "-isystem", os.path.join(home, "include"), "-isystem", os.path.join(home, "include", "torch", "csrc", "api", "include"),
+               BINDING_SOURCE, "-o", BINDING, "-L" + os.path.join(home, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
         if verbose:
             print(" ".join(cmd))
         subprocess.run(cmd, check=True)

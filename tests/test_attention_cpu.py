@@ -4,6 +4,7 @@ import ctypes
 import math
 import os
 import re
+import struct
 import subprocess
 
 import numpy as np
@@ -23,7 +24,6 @@ def test_library_exports_every_declared_symbol():
 
 
 def test_header_is_plain_c99_and_blocks_are_packed_as_declared(tmp_path):
-    import struct
     src = tmp_path / "c_caller.c"
     src.write_text('#include "pplb200_attention.h"\n#include <stdio.h>\n#include <stddef.h>\n'
                    'int main(void) {\n'
@@ -111,8 +111,7 @@ CACHE = dict(k=AT, v=AT, ks=AT, vs=AT, pages=100, page_stride=8 * 16 * 128, head
 
 
 def _cache(**kw):
-    from pplb200.attention import _pack_cache
-    return _pack_cache(*dict(CACHE, **kw).values())
+    return struct.pack("=4Q7q4i", *dict(CACHE, **kw).values())
 
 
 def test_offsets():
@@ -154,10 +153,9 @@ ATTEND = dict(q=AT, out=AT, lse=0, pages=AT, lengths=AT, ws=AT, ws_bytes=1 << 40
 
 def _calls():
     import pplb200
-    from pplb200 import attention as a
-    return (lambda c, **kw: pplb200.lib.pplb200_kv_cache_write_fp16(None, c, a._pack_write(*dict(WRITE, **kw).values())),
-            lambda **kw: pplb200.lib.pplb200_rotary_fp16(None, a._pack_rotary(*dict(ROTARY, **kw).values())),
-            lambda c, **kw: pplb200.lib.pplb200_paged_decode_attention_fp16(None, c, a._pack_attention(*dict(ATTEND, **kw).values())))
+    return (lambda c, **kw: pplb200.lib.pplb200_kv_cache_write_fp16(None, c, struct.pack("=7Q5q3if", *dict(WRITE, **kw).values())),
+            lambda **kw: pplb200.lib.pplb200_rotary_fp16(None, struct.pack("=6Q5q5if", *dict(ROTARY, **kw).values())),
+            lambda c, **kw: pplb200.lib.pplb200_paged_decode_attention_fp16(None, c, struct.pack("=6Q6q2ifi", *dict(ATTEND, **kw).values())))
 
 
 @pytest.mark.parametrize("bad,rc", BAD_CACHES)
@@ -241,17 +239,20 @@ def test_attention_workspace():
 
 @pytest.fixture
 def here(monkeypatch):
-    """The binding with CPU tensors taken for the current device's and the C calls recorded."""
+    """The binding with CPU tensors taken for the current device's and the C calls recorded, their last argument block as bytes."""
     from pplb200 import attention
-    calls = []
+    calls, keep = [], []
     monkeypatch.setattr(attention, "_here", lambda: (-1, 0))
-    for n in ("_rotary", "_write", "_read", "_attend"):
-        monkeypatch.setattr(attention, n, lambda *a, n=n: calls.append((n, a)) or 0)
-    return calls
+    vp, i64 = ctypes.c_void_p, ctypes.c_int64
+    for n, types, size in (("_rotary", (vp, vp), 112), ("_write", (vp, vp, vp), 112), ("_read", (vp, vp, vp, i64, vp, vp), 0), ("_attend", (vp, vp, vp), 112)):
+        f = ctypes.CFUNCTYPE(ctypes.c_int32, *types)(lambda *a, n=n, size=size: calls.append((n, a[:-1] + (ctypes.string_at(a[-1], size),) if size else a)) or 0)
+        keep.append(f)
+        monkeypatch.setattr(attention, n, ctypes.cast(f, vp).value)
+    yield calls
+    del keep
 
 
 def test_binding_takes_strided_heads(here):
-    import struct
     import torch
     import pplb200
     rows = torch.zeros((5, 12, 64), dtype=torch.float16)
@@ -307,14 +308,13 @@ def test_binding_refuses_other_types_shapes_and_devices(here, monkeypatch):
 
 
 def test_binding_describes_the_cache():
-    import struct
     import torch
     import pplb200
     k, v = (torch.zeros((6, 24, 4, 96), dtype=torch.int8) for _ in range(2))
     ks, vs = (torch.zeros((6, 24, 4, 12), dtype=torch.float16) for _ in range(2))
     c = pplb200.PagedKVCache(*(t.transpose(1, 2) for t in (k, v, ks, vs)))  # stored token by token
     assert (c.num_pages, c.kv_heads, c.page_size, c.head_dim, c.quant_group) == (6, 4, 24, 96, 8)
-    assert struct.unpack("=4Q7q4i", c._block) == (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), 6, 24 * 384, 96, 384, 24 * 48, 12, 48, 24, 4, 96, 8)
+    assert struct.unpack("=4Q7q4i", c._args[0]) == (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), 6, 24 * 384, 96, 384, 24 * 48, 12, 48, 24, 4, 96, 8)
     h = torch.float16
     for bad in (lambda: pplb200.PagedKVCache(k, v), lambda: pplb200.PagedKVCache(k.to(h), v.to(h), ks, vs), lambda: pplb200.PagedKVCache(k, v, ks, None),
                 lambda: pplb200.PagedKVCache(k, v[:5], ks, vs), lambda: pplb200.PagedKVCache(k, v, ks.float(), vs.float()), lambda: pplb200.PagedKVCache(k, v, ks[..., :5], vs[..., :5]),
