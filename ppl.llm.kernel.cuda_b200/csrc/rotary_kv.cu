@@ -56,10 +56,11 @@ union Eight {
     __half2 h[4];
 };
 
-// Largest magnitude of eight halves as fp16 bits.  Compared as integers: a NaN is above infinity, so that it comes through.
-__device__ __forceinline__ uint32_t absmax_bits(const uint4& a) {
-    const uint32_t m = __vmaxu2(__vmaxu2(a.x & 0x7fff7fffu, a.y & 0x7fff7fffu), __vmaxu2(a.z & 0x7fff7fffu, a.w & 0x7fff7fffu));
-    return max(m & 0xffffu, m >> 16);
+// Largest magnitude of eight halves as fp16 bits; a NaN comes through.
+__device__ __forceinline__ uint32_t absmax_bits(const Eight& e) {
+    const __half2 m = __hmax2_nan(__hmax2_nan(__habs2(e.h[0]), __habs2(e.h[1])), __hmax2_nan(__habs2(e.h[2]), __habs2(e.h[3])));
+    const uint32_t bits = *reinterpret_cast<const uint32_t*>(&m);
+    return max(bits & 0xffffu, bits >> 16);
 }
 
 // The scale of a group: amax / 127 rounded up to fp16 -- fp16 so that what is divided by is what is stored, up so that no quotient is
@@ -74,36 +75,44 @@ __device__ __forceinline__ half group_scale(uint32_t amax) {
     return __ushort_as_half((unsigned short)(amax < 0x7c00u ? min(max(s, 1u), 0x6007u) : amax));
 }
 
-// Eight quotients rounded to nearest even, as bytes.  Their magnitude is at most 127.07 (65504 / 515.5).  The product with the scale's
+// Quotients by one scale, rounded to nearest even, as bytes.  Their magnitude is at most 127.07 (65504 / 515.5).  The product with the scale's
 // reciprocal, moved by 2^-21 to either side, brackets the quotient in 32 bits (the reciprocal is off by 2^-23 at most, its moving, the
 // product and the quotient by 2^-24 each); 1.5 * 2^23 added, the low byte is the rounded number.  Where the two sides differ, and in a
 // group with an infinity or a NaN, the division decides; there NaN becomes 0, and is NaN again when it is multiplied by that group's scale.
-__device__ __forceinline__ uint2 quantize_eight(const Eight& e, half scale) {
-    const float s = __half2float(scale);
-    float inv;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
-    const float hi = inv * (1.0f + 0x1p-21f), lo = inv * (1.0f - 0x1p-21f);
-    constexpr float kMagic = 12582912.0f;
-    uint32_t b[8], differ = __half_as_ushort(scale) < 0x7c00u ? 0u : 1u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 v = __half22float2(e.h[i]);
-        b[2 * i] = __float_as_uint(__fmaf_rn(v.x, hi, kMagic));
-        b[2 * i + 1] = __float_as_uint(__fmaf_rn(v.y, hi, kMagic));
-        differ |= b[2 * i] ^ __float_as_uint(__fmaf_rn(v.x, lo, kMagic));
-        differ |= b[2 * i + 1] ^ __float_as_uint(__fmaf_rn(v.y, lo, kMagic));
+struct Quotient {
+    float s, hi, lo;
+    uint32_t special;
+    __device__ __forceinline__ explicit Quotient(half scale) {
+        s = __half2float(scale);
+        float inv;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+        hi = inv * (1.0f + 0x1p-21f);
+        lo = inv * (1.0f - 0x1p-21f);
+        special = __half_as_ushort(scale) < 0x7c00u ? 0u : 1u;
     }
-    if (differ != 0u) {
+    __device__ __forceinline__ uint2 eight(const Eight& e) const {
+        constexpr float kMagic = 12582912.0f;
+        uint32_t b[8], differ = special;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 v = __half22float2(e.h[i]);
-            b[2 * i] = (uint32_t)__float2int_rn(__fdiv_rn(v.x, s));
-            b[2 * i + 1] = (uint32_t)__float2int_rn(__fdiv_rn(v.y, s));
+            b[2 * i] = __float_as_uint(__fmaf_rn(v.x, hi, kMagic));
+            b[2 * i + 1] = __float_as_uint(__fmaf_rn(v.y, hi, kMagic));
+            differ |= b[2 * i] ^ __float_as_uint(__fmaf_rn(v.x, lo, kMagic));
+            differ |= b[2 * i + 1] ^ __float_as_uint(__fmaf_rn(v.y, lo, kMagic));
         }
+        if (differ != 0u) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 v = __half22float2(e.h[i]);
+                b[2 * i] = (uint32_t)__float2int_rn(__fdiv_rn(v.x, s));
+                b[2 * i + 1] = (uint32_t)__float2int_rn(__fdiv_rn(v.y, s));
+            }
+        }
+        return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                          __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
     }
-    return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
-                      __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
-}
+};
 
 // Cosines and sines (times the magnitude) of four and four planes: the angle modulo one turn, exactly, as a signed fraction, in half turns.
 struct Turns {
@@ -135,11 +144,15 @@ __device__ __forceinline__ void rotate(Eight& a, Eight& b, const Turns& t, bool 
 // A thread has 16 dimensions of a token: two runs of eight that are rotated against each other (half layout) or each in itself, so that
 // nothing crosses threads but the scale of a whole head; neighbouring threads have neighbouring runs, so that loads and stores fill lines.  It computes their eight sines and cosines once, while its
 // first rows are on their way, and takes every groups-th head of q, k and v with them; LANES threads side by side make a row.
+// Threads without dimensions or tokens of their own, and turns without a head, read another's row and store nothing: no load waits for
+// a branch.
 constexpr int RTPB = 128;
-template <int LANES, bool INTERLEAVED, bool STORE>
+enum : int { AS_IS = 0, HALVES = 1, INTERLEAVED = 2 }; // what is rotated against what; AS_IS keeps sixteen registers free
+enum : int { NO_STORE = 0, STORE_F16 = 1, STORE_I8_GROUPS = 2, STORE_I8_ROWS = 3 };
+template <int LANES, int LAYOUT, int STORE>
 struct RotaryKv {
     struct Row {
-        Eight a, b; // zeros where there is nothing
+        Eight a, b;
     };
     const RotaryKvParams& p;
     int64_t token;
@@ -150,19 +163,16 @@ struct RotaryKv {
 
     template <int KIND>
     __device__ __forceinline__ void fetch(int head, Row& x) const {
-        x.a.raw = x.b.raw = make_uint4(0, 0, 0, 0);
-        if (active && head < p.heads[KIND]) {
-            const half* src = p.src[KIND] + token * p.src_stride[KIND] + (int64_t)head * p.head_dim;
-            x.a.raw = ld_global_16(src + da);
-            x.b.raw = ld_global_16(src + db);
-        }
+        const half* src = p.src[KIND] + token * p.src_stride[KIND] + (int64_t)min(head, p.heads[KIND] - 1) * p.head_dim;
+        x.a.raw = ld_global_16(src + da);
+        x.b.raw = ld_global_16(src + db);
     }
     // Called by all threads of a warp.
     template <int KIND>
     __device__ __forceinline__ void finish(int head, Row& x) const {
-        if (KIND != V && turned) rotate(x.a, x.b, turns, INTERLEAVED);
+        if (KIND != V && LAYOUT != AS_IS && turned) rotate(x.a, x.b, turns, LAYOUT == INTERLEAVED);
         const bool there = active && head < p.heads[KIND];
-        if constexpr (!STORE || KIND == Q) {
+        if constexpr (STORE == NO_STORE || KIND == Q) {
             half* dst = p.dst[KIND] + token * p.dst_stride[KIND] + (int64_t)head * p.head_dim;
             if (there) {
                 *reinterpret_cast<uint4*>(dst + da) = x.a.raw;
@@ -172,35 +182,41 @@ struct RotaryKv {
             const int64_t row = at + (int64_t)head * p.cache.head_stride;
             void* const data = KIND == V ? p.cache.v : p.cache.k;
             const bool stored = there && at >= 0;
-            if (p.cache.quant_group == 0) {
+            if constexpr (STORE == STORE_F16) {
                 if (stored) {
                     *reinterpret_cast<uint4*>((half*)data + row + da) = x.a.raw;
                     *reinterpret_cast<uint4*>((half*)data + row + db) = x.b.raw;
                 }
-                return;
-            }
-            uint32_t ma = absmax_bits(x.a.raw), mb = absmax_bits(x.b.raw);
-            if (p.cache.quant_group != 8) {
-                ma = max(ma, mb);
+            } else {
+                int8_t* const dst = (int8_t*)data + row;
+                half* const scale = (half*)(KIND == V ? p.cache.v_scale : p.cache.k_scale) + scale_at + (int64_t)head * p.cache.scale_head_stride;
+                uint32_t ma = absmax_bits(x.a), mb = absmax_bits(x.b);
+                if constexpr (STORE == STORE_I8_ROWS) {
+                    ma = active ? max(ma, mb) : 0u;
 #pragma unroll
-                for (int m = LANES / 2; m >= 1; m >>= 1) ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, m));
-            }
-            if (!stored) return;
-            const half sa = group_scale(ma), sb = p.cache.quant_group == 8 ? group_scale(mb) : sa;
-            const uint2 qa = quantize_eight(x.a, sa), qb = quantize_eight(x.b, sb);
-            int8_t* dst = (int8_t*)data + row;
-            *reinterpret_cast<uint2*>(dst + da) = qa;
-            *reinterpret_cast<uint2*>(dst + db) = qb;
-            half* scale = (half*)(KIND == V ? p.cache.v_scale : p.cache.k_scale) + scale_at + (int64_t)head * p.cache.scale_head_stride;
-            if (p.cache.quant_group == 8) {
-                scale[da >> 3] = sa;
-                scale[db >> 3] = sb;
-            } else if (u == 0) {
-                scale[0] = sa;
+                    for (int m = LANES / 2; m >= 1; m >>= 1) ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, m));
+                    const half s = group_scale(ma);
+                    const Quotient by(s);
+                    const uint2 qa = by.eight(x.a), qb = by.eight(x.b);
+                    if (stored) {
+                        *reinterpret_cast<uint2*>(dst + da) = qa;
+                        *reinterpret_cast<uint2*>(dst + db) = qb;
+                        if (u == 0) scale[0] = s;
+                    }
+                } else {
+                    const half sa = group_scale(ma), sb = group_scale(mb);
+                    const uint2 qa = Quotient(sa).eight(x.a), qb = Quotient(sb).eight(x.b);
+                    if (stored) {
+                        *reinterpret_cast<uint2*>(dst + da) = qa;
+                        *reinterpret_cast<uint2*>(dst + db) = qb;
+                        scale[da >> 3] = sa;
+                        scale[db >> 3] = sb;
+                    }
+                }
             }
         }
     }
-    // Rows behind the first, two at a time.
+    // Rows behind the first, two at a time: of one tensor, or, where there is no q to go through, a key's and the value's beside it.
     template <int KIND>
     __device__ __forceinline__ void others(int group) const {
         for (int i = 1; i < p.turns_of[KIND]; i += 2) {
@@ -211,16 +227,31 @@ struct RotaryKv {
             if (i + 1 < p.turns_of[KIND]) finish<KIND>(group + (i + 1) * p.groups, y);
         }
     }
+    __device__ __forceinline__ void other_pairs(int group) const {
+        for (int i = 1; i < p.turns_of[K]; ++i) {
+            Row x, y;
+            fetch<K>(group + i * p.groups, x);
+            fetch<V>(group + i * p.groups, y);
+            finish<K>(group + i * p.groups, x);
+            finish<V>(group + i * p.groups, y);
+        }
+    }
 };
 
-template <int LANES, bool INTERLEAVED, bool STORE>
-__global__ void __launch_bounds__(RTPB, 7) rotary_kv_kernel(const __grid_constant__ RotaryKvParams p) {
+// Bound by HBM where nothing is quantized: 8192 tokens of 64 + 8 heads of 128 rotated 47 us, 97 % of a copy's rate; stored as fp16 too, 57 us,
+// 91 %.  Quantizing costs some 200 instructions for 16 elements of 32 lanes, which shows: 16384 tokens of 8 + 8 heads 22.4 us, 69 % (29 with
+// branches around the loads, keys and values one after the other and a run-time choice of the cache's type).  CTAs that share an
+// SM were tried from 5 to 10: unrotated, 10 spill (24.4 us), 6 take as long as 8 but 8.9 instead of 8.2 us for 4096 tokens in groups of 8; rotated, into groups of 8,
+// 2048 tokens of 32 + 32 heads, 22.6 us with 7, 24 with 6.
+template <int LANES, int LAYOUT, int STORE>
+__global__ void __launch_bounds__(RTPB, LAYOUT == AS_IS ? 8 : 7) rotary_kv_kernel(const __grid_constant__ RotaryKvParams p) {
     pdl_wait_prior_grid();
     const uint32_t n = blockIdx.x * (RTPB / LANES) + threadIdx.x / LANES;
-    RotaryKv<LANES, INTERLEAVED, STORE> r{p};
+    RotaryKv<LANES, LAYOUT, STORE> r{p};
     r.token = (uint32_t)((uint64_t)n * p.group_magic >> p.group_shift);
     const int group = n - (uint32_t)r.token * p.groups;
     const bool valid = r.token < p.tokens;
+    if (!valid) r.token = 0;
     r.u = threadIdx.x & (LANES - 1);
     r.active = valid && 16 * r.u < p.head_dim;
     r.turned = valid && 16 * r.u < p.rotary_dim;
@@ -228,13 +259,14 @@ __global__ void __launch_bounds__(RTPB, 7) rotary_kv_kernel(const __grid_constan
     const int behind = r.u - (p.rotary_dim >> 4);
     r.da = behind < 0 ? 8 * r.u : p.rotary_dim + 8 * behind;
     r.db = r.da + ((behind < 0 ? p.rotary_dim : p.head_dim - p.rotary_dim) >> 1);
-    typename RotaryKv<LANES, INTERLEAVED, STORE>::Row q, k, v;
-    r.template fetch<Q>(group, q);
-    r.template fetch<K>(group, k);
+    if (!r.active) r.da = 0, r.db = 0;
+    typename RotaryKv<LANES, LAYOUT, STORE>::Row q, k, v;
+    if (p.turns_of[Q] > 0) r.template fetch<Q>(group, q);
+    if (p.turns_of[K] > 0) r.template fetch<K>(group, k);
     if (STORE) r.template fetch<V>(group, v);
-    if (r.turned) {
-        const uint64_t* first = p.turns + (INTERLEAVED ? 4 : 8) * r.u; // planes of the runs: eight of both, or four of each
-        turns_at(r.turns, (uint64_t)p.positions[r.token], first, first + (INTERLEAVED ? p.rotary_dim >> 2 : 4), p.magnitude);
+    if (LAYOUT != AS_IS && r.turned) {
+        const uint64_t* first = p.turns + (LAYOUT == INTERLEAVED ? 4 : 8) * r.u; // planes of the runs: eight of both, or four of each
+        turns_at(r.turns, (uint64_t)p.positions[r.token], first, first + (LAYOUT == INTERLEAVED ? p.rotary_dim >> 2 : 4), p.magnitude);
     }
     r.at = -1;
     r.scale_at = 0;
@@ -250,26 +282,34 @@ __global__ void __launch_bounds__(RTPB, 7) rotary_kv_kernel(const __grid_constan
     if (p.turns_of[K] > 0) r.template finish<K>(group, k);
     if (STORE) r.template finish<V>(group, v);
     r.template others<Q>(group);
-    r.template others<K>(group);
-    if (STORE) r.template others<V>(group);
+    if (LAYOUT == AS_IS) {
+        r.other_pairs(group);
+    } else {
+        r.template others<K>(group);
+        if (STORE) r.template others<V>(group);
+    }
 }
 
+template <int LANES, int STORE>
+void launch_stored(cudaStream_t stream, const RotaryKvParams& p, dim3 grid) {
+    if (p.rotary_dim == 0 && STORE != NO_STORE) launch_ex(rotary_kv_kernel<LANES, STORE != NO_STORE ? AS_IS : HALVES, STORE>, grid, dim3(RTPB), stream, true, p);
+    else if (p.interleaved) launch_ex(rotary_kv_kernel<LANES, INTERLEAVED, STORE>, grid, dim3(RTPB), stream, true, p);
+    else launch_ex(rotary_kv_kernel<LANES, HALVES, STORE>, grid, dim3(RTPB), stream, true, p);
+}
 template <int LANES>
 int32_t launch_lanes(cudaStream_t stream, RotaryKvParams& p) {
     // Heads a thread: as many as spread the sines over enough of them, while the device stays full.
     const int32_t most = std::max(p.heads[Q], std::max(p.heads[K], p.heads[V]));
-    const int64_t heads = std::min<int64_t>(4, std::max<int64_t>(1, p.tokens * most * LANES / (148LL * 1024 * 2)));
+    int64_t heads = std::min<int64_t>(4, std::max<int64_t>(1, p.tokens * most * LANES / (148LL * 1024 * 2)));
+    if (most % heads && most % (heads - 1) == 0) --heads; // no turns without a head
     p.groups = (int32_t)std::min<int64_t>((most + heads - 1) / heads, std::max<int64_t>(1, 0x7fff0000LL / p.tokens));
     for (int k = 0; k < 3; ++k) p.turns_of[k] = (p.heads[k] + p.groups - 1) / p.groups;
     small_division(p.groups, p.group_magic, p.group_shift);
     const dim3 grid((unsigned)((p.tokens * p.groups + RTPB / LANES - 1) / (RTPB / LANES)));
-    if (p.store) {
-        if (p.interleaved) launch_ex(rotary_kv_kernel<LANES, true, true>, grid, dim3(RTPB), stream, true, p);
-        else launch_ex(rotary_kv_kernel<LANES, false, true>, grid, dim3(RTPB), stream, true, p);
-    } else {
-        if (p.interleaved) launch_ex(rotary_kv_kernel<LANES, true, false>, grid, dim3(RTPB), stream, true, p);
-        else launch_ex(rotary_kv_kernel<LANES, false, false>, grid, dim3(RTPB), stream, true, p);
-    }
+    if (!p.store) launch_stored<LANES, NO_STORE>(stream, p, grid);
+    else if (p.cache.quant_group == 0) launch_stored<LANES, STORE_F16>(stream, p, grid);
+    else if (p.cache.quant_group == 8) launch_stored<LANES, STORE_I8_GROUPS>(stream, p, grid);
+    else launch_stored<LANES, STORE_I8_ROWS>(stream, p, grid);
     return check_launch("rotary / cache write");
 }
 int32_t launch_rotary_kv(cudaStream_t stream, RotaryKvParams& p) {
