@@ -106,15 +106,16 @@ int32_t pplb200_kv_cache_read_fp16(pplb200_stream_t stream, const pplb200_kv_cac
 /*
  * Attention of one new token per sequence: out[b, h] = sum_t softmax_t(scale q[b, h] . k_t) v_t over the tokens t of sequence b in
  * head h / (q_heads / kv_heads) of the cache: the stored values, or values x scales, which are not rounded to fp16 in between, except
- * v with groups of 8, which is.  Sums are held in 32 bits; weights enter their products with 22, queries theirs with int8 rows with
- * 23 of the largest of their head.
+ * v with groups of 8, which is.  Scores, sums and statistics are held in 32 bits; the softmax's weights enter their product with v
+ * with 22 bits, over int8 rows that share a scale a head with the 11 of fp16.
  * q, out fp16 [batch, q_heads, head_dim], *_stride elements between sequences, heads contiguous; lengths int32 [batch]: tokens in the
  * cache, the new one among them (at most pages_per_sequence * page_size are looked at); pages int32 [batch, pages_per_sequence] with
  * pages_stride between rows: the page of token t is pages[b, t / page_size].  A page that is negative or not below num_pages is a
  * hole: its tokens take no part.  window > 0: only the last `window` tokens do.  What lies in the cache beyond a sequence's
  * tokens has no influence, whatever it is.  A sequence of which nothing is seen has zeros for its output and -inf for its lse.
  * optional_lse fp32 [batch, q_heads], contiguous: log(sum_t exp(scale q . k_t)), for joining results over parts of a context.
- * head_dim 64, 96, 128 or 256 (with quant_group 8: scales 4-byte aligned, their strides even); q_heads a multiple of kv_heads; strides multiples of 8; q and out 16-byte aligned; out may be q.
+ * head_dim 64, 96, 128 or 256 (with quant_group 8: scales 4-byte aligned, their strides even); q_heads a multiple of kv_heads; strides
+ * multiples of 8; q and out 16-byte aligned; out may be q; scale within 2^50 of zero; at most 2^30 tokens a row of the table.
  * ws: pplb200_paged_decode_attention_workspace_bytes(), 256-byte aligned, zeroed before its first use (every call leaves it fit for the
  * next, of whatever sizes), not shared by calls that may run at the same time (two captured graphs that are replayed at once need
  * one each).

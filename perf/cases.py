@@ -143,7 +143,7 @@ def _prepare_layer(case, g):
     s = dict(case, qkv=qkv)
     s["x"] = _activations(g, m, hidden, "normal")            # output of the previous layer's MLP
     s["residual"] = _activations(g, m, hidden, "outlier")    # the residual stream carries the outlier channels
-    s["attn"] = _activations(g, m, q, "normal")              # what attention, which is not this library's, returned
+    s["attn"] = _activations(g, m, q, "normal")              # what attention returned
     for name, n, k in (("qkv", qkv, hidden), ("o", hidden, q), ("gate_up", 2 * inter, hidden), ("down", hidden, inter)):
         s["w_" + name] = _weights(g, n, k)
         s["sn_" + name] = _column_scales(g, n, *_weight_range(k))

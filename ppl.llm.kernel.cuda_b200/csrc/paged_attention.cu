@@ -1,13 +1,27 @@
 // Attention of one new token per sequence over the paged key-value cache, split over the tokens and joined.
 //
+// out = sum_t w_t v_t / sum_t w_t with w_t = 2^(scale log2(e) q . k_t - top), in one pass: `top` is a reference exponent that moves only when
+// a weight would leave fp16's range, and then rescales what was summed.
+//
 // What bounds it is the cache: every key and value is read once, for a few multiply-adds per element.  So the work is laid out for
-// loads: tiles of CT tokens of one head, numbered over all sequences and heads, are dealt out evenly to as many CTAs as the device holds
-// at once, whatever the sequences' lengths; a CTA whose share begins or ends inside a sequence leaves its sums in the workspace
-// and the CTA that is last to do so joins them.  A warp takes 16 tokens at a time, and while it works on these the next ones are on their way into
-// its registers: a lane loads exactly the bytes that it will use (the dimensions of a product may be taken in any order), so that
-// nothing passes through shared memory.  Scores are computed transposed, keys [16 tokens x dimensions] x queries [dimensions x 8
-// heads]: the eight columns hold the query heads that share the key head, and the weights turn into the operand of the second
-// product, values^T x weights^T, by transposing 8 x 8 blocks between registers.
+// loads: steps of 16 or 32 tokens of one head, numbered over all sequences and heads, are dealt out evenly to as many CTAs as the device
+// holds at once, whatever the sequences' lengths; a CTA whose share begins or ends inside a sequence leaves its sums in the workspace
+// and the CTA that is last to do so joins them, where they are many in groups and then the groups.  While a warp works on its step the next one
+// is on its way into its registers, each part requested as soon as its registers are free: a lane loads exactly the bytes that it will
+// use (the dimensions of a product may be taken in any order), so that nothing passes through shared memory.  Tried instead: rings in shared memory
+// filled by cp.async, whose 64- and 128-byte row parts end at 4.2 TB/s, and by bulk copies of whole runs of rows (65 us instead of 68 with groups of
+// 8, but 149 instead of 121 with int8 rows and 103 instead of 91 in fp16: values are then read with bank conflicts); bringing the step after the next into L2
+// (66 -> 69, 116 -> 119, 88 -> 93).
+//
+// Scores are computed transposed, keys [16 tokens x dimensions] x queries [dimensions x 8 heads]: the eight columns hold the query heads that
+// share the key head, and the weights turn into the operand of the second product, values^T x weights^T, by transposing 8 x 8 blocks
+// between registers.  mma.sync, because an operand of tcgen05.mma would first have to be widened into shared memory, and the tensor pipe is
+// busy for a quarter of the time at most.
+//
+// Heads of 128 in one graph, caches larger than L2, against the bytes at a copy's 6.55 TB/s: 64 sequences of up to 8192 tokens, 64 query
+// heads over 8, int8 rows 112 us (90 %; 124 over seconds, at the power limit and 1.67 GHz); one of 131072, fp16, 89 us (92 %); 16 of up to 4096, 32
+// heads of their own, groups of 8, 66 us (72 %: 575 instructions for 16 tokens, issue slots 56 % busy at 16 warps an SM).  Short
+// ones consist of look-ups that wait for each other, lengths, pages, rows, and of the join: one of 333 tokens 9 us.
 #include "kv_cache.cuh"
 
 #include <algorithm>
@@ -29,15 +43,16 @@ struct Shape {
     static constexpr int D = D_, KIND = KIND_, NT = NT_, HEADS = 8 * NT;
     static constexpr bool PACKED = PACKED_;
     static constexpr int ES = KIND == CACHE_F16 ? 2 : 1;
-    // Tokens of a step: 32 where that leaves room for twelve warps on an SM (64 x 8192, int8 rows: 123 us with 32, 129 with 16; groups,
-    // whose scales take registers too: 16 x 4096 71 us with 32, 67 with 16).
+    // Tokens of a step: 32 where that leaves room for twelve warps on an SM (64 x 8192, int8 rows: 112 us with 32, 118 with 16; groups,
+    // whose scales take registers too: 16 x 4096 67.5 us with 32, 66 with 16).
     static constexpr int SUBS = D * ES <= 64 || (D * ES <= 128 && KIND == CACHE_I8_ROWS) ? 2 : 1, TOKENS = 16 * SUBS;
     // of 16 tokens a quad's lane holds a quarter of the dimensions of two keys, an eighth of those of four values
     static constexpr int KB = D * ES / 4, KP = piece(KB), KN = KB / KP;
     static constexpr int VB = D * ES / 8, VP = piece(VB), VN = VB / VP;
     static constexpr int KG = KP >= 8 ? KP / 8 : 1, VG = VP >= 8 ? VP / 8 : 1; // CACHE_I8_GROUPS: scales of a piece
     static constexpr int STEPS = D / 16; // of 16 dimensions in the first product, and blocks of 16 in the second
-    // Registers for the sums, the queries and the tokens on their way decide how many CTAs share an SM.
+    // Registers for the sums, the queries and the tokens on their way decide how many CTAs share an SM (groups of 8, 128 dimensions: 66 us
+    // with four, 69 with three).
     static constexpr int WORDS = NT * D / 4 + NT * D / 8 + SUBS * (D * ES / 4 + (KIND == CACHE_I8_GROUPS ? 2 * KN + 4 * VN : 0));
     // Weights enter their product in fp16 and, as a second operand, what that rounding left: 22 bits.  Not with int8 rows, where the rest of
     // the kernel draws the most power: their roundings, 2^-12 each, add up to half of what the output's own does, and without the second
@@ -153,7 +168,7 @@ __device__ __forceinline__ int32_t steps_of(const AttentionParams& p, int64_t b)
 }
 
 // What beginning a head of a sequence costs, in steps: a chain of look-ups before the first step, the joining of the warps' sums behind
-// the last, while the other CTAs of the SM go on.
+// the last, while the other CTAs of the SM go on.  Without it the heads of empty and short sequences, which cost time but no steps, pile up on one CTA.
 template <class S>
 constexpr int32_t kBeginning = 2 * S::WARPS;
 
@@ -790,8 +805,8 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                     }
                 }
             };
-            // Many pieces are joined in groups, whose sums take the place of their first piece's, and then the groups: one CTA alone reads
-            // its 4 kB a piece at 100 GB/s.
+            // Many pieces are joined in groups, whose sums take the place of their first piece's, and then the groups: one CTA alone took 8 us
+            // for 55 pieces and 50 for 500 (8 heads over one, 131072 tokens: 74 -> 22 us).
             const int32_t first_of_mine = (int32_t)blockIdx.x - c0;
             int32_t per_group = 1;
             bool ends = true;

@@ -319,6 +319,7 @@ int32_t launch_rotary_kv(cudaStream_t stream, RotaryKvParams& p) {
 
 // Eight dimensions of a key and of the value beside it are a unit, so that a warp's stores fill whole lines.  A block looks up once
 // where its tokens lie (look-ups by every thread: 207 instructions a unit, 32768 tokens 42 us) and then goes through their units.
+// Bound by HBM: 32768 tokens of 8 + 8 heads of 128 from int8 with a scale for every 8, scattered over pages of 16, 38.3 us, 87 % of a copy's rate.
 constexpr int UNITS = 4; // a thread
 struct KvReadParams {
     pplb200_kv_cache cache;
