@@ -39,6 +39,11 @@ int32_t small_integer(PyObject* o) {
     }
     return (int32_t)v;
 }
+int32_t truth(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw Refused();
+    return v;
+}
 void* address(PyObject* o) {
     void* p = PyLong_AsVoidPtr(o);
     if (!p && PyErr_Occurred()) throw Refused();
@@ -145,7 +150,7 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
         args.q_stride = q.stride; args.k_stride = k.stride; args.q_out_stride = qo.stride; args.k_out_stride = ko.stride;
         args.q_heads = q.heads; args.k_heads = k.heads;
         if (dim > INT32_MAX) refuse("%s: too many dimensions", "q");
-        args.head_dim = (int32_t)dim; args.rotary_dim = t.rotary_dim; args.interleaved = PyObject_IsTrue(a[7]); args.magnitude = t.magnitude;
+        args.head_dim = (int32_t)dim; args.rotary_dim = t.rotary_dim; args.interleaved = truth(a[7]); args.magnitude = t.magnitude;
         return [=] { return entry(stream, &args); };
     });
 }
@@ -178,7 +183,7 @@ PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t n) {
             }
             args.positions = (const int64_t*)indices(a[7], "positions", tokens, device);
             args.turns = t.turns; args.rotary_dim = t.rotary_dim; args.magnitude = t.magnitude;
-            args.interleaved = PyObject_IsTrue(a[10]);
+            args.interleaved = truth(a[10]);
         }
         return [=] { return entry(stream, cache, &args); };
     });

@@ -75,7 +75,16 @@ def _settle(device):
         torch.cuda.current_stream(device).synchronize()
 
 
-class RotaryTable:
+class _LaidOutOnce:
+    """Calls are given what an object laid out when it was made: its attributes do not change."""
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__:
+            raise AttributeError("%s of a %s is laid out once; make a new one" % (name, type(self).__name__))
+        object.__setattr__(self, name, value)
+
+
+class RotaryTable(_LaidOutOnce):
     """Frequencies of the rotated planes, laid out once on `device`.  scaling: "none", "linear", "ntk", "yarn" or "wavelength"."""
 
     def __init__(self, rotary_dim, base=10000.0, scaling="none", factor=1.0, original_length=0, keep_turns=0.0, stretch_turns=0.0,
@@ -104,7 +113,7 @@ def rotary_fp16(q, k, positions, table, interleaved=False, q_out=None, k_out=Non
     return (None if q is None else q_out), (None if k is None else k_out)
 
 
-class PagedKVCache:
+class PagedKVCache(_LaidOutOnce):
     """One layer's cache over the caller's tensors: k, v [pages, kv_heads, tokens of a page, head_dim], fp16, or int8 with fp16
     k_scale, v_scale [pages, kv_heads, tokens of a page, head_dim / group].  Any strides (k as v, k_scale as v_scale) with contiguous
     dimensions: a cache that is stored token by token is passed as its transpose(1, 2)."""
@@ -175,7 +184,7 @@ def kv_cache_read(cache, slots, k_out=None, v_out=None):
     return k_out, v_out
 
 
-class PagedDecodeAttention:
+class PagedDecodeAttention(_LaidOutOnce):
     """Attention of one new token a sequence over a PagedKVCache.  Owns the workspace for `max_batch` sequences of `max_length` tokens, so
     one object serves one stream at a time.  scale: 1 / sqrt(head_dim) unless given; window: how many of the last tokens are seen (0: all)."""
 

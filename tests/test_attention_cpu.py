@@ -307,6 +307,33 @@ def test_binding_refuses_other_types_shapes_and_devices(here, monkeypatch):
             call()
 
 
+def test_binding_takes_tensors_and_truth_values(here):
+    import torch
+    import pplb200
+    q, pos, table = torch.zeros((2, 1, 64), dtype=torch.float16), torch.zeros(2, dtype=torch.int64), pplb200.RotaryTable(64, device="cpu")
+    cache = pplb200.PagedKVCache.allocate(10, 16, 1, 64, device="cpu")
+    for call in (lambda: pplb200.rotary_fp16(q, None, [0, 1], table), lambda: pplb200.kv_cache_write(cache, q, q, None), lambda: pplb200.kv_cache_read(cache, pos, k_out=3)):
+        with pytest.raises(TypeError):
+            call()
+    with pytest.raises(ValueError):
+        pplb200.rotary_fp16(q, None, pos, table, interleaved=np.zeros(2))
+    assert not here
+    for on, flag in ((True, 1), (1, 1), (np.bool_(False), 0), (0, 0)):
+        pplb200.rotary_fp16(q, None, pos, table, interleaved=on)
+        assert struct.unpack("=6Q5q5if", here[-1][1][1])[15] == flag
+
+
+def test_objects_are_laid_out_once():
+    import torch
+    import pplb200
+    table = pplb200.RotaryTable(64, device="cpu")
+    cache = pplb200.PagedKVCache.allocate(10, 16, 1, 64, 8, device="cpu")
+    att = pplb200.PagedDecodeAttention(cache, 4, 1, 160)
+    for o, name, value in ((table, "turns", table.turns.clone()), (cache, "k", torch.zeros_like(cache.k)), (cache, "v_scale", None), (att, "ws", att.ws.clone()), (att, "scale", 1.0), (att, "window", 5), (att, "cache", cache)):
+        with pytest.raises(AttributeError):
+            setattr(o, name, value)
+
+
 def test_binding_describes_the_cache():
     import torch
     import pplb200
