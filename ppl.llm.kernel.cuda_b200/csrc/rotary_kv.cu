@@ -301,7 +301,7 @@ int32_t launch_lanes(cudaStream_t stream, RotaryKvParams& p) {
     // Heads a thread: as many as spread the sines over enough of them, while the device stays full.
     const int32_t most = std::max(p.heads[Q], std::max(p.heads[K], p.heads[V]));
     int64_t heads = std::min<int64_t>(4, std::max<int64_t>(1, p.tokens * most * LANES / (148LL * 1024 * 2)));
-    if (most % heads && most % (heads - 1) == 0) --heads; // no turns without a head
+    if (heads > 2 && most % heads && most % (heads - 1) == 0) --heads; // no turns without a head
     p.groups = (int32_t)std::min<int64_t>((most + heads - 1) / heads, std::max<int64_t>(1, 0x7fff0000LL / p.tokens));
     for (int k = 0; k < 3; ++k) p.turns_of[k] = (p.heads[k] + p.groups - 1) / p.groups;
     small_division(p.groups, p.group_magic, p.group_shift);

@@ -47,7 +47,9 @@ def _check_rotated(cuda, got, x, positions, table, interleaved):
 
 
 @pytest.mark.parametrize("tokens,hq,hk,d,rd", [(1, 1, 1, 16, 16), (1, 32, 32, 128, 128), (3, 5, 1, 64, 32), (17, 8, 2, 96, 96), (2, 7, 7, 96, 48), (33, 64, 8, 128, 64), (5, 3, 1, 256, 256),
-                                               (4, 2, 1, 256, 16), (7, 9, 4, 80, 80), (6, 4, 4, 208, 112), (1100, 6, 2, 128, 128), (1025, 40, 1, 64, 64)])
+                                               (4, 2, 1, 256, 16), (7, 9, 4, 80, 80), (6, 4, 4, 208, 112), (1100, 6, 2, 128, 128), (1025, 40, 1, 64, 64),
+                                               # several heads a thread, some of whose turns have none
+                                               (9001, 37, 5, 128, 128), (20000, 7, 2, 256, 64), (40000, 5, 3, 64, 32), (9001, 3, 37, 128, 96)])
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_rotary(cuda, pplb200, tokens, hq, hk, d, rd, interleaved):
     g = _gen(cuda, tokens * 131 + d)
@@ -108,14 +110,15 @@ def test_rotary_in_place_and_strided(cuda, pplb200, interleaved):
 # ---- the cache -------------------------------------------------------------------------------------------------------
 
 def _quantized(x, group):
-    """(int8 values, fp16 scales) of fp16 x in 64 bits."""
+    """(int8 values, fp16 scales) of fp16 x in 64 bits; a group with an infinity has that for its scale, and zeros."""
     x = x.astype(np.float64)
     y = x.reshape(x.shape[:-1] + (-1, group))
     exact = np.abs(y).max(-1, keepdims=True) / 127
     s = exact.astype(np.float16)
     s = np.where(s.astype(np.float64) < exact, np.nextafter(s, np.float16(np.inf)), s)
-    s = np.clip(s, np.float16(2.0 ** -24), np.float16(515.5))
-    return np.rint(y / s.astype(np.float64)).astype(np.int8).reshape(x.shape), s[..., 0]
+    s = np.where(np.isinf(exact), np.float16(np.inf), np.clip(s, np.float16(2.0 ** -24), np.float16(515.5)))
+    q = np.where(np.isinf(exact), 0, np.rint(np.where(np.isinf(exact), 0, y) / s.astype(np.float64)))
+    return q.astype(np.int8).reshape(x.shape), s[..., 0]
 
 
 def _cache(cuda, pplb200, pages, page, heads, d, group, order, fill):
@@ -132,7 +135,8 @@ def _rows(t, slots, page):
     return None if t is None else t[slots // page, :, slots % page]
 
 
-STORED = [(1, 1, 16, 16, 1), (3, 2, 64, 8, 5), (29, 8, 128, 16, 3), (16, 32, 128, 16, 1), (50, 3, 96, 7, 2), (33, 1, 256, 64, 1), (12, 5, 80, 24, 4), (1200, 2, 128, 16, 1), (40, 4, 208, 1, 3)]
+STORED = [(1, 1, 16, 16, 1), (3, 2, 64, 8, 5), (29, 8, 128, 16, 3), (16, 32, 128, 16, 1), (50, 3, 96, 7, 2), (33, 1, 256, 64, 1), (12, 5, 80, 24, 4), (1200, 2, 128, 16, 1), (40, 4, 208, 1, 3),
+          (12001, 7, 128, 16, 3), (14001, 3, 256, 7, 2)]  # several heads a thread, some of whose turns have none
 
 
 @pytest.mark.parametrize("tokens,heads,d,page,spare", STORED)
@@ -171,7 +175,7 @@ def test_write_and_read(cuda, pplb200, tokens, heads, d, page, spare, group, ord
         if group:
             s = _rows(scale, slots[kept], page).cpu().numpy().astype(np.float64)
             want = cuda.from_numpy((want.cpu().numpy().astype(np.float64) * np.repeat(s, group, -1)).astype(np.float16)).cuda()
-        assert cuda.equal(back[kept], want)
+        assert bool(((back[kept] == want) | (back[kept].isnan() & want.isnan())).all())
 
 
 @pytest.mark.parametrize("group", [8, 64])
@@ -207,7 +211,8 @@ def test_quantizer_at_its_edges(cuda, pplb200, group):
     assert np.all(np.abs(got - put) <= half + (np.abs(put) + half) * HALF + TINY)
 
 
-@pytest.mark.parametrize("tokens,hq,hk,d,rd,page", [(1, 8, 1, 128, 128, 16), (16, 32, 32, 128, 128, 16), (37, 7, 7, 96, 48, 5), (1030, 8, 2, 64, 64, 64), (3, 4, 2, 256, 128, 1)])
+@pytest.mark.parametrize("tokens,hq,hk,d,rd,page", [(1, 8, 1, 128, 128, 16), (16, 32, 32, 128, 128, 16), (37, 7, 7, 96, 48, 5), (1030, 8, 2, 64, 64, 64), (3, 4, 2, 256, 128, 1),
+                                                    (9001, 10, 3, 128, 128, 16), (16001, 13, 13, 64, 48, 16)])
 @pytest.mark.parametrize("group", [0, 8, -1])
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_rotating_write_is_the_two_calls(cuda, pplb200, tokens, hq, hk, d, rd, page, group, interleaved):
