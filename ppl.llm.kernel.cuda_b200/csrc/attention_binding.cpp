@@ -1,6 +1,6 @@
 // What the Python binding of rotary positions, the paged cache and decode attention does on every call: tensors are checked, the argument
 // block is filled in, the C entry point is called with the interpreter released.  Compiled, because the same in Python took 1.7 to
-// 3.7 us a call, more than the smallest of these kernels; this takes 0.2 to 0.4 (a 16-token rotation, call after call: 7.5 -> 4.3 us).  Each function takes the address of its entry point, the stream and the device
+// 3.7 us a call, more than the smallest of these kernels; now it takes 0.4 to 0.6 (a 16-token rotation, call after call: 7.5 -> 4.3 us).  Each function takes the address of its entry point, the stream and the device
 // that the tensors must be on (-1: memory of the host), and returns the entry point's code; a tensor that does not fit is a ValueError.
 #include <Python.h>
 
