@@ -78,11 +78,10 @@ __device__ __forceinline__ uint32_t ld_global_u32(const uint32_t* p) {
 }
 
 template <typename... Args>
-cudaError_t launch_ex(void (*kernel)(Args...), dim3 grid, dim3 block, size_t dynamic_smem, cudaStream_t stream, bool pdl, Args... args) {
+cudaError_t launch_ex(void (*kernel)(Args...), dim3 grid, dim3 block, cudaStream_t stream, bool pdl, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
-    cfg.dynamicSmemBytes = dynamic_smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -90,10 +89,6 @@ cudaError_t launch_ex(void (*kernel)(Args...), dim3 grid, dim3 block, size_t dyn
     cfg.attrs = &attr;
     cfg.numAttrs = pdl ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-template <typename... Args>
-cudaError_t launch_ex(void (*kernel)(Args...), dim3 grid, dim3 block, cudaStream_t stream, bool pdl, Args... args) {
-    return launch_ex(kernel, grid, block, size_t(0), stream, pdl, args...);
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
