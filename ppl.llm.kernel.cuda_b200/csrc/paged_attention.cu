@@ -82,8 +82,7 @@ struct AttentionParams {
     uint32_t unit, page_units, token_units, scale_unit, scale_page_units, scale_token_units;
     uint32_t page_magic, page_shift; // token / page_size = token * page_magic >> page_shift
     pplb200_kv_cache cache;
-    // what spread() flips: in registers, since an instruction holds one constant
-    uint32_t flip, flip_1024;
+    uint32_t flip_1024; // what spread() flips: in a register, since an instruction holds one constant
     // workspace
     uint64_t call;     // number of the call, counted by the process
     uint64_t* arrived; // [CTAs]: pieces, or groups of them, of the item that the CTA began; then [2 * CTAs]: pieces of a group
@@ -135,7 +134,7 @@ __device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uin
 __device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 
 // Bytes 0, 2 or (of w >> 8) bytes 1, 3 of a word as two halves' bits: u = value + 128, a byte with its sign bit flipped, beneath the
-// exponent that `flip` brings.  With none, the half is u * 2^-24, a subnormal number; with 0x64 above it, 1024 + u.
+// exponent that `flip` brings: with 0x64 above it, 1024 + u.
 __device__ __forceinline__ uint32_t spread(uint32_t w, uint32_t flip) {
     uint32_t r;
     asm("lop3.b32 %0, %1, 0x00ff00ff, %2, 0x6a;" : "=r"(r) : "r"(w), "r"(flip)); // (w & 0x00ff00ff) ^ flip
@@ -143,7 +142,10 @@ __device__ __forceinline__ uint32_t spread(uint32_t w, uint32_t flip) {
 }
 __device__ __forceinline__ uint32_t less_1152(uint32_t v) { return h2(__hsub2(as_h2(v), as_h2(0x64806480u))); }
 
-// The four bytes of a word as halves, 0, 2 and 1, 3 (a product's dimensions may come in any order).
+// The four bytes of a word as halves, 0, 2 and 1, 3 (a product's dimensions may come in any order): the whole numbers themselves.  Keys of rows
+// as u * 2^-24, subnormal numbers that need no subtraction, would leave 128 times the sum of a query's elements to be taken off the score,
+// which is hundreds of times the score where a row's scale comes from a dimension that the query does not see, and cost the score as many of
+// its 24 bits (64 x 8192 tokens: 109 us so, 111 with whole numbers).
 __device__ __forceinline__ void widen(const AttentionParams& p, uint32_t w, uint32_t& even, uint32_t& odd) {
     even = less_1152(spread(w, p.flip_1024));
     odd = less_1152(spread(w >> 8, p.flip_1024));
@@ -455,27 +457,6 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
         locate(ahead, step0 + warp + WARPS);
         ahead = find(step0 + warp + 2 * WARPS);
 
-        // CACHE_I8_ROWS: keys enter the product as (value + 128) * 2^-24, exactly; 128 * 2^-24 times the sum of a query's elements is taken
-        // off its scores, here for the lane's two heads.
-        float bias[S::NT][2] = {};
-        if constexpr (S::KIND == CACHE_I8_ROWS) {
-#pragma unroll
-            for (int nt = 0; nt < S::NT; ++nt) {
-                float all_dims = 0.0f;
-#pragma unroll
-                for (int s = 0; s < S::STEPS; ++s)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const float2 f = __half22float2(as_h2(q[nt][s][x]));
-                        all_dims += f.x + f.y;
-                    }
-                all_dims += __shfl_xor_sync(0xffffffffu, all_dims, 1);
-                all_dims += __shfl_xor_sync(0xffffffffu, all_dims, 2);
-                bias[nt][0] = __shfl_sync(0xffffffffu, all_dims, 8 * t) * 0x1p-17f;
-                bias[nt][1] = __shfl_sync(0xffffffffu, all_dims, 8 * t + 4) * 0x1p-17f;
-            }
-        }
-
         float o[S::NT][S::STEPS][4] = {}, top[S::NT][2], sum[S::NT][2] = {};
 #pragma unroll
         for (int nt = 0; nt < S::NT; ++nt) top[nt][0] = top[nt][1] = -1e30f;
@@ -508,8 +489,9 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                             } else if constexpr (S::KIND == CACHE_I8_ROWS) {
 #pragma unroll
                                 for (int s = 0; s < KW; ++s) {
-                                    const uint32_t w0 = kw[sub][0][i][s], w1 = kw[sub][1][i][s];
-                                    const uint32_t a0 = spread(w0, p.flip), a1 = spread(w1, p.flip), a2 = spread(w0 >> 8, p.flip), a3 = spread(w1 >> 8, p.flip);
+                                    uint32_t a0, a1, a2, a3;
+                                    widen(p, kw[sub][0][i][s], a0, a2);
+                                    widen(p, kw[sub][1][i][s], a1, a3);
 #pragma unroll
                                     for (int nt = 0; nt < S::NT; ++nt) mma(s & 1 ? c2[nt] : c[sub][nt], a0, a1, a2, a3, q[nt][i * KW + s][0], q[nt][i * KW + s][1]);
                                 }
@@ -538,12 +520,12 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
 #pragma unroll
                             for (int x = 0; x < 4; ++x) c[sub][nt][x] += c2[nt][x];
                         if constexpr (S::KIND == CACHE_I8_ROWS) {
-                            const float mine = __half2float(__ushort_as_half((unsigned short)k_scale_now)) * (p.scale_log2 * 0x1p24f);
+                            const float mine = __half2float(__ushort_as_half((unsigned short)k_scale_now)) * p.scale_log2;
                             const float k0 = __shfl_sync(0xffffffffu, mine, 16 * sub + g), k1 = __shfl_sync(0xffffffffu, mine, 16 * sub + g + 8);
 #pragma unroll
                             for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
-                                for (int x = 0; x < 4; ++x) c[sub][nt][x] = (c[sub][nt][x] - bias[nt][x & 1]) * (x < 2 ? k0 : k1);
+                                for (int x = 0; x < 4; ++x) c[sub][nt][x] *= x < 2 ? k0 : k1;
                         } else {
 #pragma unroll
                             for (int nt = 0; nt < S::NT; ++nt)
@@ -934,7 +916,6 @@ int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb2
     p.tiles = (p.shared + heads - 1) / heads;
     p.window = a->window; p.scale_log2 = a->scale * 1.4426950408889634f;
     p.cache = *cache;
-    p.flip = 0x00800080u;
     p.flip_1024 = 0x64806480u;
     static std::atomic<uint64_t> calls{0};
     p.call = ++calls;
