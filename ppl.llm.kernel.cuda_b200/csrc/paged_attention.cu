@@ -54,10 +54,6 @@ struct Shape {
     // Registers for the sums, the queries and the tokens on their way decide how many CTAs share an SM (groups of 8, 128 dimensions: 66 us
     // with four, 69 with three).
     static constexpr int WORDS = NT * D / 4 + NT * D / 8 + SUBS * (D * ES / 4 + (KIND == CACHE_I8_GROUPS ? 2 * KN + 4 * VN : 0));
-    // Weights enter their product in fp16 and, as a second operand, what that rounding left: 22 bits.  Not with int8 rows, where the rest of
-    // the kernel draws the most power: their roundings, 2^-12 each, add up to half of what the output's own does, and without the second
-    // operand 64 x 8192 tokens take 110 us instead of 115, and over seconds, at the power limit, 124 instead of 131.
-    static constexpr bool EXACT = KIND != CACHE_I8_ROWS;
     static constexpr int ROW = D + 4; // of the sums that the warps exchange
     static constexpr int WARPS = 4, THREADS = 32 * WARPS, CTAS = WORDS <= 88 ? 4 : WORDS <= 128 ? 3 : 2;
 };
@@ -592,7 +588,9 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                 }
 #pragma unroll
                 for (int sub = 0; sub < S::SUBS; ++sub) {
-                    uint32_t wh[S::NT][2], wl[S::NT][2]; // weights in fp16, and what the rounding left
+                    // Weights in fp16 and, as a second operand, what that rounding left: 22 bits.  The second operand costs int8 rows, where the rest
+                    // draws the most power, 5 % (64 x 8192 tokens 111 us without it, 116 with it), the other caches 2 % at most.
+                    uint32_t wh[S::NT][2], wl[S::NT][2];
 #pragma unroll
                     for (int nt = 0; nt < S::NT; ++nt) {
                         float w[4];
@@ -608,10 +606,8 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                         for (int r = 0; r < 2; ++r) {
                             const __half2 x = __floats2half2_rn(w[2 * r], w[2 * r + 1]);
                             wh[nt][r] = transpose8x8(h2(x));
-                            if constexpr (S::EXACT) {
-                                const float2 f = __half22float2(x);
-                                wl[nt][r] = transpose8x8(h2(__floats2half2_rn(w[2 * r] - f.x, w[2 * r + 1] - f.y)));
-                            }
+                            const float2 f = __half22float2(x);
+                            wl[nt][r] = transpose8x8(h2(__floats2half2_rn(w[2 * r] - f.x, w[2 * r + 1] - f.y)));
                         }
                     }
 
@@ -649,7 +645,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
 #pragma unroll
                                     for (int nt = 0; nt < S::NT; ++nt) {
                                         mma(o[nt][i * EP / 2 + 2 * x + y], u[2 * y], u[2 * y + 1], v[2 * y], v[2 * y + 1], wh[nt][0], wh[nt][1]);
-                                        if constexpr (S::EXACT) mma(o[nt][i * EP / 2 + 2 * x + y], u[2 * y], u[2 * y + 1], v[2 * y], v[2 * y + 1], wl[nt][0], wl[nt][1]);
+                                        mma(o[nt][i * EP / 2 + 2 * x + y], u[2 * y], u[2 * y + 1], v[2 * y], v[2 * y + 1], wl[nt][0], wl[nt][1]);
                                     }
                             }
                         }

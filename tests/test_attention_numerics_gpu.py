@@ -44,3 +44,39 @@ def test_scores_beside_a_dimension_that_the_query_does_not_see(cuda, pplb200, d,
     # d products and d - 1 sums in 32 bits, in any order; scale, scale * log2(e), their product with a row's scale and with the sum, back to
     # natural logarithms (three of those); beside them the difference to and from the reference exponent, 8 away
     assert bool(((lse.double() - score).abs() <= size * (d + 8) * 2.0 ** -24 + 2.0 ** -20).all())
+
+
+@pytest.mark.parametrize("d,shared", [(64, 1), (96, 3), (128, 1), (128, 16), (256, 2)])
+@pytest.mark.parametrize("group", [0, 8, -1])
+def test_weights_keep_22_bits(cuda, pplb200, d, shared, group):
+    """Tokens in pairs whose weighted values nearly cancel: what a rounding of the weights leaves is not hidden by the output's own.  Keys
+    with one dimension, so that scores are exact products; values of whole numbers times a power of two, so that no cache rounds them."""
+    group = d if group < 0 else group
+    hk, lengths, page = 8, [2, 4, 8, 32], 16
+    g = _gen(cuda, d + shared)
+    n = sum(lengths)
+    q = cuda.zeros((1, hk * shared, d), dtype=cuda.float16, device="cuda")
+    q[..., 1] = 4.0
+    a = cuda.rand((n // 2, hk), generator=g, device="cuda", dtype=cuda.float64) - 0.5
+    m = cuda.randint(64, 128, (2, n // 2, hk), generator=g, device="cuda").double()
+    sign = (cuda.randint(0, 2, (1, hk, d), generator=g, device="cuda") * 2 - 1).double()
+    k, v = cuda.zeros((n, hk, d), dtype=cuda.float64, device="cuda"), cuda.empty((n, hk, d), dtype=cuda.float64, device="cuda")
+    k[0::2, :, 1] = a
+    k[1::2, :, 1] = a + (m[0] / m[1]).log() / 4  # e^(4 k) m is the same for both
+    v[0::2], v[1::2] = m[0][..., None] * sign / 64, -m[1][..., None] * sign / 64
+    v[..., 7::8] = 127 / 64  # the largest of every group, so that its scale is a power of two
+    k, v = k.to(cuda.float16), v.to(cuda.float16)
+    cache = _cache(cuda, pplb200, 8, page, hk, d, group, "heads", 0)
+    pages = cuda.tensor([[0, 0], [1, 1], [2, 2], [3, 4]], dtype=cuda.int32, device="cuda")
+    slots = [pages[b].long()[cuda.arange(c, device="cuda") // page] * page + cuda.arange(c, device="cuda") % page for b, c in enumerate(lengths)]
+    pplb200.kv_cache_write(cache, k, v, cuda.cat(slots))
+    att = pplb200.PagedDecodeAttention(cache, hk * shared, 4, 2 * page, scale=1.0)
+    out = att(q.expand(4, -1, -1).contiguous(), pages, cuda.tensor(lengths, dtype=cuda.int32, device="cuda")).double()
+    for b, c in enumerate(lengths):
+        keys, values = _stored(cuda, cache, slots[b])
+        p = cuda.softmax(4 * keys[..., 1], 0)
+        want, size = (cuda.einsum("th,thd->hd", p, x).repeat_interleave(shared, 0) for x in (values, values.abs()))
+        # scores up to 4: four roundings of six, two of up to sixteen, 2^-22 of the power of two, 2^-22 left of the weight: below 2^-18,
+        # twice, since the weights' sum has it too; c sums in 32 bits, cut off rather than rounded, in both; joining the warps' sums
+        bound = size * (2.0 ** -17 + c * 2.0 ** -22 + 2.0 ** -21) + want.abs() * HALF + TINY
+        assert bool(((out[b] - want).abs() <= bound).all()), c
