@@ -537,8 +537,9 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                 // ---- weights: 2^(score - top + 8) --------------------------------------------------------------------------
                 float v0[S::SUBS], v1[S::SUBS], e0[S::SUBS] = {}, e1[S::SUBS] = {};
                 if constexpr (S::KIND == CACHE_I8_ROWS) {
-                    // a value's scale goes into its weight, the scale's logarithm into what decides about the reference exponent
-                    const float mine = __half2float(__ushort_as_half((unsigned short)v_scale)), size = fmaxf(log2_fast(fabsf(mine)), -24.0f);
+                    // a value's scale goes into its weight, the scale's logarithm into what decides about the reference exponent; an infinite one only as
+                    // far as a finite one could: the sum of the weights, of which the lse is made, is no affair of the values
+                    const float mine = __half2float(__ushort_as_half((unsigned short)v_scale)), size = fminf(fmaxf(log2_fast(fabsf(mine)), -24.0f), 16.0f);
 #pragma unroll
                     for (int sub = 0; sub < S::SUBS; ++sub) {
                         v0[sub] = __shfl_sync(0xffffffffu, mine, 16 * sub + g);

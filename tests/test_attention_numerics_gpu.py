@@ -80,3 +80,46 @@ def test_weights_keep_22_bits(cuda, pplb200, d, shared, group):
         # twice, since the weights' sum has it too; c sums in 32 bits, cut off rather than rounded, in both; joining the warps' sums
         bound = size * (2.0 ** -17 + c * 2.0 ** -22 + 2.0 ** -21) + want.abs() * HALF + TINY
         assert bool(((out[b] - want).abs() <= bound).all()), c
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("group", [0, 8, 128])
+@pytest.mark.parametrize("n", [40, 5000])
+def test_what_a_value_is_does_not_reach_the_lse(cuda, pplb200, value, group, n):
+    """An infinity or NaN among the values: its dimensions (those that share its scale) of its heads' output are lost, and nothing else."""
+    d, page = 128, 16
+    g = _gen(cuda, n)
+    cache = _cache(cuda, pplb200, -(-n // page), page, 2, d, group, "heads", 0)
+    k, v, q = _randn(cuda, g, n, 2, d), _randn(cuda, g, n, 2, d), _randn(cuda, g, 6, d)
+    at = cuda.arange(n, device="cuda")
+    pplb200.kv_cache_write(cache, k, v, at)
+    out, lse, scale = _one_sequence(cuda, pplb200, cache, q, n)
+    v[n - 3, 1, 21] = value
+    pplb200.kv_cache_write(cache, k, v, at)
+    lost, same, _ = _one_sequence(cuda, pplb200, cache, q, n)
+    keys = _stored(cuda, cache, at)[0].repeat_interleave(3, 1)
+    score, size = cuda.einsum("hd,thd->ht", q.double(), keys) * scale, cuda.einsum("hd,thd->ht", q.double().abs(), keys.abs()).amax(-1) * scale
+    # a score's products and sums and its factors, and n sums of weights, all in 32 bits
+    bound = size * (d + 8) * 2.0 ** -24 + 2.0 ** -20 + n * 2.0 ** -23
+    for x in (lse, same):
+        assert bool(((x - cuda.logsumexp(score, -1)).abs() <= bound).all())
+    odd = cuda.zeros_like(out, dtype=cuda.bool)
+    first = 21 // max(group, 1) * max(group, 1)
+    odd[3:, first:first + max(group, 1)] = True
+    assert cuda.equal(~cuda.isfinite(lost), odd) and cuda.equal(lost[~odd], out[~odd])
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("group", [8, 128])
+def test_a_lost_key_is_not_left_out(cuda, pplb200, value, group):
+    """Keys that read back as NaN make their heads' output and lse NaN, whatever the query's signs."""
+    d, n, page = 128, 50, 16
+    for seed in range(8):
+        g = _gen(cuda, seed)
+        cache = _cache(cuda, pplb200, 4, page, 2, d, group, "heads", 0)
+        k, v, q = _randn(cuda, g, n, 2, d), _randn(cuda, g, n, 2, d), _randn(cuda, g, 16, d, scale=30.0)
+        k[7 * seed % n, 0, 3] = value
+        pplb200.kv_cache_write(cache, k, v, cuda.arange(n, device="cuda"))
+        out, lse, _ = _one_sequence(cuda, pplb200, cache, q, n)
+        assert bool(out[:8].isnan().all()) and bool(lse[:8].isnan().all())
+        assert bool(cuda.isfinite(out[8:]).all()) and bool(cuda.isfinite(lse[8:]).all())
