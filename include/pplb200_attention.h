@@ -112,7 +112,8 @@ int32_t pplb200_kv_cache_read_fp16(pplb200_stream_t stream, const pplb200_kv_cac
  * cache, the new one among them (at most pages_per_sequence * page_size are looked at); pages int32 [batch, pages_per_sequence] with
  * pages_stride between rows: the page of token t is pages[b, t / page_size].  A page that is negative or not below num_pages is a
  * hole: its tokens take no part.  window > 0: only the last `window` tokens do.  What lies in the cache beyond a sequence's
- * tokens has no influence, whatever it is.  A sequence of which nothing is seen has zeros for its output and -inf for its lse.
+ * tokens has no influence, whatever it is.  A sequence of which nothing is seen has zeros for its output and -inf for its lse; one whose
+ * tokens are seen, but have scores of -inf only, NaN and -inf.
  * optional_lse fp32 [batch, q_heads], contiguous: log(sum_t exp(scale q . k_t)), for joining results over parts of a context.
  * head_dim 64, 96, 128 or 256 (with quant_group 8: scales 4-byte aligned, their strides even); q_heads a multiple of kv_heads; strides
  * multiples of 8; q and out 16-byte aligned; out may be q; scale within 2^50 of zero; at most 2^30 tokens a row of the table.

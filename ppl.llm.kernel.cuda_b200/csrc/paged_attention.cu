@@ -175,9 +175,13 @@ struct Share { // where a CTA's share begins or ends: a step of a head of a sequ
     int32_t head, step;
 };
 
+// The reference exponent of a head before its first token.  Where there was one, it ends above that, even if all scores were minus infinity: their
+// quotient is NaN, while nothing at all gives zeros.
+constexpr float kNothingSeen = -1e30f, kLowest = -0.5e30f;
+
 // Output of one query head, dimensions d to d + 3, from sums in units of 2^top.
 __device__ __forceinline__ void finish(const AttentionParams& p, int64_t b, int32_t head, int32_t dims, int32_t d, const float4& v, float top, float sum) {
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = sum != 0.0f ? 1.0f / sum : top > kNothingSeen ? __int_as_float(0x7fffffff) : 0.0f;
     const uint2 r = make_uint2(h2(__floats2half2_rn(v.x * inv, v.y * inv)), h2(__floats2half2_rn(v.z * inv, v.w * inv)));
     *reinterpret_cast<uint2*>(p.out + b * p.out_stride + (int64_t)head * dims + d) = r;
     if (p.lse && d == 0) p.lse[b * p.q_heads + head] = sum == 0.0f ? -INFINITY : (top - 8.0f + log2f(sum)) * 0.69314718055994531f;
@@ -455,7 +459,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
 
         float o[S::NT][S::STEPS][4] = {}, top[S::NT][2], sum[S::NT][2] = {};
 #pragma unroll
-        for (int nt = 0; nt < S::NT; ++nt) top[nt][0] = top[nt][1] = -1e30f;
+        for (int nt = 0; nt < S::NT; ++nt) top[nt][0] = top[nt][1] = kNothingSeen;
 
         for (int32_t step = step0 + warp; step < step1; step += WARPS) {
             float c[S::SUBS][S::NT][4];
@@ -666,15 +670,26 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
         }
 
         // ---- the warps' sums -------------------------------------------------------------------------------------------------
+        bool none = false, met = false; // no weight at all: were there tokens?  Looked up again, since a register for it in the loop costs 1 %
+#pragma unroll
+        for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) sum[nt][k] += __shfl_xor_sync(0xffffffffu, sum[nt][k], x);
+                none |= sum[nt][k] == 0.0f;
+            }
+        if (__any_sync(0xffffffffu, none))
+            for (int32_t step = step0 + warp; step < step1 && !met; step += WARPS) {
+                locate(find(step), step);
+                met = coming != 0;
+            }
 #pragma unroll
         for (int nt = 0; nt < S::NT; ++nt) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                float s = sum[nt][k];
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
                 const int h = nt * 8 + 2 * t + k;
-                if (g == 0) tops[warp * S::HEADS + h] = make_float2(top[nt][k], s);
+                if (g == 0) tops[warp * S::HEADS + h] = make_float2(met ? fmaxf(top[nt][k], kLowest) : top[nt][k], sum[nt][k]);
                 constexpr int EP = S::VP / S::ES;
 #pragma unroll
                 for (int i = 0; i < S::VN; ++i)
@@ -690,7 +705,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
         const int head0 = kvh * p.shared + q_first;
         for (int x = threadIdx.x; x < q_count * (S::D / 4); x += S::THREADS) {
             const int h = x / (S::D / 4), d = (x - h * (S::D / 4)) * 4;
-            float m = -1e30f, l = 0.0f;
+            float m = kNothingSeen, l = 0.0f;
             float4 v = make_float4(0, 0, 0, 0);
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) m = fmaxf(m, tops[w * S::HEADS + h].x);
@@ -749,7 +764,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
 #pragma unroll
                 for (int x = 0; x < ITEMS; ++x) {
                     v[x] = make_float4(0, 0, 0, 0);
-                    m[x] = -1e30f;
+                    m[x] = kNothingSeen;
                     l[x] = 0.0f;
                 }
                 for (int32_t i = 0; i < number; i += BATCH) {

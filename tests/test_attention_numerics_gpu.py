@@ -123,3 +123,36 @@ def test_a_lost_key_is_not_left_out(cuda, pplb200, value, group):
         out, lse, _ = _one_sequence(cuda, pplb200, cache, q, n)
         assert bool(out[:8].isnan().all()) and bool(lse[:8].isnan().all())
         assert bool(cuda.isfinite(out[8:]).all()) and bool(cuda.isfinite(lse[8:]).all())
+
+
+@pytest.mark.parametrize("lengths", [[1], [20, 0, 3], [4000]])
+def test_scores_of_minus_infinity_only(cuda, pplb200, lengths):
+    """Tokens that are seen, but whose scores are all minus infinity: their sum is zero, as the definition has it, and the quotient NaN; zeros
+    are for sequences of which nothing is seen.  Beside finite scores such tokens have no weight."""
+    d, page = 128, 16
+    g = _gen(cuda, 2)
+    width = -(-max(lengths) // page)
+    cache = _cache(cuda, pplb200, width, page, 1, d, 0, "heads", 0)
+    n = width * page
+    v = _randn(cuda, g, n, 1, d)
+    k = cuda.zeros_like(v)
+    k[..., 9], k[..., 10] = math.inf, 0.5
+    pplb200.kv_cache_write(cache, k, v, cuda.arange(n, device="cuda"))
+    q = cuda.ones((len(lengths), 3, d), dtype=cuda.float16, device="cuda")
+    q[:, :, 9] = -1.0
+    q[:, 0, 10] = 0.0
+    pages = cuda.arange(width, dtype=cuda.int32, device="cuda").expand(len(lengths), -1)
+    lens = cuda.tensor(lengths, dtype=cuda.int32, device="cuda")
+    att = pplb200.PagedDecodeAttention(cache, 3, len(lengths), n, scale=1.0)
+    lse = cuda.empty((len(lengths), 3), device="cuda")
+    out = att(q, pages.contiguous(), lens, lse=lse)
+    assert bool((lse == -math.inf).all())
+    for b, c in enumerate(lengths):
+        assert bool(out[b].isnan().all()) if c else not bool(out[b].any())
+    cache.k[0, 0, 0, 9] = 0.0  # one token's score is finite
+    out = att(q, pages.contiguous(), lens, lse=lse)
+    for b, c in enumerate(lengths):
+        assert not bool(out[b].any()) if c == 0 else bool((out[b] == cache.v[0, 0, 0]).all())
+        want = cuda.tensor([0.0, 0.5, 0.5] if c else [-math.inf] * 3, device="cuda")
+        # 0.5 by way of base 2: the factor, the product, 8 off and on, and back, each rounded to 32 bits
+        assert cuda.equal(lse[b], want) or bool(((lse[b] - want).abs() <= 2.0 ** -20).all())
