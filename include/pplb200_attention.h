@@ -106,7 +106,8 @@ int32_t pplb200_kv_cache_read_fp16(pplb200_stream_t stream, const pplb200_kv_cac
 /*
  * Attention of one new token per sequence: out[b, h] = sum_t softmax_t(scale q[b, h] . k_t) v_t over the tokens t of sequence b in
  * head h / (q_heads / kv_heads) of the cache: the stored values, or values x scales, which are not rounded to fp16 in between, except
- * v with groups of 8, which is.  Scores, sums and statistics are held in 32 bits; the softmax's weights enter their product with v
+ * v with groups of 8, which is.  With groups of 8 a value x scale beyond fp16's range, which no scale up to 515.5 reaches (the writer's largest), is
+ * infinite as v and makes its token's score NaN as k; rows that share a scale a head take any finite one.  Scores, sums and statistics are held in 32 bits; the softmax's weights enter their product with v
  * with 22 bits.
  * q, out fp16 [batch, q_heads, head_dim], *_stride elements between sequences, heads contiguous; lengths int32 [batch]: tokens in the
  * cache, the new one among them (at most pages_per_sequence * page_size are looked at); pages int32 [batch, pages_per_sequence] with

@@ -501,7 +501,8 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                                     uint32_t a0, a1, a2, a3;
                                     widen(p, kw[sub][0][i][s], a0, a2);
                                     widen(p, kw[sub][1][i][s], a1, a3);
-                                    // value x scale has up to 18 bits: its rounding to fp16, and what that left, as a second operand
+                                    // value x scale has up to 18 bits: its rounding to fp16, and what that left, as a second operand (beyond fp16's range, inf
+                                    // and -inf: NaN, not a wrong score)
                                     const __half2 f0 = as_h2(__byte_perm(ks[sub][0][i], 0, s < 2 ? 0x1010 : 0x3232)), f1 = as_h2(__byte_perm(ks[sub][1][i], 0, s < 2 ? 0x1010 : 0x3232));
                                     const __half2 h0 = __hmul2(as_h2(a0), f0), h1 = __hmul2(as_h2(a1), f1), h2_ = __hmul2(as_h2(a2), f0), h3 = __hmul2(as_h2(a3), f1);
                                     const uint32_t r0 = h2(__hfma2(as_h2(a0), f0, __hneg2(h0))), r1 = h2(__hfma2(as_h2(a1), f1, __hneg2(h1)));

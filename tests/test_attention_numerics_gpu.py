@@ -156,3 +156,57 @@ def test_scores_of_minus_infinity_only(cuda, pplb200, lengths):
         want = cuda.tensor([0.0, 0.5, 0.5] if c else [-math.inf] * 3, device="cuda")
         # 0.5 by way of base 2: the factor, the product, 8 off and on, and back, each rounded to 32 bits
         assert cuda.equal(lse[b], want) or bool(((lse[b] - want).abs() <= 2.0 ** -20).all())
+
+
+def _foreign(cuda, pplb200, n, hk, d, group, k_scale, v_scale, seed):
+    """A cache that another program filled: any whole numbers, scales [n, hk, d / group] (sizes; their signs are drawn)."""
+    g = _gen(cuda, seed)
+    cache = _cache(cuda, pplb200, -(-n // 16), 16, hk, d, group, "heads", 0)
+    at = cuda.arange(n, device="cuda")
+    for x, s, size in ((cache.k, cache.k_scale, k_scale), (cache.v, cache.v_scale, v_scale)):
+        x.copy_(cuda.randint(-127, 128, x.shape, generator=g, device="cuda"))
+        sign = cuda.randint(0, 2, size.shape, generator=g, device="cuda") * 2 - 1
+        s[at // 16, :, at % 16] = (size * sign).to(cuda.float16)
+    return cache
+
+
+def _check(cuda, cache, out, lse, q, n, scale, group, extra=0.0):
+    """Against the definition; group: of the cache, 8: values are rounded to fp16.  extra [hq]: of the weights' products with values' scales."""
+    shared = q.shape[0] // cache.kv_heads
+    k, v = (x.repeat_interleave(shared, 1) for x in _stored(cuda, cache, cuda.arange(n, device="cuda")))
+    score = cuda.einsum("hd,thd->ht", q.double(), k) * scale
+    p = cuda.softmax(score, -1)
+    want, size = cuda.einsum("ht,thd->hd", p, v), cuda.einsum("ht,thd->hd", p, v.abs())
+    # a score as above; a weight: twice that, 22 bits, n sums in 32 bits in it and in the product with values
+    off = cuda.einsum("hd,thd->ht", q.double().abs(), k.abs()).amax(-1) * abs(scale) * (q.shape[1] + 8) * 2.0 ** -24 + 2.0 ** -20
+    weight = 2 * off + n * 2.0 ** -22 + 2.0 ** -20 + (HALF if group == 8 else 0)
+    bound = weight[:, None] * size * (1 + HALF) + (want.abs() * HALF + 2 * TINY) + extra
+    assert bool(((out - want).abs() <= bound).all())
+    assert bool(((lse - cuda.logsumexp(score, -1)).abs() <= off + n * 2.0 ** -23).all())
+
+
+@pytest.mark.parametrize("group", [8, 128])
+def test_scales_up_to_the_largest(cuda, pplb200, group):
+    """Keys and values of the largest steps that the writer stores, 515.5; rows that share a scale take larger keys as well."""
+    n, d = 200, 128
+    for k_size, v_size in ((515.5, 1.0), (1e-3, 515.5)) + (((60000.0, 1.0),) if group == d else ()):
+        scales = [cuda.full((n, 1, d // group), x, device="cuda") for x in (k_size, v_size)]
+        cache = _foreign(cuda, pplb200, n, 1, d, group, *scales, 3)
+        q = _randn(cuda, _gen(cuda, 4), 3, d)
+        out, lse, scale = _one_sequence(cuda, pplb200, cache, q, n, scale=0.05 / k_size)
+        _check(cuda, cache, out, lse, q, n, scale, group)
+
+
+def test_products_beyond_fp16_are_not_silent(cuda, pplb200):
+    """Groups of 8: a key beyond fp16's range makes its heads NaN, and no other's; a small number of large steps is a key like any."""
+    n, d = 50, 128
+    scales = cuda.full((n, 2, d // 8), 0.01, device="cuda")
+    cache = _foreign(cuda, pplb200, n, 2, d, 8, scales, scales, 5)
+    cache.k_scale[1, 0, 4, 3], cache.k[1, 0, 4, 24:32] = 4000.0, 16
+    q = _randn(cuda, _gen(cuda, 6), 4, d) * 0.01
+    out, lse, scale = _one_sequence(cuda, pplb200, cache, q, n)
+    _check(cuda, cache, out, lse, q, n, scale, 8)
+    cache.k[1, 0, 4, 25] = 17
+    lost, lost_lse, _ = _one_sequence(cuda, pplb200, cache, q, n)
+    assert bool(lost[:2].isnan().all()) and bool(lost_lse[:2].isnan().all())
+    assert cuda.equal(lost[2:], out[2:]) and cuda.equal(lost_lse[2:], lse[2:])
