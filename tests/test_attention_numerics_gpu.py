@@ -6,7 +6,7 @@ import math
 
 import pytest
 
-from test_attention_gpu import HALF, TINY, _cache, _gen, _randn, _stored
+from test_attention_gpu import HALF, TINY, _cache, _check_attention, _gen, _randn, _run_attention, _stored
 
 pytestmark = pytest.mark.gpu
 
@@ -185,6 +185,31 @@ def _check(cuda, cache, out, lse, q, n, scale, group, extra=0.0):
     assert bool(((lse - cuda.logsumexp(score, -1)).abs() <= off + n * 2.0 ** -23).all())
 
 
+@pytest.mark.parametrize("n", [37, 3000])
+def test_rows_whose_scales_differ_by_all_of_fp16(cuda, pplb200, n):
+    """Values whose scales span fp16, from one token to the next and zeros among them, while the weights span as much the other way: the
+    reference exponent follows their product."""
+    d, hk = 128, 2
+    g = _gen(cuda, n)
+    u = cuda.rand((n, hk, 1), generator=g, device="cuda")
+    v_scale = cuda.exp2(40 * u - 24).clamp_max(1000.0)
+    v_scale[cuda.rand((n, hk, 1), generator=g, device="cuda") < 0.1] = 0.0
+    cache = _foreign(cuda, pplb200, n, hk, d, d, cuda.full((n, hk, 1), 1e-2, device="cuda"), v_scale, n)
+    cache.v.clamp_(-60, 60)  # of 1000: within fp16 on output
+    # a dimension that raises the score of tokens with small scales
+    at = cuda.arange(n, device="cuda")
+    cache.k[at // 16, :, at % 16, 0] = (127 * (1 - 2 * u[..., 0])).round().to(cuda.int8)
+    q = _randn(cuda, g, 6, d) * 0.1
+    q[:, 0] = cuda.tensor([0.0, 12.0, -12.0, 6.0, 20.0, -3.0])
+    out, lse, scale = _one_sequence(cuda, pplb200, cache, q, n, scale=1.0)
+    k, v = _stored(cuda, cache, at)
+    p = cuda.softmax(cuda.einsum("hd,thd->ht", q.double(), k.repeat_interleave(3, 1)), -1)
+    s = cache.v_scale[at // 16, :, at % 16, 0].double().abs().T.repeat_interleave(3, 0)
+    # what is left of weight x scale is rounded at 2^-25 where the largest is 2^8 at least: of every token, times up to 60 steps
+    extra = (n * 60 * 2.0 ** -33 * (p * s).amax(-1))[:, None]
+    _check(cuda, cache, out, lse, q, n, scale, d, extra)
+
+
 @pytest.mark.parametrize("group", [8, 128])
 def test_scales_up_to_the_largest(cuda, pplb200, group):
     """Keys and values of the largest steps that the writer stores, 515.5; rows that share a scale take larger keys as well."""
@@ -210,3 +235,38 @@ def test_products_beyond_fp16_are_not_silent(cuda, pplb200):
     lost, lost_lse, _ = _one_sequence(cuda, pplb200, cache, q, n)
     assert bool(lost[:2].isnan().all()) and bool(lost_lse[:2].isnan().all())
     assert cuda.equal(lost[2:], out[2:]) and cuda.equal(lost_lse[2:], lse[2:])
+
+
+@pytest.mark.parametrize("scale,q_scale", [(None, 20.0), (1.0, 8.0), (0.0, 1.0), (-0.1, 2.0), (1e-6, 1.0)])
+@pytest.mark.parametrize("hq", [2, 32])
+def test_rows_scores_of_all_sizes(cuda, pplb200, scale, q_scale, hq):
+    """Softmaxes between uniform and one-hot over int8 rows, scores of some hundreds."""
+    _check_attention(*_run_attention(cuda, pplb200, [1500, 40, 333], hq, 2, 128, 16, 128, scale=scale, q_scale=q_scale)[:3])
+
+
+@pytest.mark.parametrize("group", [8, 128])
+@pytest.mark.parametrize("size", [60000.0, 1e-4, 1e-6])
+def test_int8_values_of_all_sizes(cuda, pplb200, group, size):
+    """Values near the largest and the smallest of fp16, whose scales are the largest and subnormal: nothing overflows or vanishes."""
+    n, d = 300, 128
+    g = _gen(cuda, 2)
+    cache = _cache(cuda, pplb200, 20, 16, 1, d, group, "heads", 0)
+    v = (cuda.rand((n, 1, d), generator=g, device="cuda") * size).to(cuda.float16)
+    pplb200.kv_cache_write(cache, _randn(cuda, g, n, 1, d), v, cuda.arange(n, device="cuda"))
+    q = _randn(cuda, g, 2, d)
+    out, lse, scale = _one_sequence(cuda, pplb200, cache, q, n)
+    _check(cuda, cache, out, lse, q, n, scale, group)
+
+
+@pytest.mark.parametrize("group", [8, 128])
+def test_int8_special_values_out_of_sight(cuda, pplb200, group):
+    """NaN scales outside the window, behind the length and in another sequence's pages have no influence."""
+    out, lse, want, (att, q, table, lens, cache) = _run_attention(cuda, pplb200, [100, 100, 50], 8, 2, 128, 16, group, window=40)
+    _check_attention(out, lse, want)
+    nan = float("nan")
+    cache.k_scale[int(table[1, 1]), :, 3], cache.v_scale[int(table[1, 1]), :, 3] = nan, nan    # token 19 of 100: outside the window
+    cache.k_scale[int(table[2, 3]), :, 10], cache.v_scale[int(table[2, 3]), :, 10] = nan, nan  # token 58 of 50
+    cache.v_scale[int(table[0, 6]), 1, 1] = nan                                                # token 97 of 100: seen
+    got = att(q, table, lens)
+    assert cuda.equal(got[1:], out[1:]) and cuda.equal(got[0, :4], out[0, :4])
+    assert bool(got[0, 4:].isnan().all())
