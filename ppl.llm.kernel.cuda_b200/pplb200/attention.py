@@ -145,10 +145,11 @@ class PagedKVCache(_LaidOutOnce):
         _need(quant_group in (0, 8, head_dim), "quant_group must be 0, 8 or head_dim")
         k, v = (torch.zeros((num_pages, kv_heads, page_size, head_dim), dtype=torch.int8 if quant_group else torch.float16, device=device)
                 for _ in range(2))
-        if not quant_group:
-            return cls(k, v)
-        return cls(k, v, *(torch.zeros((num_pages, kv_heads, page_size, head_dim // quant_group), dtype=torch.float16, device=device)
-                           for _ in range(2)))
+        scales = (torch.zeros((num_pages, kv_heads, page_size, head_dim // quant_group), dtype=torch.float16, device=device)
+                  for _ in range(2 if quant_group else 0))
+        cache = cls(k, v, *scales)
+        _settle(k.device)
+        return cache
 
 
 def kv_cache_write(cache, k, v, slots):

@@ -349,3 +349,13 @@ def test_binding_describes_the_cache():
                 lambda: pplb200.PagedKVCache(k[..., ::2], v[..., ::2], ks, vs), lambda: pplb200.PagedKVCache.allocate(1, 1, 1, 64, 16, device="cpu")):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("group", [0, 8, 64])
+def test_an_allocated_cache_is_there_before_its_first_call(monkeypatch, group):
+    import pplb200
+    from pplb200 import attention
+    settled = []
+    monkeypatch.setattr(attention, "_settle", settled.append)
+    cache = pplb200.PagedKVCache.allocate(10, 16, 1, 64, group, device="cpu")
+    assert settled == [cache.k.device]

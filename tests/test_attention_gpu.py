@@ -694,3 +694,22 @@ def test_a_layers_decode_step(cuda, pplb200):
         _check_attention(out[b:b + 1], None, [_attention(cuda, qr[b], kr, vr, at >= 0, att.scale, True)])
     oq, os_ = pplb200.minmax_quantize_fp16(out.view(M, hq * d))
     assert cuda.equal(y, pplb200.gemm_i8i8(oq, wo, pplb200.EPI_DEQUANT_F16, os_, sno)) and bool(cuda.isfinite(y).all()) and pplb200.gemm_status() == 0
+
+
+@pytest.mark.parametrize("group", [0, 8, 128])
+def test_an_allocated_cache_may_be_written_on_any_stream(cuda, pplb200, group):
+    """The cache is zeroed on a stream that is busy for a while; what another stream stores meanwhile is not zeroed after it."""
+    side, busy = cuda.cuda.Stream(), cuda.ones((4096, 4096), dtype=cuda.float16, device="cuda")
+    k, slots = cuda.ones((64, 2, 128), dtype=cuda.float16, device="cuda"), cuda.arange(64, device="cuda")
+
+    def stored():
+        cache = pplb200.PagedKVCache.allocate(4, 16, 2, 128, group)
+        with cuda.cuda.stream(side):
+            pplb200.kv_cache_write(cache, k, k, slots)
+        cuda.cuda.synchronize()
+        return bool((cache.k != 0).all()) and bool((cache.v != 0).all()) and all(t is None or bool((t != 0).all()) for t in (cache.k_scale, cache.v_scale))
+
+    stored()  # memory and kernels are at hand after this
+    for _ in range(100):
+        busy @ busy
+    assert stored()
