@@ -678,5 +678,18 @@ def stream_read_probe(sizes=(16 << 20, 48 << 20, 384 << 20), pool_bytes=1536 << 
     return out
 
 
-from .attention import (PagedDecodeAttention, PagedKVCache, RotaryTable, kv_cache_read, kv_cache_write,  # noqa: E402,F401
-                        rotary_fp16, rotary_kv_cache_write)
+_ATTENTION = ("PagedDecodeAttention", "PagedKVCache", "RotaryTable", "kv_cache_read", "kv_cache_write", "rotary_fp16", "rotary_kv_cache_write")
+
+
+def __getattr__(name):
+    """The names of attention.py, which needs torch and the compiled part of the binding: loaded when one of them is first asked for."""
+    if name != "attention" and name not in _ATTENTION:
+        raise AttributeError("module %r has no attribute %r" % (__name__, name))
+    import importlib
+    module = importlib.import_module(__name__ + ".attention")
+    globals().update((n, getattr(module, n)) for n in _ATTENTION)
+    return module if name == "attention" else globals()[name]
+
+
+def __dir__():
+    return sorted(set(globals()) | set(_ATTENTION))
