@@ -8,6 +8,7 @@ import ctypes
 import importlib.util
 import os
 import struct
+import sys
 
 import torch
 
@@ -33,10 +34,15 @@ lib.pplb200_kv_cache_offset.restype = _i64
 _pack_cache = struct.Struct("=4Q7q4i").pack
 
 
+def binding_path():
+    """Compiled for this Python and this torch, as build.py names it."""
+    return os.path.join(os.path.dirname(LIB_PATH), "pplb200_attention_binding.%s.torch-%s.so" % (sys.implementation.cache_tag, torch.__version__))
+
+
 def _load_binding():
-    path = os.path.join(os.path.dirname(LIB_PATH), "pplb200_attention_binding.so")
+    path = binding_path()
     if not os.path.exists(path):
-        raise ImportError("pplb200_attention_binding.so is not built (%s); run `python ppl.llm.kernel.cuda_b200/build.py`." % os.path.normpath(path))
+        raise ImportError("the compiled part of the binding is not built (%s); run `python ppl.llm.kernel.cuda_b200/build.py`." % os.path.normpath(path))
     spec = importlib.util.spec_from_file_location("pplb200_attention_binding", os.path.normpath(path))
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)

@@ -65,3 +65,38 @@ try:
 except AttributeError as e:
     assert "no_such_name" in str(e)
 """)
+
+
+def _build_module():
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("pplb200_build_under_test", os.path.join(PKG, "build.py"))
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def test_another_torch_or_python_has_a_binding_of_its_own(monkeypatch):
+    """The binding is compiled for one torch and one Python: it is built anew for others, and never loaded by them."""
+    import torch
+    import pplb200.attention
+    build, commands = _build_module(), []
+    here = build.binding_path()
+    assert here == os.path.normpath(pplb200.attention.binding_path()) and os.path.exists(here) and torch.__version__ in here
+    monkeypatch.setattr(build.subprocess, "run", lambda cmd, **kw: commands.append(cmd))
+    monkeypatch.setattr(build, "_stale", lambda target, deps: not os.path.exists(target))
+    build.build()
+    assert not commands
+    monkeypatch.setattr(build, "torch_version", lambda: "99.1")
+    build.build()
+    assert len(commands) == 1 and build.binding_path() in commands[0] and build.binding_path() != here
+    monkeypatch.setattr(torch, "__version__", "99.1")
+    assert os.path.normpath(pplb200.attention.binding_path()) == build.binding_path()
+
+
+def test_build_says_that_there_is_no_binding_without_torch(monkeypatch, capsys):
+    build, commands = _build_module(), []
+    monkeypatch.setattr(build.subprocess, "run", lambda cmd, **kw: commands.append(cmd))
+    monkeypatch.setattr(build, "torch_home", lambda: None)
+    monkeypatch.setattr(build, "_stale", lambda target, deps: not os.path.exists(target))
+    assert build.build() == build.LIB and not commands
+    assert "torch is not installed" in capsys.readouterr().out
