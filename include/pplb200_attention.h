@@ -25,10 +25,12 @@ extern "C" {
  *   NTK         the base times factor ^ (rotary_dim / (rotary_dim - 2)): the slowest plane is divided by factor, the fastest kept
  *   YARN        f_i for planes that turn at least keep_turns times within original_length positions, f_i / factor for those
  *               that turn at most stretch_turns times, a blend that is linear in the plane's index between them (the two
- *               limits rounded outwards to whole planes); rotated values times 0.1 ln(factor) + 1
+ *               limits rounded outwards to whole planes, and to 0 and rotary_dim - 1 where they lie beyond these); rotated
+ *               values times 0.1 ln(factor) + 1
  *   WAVELENGTH  the same limits, the blend linear in the number of turns; no factor on the values
- * turns_host[i] (HOST, rotary_dim / 2 words) receives f_i / (2 pi) as a fraction of a turn in units of 2^-64, so that position *
- * turns_host[i] modulo 2^64 is the angle, exactly, however far the position; magnitude_host (HOST) the factor on the values.
+ * turns_host[i] (HOST, rotary_dim / 2 words) receives f_i / (2 pi) as a fraction of a turn in units of 2^-64, within four of them (where
+ * long double has 64 bits or more); position * turns_host[i] modulo 2^64, which is taken without a rounding, is the angle, within |position| *
+ * 2^-62 turns: 2^-22 of a turn at a position of 2^40.  magnitude_host (HOST) receives the factor on the values.
  * To be called once; the caller keeps a copy of turns_host on the device.
  */
 enum {

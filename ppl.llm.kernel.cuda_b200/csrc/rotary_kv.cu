@@ -431,25 +431,26 @@ int32_t pplb200_rotary_frequencies(int32_t rotary_dim, double base, int32_t scal
     const bool blend = scaling == PPLB200_ROTARY_YARN || scaling == PPLB200_ROTARY_WAVELENGTH;
     if (blend && (!(original_length > 0.0) || !std::isfinite(original_length) || !(stretch_turns > 0.0) || !(keep_turns > stretch_turns) || !std::isfinite(keep_turns)))
         return fail(RC_INVALID_VALUE, "a blend needs original_length > 0 and keep_turns > stretch_turns > 0");
-    const double two_pi = 6.283185307179586476925286766559;
-    const double rd = rotary_dim;
-    const double b = scaling == PPLB200_ROTARY_NTK ? base * std::pow(factor, rd / (rd - 2.0)) : base;
+    // The frequencies in 64-bit mantissas (long double): a word is off by a few of its units, and an angle by that times the position.
+    const long double two_pi = 6.283185307179586476925286766559005768L, ld_base = base, ld_factor = factor;
+    const double rd = rotary_dim, turn = (double)two_pi;
+    const long double b = scaling == PPLB200_ROTARY_NTK ? ld_base * std::pow(ld_factor, (long double)rd / (rd - 2.0)) : ld_base;
     // planes between which YARN blends: those that turn keep_turns and stretch_turns times within the original length
     double first = 0.0, last = 0.0;
     if (scaling == PPLB200_ROTARY_YARN) {
-        first = std::fmax(std::floor(rd * std::log(original_length / (keep_turns * two_pi)) / (2.0 * std::log(base))), 0.0);
-        last = std::fmin(std::ceil(rd * std::log(original_length / (stretch_turns * two_pi)) / (2.0 * std::log(base))), rd - 1.0);
+        first = std::fmax(std::floor(rd * std::log(original_length / (keep_turns * turn)) / (2.0 * std::log(base))), 0.0);
+        last = std::fmin(std::ceil(rd * std::log(original_length / (stretch_turns * turn)) / (2.0 * std::log(base))), rd - 1.0);
     }
     for (int32_t i = 0; i < rotary_dim / 2; ++i) {
-        double f = std::pow(b, -2.0 * i / rd);
-        if (scaling == PPLB200_ROTARY_LINEAR) f /= factor;
+        long double f = std::pow(b, -2.0L * i / rd);
+        if (scaling == PPLB200_ROTARY_LINEAR) f /= ld_factor;
         if (blend) {
-            const double keep = scaling == PPLB200_ROTARY_YARN ? 1.0 - (i - first) / std::fmax(last - first, 0.001)
-                                                               : (original_length * f / two_pi - stretch_turns) / (keep_turns - stretch_turns);
-            const double part = std::fmin(std::fmax(keep, 0.0), 1.0);
-            f = f * part + f / factor * (1.0 - part);
+            const long double keep = scaling == PPLB200_ROTARY_YARN ? 1.0L - (i - first) / (long double)std::fmax(last - first, 0.001)
+                                                                    : (original_length * f / two_pi - stretch_turns) / ((long double)keep_turns - stretch_turns);
+            const long double part = std::fmin(std::fmax(keep, 0.0L), 1.0L);
+            f = f * part + f / ld_factor * (1.0L - part);
         }
-        turns_host[i] = (uint64_t)std::floor(f / two_pi * 0x1p64 + 0.5); // f <= 1: below 2^62
+        turns_host[i] = (uint64_t)std::floor(f / two_pi * 0x1p64L + 0.5L); // f <= 1: below 2^62
     }
     *magnitude_host = scaling == PPLB200_ROTARY_YARN ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
     return RC_SUCCESS;

@@ -82,6 +82,34 @@ def test_frequencies(kind, factor, original, keep, stretch, rd, base):
     assert t.magnitude == np.float32(0.1 * math.log(factor) + 1.0 if kind == "yarn" else 1.0)
 
 
+@pytest.mark.parametrize("kind,factor,original,keep,stretch", [
+    ("none", 1.0, 0, 0, 0), ("linear", 3.0, 0, 0, 0), ("ntk", 8.0, 0, 0, 0), ("yarn", 32.0, 4096, 32, 1), ("wavelength", 7.0, 8192, 4, 1)])
+@pytest.mark.parametrize("rd,base", [(16, 10000.0), (96, 500000.0), (128, 10000.0), (256, 1000000.0)])
+def test_words_of_a_turn_hold_to_their_last_bits(kind, factor, original, keep, stretch, rd, base):
+    """An error of a word grows with the position; in the words of 64-bit arithmetic it was 2^-56 of a turn."""
+    import decimal
+    import pplb200
+    D = decimal.Decimal
+    t = pplb200.RotaryTable(rd, base=base, scaling=kind, factor=factor, original_length=original, keep_turns=keep, stretch_turns=stretch, device="cpu")
+    with decimal.localcontext() as context:
+        context.prec = 60
+        two_pi = 2 * D("3.14159265358979323846264338327950288419716939937510582097494459")
+        for i, word in enumerate(t.turns.numpy().view(np.uint64)):
+            b = D(base) * D(factor) ** (D(rd) / (rd - 2)) if kind == "ntk" else D(base)
+            f = b ** (D(-2 * i) / rd)
+            part = D(1)
+            if kind == "yarn":
+                ends = [rd * math.log(original / (x * 2 * math.pi)) / (2 * math.log(base)) for x in (keep, stretch)]
+                first, last = max(math.floor(ends[0]), 0), min(math.ceil(ends[1]), rd - 1)
+                part = 1 - D(i - first) / max(last - first, D("0.001"))
+            elif kind == "wavelength":
+                part = (original * f / two_pi - D(stretch)) / (D(keep) - D(stretch))
+            part = min(D(1), max(D(0), part)) if kind != "linear" else D(0)
+            f = f * part + f / D(factor) * (1 - part)
+            # half a unit for the word; in front of it some ten roundings to 64 bits of numbers below 2^62 of these units
+            assert abs(D(int(word)) - f / two_pi * 2 ** 64) <= 4
+
+
 @pytest.mark.parametrize("args,rc", [
     (dict(rotary_dim=0), 4), (dict(rotary_dim=24), 4), (dict(rotary_dim=272), 4), (dict(rotary_dim=64, base=1.0), 4), (dict(rotary_dim=64, base=float("nan")), 4),
     (dict(rotary_dim=64, base=float("inf")), 4), (dict(rotary_dim=64, scaling="linear", factor=0.5), 4), (dict(rotary_dim=64, scaling="ntk", factor=float("nan")), 4),
