@@ -69,7 +69,8 @@ int32_t pplb200_rotary_fp16(pplb200_stream_t stream, const pplb200_rotary_args* 
  * from v.  Both orders of heads and a page's tokens are a matter of the strides.  Strides are in elements (scales: in scales), not
  * negative, those of k and v multiples of 16 bytes; k and v 16-byte aligned.
  * quant_group 0: k and v are fp16.  quant_group 8 or head_dim: int8, and every quant_group dimensions share an fp16 scale,
- * head_dim / quant_group contiguous scales for a token and head.  head_dim a multiple of 16, at most 256.
+ * head_dim / quant_group contiguous scales for a token and head.  head_dim a multiple of 16, at most 256; at most 65535 heads; the last
+ * element, and the last scale, less than 2^61 from the first.
  */
 typedef struct pplb200_kv_cache {
     void *k, *v, *k_scale, *v_scale;
@@ -119,7 +120,9 @@ int32_t pplb200_kv_cache_read_fp16(pplb200_stream_t stream, const pplb200_kv_cac
  * tokens are seen, but have scores of -inf only, NaN and -inf.
  * optional_lse fp32 [batch, q_heads], contiguous: log(sum_t exp(scale q . k_t)), for joining results over parts of a context.
  * head_dim 64, 96, 128 or 256 (with quant_group 8: scales 4-byte aligned, their strides even); q_heads a multiple of kv_heads; strides
- * multiples of 8; q and out 16-byte aligned; out may be q; scale within 2^50 of zero; at most 2^30 tokens a row of the table.
+ * multiples of 8; q and out 16-byte aligned; out may be q; scale within 2^50 of zero; at most 2^30 tokens a row of the table, 65535
+ * sequences and 65535 query heads; rows of one head of the cache, and their scales, less than 2^32 times the largest power of two (up to
+ * 2^30 bytes) that divides their distances apart.
  * ws: pplb200_paged_decode_attention_workspace_bytes(), 256-byte aligned, zeroed before its first use (every call leaves it fit for the
  * next, of whatever sizes), not shared by calls that may run at the same time (two captured graphs that are replayed at once need
  * one each).
@@ -142,8 +145,12 @@ int64_t pplb200_paged_decode_attention_workspace_bytes(int64_t batch, int64_t ma
 int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache,
                                             const pplb200_paged_attention_args* args);
 
-/* Host-only: offset in elements of head `head` of a slot from cache->k, as the kernels compute it; -1 where the slot is not in the cache. */
+/*
+ * Host-only: offset in elements of head `head` of a slot from cache->k, as the kernels that write and read the cache compute it, and as
+ * attention's does, which has arithmetic of its own; -1 where the slot is not in the cache, or the cache is refused.
+ */
 int64_t pplb200_kv_cache_offset(const pplb200_kv_cache* cache, int64_t slot, int32_t head);
+int64_t pplb200_paged_attention_offset(const pplb200_kv_cache* cache, int64_t slot, int32_t head);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

@@ -843,6 +843,13 @@ bool row_units(int64_t pages, int64_t page_size, int64_t page_bytes, int64_t tok
     return (last >> shift) < ((__int128)1 << 32);
 }
 
+// Units of the rows, and of the scales, of a cache that has been checked.
+bool cache_units(const pplb200_kv_cache* c, AttentionParams& p) {
+    const int bytes = c->quant_group ? 1 : 2;
+    return row_units(c->num_pages, c->page_size, c->page_stride * bytes, c->token_stride * bytes, p.unit, p.page_units, p.token_units) &&
+           (!c->quant_group || row_units(c->num_pages, c->page_size, c->scale_page_stride * 2, c->scale_token_stride * 2, p.scale_unit, p.scale_page_units, p.scale_token_units));
+}
+
 // Query heads that a CTA takes at once: two blocks of eight where that many share a key-value head and registers allow.
 int heads_at_once(int32_t head_dim, int32_t shared) { return shared > 8 && head_dim <= 128 ? 16 : 8; }
 template <class S>
@@ -913,10 +920,7 @@ int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb2
     if (cache->quant_group == 8 && ((((uintptr_t)cache->k_scale | (uintptr_t)cache->v_scale) & 3) ||
                                     ((cache->scale_page_stride | cache->scale_head_stride | cache->scale_token_stride) & 1)))
         return fail(RC_INVALID_VALUE, "attention: scales of groups of 8 must be 4-byte aligned, and their strides even");
-    if (!row_units(cache->num_pages, cache->page_size, cache->page_stride * (cache->quant_group ? 1 : 2), cache->token_stride * (cache->quant_group ? 1 : 2),
-                   p.unit, p.page_units, p.token_units) ||
-        (cache->quant_group && !row_units(cache->num_pages, cache->page_size, cache->scale_page_stride * 2, cache->scale_token_stride * 2, p.scale_unit,
-                                          p.scale_page_units, p.scale_token_units)))
+    if (!cache_units(cache, p))
         return fail(RC_UNSUPPORTED, "attention: the rows of a head lie further apart than 2^32 times their alignment");
     small_division(cache->page_size, p.page_magic, p.page_shift);
     p.num_pages = (int32_t)std::min<int64_t>(cache->num_pages, 0x7fffffff); // a table's entry is no larger
@@ -941,6 +945,15 @@ int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb2
     if (D == 96) return launch_dim<96>(s, p, p.tokens_in_table, packed);
     if (D == 128) return launch_dim<128>(s, p, p.tokens_in_table, packed);
     return launch_dim<256>(s, p, p.tokens_in_table, packed);
+}
+
+int64_t pplb200_paged_attention_offset(const pplb200_kv_cache* c, int64_t slot, int32_t head) {
+    AttentionParams p = {};
+    int64_t page;
+    int32_t in_page;
+    if (check_kv_cache(c) != RC_SUCCESS || !cache_units(c, p) || head < 0 || head >= c->kv_heads || !kv_find(slot, c->num_pages, c->page_size, page, in_page)) return -1;
+    const uint32_t row = (uint32_t)page * p.page_units + (uint32_t)in_page * p.token_units;
+    return head * c->head_stride + (int64_t)((uint64_t)row * p.unit / (c->quant_group ? 1 : 2));
 }
 
 } // extern "C"

@@ -26,6 +26,13 @@ int32_t check_kv_cache(const pplb200_kv_cache* c) {
             return fail(RC_INVALID_VALUE, "negative scale stride");
         if (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 1) return fail(RC_INVALID_VALUE, "scales must be 2-byte aligned");
     }
+    // offsets, in bytes too, fit 64 bits
+    const auto last = [&](int64_t page, int64_t head, int64_t token) {
+        return (__int128)(c->num_pages - 1) * page + (__int128)(c->kv_heads - 1) * head + (__int128)(c->page_size - 1) * token + c->head_dim;
+    };
+    if (last(c->page_stride, c->head_stride, c->token_stride) >> 61 ||
+        (c->quant_group && last(c->scale_page_stride, c->scale_head_stride, c->scale_token_stride) >> 61))
+        return fail(RC_INVALID_VALUE, "a cache whose elements lie 2^61 apart");
     return RC_SUCCESS;
 }
 

@@ -17,6 +17,7 @@ from . import LIB_PATH, PplError, _check, lib
 EXPORTS = [
     "pplb200_rotary_frequencies", "pplb200_rotary_fp16", "pplb200_kv_cache_write_fp16", "pplb200_kv_cache_read_fp16",
     "pplb200_paged_decode_attention_workspace_bytes", "pplb200_paged_decode_attention_fp16", "pplb200_kv_cache_offset",
+    "pplb200_paged_attention_offset",
 ]
 ROTARY_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "wavelength": 4}
 
@@ -28,8 +29,8 @@ lib.pplb200_kv_cache_read_fp16.argtypes = [_vp, _blk, _vp, _i64, _vp, _vp]
 lib.pplb200_paged_decode_attention_workspace_bytes.argtypes = [_i64, _i64, _i32, _i32, _i32]
 lib.pplb200_paged_decode_attention_workspace_bytes.restype = _i64
 lib.pplb200_paged_decode_attention_fp16.argtypes = [_vp, _blk, _blk]
-lib.pplb200_kv_cache_offset.argtypes = [_blk, _i64, _i32]
-lib.pplb200_kv_cache_offset.restype = _i64
+lib.pplb200_kv_cache_offset.argtypes = lib.pplb200_paged_attention_offset.argtypes = [_blk, _i64, _i32]
+lib.pplb200_kv_cache_offset.restype = lib.pplb200_paged_attention_offset.restype = _i64
 
 _pack_cache = struct.Struct("=4Q7q4i").pack
 

@@ -232,6 +232,52 @@ def test_attention_refusals(bad, rc):
     assert _calls()[2](_cache(), **bad) == rc and pplb200.last_error()
 
 
+@pytest.mark.parametrize("cache,rc", [
+    # scales of groups of 8 are read two at a time
+    (dict(group=8, ks=AT + 2), 4), (dict(group=8, vs=AT + 2), 4), (dict(group=8, spage=8 * 256 + 1), 4), (dict(group=8, shead=255), 4), (dict(group=8, stoken=17), 4),
+    # rows of a head 2^32 times their alignment apart, in keys and values, and in scales
+    (dict(pages=(1 << 28) + 1, page_stride=(1 << 8) + 16, token_stride=0), 2), (dict(group=0, pages=(1 << 31) - 1, page_stride=24, token_stride=8), 2),
+    (dict(pages=1 << 30, page_stride=0, token_stride=0, spage=9), 2), (dict(pages=1 << 30, page_stride=0, token_stride=0, group=8, spage=18, stoken=0), 2)])
+def test_attention_refusals_of_caches(cache, rc):
+    import pplb200
+    assert _calls()[2](_cache(**cache)) == rc and pplb200.last_error()
+
+
+@pytest.mark.parametrize("bad", [dict(page_stride=1 << 62), dict(pages=1 << 60, page_stride=16), dict(head_stride=1 << 60), dict(token_stride=(1 << 58)), dict(page=1 << 30, token_stride=1 << 40),
+                                 dict(spage=1 << 62), dict(shead=1 << 60), dict(page=1 << 30, stoken=1 << 40), dict(group=0, ks=0, vs=0, page_stride=1 << 62)])
+def test_caches_beyond_any_memory(bad):
+    """Offsets whose products would not fit 64 bits."""
+    import pplb200
+    write, _, attend = _calls()
+    c = _cache(**bad)
+    assert write(c) == attend(c) == pplb200.lib.pplb200_kv_cache_read_fp16(None, c, AT, 4, AT, AT) == 4 and pplb200.last_error()
+    assert pplb200.lib.pplb200_kv_cache_offset(c, 0, 0) == pplb200.lib.pplb200_paged_attention_offset(c, 0, 0) == -1
+
+
+def test_attention_offsets_are_the_caches():
+    """Attention's kernel computes them with 32-bit numbers of a unit of its own; up to the largest that it takes."""
+    import pplb200
+    lib = pplb200.lib
+    edge = 1 << 32  # units
+    for kw in (dict(), dict(group=0), dict(page=1), dict(page=7, head_stride=7 * 128, page_stride=7 * 1024), dict(head_stride=128, token_stride=1024), dict(pages=70000, page=64, page_stride=64 * 1024, head_stride=64 * 128),
+               dict(group=0, pages=36000, page=64, page_stride=64 * 1024, head_stride=64 * 128), dict(pages=1, page_stride=16), dict(page=1, token_stride=0), dict(page_stride=0, head_stride=0, token_stride=0),
+               # the last row is the last unit, of 16 bytes (int8: 16 elements, fp16: 8) and of more
+               dict(pages=edge, page=1, page_stride=16), dict(pages=edge // 16, page_stride=256, token_stride=16), dict(group=0, pages=edge, page=1, page_stride=8),
+               dict(pages=edge, page=1, page_stride=4096), dict(pages=edge // 2, page=2, page_stride=48, token_stride=16), dict(pages=1 << 22, page=64, page_stride=64 * 1024 * 16, head_stride=16, token_stride=1024 * 16)):
+        c = _cache(**dict(dict(spage=0, shead=0, stoken=0), **kw))
+        full = dict(CACHE, **kw)
+        slots = full["pages"] * full["page"]
+        for slot in (0, 1, full["page"] - 1, full["page"], slots // 2, slots // 3, slots - 1):
+            for head in (0, 3, 7):
+                want = lib.pplb200_kv_cache_offset(c, slot, head)
+                if kw == dict(pages=edge // 2, page=2, page_stride=48, token_stride=16):  # 3 / 2 times as far as it takes
+                    assert want >= 0 and lib.pplb200_paged_attention_offset(c, slot, head) == -1
+                elif slot < slots:
+                    assert want >= 0 and lib.pplb200_paged_attention_offset(c, slot, head) == want, (kw, slot, head)
+        assert lib.pplb200_paged_attention_offset(c, slots, 0) == lib.pplb200_paged_attention_offset(c, -1, 0) == lib.pplb200_paged_attention_offset(c, 0, 8) == -1
+    assert lib.pplb200_paged_attention_offset(_cache(pages=edge + 1, page=1, page_stride=16, spage=0, shead=0, stoken=0), 0, 0) == -1
+
+
 def test_attention_head_dimensions():
     import pplb200
     attend = _calls()[2]
