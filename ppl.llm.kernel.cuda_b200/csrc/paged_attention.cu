@@ -735,8 +735,9 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
             const int32_t c0 = (int32_t)(((begin + 1) * ctas + all - 1) / all) - 1; // began the item
             const int32_t pieces = (int32_t)((end * ctas + all - 1) / all) - c0;
             // The barrier puts the other threads' sums ahead of this thread's release, and its acquire ahead of their reads.  A counter is
-            // the call's number above 16 bits of arrivals, none between calls; the maximum throws out what calls that ran at the same time
-            // on this workspace, against the rules, have left.
+            // the call's number above 16 bits of arrivals, none between calls; the maximum throws out what earlier calls that ran at the same time
+            // on this workspace, against the rules, have left.  A captured call keeps the number of its capture, so that its replays get rid only of
+            // what calls before the capture have left.
             auto last_of = [&](uint64_t* counter, int32_t number) {
                 __syncthreads();
                 if (threadIdx.x == 0) {
