@@ -67,7 +67,7 @@ int32_t pplb200_rotary_fp16(pplb200_stream_t stream, const pplb200_rotary_args* 
  * A paged key-value cache of one layer.  Token `slot` lies on page slot / page_size, at slot % page_size of it; its keys of head h
  * are the head_dim elements from k + page * page_stride + h * head_stride + (slot % page_size) * token_stride, its values the same
  * from v.  Both orders of heads and a page's tokens are a matter of the strides.  Strides are in elements (scales: in scales), not
- * negative, those of k and v multiples of 16 bytes; k and v 16-byte aligned.
+ * negative, those of k and v multiples of 16 bytes; k and v 16-byte aligned.  Rows may overlap (a stride of 0) where nothing is written.
  * quant_group 0: k and v are fp16.  quant_group 8 or head_dim: int8, and every quant_group dimensions share an fp16 scale,
  * head_dim / quant_group contiguous scales for a token and head.  head_dim a multiple of 16, at most 256; at most 65535 heads; the last
  * element, and the last scale, less than 2^61 from the first.

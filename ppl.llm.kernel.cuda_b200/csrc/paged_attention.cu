@@ -9,18 +9,18 @@
 // and the CTA that is last to do so joins them, where they are many in groups and then the groups.  While a warp works on its step the next one
 // is on its way into its registers, each part requested as soon as its registers are free: a lane loads exactly the bytes that it will
 // use (the dimensions of a product may be taken in any order), so that nothing passes through shared memory.  Tried instead: rings in shared memory
-// filled by cp.async, whose 64- and 128-byte row parts end at 4.2 TB/s, and by bulk copies of whole runs of rows (65 us instead of 68 with groups of
-// 8, but 149 instead of 121 with int8 rows and 103 instead of 91 in fp16: values are then read with bank conflicts); bringing the step after the next into L2
-// (66 -> 69, 116 -> 119, 88 -> 93).
+// filled by cp.async, whose 64- and 128-byte row parts end at 4.2 TB/s, and by bulk copies of whole runs of rows (65 us instead of what were then
+// 68 with groups of 8, but 149 instead of 121 with int8 rows and 103 instead of 91 in fp16: values are then read with bank conflicts); bringing the step
+// after the next into L2 (then 66 -> 69, 116 -> 119, 88 -> 93).
 //
 // Scores are computed transposed, keys [16 tokens x dimensions] x queries [dimensions x 8 heads]: the eight columns hold the query heads that
 // share the key head, and the weights turn into the operand of the second product, values^T x weights^T, by transposing 8 x 8 blocks
 // between registers.  mma.sync, because an operand of tcgen05.mma would first have to be widened into shared memory, and the tensor pipe is
-// busy for a quarter of the time at most.
+// busy for a quarter of the time.
 //
 // Heads of 128 in one graph, caches larger than L2, against the bytes at a copy's 6.55 TB/s: 64 sequences of up to 8192 tokens, 64 query
-// heads over 8, int8 rows 112 us (90 %; 124 over seconds, at the power limit and 1.67 GHz); one of 131072, fp16, 89 us (92 %); 16 of up to 4096, 32
-// heads of their own, groups of 8, 66 us (72 %: 575 instructions for 16 tokens, issue slots 56 % busy at 16 warps an SM).  Short
+// heads over 8, int8 rows 118 us (86 %; 135 over seconds, at the power limit and 1.67 GHz); one of 131072, fp16, 89 us (92 %); 16 of up to 4096, 32
+// heads of their own, groups of 8, 67 us (71 %: 575 instructions for 16 tokens, issue slots 55 % busy at 16 warps an SM).  Short
 // ones consist of look-ups that wait for each other, lengths, pages, rows, and of the join: one of 333 tokens 9 us.
 #include "kv_cache.cuh"
 
@@ -37,14 +37,17 @@ enum : int { CACHE_F16 = 0, CACHE_I8_GROUPS = 1, CACHE_I8_ROWS = 2 };
 constexpr int piece(int bytes) { return bytes % 16 == 0 ? 16 : bytes % 8 == 0 ? 8 : 4; }
 
 // Sizes of one variant: D dimensions, KIND of cache, NT blocks of eight query heads.  PACKED: a page has a multiple of 16 tokens, whose
-// rows follow each other, so that 16 tokens are one address and offsets that the instructions hold.
+// rows follow each other, so that 16 tokens are one address and offsets that the instructions hold.  Other pages (of 8 or 24 tokens) take 4 to 7 %
+// longer over int8 caches, tokens ahead of heads or pages of one token 10 to 12 %, over fp16 ones nothing (16 x 2048 groups 64.7, 67, 71 us;
+// 32 x 4096 rows 51, 55, 57; 16 x 4096 fp16 46).
 template <int D_, int KIND_, int NT_, bool PACKED_>
 struct Shape {
     static constexpr int D = D_, KIND = KIND_, NT = NT_, HEADS = 8 * NT;
     static constexpr bool PACKED = PACKED_;
     static constexpr int ES = KIND == CACHE_F16 ? 2 : 1;
-    // Tokens of a step: 32 where that leaves room for twelve warps on an SM (64 x 8192, int8 rows: 112 us with 32, 118 with 16; groups,
-    // whose scales take registers too: 16 x 4096 67.5 us with 32, 66 with 16).
+    // Tokens of a step: 32 where that leaves a form for eight query heads room for twelve warps on an SM (64 x 8192, int8 rows: 118 us with 32,
+    // 129 with 16; groups, whose scales take registers too: 16 x 4096 68.2 us with 32, 66.7 with 16).  Forms for sixteen take as many tokens as
+    // those for eight, although int8 rows of 128 then leave room for eight warps only; 16 tokens have not been measured there.
     static constexpr int SUBS = D * ES <= 64 || (D * ES <= 128 && KIND == CACHE_I8_ROWS) ? 2 : 1, TOKENS = 16 * SUBS;
     // of 16 tokens a quad's lane holds a quarter of the dimensions of two keys, an eighth of those of four values
     static constexpr int KB = D * ES / 4, KP = piece(KB), KN = KB / KP;
@@ -637,7 +640,9 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                                 widen_pairs(p, w[0][i][x], w[1][i][x], u);
                                 widen_pairs(p, w[2][i][x], w[3][i][x], v);
                                 if constexpr (S::KIND == CACHE_I8_GROUPS) {
-                                    // these four dimensions are of one group; value x scale is rounded to fp16, as it is when it is read back
+                                    // These four dimensions are of one group; value x scale is rounded to fp16, as it is when it is read back.  What that
+                                    // leaves, in a third product, would take 17 % more time (16 x 4096 tokens 64 -> 75 us) for an error of 0.00021 instead
+                                    // of 0.00029 (2-norm; the output's own rounding alone 0.00020).
                                     const __half2 fu = as_h2(__byte_perm(vs[sub][0][i], vs[sub][1][i], x < 2 ? 0x5410 : 0x7632));
                                     const __half2 fv = as_h2(__byte_perm(vs[sub][2][i], vs[sub][3][i], x < 2 ? 0x5410 : 0x7632));
 #pragma unroll
@@ -851,7 +856,9 @@ bool cache_units(const pplb200_kv_cache* c, AttentionParams& p) {
            (!c->quant_group || row_units(c->num_pages, c->page_size, c->scale_page_stride * 2, c->scale_token_stride * 2, p.scale_unit, p.scale_page_units, p.scale_token_units));
 }
 
-// Query heads that a CTA takes at once: two blocks of eight where that many share a key-value head and registers allow.
+// Query heads that a CTA takes at once: two blocks of eight where that many share a key-value head and registers allow.  16 sequences of up to
+// 4096 tokens, 128 heads over 8: heads of 128 in fp16 50 us (79 if eight at a time), int8 rows 44 (52), groups of 8 52 (64); of 64 in fp16 31 (40), of
+// 96 43 (59).
 int heads_at_once(int32_t head_dim, int32_t shared) { return shared > 8 && head_dim <= 128 ? 16 : 8; }
 template <class S>
 int32_t launch(cudaStream_t stream, AttentionParams& p, int64_t tokens) {

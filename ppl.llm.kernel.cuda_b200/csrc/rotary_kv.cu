@@ -248,7 +248,7 @@ struct RotaryKv {
 // Bound by HBM where nothing is quantized: 8192 tokens of 64 + 8 heads of 128 rotated 47 us, 97 % of a copy's rate; stored as fp16 too, 57 us,
 // 91 %.  Quantizing costs some 200 instructions for 16 elements of 32 lanes, which shows: 16384 tokens of 8 + 8 heads 22.4 us, 69 % (29 with
 // branches around the loads, keys and values one after the other and a run-time choice of the cache's type).  CTAs that share an
-// SM were tried from 5 to 10: unrotated, 10 spill (24.4 us), 6 take as long as 8 but 8.9 instead of 8.2 us for 4096 tokens in groups of 8; rotated, into groups of 8,
+// SM were tried from 5 to 10 (at the bounds taken, the forms that store int8 rows spill 8 to 16 bytes): unrotated, 10 spill more (24.4 us), 6 take as long as 8 but 8.9 instead of 8.2 us for 4096 tokens in groups of 8; rotated, into groups of 8,
 // 2048 tokens of 32 + 32 heads, 22.6 us with 7, 24 with 6.
 template <int LANES, int LAYOUT, int STORE>
 __global__ void __launch_bounds__(RTPB, LAYOUT == AS_IS ? 8 : 7) rotary_kv_kernel(const __grid_constant__ RotaryKvParams p) {

@@ -194,7 +194,7 @@ def kv_cache_read(cache, slots, k_out=None, v_out=None):
 
 class PagedDecodeAttention(_LaidOutOnce):
     """Attention of one new token a sequence over a PagedKVCache.  Owns the workspace for `max_batch` sequences of `max_length` tokens, so
-    one object serves one stream at a time.  scale: 1 / sqrt(head_dim) unless given; window: how many of the last tokens are seen (0: all)."""
+    one object serves one stream at a time, and is kept until its calls have run.  scale: 1 / sqrt(head_dim) unless given; window: how many of the last tokens are seen (0: all)."""
 
     def __init__(self, cache, q_heads, max_batch, max_length, scale=None, window=0):
         _need(q_heads > 0 and q_heads % cache.kv_heads == 0, "q_heads must be a multiple of the cache's heads")
