@@ -270,3 +270,31 @@ def test_int8_special_values_out_of_sight(cuda, pplb200, group):
     got = att(q, table, lens)
     assert cuda.equal(got[1:], out[1:]) and cuda.equal(got[0, :4], out[0, :4])
     assert bool(got[0, 4:].isnan().all())
+
+
+@pytest.mark.parametrize("batch,heads", [(65535, 1), (3, 65535), (9000, 40)])
+@pytest.mark.parametrize("group", [0, 64])
+def test_the_most_sequences_and_heads(cuda, pplb200, batch, heads, group):
+    """As many sequences and heads as are taken, of none to three tokens: every row is written, from its own pages.  With values that are the
+    same for all tokens of a sequence and head, the output is that value, whatever the weights."""
+    d, page = 64, 3
+    g = _gen(cuda, batch)
+    pages = batch
+    cache = _cache(cuda, pplb200, pages, page, heads, d, group, "heads", 0)
+    size = cuda.randint(1, 100, (pages, heads), generator=g, device="cuda").to(cuda.float16)
+    cache.k.copy_(cuda.randint(-3, 4, (1, 1, page, d), generator=g, device="cuda").expand(cache.k.shape))
+    if group:
+        cache.k_scale.fill_(0.125)
+        cache.v.fill_(1)
+        cache.v_scale.copy_(size[:, :, None, None].expand(cache.v_scale.shape))
+    else:
+        cache.v.copy_(size[:, :, None, None].expand(cache.v.shape))
+    table = cuda.randperm(pages, generator=g, device="cuda").to(cuda.int32)[:, None].contiguous()
+    lens = cuda.randint(0, page + 1, (batch,), generator=g, device="cuda").to(cuda.int32)
+    q = _randn(cuda, g, 1, 1, d).expand(batch, heads, d).contiguous()
+    att = pplb200.PagedDecodeAttention(cache, heads, batch, page)
+    out = att(q, table, lens, out=cuda.full_like(q, 7.0))
+    want = size[table[:, 0].long()].float()
+    want[lens == 0] = 0
+    # three weights and their sum: a few roundings at 2^-22, and the output's
+    assert bool(((out.float() - want[..., None]).abs() <= want[..., None] * (HALF + 2.0 ** -19)).all())
