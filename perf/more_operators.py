@@ -257,7 +257,7 @@ def prepare(case, seed):
             pages = -(-t * block // page)
             at = _scattered(g, t, pages * (page // block))
             s["slots"] = at * block + torch.where(torch.arange(t, device="cuda") % 16 == 15, block - 1, torch.arange(t, device="cuda") % (block - 1))
-            s["done"] = at[15::16]
+            s["done"] = at[15::16].contiguous()
         s["cache"] = _filled_cache(g, pages, hk, page, d, group)
         s["bounds"], s["bound_scales"] = _no_bounds(case, pages)
         s["lo"], s["hi"] = (torch.empty((s["done"].shape[0], hk, d), device="cuda") for _ in range(2))
