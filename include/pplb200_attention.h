@@ -64,6 +64,27 @@ typedef struct pplb200_rotary_args {
 int32_t pplb200_rotary_fp16(pplb200_stream_t stream, const pplb200_rotary_args* args);
 
 /*
+ * Rotary positions with several axes, as tokens of images and videos have them (time, height, width): every plane belongs to one of
+ * up to four axes and is turned by the token's position on that axis.
+ * pplb200_rotary_axes_frequencies: planes_host[a] (HOST, `axes` numbers, not negative, rotary_dim / 2 together) planes belong to axis a: one axis behind the
+ * other, or, with `alternating`, dealt out in turn (axis 0, 1, ..., 0, 1, ...), an axis that has all its planes being passed over.  The planes' frequencies are those of
+ * pplb200_rotary_frequencies; with `restart` the n planes of each axis have those of a rotary_dim of 2 n, in order, instead.  axis_of_plane_host (HOST,
+ * rotary_dim / 2 bytes) receives the axes; the caller keeps a copy on the device, as of turns_host.
+ * The calls: as those with one axis, but positions int64 [axes, tokens], axis_stride elements between axes.  axis_of_plane (device, 4-byte aligned): a
+ * number beyond the axes stands for the last one.
+ */
+enum { PPLB200_ROTARY_MAX_AXES = 4 };
+typedef struct pplb200_rotary_axes {
+    const uint8_t* axis_of_plane;
+    int64_t axis_stride;
+    int32_t axes, reserved;
+} pplb200_rotary_axes;
+int32_t pplb200_rotary_axes_frequencies(int32_t rotary_dim, double base, int32_t scaling, double factor, double original_length,
+                                        double keep_turns, double stretch_turns, int32_t axes, const int32_t* planes_host, int32_t alternating,
+                                        int32_t restart, uint64_t* turns_host, uint8_t* axis_of_plane_host, float* magnitude_host);
+int32_t pplb200_rotary_axes_fp16(pplb200_stream_t stream, const pplb200_rotary_args* args, const pplb200_rotary_axes* axes);
+
+/*
  * A paged key-value cache of one layer.  Token `slot` lies on page slot / page_size, at slot % page_size of it; its keys of head h
  * are the head_dim elements from k + page * page_stride + h * head_stride + (slot % page_size) * token_stride, its values the same
  * from v.  Both orders of heads and a page's tokens are a matter of the strides.  Strides are in elements (scales: in scales), not
@@ -98,6 +119,9 @@ typedef struct pplb200_kv_write_args {
     float magnitude;
 } pplb200_kv_write_args;
 int32_t pplb200_kv_cache_write_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_kv_write_args* args);
+/* The same with positions of several axes (rotary_dim > 0). */
+int32_t pplb200_kv_cache_write_axes_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_kv_write_args* args,
+                                         const pplb200_rotary_axes* axes);
 
 /*
  * Reads tokens back: k_out, v_out fp16 [tokens, kv_heads, head_dim], contiguous, 16-byte aligned = the stored values, or value x
@@ -145,6 +169,66 @@ int64_t pplb200_paged_decode_attention_workspace_bytes(int64_t batch, int64_t ma
                                                        int32_t head_dim);
 int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache,
                                             const pplb200_paged_attention_args* args);
+
+/*
+ * Attention of one new token per sequence for a batch whose sequences begin with the same tokens, which lie in the cache once: out[b, h] as
+ * above over the prefix's tokens and sequence b's own, of which `lengths` counts and `pages` lists only the latter.  The prefix is read once for the
+ * batch.  prefix->pages int32 [prefix->num_pages], prefix->length int32 [1], both on the device: how many tokens (at most num_pages * page_size are
+ * looked at); pages that are not in the cache are holes.  A sequence with a length of 0 sees the prefix alone; a negative length stands for a row that is
+ * no sequence: zeros and -inf, whatever its q.  As above otherwise, but window has to be 0, at most 2^24 rows of q (batch * q_heads), and: over the prefix
+ * the softmax's weights enter their product with v with 11 bits, and v of int8 rows and groups as there, where batch * q_heads / kv_heads passes 16 (8 for heads of 256).
+ * ws: pplb200_shared_prefix_attention_workspace_bytes(), with the rules above.
+ */
+typedef struct pplb200_shared_prefix {
+    const int32_t *pages, *length;
+    int64_t num_pages;
+} pplb200_shared_prefix;
+int64_t pplb200_shared_prefix_attention_workspace_bytes(int64_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim);
+int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache,
+                                             const pplb200_paged_attention_args* args, const pplb200_shared_prefix* prefix);
+
+/*
+ * Bounds of the keys of blocks of tokens, for choosing among them.  A page has page_size / block blocks, block a multiple of 16; block x of page p is block
+ * number p * (page_size / block) + x of the cache.  bounds int8 [num_pages, kv_heads, page_size / block, 2, head_dim], contiguous, 16-byte aligned: in every
+ * dimension the least and the greatest of the block's keys (as they are stored: fp16, or values x scales), divided by the block's scale and rounded outwards
+ * to whole numbers; scale fp16 [num_pages, kv_heads, page_size / block], contiguous: the largest of the magnitudes / 127, rounded up to fp16, at least 2^-24.
+ * A block with a key that is infinite or NaN, or whose scale would be beyond fp16's range, has zeros and an infinite scale.  head_dim as for attention.
+ * pplb200_key_bounds_update: slots int64 [tokens], those that have been written: every block whose LAST token is among them is taken to be complete, and
+ * its bounds are computed from what the cache then holds.  Slots that are not in the cache are passed over; no slot comes twice.
+ * pplb200_key_bounds_read: blocks int64 [count], block numbers -> lo, hi fp32 [count, kv_heads, head_dim], contiguous, 16-byte aligned: whole numbers x scale
+ * (-inf and inf for a block with an infinite scale; zeros for a number that is not in the cache).
+ */
+typedef struct pplb200_key_bounds {
+    void *bounds, *scale;
+    int32_t block, reserved;
+} pplb200_key_bounds;
+int32_t pplb200_key_bounds_update(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_key_bounds* bounds, const int64_t* slots,
+                                  int64_t tokens);
+int32_t pplb200_key_bounds_read(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_key_bounds* bounds, const int64_t* blocks,
+                                int64_t count, float* lo, float* hi);
+
+/*
+ * Attention of one new token per sequence over some of its blocks.  A sequence of n tokens has ceil(n / block) blocks in order, the last of which may be
+ * begun only.  The first choice->first and the last choice->last of them are attended, and of those between the choice->top with the highest scores,
+ * each key head choosing its own; all, where there are no more.  The score of a block is the largest over the key head's query heads of
+ *   sum_d max(q8_d lo_d, q8_d hi_d), the whole numbers of the bounds, times (q's scale x the block's scale), rounded once to fp32,
+ * where q8 is q of that head quantized to int8: divided by its scale (the head's largest magnitude / 127, rounded up to fp16, at least 2^-24) and rounded to
+ * nearest even.  Whole numbers throughout, so that the same blocks are chosen everywhere; among equal scores the lowest block.  The score is an upper bound of
+ * q . k for the block's keys, up to the rounding of q.  A block with an infinite scale comes before all others; a block on a page that is not in the
+ * cache comes behind all others (it is a hole, chosen or not); a query head with an infinity or a NaN has no say.
+ * Then as pplb200_paged_decode_attention_fp16 over the chosen blocks' tokens, which are joined in order; args->window has to be 0.  Bounds are looked at for blocks between
+ * the first and the last ones only: with choice->last >= 1 these are complete.
+ * optional_blocks int32 [batch, kv_heads, first + last + top], contiguous: receives the chosen blocks of the sequence in ascending order, then -1.
+ * first, last, top not negative, last at least 1, first + last + top at most 65536; at most 2^18 blocks a row of the page table; num_pages * (page_size / block) below 2^31; batch * kv_heads at most 2^24.
+ * ws: pplb200_block_sparse_attention_workspace_bytes(), with the rules above.
+ */
+typedef struct pplb200_block_choice {
+    int32_t first, last, top, reserved;
+    int32_t* optional_blocks;
+} pplb200_block_choice;
+int64_t pplb200_block_sparse_attention_workspace_bytes(int64_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t attended_blocks);
+int32_t pplb200_block_sparse_attention_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_key_bounds* bounds,
+                                            const pplb200_paged_attention_args* args, const pplb200_block_choice* choice);
 
 /*
  * Host-only: offset in elements of head `head` of a slot from cache->k, as the kernels that write and read the cache compute it, and as

@@ -7,6 +7,7 @@ nvcc cross-compiles without a GPU.  The explicit -gencode form matters: tcgen05 
 accepted for the arch-specific target sm_100a, and plain -arch=sm_100a would also emit a
 generic compute_100 PTX image in which it is rejected.
 """
+import concurrent.futures
 import importlib.util
 import os
 import runpy
@@ -18,7 +19,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libpplb200_i8i8.so")
-SOURCES = ["capi.cu", "quantize.cu", "rmsnorm_quantize.cu", "activation_requant.cu", "gemm_i8_tcgen05.cu", "gemm_i8_decode.cu", "gemm_i8_token_pair.cu", "tensor_parallel.cu", "p2p_row_parallel.cu", "no_alloc.cu", "rotary_kv.cu", "paged_attention.cu", "probes.cu"]
+SOURCES = ["capi.cu", "quantize.cu", "rmsnorm_quantize.cu", "activation_requant.cu", "gemm_i8_tcgen05.cu", "gemm_i8_decode.cu", "gemm_i8_token_pair.cu", "tensor_parallel.cu", "p2p_row_parallel.cu", "no_alloc.cu", "rotary_kv.cu", "paged_attention.cu", "paged_attention_general.cu", "shared_prefix.cu", "block_sparse.cu", "probes.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 BINDING_SOURCE = os.path.join(CSRC, "attention_binding.cpp")
 FLAGS = [
@@ -55,16 +56,17 @@ def build(force=False, verbose=False):
     os.makedirs(LIBDIR, exist_ok=True)
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
     headers += [os.path.join(HERE, "..", "include", f) for f in ("pplb200_i8i8.h", "pplb200_attention.h")]
-    objs = []
+    objs, cmds = [], []
     for src in SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(LIBDIR, src.replace(".cu", ".o"))
         objs.append(o)
         if force or _stale(o, [s] + headers):
-            cmd = [NVCC] + FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-c", s, "-o", o]
+            cmds.append([NVCC] + FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-c", s, "-o", o])
             if verbose:
-                print(" ".join(cmd))
-            subprocess.run(cmd, check=True)
+                print(" ".join(cmds[-1]))
+    with concurrent.futures.ThreadPoolExecutor(os.cpu_count()) as pool:  # files compile side by side
+        list(pool.map(lambda cmd: subprocess.run(cmd, check=True), cmds))
     if force or _stale(LIB, objs):
         cmd = [NVCC, "-shared", "-o", LIB] + objs + ["-ldl"]
         if verbose:

@@ -1,0 +1,587 @@
+// Attention of one new token per sequence over blocks that a cheap score selects: bounds of the keys of complete blocks, the choice, and the attention
+// over what was chosen.
+#include "paged_attention.cuh"
+#include "ptx.cuh"
+
+namespace pplb200 {
+namespace {
+
+using ptx::cluster_ctarank;
+using ptx::cluster_sync_all;
+using ptx::map_to_cta;
+
+// The smallest fp16 of which 127 are no less than amax, at least 2^-24; two roundings upwards are one.
+__device__ __forceinline__ half outer_scale(float amax) {
+    const uint32_t s = __half_as_ushort(__float2half_ru(__fdiv_ru(amax, 127.0f)));
+    return __ushort_as_half((unsigned short)max(s, 1u));
+}
+__device__ __forceinline__ bool is_finite(half s) { return (__half_as_ushort(s) & 0x7c00u) != 0x7c00u; }
+
+// ---- bounds ------------------------------------------------------------------------------------------------------------
+// A CTA looks through a few slots for those that end a block, and goes through these blocks one after the other, for one head: a thread has eight
+// dimensions, head_dim / 8 neighbouring threads a token's row, so that as many rows are on their way as the CTA has threads for.
+// Bound by HBM in a long prompt: the keys once, 2 bytes in 2 * block * element back.
+constexpr int BTPB = 128;
+struct BoundsParams {
+    pplb200_kv_cache cache;
+    int8_t* bounds;
+    half* scale;
+    const int64_t* slots;
+    int64_t tokens;
+    int32_t block, per_page, slots_here;
+    uint32_t block_magic, block_shift;
+};
+
+template <int KIND>
+__global__ void __launch_bounds__(BTPB) key_bounds_kernel(const __grid_constant__ BoundsParams p) {
+    __shared__ int64_t block_of[BTPB];
+    __shared__ int32_t found;
+    __shared__ float lows[BTPB][8 + 1], highs[BTPB][8 + 1];
+    __shared__ float most[BTPB];
+    __shared__ int32_t any_bad;
+    const pplb200_kv_cache& c = p.cache;
+    const int lanes = c.head_dim >> 3, rows = BTPB / lanes;
+    const int row = threadIdx.x / lanes, lane = threadIdx.x - row * lanes;
+    const bool active = row < rows;
+    const int64_t head = blockIdx.y;
+    if (threadIdx.x == 0) found = 0;
+    pdl_wait_prior_grid();
+    __syncthreads();
+    const int64_t first_slot = (int64_t)blockIdx.x * p.slots_here;
+    if (threadIdx.x < p.slots_here && first_slot + threadIdx.x < p.tokens) {
+        int64_t page;
+        int32_t in_page;
+        if (kv_find(p.slots[first_slot + threadIdx.x], c.num_pages, c.page_size, page, in_page)) {
+            const int32_t x = (uint32_t)((uint64_t)(uint32_t)in_page * p.block_magic >> p.block_shift);
+            if (in_page - x * p.block == p.block - 1) block_of[atomicAdd(&found, 1)] = page * p.per_page + x;
+        }
+    }
+    __syncthreads();
+    const int number = found;
+    for (int i = 0; i < number; ++i) {
+        const int64_t page = block_of[i] / p.per_page;
+        const int32_t token0 = (int32_t)(block_of[i] - page * p.per_page) * p.block;
+        const int64_t at = kv_row(page, token0, head, c.page_stride, c.head_stride, c.token_stride) + lane * 8;
+        const int64_t scale_at = kv_row(page, token0, head, c.scale_page_stride, c.scale_head_stride, c.scale_token_stride) + (KIND == CACHE_I8_GROUPS ? lane : 0);
+        float lo[8], hi[8];
+        bool bad = false;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) lo[d] = INFINITY, hi[d] = -INFINITY;
+        if (active) {
+            if constexpr (KIND == CACHE_F16) {
+                __half2 l[4], h[4];
+                uint32_t largest = 0;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) l[d] = __half2half2(__ushort_as_half(0x7c00)), h[d] = __half2half2(__ushort_as_half(0xfc00));
+#pragma unroll 8
+                for (int t = row; t < p.block; t += rows) {
+                    const uint4 raw = ld_global_16((const half*)c.k + at + t * c.token_stride);
+                    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        l[d] = __hmin2(l[d], as_h2(w[d]));
+                        h[d] = __hmax2(h[d], as_h2(w[d]));
+                        const uint32_t magnitude = w[d] & 0x7fff7fffu;
+                        largest = max(largest, max(magnitude & 0xffffu, magnitude >> 16));
+                    }
+                }
+                bad = largest >= 0x7c00u;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const float2 a = __half22float2(l[d]), b = __half22float2(h[d]);
+                    lo[2 * d] = a.x; lo[2 * d + 1] = a.y;
+                    hi[2 * d] = b.x; hi[2 * d + 1] = b.y;
+                }
+            } else {
+#pragma unroll 8
+                for (int t = row; t < p.block; t += rows) {
+                    uint2 w;
+                    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "l"((const int8_t*)c.k + at + t * c.token_stride));
+                    const half s = ld_global_half((const half*)c.k_scale + scale_at + t * c.scale_token_stride);
+                    bad |= !is_finite(s);
+                    const float f = __half2float(s);
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) {
+                        const float v = (float)(int8_t)((d < 4 ? w.x : w.y) >> (8 * (d & 3))) * f;
+                        lo[d] = fminf(lo[d], v);
+                        hi[d] = fmaxf(hi[d], v);
+                    }
+                }
+            }
+        }
+        if (threadIdx.x == 0) any_bad = 0;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) lows[threadIdx.x][d] = lo[d], highs[threadIdx.x][d] = hi[d];
+        __syncthreads();
+        if (bad) any_bad = 1;
+        if (row == 0) { // the other rows' bounds of these dimensions
+            float amax = 0.0f;
+            for (int r = 1; r < min(rows, p.block); ++r)
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    lo[d] = fminf(lo[d], lows[r * lanes + lane][d]);
+                    hi[d] = fmaxf(hi[d], highs[r * lanes + lane][d]);
+                }
+#pragma unroll
+            for (int d = 0; d < 8; ++d) amax = fmaxf(amax, fmaxf(fabsf(lo[d]), fabsf(hi[d])));
+            most[lane] = amax;
+        }
+        __syncthreads();
+        if (row == 0) {
+            float amax = 0.0f;
+            for (int x = 0; x < lanes; ++x) amax = fmaxf(amax, most[x]);
+            half s = outer_scale(amax);
+            const bool lost = any_bad || !is_finite(s);
+            if (lost) s = __ushort_as_half(0x7c00);
+            const float step = __half2float(s);
+            uint32_t l[2] = {}, h[2] = {};
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+                const int a = lost ? 0 : (int)floorf(__fdiv_rn(lo[d], step)), b = lost ? 0 : (int)ceilf(__fdiv_rn(hi[d], step));
+                l[d >> 2] |= (uint32_t)(a & 0xff) << (8 * (d & 3));
+                h[d >> 2] |= (uint32_t)(b & 0xff) << (8 * (d & 3));
+            }
+            const int64_t of = (page * c.kv_heads + head) * p.per_page + token0 / p.block;
+            *reinterpret_cast<uint2*>(p.bounds + of * 2 * c.head_dim + lane * 8) = make_uint2(l[0], l[1]);
+            *reinterpret_cast<uint2*>(p.bounds + (of * 2 + 1) * c.head_dim + lane * 8) = make_uint2(h[0], h[1]);
+            if (lane == 0) p.scale[of] = s;
+        }
+        __syncthreads();
+    }
+}
+
+struct BoundsReadParams {
+    const int8_t* bounds;
+    const half* scale;
+    const int64_t* blocks;
+    float *lo, *hi;
+    int64_t count, all_blocks;
+    int32_t per_page, kv_heads, head_dim;
+};
+// A thread has four dimensions of one of the two bounds.
+__global__ void __launch_bounds__(BTPB) key_bounds_read_kernel(const __grid_constant__ BoundsReadParams p) {
+    pdl_wait_prior_grid();
+    const int quads = p.head_dim >> 2, of_head = 2 * quads, all = p.kv_heads * of_head;
+    for (int64_t i = blockIdx.x; i < p.count; i += gridDim.x) {
+        const int64_t block = p.blocks[i], page = block / p.per_page;
+        const bool there = block >= 0 && block < p.all_blocks;
+        for (int x = blockIdx.y * BTPB + threadIdx.x; x < all; x += gridDim.y * BTPB) {
+            const int head = x / of_head, rest = x - head * of_head, high = rest >= quads, d = (rest - high * quads) * 4;
+            float4 v = make_float4(0, 0, 0, 0);
+            if (there) {
+                const int64_t at = (page * p.kv_heads + head) * p.per_page + (block - page * p.per_page);
+                const uint32_t w = ld_global_u32((const uint32_t*)(p.bounds + (at * 2 + high) * p.head_dim + d));
+                const half s = ld_global_half(p.scale + at);
+                const float f = __half2float(s);
+                v = make_float4((float)(int8_t)w * f, (float)(int8_t)(w >> 8) * f, (float)(int8_t)(w >> 16) * f, (float)(int8_t)(w >> 24) * f);
+                if (!is_finite(s)) v.x = v.y = v.z = v.w = high ? INFINITY : -INFINITY;
+            }
+            *reinterpret_cast<float4*>((high ? p.hi : p.lo) + (i * p.kv_heads + head) * p.head_dim + d) = v;
+        }
+    }
+}
+
+// ---- the choice ----------------------------------------------------------------------------------------------------------
+// One cluster of CTAs for each sequence and key head.  A CTA scores its share of the blocks, 16 a warp at a time, on int8 mma.sync (16 blocks x 32
+// dimensions x 8 query heads; the product is tiny, what counts is that the bounds are read once and wide): sum_d max(q lo, q hi) is the product of q's
+// positive part with the greatest and of its negative part with the least.  The scores stay in shared memory as numbers that order alike.  The
+// threshold is found by four histograms of eight bits that the cluster's CTAs fill together in the first one's shared memory; then every CTA
+// writes those of its blocks that are above it, and as many of those at it, from the lowest on, as there is room for.
+constexpr int STPB = 256, SWARPS = STPB / 32, MAX_CLUSTER = 8;
+constexpr int64_t MAX_BLOCKS = 1 << 18, MAX_TOTAL = 65536, MAX_ITEMS = 1 << 24;
+struct ChoiceParams {
+    const half* q;
+    int64_t q_stride, pages_stride;
+    const int8_t* bounds;
+    const half* scale;
+    const int32_t *pages, *lengths;
+    int32_t* lists;           // [batch, kv_heads, total]: blocks of the cache, or -1
+    int32_t* listed_tokens;   // [batch]
+    int32_t* optional_blocks; // [batch, kv_heads, total]
+    int64_t tokens_in_table, items;
+    int32_t kv_heads, shared, block, per_page, num_pages, first, last, top, total;
+    uint32_t block_magic, block_shift, page_magic, page_shift; // / block, / per_page
+    int32_t share; // blocks of a CTA at most, a multiple of 16
+};
+
+__device__ __forceinline__ void mma_s8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Numbers that order as the floats do; 0 is below all of them.
+__device__ __forceinline__ uint32_t ordered(float f) {
+    const uint32_t b = __float_as_uint(f);
+    return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ void add_in_cluster(uint32_t addr, uint32_t v) {
+    asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_in_cluster(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+template <int D>
+__global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_constant__ ChoiceParams p) {
+    constexpr int KB = D / 4, KP = piece(KB), KN = KB / KP, KW = KP / 4; // a quad's lane has a quarter of a row, in pieces
+    constexpr int MMAS = D / 32;
+    extern __shared__ uint32_t keys[]; // [share]
+    __shared__ __align__(16) uint32_t q8[8][D / 4];
+    __shared__ uint32_t q_bits[8];
+    __shared__ uint32_t histogram[4][256];
+    __shared__ uint32_t above, at_threshold, found[2]; // counts of this CTA; digit and rest
+    __shared__ uint32_t scan[SWARPS][2];
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, t = lane & 3;
+    const int32_t ctas = gridDim.x, rank = blockIdx.x; // one cluster along x
+    const int64_t item = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+    if (item >= p.items) return; // (the whole cluster)
+    const int64_t b = item / p.kv_heads;
+    const int32_t kvh = (int32_t)(item - b * p.kv_heads);
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+    const int32_t n = (int32_t)min((int64_t)max(p.lengths[b], 0), p.tokens_in_table);
+    const int32_t blocks = (uint32_t)((uint64_t)(uint32_t)(n + p.block - 1) * p.block_magic >> p.block_shift);
+    const int32_t* const row_pages = p.pages + b * p.pages_stride;
+    int32_t* const list = p.lists + item * p.total;
+    int32_t* const told = p.optional_blocks ? p.optional_blocks + item * p.total : nullptr;
+    const int32_t count = min(blocks, p.total);
+    auto put = [&](int32_t at, int32_t block) {
+        const int32_t index = (uint32_t)((uint64_t)(uint32_t)block * p.page_magic >> p.page_shift), page = row_pages[index];
+        list[at] = (uint32_t)page < (uint32_t)p.num_pages ? page * p.per_page + (block - index * p.per_page) : -1;
+        if (told) told[at] = block;
+    };
+    if (rank == 0 && kvh == 0 && threadIdx.x == 0) p.listed_tokens[b] = count == 0 ? 0 : n - (blocks - count) * p.block;
+    if (told)
+        for (int32_t i = count + rank * STPB + threadIdx.x; i < p.total; i += ctas * STPB) told[i] = -1;
+    if (blocks <= p.total) { // all of them
+        for (int32_t i = rank * STPB + threadIdx.x; i < count; i += ctas * STPB) put(i, i);
+        return;
+    }
+    if (rank == 0) {
+        for (int32_t i = threadIdx.x; i < p.first; i += STPB) put(i, i);
+        for (int32_t i = threadIdx.x; i < p.last; i += STPB) put(p.first + p.top + i, blocks - p.last + i);
+    }
+    const int32_t between = blocks - p.first - p.last; // more than p.top
+    if (p.top == 0) return;
+
+    // ---- scores of this CTA's share ------------------------------------------------------------------------------------------
+    const int32_t share = (between + ctas * 16 - 1) / (ctas * 16) * 16;
+    const int32_t begin = min(between, rank * share), mine = min(between, begin + share) - begin;
+    for (int32_t head0 = 0; head0 < p.shared; head0 += 8) {
+        const int heads = min(8, p.shared - head0);
+        const half* const q = p.q + b * p.q_stride + (int64_t)(kvh * p.shared + head0) * D;
+        if (threadIdx.x < 8) q_bits[threadIdx.x] = 0;
+        for (int x = threadIdx.x; x < 4 * 256 && head0 == 0; x += STPB) histogram[x >> 8][x & 255] = 0;
+        __syncthreads();
+        for (int x = threadIdx.x; x < heads * (D / 8); x += STPB) {
+            const uint4 raw = ld_global_16(q + x * 8);
+            const uint32_t w[4] = {raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu, raw.z & 0x7fff7fffu, raw.w & 0x7fff7fffu};
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = max(m, max(w[i] & 0xffffu, w[i] >> 16));
+            atomicMax(&q_bits[x / (D / 8)], m);
+        }
+        __syncthreads();
+        for (int x = threadIdx.x; x < 8 * (D / 8); x += STPB) {
+            const int h = x / (D / 8);
+            uint32_t o[2] = {};
+            if (h < heads && q_bits[h] < 0x7c00u) {
+                const uint4 raw = ld_global_16(q + x * 8);
+                const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+                const float s = __half2float(outer_scale(__half2float(__ushort_as_half((unsigned short)q_bits[h]))));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float v = __half2float(__ushort_as_half((unsigned short)(w[i >> 1] >> (16 * (i & 1)))));
+                    o[i >> 2] |= (uint32_t)(__float2int_rn(__fdiv_rn(v, s)) & 0xff) << (8 * (i & 3));
+                }
+            }
+            q8[h][(x - h * (D / 8)) * 2] = o[0];
+            q8[h][(x - h * (D / 8)) * 2 + 1] = o[1];
+        }
+        __syncthreads();
+        // a product's dimensions come as the lane has them: words 2 m and 2 m + 1 of its own
+        uint32_t plus[MMAS][2], minus[MMAS][2];
+#pragma unroll
+        for (int m = 0; m < MMAS; ++m)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int word = 2 * m + x, i = word / KW, s = word - i * KW;
+                const uint32_t w = q8[g][(i * 4 + t) * KW + s];
+                plus[m][x] = __vmaxs4(w, 0);
+                minus[m][x] = __vmins4(w, 0);
+            }
+        float qs[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) { // heads 2 t and 2 t + 1; one without a say or beyond the last: NaN
+            const int h = 2 * t + x;
+            qs[x] = h < heads && q_bits[h] < 0x7c00u ? __half2float(outer_scale(__half2float(__ushort_as_half((unsigned short)q_bits[h])))) : __int_as_float(0x7fffffff);
+        }
+        for (int32_t tile = warp * 16; tile < mine; tile += SWARPS * 16) {
+            uint32_t lo[2][KN][KW], hi[2][KN][KW];
+            half scale[2];
+            bool there[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int32_t x = min(tile + g + 8 * r, mine - 1), block = p.first + begin + x;
+                const int32_t index = (uint32_t)((uint64_t)(uint32_t)block * p.page_magic >> p.page_shift), page = row_pages[index];
+                there[r] = (uint32_t)page < (uint32_t)p.num_pages;
+                const int64_t at = ((int64_t)(there[r] ? page : 0) * p.kv_heads + kvh) * p.per_page + (block - index * p.per_page);
+                const char* src = (const char*)p.bounds + at * 2 * D + t * KP;
+#pragma unroll
+                for (int i = 0; i < KN; ++i) {
+#pragma unroll
+                    for (int w = 0; w < KW; ++w) lo[r][i][w] = hi[r][i][w] = 0;
+                    if (there[r]) {
+                        load_piece<KP>(lo[r][i], src + i * 4 * KP);
+                        load_piece<KP>(hi[r][i], src + D + i * 4 * KP);
+                    }
+                }
+                scale[r] = there[r] ? ld_global_half(p.scale + at) : __ushort_as_half(0);
+            }
+            int32_t c[4] = {}, c2[4] = {};
+#pragma unroll
+            for (int m = 0; m < MMAS; ++m) {
+                constexpr int W = KW;
+                const int w = 2 * m, i = w / W, s = w - i * W;
+                mma_s8(c, lo[0][i][s], lo[1][i][s], lo[0][i][s + 1], lo[1][i][s + 1], minus[m][0], minus[m][1]);
+                mma_s8(c2, hi[0][i][s], hi[1][i][s], hi[0][i][s + 1], hi[1][i][s + 1], plus[m][0], plus[m][1]);
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float f = __half2float(scale[r]);
+                uint32_t key = 0;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const float score = __fmul_rn((float)(c[2 * r + x] + c2[2 * r + x]), qs[x] * f);
+                    if (qs[x] == qs[x]) key = max(key, ordered(score));
+                }
+                key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
+                key = max(key, __shfl_xor_sync(0xffffffffu, key, 2));
+                if (!is_finite(scale[r])) key = 0xffffffffu;
+                if (!there[r]) key = 0;
+                // a score that is there is 1 at least, so that holes come behind it
+                if (there[r]) key = max(key, 1u);
+                const int32_t x = tile + g + 8 * r;
+                if (t == 0 && x < mine) keys[x] = head0 == 0 ? key : max(keys[x], key);
+            }
+        }
+        __syncthreads();
+    }
+
+    // ---- the threshold: the top-th largest key, digit by digit ------------------------------------------------------------------
+    uint32_t prefix = 0, room = p.top; // of the keys that begin with prefix, `room` are taken
+    const uint32_t hist0 = map_to_cta(ptx::smem_addr(histogram), 0);
+    cluster_sync_all(); // the first CTA's histograms are zero
+    for (int digit = 0; digit < 4; ++digit) {
+        const int shift = 24 - 8 * digit;
+        for (int32_t x = threadIdx.x; x < mine; x += STPB) {
+            const uint32_t key = keys[x];
+            if (digit == 0 || key >> (shift + 8) == prefix) add_in_cluster(hist0 + (digit * 256 + (key >> shift & 255u)) * 4, 1);
+        }
+        cluster_sync_all();
+        // bins from the highest down: thread x has bin 255 - x
+        const uint32_t bin = 255 - threadIdx.x, mine_here = ld_in_cluster(hist0 + (digit * 256 + bin) * 4);
+        uint32_t sum = mine_here;
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, sum, m);
+            if (lane >= m) sum += v;
+        }
+        if (lane == 31) scan[warp][0] = sum;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) sum += scan[w][0];
+        if (sum >= room && sum - mine_here < room) found[0] = bin, found[1] = room - (sum - mine_here);
+        __syncthreads();
+        prefix = prefix << 8 | found[0];
+        room = found[1];
+        __syncthreads();
+    }
+
+    // ---- what is above the threshold, and the first `room` of those at it, in order ------------------------------------------------
+    if (threadIdx.x == 0) above = at_threshold = 0;
+    __syncthreads();
+    uint32_t counts[2] = {};
+    for (int32_t x = threadIdx.x; x < mine; x += STPB) {
+        counts[0] += keys[x] > prefix;
+        counts[1] += keys[x] == prefix;
+    }
+    if (counts[0]) atomicAdd(&above, counts[0]);
+    if (counts[1]) atomicAdd(&at_threshold, counts[1]);
+    cluster_sync_all();
+    uint32_t before[2] = {};
+    for (int32_t r = 0; r < rank; ++r) {
+        before[0] += ld_in_cluster(map_to_cta(ptx::smem_addr(&above), r));
+        before[1] += ld_in_cluster(map_to_cta(ptx::smem_addr(&at_threshold), r));
+    }
+    for (int32_t x0 = 0; x0 < mine; x0 += STPB) {
+        const int32_t x = x0 + threadIdx.x;
+        const uint32_t key = x < mine ? keys[x] : 0u;
+        const bool over = x < mine && key > prefix, same = x < mine && key == prefix;
+        const uint32_t overs = __ballot_sync(0xffffffffu, over), sames = __ballot_sync(0xffffffffu, same), below = (1u << lane) - 1;
+        if (lane == 0) scan[warp][0] = __popc(overs), scan[warp][1] = __popc(sames);
+        __syncthreads();
+        uint32_t o = before[0] + __popc(overs & below), s = before[1] + __popc(sames & below);
+        for (int w = 0; w < SWARPS; ++w) {
+            if (w < warp) o += scan[w][0], s += scan[w][1];
+            before[0] += scan[w][0];
+            before[1] += scan[w][1];
+        }
+        if (over || (same && s < room)) put(p.first + o + min(s, room), p.first + begin + x);
+        __syncthreads();
+    }
+    cluster_sync_all(); // no CTA leaves while another reads its shared memory
+}
+
+int32_t check_bounds(const pplb200_kv_cache* c, const pplb200_key_bounds* k) {
+    const int32_t rc = check_kv_cache(c);
+    if (rc != RC_SUCCESS) return rc;
+    if (!k) return fail(RC_INVALID_VALUE, "null bounds");
+    if (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128 && c->head_dim != 256)
+        return fail(RC_UNSUPPORTED, "key bounds: head_dim must be 64, 96, 128 or 256, got %d", c->head_dim);
+    if (k->block <= 0 || k->block % 16 || c->page_size % k->block)
+        return fail(RC_INVALID_VALUE, "a block must be a multiple of 16 tokens that divides a page (%d), got %d", c->page_size, k->block);
+    if (c->num_pages == 0) return RC_SUCCESS;
+    if (!k->bounds || !k->scale || !aligned16(k->bounds) || ((uintptr_t)k->scale & 1)) return fail(RC_INVALID_VALUE, "bounds must be 16-byte, their scales 2-byte aligned pointers");
+    if ((__int128)c->num_pages * c->kv_heads * (c->page_size / k->block) * 2 * c->head_dim >> 61) return fail(RC_INVALID_VALUE, "bounds of too many blocks");
+    return RC_SUCCESS;
+}
+
+int64_t list_bytes(int64_t batch, int32_t kv_heads, int64_t total) { return round_up(batch * kv_heads * total * 4, 256) + round_up(batch * 4, 256); }
+
+template <int D>
+int32_t launch_choice(cudaStream_t stream, const ChoiceParams& p, int32_t cluster) {
+    const int64_t y = std::min<int64_t>(p.items, 32768);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)cluster, (unsigned)y, (unsigned)((p.items + y - 1) / y));
+    cfg.blockDim = dim3(STPB);
+    cfg.dynamicSmemBytes = (size_t)p.share * 4;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    if (cfg.dynamicSmemBytes > 32768) { // beyond what a kernel has without being asked for, its static 7 KB included
+        const cudaError_t e = cudaFuncSetAttribute(choose_blocks_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+        if (e != cudaSuccess) return fail(RC_DEVICE_RUNTIME_ERROR, "choice of blocks: %s", cudaGetErrorString(e));
+    }
+    cudaLaunchKernelEx(&cfg, choose_blocks_kernel<D>, p);
+    return check_launch("choice of blocks");
+}
+
+} // namespace
+} // namespace pplb200
+
+using namespace pplb200;
+
+extern "C" {
+
+int32_t pplb200_key_bounds_update(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_key_bounds* bounds, const int64_t* slots, int64_t tokens) {
+    const int32_t rc = check_bounds(cache, bounds);
+    if (rc != RC_SUCCESS) return rc;
+    if (tokens < 0) return fail(RC_INVALID_VALUE, "negative extent");
+    if (tokens > 0x7fffffffLL) return fail(RC_UNSUPPORTED, "more than 2^31 - 1 tokens");
+    if (tokens == 0) return RC_SUCCESS;
+    if (!slots || ((uintptr_t)slots & 7)) return fail(RC_INVALID_VALUE, "slots must be an 8-byte aligned pointer");
+    if (cache->num_pages == 0) return RC_SUCCESS;
+    BoundsParams p = {};
+    p.cache = *cache;
+    p.bounds = (int8_t*)bounds->bounds; p.scale = (half*)bounds->scale;
+    p.slots = slots; p.tokens = tokens;
+    p.block = bounds->block; p.per_page = cache->page_size / bounds->block;
+    small_division(p.block, p.block_magic, p.block_shift);
+    // one slot a CTA while that makes no more than eight CTAs an SM, then as many as a block has, so that a prompt's CTA has one block
+    p.slots_here = (int32_t)std::min<int64_t>(std::min(p.block, BTPB), std::max<int64_t>(1, tokens * cache->kv_heads / (8 * kSms)));
+    const dim3 grid((unsigned)((tokens + p.slots_here - 1) / p.slots_here), (unsigned)cache->kv_heads);
+    if (cache->quant_group == 0) launch_ex(key_bounds_kernel<CACHE_F16>, grid, dim3(BTPB), (cudaStream_t)stream, true, p);
+    else if (cache->quant_group == 8) launch_ex(key_bounds_kernel<CACHE_I8_GROUPS>, grid, dim3(BTPB), (cudaStream_t)stream, true, p);
+    else launch_ex(key_bounds_kernel<CACHE_I8_ROWS>, grid, dim3(BTPB), (cudaStream_t)stream, true, p);
+    return check_launch("key bounds");
+}
+
+int32_t pplb200_key_bounds_read(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_key_bounds* bounds, const int64_t* blocks, int64_t count,
+                                float* lo, float* hi) {
+    const int32_t rc = check_bounds(cache, bounds);
+    if (rc != RC_SUCCESS) return rc;
+    if (count < 0) return fail(RC_INVALID_VALUE, "negative extent");
+    if (count == 0) return RC_SUCCESS;
+    if (!blocks || ((uintptr_t)blocks & 7)) return fail(RC_INVALID_VALUE, "blocks must be an 8-byte aligned pointer");
+    if (!lo || !hi || !aligned16(lo) || !aligned16(hi)) return fail(RC_INVALID_VALUE, "lo and hi must be 16-byte aligned pointers");
+    if (count > (1LL << 38) / (cache->kv_heads * (int64_t)cache->head_dim)) return fail(RC_UNSUPPORTED, "too many elements");
+    BoundsReadParams p = {};
+    p.bounds = (const int8_t*)bounds->bounds; p.scale = (const half*)bounds->scale;
+    p.blocks = blocks; p.lo = lo; p.hi = hi; p.count = count;
+    p.per_page = cache->page_size / bounds->block; p.kv_heads = cache->kv_heads; p.head_dim = cache->head_dim;
+    p.all_blocks = cache->num_pages * p.per_page;
+    const int64_t shares = ((int64_t)p.kv_heads * p.head_dim / 2 + BTPB - 1) / BTPB;
+    launch_ex(key_bounds_read_kernel, dim3((unsigned)std::min<int64_t>(count, 1 << 20), (unsigned)std::min<int64_t>(shares, 65535)), dim3(BTPB), (cudaStream_t)stream, true, p);
+    return check_launch("key bounds read");
+}
+
+int64_t pplb200_block_sparse_attention_workspace_bytes(int64_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t attended_blocks) {
+    if (batch < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0 || attended_blocks < 0 || batch > MAX_ITEMS / kv_heads) return -1;
+    return workspace_bytes(q_heads / kv_heads, head_dim) + list_bytes(batch, kv_heads, attended_blocks);
+}
+
+int32_t pplb200_block_sparse_attention_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_key_bounds* bounds,
+                                            const pplb200_paged_attention_args* a, const pplb200_block_choice* choice) {
+    AttentionParams own = {};
+    int32_t rc = take_call(cache, a, own);
+    if (rc != RC_SUCCESS) return rc;
+    if ((rc = check_bounds(cache, bounds)) != RC_SUCCESS) return rc;
+    if (!choice) return fail(RC_INVALID_VALUE, "null choice");
+    if (a->window) return fail(RC_UNSUPPORTED, "chosen blocks are not seen through a window");
+    if (choice->first < 0 || choice->last < 1 || choice->top < 0) return fail(RC_INVALID_VALUE, "first and top must not be negative, last at least 1");
+    const int64_t total = (int64_t)choice->first + choice->last + choice->top;
+    const int64_t per_page = cache->page_size / bounds->block, in_table = a->pages_per_sequence * per_page;
+    if (total > MAX_TOTAL || total * bounds->block > (1LL << 30)) return fail(RC_UNSUPPORTED, "too many blocks to attend: %lld", (long long)total);
+    if (in_table > MAX_BLOCKS) return fail(RC_UNSUPPORTED, "a page table of more than 2^18 blocks");
+    if ((__int128)cache->num_pages * per_page > 0x7fffffff) return fail(RC_UNSUPPORTED, "a cache of 2^31 blocks");
+    if (a->batch > MAX_ITEMS / cache->kv_heads) return fail(RC_UNSUPPORTED, "more than 2^24 choices");
+    if ((uintptr_t)choice->optional_blocks & 3) return fail(RC_INVALID_VALUE, "the chosen blocks must be 4-byte aligned");
+    if (a->batch == 0) return RC_SUCCESS;
+    const int64_t need = pplb200_block_sparse_attention_workspace_bytes(a->batch, a->q_heads, cache->kv_heads, cache->head_dim, (int32_t)total);
+    if (!a->ws || a->ws_bytes < need || ((uintptr_t)a->ws & 255))
+        return fail(RC_INVALID_VALUE, "workspace of %lld bytes (256-byte aligned) needed, got %lld", (long long)need, (long long)a->ws_bytes);
+    int32_t* const lists = (int32_t*)((char*)a->ws + need - list_bytes(a->batch, cache->kv_heads, total));
+    ChoiceParams p = {};
+    p.q = own.q; p.q_stride = own.q_stride; p.pages = own.pages; p.pages_stride = own.pages_stride; p.lengths = own.lengths;
+    p.bounds = (const int8_t*)bounds->bounds; p.scale = (const half*)bounds->scale;
+    p.lists = lists;
+    p.listed_tokens = (int32_t*)((char*)lists + round_up(a->batch * cache->kv_heads * total * 4, 256));
+    p.optional_blocks = choice->optional_blocks;
+    p.tokens_in_table = own.tokens_in_table;
+    p.items = a->batch * cache->kv_heads;
+    p.kv_heads = cache->kv_heads; p.shared = a->q_heads / cache->kv_heads;
+    p.block = bounds->block; p.per_page = (int32_t)per_page; p.num_pages = own.num_pages;
+    p.first = choice->first; p.last = choice->last; p.top = choice->top; p.total = (int32_t)total;
+    small_division(p.block, p.block_magic, p.block_shift);
+    small_division(p.per_page, p.page_magic, p.page_shift);
+    // CTAs of a choice: two on an SM, a round of 16 blocks a warp for each, and no more than 128 KB of scores
+    int32_t cluster = 1;
+    while (cluster < MAX_CLUSTER && ((p.items * cluster * 2 <= 2 * kSms && in_table > cluster * SWARPS * 16) || in_table > cluster * 32768LL)) cluster *= 2;
+    p.share = (int32_t)std::max<int64_t>(16, (in_table + cluster * 16 - 1) / (cluster * 16) * 16);
+    const cudaStream_t s = (cudaStream_t)stream;
+    if (cache->head_dim == 64) rc = launch_choice<64>(s, p, cluster);
+    else if (cache->head_dim == 96) rc = launch_choice<96>(s, p, cluster);
+    else if (cache->head_dim == 128) rc = launch_choice<128>(s, p, cluster);
+    else rc = launch_choice<256>(s, p, cluster);
+    if (rc != RC_SUCCESS) return rc;
+    own.pages = lists;
+    own.pages_stride = cache->kv_heads * total;
+    own.pages_head_stride = total;
+    own.lengths = p.listed_tokens;
+    own.tokens_in_table = total * bounds->block;
+    own.unit_tokens = bounds->block;
+    own.units_per_page = (int32_t)per_page;
+    own.num_units = (int32_t)(own.num_pages * per_page);
+    own.rows_per_head = p.shared;
+    lay_out(own, a->ws, p.shared);
+    return launch_general(s, own);
+}
+
+} // extern "C"

@@ -49,8 +49,10 @@ struct RotaryKvParams {
     int32_t heads[3], turns_of[3]; // rows of a token, and how many of them a thread takes at most
     const int64_t *positions, *slots;
     const uint64_t* turns;
+    const uint8_t* axis_of_plane; // axes > 0: positions of several axes, axis_stride apart
+    int64_t axis_stride;
     int64_t tokens;
-    int32_t head_dim, rotary_dim, interleaved;
+    int32_t head_dim, rotary_dim, interleaved, axes;
     float magnitude;
     int32_t store; // keys go to the cache instead of dst[K], values too
     int32_t groups;                    // threads that share a token's rows, for each 16 dimensions
@@ -133,6 +135,24 @@ __device__ __forceinline__ void turns_at(Turns& t, uint64_t position, const uint
         t.s[i] *= magnitude;
     }
 }
+// The same where each plane has an axis, and the token a position on each: all of them are loaded side by side, and each plane picks its
+// own (three selections beside some forty instructions of a sine and cosine: 8192 tokens of 72 heads take what they take with one axis).
+struct AxisPositions {
+    uint64_t at[PPLB200_ROTARY_MAX_AXES];
+    uint32_t first, second; // axes of four and four planes
+    __device__ __forceinline__ uint64_t of(int i) const {
+        const uint32_t axis = (i < 4 ? first : second) >> (8 * (i & 3)) & 0xffu;
+        return axis == 0 ? at[0] : axis == 1 ? at[1] : axis == 2 ? at[2] : at[3];
+    }
+};
+__device__ __forceinline__ void turns_at(Turns& t, const AxisPositions& position, const uint64_t* first, const uint64_t* second, float magnitude) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        sincospif((float)(int64_t)(position.of(i) * (i < 4 ? first[i] : second[i - 4])) * 0x1p-63f, &t.s[i], &t.c[i]);
+        t.c[i] *= magnitude;
+        t.s[i] *= magnitude;
+    }
+}
 // a and b against each other, or (interleaved) neighbours within a and within b.
 __device__ __forceinline__ void rotate(Eight& a, Eight& b, const Turns& t, bool interleaved) {
 #pragma unroll
@@ -156,7 +176,7 @@ __device__ __forceinline__ void rotate(Eight& a, Eight& b, const Turns& t, bool 
 constexpr int RTPB = 128;
 enum : int { AS_IS = 0, HALVES = 1, INTERLEAVED = 2 }; // what is rotated against what; AS_IS keeps sixteen registers free
 enum : int { NO_STORE = 0, STORE_F16 = 1, STORE_I8_GROUPS = 2, STORE_I8_ROWS = 3 };
-template <int LANES, int LAYOUT, int STORE>
+template <int LANES, int LAYOUT, int STORE, bool AXES>
 struct RotaryKv {
     struct Row {
         Eight a, b;
@@ -250,11 +270,11 @@ struct RotaryKv {
 // branches around the loads, keys and values one after the other and a run-time choice of the cache's type).  CTAs that share an
 // SM were tried from 5 to 10 (at the bounds taken, the forms that store int8 rows spill 8 to 16 bytes): unrotated, 10 spill more (24.4 us), 6 take as long as 8 but 8.9 instead of 8.2 us for 4096 tokens in groups of 8; rotated, into groups of 8,
 // 2048 tokens of 32 + 32 heads, 22.6 us with 7, 24 with 6.
-template <int LANES, int LAYOUT, int STORE>
+template <int LANES, int LAYOUT, int STORE, bool AXES>
 __global__ void __launch_bounds__(RTPB, LAYOUT == AS_IS ? 8 : 7) rotary_kv_kernel(const __grid_constant__ RotaryKvParams p) {
     pdl_wait_prior_grid();
     const uint32_t n = blockIdx.x * (RTPB / LANES) + threadIdx.x / LANES;
-    RotaryKv<LANES, LAYOUT, STORE> r{p};
+    RotaryKv<LANES, LAYOUT, STORE, AXES> r{p};
     r.token = (uint32_t)((uint64_t)n * p.group_magic >> p.group_shift);
     const int group = n - (uint32_t)r.token * p.groups;
     const bool valid = r.token < p.tokens;
@@ -267,13 +287,24 @@ __global__ void __launch_bounds__(RTPB, LAYOUT == AS_IS ? 8 : 7) rotary_kv_kerne
     r.da = behind < 0 ? 8 * r.u : p.rotary_dim + 8 * behind;
     r.db = r.da + ((behind < 0 ? p.rotary_dim : p.head_dim - p.rotary_dim) >> 1);
     if (!r.active) r.da = 0, r.db = 0;
-    typename RotaryKv<LANES, LAYOUT, STORE>::Row q, k, v;
+    typename RotaryKv<LANES, LAYOUT, STORE, AXES>::Row q, k, v;
     if (p.turns_of[Q] > 0) r.template fetch<Q>(group, q);
     if (p.turns_of[K] > 0) r.template fetch<K>(group, k);
     if (STORE) r.template fetch<V>(group, v);
     if (LAYOUT != AS_IS && r.turned) {
         const uint64_t* first = p.turns + (LAYOUT == INTERLEAVED ? 4 : 8) * r.u; // planes of the runs: eight of both, or four of each
-        turns_at(r.turns, (uint64_t)p.positions[r.token], first, first + (LAYOUT == INTERLEAVED ? p.rotary_dim >> 2 : 4), p.magnitude);
+        const int apart = LAYOUT == INTERLEAVED ? p.rotary_dim >> 2 : 4;
+        if constexpr (AXES) {
+            AxisPositions at;
+            const uint8_t* axis = p.axis_of_plane + (first - p.turns);
+            at.first = *reinterpret_cast<const uint32_t*>(axis);
+            at.second = *reinterpret_cast<const uint32_t*>(axis + apart);
+#pragma unroll
+            for (int a = 0; a < PPLB200_ROTARY_MAX_AXES; ++a) at.at[a] = (uint64_t)p.positions[min(a, p.axes - 1) * p.axis_stride + r.token];
+            turns_at(r.turns, at, first, first + apart, p.magnitude);
+        } else {
+            turns_at(r.turns, (uint64_t)p.positions[r.token], first, first + apart, p.magnitude);
+        }
     }
     r.at = -1;
     r.scale_at = 0;
@@ -299,9 +330,9 @@ __global__ void __launch_bounds__(RTPB, LAYOUT == AS_IS ? 8 : 7) rotary_kv_kerne
 
 template <int LANES, int STORE>
 void launch_stored(cudaStream_t stream, const RotaryKvParams& p, dim3 grid) {
-    if (p.rotary_dim == 0 && STORE != NO_STORE) launch_ex(rotary_kv_kernel<LANES, STORE != NO_STORE ? AS_IS : HALVES, STORE>, grid, dim3(RTPB), stream, true, p);
-    else if (p.interleaved) launch_ex(rotary_kv_kernel<LANES, INTERLEAVED, STORE>, grid, dim3(RTPB), stream, true, p);
-    else launch_ex(rotary_kv_kernel<LANES, HALVES, STORE>, grid, dim3(RTPB), stream, true, p);
+    if (p.rotary_dim == 0 && STORE != NO_STORE) launch_ex(rotary_kv_kernel<LANES, STORE != NO_STORE ? AS_IS : HALVES, STORE, false>, grid, dim3(RTPB), stream, true, p);
+    else if (p.interleaved) launch_ex(p.axes ? rotary_kv_kernel<LANES, INTERLEAVED, STORE, true> : rotary_kv_kernel<LANES, INTERLEAVED, STORE, false>, grid, dim3(RTPB), stream, true, p);
+    else launch_ex(p.axes ? rotary_kv_kernel<LANES, HALVES, STORE, true> : rotary_kv_kernel<LANES, HALVES, STORE, false>, grid, dim3(RTPB), stream, true, p);
 }
 template <int LANES>
 int32_t launch_lanes(cudaStream_t stream, RotaryKvParams& p) {
@@ -420,25 +451,24 @@ int32_t check_rows(const char* name, const void* p, int64_t stride, int64_t head
     return RC_SUCCESS;
 }
 
-} // namespace
-} // namespace pplb200
-
-using namespace pplb200;
-
-extern "C" {
-
-int32_t pplb200_rotary_frequencies(int32_t rotary_dim, double base, int32_t scaling, double factor, double original_length,
-                                   double keep_turns, double stretch_turns, uint64_t* turns_host, float* magnitude_host) {
+// What is wrong with a scaling, or RC_SUCCESS.
+int32_t check_scaling(int32_t rotary_dim, double base, int32_t scaling, double factor, double original_length, double keep_turns, double stretch_turns) {
     if (rotary_dim <= 0 || rotary_dim % 16 || rotary_dim > kMaxHeadDim)
         return fail(RC_INVALID_VALUE, "rotary_dim must be a multiple of 16 up to %d, got %d", kMaxHeadDim, rotary_dim);
     if (scaling < PPLB200_ROTARY_NONE || scaling > PPLB200_ROTARY_WAVELENGTH) return fail(RC_UNSUPPORTED, "unknown rotary scaling %d", scaling);
-    if (!turns_host || !magnitude_host) return fail(RC_INVALID_VALUE, "null pointer");
     if (!(base > 1.0) || !std::isfinite(base)) return fail(RC_INVALID_VALUE, "the base must be above 1");
     if (scaling != PPLB200_ROTARY_NONE && (!(factor >= 1.0) || !std::isfinite(factor))) return fail(RC_INVALID_VALUE, "the factor must be at least 1");
     const bool blend = scaling == PPLB200_ROTARY_YARN || scaling == PPLB200_ROTARY_WAVELENGTH;
     if (blend && (!(original_length > 0.0) || !std::isfinite(original_length) || !(stretch_turns > 0.0) || !(keep_turns > stretch_turns) || !std::isfinite(keep_turns)))
         return fail(RC_INVALID_VALUE, "a blend needs original_length > 0 and keep_turns > stretch_turns > 0");
-    // The frequencies in 64-bit mantissas (long double): a word is off by a few of its units, and an angle by that times the position.
+    return RC_SUCCESS;
+}
+
+// The words of a scaling that has been checked: put(i, word) for each of rotary_dim / 2 planes; returns the factor on the values.
+// The frequencies in 64-bit mantissas (long double): a word is off by a few of its units, and an angle by that times the position.
+template <class Put>
+float turn_words(int32_t rotary_dim, double base, int32_t scaling, double factor, double original_length, double keep_turns, double stretch_turns, Put put) {
+    const bool blend = scaling == PPLB200_ROTARY_YARN || scaling == PPLB200_ROTARY_WAVELENGTH;
     const long double two_pi = 6.283185307179586476925286766559005768L, ld_base = base, ld_factor = factor;
     const double rd = rotary_dim, turn = (double)two_pi;
     const long double b = scaling == PPLB200_ROTARY_NTK ? ld_base * std::pow(ld_factor, (long double)rd / (rd - 2.0)) : ld_base;
@@ -449,7 +479,7 @@ int32_t pplb200_rotary_frequencies(int32_t rotary_dim, double base, int32_t scal
         last = std::fmin(std::ceil(rd * std::log(original_length / (stretch_turns * turn)) / (2.0 * std::log(base))), rd - 1.0);
     }
     for (int32_t i = 0; i < rotary_dim / 2; ++i) {
-        long double f = std::pow(b, -2.0L * i / rd);
+        long double f = i ? std::pow(b, -2.0L * i / rd) : 1.0L;
         if (scaling == PPLB200_ROTARY_LINEAR) f /= ld_factor;
         if (blend) {
             const long double keep = scaling == PPLB200_ROTARY_YARN ? 1.0L - (i - first) / (long double)std::fmax(last - first, 0.001)
@@ -457,13 +487,24 @@ int32_t pplb200_rotary_frequencies(int32_t rotary_dim, double base, int32_t scal
             const long double part = std::fmin(std::fmax(keep, 0.0L), 1.0L);
             f = f * part + f / ld_factor * (1.0L - part);
         }
-        turns_host[i] = (uint64_t)std::floor(f / two_pi * 0x1p64L + 0.5L); // f <= 1: below 2^62
+        put(i, (uint64_t)std::floor(f / two_pi * 0x1p64L + 0.5L)); // f <= 1: below 2^62
     }
-    *magnitude_host = scaling == PPLB200_ROTARY_YARN ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+    return scaling == PPLB200_ROTARY_YARN ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+}
+
+// RC_SUCCESS, with the axes in p, or what is wrong with them.
+int32_t take_axes(const pplb200_rotary_axes* axes, int64_t tokens, RotaryKvParams& p) {
+    if (!axes) return fail(RC_INVALID_VALUE, "null axes");
+    if (axes->axes < 1 || axes->axes > PPLB200_ROTARY_MAX_AXES) return fail(RC_UNSUPPORTED, "1 to %d axes, got %d", PPLB200_ROTARY_MAX_AXES, axes->axes);
+    if (!axes->axis_of_plane || ((uintptr_t)axes->axis_of_plane & 3)) return fail(RC_INVALID_VALUE, "axis_of_plane must be a 4-byte aligned pointer");
+    if (axes->axis_stride < 0 || (axes->axes > 1 && axes->axis_stride < tokens)) return fail(RC_INVALID_VALUE, "the positions of the axes overlap");
+    p.axis_of_plane = axes->axis_of_plane;
+    p.axis_stride = axes->axis_stride;
+    p.axes = axes->axes;
     return RC_SUCCESS;
 }
 
-int32_t pplb200_rotary_fp16(pplb200_stream_t stream, const pplb200_rotary_args* a) {
+int32_t rotary_call(pplb200_stream_t stream, const pplb200_rotary_args* a, const pplb200_rotary_axes* axes, bool several) {
     if (!a) return fail(RC_INVALID_VALUE, "null arguments");
     if (a->tokens < 0) return fail(RC_INVALID_VALUE, "negative extent");
     if (a->tokens > 0x7fffffffLL) return fail(RC_UNSUPPORTED, "more than 2^31 - 1 tokens");
@@ -477,6 +518,7 @@ int32_t pplb200_rotary_fp16(pplb200_stream_t stream, const pplb200_rotary_args* 
     if (rc == RC_SUCCESS) rc = check_rows("k_out", a->k_out, a->k_out_stride, a->k_heads, a->head_dim, a->tokens);
     if (rc != RC_SUCCESS) return rc;
     RotaryKvParams p = {};
+    if (several && (rc = take_axes(axes, a->tokens, p)) != RC_SUCCESS) return rc;
     p.src[0] = (const half*)a->q; p.src[1] = (const half*)a->k;
     p.dst[0] = (half*)a->q_out; p.dst[1] = (half*)a->k_out;
     p.src_stride[0] = a->q_stride; p.src_stride[1] = a->k_stride;
@@ -488,7 +530,7 @@ int32_t pplb200_rotary_fp16(pplb200_stream_t stream, const pplb200_rotary_args* 
     return launch_rotary_kv((cudaStream_t)stream, p);
 }
 
-int32_t pplb200_kv_cache_write_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_kv_write_args* a) {
+int32_t write_call(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_kv_write_args* a, const pplb200_rotary_axes* axes, bool several) {
     int32_t rc = check_kv_cache(cache);
     if (rc != RC_SUCCESS) return rc;
     if (!a) return fail(RC_INVALID_VALUE, "null arguments");
@@ -504,6 +546,8 @@ int32_t pplb200_kv_cache_write_fp16(pplb200_stream_t stream, const pplb200_kv_ca
     if (rc == RC_SUCCESS) rc = check_rows("v", a->v, a->v_stride, cache->kv_heads, cache->head_dim, a->tokens);
     if (rc != RC_SUCCESS) return rc;
     RotaryKvParams p = {};
+    if (several && (rc = take_axes(axes, a->tokens, p)) != RC_SUCCESS) return rc;
+    if (several && !a->rotary_dim) return fail(RC_INVALID_VALUE, "axes without rotary_dim");
     p.src[0] = (const half*)a->q; p.src[1] = (const half*)a->k; p.src[2] = (const half*)a->v;
     p.dst[0] = (half*)a->q_out;
     p.src_stride[0] = a->q_stride; p.src_stride[1] = a->k_stride; p.src_stride[2] = a->v_stride;
@@ -515,6 +559,66 @@ int32_t pplb200_kv_cache_write_fp16(pplb200_stream_t stream, const pplb200_kv_ca
     p.store = 1;
     p.cache = *cache;
     return launch_rotary_kv((cudaStream_t)stream, p);
+}
+
+} // namespace
+} // namespace pplb200
+
+using namespace pplb200;
+
+extern "C" {
+
+int32_t pplb200_rotary_frequencies(int32_t rotary_dim, double base, int32_t scaling, double factor, double original_length,
+                                   double keep_turns, double stretch_turns, uint64_t* turns_host, float* magnitude_host) {
+    const int32_t rc = check_scaling(rotary_dim, base, scaling, factor, original_length, keep_turns, stretch_turns);
+    if (rc != RC_SUCCESS) return rc;
+    if (!turns_host || !magnitude_host) return fail(RC_INVALID_VALUE, "null pointer");
+    *magnitude_host = turn_words(rotary_dim, base, scaling, factor, original_length, keep_turns, stretch_turns, [&](int32_t i, uint64_t word) { turns_host[i] = word; });
+    return RC_SUCCESS;
+}
+
+int32_t pplb200_rotary_axes_frequencies(int32_t rotary_dim, double base, int32_t scaling, double factor, double original_length,
+                                        double keep_turns, double stretch_turns, int32_t axes, const int32_t* planes_host, int32_t alternating,
+                                        int32_t restart, uint64_t* turns_host, uint8_t* axis_of_plane_host, float* magnitude_host) {
+    const int32_t rc = check_scaling(rotary_dim, base, scaling, factor, original_length, keep_turns, stretch_turns);
+    if (rc != RC_SUCCESS) return rc;
+    if (!planes_host || !turns_host || !axis_of_plane_host || !magnitude_host) return fail(RC_INVALID_VALUE, "null pointer");
+    if (axes < 1 || axes > PPLB200_ROTARY_MAX_AXES) return fail(RC_UNSUPPORTED, "1 to %d axes, got %d", PPLB200_ROTARY_MAX_AXES, axes);
+    const int32_t planes = rotary_dim / 2;
+    int64_t together = 0;
+    for (int32_t a = 0; a < axes; ++a) {
+        if (planes_host[a] < 0) return fail(RC_INVALID_VALUE, "axis %d has %d planes", a, planes_host[a]);
+        together += planes_host[a];
+    }
+    if (together != planes) return fail(RC_INVALID_VALUE, "the axes have %lld planes together, of %d", (long long)together, planes);
+    int32_t left[PPLB200_ROTARY_MAX_AXES] = {}, at = 0;
+    for (int32_t a = 0; a < axes; ++a) left[a] = planes_host[a];
+    while (at < planes)
+        for (int32_t a = 0; a < axes; ++a)
+            for (int32_t n = alternating ? std::min(left[a], 1) : left[a]; n > 0; --n, --left[a]) axis_of_plane_host[at++] = (uint8_t)a;
+    if (!restart) {
+        *magnitude_host = turn_words(rotary_dim, base, scaling, factor, original_length, keep_turns, stretch_turns, [&](int32_t i, uint64_t word) { turns_host[i] = word; });
+        return RC_SUCCESS;
+    }
+    for (int32_t a = 0; a < axes; ++a) {
+        int32_t next = 0; // planes of the axis come in order
+        *magnitude_host = turn_words(2 * planes_host[a], base, scaling, factor, original_length, keep_turns, stretch_turns, [&](int32_t, uint64_t word) {
+            while (axis_of_plane_host[next] != a) ++next;
+            turns_host[next++] = word;
+        });
+    }
+    return RC_SUCCESS;
+}
+
+int32_t pplb200_rotary_fp16(pplb200_stream_t stream, const pplb200_rotary_args* args) { return rotary_call(stream, args, nullptr, false); }
+int32_t pplb200_rotary_axes_fp16(pplb200_stream_t stream, const pplb200_rotary_args* args, const pplb200_rotary_axes* axes) {
+    return rotary_call(stream, args, axes, true);
+}
+int32_t pplb200_kv_cache_write_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_kv_write_args* args) {
+    return write_call(stream, cache, args, nullptr, false);
+}
+int32_t pplb200_kv_cache_write_axes_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_kv_write_args* args, const pplb200_rotary_axes* axes) {
+    return write_call(stream, cache, args, axes, true);
 }
 
 int32_t pplb200_kv_cache_read_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache, const int64_t* slots, int64_t tokens,

@@ -678,7 +678,8 @@ def stream_read_probe(sizes=(16 << 20, 48 << 20, 384 << 20), pool_bytes=1536 << 
     return out
 
 
-_ATTENTION = ("PagedDecodeAttention", "PagedKVCache", "RotaryTable", "kv_cache_read", "kv_cache_write", "rotary_fp16", "rotary_kv_cache_write")
+_ATTENTION = ("BlockSparseDecodeAttention", "KeyBlockBounds", "PagedDecodeAttention", "PagedKVCache", "RotaryTable", "SharedPrefixDecodeAttention",
+              "key_bounds_read", "key_bounds_update", "kv_cache_read", "kv_cache_write", "rotary_fp16", "rotary_kv_cache_write")
 
 
 def __getattr__(name):
