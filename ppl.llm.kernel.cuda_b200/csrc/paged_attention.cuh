@@ -253,6 +253,7 @@ __device__ __forceinline__ void finish(const AttentionParams& p, int64_t b, int3
             } else {
                 for (int32_t i = 0; i < p.parts; ++i) {
                     const float2 s = __ldcg(&p.part_tops[i * p.part_rows + at]);
+                    if (s.x == kNothingSeen) continue; // its sums need not have been written
                     const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_sums + (i * p.part_rows + at) * S::D + d));
                     const float up = fmaxf(top, s.x), keep = exp2_fast(top - up), f = exp2_fast(s.x - up);
                     top = up;

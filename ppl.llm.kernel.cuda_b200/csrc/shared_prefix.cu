@@ -1,14 +1,69 @@
 // Attention of one new token per sequence for a batch that shares a prefix: the prefix for the rows of all sequences at once, then each sequence's
 // own tokens, whose sums are joined with the prefix's where the output is written.
-#include "paged_attention.cuh"
+#include "shared_prefix.cuh"
 
 namespace pplb200 {
 namespace {
 
+using namespace prefix;
+
 constexpr int64_t kMaxRows = 1 << 24;
 
-// Sums over the prefix: reference exponents and sums of weights, then sums of values.
-int64_t part_bytes(int64_t rows, int32_t head_dim) { return round_up(rows * 8, 256) + round_up(rows * head_dim * 4, 256); }
+// Rows of a key head up to which the decode kernel, whose matrix instructions take 8 or 16 of them at once, goes through the prefix.
+int32_t few_rows(int32_t head_dim) { return head_dim <= 128 ? 16 : 8; }
+
+// Tiles of rows that a CTA takes at once: two share what is loaded, unless the last of an odd number would leave half of a CTA idle that counts.
+int32_t tiles_at_once(int64_t rows, int32_t most) {
+    const int64_t tiles = (rows + 127) / 128;
+    return most == 2 && tiles > 1 && (tiles % 2 == 0 || tiles >= 7) ? 2 : 1;
+}
+// Parts that the prefix is cut into, so that there is a CTA for every SM.
+int32_t splits_of(int64_t items) { return (int32_t)std::max<int64_t>(1, kSms / items); }
+
+// Sums over the parts of the prefix: reference exponents and sums of weights, then sums of values.
+int64_t part_bytes(int64_t rows, int32_t head_dim, int64_t parts) { return round_up(parts * rows * 8, 256) + round_up(parts * rows * head_dim * 4, 256); }
+// As many parts as any kind of cache asks for.
+int64_t most_parts(int64_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
+    const int64_t rows = batch * (q_heads / kv_heads);
+    if (rows <= few_rows(head_dim)) return 1;
+    return splits_of(kv_heads * ((rows + 255) / 256));
+}
+
+template <int D, int KIND>
+int32_t launch_tiles(cudaStream_t stream, PrefixParams& p) {
+    using T = Tile<D, KIND>;
+    static_assert(T::SMEM + 8192 <= 232448);
+    p.tiles = tiles_at_once(p.rows, T::TILES);
+    p.items = p.cache.kv_heads * (int32_t)((p.rows + p.tiles * 128 - 1) / (p.tiles * 128));
+    const int64_t blocks = std::max<int64_t>(1, (p.tokens_in_table + T::NB - 1) / T::NB);
+    p.splits = (int32_t)std::min<int64_t>(splits_of(p.items), blocks);
+    const cudaError_t e = cudaFuncSetAttribute(prefix_tile_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
+    if (e != cudaSuccess) return fail(RC_DEVICE_RUNTIME_ERROR, "shared prefix: %s", cudaGetErrorString(e));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.items * p.splits));
+    cfg.blockDim = dim3(T::THREADS);
+    cfg.dynamicSmemBytes = T::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, prefix_tile_kernel<T>, p);
+    return check_launch("shared prefix");
+}
+template <int D>
+int32_t launch_kind(cudaStream_t stream, PrefixParams& p) {
+    if (p.cache.quant_group == 0) return launch_tiles<D, CACHE_F16>(stream, p);
+    if (p.cache.quant_group == 8) return launch_tiles<D, CACHE_I8_GROUPS>(stream, p);
+    return launch_tiles<D, CACHE_I8_ROWS>(stream, p);
+}
+int32_t launch_prefix(cudaStream_t stream, PrefixParams& p) {
+    if (p.cache.head_dim == 64) return launch_kind<64>(stream, p);
+    if (p.cache.head_dim == 96) return launch_kind<96>(stream, p);
+    if (p.cache.head_dim == 128) return launch_kind<128>(stream, p);
+    return launch_kind<256>(stream, p);
+}
 
 } // namespace
 } // namespace pplb200
@@ -20,7 +75,8 @@ extern "C" {
 int64_t pplb200_shared_prefix_attention_workspace_bytes(int64_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
     if (batch < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0 || batch > kMaxRows / q_heads) return -1;
     const int32_t shared = q_heads / kv_heads;
-    return std::max(workspace_bytes(shared, head_dim), workspace_bytes(batch * shared, head_dim)) + part_bytes(batch * q_heads, head_dim);
+    return std::max(workspace_bytes(shared, head_dim), workspace_bytes(batch * shared, head_dim)) +
+           part_bytes(batch * q_heads, head_dim, most_parts(batch, q_heads, kv_heads, head_dim));
 }
 
 int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_paged_attention_args* a,
@@ -44,21 +100,40 @@ int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb
     own.units_per_page = 1;
     own.num_units = own.num_pages;
     own.rows_per_head = shared;
+    const int64_t parts = most_parts(a->batch, a->q_heads, cache->kv_heads, cache->head_dim);
     own.part_rows = rows;
-    own.part_tops = (float2*)((char*)a->ws + need - part_bytes(rows, cache->head_dim));
-    own.part_sums = (float*)((char*)own.part_tops + round_up(rows * 8, 256));
-    // the prefix: one sequence, whose key heads are asked by the rows of all
-    AttentionParams first = own;
-    first.batch = 1;
-    first.pages = prefix->pages;
-    first.lengths = prefix->length;
-    first.pages_stride = prefix->num_pages;
-    first.tokens_in_table = prefix->num_pages * cache->page_size;
-    first.keep_parts = true;
-    lay_out(first, a->ws, a->batch * shared);
-    const int32_t done = launch_general((cudaStream_t)stream, first);
-    if (done != RC_SUCCESS) return done;
+    own.part_tops = (float2*)((char*)a->ws + need - part_bytes(rows, cache->head_dim, parts));
+    own.part_sums = (float*)((char*)own.part_tops + round_up(parts * rows * 8, 256));
     own.parts = 1;
+    if (a->batch * shared <= few_rows(cache->head_dim)) {
+        // the prefix as one sequence, whose key heads are asked by the rows of all
+        AttentionParams first = own;
+        first.batch = 1;
+        first.pages = prefix->pages;
+        first.lengths = prefix->length;
+        first.pages_stride = prefix->num_pages;
+        first.tokens_in_table = prefix->num_pages * cache->page_size;
+        first.parts = 0;
+        first.keep_parts = true;
+        lay_out(first, a->ws, a->batch * shared);
+        const int32_t done = launch_general((cudaStream_t)stream, first);
+        if (done != RC_SUCCESS) return done;
+    } else {
+        PrefixParams p = {};
+        p.q = own.q; p.q_stride = own.q_stride;
+        p.pages = prefix->pages; p.length = prefix->length;
+        p.tokens_in_table = prefix->num_pages * cache->page_size;
+        p.num_pages = own.num_pages; p.rows = (int32_t)(a->batch * shared);
+        p.rows_per_head = shared; p.q_heads = a->q_heads;
+        small_division(shared, p.rows_magic, p.rows_shift);
+        small_division(cache->page_size, p.page_magic, p.page_shift);
+        p.scale_log2 = own.scale_log2;
+        p.cache = *cache;
+        p.part_rows = rows; p.part_tops = own.part_tops; p.part_sums = own.part_sums;
+        const int32_t done = launch_prefix((cudaStream_t)stream, p);
+        if (done != RC_SUCCESS) return done;
+        own.parts = p.splits;
+    }
     lay_out(own, a->ws, shared);
     return launch_general((cudaStream_t)stream, own);
 }
