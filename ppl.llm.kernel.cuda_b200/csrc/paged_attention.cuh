@@ -96,6 +96,7 @@ struct AttentionParams {
     uint32_t rows_magic, rows_shift;
     int32_t parts;                             // sums of earlier calls that are joined
     bool keep_parts;                           // leave the sums, as part 0
+    bool late_wait;
     int64_t part_rows;                         // rows of a part: query heads of all sequences
     float2* part_tops;                         // [parts][part_rows]
     float* part_sums;                          // [parts][part_rows][D]
@@ -251,14 +252,33 @@ __device__ __forceinline__ void finish(const AttentionParams& p, int64_t b, int3
                 top = kNothingSeen;
                 sum = 0.0f;
             } else {
-                for (int32_t i = 0; i < p.parts; ++i) {
-                    const float2 s = __ldcg(&p.part_tops[i * p.part_rows + at]);
-                    if (s.x == kNothingSeen) continue; // its sums need not have been written
-                    const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_sums + (i * p.part_rows + at) * S::D + d));
-                    const float up = fmaxf(top, s.x), keep = exp2_fast(top - up), f = exp2_fast(s.x - up);
+                // four parts at once, eight loads on their way
+                for (int32_t i = 0; i < p.parts; i += 4) {
+                    float2 s[4];
+                    float4 a[4];
+                    float up = top;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int64_t from = min(i + j, p.parts - 1) * p.part_rows + at;
+                        s[j] = __ldcg(&p.part_tops[from]);
+                        a[j] = __ldcg(reinterpret_cast<const float4*>(p.part_sums + from * S::D + d));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (i + j >= p.parts) s[j] = make_float2(kNothingSeen, 0.0f);
+                        up = fmaxf(up, s[j].x);
+                    }
+                    const float keep = exp2_fast(top - up);
                     top = up;
-                    sum = sum * keep + s.y * f;
-                    v.x = v.x * keep + a.x * f; v.y = v.y * keep + a.y * f; v.z = v.z * keep + a.z * f; v.w = v.w * keep + a.w * f;
+                    sum *= keep;
+                    v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (s[j].x != kNothingSeen) { // else its sums need not have been written
+                            const float f = exp2_fast(s[j].x - up);
+                            sum += s[j].y * f;
+                            v.x += a[j].x * f; v.y += a[j].y * f; v.z += a[j].z * f; v.w += a[j].w * f;
+                        }
                 }
             }
         }
@@ -277,7 +297,10 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
     // the warp's number from a shuffle, so that the compiler knows that it is the same in all lanes
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, t = lane & 3;
     const int heads_per_sequence = p.cache.kv_heads * p.tiles;
-    pdl_wait_prior_grid();
+    // late_wait: the grid before this one belongs to the same call, all of it had started behind its own wait when this one could, and only the sums that
+    // it leaves are needed from it: where an item's output is written.
+    const bool late = S::GENERAL && p.late_wait;
+    if (!late) pdl_wait_prior_grid();
     pdl_launch_dependents();
 
     // ---- this CTA's share -----------------------------------------------------------------------------------------------
@@ -318,7 +341,10 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
         // Joining takes about as long as three rounds of steps.
         const bool whole_items = items <= gridDim.x && most <= all / ctas + 3 * WARPS;
         if (whole_items) ctas = (int32_t)items;
-        if (blockIdx.x >= ctas) return;
+        if (blockIdx.x >= ctas) {
+            if (late) pdl_wait_prior_grid();
+            return;
+        }
         if (whole_items) {
             from.b = blockIdx.x / heads_per_sequence;
             from.head = blockIdx.x - (int32_t)from.b * heads_per_sequence;
@@ -797,6 +823,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
             }
         }
         __syncthreads();
+        if (late) pdl_wait_prior_grid();
         const bool whole = step0 == 0 && step1 == steps;
         const int64_t slot = 2 * (int64_t)blockIdx.x + (step0 == 0 ? 1 : 0);
         for (int x = threadIdx.x; x < q_count * (S::D / 4); x += S::THREADS) {
@@ -926,6 +953,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
         __syncthreads();
         if (++hh == heads_per_sequence) hh = 0, ++b;
     }
+    if (late) pdl_wait_prior_grid();
 }
 
 template <class S>

@@ -2,6 +2,8 @@
 // own tokens, whose sums are joined with the prefix's where the output is written.
 #include "shared_prefix.cuh"
 
+#include <cuda.h>
+
 namespace pplb200 {
 namespace {
 
@@ -29,6 +31,27 @@ int64_t most_parts(int64_t batch, int32_t q_heads, int32_t kv_heads, int32_t hea
     return splits_of(kv_heads * ((rows + 255) / 256));
 }
 
+// A map of keys or values for boxes of box_rows tokens by 64 dimensions; false where there is none for such strides.
+bool make_page_map(CUtensorMap* map, const pplb200_kv_cache& c, const void* base, int32_t box_rows) {
+    static const decltype(&cuTensorMapEncodeTiled) encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) == cudaSuccess && found == cudaDriverEntryPointSuccess;
+        return ok ? (decltype(&cuTensorMapEncodeTiled))f : nullptr;
+    }();
+    const int64_t strides_of[3] = {c.token_stride * 2, c.head_stride * 2, c.page_stride * 2};
+    const int64_t extents[3] = {c.page_size, c.kv_heads, c.num_pages};
+    cuuint64_t dims[4] = {(cuuint64_t)c.head_dim}, strides[3];
+    for (int i = 0; i < 3; ++i) {
+        if (extents[i] > 0x7fffffff || strides_of[i] >= 1LL << 40 || (strides_of[i] == 0 && extents[i] > 1)) return false;
+        dims[1 + i] = (cuuint64_t)extents[i];
+        strides[i] = (cuuint64_t)(strides_of[i] ? strides_of[i] : 16); // (of one: not used)
+    }
+    const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, steps[4] = {1, 1, 1, 1};
+    return encode && encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, int KIND>
 int32_t launch_tiles(cudaStream_t stream, PrefixParams& p) {
     using T = Tile<D, KIND>;
@@ -37,6 +60,11 @@ int32_t launch_tiles(cudaStream_t stream, PrefixParams& p) {
     p.items = p.cache.kv_heads * (int32_t)((p.rows + p.tiles * 128 - 1) / (p.tiles * 128));
     const int64_t blocks = std::max<int64_t>(1, (p.tokens_in_table + T::NB - 1) / T::NB);
     p.splits = (int32_t)std::min<int64_t>(splits_of(p.items), blocks);
+    p.box_rows = 0;
+    if (KIND == CACHE_F16 && p.cache.page_size % 16 == 0 && p.cache.num_pages > 0) {
+        const int32_t rows = std::min(p.cache.page_size & -p.cache.page_size, T::NB);
+        if (make_page_map(&p.kmap, p.cache, p.cache.k, rows) && make_page_map(&p.vmap, p.cache, p.cache.v, rows)) p.box_rows = rows;
+    }
     const cudaError_t e = cudaFuncSetAttribute(prefix_tile_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
     if (e != cudaSuccess) return fail(RC_DEVICE_RUNTIME_ERROR, "shared prefix: %s", cudaGetErrorString(e));
     cudaLaunchConfig_t cfg = {};
@@ -133,6 +161,7 @@ int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb
         const int32_t done = launch_prefix((cudaStream_t)stream, p);
         if (done != RC_SUCCESS) return done;
         own.parts = p.splits;
+        own.late_wait = true;
     }
     lay_out(own, a->ws, shared);
     return launch_general((cudaStream_t)stream, own);

@@ -38,7 +38,11 @@ struct Tile {
     static constexpr int RING = TILES * Q_BYTES, V_RING = RING + KS * K_BYTES, INFO = V_RING + VS * V_BYTES;
     static constexpr int INFOS = 8; // blocks whose masks and scales are kept: more than stages of values
     static constexpr int SCALES = KIND == CACHE_I8_ROWS ? INFOS * NB * 8 : 0;
-    static constexpr int SMEM = INFO + SCALES + 1024; // the base is rounded up to 1024
+    // What is read back of the sums lies over the rings and q, behind the sums that the two groups of one tile exchange (tiles' sums and these are not there at
+    // the same time, and one tile's are half as long).
+    static constexpr int STAGED_BYTES = STREAMS * 128 * (D + 4) * 4, EXCHANGE = STREAMS == 2 ? D * 512 : 0, ONE_TILE = EXCHANGE + 128 * (D + 4) * 4;
+    static constexpr int BODY = INFO + SCALES, LEAST = STAGED_BYTES > ONE_TILE ? STAGED_BYTES : ONE_TILE;
+    static constexpr int SMEM = (BODY > LEAST ? BODY : LEAST) + 1024; // the base is rounded up to 1024
     static constexpr int CH = D * ES / 16, LOADS = CH * NB / 128; // pieces of 16 bytes: of a row, and of a block for a thread
     static_assert(CH * NB % 128 == 0 && VS < INFOS);
     static constexpr int THREADS = 512;
@@ -46,6 +50,8 @@ struct Tile {
 };
 
 struct PrefixParams {
+    CUtensorMap kmap, vmap; // box_rows > 0: fp16 pages as [pages, heads, tokens, dimensions]
+    int32_t box_rows;       // tokens of a box: a power of two, 16 at least, that divides a page
     const half* q;
     int64_t q_stride;
     const int32_t *pages, *length;
@@ -78,7 +84,7 @@ __device__ __forceinline__ void whole_numbers(const uint4& raw, uint32_t (&o)[8]
 template <class T>
 __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid_constant__ PrefixParams p) {
     extern __shared__ uint8_t raw_smem[];
-    __shared__ __align__(8) uint64_t full_k[T::KS], empty_k[T::KS], full_v[T::VS], empty_v[T::VS], info_full[T::INFOS], score_full[2], weight_full[2], sum_done[2], q_full, all_done;
+    __shared__ __align__(8) uint64_t full_k[T::KS], empty_k[T::KS], full_v[T::VS], empty_v[T::VS], info_full[T::INFOS], score_full[2], weight_half[2], weight_full[2], sum_done[2], q_full, all_done, tail_full;
     __shared__ uint32_t tmem_slot;
     __shared__ uint32_t masks[T::INFOS][4];
     __shared__ float sizes[T::INFOS][4];
@@ -87,11 +93,13 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t smem = (ptx::smem_addr(raw_smem) + 1023u) & ~1023u;
     auto bar = [](uint64_t& b) { return ptx::smem_addr(&b); };
+    const bool boxes = T::KIND == CACHE_F16 && p.box_rows > 0; // whole boxes by the TMA unit: one thread reports
     if (threadIdx.x == 0) {
-        for (int i = 0; i < T::KS; ++i) ptx::mbar_init(bar(full_k[i]), 128), ptx::mbar_init(bar(empty_k[i]), 1);
-        for (int i = 0; i < T::VS; ++i) ptx::mbar_init(bar(full_v[i]), 128), ptx::mbar_init(bar(empty_v[i]), 1);
-        for (int i = 0; i < T::INFOS; ++i) ptx::mbar_init(bar(info_full[i]), 128);
-        for (int i = 0; i < 2; ++i) ptx::mbar_init(bar(score_full[i]), 1), ptx::mbar_init(bar(weight_full[i]), 128), ptx::mbar_init(bar(sum_done[i]), 1);
+        for (int i = 0; i < T::KS; ++i) ptx::mbar_init(bar(full_k[i]), boxes ? 1 : 128), ptx::mbar_init(bar(empty_k[i]), 1);
+        for (int i = 0; i < T::VS; ++i) ptx::mbar_init(bar(full_v[i]), boxes ? 1 : 128), ptx::mbar_init(bar(empty_v[i]), 1);
+        for (int i = 0; i < T::INFOS; ++i) ptx::mbar_init(bar(info_full[i]), boxes ? 1 : 128);
+        ptx::mbar_init(bar(tail_full), 1);
+        for (int i = 0; i < 2; ++i) ptx::mbar_init(bar(score_full[i]), 1), ptx::mbar_init(bar(weight_half[i]), 128), ptx::mbar_init(bar(weight_full[i]), 128), ptx::mbar_init(bar(sum_done[i]), 1);
         ptx::mbar_init(bar(q_full), 256);
         ptx::mbar_init(bar(all_done), 1);
         ptx::fence_mbar_init();
@@ -142,12 +150,18 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
             if (tasks > 1) scores(1);
             for (int32_t i = 0; i < tasks && ok; ++i) {
                 const int32_t j = i >> shift, stage = j % T::VS;
-                if (!(ok = ptx::mbar_wait(bar(full_v[stage]), (j / T::VS) & 1, &g_status, ST_MMA) && ptx::mbar_wait(bar(weight_full[i & 1]), (i >> 1) & 1, &g_status, ST_MMA))) break;
-                ptx::tc_fence_after();
+                if (!(ok = ptx::mbar_wait(bar(full_v[stage]), (j / T::VS) & 1, &g_status, ST_MMA))) break;
                 const uint32_t v = mn_desc_lo(smem + T::V_RING + stage * T::V_BYTES, T::NB * 128);
                 const uint32_t d = tmem + T::O_COLUMN + (T::STREAMS == 2 ? (i & 1) * T::DP : 0), w = tmem + (i & 1) * 128;
+                // the weights of the block's first half are worked with while the others are computed
 #pragma unroll
-                for (int s = 0; s < T::NB / 16; ++s) ptx::mma_f16_tmem(d, w + s * 8, ptx::desc_from_lo(v + s * (2048 / 16)), PV, (T::STREAMS == 2 ? i > 1 : i > 0) || s > 0);
+                for (int half = 0; half < 2 && ok; ++half) {
+                    if (!(ok = ptx::mbar_wait(bar(half ? weight_full[i & 1] : weight_half[i & 1]), (i >> 1) & 1, &g_status, ST_MMA))) break;
+                    ptx::tc_fence_after();
+#pragma unroll
+                    for (int s = half * T::NB / 32; s < (half + 1) * T::NB / 32; ++s)
+                        ptx::mma_f16_tmem(d, w + s * 8, ptx::desc_from_lo(v + s * (2048 / 16)), PV, (T::STREAMS == 2 ? i > 1 : i > 0) || s > 0);
+                }
                 ptx::mma_commit(bar(sum_done[i & 1]));
                 if (tiles == 1 || (i & 1)) ptx::mma_commit(bar(empty_v[stage]));
                 if (i + 2 < tasks) scores(i + 2);
@@ -160,43 +174,46 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
         const int id = threadIdx.x - 256;
         const char *const kbase = (const char*)p.cache.k + (int64_t)kvh * p.cache.head_stride * T::ES, *const vbase = (const char*)p.cache.v + (int64_t)kvh * p.cache.head_stride * T::ES;
         const char *const ksbase = (const char*)p.cache.k_scale + (int64_t)kvh * p.cache.scale_head_stride * 2, *const vsbase = (const char*)p.cache.v_scale + (int64_t)kvh * p.cache.scale_head_stride * 2;
-        // where block j's tokens lie, which of them are there, and (rows) their scales
+        // Where a block's tokens lie, which of them are there, and (rows) their scales: thread id looks after token id, its page one block ahead.
+        int32_t page = -1;
+        bool there = false;
+        float k_scale = 0.0f, v_scale = 0.0f;
+        auto request = [&](int32_t j) {
+            const int32_t token = (block0 + j) * T::NB + id;
+            page = -1;
+            if (j < blocks && id < T::NB && token < n) page = p.pages[(uint32_t)((uint64_t)(uint32_t)token * p.page_magic >> p.page_shift)];
+        };
         auto locate = [&](int32_t j) {
             const int32_t token = (block0 + j) * T::NB + id;
-            bool there = false;
-            int64_t row = -1, scale_row = 0;
-            if (id < T::NB && token < n) {
-                const uint32_t index = (uint32_t)((uint64_t)(uint32_t)token * p.page_magic >> p.page_shift);
-                const int32_t page = p.pages[index], in_page = token - index * p.cache.page_size;
-                there = (uint32_t)page < (uint32_t)p.num_pages;
-                if (there) {
-                    row = kv_row(page, in_page, 0, p.cache.page_stride, 0, p.cache.token_stride) * T::ES;
-                    if constexpr (T::KIND != CACHE_F16) scale_row = kv_row(page, in_page, 0, p.cache.scale_page_stride, 0, p.cache.scale_token_stride) * 2;
+            there = j < blocks && (uint32_t)page < (uint32_t)p.num_pages;
+            const int32_t in_page = token - (int32_t)((uint32_t)((uint64_t)(uint32_t)token * p.page_magic >> p.page_shift)) * p.cache.page_size;
+            if (id < T::NB) row_at[j & 1][id] = there ? kv_row(page, in_page, 0, p.cache.page_stride, 0, p.cache.token_stride) * T::ES : -1;
+            if constexpr (T::KIND != CACHE_F16) {
+                const int64_t scale_row = there ? kv_row(page, in_page, 0, p.cache.scale_page_stride, 0, p.cache.scale_token_stride) * 2 : 0;
+                if (id < T::NB) scale_at[j & 1][id] = scale_row;
+                if constexpr (T::KIND == CACHE_I8_ROWS) {
+                    k_scale = there ? __half2float(__ushort_as_half((unsigned short)load_scales<1>(ksbase + scale_row))) : 0.0f;
+                    v_scale = there ? __half2float(__ushort_as_half((unsigned short)load_scales<1>(vsbase + scale_row))) : 0.0f;
                 }
             }
+        };
+        auto publish = [&](int32_t j) {
             const int slot = j % T::INFOS;
-            if (id < T::NB) {
-                row_at[j & 1][id] = row;
-                if constexpr (T::KIND != CACHE_F16) scale_at[j & 1][id] = scale_row;
-            }
             const uint32_t mask = __ballot_sync(0xffffffffu, there);
             if (lane == 0) masks[slot][id >> 5] = mask;
             if constexpr (T::KIND == CACHE_I8_ROWS) {
-                const float ks = there ? __half2float(__ushort_as_half((unsigned short)load_scales<1>(ksbase + scale_row))) : 0.0f;
-                const float vs = there ? __half2float(__ushort_as_half((unsigned short)load_scales<1>(vsbase + scale_row))) : 0.0f;
                 // a value's scale goes into its weight, its logarithm into what decides about the reference exponent, as far as a finite one could
-                float size = fminf(fmaxf(log2_fast(fabsf(vs)), -24.0f), 16.0f);
+                float size = fminf(fmaxf(log2_fast(fabsf(v_scale)), -24.0f), 16.0f);
 #pragma unroll
                 for (int m = 16; m > 0; m >>= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, m));
-                if (lane == 0) sizes[slot][id >> 5] = id < T::NB ? size : -24.0f;
+                if (lane == 0) sizes[slot][id >> 5] = size;
                 if (id < T::NB) {
                     float* const scales = reinterpret_cast<float*>(raw_smem + (smem - ptx::smem_addr(raw_smem)) + T::INFO) + slot * T::NB * 2;
-                    scales[id] = ks * p.scale_log2;
-                    scales[T::NB + id] = vs;
+                    scales[id] = k_scale * p.scale_log2;
+                    scales[T::NB + id] = v_scale;
                 }
             }
             ptx::mbar_arrive(bar(info_full[slot]));
-            ptx::named_barrier(1, 128);
         };
         // piece i of this thread: of token (id + 128 i) / CH
         auto token_of = [&](int i) { return (id + 128 * i) / T::CH; };
@@ -205,46 +222,107 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
         auto place = [](int token, int c) { return (uint32_t)((c >> 3) * (T::NB * 128) + token * 128 + (((c & 7) ^ (token & 7)) << 4)); };
         bool ok = true;
         if constexpr (T::KIND == CACHE_F16) {
-            // loads 2 j (keys) and 2 j + 1 (values); up to three are on their way when the next is issued
-            int32_t arrived = 0, issued = 0;
-            auto arrive = [&] {
-                ptx::fence_proxy_async_smem();
-                ptx::mbar_arrive(arrived & 1 ? bar(full_v[(arrived >> 1) % T::VS]) : bar(full_k[(arrived >> 1) % T::KS]));
-                ++arrived;
-            };
-            auto settle = [&] {
-                ptx::cp_async_wait<0>();
-                while (arrived < issued) arrive();
-            };
-            for (int32_t j = 0; j < blocks; ++j) {
-                locate(j);
+            if (boxes) {
+                // Warp 8 brings keys, warp 9 values: lane i the box of tokens from i * box_rows on; a box that is not there lies on the page behind the last
+                // and reads as zeros.  Tokens behind the prefix's last in a box that is there are what the page holds: masked as keys, as values overwritten with zeros.
+                if (warp < 10) {
+                    const bool values = warp == 9;
+                    const int stages = values ? T::VS : T::KS, groups = T::NB / p.box_rows;
+                    const uint32_t ring = smem + (values ? T::V_RING : T::RING);
+                    const CUtensorMap* const map = values ? &p.vmap : &p.kmap;
+                    if (lane == 0) ptx::prefetch_tensormap(map);
+                    order_before_tma();
+                    auto page_of = [&](int32_t j) {
+                        const int32_t token = (block0 + j) * T::NB + lane * p.box_rows;
+                        return j < blocks && lane < groups && token < n ? p.pages[(uint32_t)((uint64_t)(uint32_t)token * p.page_magic >> p.page_shift)] : -1;
+                    };
+                    int32_t next = page_of(0);
+                    for (int32_t j = 0; j < blocks; ++j) {
+                        const int32_t now = next, first = (block0 + j) * T::NB, token = first + lane * p.box_rows;
+                        next = page_of(j + 1);
+                        const bool here = (uint32_t)now < (uint32_t)p.num_pages;
+                        const uint32_t present = __ballot_sync(0xffffffffu, here);
+                        const int stage = j % stages;
+                        const uint32_t full = values ? bar(full_v[stage]) : bar(full_k[stage]);
+                        ok = __all_sync(0xffffffffu, ptx::mbar_wait(values ? bar(empty_v[stage]) : bar(empty_k[stage]), ((j / stages) & 1) ^ 1, &g_status, ST_LOAD));
+                        if (!ok) break;
+                        if (!values) { // the scores' masks: bit x of word w is token 32 w + x
+                            if (lane < T::NB / 32) {
+                                const uint32_t half0 = present >> (lane * 32 / p.box_rows) & 1, half1 = present >> ((lane * 32 + 16) / p.box_rows) & 1;
+                                const int32_t left = n - first - lane * 32;
+                                masks[j % T::INFOS][lane] = (half0 * 0xffffu | half1 * 0xffff0000u) & (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1);
+                            }
+                            __syncwarp();
+                            if (lane == 0) ptx::mbar_arrive(bar(info_full[j % T::INFOS]));
+                        }
+                        const bool tail = values && first + T::NB > n;
+                        const uint32_t landed = tail ? bar(tail_full) : full;
+                        if (lane == 0) ptx::mbar_arrive_expect_tx(landed, T::V_BYTES);
+                        __syncwarp();
+                        if (lane < groups) {
+                            const int32_t in_page = token - (int32_t)((uint32_t)((uint64_t)(uint32_t)token * p.page_magic >> p.page_shift)) * p.cache.page_size;
 #pragma unroll
-                for (int values = 0; values < 2; ++values) {
-                    const int stages = values ? T::VS : T::KS, stage = j % stages;
-                    const uint32_t empty = values ? bar(empty_v[stage]) : bar(empty_k[stage]), parity = ((j / stages) & 1) ^ 1;
-                    if (ok && !ptx::mbar_try_wait(empty, parity)) { // what is on its way may be what the place waits for
-                        settle();
-                        ok = ptx::mbar_wait(empty, parity, &g_status, ST_LOAD);
-                    }
-                    if (!ok) continue; // (every thread comes to every barrier of locate)
-                    const uint32_t dst = smem + (values ? T::V_RING + stage * T::V_BYTES : T::RING + stage * T::K_BYTES);
-                    const char* const base = values ? vbase : kbase;
+                            for (int a = 0; a < T::ATOMS; ++a)
+                                ptx::tma_load_4d(ring + stage * T::V_BYTES + a * (T::NB * 128) + lane * p.box_rows * 128, map, landed, a * 64, here ? in_page : 0, kvh, here ? now : p.num_pages);
+                        }
+                        if (tail) { // the last block
+                            ok = __all_sync(0xffffffffu, ptx::mbar_wait(landed, 0, &g_status, ST_LOAD));
+                            if (!ok) break;
+                            for (int32_t x = (n - first) * 8 + lane; x < T::NB * 8; x += 32)
 #pragma unroll
-                    for (int i = 0; i < T::LOADS; ++i) {
-                        const int token = token_of(i), c = piece_of(i);
-                        const int64_t at = row_at[j & 1][token];
-                        ptx::cp_async_16(dst + place(token, c), base + (at < 0 ? 0 : at) + c * 16, at >= 0);
-                    }
-                    ptx::cp_async_commit();
-                    ++issued;
-                    if (issued - arrived > 3) {
-                        ptx::cp_async_wait<3>();
-                        arrive();
+                                for (int a = 0; a < T::ATOMS; ++a) ptx::st_shared_v4(ring + stage * T::V_BYTES + a * (T::NB * 128) + x * 16, make_uint4(0, 0, 0, 0));
+                            ptx::fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) ptx::mbar_arrive(full);
+                        }
                     }
                 }
+            } else {
+                // loads of keys and of values in turn; up to three are on their way when the next is issued
+                int32_t arrived = 0, issued = 0;
+                auto arrive = [&] {
+                    ptx::fence_proxy_async_smem();
+                    ptx::mbar_arrive(arrived & 1 ? bar(full_v[(arrived >> 1) % T::VS]) : bar(full_k[(arrived >> 1) % T::KS]));
+                    ++arrived;
+                };
+                auto settle = [&] {
+                    ptx::cp_async_wait<0>();
+                    while (arrived < issued) arrive();
+                };
+                request(0);
+                for (int32_t j = 0; j < blocks; ++j) {
+                    locate(j);
+                    request(j + 1);
+                    ptx::named_barrier(1, 128);
+                    int64_t at[T::LOADS];
+#pragma unroll
+                    for (int i = 0; i < T::LOADS; ++i) at[i] = row_at[j & 1][token_of(i)];
+#pragma unroll
+                    for (int values = 0; values < 2; ++values) {
+                        const int stages = values ? T::VS : T::KS, stage = j % stages;
+                        const uint32_t empty = values ? bar(empty_v[stage]) : bar(empty_k[stage]), parity = ((j / stages) & 1) ^ 1;
+                        if (ok && !ptx::mbar_try_wait(empty, parity)) { // what is on its way may be what the place waits for
+                            settle();
+                            ok = ptx::mbar_wait(empty, parity, &g_status, ST_LOAD);
+                        }
+                        if (!values) publish(j); // (every thread comes to every barrier and ballot)
+                        if (!ok) continue;
+                        const uint32_t dst = smem + (values ? T::V_RING + stage * T::V_BYTES : T::RING + stage * T::K_BYTES);
+                        const char* const base = values ? vbase : kbase;
+#pragma unroll
+                        for (int i = 0; i < T::LOADS; ++i) ptx::cp_async_16(dst + place(token_of(i), piece_of(i)), base + (at[i] < 0 ? 0 : at[i]) + piece_of(i) * 16, at[i] >= 0);
+                        ptx::cp_async_commit();
+                        ++issued;
+                        if (issued - arrived > 3) {
+                            ptx::cp_async_wait<3>();
+                            arrive();
+                        }
+                    }
+                }
+                settle();
             }
-            settle();
         } else {
+            // a block's pieces are requested when the block before has been put into its place
             uint4 kw[T::LOADS], vw[T::LOADS];
             uint32_t ks[T::LOADS], vs[T::LOADS];
             auto fetch = [&](int32_t j, uint4 (&w)[T::LOADS], uint32_t (&s)[T::LOADS], const char* base, const char* sbase) {
@@ -282,43 +360,57 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                 ptx::fence_proxy_async_smem();
             };
             if (blocks > 0) {
+                request(0);
                 locate(0);
+                request(1);
+                ptx::named_barrier(1, 128);
                 fetch(0, kw, ks, kbase, ksbase);
+                fetch(0, vw, vs, vbase, vsbase);
+                publish(0);
             }
             for (int32_t j = 0; j < blocks; ++j) {
-                fetch(j, vw, vs, vbase, vsbase);
+                locate(j + 1);
+                request(j + 2);
+                ptx::named_barrier(1, 128);
                 const int kstage = j % T::KS, vstage = j % T::VS;
-                // (after a wait that ran out nothing is stored any more, but every thread comes to every barrier of locate)
+                // (after a wait that ran out nothing is stored any more, but every thread comes to every barrier and ballot)
                 ok = ok && ptx::mbar_wait(bar(empty_k[kstage]), ((j / T::KS) & 1) ^ 1, &g_status, ST_LOAD);
                 if (ok) {
                     put(smem + T::RING + kstage * T::K_BYTES, kw, ks, true);
                     ptx::mbar_arrive(bar(full_k[kstage]));
                 }
-                ok = ok && ptx::mbar_wait(bar(empty_v[vstage]), ((j / T::VS) & 1) ^ 1, &g_status, ST_LOAD);
                 if (j + 1 < blocks) {
-                    locate(j + 1);
                     fetch(j + 1, kw, ks, kbase, ksbase);
+                    publish(j + 1);
                 }
+                ok = ok && ptx::mbar_wait(bar(empty_v[vstage]), ((j / T::VS) & 1) ^ 1, &g_status, ST_LOAD);
                 if (ok) {
                     put(smem + T::V_RING + vstage * T::V_BYTES, vw, vs, false);
                     ptx::mbar_arrive(bar(full_v[vstage]));
                 }
+                if (j + 1 < blocks) fetch(j + 1, vw, vs, vbase, vsbase);
             }
         }
     } else {
         ptx::registers_up<176>();
         // ---- softmax ---------------------------------------------------------------------------------------------------------------
         const int stream = warp >> 2, r = threadIdx.x & 127;
-        for (int t = 0; t < tiles; ++t)
-            for (int x = threadIdx.x; x < 128 * (T::D / 8); x += 256) {
-                const int row = x / (T::D / 8), c = x - row * (T::D / 8), of = row0 + t * 128 + row;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (of < p.rows) {
-                    const int32_t sequence = (uint32_t)((uint64_t)(uint32_t)of * p.rows_magic >> p.rows_shift);
-                    v = ld_global_16(p.q + sequence * p.q_stride + (int64_t)(kvh * p.rows_per_head + of - sequence * p.rows_per_head) * T::D + c * 8);
-                }
-                ptx::st_shared_v4(smem + t * T::Q_BYTES + (c >> 3) * (128 * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4), v);
+        // the rows of q: a tile at a time, requested together
+        for (int t = 0; t < tiles; ++t) {
+            constexpr int PIECES = 128 * (T::D / 8) / 256;
+            uint4 v[PIECES];
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int x = threadIdx.x + 256 * i, row = x / (T::D / 8), c = x - row * (T::D / 8), of = row0 + t * 128 + row;
+                const int32_t sequence = (uint32_t)((uint64_t)(uint32_t)of * p.rows_magic >> p.rows_shift);
+                v[i] = of < p.rows ? ld_global_16(p.q + sequence * p.q_stride + (int64_t)(kvh * p.rows_per_head + of - sequence * p.rows_per_head) * T::D + c * 8) : make_uint4(0, 0, 0, 0);
             }
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int x = threadIdx.x + 256 * i, row = x / (T::D / 8), c = x - row * (T::D / 8);
+                ptx::st_shared_v4(smem + t * T::Q_BYTES + (c >> 3) * (128 * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4), v[i]);
+            }
+        }
         ptx::fence_proxy_async_smem();
         ptx::mbar_arrive(bar(q_full));
 
@@ -342,15 +434,19 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
 #pragma unroll
                 for (int c = 0; c < T::NB; ++c) s[c] = __uint_as_float(bits[c]);
                 const float4* const ks = reinterpret_cast<const float4*>(raw_smem + (smem - ptx::smem_addr(raw_smem)) + T::INFO) + slot * T::NB / 2;
+                float factor = 1.0f; // of a score, where it is not in it
+                if constexpr (T::KIND == CACHE_I8_ROWS) {
 #pragma unroll
-                for (int c = 0; c < T::NB; c += 4) {
-                    if constexpr (T::KIND == CACHE_I8_ROWS) {
+                    for (int c = 0; c < T::NB; c += 4) {
                         const float4 f = ks[c / 4];
-                        s[c] *= f.x; s[c + 1] *= f.y; s[c + 2] *= f.z; s[c + 3] *= f.w;
-                    } else {
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) s[c + x] *= p.scale_log2;
+                        const float2 a = ptx::mul2(make_float2(s[c], s[c + 1]), make_float2(f.x, f.y)), b = ptx::mul2(make_float2(s[c + 2], s[c + 3]), make_float2(f.z, f.w));
+                        s[c] = a.x; s[c + 1] = a.y; s[c + 2] = b.x; s[c + 3] = b.y;
                     }
+                } else if (p.scale_log2 > 0.0f) { // the largest stays the largest
+                    factor = p.scale_log2;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < T::NB; ++c) s[c] *= p.scale_log2;
                 }
                 uint32_t any = 0;
 #pragma unroll
@@ -364,12 +460,12 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                     }
                 }
                 met |= any != 0;
-                float high[4] = {s[0], s[1], s[2], s[3]};
+                float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 4; c < T::NB; c += 4)
+                for (int c = 0; c < T::NB; c += 8)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) high[x] = fmaxf(high[x], s[c + x]);
-                float m = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
+                    for (int x = 0; x < 4; ++x) high[x] = fmaxf(high[x], fmaxf(s[c + x], s[c + 4 + x]));
+                float m = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * factor;
                 if constexpr (T::KIND == CACHE_I8_ROWS) m += fmaxf(fmaxf(sizes[slot][0], sizes[slot][1]), fmaxf(sizes[slot][2], sizes[slot][3]));
                 // the reference exponent moves when a weight would pass 2^14, each row's for itself
                 const bool higher = m > top + 6.0f;
@@ -394,29 +490,28 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                         }
                     }
                 }
-                const float reference = top - 8.0f;
-                float sums[4] = {};
+                const float2 reference = make_float2(8.0f - top, 8.0f - top), factors = make_float2(factor, factor);
+                float2 sums[2] = {};
 #pragma unroll
                 for (int c = 0; c < T::NB; c += 32) {
                     uint32_t w[16];
 #pragma unroll
-                    for (int x = 0; x < 32; x += 4) {
-                        float e[4];
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            e[y] = exp2_fast(s[c + x + y] - reference);
-                            sums[y] += e[y];
-                        }
-                        if constexpr (T::KIND == CACHE_I8_ROWS) {
-                            const float4 f = ks[T::NB / 4 + (c + x) / 4];
-                            e[0] *= f.x; e[1] *= f.y; e[2] *= f.z; e[3] *= f.w;
-                        }
-                        w[x / 2] = h2(__floats2half2_rn(e[0], e[1]));
-                        w[x / 2 + 1] = h2(__floats2half2_rn(e[2], e[3]));
+                    for (int x = 0; x < 32; x += 2) {
+                        float2 e = ptx::fma2(make_float2(s[c + x], s[c + x + 1]), factors, reference);
+                        e.x = exp2_fast(e.x);
+                        e.y = exp2_fast(e.y);
+                        sums[x >> 1 & 1] = ptx::add2(sums[x >> 1 & 1], e);
+                        if constexpr (T::KIND == CACHE_I8_ROWS) e = ptx::mul2(e, reinterpret_cast<const float2*>(ks)[T::NB / 2 + (c + x) / 2]);
+                        w[x / 2] = h2(__floats2half2_rn(e.x, e.y));
                     }
                     ptx::tmem_st_32x16(at + c / 2, w);
+                    if (c + 32 == T::NB / 2) {
+                        ptx::tmem_st_wait();
+                        ptx::tc_fence_before();
+                        ptx::mbar_arrive(bar(weight_half[i & 1]));
+                    }
                 }
-                sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
                 ptx::tmem_st_wait();
                 ptx::tc_fence_before();
                 ptx::mbar_arrive(bar(weight_full[i & 1]));
@@ -429,7 +524,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
         if (!ok) top = sum = __int_as_float(0x7fffffff); // a wait ran out: not a number rather than a wrong one
         float own = 1.0f, other = 0.0f;
         const bool mine = T::STREAMS == 2 ? (tiles == 2 || stream == 0) : stream == 0; // whether this group writes a tile
-        float* const exchange = reinterpret_cast<float*>(raw_smem + (smem - ptx::smem_addr(raw_smem)) + T::RING); // [D][128]: the rings are idle
+        float* const exchange = reinterpret_cast<float*>(raw_smem + (smem - ptx::smem_addr(raw_smem))); // [D][128]: the rings and q are idle
         const bool joined = T::STREAMS == 2 && tiles == 1 && tasks > 1; // two groups' sums of one tile
         if (joined) {
             if (stream == 1) {
@@ -460,6 +555,9 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
         const bool there = mine && of < p.rows;
         if (there) __stcg(&p.part_tops[at], make_float2(top, sum));
         if (mine && tasks > 0) {
+            // by way of shared memory, so that a row leaves in whole lines: 32 rows of a warp, which it alone writes and reads
+            constexpr int PITCH = T::D + 4;
+            float* const rows = reinterpret_cast<float*>(raw_smem + (smem - ptx::smem_addr(raw_smem)) + (joined ? T::EXCHANGE : 0)) + (threadIdx.x >> 5) * 32 * PITCH;
 #pragma unroll 1
             for (int c = 0; c < T::D; c += 32) {
                 uint32_t o[32];
@@ -471,9 +569,16 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                     v[x] = __uint_as_float(o[x]);
                     if (joined) v[x] = v[x] * own + exchange[(c + x) * 128 + r] * other;
                 }
-                if (there)
 #pragma unroll
-                    for (int x = 0; x < 32; x += 4) __stcg(reinterpret_cast<float4*>(p.part_sums + at * T::D + c + x), make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]));
+                for (int x = 0; x < 32; x += 4) *reinterpret_cast<float4*>(rows + lane * PITCH + c + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+            }
+            __syncwarp();
+            const int64_t mine_at = there ? at : -1;
+#pragma unroll 4
+            for (int x = 0; x < 32; ++x) {
+                const int64_t row = __shfl_sync(0xffffffffu, mine_at, x);
+                if (row >= 0)
+                    for (int c = lane * 4; c < T::D; c += 128) __stcg(reinterpret_cast<float4*>(p.part_sums + row * T::D + c), *reinterpret_cast<const float4*>(rows + x * PITCH + c));
             }
         }
     }
