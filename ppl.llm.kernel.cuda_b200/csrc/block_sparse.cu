@@ -185,9 +185,11 @@ __global__ void __launch_bounds__(BTPB) key_bounds_read_kernel(const __grid_cons
 // One cluster of CTAs for each sequence and key head.  A CTA scores its share of the blocks, 16 a warp at a time, on int8 mma.sync (16 blocks x 32
 // dimensions x 8 query heads; the product is tiny, what counts is that the bounds are read once and wide): sum_d max(q lo, q hi) is the product of q's
 // positive part with the greatest and of its negative part with the least.  The scores stay in shared memory as numbers that order alike.  The
-// threshold is found by four histograms of eight bits that the cluster's CTAs fill together in the first one's shared memory; then every CTA
-// writes those of its blocks that are above it, and as many of those at it, from the lowest on, as there is room for.
-constexpr int STPB = 256, SWARPS = STPB / 32, MAX_CLUSTER = 8;
+// threshold is found by histograms that the cluster's CTAs fill together in the first one's shared memory: of 2048 bins over the range that the scores
+// have, then over the bin with the threshold in it, until that holds nothing but scores that are taken, or one value; two or three rounds.  (Digits of the scores
+// themselves, whose leading ones hardly differ, put all on a few counters: 25 us where this takes 10.)  Then every CTA writes those of its blocks that are
+// above the threshold, and as many of those at it, from the lowest on, as there is room for.
+constexpr int STPB = 256, SWARPS = STPB / 32, MAX_CLUSTER = 8, BINS = 2048;
 constexpr int64_t MAX_BLOCKS = 1 << 18, MAX_TOTAL = 65536, MAX_ITEMS = 1 << 24;
 struct ChoiceParams {
     const half* q;
@@ -216,6 +218,12 @@ __device__ __forceinline__ uint32_t ordered(float f) {
 __device__ __forceinline__ void add_in_cluster(uint32_t addr, uint32_t v) {
     asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
+__device__ __forceinline__ void min_in_cluster(uint32_t addr, uint32_t v) {
+    asm volatile("red.relaxed.cluster.shared::cluster.min.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void max_in_cluster(uint32_t addr, uint32_t v) {
+    asm volatile("red.relaxed.cluster.shared::cluster.max.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
 __device__ __forceinline__ uint32_t ld_in_cluster(uint32_t addr) {
     uint32_t v;
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -229,8 +237,10 @@ __global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_consta
     extern __shared__ uint32_t keys[]; // [share]
     __shared__ __align__(16) uint32_t q8[8][D / 4];
     __shared__ uint32_t q_bits[8];
-    __shared__ uint32_t histogram[4][256];
-    __shared__ uint32_t above, at_threshold, found[2]; // counts of this CTA; digit and rest
+    // of the cluster's first CTA: bins; least and greatest of the range; how many of it are taken; whether these are all of it
+    __shared__ __align__(16) uint32_t histogram[BINS];
+    __shared__ uint32_t range[2], taken[2];
+    __shared__ uint32_t above, at_threshold; // counts of this CTA
     __shared__ uint32_t scan[SWARPS][2];
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, t = lane & 3;
     const int32_t ctas = gridDim.x, rank = blockIdx.x; // one cluster along x
@@ -268,32 +278,43 @@ __global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_consta
     // ---- scores of this CTA's share ------------------------------------------------------------------------------------------
     const int32_t share = (between + ctas * 16 - 1) / (ctas * 16) * 16;
     const int32_t begin = min(between, rank * share), mine = min(between, begin + share) - begin;
+    for (int x = threadIdx.x; x < BINS; x += STPB) histogram[x] = 0;
+    if (threadIdx.x == 0) range[0] = 0xffffffffu, range[1] = 0, above = at_threshold = 0;
     for (int32_t head0 = 0; head0 < p.shared; head0 += 8) {
         const int heads = min(8, p.shared - head0);
         const half* const q = p.q + b * p.q_stride + (int64_t)(kvh * p.shared + head0) * D;
+        // pieces of eight dimensions, PIECES a thread
+        constexpr int PIECES = (8 * (D / 8) + STPB - 1) / STPB;
+        uint4 raw[PIECES];
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int x = threadIdx.x + i * STPB;
+            raw[i] = x < heads * (D / 8) ? ld_global_16(q + x * 8) : make_uint4(0, 0, 0, 0);
+        }
         if (threadIdx.x < 8) q_bits[threadIdx.x] = 0;
-        for (int x = threadIdx.x; x < 4 * 256 && head0 == 0; x += STPB) histogram[x >> 8][x & 255] = 0;
         __syncthreads();
-        for (int x = threadIdx.x; x < heads * (D / 8); x += STPB) {
-            const uint4 raw = ld_global_16(q + x * 8);
-            const uint32_t w[4] = {raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu, raw.z & 0x7fff7fffu, raw.w & 0x7fff7fffu};
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int x = threadIdx.x + i * STPB;
+            const uint32_t w[4] = {raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu, raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu};
             uint32_t m = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) m = max(m, max(w[i] & 0xffffu, w[i] >> 16));
-            atomicMax(&q_bits[x / (D / 8)], m);
+            for (int k = 0; k < 4; ++k) m = max(m, max(w[k] & 0xffffu, w[k] >> 16));
+            if (x < heads * (D / 8)) atomicMax(&q_bits[x / (D / 8)], m);
         }
         __syncthreads();
-        for (int x = threadIdx.x; x < 8 * (D / 8); x += STPB) {
-            const int h = x / (D / 8);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int x = threadIdx.x + i * STPB, h = x / (D / 8);
+            if (x >= 8 * (D / 8)) break;
             uint32_t o[2] = {};
             if (h < heads && q_bits[h] < 0x7c00u) {
-                const uint4 raw = ld_global_16(q + x * 8);
-                const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+                const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
                 const float s = __half2float(outer_scale(__half2float(__ushort_as_half((unsigned short)q_bits[h]))));
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float v = __half2float(__ushort_as_half((unsigned short)(w[i >> 1] >> (16 * (i & 1)))));
-                    o[i >> 2] |= (uint32_t)(__float2int_rn(__fdiv_rn(v, s)) & 0xff) << (8 * (i & 3));
+                for (int k = 0; k < 8; ++k) {
+                    const float v = __half2float(__ushort_as_half((unsigned short)(w[k >> 1] >> (16 * (k & 1)))));
+                    o[k >> 2] |= (uint32_t)(__float2int_rn(__fdiv_rn(v, s)) & 0xff) << (8 * (k & 3));
                 }
             }
             q8[h][(x - h * (D / 8)) * 2] = o[0];
@@ -317,6 +338,13 @@ __global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_consta
             const int h = 2 * t + x;
             qs[x] = h < heads && q_bits[h] < 0x7c00u ? __half2float(outer_scale(__half2float(__ushort_as_half((unsigned short)q_bits[h])))) : __int_as_float(0x7fffffff);
         }
+        int32_t pages[2]; // of the lane's two blocks, a round ahead
+        auto look_up = [&](int32_t tile) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+                pages[r] = tile < mine ? row_pages[(uint32_t)((uint64_t)(uint32_t)(p.first + begin + min(tile + g + 8 * r, mine - 1)) * p.page_magic >> p.page_shift)] : -1;
+        };
+        look_up(warp * 16);
         for (int32_t tile = warp * 16; tile < mine; tile += SWARPS * 16) {
             uint32_t lo[2][KN][KW], hi[2][KN][KW];
             half scale[2];
@@ -324,7 +352,7 @@ __global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_consta
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int32_t x = min(tile + g + 8 * r, mine - 1), block = p.first + begin + x;
-                const int32_t index = (uint32_t)((uint64_t)(uint32_t)block * p.page_magic >> p.page_shift), page = row_pages[index];
+                const int32_t index = (uint32_t)((uint64_t)(uint32_t)block * p.page_magic >> p.page_shift), page = pages[r];
                 there[r] = (uint32_t)page < (uint32_t)p.num_pages;
                 const int64_t at = ((int64_t)(there[r] ? page : 0) * p.kv_heads + kvh) * p.per_page + (block - index * p.per_page);
                 const char* src = (const char*)p.bounds + at * 2 * D + t * KP;
@@ -339,6 +367,7 @@ __global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_consta
                 }
                 scale[r] = there[r] ? ld_global_half(p.scale + at) : __ushort_as_half(0);
             }
+            look_up(tile + SWARPS * 16);
             int32_t c[4] = {}, c2[4] = {};
 #pragma unroll
             for (int m = 0; m < MMAS; ++m) {
@@ -369,46 +398,81 @@ __global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_consta
         __syncthreads();
     }
 
-    // ---- the threshold: the top-th largest key, digit by digit ------------------------------------------------------------------
-    uint32_t prefix = 0, room = p.top; // of the keys that begin with prefix, `room` are taken
-    const uint32_t hist0 = map_to_cta(ptx::smem_addr(histogram), 0);
-    cluster_sync_all(); // the first CTA's histograms are zero
-    for (int digit = 0; digit < 4; ++digit) {
-        const int shift = 24 - 8 * digit;
-        for (int32_t x = threadIdx.x; x < mine; x += STPB) {
-            const uint32_t key = keys[x];
-            if (digit == 0 || key >> (shift + 8) == prefix) add_in_cluster(hist0 + (digit * 256 + (key >> shift & 255u)) * 4, 1);
-        }
-        cluster_sync_all();
-        // bins from the highest down: thread x has bin 255 - x
-        const uint32_t bin = 255 - threadIdx.x, mine_here = ld_in_cluster(hist0 + (digit * 256 + bin) * 4);
-        uint32_t sum = mine_here;
+    // ---- the threshold ---------------------------------------------------------------------------------------------------------
+    auto sync = [&] {
+        if (ctas > 1) cluster_sync_all();
+        else __syncthreads();
+    };
+    const uint32_t bins0 = map_to_cta(ptx::smem_addr(histogram), 0), range0 = map_to_cta(ptx::smem_addr(range), 0), taken0 = map_to_cta(ptx::smem_addr(taken), 0);
+    sync(); // the first CTA's histogram and range are there
+    {
+        uint32_t least = 0xffffffffu, most = 0;
+        for (int32_t x = threadIdx.x; x < mine; x += STPB) least = min(least, keys[x]), most = max(most, keys[x]);
+        least = __reduce_min_sync(0xffffffffu, least);
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0 && least <= most) min_in_cluster(range0, least), max_in_cluster(range0 + 4, most);
+    }
+    sync();
+    uint32_t least = ld_in_cluster(range0), most = ld_in_cluster(range0 + 4), room = p.top, all = 0; // of the scores in [least, most], `room` are taken
+    for (;;) {
+        const uint32_t shift = max(0, 21 - __clz((int)(most - least))); // 2048 bins at most
+        for (int32_t x = threadIdx.x; x < mine; x += STPB)
+            if (keys[x] >= least && keys[x] <= most) add_in_cluster(bins0 + ((keys[x] - least) >> shift) * 4, 1);
+        sync();
+        if (rank == 0) {
+            // bins from the highest down: thread x has those from BINS - 8 x - 1 on
+            uint4* const here = reinterpret_cast<uint4*>(histogram + BINS - 8 - 8 * threadIdx.x);
+            const uint4 low = here[0], high = here[1];
+            here[0] = here[1] = make_uint4(0, 0, 0, 0);
+            const uint32_t n8[8] = {high.w, high.z, high.y, high.x, low.w, low.z, low.y, low.x};
+            uint32_t own = 0;
 #pragma unroll
-        for (int m = 1; m < 32; m <<= 1) {
-            const uint32_t v = __shfl_up_sync(0xffffffffu, sum, m);
-            if (lane >= m) sum += v;
+            for (int k = 0; k < 8; ++k) own += n8[k];
+            uint32_t sum = own;
+#pragma unroll
+            for (int m = 1; m < 32; m <<= 1) {
+                const uint32_t v = __shfl_up_sync(0xffffffffu, sum, m);
+                if (lane >= m) sum += v;
+            }
+            if (lane == 31) scan[warp][0] = sum;
+            __syncthreads();
+            for (int w = 0; w < warp; ++w) sum += scan[w][0];
+            uint32_t over = sum - own;
+            if (over < room && sum >= room) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if (over < room && over + n8[k] >= room) {
+                        const uint32_t bin = BINS - 1 - 8 * threadIdx.x - k;
+                        const uint32_t first = least + (bin << shift), width = (1u << shift) - 1;
+                        range[0] = first;
+                        range[1] = most - first < width ? most : first + width;
+                        taken[0] = room - over;
+                        taken[1] = n8[k] == room - over;
+                    }
+                    over += n8[k];
+                }
+            }
         }
-        if (lane == 31) scan[warp][0] = sum;
-        __syncthreads();
-        for (int w = 0; w < warp; ++w) sum += scan[w][0];
-        if (sum >= room && sum - mine_here < room) found[0] = bin, found[1] = room - (sum - mine_here);
-        __syncthreads();
-        prefix = prefix << 8 | found[0];
-        room = found[1];
-        __syncthreads();
+        sync();
+        least = ld_in_cluster(range0);
+        most = ld_in_cluster(range0 + 4);
+        room = ld_in_cluster(taken0);
+        all = ld_in_cluster(taken0 + 4);
+        if (shift == 0 || all) break;
     }
 
     // ---- what is above the threshold, and the first `room` of those at it, in order ------------------------------------------------
-    if (threadIdx.x == 0) above = at_threshold = 0;
-    __syncthreads();
+    auto over_it = [&](uint32_t key) { return all ? key >= least : key > least; };
+    auto at_it = [&](uint32_t key) { return !all && key == least; };
     uint32_t counts[2] = {};
     for (int32_t x = threadIdx.x; x < mine; x += STPB) {
-        counts[0] += keys[x] > prefix;
-        counts[1] += keys[x] == prefix;
+        counts[0] += over_it(keys[x]);
+        counts[1] += at_it(keys[x]);
     }
-    if (counts[0]) atomicAdd(&above, counts[0]);
-    if (counts[1]) atomicAdd(&at_threshold, counts[1]);
-    cluster_sync_all();
+    counts[0] = __reduce_add_sync(0xffffffffu, counts[0]);
+    counts[1] = __reduce_add_sync(0xffffffffu, counts[1]);
+    if (lane == 0) atomicAdd(&above, counts[0]), atomicAdd(&at_threshold, counts[1]);
+    sync();
     uint32_t before[2] = {};
     for (int32_t r = 0; r < rank; ++r) {
         before[0] += ld_in_cluster(map_to_cta(ptx::smem_addr(&above), r));
@@ -417,7 +481,7 @@ __global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_consta
     for (int32_t x0 = 0; x0 < mine; x0 += STPB) {
         const int32_t x = x0 + threadIdx.x;
         const uint32_t key = x < mine ? keys[x] : 0u;
-        const bool over = x < mine && key > prefix, same = x < mine && key == prefix;
+        const bool over = x < mine && over_it(key), same = x < mine && at_it(key);
         const uint32_t overs = __ballot_sync(0xffffffffu, over), sames = __ballot_sync(0xffffffffu, same), below = (1u << lane) - 1;
         if (lane == 0) scan[warp][0] = __popc(overs), scan[warp][1] = __popc(sames);
         __syncthreads();
@@ -430,7 +494,7 @@ __global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_consta
         if (over || (same && s < room)) put(p.first + o + min(s, room), p.first + begin + x);
         __syncthreads();
     }
-    cluster_sync_all(); // no CTA leaves while another reads its shared memory
+    sync(); // no CTA leaves while another reads its shared memory
 }
 
 int32_t check_bounds(const pplb200_kv_cache* c, const pplb200_key_bounds* k) {

@@ -6,7 +6,7 @@
 //
 //   warps 0 - 3, 4 - 7   softmax of one tile each, a thread a row (tensor memory's lanes): scores in, weights of 11 bits out, in place
 //   warps 8 - 11         keys and values from the pages into shared memory; int8 ones are widened on the way
-//   warp 12              one thread issues all products; the warp owns the tensor memory
+//   warp 12              issues all products, and owns the tensor memory
 //
 // The two tiles' products and softmaxes alternate, so that the tensor cores work on one while the exponentials of the other are computed.  Where a CTA has one
 // tile only, the two softmax groups take turns at the blocks of it, each with a sum of its own (heads of 256: one group, whose sum alone fills
@@ -127,46 +127,47 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
 
     if (warp >= 12) {
         ptx::registers_down<40>();
-        if (warp == 12 && lane == 0 && tasks > 0) {
-            // ---- products --------------------------------------------------------------------------------------------------
+        if (warp == 12 && tasks > 0) {
+            // ---- products, by one lane of a warp that does the same in all -------------------------------------------------------------------------------------------------
             constexpr uint32_t QK = ptx::make_f16_idesc(128, T::NB, false), PV = ptx::make_f16_idesc(128, T::D, true);
-            bool ok = ptx::mbar_wait(bar(q_full), 0, &g_status, ST_MMA);
+            const uint32_t leads = ptx::elect_one();
+            bool ok = __all_sync(0xffffffffu, ptx::mbar_wait(bar(q_full), 0, &g_status, ST_MMA));
             auto scores = [&](int32_t i) {
                 const int32_t j = i >> shift, stage = j % T::KS;
-                if (!(ok = ok && ptx::mbar_wait(bar(full_k[stage]), (j / T::KS) & 1, &g_status, ST_MMA))) return;
+                if (!(ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(bar(full_k[stage]), (j / T::KS) & 1, &g_status, ST_MMA)))) return;
                 ptx::tc_fence_after();
                 const uint32_t q = ptx::desc_lo_sw128(smem + (tiles == 2 ? (i & 1) * T::Q_BYTES : 0)), k = ptx::desc_lo_sw128(smem + T::RING + stage * T::K_BYTES);
                 const uint32_t d = tmem + (i & 1) * 128;
 #pragma unroll
                 for (int s = 0; s < T::D / 16; ++s) {
                     const uint32_t a = q + ((s / 4) * (128 * 128) + (s % 4) * 32) / 16, b = k + ((s / 4) * (T::NB * 128) + (s % 4) * 32) / 16;
-                    ptx::mma_f16(d, ptx::desc_from_lo(a), ptx::desc_from_lo(b), QK, s > 0);
-                    if constexpr (T::LOW) ptx::mma_f16(d, ptx::desc_from_lo(a), ptx::desc_from_lo(b + T::V_BYTES / 16), QK, 1);
+                    ptx::mma_f16(d, ptx::desc_from_lo(a), ptx::desc_from_lo(b), QK, s > 0, leads);
+                    if constexpr (T::LOW) ptx::mma_f16(d, ptx::desc_from_lo(a), ptx::desc_from_lo(b + T::V_BYTES / 16), QK, 1, leads);
                 }
-                ptx::mma_commit(bar(score_full[i & 1]));
-                if (tiles == 1 || (i & 1)) ptx::mma_commit(bar(empty_k[stage]));
+                ptx::mma_commit_by(bar(score_full[i & 1]), leads);
+                if (tiles == 1 || (i & 1)) ptx::mma_commit_by(bar(empty_k[stage]), leads);
             };
             scores(0);
             if (tasks > 1) scores(1);
             for (int32_t i = 0; i < tasks && ok; ++i) {
                 const int32_t j = i >> shift, stage = j % T::VS;
-                if (!(ok = ptx::mbar_wait(bar(full_v[stage]), (j / T::VS) & 1, &g_status, ST_MMA))) break;
+                if (!(ok = __all_sync(0xffffffffu, ptx::mbar_wait(bar(full_v[stage]), (j / T::VS) & 1, &g_status, ST_MMA)))) break;
                 const uint32_t v = mn_desc_lo(smem + T::V_RING + stage * T::V_BYTES, T::NB * 128);
                 const uint32_t d = tmem + T::O_COLUMN + (T::STREAMS == 2 ? (i & 1) * T::DP : 0), w = tmem + (i & 1) * 128;
                 // the weights of the block's first half are worked with while the others are computed
 #pragma unroll
                 for (int half = 0; half < 2 && ok; ++half) {
-                    if (!(ok = ptx::mbar_wait(bar(half ? weight_full[i & 1] : weight_half[i & 1]), (i >> 1) & 1, &g_status, ST_MMA))) break;
+                    if (!(ok = __all_sync(0xffffffffu, ptx::mbar_wait(bar(half ? weight_full[i & 1] : weight_half[i & 1]), (i >> 1) & 1, &g_status, ST_MMA)))) break;
                     ptx::tc_fence_after();
 #pragma unroll
                     for (int s = half * T::NB / 32; s < (half + 1) * T::NB / 32; ++s)
-                        ptx::mma_f16_tmem(d, w + s * 8, ptx::desc_from_lo(v + s * (2048 / 16)), PV, (T::STREAMS == 2 ? i > 1 : i > 0) || s > 0);
+                        ptx::mma_f16_tmem(d, w + s * 8, ptx::desc_from_lo(v + s * (2048 / 16)), PV, (T::STREAMS == 2 ? i > 1 : i > 0) || s > 0, leads);
                 }
-                ptx::mma_commit(bar(sum_done[i & 1]));
-                if (tiles == 1 || (i & 1)) ptx::mma_commit(bar(empty_v[stage]));
+                ptx::mma_commit_by(bar(sum_done[i & 1]), leads);
+                if (tiles == 1 || (i & 1)) ptx::mma_commit_by(bar(empty_v[stage]), leads);
                 if (i + 2 < tasks) scores(i + 2);
             }
-            ptx::mma_commit(bar(all_done)); // all that was issued
+            ptx::mma_commit_by(bar(all_done), leads); // all that was issued
         }
     } else if (warp >= 8) {
         ptx::registers_down<120>();
