@@ -3,6 +3,8 @@
 #include "paged_attention.cuh"
 #include "ptx.cuh"
 
+#include <type_traits>
+
 namespace pplb200 {
 namespace {
 
@@ -18,10 +20,10 @@ __device__ __forceinline__ half outer_scale(float amax) {
 __device__ __forceinline__ bool is_finite(half s) { return (__half_as_ushort(s) & 0x7c00u) != 0x7c00u; }
 
 // ---- bounds ------------------------------------------------------------------------------------------------------------
-// A CTA looks through a few slots for those that end a block, and goes through these blocks one after the other, for one head: a thread has eight
-// dimensions, head_dim / 8 neighbouring threads a token's row, so that as many rows are on their way as the CTA has threads for.
-// Bound by HBM in a long prompt: the keys once, 2 bytes in 2 * block * element back.
-constexpr int BTPB = 128;
+// A CTA looks through a few slots for those that end a block; its warps then take these blocks, a head each: head_dim / 8 lanes have a token's row, eight
+// dimensions a lane, and as many rows are on their way as eight loads a lane bring.  Nothing is shared but the warp's last few shuffles.
+// Bound by HBM in a long prompt, the keys once (16384 tokens of 8 heads of 128 in fp16, blocks of 64: FIGURE); by look-ups in a decode step.
+constexpr int BWARPS = 4, BTPB = 32 * BWARPS;
 struct BoundsParams {
     pplb200_kv_cache cache;
     int8_t* bounds;
@@ -32,18 +34,17 @@ struct BoundsParams {
     uint32_t block_magic, block_shift;
 };
 
-template <int KIND>
+template <int D, int KIND>
 __global__ void __launch_bounds__(BTPB) key_bounds_kernel(const __grid_constant__ BoundsParams p) {
-    __shared__ int64_t block_of[BTPB];
+    constexpr int LANES = D / 8, ROWS = 32 / LANES, BATCH = 8; // of a row; rows at once; loads on their way
+    struct Block {
+        int64_t page;
+        int32_t x;
+    };
+    __shared__ Block block_of[BTPB];
     __shared__ int32_t found;
-    __shared__ float lows[BTPB][8 + 1], highs[BTPB][8 + 1];
-    __shared__ float most[BTPB];
-    __shared__ int32_t any_bad;
     const pplb200_kv_cache& c = p.cache;
-    const int lanes = c.head_dim >> 3, rows = BTPB / lanes;
-    const int row = threadIdx.x / lanes, lane = threadIdx.x - row * lanes;
-    const bool active = row < rows;
-    const int64_t head = blockIdx.y;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) found = 0;
     pdl_wait_prior_grid();
     __syncthreads();
@@ -53,100 +54,102 @@ __global__ void __launch_bounds__(BTPB) key_bounds_kernel(const __grid_constant_
         int32_t in_page;
         if (kv_find(p.slots[first_slot + threadIdx.x], c.num_pages, c.page_size, page, in_page)) {
             const int32_t x = (uint32_t)((uint64_t)(uint32_t)in_page * p.block_magic >> p.block_shift);
-            if (in_page - x * p.block == p.block - 1) block_of[atomicAdd(&found, 1)] = page * p.per_page + x;
+            if (in_page - x * p.block == p.block - 1) block_of[atomicAdd(&found, 1)] = {page, x};
         }
     }
     __syncthreads();
-    const int number = found;
-    for (int i = 0; i < number; ++i) {
-        const int64_t page = block_of[i] / p.per_page;
-        const int32_t token0 = (int32_t)(block_of[i] - page * p.per_page) * p.block;
-        const int64_t at = kv_row(page, token0, head, c.page_stride, c.head_stride, c.token_stride) + lane * 8;
-        const int64_t scale_at = kv_row(page, token0, head, c.scale_page_stride, c.scale_head_stride, c.scale_token_stride) + (KIND == CACHE_I8_GROUPS ? lane : 0);
+    const int64_t head = (int64_t)blockIdx.y * BWARPS + warp;
+    if (head >= c.kv_heads) return;
+    const int row = lane / LANES, part = lane - row * LANES;
+    const bool active = row < ROWS; // (heads of 96: 24 lanes)
+    for (int i = 0; i < found; ++i) {
+        const int64_t page = block_of[i].page;
+        const int32_t x = block_of[i].x, token0 = x * p.block + (active ? row : 0);
+        const int64_t at = kv_row(page, token0, head, c.page_stride, c.head_stride, c.token_stride) + part * 8;
+        const int64_t scale_at = kv_row(page, token0, head, c.scale_page_stride, c.scale_head_stride, c.scale_token_stride) + (KIND == CACHE_I8_GROUPS ? part : 0);
         float lo[8], hi[8];
-        bool bad = false;
+        bool bad = false; // a scale that is infinite or NaN; of fp16 keys, these come through in the bounds
+        if constexpr (KIND == CACHE_F16) {
+            __half2 l[4], h[4];
 #pragma unroll
-        for (int d = 0; d < 8; ++d) lo[d] = INFINITY, hi[d] = -INFINITY;
-        if (active) {
-            if constexpr (KIND == CACHE_F16) {
-                __half2 l[4], h[4];
-                uint32_t largest = 0;
+            for (int d = 0; d < 4; ++d) l[d] = as_h2(0x7c007c00u), h[d] = as_h2(0xfc00fc00u);
+            for (int32_t t = 0; t < p.block; t += BATCH * ROWS) { // (ROWS divides 16, and 16 the block)
+                uint4 w[BATCH];
 #pragma unroll
-                for (int d = 0; d < 4; ++d) l[d] = __half2half2(__ushort_as_half(0x7c00)), h[d] = __half2half2(__ushort_as_half(0xfc00));
-#pragma unroll 8
-                for (int t = row; t < p.block; t += rows) {
-                    const uint4 raw = ld_global_16((const half*)c.k + at + t * c.token_stride);
-                    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+                for (int k = 0; k < BATCH; ++k)
+                    if (t + k * ROWS < p.block) w[k] = ld_global_16((const half*)c.k + at + (t + k * ROWS) * c.token_stride);
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        l[d] = __hmin2(l[d], as_h2(w[d]));
-                        h[d] = __hmax2(h[d], as_h2(w[d]));
-                        const uint32_t magnitude = w[d] & 0x7fff7fffu;
-                        largest = max(largest, max(magnitude & 0xffffu, magnitude >> 16));
+                for (int k = 0; k < BATCH; ++k)
+                    if (t + k * ROWS < p.block) {
+                        const uint32_t words[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) l[d] = __hmin2_nan(l[d], as_h2(words[d])), h[d] = __hmax2_nan(h[d], as_h2(words[d]));
                     }
-                }
-                bad = largest >= 0x7c00u;
+            }
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const float2 a = __half22float2(l[d]), b = __half22float2(h[d]);
-                    lo[2 * d] = a.x; lo[2 * d + 1] = a.y;
-                    hi[2 * d] = b.x; hi[2 * d + 1] = b.y;
-                }
-            } else {
-#pragma unroll 8
-                for (int t = row; t < p.block; t += rows) {
-                    uint2 w;
-                    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "l"((const int8_t*)c.k + at + t * c.token_stride));
-                    const half s = ld_global_half((const half*)c.k_scale + scale_at + t * c.scale_token_stride);
-                    bad |= !is_finite(s);
-                    const float f = __half2float(s);
+            for (int d = 0; d < 4; ++d) {
+                const float2 a = __half22float2(l[d]), b = __half22float2(h[d]);
+                lo[2 * d] = a.x; lo[2 * d + 1] = a.y;
+                hi[2 * d] = b.x; hi[2 * d + 1] = b.y;
+            }
 #pragma unroll
-                    for (int d = 0; d < 8; ++d) {
-                        const float v = (float)(int8_t)((d < 4 ? w.x : w.y) >> (8 * (d & 3))) * f;
-                        lo[d] = fminf(lo[d], v);
-                        hi[d] = fmaxf(hi[d], v);
+            for (int d = 0; d < 8; ++d) bad |= !(fabsf(lo[d]) < INFINITY) || !(fabsf(hi[d]) < INFINITY);
+        } else {
+#pragma unroll
+            for (int d = 0; d < 8; ++d) lo[d] = INFINITY, hi[d] = -INFINITY;
+            for (int32_t t = 0; t < p.block; t += BATCH * ROWS) {
+                uint2 w[BATCH];
+                half s[BATCH];
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k)
+                    if (t + k * ROWS < p.block) {
+                        asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(w[k].x), "=r"(w[k].y) : "l"((const int8_t*)c.k + at + (t + k * ROWS) * c.token_stride));
+                        s[k] = ld_global_half((const half*)c.k_scale + scale_at + (t + k * ROWS) * c.scale_token_stride);
                     }
-                }
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k)
+                    if (t + k * ROWS < p.block) {
+                        bad |= !is_finite(s[k]);
+                        const float f = __half2float(s[k]);
+#pragma unroll
+                        for (int d = 0; d < 8; ++d) {
+                            const float v = (float)(int8_t)((d < 4 ? w[k].x : w[k].y) >> (8 * (d & 3))) * f;
+                            lo[d] = fminf(lo[d], v);
+                            hi[d] = fmaxf(hi[d], v);
+                        }
+                    }
             }
         }
-        if (threadIdx.x == 0) any_bad = 0;
+        // the other rows' bounds of these dimensions
 #pragma unroll
-        for (int d = 0; d < 8; ++d) lows[threadIdx.x][d] = lo[d], highs[threadIdx.x][d] = hi[d];
-        __syncthreads();
-        if (bad) any_bad = 1;
-        if (row == 0) { // the other rows' bounds of these dimensions
-            float amax = 0.0f;
-            for (int r = 1; r < min(rows, p.block); ++r)
-#pragma unroll
-                for (int d = 0; d < 8; ++d) {
-                    lo[d] = fminf(lo[d], lows[r * lanes + lane][d]);
-                    hi[d] = fmaxf(hi[d], highs[r * lanes + lane][d]);
-                }
-#pragma unroll
-            for (int d = 0; d < 8; ++d) amax = fmaxf(amax, fmaxf(fabsf(lo[d]), fabsf(hi[d])));
-            most[lane] = amax;
-        }
-        __syncthreads();
-        if (row == 0) {
-            float amax = 0.0f;
-            for (int x = 0; x < lanes; ++x) amax = fmaxf(amax, most[x]);
-            half s = outer_scale(amax);
-            const bool lost = any_bad || !is_finite(s);
-            if (lost) s = __ushort_as_half(0x7c00);
-            const float step = __half2float(s);
-            uint32_t l[2] = {}, h[2] = {};
+        for (int r = 1; r < ROWS; r <<= 1)
 #pragma unroll
             for (int d = 0; d < 8; ++d) {
-                const int a = lost ? 0 : (int)floorf(__fdiv_rn(lo[d], step)), b = lost ? 0 : (int)ceilf(__fdiv_rn(hi[d], step));
-                l[d >> 2] |= (uint32_t)(a & 0xff) << (8 * (d & 3));
-                h[d >> 2] |= (uint32_t)(b & 0xff) << (8 * (d & 3));
+                lo[d] = fminf(lo[d], __shfl_down_sync(0xffffffffu, lo[d], r * LANES));
+                hi[d] = fmaxf(hi[d], __shfl_down_sync(0xffffffffu, hi[d], r * LANES));
             }
-            const int64_t of = (page * c.kv_heads + head) * p.per_page + token0 / p.block;
-            *reinterpret_cast<uint2*>(p.bounds + of * 2 * c.head_dim + lane * 8) = make_uint2(l[0], l[1]);
-            *reinterpret_cast<uint2*>(p.bounds + (of * 2 + 1) * c.head_dim + lane * 8) = make_uint2(h[0], h[1]);
+        const bool lost_key = __any_sync(0xffffffffu, bad && active);
+        float amax = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) amax = fmaxf(amax, fmaxf(fabsf(lo[d]), fabsf(hi[d])));
+        amax = __uint_as_float(__reduce_max_sync(0xffffffffu, row == 0 ? __float_as_uint(amax) : 0u));
+        half s = outer_scale(amax);
+        const bool lost = lost_key || !is_finite(s);
+        if (lost) s = __ushort_as_half(0x7c00);
+        const float step = __half2float(s);
+        uint32_t l[2] = {}, h[2] = {};
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            const int a = lost ? 0 : (int)floorf(__fdiv_rn(lo[d], step)), b = lost ? 0 : (int)ceilf(__fdiv_rn(hi[d], step));
+            l[d >> 2] |= (uint32_t)(a & 0xff) << (8 * (d & 3));
+            h[d >> 2] |= (uint32_t)(b & 0xff) << (8 * (d & 3));
+        }
+        if (row == 0) {
+            const int64_t of = (page * c.kv_heads + head) * p.per_page + x;
+            *reinterpret_cast<uint2*>(p.bounds + of * 2 * D + part * 8) = make_uint2(l[0], l[1]);
+            *reinterpret_cast<uint2*>(p.bounds + (of * 2 + 1) * D + part * 8) = make_uint2(h[0], h[1]);
             if (lane == 0) p.scale[of] = s;
         }
-        __syncthreads();
     }
 }
 
@@ -189,7 +192,7 @@ __global__ void __launch_bounds__(BTPB) key_bounds_read_kernel(const __grid_cons
 // have, then over the bin with the threshold in it, until that holds nothing but scores that are taken, or one value; two or three rounds.  (Digits of the scores
 // themselves, whose leading ones hardly differ, put all on a few counters: 25 us where this takes 10.)  Then every CTA writes those of its blocks that are
 // above the threshold, and as many of those at it, from the lowest on, as there is room for.
-constexpr int STPB = 256, SWARPS = STPB / 32, MAX_CLUSTER = 8, BINS = 2048;
+constexpr int MAX_CLUSTER = 8, BINS = 2048;
 constexpr int64_t MAX_BLOCKS = 1 << 18, MAX_TOTAL = 65536, MAX_ITEMS = 1 << 24;
 struct ChoiceParams {
     const half* q;
@@ -203,7 +206,8 @@ struct ChoiceParams {
     int64_t tokens_in_table, items;
     int32_t kv_heads, shared, block, per_page, num_pages, first, last, top, total;
     uint32_t block_magic, block_shift, page_magic, page_shift; // / block, / per_page
-    int32_t share; // blocks of a CTA at most, a multiple of 16
+    int32_t share;   // blocks of a CTA at most, a multiple of 16
+    bool units_kept; // shared memory for the blocks' numbers beside their scores
 };
 
 __device__ __forceinline__ void mma_s8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -230,72 +234,104 @@ __device__ __forceinline__ uint32_t ld_in_cluster(uint32_t addr) {
     return v;
 }
 
-template <int D>
-__global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_constant__ ChoiceParams p) {
+template <int D, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_constant__ ChoiceParams p) {
+    constexpr int TPB = 32 * WARPS;
     constexpr int KB = D / 4, KP = piece(KB), KN = KB / KP, KW = KP / 4; // a quad's lane has a quarter of a row, in pieces
-    constexpr int MMAS = D / 32;
-    extern __shared__ uint32_t keys[]; // [share]
+    constexpr int MMAS = D / 32, TILES = D == 256 ? 1 : 2;               // tiles of 16 blocks that a warp has on their way together
+    constexpr int PIECES = (D + TPB - 1) / TPB;                          // of q, eight dimensions each, a thread
+    extern __shared__ uint32_t keys[];       // [share]: scores; where there is room, units[share]: the blocks' numbers in the cache
+    int32_t* const units = p.units_kept ? reinterpret_cast<int32_t*>(keys + p.share) : nullptr;
     __shared__ __align__(16) uint32_t q8[8][D / 4];
     __shared__ uint32_t q_bits[8];
     // of the cluster's first CTA: bins; least and greatest of the range; how many of it are taken; whether these are all of it
     __shared__ __align__(16) uint32_t histogram[BINS];
     __shared__ uint32_t range[2], taken[2];
     __shared__ uint32_t above, at_threshold; // counts of this CTA
-    __shared__ uint32_t scan[SWARPS][2];
+    __shared__ uint32_t scan[WARPS][2];
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, t = lane & 3;
     const int32_t ctas = gridDim.x, rank = blockIdx.x; // one cluster along x
     const int64_t item = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
     if (item >= p.items) return; // (the whole cluster)
     const int64_t b = item / p.kv_heads;
     const int32_t kvh = (int32_t)(item - b * p.kv_heads);
+    for (int x = threadIdx.x; x < BINS; x += TPB) histogram[x] = 0;
+    if (threadIdx.x == 0) range[0] = 0xffffffffu, range[1] = 0, above = at_threshold = 0;
     pdl_wait_prior_grid();
     pdl_launch_dependents();
+
+    // q of up to eight heads, and the length: on their way together
+    const half* const q = p.q + b * p.q_stride + (int64_t)kvh * p.shared * D;
+    uint4 raw[PIECES];
+    auto load_q = [&](int32_t head0) {
+        const int heads = min(8, p.shared - head0);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int x = threadIdx.x + i * TPB;
+            raw[i] = x < heads * (D / 8) ? ld_global_16(q + (int64_t)head0 * D + x * 8) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    load_q(0);
     const int32_t n = (int32_t)min((int64_t)max(p.lengths[b], 0), p.tokens_in_table);
     const int32_t blocks = (uint32_t)((uint64_t)(uint32_t)(n + p.block - 1) * p.block_magic >> p.block_shift);
     const int32_t* const row_pages = p.pages + b * p.pages_stride;
     int32_t* const list = p.lists + item * p.total;
     int32_t* const told = p.optional_blocks ? p.optional_blocks + item * p.total : nullptr;
     const int32_t count = min(blocks, p.total);
-    auto put = [&](int32_t at, int32_t block) {
-        const int32_t index = (uint32_t)((uint64_t)(uint32_t)block * p.page_magic >> p.page_shift), page = row_pages[index];
-        list[at] = (uint32_t)page < (uint32_t)p.num_pages ? page * p.per_page + (block - index * p.per_page) : -1;
+    auto page_index = [&](int32_t block) { return (int32_t)(uint32_t)((uint64_t)(uint32_t)block * p.page_magic >> p.page_shift); };
+    auto unit_of = [&](int32_t block, int32_t page) { return (uint32_t)page < (uint32_t)p.num_pages ? page * p.per_page + (block - page_index(block) * p.per_page) : -1; };
+    auto put = [&](int32_t at, int32_t block, int32_t unit) {
+        list[at] = unit;
         if (told) told[at] = block;
     };
     if (rank == 0 && kvh == 0 && threadIdx.x == 0) p.listed_tokens[b] = count == 0 ? 0 : n - (blocks - count) * p.block;
     if (told)
-        for (int32_t i = count + rank * STPB + threadIdx.x; i < p.total; i += ctas * STPB) told[i] = -1;
+        for (int32_t i = count + rank * TPB + threadIdx.x; i < p.total; i += ctas * TPB) told[i] = -1;
     if (blocks <= p.total) { // all of them
-        for (int32_t i = rank * STPB + threadIdx.x; i < count; i += ctas * STPB) put(i, i);
+        for (int32_t i = rank * TPB + threadIdx.x; i < count; i += ctas * TPB) put(i, i, unit_of(i, row_pages[page_index(i)]));
         return;
     }
-    if (rank == 0) {
-        for (int32_t i = threadIdx.x; i < p.first; i += STPB) put(i, i);
-        for (int32_t i = threadIdx.x; i < p.last; i += STPB) put(p.first + p.top + i, blocks - p.last + i);
+    // the first and the last ones: their pages are looked up now, by the cluster's last CTA, and used at the end (the first TPB of them)
+    const int32_t kept = p.first + p.last;
+    auto kept_block = [&](int32_t i) { return i < p.first ? i : blocks - kept + i; };
+    const bool keeps = rank == ctas - 1;
+    int32_t kept_page = keeps && (int32_t)threadIdx.x < kept ? row_pages[page_index(kept_block(threadIdx.x))] : -1;
+    auto put_kept = [&] {
+        if (!keeps) return;
+        for (int32_t i = threadIdx.x; i < kept; i += TPB) {
+            const int32_t block = kept_block(i), page = i < TPB ? kept_page : row_pages[page_index(block)];
+            put(i < p.first ? i : p.top + i, block, unit_of(block, page));
+        }
+    };
+    const int32_t between = blocks - kept; // more than p.top
+    if (p.top == 0) {
+        put_kept();
+        return;
     }
-    const int32_t between = blocks - p.first - p.last; // more than p.top
-    if (p.top == 0) return;
 
     // ---- scores of this CTA's share ------------------------------------------------------------------------------------------
     const int32_t share = (between + ctas * 16 - 1) / (ctas * 16) * 16;
     const int32_t begin = min(between, rank * share), mine = min(between, begin + share) - begin;
-    for (int x = threadIdx.x; x < BINS; x += STPB) histogram[x] = 0;
-    if (threadIdx.x == 0) range[0] = 0xffffffffu, range[1] = 0, above = at_threshold = 0;
+    int32_t pages[TILES][2]; // of the lane's blocks, a round ahead
+    auto look_up = [&](int32_t tile) {
+#pragma unroll
+        for (int m = 0; m < TILES; ++m)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int32_t x = tile + m * WARPS * 16 + g + 8 * r;
+                pages[m][r] = x < mine ? row_pages[page_index(p.first + begin + x)] : -1;
+            }
+    };
+    uint32_t lowest = 0xffffffffu, highest = 0;
     for (int32_t head0 = 0; head0 < p.shared; head0 += 8) {
         const int heads = min(8, p.shared - head0);
-        const half* const q = p.q + b * p.q_stride + (int64_t)(kvh * p.shared + head0) * D;
-        // pieces of eight dimensions, PIECES a thread
-        constexpr int PIECES = (8 * (D / 8) + STPB - 1) / STPB;
-        uint4 raw[PIECES];
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int x = threadIdx.x + i * STPB;
-            raw[i] = x < heads * (D / 8) ? ld_global_16(q + x * 8) : make_uint4(0, 0, 0, 0);
-        }
+        const bool ends = head0 + 8 >= p.shared;
+        look_up(warp * 16);
         if (threadIdx.x < 8) q_bits[threadIdx.x] = 0;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const int x = threadIdx.x + i * STPB;
+            const int x = threadIdx.x + i * TPB;
             const uint32_t w[4] = {raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu, raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu};
             uint32_t m = 0;
 #pragma unroll
@@ -305,7 +341,7 @@ __global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_consta
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const int x = threadIdx.x + i * STPB, h = x / (D / 8);
+            const int x = threadIdx.x + i * TPB, h = x / (D / 8);
             if (x >= 8 * (D / 8)) break;
             uint32_t o[2] = {};
             if (h < heads && q_bits[h] < 0x7c00u) {
@@ -321,6 +357,7 @@ __global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_consta
             q8[h][(x - h * (D / 8)) * 2 + 1] = o[1];
         }
         __syncthreads();
+        if (!ends) load_q(head0 + 8);
         // a product's dimensions come as the lane has them: words 2 m and 2 m + 1 of its own
         uint32_t plus[MMAS][2], minus[MMAS][2];
 #pragma unroll
@@ -338,64 +375,62 @@ __global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_consta
             const int h = 2 * t + x;
             qs[x] = h < heads && q_bits[h] < 0x7c00u ? __half2float(outer_scale(__half2float(__ushort_as_half((unsigned short)q_bits[h])))) : __int_as_float(0x7fffffff);
         }
-        int32_t pages[2]; // of the lane's two blocks, a round ahead
-        auto look_up = [&](int32_t tile) {
+        for (int32_t tile = warp * 16; tile < mine; tile += TILES * WARPS * 16) {
+            uint32_t lo[TILES][2][KN][KW], hi[TILES][2][KN][KW];
+            half scale[TILES][2];
+            int32_t unit[TILES][2];
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
-                pages[r] = tile < mine ? row_pages[(uint32_t)((uint64_t)(uint32_t)(p.first + begin + min(tile + g + 8 * r, mine - 1)) * p.page_magic >> p.page_shift)] : -1;
-        };
-        look_up(warp * 16);
-        for (int32_t tile = warp * 16; tile < mine; tile += SWARPS * 16) {
-            uint32_t lo[2][KN][KW], hi[2][KN][KW];
-            half scale[2];
-            bool there[2];
+            for (int m = 0; m < TILES; ++m)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int32_t x = min(tile + g + 8 * r, mine - 1), block = p.first + begin + x;
-                const int32_t index = (uint32_t)((uint64_t)(uint32_t)block * p.page_magic >> p.page_shift), page = pages[r];
-                there[r] = (uint32_t)page < (uint32_t)p.num_pages;
-                const int64_t at = ((int64_t)(there[r] ? page : 0) * p.kv_heads + kvh) * p.per_page + (block - index * p.per_page);
-                const char* src = (const char*)p.bounds + at * 2 * D + t * KP;
+                for (int r = 0; r < 2; ++r) {
+                    const int32_t x = tile + m * WARPS * 16 + g + 8 * r, block = p.first + begin + x, page = pages[m][r];
+                    unit[m][r] = x < mine ? unit_of(block, page) : -1;
+                    const int64_t at = ((int64_t)page * p.kv_heads + kvh) * p.per_page + (block - page_index(block) * p.per_page);
+                    const char* src = (const char*)p.bounds + at * 2 * D + t * KP;
 #pragma unroll
-                for (int i = 0; i < KN; ++i) {
+                    for (int i = 0; i < KN; ++i) {
 #pragma unroll
-                    for (int w = 0; w < KW; ++w) lo[r][i][w] = hi[r][i][w] = 0;
-                    if (there[r]) {
-                        load_piece<KP>(lo[r][i], src + i * 4 * KP);
-                        load_piece<KP>(hi[r][i], src + D + i * 4 * KP);
+                        for (int w = 0; w < KW; ++w) lo[m][r][i][w] = hi[m][r][i][w] = 0;
+                        if (unit[m][r] >= 0) {
+                            load_piece<KP>(lo[m][r][i], src + i * 4 * KP);
+                            load_piece<KP>(hi[m][r][i], src + D + i * 4 * KP);
+                        }
+                    }
+                    scale[m][r] = unit[m][r] >= 0 ? ld_global_half(p.scale + at) : __ushort_as_half(0);
+                }
+            look_up(tile + TILES * WARPS * 16);
+#pragma unroll
+            for (int m = 0; m < TILES; ++m) {
+                int32_t c[4] = {}, c2[4] = {};
+#pragma unroll
+                for (int k = 0; k < MMAS; ++k) {
+                    const int w = 2 * k, i = w / KW, s = w - i * KW;
+                    mma_s8(c, lo[m][0][i][s], lo[m][1][i][s], lo[m][0][i][s + 1], lo[m][1][i][s + 1], minus[k][0], minus[k][1]);
+                    mma_s8(c2, hi[m][0][i][s], hi[m][1][i][s], hi[m][0][i][s + 1], hi[m][1][i][s + 1], plus[k][0], plus[k][1]);
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float f = __half2float(scale[m][r]);
+                    uint32_t key = 0;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float score = __fmul_rn((float)(c[2 * r + x] + c2[2 * r + x]), qs[x] * f);
+                        if (qs[x] == qs[x]) key = max(key, ordered(score));
+                    }
+                    key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
+                    key = max(key, __shfl_xor_sync(0xffffffffu, key, 2));
+                    if (!is_finite(scale[m][r])) key = 0xffffffffu;
+                    key = unit[m][r] >= 0 ? max(key, 1u) : 0u; // holes come behind everything that is there
+                    const int32_t x = tile + m * WARPS * 16 + g + 8 * r;
+                    if (t == 0 && x < mine) {
+                        if (head0 > 0) key = max(key, keys[x]);
+                        keys[x] = key;
+                        if (units) units[x] = unit[m][r];
+                        if (ends) lowest = min(lowest, key), highest = max(highest, key);
                     }
                 }
-                scale[r] = there[r] ? ld_global_half(p.scale + at) : __ushort_as_half(0);
-            }
-            look_up(tile + SWARPS * 16);
-            int32_t c[4] = {}, c2[4] = {};
-#pragma unroll
-            for (int m = 0; m < MMAS; ++m) {
-                constexpr int W = KW;
-                const int w = 2 * m, i = w / W, s = w - i * W;
-                mma_s8(c, lo[0][i][s], lo[1][i][s], lo[0][i][s + 1], lo[1][i][s + 1], minus[m][0], minus[m][1]);
-                mma_s8(c2, hi[0][i][s], hi[1][i][s], hi[0][i][s + 1], hi[1][i][s + 1], plus[m][0], plus[m][1]);
-            }
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const float f = __half2float(scale[r]);
-                uint32_t key = 0;
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const float score = __fmul_rn((float)(c[2 * r + x] + c2[2 * r + x]), qs[x] * f);
-                    if (qs[x] == qs[x]) key = max(key, ordered(score));
-                }
-                key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
-                key = max(key, __shfl_xor_sync(0xffffffffu, key, 2));
-                if (!is_finite(scale[r])) key = 0xffffffffu;
-                if (!there[r]) key = 0;
-                // a score that is there is 1 at least, so that holes come behind it
-                if (there[r]) key = max(key, 1u);
-                const int32_t x = tile + g + 8 * r;
-                if (t == 0 && x < mine) keys[x] = head0 == 0 ? key : max(keys[x], key);
             }
         }
-        __syncthreads();
     }
 
     // ---- the threshold ---------------------------------------------------------------------------------------------------------
@@ -404,30 +439,29 @@ __global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_consta
         else __syncthreads();
     };
     const uint32_t bins0 = map_to_cta(ptx::smem_addr(histogram), 0), range0 = map_to_cta(ptx::smem_addr(range), 0), taken0 = map_to_cta(ptx::smem_addr(taken), 0);
+    lowest = __reduce_min_sync(0xffffffffu, lowest);
+    highest = __reduce_max_sync(0xffffffffu, highest);
     sync(); // the first CTA's histogram and range are there
-    {
-        uint32_t least = 0xffffffffu, most = 0;
-        for (int32_t x = threadIdx.x; x < mine; x += STPB) least = min(least, keys[x]), most = max(most, keys[x]);
-        least = __reduce_min_sync(0xffffffffu, least);
-        most = __reduce_max_sync(0xffffffffu, most);
-        if (lane == 0 && least <= most) min_in_cluster(range0, least), max_in_cluster(range0 + 4, most);
-    }
+    if (lane == 0 && lowest <= highest) min_in_cluster(range0, lowest), max_in_cluster(range0 + 4, highest);
     sync();
     uint32_t least = ld_in_cluster(range0), most = ld_in_cluster(range0 + 4), room = p.top, all = 0; // of the scores in [least, most], `room` are taken
     for (;;) {
         const uint32_t shift = max(0, 21 - __clz((int)(most - least))); // 2048 bins at most
-        for (int32_t x = threadIdx.x; x < mine; x += STPB)
+        for (int32_t x = threadIdx.x; x < mine; x += TPB)
             if (keys[x] >= least && keys[x] <= most) add_in_cluster(bins0 + ((keys[x] - least) >> shift) * 4, 1);
         sync();
         if (rank == 0) {
-            // bins from the highest down: thread x has those from BINS - 8 x - 1 on
-            uint4* const here = reinterpret_cast<uint4*>(histogram + BINS - 8 - 8 * threadIdx.x);
-            const uint4 low = here[0], high = here[1];
-            here[0] = here[1] = make_uint4(0, 0, 0, 0);
-            const uint32_t n8[8] = {high.w, high.z, high.y, high.x, low.w, low.z, low.y, low.x};
-            uint32_t own = 0;
+            // bins from the highest down: thread x has EACH of them, from BINS - EACH x - 1 on
+            constexpr int EACH = BINS / TPB;
+            uint32_t n_of[EACH], own = 0;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) own += n8[k];
+            for (int k = 0; k < EACH; k += 4) {
+                uint4* const here = reinterpret_cast<uint4*>(histogram + BINS - EACH * threadIdx.x - 4 - k);
+                const uint4 v = *here;
+                *here = make_uint4(0, 0, 0, 0);
+                n_of[k] = v.w; n_of[k + 1] = v.z; n_of[k + 2] = v.y; n_of[k + 3] = v.x;
+                own += v.x + v.y + v.z + v.w;
+            }
             uint32_t sum = own;
 #pragma unroll
             for (int m = 1; m < 32; m <<= 1) {
@@ -440,16 +474,16 @@ __global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_consta
             uint32_t over = sum - own;
             if (over < room && sum >= room) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    if (over < room && over + n8[k] >= room) {
-                        const uint32_t bin = BINS - 1 - 8 * threadIdx.x - k;
+                for (int k = 0; k < EACH; ++k) {
+                    if (over < room && over + n_of[k] >= room) {
+                        const uint32_t bin = BINS - 1 - EACH * threadIdx.x - k;
                         const uint32_t first = least + (bin << shift), width = (1u << shift) - 1;
                         range[0] = first;
                         range[1] = most - first < width ? most : first + width;
                         taken[0] = room - over;
-                        taken[1] = n8[k] == room - over;
+                        taken[1] = n_of[k] == room - over;
                     }
-                    over += n8[k];
+                    over += n_of[k];
                 }
             }
         }
@@ -464,37 +498,43 @@ __global__ void __launch_bounds__(STPB) choose_blocks_kernel(const __grid_consta
     // ---- what is above the threshold, and the first `room` of those at it, in order ------------------------------------------------
     auto over_it = [&](uint32_t key) { return all ? key >= least : key > least; };
     auto at_it = [&](uint32_t key) { return !all && key == least; };
-    uint32_t counts[2] = {};
-    for (int32_t x = threadIdx.x; x < mine; x += STPB) {
-        counts[0] += over_it(keys[x]);
-        counts[1] += at_it(keys[x]);
-    }
-    counts[0] = __reduce_add_sync(0xffffffffu, counts[0]);
-    counts[1] = __reduce_add_sync(0xffffffffu, counts[1]);
-    if (lane == 0) atomicAdd(&above, counts[0]), atomicAdd(&at_threshold, counts[1]);
-    sync();
     uint32_t before[2] = {};
-    for (int32_t r = 0; r < rank; ++r) {
-        before[0] += ld_in_cluster(map_to_cta(ptx::smem_addr(&above), r));
-        before[1] += ld_in_cluster(map_to_cta(ptx::smem_addr(&at_threshold), r));
+    if (ctas > 1) { // those of the CTAs before this one
+        uint32_t counts[2] = {};
+        for (int32_t x = threadIdx.x; x < mine; x += TPB) {
+            counts[0] += over_it(keys[x]);
+            counts[1] += at_it(keys[x]);
+        }
+        counts[0] = __reduce_add_sync(0xffffffffu, counts[0]);
+        counts[1] = __reduce_add_sync(0xffffffffu, counts[1]);
+        if (lane == 0) atomicAdd(&above, counts[0]), atomicAdd(&at_threshold, counts[1]);
+        cluster_sync_all();
+        for (int32_t r = 0; r < rank; ++r) {
+            before[0] += ld_in_cluster(map_to_cta(ptx::smem_addr(&above), r));
+            before[1] += ld_in_cluster(map_to_cta(ptx::smem_addr(&at_threshold), r));
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); // nothing of another CTA's is read any more
     }
-    for (int32_t x0 = 0; x0 < mine; x0 += STPB) {
-        const int32_t x = x0 + threadIdx.x;
+    for (int32_t x0 = 0; x0 < mine; x0 += TPB) {
+        const int32_t x = x0 + threadIdx.x, block = p.first + begin + x;
         const uint32_t key = x < mine ? keys[x] : 0u;
         const bool over = x < mine && over_it(key), same = x < mine && at_it(key);
+        int32_t unit = -1;
+        if (over || same) unit = units ? units[x] : unit_of(block, row_pages[page_index(block)]);
         const uint32_t overs = __ballot_sync(0xffffffffu, over), sames = __ballot_sync(0xffffffffu, same), below = (1u << lane) - 1;
         if (lane == 0) scan[warp][0] = __popc(overs), scan[warp][1] = __popc(sames);
         __syncthreads();
         uint32_t o = before[0] + __popc(overs & below), s = before[1] + __popc(sames & below);
-        for (int w = 0; w < SWARPS; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             if (w < warp) o += scan[w][0], s += scan[w][1];
             before[0] += scan[w][0];
             before[1] += scan[w][1];
         }
-        if (over || (same && s < room)) put(p.first + o + min(s, room), p.first + begin + x);
+        if (over || (same && s < room)) put(p.first + o + min(s, room), block, unit);
         __syncthreads();
     }
-    sync(); // no CTA leaves while another reads its shared memory
+    put_kept();
+    if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); // no CTA leaves while another reads its shared memory
 }
 
 int32_t check_bounds(const pplb200_kv_cache* c, const pplb200_key_bounds* k) {
@@ -514,12 +554,19 @@ int32_t check_bounds(const pplb200_kv_cache* c, const pplb200_key_bounds* k) {
 int64_t list_bytes(int64_t batch, int32_t kv_heads, int64_t total) { return round_up(batch * kv_heads * total * 4, 256) + round_up(batch * 4, 256); }
 
 template <int D>
+void launch_bounds_of(cudaStream_t stream, const BoundsParams& p, dim3 grid) {
+    if (p.cache.quant_group == 0) launch_ex(key_bounds_kernel<D, CACHE_F16>, grid, dim3(BTPB), stream, true, p);
+    else if (p.cache.quant_group == 8) launch_ex(key_bounds_kernel<D, CACHE_I8_GROUPS>, grid, dim3(BTPB), stream, true, p);
+    else launch_ex(key_bounds_kernel<D, CACHE_I8_ROWS>, grid, dim3(BTPB), stream, true, p);
+}
+
+template <int D, int WARPS>
 int32_t launch_choice(cudaStream_t stream, const ChoiceParams& p, int32_t cluster) {
     const int64_t y = std::min<int64_t>(p.items, 32768);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)cluster, (unsigned)y, (unsigned)((p.items + y - 1) / y));
-    cfg.blockDim = dim3(STPB);
-    cfg.dynamicSmemBytes = (size_t)p.share * 4;
+    cfg.blockDim = dim3(32 * WARPS);
+    cfg.dynamicSmemBytes = (size_t)p.share * (p.units_kept ? 8 : 4);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -529,11 +576,11 @@ int32_t launch_choice(cudaStream_t stream, const ChoiceParams& p, int32_t cluste
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    if (cfg.dynamicSmemBytes > 32768) { // beyond what a kernel has without being asked for, its static 7 KB included
-        const cudaError_t e = cudaFuncSetAttribute(choose_blocks_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+    if (cfg.dynamicSmemBytes > 32768) { // beyond what a kernel has without being asked for, its static 11 KB included
+        const cudaError_t e = cudaFuncSetAttribute(choose_blocks_kernel<D, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
         if (e != cudaSuccess) return fail(RC_DEVICE_RUNTIME_ERROR, "choice of blocks: %s", cudaGetErrorString(e));
     }
-    cudaLaunchKernelEx(&cfg, choose_blocks_kernel<D>, p);
+    cudaLaunchKernelEx(&cfg, choose_blocks_kernel<D, WARPS>, p);
     return check_launch("choice of blocks");
 }
 
@@ -558,12 +605,14 @@ int32_t pplb200_key_bounds_update(pplb200_stream_t stream, const pplb200_kv_cach
     p.slots = slots; p.tokens = tokens;
     p.block = bounds->block; p.per_page = cache->page_size / bounds->block;
     small_division(p.block, p.block_magic, p.block_shift);
-    // one slot a CTA while that makes no more than eight CTAs an SM, then as many as a block has, so that a prompt's CTA has one block
-    p.slots_here = (int32_t)std::min<int64_t>(std::min(p.block, BTPB), std::max<int64_t>(1, tokens * cache->kv_heads / (8 * kSms)));
-    const dim3 grid((unsigned)((tokens + p.slots_here - 1) / p.slots_here), (unsigned)cache->kv_heads);
-    if (cache->quant_group == 0) launch_ex(key_bounds_kernel<CACHE_F16>, grid, dim3(BTPB), (cudaStream_t)stream, true, p);
-    else if (cache->quant_group == 8) launch_ex(key_bounds_kernel<CACHE_I8_GROUPS>, grid, dim3(BTPB), (cudaStream_t)stream, true, p);
-    else launch_ex(key_bounds_kernel<CACHE_I8_ROWS>, grid, dim3(BTPB), (cudaStream_t)stream, true, p);
+    // one slot a CTA while that makes no more than eight CTAs an SM, then up to as many as a block has, so that a prompt's CTA has one block
+    const int64_t heads = (cache->kv_heads + BWARPS - 1) / BWARPS;
+    p.slots_here = (int32_t)std::min<int64_t>(std::min(p.block, BTPB), std::max<int64_t>(1, tokens * heads / (8 * kSms)));
+    const dim3 grid((unsigned)((tokens + p.slots_here - 1) / p.slots_here), (unsigned)heads);
+    if (cache->head_dim == 64) launch_bounds_of<64>((cudaStream_t)stream, p, grid);
+    else if (cache->head_dim == 96) launch_bounds_of<96>((cudaStream_t)stream, p, grid);
+    else if (cache->head_dim == 128) launch_bounds_of<128>((cudaStream_t)stream, p, grid);
+    else launch_bounds_of<256>((cudaStream_t)stream, p, grid);
     return check_launch("key bounds");
 }
 
@@ -625,15 +674,22 @@ int32_t pplb200_block_sparse_attention_fp16(pplb200_stream_t stream, const pplb2
     p.first = choice->first; p.last = choice->last; p.top = choice->top; p.total = (int32_t)total;
     small_division(p.block, p.block_magic, p.block_shift);
     small_division(p.per_page, p.page_magic, p.page_shift);
-    // CTAs of a choice: two on an SM, a round of 16 blocks a warp for each, and no more than 128 KB of scores
+    // Sixteen warps a CTA where there are few choices, which then take 512 blocks in one round of loads; four for many or short ones, so that several share
+    // an SM.  Clusters, whose barriers cost a microsecond each, only where a CTA would have more rounds to go, and for room for the scores (128 KB).
+    const bool wide = p.items <= kSms && in_table > 128;
     int32_t cluster = 1;
-    while (cluster < MAX_CLUSTER && ((p.items * cluster * 2 <= 2 * kSms && in_table > cluster * SWARPS * 16) || in_table > cluster * 32768LL)) cluster *= 2;
+    while (cluster < MAX_CLUSTER && ((p.items * cluster * 2 <= kSms && in_table > cluster * 512) || in_table > cluster * 32768LL)) cluster *= 2;
     p.share = (int32_t)std::max<int64_t>(16, (in_table + cluster * 16 - 1) / (cluster * 16) * 16);
+    p.units_kept = p.share <= 16384;
     const cudaStream_t s = (cudaStream_t)stream;
-    if (cache->head_dim == 64) rc = launch_choice<64>(s, p, cluster);
-    else if (cache->head_dim == 96) rc = launch_choice<96>(s, p, cluster);
-    else if (cache->head_dim == 128) rc = launch_choice<128>(s, p, cluster);
-    else rc = launch_choice<256>(s, p, cluster);
+    const auto launch_dims = [&](auto warps) {
+        constexpr int W = decltype(warps)::value;
+        if (cache->head_dim == 64) return launch_choice<64, W>(s, p, cluster);
+        if (cache->head_dim == 96) return launch_choice<96, W>(s, p, cluster);
+        if (cache->head_dim == 128) return launch_choice<128, W>(s, p, cluster);
+        return launch_choice<256, W>(s, p, cluster);
+    };
+    rc = wide ? launch_dims(std::integral_constant<int, 16>()) : launch_dims(std::integral_constant<int, 4>());
     if (rc != RC_SUCCESS) return rc;
     own.pages = lists;
     own.pages_stride = cache->kv_heads * total;

@@ -88,7 +88,10 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
     __shared__ uint32_t tmem_slot;
     __shared__ uint32_t masks[T::INFOS][4];
     __shared__ float sizes[T::INFOS][4];
-    __shared__ int64_t row_at[2][T::NB], scale_at[2][T::KIND == CACHE_F16 ? 1 : T::NB];
+    struct __align__(16) Row {
+        int64_t at, scale; // in bytes; at < 0: not there
+    };
+    __shared__ Row row_at[2][T::NB];
     __shared__ float2 joint[128];
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t smem = (ptx::smem_addr(raw_smem) + 1023u) & ~1023u;
@@ -119,7 +122,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
     const int32_t per_head = p.items / p.cache.kv_heads, kvh = item / per_head;
     const int32_t row0 = (item - kvh * per_head) * p.tiles * 128;
     const int32_t tiles = p.tiles == 2 && p.rows - row0 > 128 ? 2 : 1;
-    const int32_t n = (int32_t)min((int64_t)max(*(const volatile int32_t*)p.length, 0), p.tokens_in_table);
+    const int32_t n = p.num_pages > 0 ? (int32_t)min((int64_t)max(*(const volatile int32_t*)p.length, 0), p.tokens_in_table) : 0;
     const int32_t all_blocks = (n + T::NB - 1) / T::NB;
     const int32_t block0 = (int32_t)((int64_t)all_blocks * split / p.splits), blocks = (int32_t)((int64_t)all_blocks * (split + 1) / p.splits) - block0;
     const int32_t tasks = tiles * blocks; // task i: buffer i & 1, block i / tiles; with two streams also stream i & 1
@@ -188,10 +191,9 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
             const int32_t token = (block0 + j) * T::NB + id;
             there = j < blocks && (uint32_t)page < (uint32_t)p.num_pages;
             const int32_t in_page = token - (int32_t)((uint32_t)((uint64_t)(uint32_t)token * p.page_magic >> p.page_shift)) * p.cache.page_size;
-            if (id < T::NB) row_at[j & 1][id] = there ? kv_row(page, in_page, 0, p.cache.page_stride, 0, p.cache.token_stride) * T::ES : -1;
+            const int64_t scale_row = T::KIND != CACHE_F16 && there ? kv_row(page, in_page, 0, p.cache.scale_page_stride, 0, p.cache.scale_token_stride) * 2 : 0;
+            if (id < T::NB) row_at[j & 1][id] = {there ? kv_row(page, in_page, 0, p.cache.page_stride, 0, p.cache.token_stride) * T::ES : -1, scale_row};
             if constexpr (T::KIND != CACHE_F16) {
-                const int64_t scale_row = there ? kv_row(page, in_page, 0, p.cache.scale_page_stride, 0, p.cache.scale_token_stride) * 2 : 0;
-                if (id < T::NB) scale_at[j & 1][id] = scale_row;
                 if constexpr (T::KIND == CACHE_I8_ROWS) {
                     k_scale = there ? __half2float(__ushort_as_half((unsigned short)load_scales<1>(ksbase + scale_row))) : 0.0f;
                     v_scale = there ? __half2float(__ushort_as_half((unsigned short)load_scales<1>(vsbase + scale_row))) : 0.0f;
@@ -297,7 +299,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                     ptx::named_barrier(1, 128);
                     int64_t at[T::LOADS];
 #pragma unroll
-                    for (int i = 0; i < T::LOADS; ++i) at[i] = row_at[j & 1][token_of(i)];
+                    for (int i = 0; i < T::LOADS; ++i) at[i] = row_at[j & 1][token_of(i)].at;
 #pragma unroll
                     for (int values = 0; values < 2; ++values) {
                         const int stages = values ? T::VS : T::KS, stage = j % stages;
@@ -325,22 +327,26 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
         } else {
             // a block's pieces are requested when the block before has been put into its place
             uint4 kw[T::LOADS], vw[T::LOADS];
-            uint32_t ks[T::LOADS], vs[T::LOADS];
-            auto fetch = [&](int32_t j, uint4 (&w)[T::LOADS], uint32_t (&s)[T::LOADS], const char* base, const char* sbase) {
+            uint32_t ks[T::LOADS], vs[T::LOADS], k_there = 0, v_there = 0; // a bit a piece; what is not there is read from the cache's first row, and is nothing
+            auto fetch = [&](int32_t j, uint4 (&w)[T::LOADS], uint32_t (&s)[T::LOADS], uint32_t& there_bits, const char* base, const char* sbase) {
+                there_bits = 0;
 #pragma unroll
                 for (int i = 0; i < T::LOADS; ++i) {
                     const int token = token_of(i), c = piece_of(i);
-                    const int64_t at = row_at[j & 1][token];
-                    w[i] = at >= 0 ? ld_global_16(base + at + c * 16) : make_uint4(0, 0, 0, 0);
-                    if constexpr (T::KIND == CACHE_I8_GROUPS) s[i] = at >= 0 ? load_scales<2>(sbase + scale_at[j & 1][token] + c * 4) : 0u;
+                    const Row row = row_at[j & 1][token];
+                    w[i] = ld_global_16(base + (row.at < 0 ? 0 : row.at) + c * 16);
+                    if constexpr (T::KIND == CACHE_I8_GROUPS) s[i] = load_scales<2>(sbase + row.scale + c * 4);
+                    there_bits |= (row.at < 0 ? 0u : 1u) << i;
                 }
             };
-            auto put = [&](uint32_t dst, const uint4 (&w)[T::LOADS], const uint32_t (&s)[T::LOADS], bool keys) {
+            auto put = [&](uint32_t dst, const uint4 (&w)[T::LOADS], const uint32_t (&scales)[T::LOADS], uint32_t there_bits, bool keys) {
 #pragma unroll
                 for (int i = 0; i < T::LOADS; ++i) {
                     const int token = token_of(i), c = 2 * piece_of(i);
-                    uint32_t o[8], r[8] = {};
-                    whole_numbers(w[i], o);
+                    uint32_t o[8], r[8] = {}, s[T::LOADS] = {};
+                    const uint32_t all = 0u - (there_bits >> i & 1);
+                    whole_numbers(make_uint4(w[i].x & all, w[i].y & all, w[i].z & all, w[i].w & all), o);
+                    if constexpr (T::KIND == CACHE_I8_GROUPS) s[i] = scales[i] & all;
                     if constexpr (T::KIND == CACHE_I8_GROUPS) {
 #pragma unroll
                         for (int x = 0; x < 8; ++x) {
@@ -365,8 +371,8 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                 locate(0);
                 request(1);
                 ptx::named_barrier(1, 128);
-                fetch(0, kw, ks, kbase, ksbase);
-                fetch(0, vw, vs, vbase, vsbase);
+                fetch(0, kw, ks, k_there, kbase, ksbase);
+                fetch(0, vw, vs, v_there, vbase, vsbase);
                 publish(0);
             }
             for (int32_t j = 0; j < blocks; ++j) {
@@ -377,19 +383,19 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                 // (after a wait that ran out nothing is stored any more, but every thread comes to every barrier and ballot)
                 ok = ok && ptx::mbar_wait(bar(empty_k[kstage]), ((j / T::KS) & 1) ^ 1, &g_status, ST_LOAD);
                 if (ok) {
-                    put(smem + T::RING + kstage * T::K_BYTES, kw, ks, true);
+                    put(smem + T::RING + kstage * T::K_BYTES, kw, ks, k_there, true);
                     ptx::mbar_arrive(bar(full_k[kstage]));
                 }
                 if (j + 1 < blocks) {
-                    fetch(j + 1, kw, ks, kbase, ksbase);
+                    fetch(j + 1, kw, ks, k_there, kbase, ksbase);
                     publish(j + 1);
                 }
                 ok = ok && ptx::mbar_wait(bar(empty_v[vstage]), ((j / T::VS) & 1) ^ 1, &g_status, ST_LOAD);
                 if (ok) {
-                    put(smem + T::V_RING + vstage * T::V_BYTES, vw, vs, false);
+                    put(smem + T::V_RING + vstage * T::V_BYTES, vw, vs, v_there, false);
                     ptx::mbar_arrive(bar(full_v[vstage]));
                 }
-                if (j + 1 < blocks) fetch(j + 1, vw, vs, vbase, vsbase);
+                if (j + 1 < blocks) fetch(j + 1, vw, vs, v_there, vbase, vsbase);
             }
         }
     } else {
