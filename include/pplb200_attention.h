@@ -175,8 +175,8 @@ int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb2
  * above over the prefix's tokens and sequence b's own, of which `lengths` counts and `pages` lists only the latter.  The prefix is read once for the
  * batch.  prefix->pages int32 [prefix->num_pages], prefix->length int32 [1], both on the device: how many tokens (at most num_pages * page_size are
  * looked at); pages that are not in the cache are holes.  A sequence with a length of 0 sees the prefix alone; a negative length stands for a row that is
- * no sequence: zeros and -inf, whatever its q.  As above otherwise, but window has to be 0, at most 2^24 rows of q (batch * q_heads), and: over the prefix
- * the softmax's weights enter their product with v with 11 bits, and v of int8 rows and groups as there, where batch * q_heads / kv_heads passes 16 (8 for heads of 256).
+ * no sequence: zeros and -inf, whatever its q.  As above otherwise, but window has to be 0, at most 2^24 rows of q (batch * q_heads), and where batch * q_heads / kv_heads
+ * passes 16 (8 for heads of 256): over the prefix the softmax's weights enter their product with v with 11 bits, and v of int8 rows is rounded to fp16 as that of groups is.
  * ws: pplb200_shared_prefix_attention_workspace_bytes(), with the rules above.
  */
 typedef struct pplb200_shared_prefix {

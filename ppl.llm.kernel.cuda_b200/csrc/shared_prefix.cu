@@ -55,7 +55,7 @@ bool make_page_map(CUtensorMap* map, const pplb200_kv_cache& c, const void* base
 template <int D, int KIND>
 int32_t launch_tiles(cudaStream_t stream, PrefixParams& p) {
     using T = Tile<D, KIND>;
-    static_assert(T::SMEM + 8192 <= 232448);
+    static_assert(T::SMEM + 18 * 1024 <= 232448);
     p.tiles = tiles_at_once(p.rows, T::TILES);
     p.items = p.cache.kv_heads * (int32_t)((p.rows + p.tiles * 128 - 1) / (p.tiles * 128));
     const int64_t blocks = std::max<int64_t>(1, (p.tokens_in_table + T::NB - 1) / T::NB);

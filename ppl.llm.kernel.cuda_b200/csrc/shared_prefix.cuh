@@ -5,8 +5,9 @@
 // prefix in blocks of NB tokens; its sums and reference exponents are left as one of `splits` parts, which are joined where the output is written.
 //
 //   warps 0 - 3, 4 - 7   softmax of one tile each, a thread a row (tensor memory's lanes): scores in, weights of 11 bits out, in place
-//   warps 8 - 11         keys and values from the pages into shared memory; int8 ones are widened on the way
-//   warp 12              issues all products, and owns the tensor memory
+//   warps 8 - 11         keys from the pages into shared memory; int8 ones are widened on the way
+//   warps 12 - 15        values
+//   warp 16              issues all products, and owns the tensor memory
 //
 // The two tiles' products and softmaxes alternate, so that the tensor cores work on one while the exponentials of the other are computed.  Where a CTA has one
 // tile only, the two softmax groups take turns at the blocks of it, each with a sum of its own (heads of 256: one group, whose sum alone fills
@@ -17,12 +18,16 @@
 #include "paged_attention.cuh"
 #include "ptx.cuh"
 
+#include <type_traits>
+
 namespace pplb200 {
 namespace prefix {
 
 using namespace paged;
 
 __device__ unsigned int g_status = 0;
+__device__ uint4 g_nothing[32]; // zeros: what a token that is not there reads
+constexpr float kAbove = 4.0f;
 constexpr unsigned ST_LOAD = 1u, ST_MMA = 2u, ST_SOFTMAX = 4u;
 
 template <int D_, int KIND_>
@@ -37,7 +42,7 @@ struct Tile {
     static constexpr int Q_BYTES = 128 * DP * 2, V_BYTES = NB * DP * 2, K_BYTES = V_BYTES * (LOW ? 2 : 1);
     static constexpr int RING = TILES * Q_BYTES, V_RING = RING + KS * K_BYTES, INFO = V_RING + VS * V_BYTES;
     static constexpr int INFOS = 8; // blocks whose masks and scales are kept: more than stages of values
-    static constexpr int SCALES = KIND == CACHE_I8_ROWS ? INFOS * NB * 8 : 0;
+    static constexpr int SCALES = KIND == CACHE_I8_ROWS ? INFOS * NB * 2 : 0; // of keys
     // What is read back of the sums lies over the rings and q, behind the sums that the two groups of one tile exchange (tiles' sums and these are not there at
     // the same time, and one tile's are half as long).
     static constexpr int STAGED_BYTES = STREAMS * 128 * (D + 4) * 4, EXCHANGE = STREAMS == 2 ? D * 512 : 0, ONE_TILE = EXCHANGE + 128 * (D + 4) * 4;
@@ -45,7 +50,11 @@ struct Tile {
     static constexpr int SMEM = (BODY > LEAST ? BODY : LEAST) + 1024; // the base is rounded up to 1024
     static constexpr int CH = D * ES / 16, LOADS = CH * NB / 128; // pieces of 16 bytes: of a row, and of a block for a thread
     static_assert(CH * NB % 128 == 0 && VS < INFOS);
-    static constexpr int THREADS = 512;
+    static constexpr int THREADS = 640;
+    // Registers of softmax, loading and issuing threads: what 640 threads are launched with, 96 each.
+    static constexpr int R_SOFTMAX = KIND == CACHE_F16 ? 176 : 152, R_LOAD = KIND == CACHE_F16 ? 48 : 72, R_ISSUE = 32;
+    static constexpr int KEPT = KIND == CACHE_F16 ? NB : NB / 2; // scores of a row that a softmax thread keeps
+    static_assert(2 * R_SOFTMAX + 2 * R_LOAD + R_ISSUE <= 5 * 96);
     static constexpr uint32_t O_COLUMN = 256; // scores: columns 0 and 128
 };
 
@@ -86,28 +95,31 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
     extern __shared__ uint8_t raw_smem[];
     __shared__ __align__(8) uint64_t full_k[T::KS], empty_k[T::KS], full_v[T::VS], empty_v[T::VS], info_full[T::INFOS], score_full[2], weight_half[2], weight_full[2], sum_done[2], q_full, all_done, tail_full;
     __shared__ uint32_t tmem_slot;
-    __shared__ uint32_t masks[T::INFOS][4];
-    __shared__ float sizes[T::INFOS][4];
-    struct __align__(16) Row {
-        int64_t at, scale; // in bytes; at < 0: not there
+    __shared__ __align__(16) uint32_t masks[T::INFOS][4]; // (blocks of 64 tokens: two, and two that say that all is there)
+    struct __align__(16) Row { // where a token's row and its scales begin
+        const char *at, *scale;
     };
-    __shared__ Row row_at[2][T::NB];
+    __shared__ Row row_at[2][4][T::NB]; // keys and values, of four blocks
     __shared__ float2 joint[128];
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t smem = (ptx::smem_addr(raw_smem) + 1023u) & ~1023u;
     auto bar = [](uint64_t& b) { return ptx::smem_addr(&b); };
+    auto report = [&](uint32_t b) { // a warp's threads have done their part: one arrival
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(b);
+    };
     const bool boxes = T::KIND == CACHE_F16 && p.box_rows > 0; // whole boxes by the TMA unit: one thread reports
     if (threadIdx.x == 0) {
-        for (int i = 0; i < T::KS; ++i) ptx::mbar_init(bar(full_k[i]), boxes ? 1 : 128), ptx::mbar_init(bar(empty_k[i]), 1);
-        for (int i = 0; i < T::VS; ++i) ptx::mbar_init(bar(full_v[i]), boxes ? 1 : 128), ptx::mbar_init(bar(empty_v[i]), 1);
-        for (int i = 0; i < T::INFOS; ++i) ptx::mbar_init(bar(info_full[i]), boxes ? 1 : 128);
+        for (int i = 0; i < T::KS; ++i) ptx::mbar_init(bar(full_k[i]), boxes ? 1 : 4), ptx::mbar_init(bar(empty_k[i]), 1);
+        for (int i = 0; i < T::VS; ++i) ptx::mbar_init(bar(full_v[i]), boxes ? 1 : 4), ptx::mbar_init(bar(empty_v[i]), 1);
+        for (int i = 0; i < T::INFOS; ++i) ptx::mbar_init(bar(info_full[i]), boxes ? 1 : 4);
         ptx::mbar_init(bar(tail_full), 1);
-        for (int i = 0; i < 2; ++i) ptx::mbar_init(bar(score_full[i]), 1), ptx::mbar_init(bar(weight_half[i]), 128), ptx::mbar_init(bar(weight_full[i]), 128), ptx::mbar_init(bar(sum_done[i]), 1);
-        ptx::mbar_init(bar(q_full), 256);
+        for (int i = 0; i < 2; ++i) ptx::mbar_init(bar(score_full[i]), 1), ptx::mbar_init(bar(weight_half[i]), 4), ptx::mbar_init(bar(weight_full[i]), 4), ptx::mbar_init(bar(sum_done[i]), 1);
+        ptx::mbar_init(bar(q_full), 8);
         ptx::mbar_init(bar(all_done), 1);
         ptx::fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == 16) {
         ptx::tmem_alloc(ptx::smem_addr(&tmem_slot), 512);
         ptx::tmem_relinquish();
     }
@@ -128,9 +140,9 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
     const int32_t tasks = tiles * blocks; // task i: buffer i & 1, block i / tiles; with two streams also stream i & 1
     const int32_t shift = tiles - 1;
 
-    if (warp >= 12) {
-        ptx::registers_down<40>();
-        if (warp == 12 && tasks > 0) {
+    if (warp >= 16) {
+        ptx::registers_down<T::R_ISSUE>();
+        if (warp == 16 && tasks > 0) {
             // ---- products, by one lane of a warp that does the same in all -------------------------------------------------------------------------------------------------
             constexpr uint32_t QK = ptx::make_f16_idesc(128, T::NB, false), PV = ptx::make_f16_idesc(128, T::D, true);
             const uint32_t leads = ptx::elect_one();
@@ -173,15 +185,21 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
             ptx::mma_commit_by(bar(all_done), leads); // all that was issued
         }
     } else if (warp >= 8) {
-        ptx::registers_down<120>();
+        ptx::registers_down<T::R_LOAD>();
         // ---- keys and values ---------------------------------------------------------------------------------------------------
-        const int id = threadIdx.x - 256;
-        const char *const kbase = (const char*)p.cache.k + (int64_t)kvh * p.cache.head_stride * T::ES, *const vbase = (const char*)p.cache.v + (int64_t)kvh * p.cache.head_stride * T::ES;
-        const char *const ksbase = (const char*)p.cache.k_scale + (int64_t)kvh * p.cache.scale_head_stride * 2, *const vsbase = (const char*)p.cache.v_scale + (int64_t)kvh * p.cache.scale_head_stride * 2;
-        // Where a block's tokens lie, which of them are there, and (rows) their scales: thread id looks after token id, its page one block ahead.
+        const int id = threadIdx.x & 127;
+        const bool values = warp >= 12;
+        const int stages = values ? T::VS : T::KS, stage_bytes = values ? T::V_BYTES : T::K_BYTES;
+        const uint32_t ring = smem + (values ? T::V_RING : T::RING);
+        const char* const base = (const char*)(values ? p.cache.v : p.cache.k) + (int64_t)kvh * p.cache.head_stride * T::ES;
+        const char* const sbase = (const char*)(values ? p.cache.v_scale : p.cache.k_scale) + (int64_t)kvh * p.cache.scale_head_stride * 2;
+        auto full = [&](int stage) { return values ? bar(full_v[stage]) : bar(full_k[stage]); };
+        auto empty = [&](int stage) { return values ? bar(empty_v[stage]) : bar(empty_k[stage]); };
+        // Where a block's tokens lie, which of them are there, and (rows) the keys' scales: thread id looks after token id, its page three blocks ahead, its row
+        // two, and what the softmax has to know is published one ahead.
         int32_t page = -1;
         bool there = false;
-        float k_scale = 0.0f, v_scale = 0.0f;
+        uint32_t scale = 0; // fp16
         auto request = [&](int32_t j) {
             const int32_t token = (block0 + j) * T::NB + id;
             page = -1;
@@ -191,47 +209,56 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
             const int32_t token = (block0 + j) * T::NB + id;
             there = j < blocks && (uint32_t)page < (uint32_t)p.num_pages;
             const int32_t in_page = token - (int32_t)((uint32_t)((uint64_t)(uint32_t)token * p.page_magic >> p.page_shift)) * p.cache.page_size;
-            const int64_t scale_row = T::KIND != CACHE_F16 && there ? kv_row(page, in_page, 0, p.cache.scale_page_stride, 0, p.cache.scale_token_stride) * 2 : 0;
-            if (id < T::NB) row_at[j & 1][id] = {there ? kv_row(page, in_page, 0, p.cache.page_stride, 0, p.cache.token_stride) * T::ES : -1, scale_row};
-            if constexpr (T::KIND != CACHE_F16) {
-                if constexpr (T::KIND == CACHE_I8_ROWS) {
-                    k_scale = there ? __half2float(__ushort_as_half((unsigned short)load_scales<1>(ksbase + scale_row))) : 0.0f;
-                    v_scale = there ? __half2float(__ushort_as_half((unsigned short)load_scales<1>(vsbase + scale_row))) : 0.0f;
-                }
+            Row to = {reinterpret_cast<const char*>(g_nothing), reinterpret_cast<const char*>(g_nothing)};
+            if (there) {
+                to.at = base + kv_row(page, in_page, 0, p.cache.page_stride, 0, p.cache.token_stride) * T::ES;
+                if constexpr (T::KIND != CACHE_F16) to.scale = sbase + kv_row(page, in_page, 0, p.cache.scale_page_stride, 0, p.cache.scale_token_stride) * 2;
             }
+            if (id < T::NB) row_at[values][j & 3][id] = to;
+            if constexpr (T::KIND == CACHE_I8_ROWS)
+                if (!values) scale = load_scales<1>(to.scale);
         };
-        auto publish = [&](int32_t j) {
+        auto publish = [&](int32_t j) { // to the softmax: by the keys' threads
             const int slot = j % T::INFOS;
             const uint32_t mask = __ballot_sync(0xffffffffu, there);
-            if (lane == 0) masks[slot][id >> 5] = mask;
-            if constexpr (T::KIND == CACHE_I8_ROWS) {
-                // a value's scale goes into its weight, its logarithm into what decides about the reference exponent, as far as a finite one could
-                float size = fminf(fmaxf(log2_fast(fabsf(v_scale)), -24.0f), 16.0f);
-#pragma unroll
-                for (int m = 16; m > 0; m >>= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, m));
-                if (lane == 0) sizes[slot][id >> 5] = size;
-                if (id < T::NB) {
-                    float* const scales = reinterpret_cast<float*>(raw_smem + (smem - ptx::smem_addr(raw_smem)) + T::INFO) + slot * T::NB * 2;
-                    scales[id] = k_scale * p.scale_log2;
-                    scales[T::NB + id] = v_scale;
-                }
-            }
-            ptx::mbar_arrive(bar(info_full[slot]));
+            if (values) return;
+            if (lane == 0) masks[slot][id >> 5] = id < T::NB ? mask : 0xffffffffu;
+            if constexpr (T::KIND == CACHE_I8_ROWS)
+                if (id < T::NB) reinterpret_cast<uint16_t*>(raw_smem + (smem - ptx::smem_addr(raw_smem)) + T::INFO)[slot * T::NB + id] = (uint16_t)scale;
+            report(bar(info_full[slot]));
         };
-        // piece i of this thread: of token (id + 128 i) / CH
-        auto token_of = [&](int i) { return (id + 128 * i) / T::CH; };
-        auto piece_of = [&](int i) { return (id + 128 * i) % T::CH; };
+        const int barrier_id = values ? 3 : 1;
+        // Blocks 0 and 1 are located before the first is loaded; then, with every block, the next one is published, the one behind it located and the third's
+        // pages requested.
+        auto begin = [&] {
+            request(0);
+            locate(0);
+            request(1);
+            publish(0);
+            locate(1);
+            request(2);
+            ptx::named_barrier(barrier_id, 128);
+        };
+        auto go_on = [&](int32_t j) {
+            if (j + 1 < blocks) publish(j + 1);
+            locate(j + 2);
+            request(j + 3);
+            ptx::named_barrier(barrier_id, 128);
+        };
+        // piece i of this thread: of which token, and which of its row (CH divides 128 but for heads of 96)
+        constexpr bool even = 128 % T::CH == 0;
+        const uint32_t id_token = (uint32_t)id / T::CH, id_piece = (uint32_t)id % T::CH;
+        auto token_of = [&](int i) { return even ? id_token + i * (128 / T::CH) : (uint32_t)(id + 128 * i) / T::CH; };
+        auto piece_of = [&](int i) { return even ? id_piece : (uint32_t)(id + 128 * i) % T::CH; };
         // where 16 bytes of fp16 (dimensions 8 c on) of a token lie in a tile
-        auto place = [](int token, int c) { return (uint32_t)((c >> 3) * (T::NB * 128) + token * 128 + (((c & 7) ^ (token & 7)) << 4)); };
+        auto place = [](uint32_t token, uint32_t c) { return (c >> 3) * (T::NB * 128) + token * 128 + (((c & 7) ^ (token & 7)) << 4); };
         bool ok = true;
         if constexpr (T::KIND == CACHE_F16) {
             if (boxes) {
-                // Warp 8 brings keys, warp 9 values: lane i the box of tokens from i * box_rows on; a box that is not there lies on the page behind the last
+                // Warp 8 brings keys, warp 12 values: lane i the box of tokens from i * box_rows on; a box that is not there lies on the page behind the last
                 // and reads as zeros.  Tokens behind the prefix's last in a box that is there are what the page holds: masked as keys, as values overwritten with zeros.
-                if (warp < 10) {
-                    const bool values = warp == 9;
-                    const int stages = values ? T::VS : T::KS, groups = T::NB / p.box_rows;
-                    const uint32_t ring = smem + (values ? T::V_RING : T::RING);
+                if ((warp & 3) == 0) {
+                    const int groups = T::NB / p.box_rows;
                     const CUtensorMap* const map = values ? &p.vmap : &p.kmap;
                     if (lane == 0) ptx::prefetch_tensormap(map);
                     order_before_tma();
@@ -246,10 +273,10 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                         const bool here = (uint32_t)now < (uint32_t)p.num_pages;
                         const uint32_t present = __ballot_sync(0xffffffffu, here);
                         const int stage = j % stages;
-                        const uint32_t full = values ? bar(full_v[stage]) : bar(full_k[stage]);
-                        ok = __all_sync(0xffffffffu, ptx::mbar_wait(values ? bar(empty_v[stage]) : bar(empty_k[stage]), ((j / stages) & 1) ^ 1, &g_status, ST_LOAD));
+                        ok = __all_sync(0xffffffffu, ptx::mbar_wait(empty(stage), ((j / stages) & 1) ^ 1, &g_status, ST_LOAD));
                         if (!ok) break;
                         if (!values) { // the scores' masks: bit x of word w is token 32 w + x
+                            if (lane >= T::NB / 32 && lane < 4) masks[j % T::INFOS][lane] = 0xffffffffu;
                             if (lane < T::NB / 32) {
                                 const uint32_t half0 = present >> (lane * 32 / p.box_rows) & 1, half1 = present >> ((lane * 32 + 16) / p.box_rows) & 1;
                                 const int32_t left = n - first - lane * 32;
@@ -259,7 +286,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                             if (lane == 0) ptx::mbar_arrive(bar(info_full[j % T::INFOS]));
                         }
                         const bool tail = values && first + T::NB > n;
-                        const uint32_t landed = tail ? bar(tail_full) : full;
+                        const uint32_t landed = tail ? bar(tail_full) : full(stage);
                         if (lane == 0) ptx::mbar_arrive_expect_tx(landed, T::V_BYTES);
                         __syncwarp();
                         if (lane < groups) {
@@ -276,130 +303,103 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                                 for (int a = 0; a < T::ATOMS; ++a) ptx::st_shared_v4(ring + stage * T::V_BYTES + a * (T::NB * 128) + x * 16, make_uint4(0, 0, 0, 0));
                             ptx::fence_proxy_async_smem();
                             __syncwarp();
-                            if (lane == 0) ptx::mbar_arrive(full);
+                            if (lane == 0) ptx::mbar_arrive(full(stage));
                         }
                     }
                 }
             } else {
-                // loads of keys and of values in turn; up to three are on their way when the next is issued
-                int32_t arrived = 0, issued = 0;
-                auto arrive = [&] {
-                    ptx::fence_proxy_async_smem();
-                    ptx::mbar_arrive(arrived & 1 ? bar(full_v[(arrived >> 1) % T::VS]) : bar(full_k[(arrived >> 1) % T::KS]));
-                    ++arrived;
-                };
-                auto settle = [&] {
+                // one block's pieces on their way while the next one's are issued
+                int32_t arrived = 0;
+                auto settle = [&](int32_t issued) { // what is issued has landed
                     ptx::cp_async_wait<0>();
-                    while (arrived < issued) arrive();
+                    for (; arrived < issued; ++arrived) {
+                        ptx::fence_proxy_async_smem();
+                        report(full(arrived % stages));
+                    }
                 };
-                request(0);
+                if (blocks > 0) begin();
                 for (int32_t j = 0; j < blocks; ++j) {
-                    locate(j);
-                    request(j + 1);
-                    ptx::named_barrier(1, 128);
-                    int64_t at[T::LOADS];
+                    go_on(j);
+                    const int stage = j % stages;
+                    const uint32_t parity = ((j / stages) & 1) ^ 1;
+                    if (ok && !__all_sync(0xffffffffu, ptx::mbar_try_wait(empty(stage), parity))) { // what is on its way may be what the place waits for
+                        settle(j);
+                        ok = __all_sync(0xffffffffu, ptx::mbar_wait(empty(stage), parity, &g_status, ST_LOAD));
+                    }
+                    if (!ok) continue; // (every thread comes to every barrier and ballot)
 #pragma unroll
-                    for (int i = 0; i < T::LOADS; ++i) at[i] = row_at[j & 1][token_of(i)].at;
-#pragma unroll
-                    for (int values = 0; values < 2; ++values) {
-                        const int stages = values ? T::VS : T::KS, stage = j % stages;
-                        const uint32_t empty = values ? bar(empty_v[stage]) : bar(empty_k[stage]), parity = ((j / stages) & 1) ^ 1;
-                        if (ok && !ptx::mbar_try_wait(empty, parity)) { // what is on its way may be what the place waits for
-                            settle();
-                            ok = ptx::mbar_wait(empty, parity, &g_status, ST_LOAD);
-                        }
-                        if (!values) publish(j); // (every thread comes to every barrier and ballot)
-                        if (!ok) continue;
-                        const uint32_t dst = smem + (values ? T::V_RING + stage * T::V_BYTES : T::RING + stage * T::K_BYTES);
-                        const char* const base = values ? vbase : kbase;
-#pragma unroll
-                        for (int i = 0; i < T::LOADS; ++i) ptx::cp_async_16(dst + place(token_of(i), piece_of(i)), base + (at[i] < 0 ? 0 : at[i]) + piece_of(i) * 16, at[i] >= 0);
-                        ptx::cp_async_commit();
-                        ++issued;
-                        if (issued - arrived > 3) {
-                            ptx::cp_async_wait<3>();
-                            arrive();
-                        }
+                    for (int i = 0; i < T::LOADS; ++i) {
+                        ptx::cp_async_16(ring + stage * stage_bytes + place(token_of(i), piece_of(i)), row_at[values][j & 3][token_of(i)].at + piece_of(i) * 16);
+                    }
+                    ptx::cp_async_commit();
+                    if (j > arrived) {
+                        ptx::cp_async_wait<1>();
+                        ptx::fence_proxy_async_smem();
+                        report(full(arrived % stages));
+                        ++arrived;
                     }
                 }
-                settle();
+                if (ok) settle(blocks);
             }
         } else {
-            // a block's pieces are requested when the block before has been put into its place
-            uint4 kw[T::LOADS], vw[T::LOADS];
-            uint32_t ks[T::LOADS], vs[T::LOADS], k_there = 0, v_there = 0; // a bit a piece; what is not there is read from the cache's first row, and is nothing
-            auto fetch = [&](int32_t j, uint4 (&w)[T::LOADS], uint32_t (&s)[T::LOADS], uint32_t& there_bits, const char* base, const char* sbase) {
-                there_bits = 0;
-#pragma unroll
-                for (int i = 0; i < T::LOADS; ++i) {
-                    const int token = token_of(i), c = piece_of(i);
-                    const Row row = row_at[j & 1][token];
-                    w[i] = ld_global_16(base + (row.at < 0 ? 0 : row.at) + c * 16);
-                    if constexpr (T::KIND == CACHE_I8_GROUPS) s[i] = load_scales<2>(sbase + row.scale + c * 4);
-                    there_bits |= (row.at < 0 ? 0u : 1u) << i;
-                }
+            uint4 w[T::LOADS];
+            uint32_t scales[T::LOADS];
+            auto fetch = [&](int32_t j, int i) {
+                const Row row = row_at[values][j & 3][token_of(i)];
+                w[i] = ld_global_16(row.at + piece_of(i) * 16);
+                if constexpr (T::KIND == CACHE_I8_GROUPS) scales[i] = load_scales<2>(row.scale + piece_of(i) * 4);
+                else if (values) scales[i] = load_scales<1>(row.scale);
             };
-            auto put = [&](uint32_t dst, const uint4 (&w)[T::LOADS], const uint32_t (&scales)[T::LOADS], uint32_t there_bits, bool keys) {
+            // into its place, and each piece's successor of the next block is requested
+            auto put = [&](uint32_t dst, int32_t next) {
 #pragma unroll
                 for (int i = 0; i < T::LOADS; ++i) {
-                    const int token = token_of(i), c = 2 * piece_of(i);
-                    uint32_t o[8], r[8] = {}, s[T::LOADS] = {};
-                    const uint32_t all = 0u - (there_bits >> i & 1);
-                    whole_numbers(make_uint4(w[i].x & all, w[i].y & all, w[i].z & all, w[i].w & all), o);
-                    if constexpr (T::KIND == CACHE_I8_GROUPS) s[i] = scales[i] & all;
+                    uint32_t o[8], r[8] = {};
+                    whole_numbers(w[i], o);
                     if constexpr (T::KIND == CACHE_I8_GROUPS) {
+                        const uint32_t s = scales[i];
 #pragma unroll
                         for (int x = 0; x < 8; ++x) {
-                            const __half2 f = as_h2(__byte_perm(s[i], 0, x < 4 ? 0x1010 : 0x3232));
+                            const __half2 f = as_h2(__byte_perm(s, 0, x < 4 ? 0x1010 : 0x3232));
                             const __half2 h = __hmul2(as_h2(o[x]), f);
-                            if (keys) r[x] = h2(__hfma2(as_h2(o[x]), f, __hneg2(h)));
+                            r[x] = h2(__hfma2(as_h2(o[x]), f, __hneg2(h)));
                             o[x] = h2(h);
                         }
+                    } else if (values) { // (keys' scales go into the scores)
+                        const __half2 f = as_h2(__byte_perm(scales[i], 0, 0x1010));
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) o[x] = h2(__hmul2(as_h2(o[x]), f));
                     }
-                    const uint32_t a = dst + place(token, c), b = dst + place(token, c + 1);
+                    // (eight threads meet the banks twice; a store the other way round for every second 64 dimensions costs more instructions than that time)
+                    const uint32_t c = 2 * piece_of(i), a = dst + place(token_of(i), c), b = dst + place(token_of(i), c + 1);
                     ptx::st_shared_v4(a, make_uint4(o[0], o[1], o[2], o[3]));
                     ptx::st_shared_v4(b, make_uint4(o[4], o[5], o[6], o[7]));
-                    if (T::LOW && keys) {
+                    if (T::LOW && !values) {
                         ptx::st_shared_v4(a + T::V_BYTES, make_uint4(r[0], r[1], r[2], r[3]));
                         ptx::st_shared_v4(b + T::V_BYTES, make_uint4(r[4], r[5], r[6], r[7]));
                     }
+                    if (next < blocks) fetch(next, i);
                 }
                 ptx::fence_proxy_async_smem();
             };
             if (blocks > 0) {
-                request(0);
-                locate(0);
-                request(1);
-                ptx::named_barrier(1, 128);
-                fetch(0, kw, ks, k_there, kbase, ksbase);
-                fetch(0, vw, vs, v_there, vbase, vsbase);
-                publish(0);
+                begin();
+#pragma unroll
+                for (int i = 0; i < T::LOADS; ++i) fetch(0, i);
             }
             for (int32_t j = 0; j < blocks; ++j) {
-                locate(j + 1);
-                request(j + 2);
-                ptx::named_barrier(1, 128);
-                const int kstage = j % T::KS, vstage = j % T::VS;
+                go_on(j);
+                const int stage = j % stages;
                 // (after a wait that ran out nothing is stored any more, but every thread comes to every barrier and ballot)
-                ok = ok && ptx::mbar_wait(bar(empty_k[kstage]), ((j / T::KS) & 1) ^ 1, &g_status, ST_LOAD);
+                ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(empty(stage), ((j / stages) & 1) ^ 1, &g_status, ST_LOAD));
                 if (ok) {
-                    put(smem + T::RING + kstage * T::K_BYTES, kw, ks, k_there, true);
-                    ptx::mbar_arrive(bar(full_k[kstage]));
+                    put(ring + stage * stage_bytes, j + 1);
+                    report(full(stage));
                 }
-                if (j + 1 < blocks) {
-                    fetch(j + 1, kw, ks, k_there, kbase, ksbase);
-                    publish(j + 1);
-                }
-                ok = ok && ptx::mbar_wait(bar(empty_v[vstage]), ((j / T::VS) & 1) ^ 1, &g_status, ST_LOAD);
-                if (ok) {
-                    put(smem + T::V_RING + vstage * T::V_BYTES, vw, vs, v_there, false);
-                    ptx::mbar_arrive(bar(full_v[vstage]));
-                }
-                if (j + 1 < blocks) fetch(j + 1, vw, vs, v_there, vbase, vsbase);
             }
         }
     } else {
-        ptx::registers_up<176>();
+        ptx::registers_up<T::R_SOFTMAX>();
         // ---- softmax ---------------------------------------------------------------------------------------------------------------
         const int stream = warp >> 2, r = threadIdx.x & 127;
         // the rows of q: a tile at a time, requested together
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
             }
         }
         ptx::fence_proxy_async_smem();
-        ptx::mbar_arrive(bar(q_full));
+        report(bar(q_full));
 
         const uint32_t lanes = (uint32_t)(warp & 3) << 21; // 32 (warp & 3) in the address's upper half
         const uint32_t sum_at = tmem + lanes + T::O_COLUMN + (T::STREAMS == 2 ? stream * T::DP : 0);
@@ -429,56 +429,85 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
             for (int32_t i = T::STREAMS == 2 ? stream : 0; i < tasks && ok; i += T::STREAMS) {
                 const int32_t j = i >> shift;
                 const int slot = j % T::INFOS;
-                ok = ptx::mbar_wait(bar(info_full[slot]), (j / T::INFOS) & 1, &g_status, ST_SOFTMAX) && ptx::mbar_wait(bar(score_full[i & 1]), (i >> 1) & 1, &g_status, ST_SOFTMAX);
+                ok = ok && ptx::mbar_wait(bar(info_full[slot]), (j / T::INFOS) & 1, &g_status, ST_SOFTMAX) && ptx::mbar_wait(bar(score_full[i & 1]), (i >> 1) & 1, &g_status, ST_SOFTMAX);
                 if (!(ok = __all_sync(0xffffffffu, ok))) break;
                 ptx::tc_fence_after();
                 const uint32_t at = tmem + lanes + (i & 1) * 128;
-                uint32_t bits[T::NB];
+                // Where registers hold half of the scores (KEPT), the others are looked at for the largest and loaded again when the first half's weights are on their way.
+                constexpr int HALF = T::NB / 2, KEPT = T::KEPT;
+                const bool straight = p.scale_log2 > 0.0f; // the largest product stays the largest score
+                const float factor = straight ? p.scale_log2 : 1.0f; // of what score() gives
+                const uint4 mask4 = *reinterpret_cast<const uint4*>(masks[slot]);
+                met |= (mask4.x | mask4.y | (T::NB == 128 ? mask4.z | mask4.w : 0u)) != 0;
+                const bool whole = (mask4.x & mask4.y & mask4.z & mask4.w) == 0xffffffffu;
+                auto score = [&](const uint32_t (&bits)[32], float (&x)[32], int c) { // of tokens c to c + 31
+                    if constexpr (T::KIND == CACHE_I8_ROWS) { // the scales of 32 keys, read as they are: in 32 bits they would take half of the shared memory's time
+                        const uint4* const ks = reinterpret_cast<const uint4*>(raw_smem + (smem - ptx::smem_addr(raw_smem)) + T::INFO) + (slot * T::NB + c) / 8;
 #pragma unroll
-                for (int c = 0; c < T::NB; c += 32) ptx::tmem_ld_32x32(at + c, reinterpret_cast<uint32_t(&)[32]>(bits[c]));
-                ptx::tmem_ld_wait();
-                float s[T::NB];
+                        for (int k = 0; k < 32; k += 8) {
+                            const uint4 f = ks[k / 8];
+                            const uint32_t f4[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-                for (int c = 0; c < T::NB; ++c) s[c] = __uint_as_float(bits[c]);
-                const float4* const ks = reinterpret_cast<const float4*>(raw_smem + (smem - ptx::smem_addr(raw_smem)) + T::INFO) + slot * T::NB / 2;
-                float factor = 1.0f; // of a score, where it is not in it
-                if constexpr (T::KIND == CACHE_I8_ROWS) {
+                            for (int y = 0; y < 4; ++y) {
+                                const float2 u = ptx::mul2(make_float2(__uint_as_float(bits[k + 2 * y]), __uint_as_float(bits[k + 2 * y + 1])), __half22float2(as_h2(f4[y])));
+                                x[k + 2 * y] = u.x; x[k + 2 * y + 1] = u.y;
+                            }
+                        }
+                    } else {
 #pragma unroll
-                    for (int c = 0; c < T::NB; c += 4) {
-                        const float4 f = ks[c / 4];
-                        const float2 a = ptx::mul2(make_float2(s[c], s[c + 1]), make_float2(f.x, f.y)), b = ptx::mul2(make_float2(s[c + 2], s[c + 3]), make_float2(f.z, f.w));
-                        s[c] = a.x; s[c + 1] = a.y; s[c + 2] = b.x; s[c + 3] = b.y;
+                        for (int k = 0; k < 32; ++k) x[k] = __uint_as_float(bits[k]);
                     }
-                } else if (p.scale_log2 > 0.0f) { // the largest stays the largest
-                    factor = p.scale_log2;
-                } else {
+                    if (!straight)
 #pragma unroll
-                    for (int c = 0; c < T::NB; ++c) s[c] *= p.scale_log2;
+                        for (int k = 0; k < 32; ++k) x[k] *= p.scale_log2;
+                    if (!whole) {
+                        const uint32_t mask = c == 0 ? mask4.x : c == 32 ? mask4.y : c == 64 ? mask4.z : mask4.w;
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (!(mask >> k & 1)) x[k] = -INFINITY;
+                    }
+                };
+                float high[8];
+#pragma unroll
+                for (int y = 0; y < 8; ++y) high[y] = -INFINITY;
+                auto look = [&](const float (&x)[32]) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 16)
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) high[y] = fmaxf(high[y], fmaxf(x[k + y], x[k + 8 + y]));
+                };
+#pragma unroll
+                for (int c = KEPT; c < T::NB; c += 32) {
+                    uint32_t bits[32];
+                    float x[32];
+                    ptx::tmem_ld_32x32(at + c, bits);
+                    ptx::tmem_ld_wait();
+                    score(bits, x, c);
+                    look(x);
                 }
-                uint32_t any = 0;
+                float s[KEPT / 32][32];
+                {
+                    uint32_t bits[KEPT / 32][32];
 #pragma unroll
-                for (int c = 0; c < T::NB; c += 32) {
-                    const uint32_t mask = masks[slot][c / 32];
-                    any |= mask;
-                    if (mask != 0xffffffffu) {
+                    for (int c = 0; c < KEPT; c += 32) ptx::tmem_ld_32x32(at + c, bits[c / 32]);
+                    ptx::tmem_ld_wait();
 #pragma unroll
-                        for (int x = 0; x < 32; ++x)
-                            if (!(mask >> x & 1)) s[c + x] = -INFINITY;
+                    for (int c = 0; c < KEPT; c += 32) {
+                        score(bits[c / 32], s[c / 32], c);
+                        look(s[c / 32]);
                     }
                 }
-                met |= any != 0;
-                float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < T::NB; c += 8)
+                for (int y = 4; y > 0; y >>= 1)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) high[x] = fmaxf(high[x], fmaxf(s[c + x], s[c + 4 + x]));
-                float m = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * factor;
-                if constexpr (T::KIND == CACHE_I8_ROWS) m += fmaxf(fmaxf(sizes[slot][0], sizes[slot][1]), fmaxf(sizes[slot][2], sizes[slot][3]));
-                // the reference exponent moves when a weight would pass 2^14, each row's for itself
+                    for (int k = 0; k < y; ++k) high[k] = fmaxf(high[k], high[k + y]);
+                const float m = high[0] * factor;
+                // The reference exponent moves when a weight would pass 2^14, each row's for itself, and then to kAbove above the largest score: some row of 32 meets a score
+                // 2^6 times as heavy again and again where keys have a few large dimensions.  The largest weight is 2^4 at least; those below 2^-18 of it lose bits.
                 const bool higher = m > top + 6.0f;
                 if (__any_sync(0xffffffffu, higher)) {
-                    const float keep = higher ? exp2_fast(top - m) : 1.0f;
-                    if (higher) top = m;
+                    const float to = higher ? m + kAbove : top, keep = exp2_fast(top - to);
+                    top = to;
                     sum *= keep;
                     const int32_t before = T::STREAMS == 2 ? i - 2 : i - 1; // the last task that has added to these sums
                     if (before >= 0) {
@@ -499,29 +528,40 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                 }
                 const float2 reference = make_float2(8.0f - top, 8.0f - top), factors = make_float2(factor, factor);
                 float2 sums[2] = {};
-#pragma unroll
-                for (int c = 0; c < T::NB; c += 32) {
+                auto weigh = [&](const float (&x)[32], int c) { // weights of tokens c to c + 31 into their place
                     uint32_t w[16];
 #pragma unroll
-                    for (int x = 0; x < 32; x += 2) {
-                        float2 e = ptx::fma2(make_float2(s[c + x], s[c + x + 1]), factors, reference);
+                    for (int k = 0; k < 32; k += 2) {
+                        float2 e = ptx::fma2(make_float2(x[k], x[k + 1]), factors, reference);
                         e.x = exp2_fast(e.x);
                         e.y = exp2_fast(e.y);
-                        sums[x >> 1 & 1] = ptx::add2(sums[x >> 1 & 1], e);
-                        if constexpr (T::KIND == CACHE_I8_ROWS) e = ptx::mul2(e, reinterpret_cast<const float2*>(ks)[T::NB / 2 + (c + x) / 2]);
-                        w[x / 2] = h2(__floats2half2_rn(e.x, e.y));
+                        sums[k >> 1 & 1] = ptx::add2(sums[k >> 1 & 1], e);
+                        w[k / 2] = h2(__floats2half2_rn(e.x, e.y));
                     }
                     ptx::tmem_st_32x16(at + c / 2, w);
-                    if (c + 32 == T::NB / 2) {
+                };
+#pragma unroll
+                for (int c = 0; c < KEPT; c += 32) {
+                    weigh(s[c / 32], c);
+                    if (c + 32 == HALF) {
                         ptx::tmem_st_wait();
                         ptx::tc_fence_before();
-                        ptx::mbar_arrive(bar(weight_half[i & 1]));
+                        report(bar(weight_half[i & 1]));
                     }
+                }
+#pragma unroll
+                for (int c = KEPT; c < T::NB; c += 32) {
+                    uint32_t bits[32];
+                    float x[32];
+                    ptx::tmem_ld_32x32(at + c, bits);
+                    ptx::tmem_ld_wait();
+                    score(bits, x, c);
+                    weigh(x, c);
                 }
                 sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
                 ptx::tmem_st_wait();
                 ptx::tc_fence_before();
-                ptx::mbar_arrive(bar(weight_full[i & 1]));
+                report(bar(weight_full[i & 1]));
             }
         }
         // ---- the sums ---------------------------------------------------------------------------------------------------------------
@@ -591,7 +631,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
     }
     ptx::tc_fence_before();
     __syncthreads();
-    if (warp == 12) ptx::tmem_dealloc(tmem, 512);
+    if (warp == 16) ptx::tmem_dealloc(tmem, 512);
 }
 
 } // namespace prefix

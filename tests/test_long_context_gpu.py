@@ -443,7 +443,7 @@ def _run_prefix(cuda, pplb200, prefix, lengths, hq, hk, d, page, group, order="h
     for b, n in enumerate(lengths):
         k, v = (cuda.cat([written[0][x], written[1 + b][x]]) for x in (0, 1))
         seen = cuda.cat([shared[0], shared[1 + b]])
-        want.append(_attention(cuda, q[b], k, v, seen if n >= 0 else cuda.zeros_like(seen), att.scale, group == 8))
+        want.append(_attention(cuda, q[b], k, v, seen if n >= 0 else cuda.zeros_like(seen), att.scale, group > 0))  # v of int8 caches is rounded to fp16
     return out, lse, want, (att, call, cache)
 
 
