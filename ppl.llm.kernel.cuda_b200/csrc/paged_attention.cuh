@@ -97,6 +97,7 @@ struct AttentionParams {
     int32_t parts;                             // sums of earlier calls that are joined
     bool keep_parts;                           // leave the sums, as part 0
     bool late_wait;
+    bool whole_items; // as many CTAs as items, one each
     int64_t part_rows;                         // rows of a part: query heads of all sequences
     float2* part_tops;                         // [parts][part_rows]
     float* part_sums;                          // [parts][part_rows][D]
@@ -252,19 +253,20 @@ __device__ __forceinline__ void finish(const AttentionParams& p, int64_t b, int3
                 top = kNothingSeen;
                 sum = 0.0f;
             } else {
-                // four parts at once, eight loads on their way
-                for (int32_t i = 0; i < p.parts; i += 4) {
-                    float2 s[4];
-                    float4 a[4];
+                // eight parts at once, sixteen loads on their way
+                constexpr int BATCH = 8;
+                for (int32_t i = 0; i < p.parts; i += BATCH) {
+                    float2 s[BATCH];
+                    float4 a[BATCH];
                     float up = top;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < BATCH; ++j) {
                         const int64_t from = min(i + j, p.parts - 1) * p.part_rows + at;
                         s[j] = __ldcg(&p.part_tops[from]);
                         a[j] = __ldcg(reinterpret_cast<const float4*>(p.part_sums + from * S::D + d));
                     }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < BATCH; ++j) {
                         if (i + j >= p.parts) s[j] = make_float2(kNothingSeen, 0.0f);
                         up = fmaxf(up, s[j].x);
                     }
@@ -273,7 +275,7 @@ __device__ __forceinline__ void finish(const AttentionParams& p, int64_t b, int3
                     sum *= keep;
                     v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                    for (int j = 0; j < BATCH; ++j)
                         if (s[j].x != kNothingSeen) { // else its sums need not have been written
                             const float f = exp2_fast(s[j].x - up);
                             sum += s[j].y * f;
@@ -310,7 +312,14 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
     Share from, to;
     int64_t all;
     int32_t ctas;
-    {
+    if (S::GENERAL && p.whole_items) { // known without the lengths
+        all = ctas = gridDim.x;
+        from.b = blockIdx.x / heads_per_sequence;
+        from.head = blockIdx.x - (int32_t)from.b * heads_per_sequence;
+        to.b = (blockIdx.x + 1) / heads_per_sequence;
+        to.head = blockIdx.x + 1 - (int32_t)to.b * heads_per_sequence;
+        from.step = to.step = 0;
+    } else {
         const int64_t per_thread = (p.batch + S::THREADS - 1) / S::THREADS, b0 = min(p.batch, threadIdx.x * per_thread), b1 = min(p.batch, b0 + per_thread);
         int64_t mine = 0;
         int32_t most = 0;
@@ -961,7 +970,10 @@ int32_t launch(cudaStream_t stream, AttentionParams& p, int64_t tokens) {
     // No more CTAs than there can be work for: the lengths are known on the device only.
     const int64_t steps = std::max<int64_t>(1, (tokens + S::TOKENS - 1) / S::TOKENS), items = p.batch * p.cache.kv_heads * p.tiles;
     const int64_t most = S::CTAS * kSms, ctas = items >= most ? most : std::min(most, std::max(items, items * (steps + kBeginning<S>) / S::WARPS));
-    launch_ex(paged_attention_kernel<S>, dim3((unsigned)ctas), dim3(S::THREADS), stream, true, p);
+    // Items that are short whatever their lengths, and no more than there are CTAs: a CTA each, without looking through the lengths first (64 sequences of 8 heads
+    // behind a prefix: 2 us less).
+    p.whole_items = S::GENERAL && items <= most && 4 * items >= most && steps <= 8 * S::WARPS;
+    launch_ex(paged_attention_kernel<S>, dim3((unsigned)(p.whole_items ? items : ctas)), dim3(S::THREADS), stream, true, p);
     return check_launch("paged attention");
 }
 

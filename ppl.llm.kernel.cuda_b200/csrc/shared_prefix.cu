@@ -14,10 +14,12 @@ constexpr int64_t kMaxRows = 1 << 24;
 // Rows of a key head up to which the decode kernel, whose matrix instructions take 8 or 16 of them at once, goes through the prefix.
 int32_t few_rows(int32_t head_dim) { return head_dim <= 128 ? 16 : 8; }
 
-// Tiles of rows that a CTA takes at once: two share what is loaded, unless the last of an odd number would leave half of a CTA idle that counts.
-int32_t tiles_at_once(int64_t rows, int32_t most) {
-    const int64_t tiles = (rows + 127) / 128;
-    return most == 2 && tiles > 1 && (tiles % 2 == 0 || tiles >= 7) ? 2 : 1;
+// Tiles of rows that a CTA takes at once.  Two share what is loaded, but leave twice as many sums to be joined: one, unless a CTA then had many blocks of a prefix to go
+// through that is not to be had from L2 (256 rows of 8 heads over 1, 4096 and 32768 tokens: 19 and 47 us with one, 22 and 49 with two; 512 rows of 64 over 8, 4096, 12345 and
+// 32768 tokens: 28, 47, 89 and 32, 47, 84).
+int32_t tiles_at_once(const PrefixParams& p, int32_t most, int64_t blocks, int64_t bytes) {
+    const int64_t tiles = (p.rows + 127) / 128, ctas = std::max<int64_t>(1, kSms / (p.cache.kv_heads * tiles));
+    return most == 2 && tiles > 1 && (tiles % 2 == 0 || tiles >= 7) && blocks > 24 * ctas && bytes > (64LL << 20) ? 2 : 1;
 }
 // Parts that the prefix is cut into, so that there is a CTA for every SM.
 int32_t splits_of(int64_t items) { return (int32_t)std::max<int64_t>(1, kSms / items); }
@@ -56,9 +58,9 @@ template <int D, int KIND>
 int32_t launch_tiles(cudaStream_t stream, PrefixParams& p) {
     using T = Tile<D, KIND>;
     static_assert(T::SMEM + 18 * 1024 <= 232448);
-    p.tiles = tiles_at_once(p.rows, T::TILES);
-    p.items = p.cache.kv_heads * (int32_t)((p.rows + p.tiles * 128 - 1) / (p.tiles * 128));
     const int64_t blocks = std::max<int64_t>(1, (p.tokens_in_table + T::NB - 1) / T::NB);
+    p.tiles = tiles_at_once(p, T::TILES, blocks, p.tokens_in_table * p.cache.kv_heads * D * 2 * T::ES);
+    p.items = p.cache.kv_heads * (int32_t)((p.rows + p.tiles * 128 - 1) / (p.tiles * 128));
     p.splits = (int32_t)std::min<int64_t>(splits_of(p.items), blocks);
     p.box_rows = 0;
     if (KIND == CACHE_F16 && p.cache.page_size % 16 == 0 && p.cache.num_pages > 0) {
