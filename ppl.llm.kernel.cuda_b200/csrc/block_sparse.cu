@@ -2,6 +2,7 @@
 // over what was chosen.
 #include "paged_attention.cuh"
 #include "ptx.cuh"
+#include "quotient.cuh"
 
 #include <type_traits>
 
@@ -187,11 +188,11 @@ __global__ void __launch_bounds__(BTPB) key_bounds_read_kernel(const __grid_cons
 // ---- the choice ----------------------------------------------------------------------------------------------------------
 // One cluster of CTAs for each sequence and key head.  A CTA scores its share of the blocks, 16 a warp at a time, on int8 mma.sync (16 blocks x 32
 // dimensions x 8 query heads; the product is tiny, what counts is that the bounds are read once and wide): sum_d max(q lo, q hi) is the product of q's
-// positive part with the greatest and of its negative part with the least.  The scores stay in shared memory as numbers that order alike.  The
-// threshold is found by histograms that the cluster's CTAs fill together in the first one's shared memory: of 2048 bins over the range that the scores
-// have, then over the bin with the threshold in it, until that holds nothing but scores that are taken, or one value; two or three rounds.  (Digits of the scores
-// themselves, whose leading ones hardly differ, put all on a few counters: 25 us where this takes 10.)  Then every CTA writes those of its blocks that are
-// above the threshold, and as many of those at it, from the lowest on, as there is room for.
+// positive part with the greatest and of its negative part with the least.  The scores stay in shared memory as numbers that order alike; a cluster's CTAs tell
+// each other theirs, where all have room for them, and then each finds the threshold by itself.  It is found by histograms: of 2048 bins over the range that the scores
+// have, then over the bin with the threshold in it, until that holds nothing but scores that are taken, or one value; one to three rounds.  (Digits of the scores
+// themselves, whose leading ones hardly differ, put all on a few counters; histograms that a cluster fills together cost two of its barriers a round, 2 us.)  Then
+// every CTA writes those of its blocks that are above the threshold, and as many of those at it, from the lowest on, as there is room for.
 constexpr int MAX_CLUSTER = 8, BINS = 2048;
 constexpr int64_t MAX_BLOCKS = 1 << 18, MAX_TOTAL = 65536, MAX_ITEMS = 1 << 24;
 struct ChoiceParams {
@@ -206,8 +207,8 @@ struct ChoiceParams {
     int64_t tokens_in_table, items;
     int32_t kv_heads, shared, block, per_page, num_pages, first, last, top, total;
     uint32_t block_magic, block_shift, page_magic, page_shift; // / block, / per_page
-    int32_t share;   // blocks of a CTA at most, a multiple of 16
-    bool units_kept; // shared memory for the blocks' numbers beside their scores
+    int32_t share, kept_keys; // blocks of a CTA at most, a multiple of 16; scores that it keeps
+    bool gathered, units_kept;
 };
 
 __device__ __forceinline__ void mma_s8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -228,6 +229,11 @@ __device__ __forceinline__ void min_in_cluster(uint32_t addr, uint32_t v) {
 __device__ __forceinline__ void max_in_cluster(uint32_t addr, uint32_t v) {
     asm volatile("red.relaxed.cluster.shared::cluster.max.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
+__device__ __forceinline__ uint4 ld4_in_cluster(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ uint32_t ld_in_cluster(uint32_t addr) {
     uint32_t v;
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -240,13 +246,14 @@ __global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_
     constexpr int KB = D / 4, KP = piece(KB), KN = KB / KP, KW = KP / 4; // a quad's lane has a quarter of a row, in pieces
     constexpr int MMAS = D / 32, TILES = D == 256 ? 1 : 2;               // tiles of 16 blocks that a warp has on their way together
     constexpr int PIECES = (D + TPB - 1) / TPB;                          // of q, eight dimensions each, a thread
-    extern __shared__ uint32_t keys[];       // [share]: scores; where there is room, units[share]: the blocks' numbers in the cache
-    int32_t* const units = p.units_kept ? reinterpret_cast<int32_t*>(keys + p.share) : nullptr;
+    // Scores: of the CTA's share; gathered: of all blocks, each CTA's share in every CTA.  Where there is room, the share's blocks' numbers in the cache.
+    extern __shared__ uint32_t keys[];
+    int32_t* const units = p.units_kept ? reinterpret_cast<int32_t*>(keys + p.kept_keys) : nullptr;
     __shared__ __align__(16) uint32_t q8[8][D / 4];
     __shared__ uint32_t q_bits[8];
-    // of the cluster's first CTA: bins; least and greatest of the range; how many of it are taken; whether these are all of it
+    // each CTA's own where scores are gathered, else the cluster's first CTA's
     __shared__ __align__(16) uint32_t histogram[BINS];
-    __shared__ uint32_t range[2], taken[2];
+    __shared__ __align__(16) uint32_t found[4]; // least and greatest of the range; how many of it are taken; whether these are all of it
     __shared__ uint32_t above, at_threshold; // counts of this CTA
     __shared__ uint32_t scan[WARPS][2];
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, t = lane & 3;
@@ -256,7 +263,7 @@ __global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_
     const int64_t b = item / p.kv_heads;
     const int32_t kvh = (int32_t)(item - b * p.kv_heads);
     for (int x = threadIdx.x; x < BINS; x += TPB) histogram[x] = 0;
-    if (threadIdx.x == 0) range[0] = 0xffffffffu, range[1] = 0, above = at_threshold = 0;
+    if (threadIdx.x == 0) found[0] = 0xffffffffu, found[1] = 0, above = at_threshold = 0;
     pdl_wait_prior_grid();
     pdl_launch_dependents();
 
@@ -312,6 +319,7 @@ __global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_
     // ---- scores of this CTA's share ------------------------------------------------------------------------------------------
     const int32_t share = (between + ctas * 16 - 1) / (ctas * 16) * 16;
     const int32_t begin = min(between, rank * share), mine = min(between, begin + share) - begin;
+    uint32_t* const mine_keys = keys + (p.gathered ? begin : 0);
     int32_t pages[TILES][2]; // of the lane's blocks, a round ahead
     auto look_up = [&](int32_t tile) {
 #pragma unroll
@@ -343,18 +351,14 @@ __global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_
         for (int i = 0; i < PIECES; ++i) {
             const int x = threadIdx.x + i * TPB, h = x / (D / 8);
             if (x >= 8 * (D / 8)) break;
-            uint32_t o[2] = {};
+            uint2 o = make_uint2(0, 0);
             if (h < heads && q_bits[h] < 0x7c00u) {
-                const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-                const float s = __half2float(outer_scale(__half2float(__ushort_as_half((unsigned short)q_bits[h]))));
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const float v = __half2float(__ushort_as_half((unsigned short)(w[k >> 1] >> (16 * (k & 1)))));
-                    o[k >> 2] |= (uint32_t)(__float2int_rn(__fdiv_rn(v, s)) & 0xff) << (8 * (k & 3));
-                }
+                Eight e;
+                e.raw = raw[i];
+                o = Quotient(outer_scale(__half2float(__ushort_as_half((unsigned short)q_bits[h])))).eight(e);
             }
-            q8[h][(x - h * (D / 8)) * 2] = o[0];
-            q8[h][(x - h * (D / 8)) * 2 + 1] = o[1];
+            q8[h][(x - h * (D / 8)) * 2] = o.x;
+            q8[h][(x - h * (D / 8)) * 2 + 1] = o.y;
         }
         __syncthreads();
         if (!ends) load_q(head0 + 8);
@@ -423,8 +427,8 @@ __global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_
                     key = unit[m][r] >= 0 ? max(key, 1u) : 0u; // holes come behind everything that is there
                     const int32_t x = tile + m * WARPS * 16 + g + 8 * r;
                     if (t == 0 && x < mine) {
-                        if (head0 > 0) key = max(key, keys[x]);
-                        keys[x] = key;
+                        if (head0 > 0) key = max(key, mine_keys[x]);
+                        mine_keys[x] = key;
                         if (units) units[x] = unit[m][r];
                         if (ends) lowest = min(lowest, key), highest = max(highest, key);
                     }
@@ -434,23 +438,39 @@ __global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_
     }
 
     // ---- the threshold ---------------------------------------------------------------------------------------------------------
+    const bool alone = ctas == 1 || p.gathered; // every CTA finds it by itself, with barriers of its own
     auto sync = [&] {
-        if (ctas > 1) cluster_sync_all();
-        else __syncthreads();
+        if (alone) __syncthreads();
+        else cluster_sync_all();
     };
-    const uint32_t bins0 = map_to_cta(ptx::smem_addr(histogram), 0), range0 = map_to_cta(ptx::smem_addr(range), 0), taken0 = map_to_cta(ptx::smem_addr(taken), 0);
+    if (ctas > 1 && p.gathered) {
+        __syncthreads();
+        cluster_sync_all(); // all CTAs are there
+        for (int32_t r = 0; r < ctas; ++r) {
+            if (r == rank) continue;
+            const uint32_t there = map_to_cta(ptx::smem_addr(mine_keys), r);
+            for (int32_t x = threadIdx.x; x < mine; x += TPB) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there + x * 4), "r"(mine_keys[x]) : "memory");
+        }
+        cluster_sync_all(); // from here on nobody looks into another CTA
+        lowest = 0xffffffffu;
+        highest = 0;
+        for (int32_t x = threadIdx.x; x < between; x += TPB) lowest = min(lowest, keys[x]), highest = max(highest, keys[x]);
+    }
+    const int32_t looked_at = ctas > 1 && p.gathered ? between : mine;
+    const uint32_t first = alone ? rank : 0, bins0 = map_to_cta(ptx::smem_addr(histogram), first), found0 = map_to_cta(ptx::smem_addr(found), first);
     lowest = __reduce_min_sync(0xffffffffu, lowest);
     highest = __reduce_max_sync(0xffffffffu, highest);
-    sync(); // the first CTA's histogram and range are there
-    if (lane == 0 && lowest <= highest) min_in_cluster(range0, lowest), max_in_cluster(range0 + 4, highest);
+    sync(); // the histogram and the range are there
+    if (lane == 0 && lowest <= highest) min_in_cluster(found0, lowest), max_in_cluster(found0 + 4, highest);
     sync();
-    uint32_t least = ld_in_cluster(range0), most = ld_in_cluster(range0 + 4), room = p.top, all = 0; // of the scores in [least, most], `room` are taken
+    uint4 now = ld4_in_cluster(found0);
+    uint32_t least = now.x, most = now.y, room = p.top, all = 0; // of the scores in [least, most], `room` are taken
     for (;;) {
         const uint32_t shift = max(0, 21 - __clz((int)(most - least))); // 2048 bins at most
-        for (int32_t x = threadIdx.x; x < mine; x += TPB)
+        for (int32_t x = threadIdx.x; x < looked_at; x += TPB)
             if (keys[x] >= least && keys[x] <= most) add_in_cluster(bins0 + ((keys[x] - least) >> shift) * 4, 1);
         sync();
-        if (rank == 0) {
+        if (alone || rank == 0) {
             // bins from the highest down: thread x has EACH of them, from BINS - EACH x - 1 on
             constexpr int EACH = BINS / TPB;
             uint32_t n_of[EACH], own = 0;
@@ -470,28 +490,23 @@ __global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_
             }
             if (lane == 31) scan[warp][0] = sum;
             __syncthreads();
-            for (int w = 0; w < warp; ++w) sum += scan[w][0];
+            sum += __reduce_add_sync(0xffffffffu, lane < warp ? scan[lane][0] : 0u);
             uint32_t over = sum - own;
             if (over < room && sum >= room) {
 #pragma unroll
                 for (int k = 0; k < EACH; ++k) {
                     if (over < room && over + n_of[k] >= room) {
                         const uint32_t bin = BINS - 1 - EACH * threadIdx.x - k;
-                        const uint32_t first = least + (bin << shift), width = (1u << shift) - 1;
-                        range[0] = first;
-                        range[1] = most - first < width ? most : first + width;
-                        taken[0] = room - over;
-                        taken[1] = n_of[k] == room - over;
+                        const uint32_t begins = least + (bin << shift), width = (1u << shift) - 1;
+                        *reinterpret_cast<uint4*>(found) = make_uint4(begins, most - begins < width ? most : begins + width, room - over, n_of[k] == room - over);
                     }
                     over += n_of[k];
                 }
             }
         }
         sync();
-        least = ld_in_cluster(range0);
-        most = ld_in_cluster(range0 + 4);
-        room = ld_in_cluster(taken0);
-        all = ld_in_cluster(taken0 + 4);
+        now = ld4_in_cluster(found0);
+        least = now.x; most = now.y; room = now.z; all = now.w;
         if (shift == 0 || all) break;
     }
 
@@ -499,42 +514,47 @@ __global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_
     auto over_it = [&](uint32_t key) { return all ? key >= least : key > least; };
     auto at_it = [&](uint32_t key) { return !all && key == least; };
     uint32_t before[2] = {};
-    if (ctas > 1) { // those of the CTAs before this one
+    if (ctas > 1) { // those of the shares before this one
         uint32_t counts[2] = {};
-        for (int32_t x = threadIdx.x; x < mine; x += TPB) {
+        const int32_t end = p.gathered ? begin : mine;
+        for (int32_t x = threadIdx.x; x < end; x += TPB) {
             counts[0] += over_it(keys[x]);
             counts[1] += at_it(keys[x]);
         }
         counts[0] = __reduce_add_sync(0xffffffffu, counts[0]);
         counts[1] = __reduce_add_sync(0xffffffffu, counts[1]);
         if (lane == 0) atomicAdd(&above, counts[0]), atomicAdd(&at_threshold, counts[1]);
-        cluster_sync_all();
-        for (int32_t r = 0; r < rank; ++r) {
-            before[0] += ld_in_cluster(map_to_cta(ptx::smem_addr(&above), r));
-            before[1] += ld_in_cluster(map_to_cta(ptx::smem_addr(&at_threshold), r));
+        sync();
+        if (p.gathered) {
+            before[0] = above;
+            before[1] = at_threshold;
+        } else {
+            for (int32_t r = 0; r < rank; ++r) {
+                before[0] += ld_in_cluster(map_to_cta(ptx::smem_addr(&above), r));
+                before[1] += ld_in_cluster(map_to_cta(ptx::smem_addr(&at_threshold), r));
+            }
+            asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); // nothing of another CTA's is read any more
         }
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); // nothing of another CTA's is read any more
     }
     for (int32_t x0 = 0; x0 < mine; x0 += TPB) {
         const int32_t x = x0 + threadIdx.x, block = p.first + begin + x;
-        const uint32_t key = x < mine ? keys[x] : 0u;
+        const uint32_t key = x < mine ? mine_keys[x] : 0u;
         const bool over = x < mine && over_it(key), same = x < mine && at_it(key);
         int32_t unit = -1;
         if (over || same) unit = units ? units[x] : unit_of(block, row_pages[page_index(block)]);
         const uint32_t overs = __ballot_sync(0xffffffffu, over), sames = __ballot_sync(0xffffffffu, same), below = (1u << lane) - 1;
         if (lane == 0) scan[warp][0] = __popc(overs), scan[warp][1] = __popc(sames);
         __syncthreads();
-        uint32_t o = before[0] + __popc(overs & below), s = before[1] + __popc(sames & below);
-        for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) o += scan[w][0], s += scan[w][1];
-            before[0] += scan[w][0];
-            before[1] += scan[w][1];
-        }
+        const uint32_t in_warps[2] = {lane < WARPS ? scan[lane][0] : 0u, lane < WARPS ? scan[lane][1] : 0u};
+        const uint32_t o = before[0] + __popc(overs & below) + __reduce_add_sync(0xffffffffu, lane < warp ? in_warps[0] : 0u);
+        const uint32_t s = before[1] + __popc(sames & below) + __reduce_add_sync(0xffffffffu, lane < warp ? in_warps[1] : 0u);
+        before[0] += __reduce_add_sync(0xffffffffu, in_warps[0]);
+        before[1] += __reduce_add_sync(0xffffffffu, in_warps[1]);
         if (over || (same && s < room)) put(p.first + o + min(s, room), block, unit);
         __syncthreads();
     }
     put_kept();
-    if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); // no CTA leaves while another reads its shared memory
+    if (!alone) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); // no CTA leaves while another reads its shared memory
 }
 
 int32_t check_bounds(const pplb200_kv_cache* c, const pplb200_key_bounds* k) {
@@ -566,7 +586,7 @@ int32_t launch_choice(cudaStream_t stream, const ChoiceParams& p, int32_t cluste
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)cluster, (unsigned)y, (unsigned)((p.items + y - 1) / y));
     cfg.blockDim = dim3(32 * WARPS);
-    cfg.dynamicSmemBytes = (size_t)p.share * (p.units_kept ? 8 : 4);
+    cfg.dynamicSmemBytes = (size_t)(p.kept_keys + (p.units_kept ? p.share : 0)) * 4;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -680,6 +700,8 @@ int32_t pplb200_block_sparse_attention_fp16(pplb200_stream_t stream, const pplb2
     int32_t cluster = 1;
     while (cluster < MAX_CLUSTER && ((p.items * cluster * 2 <= kSms && in_table > cluster * 512) || in_table > cluster * 32768LL)) cluster *= 2;
     p.share = (int32_t)std::max<int64_t>(16, (in_table + cluster * 16 - 1) / (cluster * 16) * 16);
+    p.gathered = cluster > 1 && (int64_t)p.share * cluster <= 16384;
+    p.kept_keys = p.gathered ? p.share * cluster : p.share;
     p.units_kept = p.share <= 16384;
     const cudaStream_t s = (cudaStream_t)stream;
     const auto launch_dims = [&](auto warps) {
