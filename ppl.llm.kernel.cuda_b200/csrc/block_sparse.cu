@@ -251,6 +251,7 @@ __global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_
     int32_t* const units = p.units_kept ? reinterpret_cast<int32_t*>(keys + p.kept_keys) : nullptr;
     __shared__ __align__(16) uint32_t q8[8][D / 4];
     __shared__ uint32_t q_bits[8];
+    __shared__ float q_scale[8]; // of a head without a say, or beyond the last: NaN
     // each CTA's own where scores are gathered, else the cluster's first CTA's
     __shared__ __align__(16) uint32_t histogram[BINS];
     __shared__ __align__(16) uint32_t found[4]; // least and greatest of the range; how many of it are taken; whether these are all of it
@@ -317,24 +318,49 @@ __global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_
     }
 
     // ---- scores of this CTA's share ------------------------------------------------------------------------------------------
+    if (ctas > 1 && p.gathered) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     const int32_t share = (between + ctas * 16 - 1) / (ctas * 16) * 16;
     const int32_t begin = min(between, rank * share), mine = min(between, begin + share) - begin;
     uint32_t* const mine_keys = keys + (p.gathered ? begin : 0);
-    int32_t pages[TILES][2]; // of the lane's blocks, a round ahead
+    // A warp has up to TILES * 16 neighbouring blocks at once; lane l looks after block l of them: its page, a round ahead, its place, its scale.
+    const int32_t at_once = mine > WARPS * 16 ? TILES * 16 : 16;
+    int32_t page_of_mine = -1;
     auto look_up = [&](int32_t tile) {
+        const int32_t x = tile + lane;
+        page_of_mine = lane < at_once && x < mine ? row_pages[page_index(p.first + begin + x)] : -1;
+    };
+    // Bounds and scales of a round of blocks.  What is not there reads those of the cache's first block, and
+    // comes behind everything.
+    uint32_t lo[TILES][2][KN][KW], hi[TILES][2][KN][KW], state = 0; // state: the scale, and above it whether the block is there
+    auto load = [&](int32_t tile) {
+        const int32_t unit = lane < at_once && tile + lane < mine ? unit_of(p.first + begin + tile + lane, page_of_mine) : -1;
+        const int64_t of_mine = unit >= 0 ? ((int64_t)page_of_mine * p.kv_heads + kvh) * p.per_page + (unit - page_of_mine * p.per_page) : 0;
+        state = unit >= 0 ? 0x10000u : 0u;
+        if (p.num_pages > 0) {
+            state |= __half_as_ushort(ld_global_half(p.scale + of_mine));
 #pragma unroll
-        for (int m = 0; m < TILES; ++m)
+            for (int m = 0; m < TILES; ++m)
+                if (m * 16 < at_once) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int32_t x = tile + m * WARPS * 16 + g + 8 * r;
-                pages[m][r] = x < mine ? row_pages[page_index(p.first + begin + x)] : -1;
-            }
+                    for (int r = 0; r < 2; ++r) {
+                        const int64_t at = __shfl_sync(0xffffffffu, of_mine, m * 16 + g + 8 * r);
+                        const char* const src = (const char*)p.bounds + at * 2 * D + t * KP;
+#pragma unroll
+                        for (int i = 0; i < KN; ++i) {
+                            load_piece<KP>(lo[m][r][i], src + i * 4 * KP);
+                            load_piece<KP>(hi[m][r][i], src + D + i * 4 * KP);
+                        }
+                    }
+                }
+        }
+        if (units && lane < at_once && tile + lane < mine) units[tile + lane] = unit;
+        look_up(tile + WARPS * at_once);
     };
     uint32_t lowest = 0xffffffffu, highest = 0;
     for (int32_t head0 = 0; head0 < p.shared; head0 += 8) {
         const int heads = min(8, p.shared - head0);
         const bool ends = head0 + 8 >= p.shared;
-        look_up(warp * 16);
+        look_up(warp * at_once);
         if (threadIdx.x < 8) q_bits[threadIdx.x] = 0;
         __syncthreads();
 #pragma unroll
@@ -344,7 +370,13 @@ __global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_
             uint32_t m = 0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) m = max(m, max(w[k] & 0xffffu, w[k] >> 16));
-            if (x < heads * (D / 8)) atomicMax(&q_bits[x / (D / 8)], m);
+            if constexpr (32 % (D / 8) == 0) { // a head's pieces lie in one warp
+#pragma unroll
+                for (int k = 1; k < D / 8; k <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, k));
+                if (x < heads * (D / 8) && x % (D / 8) == 0) q_bits[x / (D / 8)] = m;
+            } else if (x < heads * (D / 8)) {
+                atomicMax(&q_bits[x / (D / 8)], m);
+            }
         }
         __syncthreads();
 #pragma unroll
@@ -352,15 +384,20 @@ __global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_
             const int x = threadIdx.x + i * TPB, h = x / (D / 8);
             if (x >= 8 * (D / 8)) break;
             uint2 o = make_uint2(0, 0);
+            float scale = __int_as_float(0x7fffffff);
             if (h < heads && q_bits[h] < 0x7c00u) {
+                const half s = outer_scale(__half2float(__ushort_as_half((unsigned short)q_bits[h])));
+                scale = __half2float(s);
                 Eight e;
                 e.raw = raw[i];
-                o = Quotient(outer_scale(__half2float(__ushort_as_half((unsigned short)q_bits[h])))).eight(e);
+                o = Quotient(s).eight(e);
             }
+            if (x % (D / 8) == 0) q_scale[h] = scale;
             q8[h][(x - h * (D / 8)) * 2] = o.x;
             q8[h][(x - h * (D / 8)) * 2 + 1] = o.y;
         }
         __syncthreads();
+        load(warp * at_once);
         if (!ends) load_q(head0 + 8);
         // a product's dimensions come as the lane has them: words 2 m and 2 m + 1 of its own
         uint32_t plus[MMAS][2], minus[MMAS][2];
@@ -369,73 +406,49 @@ __global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int word = 2 * m + x, i = word / KW, s = word - i * KW;
-                const uint32_t w = q8[g][(i * 4 + t) * KW + s];
-                plus[m][x] = __vmaxs4(w, 0);
-                minus[m][x] = __vmins4(w, 0);
+                const uint32_t w = q8[g][(i * 4 + t) * KW + s], negative = ((w >> 7) & 0x01010101u) * 255u;
+                plus[m][x] = w & ~negative;
+                minus[m][x] = w & negative;
             }
-        float qs[2];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) { // heads 2 t and 2 t + 1; one without a say or beyond the last: NaN
-            const int h = 2 * t + x;
-            qs[x] = h < heads && q_bits[h] < 0x7c00u ? __half2float(outer_scale(__half2float(__ushort_as_half((unsigned short)q_bits[h])))) : __int_as_float(0x7fffffff);
-        }
-        for (int32_t tile = warp * 16; tile < mine; tile += TILES * WARPS * 16) {
-            uint32_t lo[TILES][2][KN][KW], hi[TILES][2][KN][KW];
-            half scale[TILES][2];
-            int32_t unit[TILES][2];
+        const float qs[2] = {q_scale[2 * t], q_scale[2 * t + 1]}; // of heads 2 t and 2 t + 1
+        for (int32_t tile = warp * at_once; tile < mine; tile += WARPS * at_once) {
 #pragma unroll
             for (int m = 0; m < TILES; ++m)
+                if (m * 16 < at_once) {
+                    int32_t c[4] = {}, c2[4] = {};
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int32_t x = tile + m * WARPS * 16 + g + 8 * r, block = p.first + begin + x, page = pages[m][r];
-                    unit[m][r] = x < mine ? unit_of(block, page) : -1;
-                    const int64_t at = ((int64_t)page * p.kv_heads + kvh) * p.per_page + (block - page_index(block) * p.per_page);
-                    const char* src = (const char*)p.bounds + at * 2 * D + t * KP;
+                    for (int k = 0; k < MMAS; ++k) {
+                        const int w = 2 * k, i = w / KW, s = w - i * KW;
+                        mma_s8(c, lo[m][0][i][s], lo[m][1][i][s], lo[m][0][i][s + 1], lo[m][1][i][s + 1], minus[k][0], minus[k][1]);
+                        mma_s8(c2, hi[m][0][i][s], hi[m][1][i][s], hi[m][0][i][s + 1], hi[m][1][i][s + 1], plus[k][0], plus[k][1]);
+                    }
 #pragma unroll
-                    for (int i = 0; i < KN; ++i) {
+                    for (int r = 0; r < 2; ++r) {
+                        const uint32_t of_row = __shfl_sync(0xffffffffu, state, m * 16 + g + 8 * r);
+                        const half scale = __ushort_as_half((unsigned short)of_row);
+                        const float f = __half2float(scale);
+                        uint32_t key = 0;
 #pragma unroll
-                        for (int w = 0; w < KW; ++w) lo[m][r][i][w] = hi[m][r][i][w] = 0;
-                        if (unit[m][r] >= 0) {
-                            load_piece<KP>(lo[m][r][i], src + i * 4 * KP);
-                            load_piece<KP>(hi[m][r][i], src + D + i * 4 * KP);
+                        for (int x = 0; x < 2; ++x) {
+                            const float score = __fmul_rn((float)(c[2 * r + x] + c2[2 * r + x]), qs[x] * f);
+                            if (qs[x] == qs[x]) key = max(key, ordered(score));
+                        }
+                        key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
+                        key = max(key, __shfl_xor_sync(0xffffffffu, key, 2));
+                        if (!is_finite(scale)) key = 0xffffffffu;
+                        key = of_row >> 16 ? max(key, 1u) : 0u; // holes come behind everything that is there
+                        const int32_t x = tile + m * 16 + g + 8 * r;
+                        if (t == 0 && x < mine) {
+                            if (head0 > 0) key = max(key, mine_keys[x]);
+                            mine_keys[x] = key;
+                            if (ends) lowest = min(lowest, key), highest = max(highest, key);
                         }
                     }
-                    scale[m][r] = unit[m][r] >= 0 ? ld_global_half(p.scale + at) : __ushort_as_half(0);
                 }
-            look_up(tile + TILES * WARPS * 16);
-#pragma unroll
-            for (int m = 0; m < TILES; ++m) {
-                int32_t c[4] = {}, c2[4] = {};
-#pragma unroll
-                for (int k = 0; k < MMAS; ++k) {
-                    const int w = 2 * k, i = w / KW, s = w - i * KW;
-                    mma_s8(c, lo[m][0][i][s], lo[m][1][i][s], lo[m][0][i][s + 1], lo[m][1][i][s + 1], minus[k][0], minus[k][1]);
-                    mma_s8(c2, hi[m][0][i][s], hi[m][1][i][s], hi[m][0][i][s + 1], hi[m][1][i][s + 1], plus[k][0], plus[k][1]);
-                }
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float f = __half2float(scale[m][r]);
-                    uint32_t key = 0;
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const float score = __fmul_rn((float)(c[2 * r + x] + c2[2 * r + x]), qs[x] * f);
-                        if (qs[x] == qs[x]) key = max(key, ordered(score));
-                    }
-                    key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
-                    key = max(key, __shfl_xor_sync(0xffffffffu, key, 2));
-                    if (!is_finite(scale[m][r])) key = 0xffffffffu;
-                    key = unit[m][r] >= 0 ? max(key, 1u) : 0u; // holes come behind everything that is there
-                    const int32_t x = tile + m * WARPS * 16 + g + 8 * r;
-                    if (t == 0 && x < mine) {
-                        if (head0 > 0) key = max(key, mine_keys[x]);
-                        mine_keys[x] = key;
-                        if (units) units[x] = unit[m][r];
-                        if (ends) lowest = min(lowest, key), highest = max(highest, key);
-                    }
-                }
-            }
+            if (tile + WARPS * at_once < mine) load(tile + WARPS * at_once);
         }
     }
+    put_kept(); // their pages are there by now
 
     // ---- the threshold ---------------------------------------------------------------------------------------------------------
     const bool alone = ctas == 1 || p.gathered; // every CTA finds it by itself, with barriers of its own
@@ -444,8 +457,8 @@ __global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_
         else cluster_sync_all();
     };
     if (ctas > 1 && p.gathered) {
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); // all CTAs are there
         __syncthreads();
-        cluster_sync_all(); // all CTAs are there
         for (int32_t r = 0; r < ctas; ++r) {
             if (r == rank) continue;
             const uint32_t there = map_to_cta(ptx::smem_addr(mine_keys), r);
@@ -553,7 +566,6 @@ __global__ void __launch_bounds__(32 * WARPS) choose_blocks_kernel(const __grid_
         if (over || (same && s < room)) put(p.first + o + min(s, room), block, unit);
         __syncthreads();
     }
-    put_kept();
     if (!alone) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); // no CTA leaves while another reads its shared memory
 }
 
