@@ -92,15 +92,12 @@ __device__ __forceinline__ void turns_at(Turns& t, uint64_t position, const uint
         t.s[i] *= magnitude;
     }
 }
-// The same where each plane has an axis, and the token a position on each: all of them are loaded side by side, and each plane picks its
-// own (three selections beside some forty instructions of a sine and cosine: 8192 tokens of 72 heads take what they take with one axis).
+// The same where each plane has an axis, and the token a position on each, which lie in shared memory: a plane's is one load (chosen by selections
+// among registers, 8192 tokens of 64 heads took 49 us where they take 43 with one axis).
 struct AxisPositions {
-    uint64_t at[PPLB200_ROTARY_MAX_AXES];
+    const uint64_t* at;     // [PPLB200_ROTARY_MAX_AXES]
     uint32_t first, second; // axes of four and four planes
-    __device__ __forceinline__ uint64_t of(int i) const {
-        const uint32_t axis = (i < 4 ? first : second) >> (8 * (i & 3)) & 0xffu;
-        return axis == 0 ? at[0] : axis == 1 ? at[1] : axis == 2 ? at[2] : at[3];
-    }
+    __device__ __forceinline__ uint64_t of(int i) const { return at[(i < 4 ? first : second) >> (8 * (i & 3)) & 3u]; }
 };
 __device__ __forceinline__ void turns_at(Turns& t, const AxisPositions& position, const uint64_t* first, const uint64_t* second, float magnitude) {
 #pragma unroll
@@ -248,16 +245,17 @@ __global__ void __launch_bounds__(RTPB, LAYOUT == AS_IS ? 8 : 7) rotary_kv_kerne
     if (p.turns_of[Q] > 0) r.template fetch<Q>(group, q);
     if (p.turns_of[K] > 0) r.template fetch<K>(group, k);
     if (STORE) r.template fetch<V>(group, v);
+    __shared__ uint64_t axis_positions[AXES ? RTPB / LANES : 1][PPLB200_ROTARY_MAX_AXES];
+    if constexpr (AXES) { // the LANES threads of a row, which lie in one warp, bring a position each
+        if (r.u < PPLB200_ROTARY_MAX_AXES) axis_positions[threadIdx.x / LANES][r.u] = (uint64_t)p.positions[min(r.u, p.axes - 1) * p.axis_stride + r.token];
+        __syncwarp();
+    }
     if (LAYOUT != AS_IS && r.turned) {
         const uint64_t* first = p.turns + (LAYOUT == INTERLEAVED ? 4 : 8) * r.u; // planes of the runs: eight of both, or four of each
         const int apart = LAYOUT == INTERLEAVED ? p.rotary_dim >> 2 : 4;
         if constexpr (AXES) {
-            AxisPositions at;
             const uint8_t* axis = p.axis_of_plane + (first - p.turns);
-            at.first = *reinterpret_cast<const uint32_t*>(axis);
-            at.second = *reinterpret_cast<const uint32_t*>(axis + apart);
-#pragma unroll
-            for (int a = 0; a < PPLB200_ROTARY_MAX_AXES; ++a) at.at[a] = (uint64_t)p.positions[min(a, p.axes - 1) * p.axis_stride + r.token];
+            const AxisPositions at = {axis_positions[threadIdx.x / LANES], *reinterpret_cast<const uint32_t*>(axis), *reinterpret_cast<const uint32_t*>(axis + apart)};
             turns_at(r.turns, at, first, first + apart, p.magnitude);
         } else {
             turns_at(r.turns, (uint64_t)p.positions[r.token], first, first + apart, p.magnitude);
