@@ -24,13 +24,21 @@ int32_t tiles_at_once(const PrefixParams& p, int32_t most, int64_t blocks, int64
 // Parts that the prefix is cut into, so that there is a CTA for every SM.
 int32_t splits_of(int64_t items) { return (int32_t)std::max<int64_t>(1, kSms / items); }
 
-// Sums over the parts of the prefix: reference exponents and sums of weights, then sums of values.
-int64_t part_bytes(int64_t rows, int32_t head_dim, int64_t parts) { return round_up(parts * rows * 8, 256) + round_up(parts * rows * head_dim * 4, 256); }
-// As many parts as any kind of cache asks for.
-int64_t most_parts(int64_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
-    const int64_t rows = batch * (q_heads / kv_heads);
-    if (rows <= few_rows(head_dim)) return 1;
-    return splits_of(kv_heads * ((rows + 255) / 256));
+// Workspace: counters of the decode kernel where it goes through the prefix, which have to be zero between calls of whatever sizes; what it needs for the own
+// tokens, which it begins to go through before the other ends; sums over the parts of the prefix, and what the decode kernel needs for few rows' prefix.
+constexpr int64_t kCounters = (3 * kCtas * 8 + 255) / 256 * 256;
+// Reference exponents and sums of weights, then sums of values.
+int64_t part_bytes(int64_t sums, int32_t head_dim) { return round_up(sums * 8, 256) + round_up(sums * head_dim * 4, 256); }
+// Parts as many as any kind of cache asks for.
+int64_t most_parts(int64_t rows, int32_t kv_heads, int32_t head_dim) { return rows <= few_rows(head_dim) ? 1 : splits_of(kv_heads * ((rows + 255) / 256)); }
+// Sums for up to `rows` of a key head: fewer rows can need more, in more parts.
+int64_t most_sums(int64_t rows, int32_t kv_heads) {
+    int64_t most = 0;
+    for (int64_t r = std::min<int64_t>(rows, 256); r > 0; r = std::min(rows, r + 256)) {
+        most = std::max(most, kv_heads * r * splits_of(kv_heads * ((r + 255) / 256)));
+        if (r == rows || r >= 256 * kSms) break; // (one part from there on)
+    }
+    return std::max(most, kv_heads * rows);
 }
 
 // A map of keys or values for boxes of box_rows tokens by 64 dimensions; false where there is none for such strides.
@@ -105,8 +113,9 @@ extern "C" {
 int64_t pplb200_shared_prefix_attention_workspace_bytes(int64_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
     if (batch < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0 || batch > kMaxRows / q_heads) return -1;
     const int32_t shared = q_heads / kv_heads;
-    return std::max(workspace_bytes(shared, head_dim), workspace_bytes(batch * shared, head_dim)) +
-           part_bytes(batch * q_heads, head_dim, most_parts(batch, q_heads, kv_heads, head_dim));
+    const int64_t rows = batch * shared, few = std::min<int64_t>(rows, few_rows(head_dim));
+    return kCounters + workspace_bytes(shared, head_dim) +
+           std::max(part_bytes(most_sums(rows, kv_heads), head_dim), part_bytes(kv_heads * few, head_dim) + workspace_bytes(few, head_dim));
 }
 
 int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache, const pplb200_paged_attention_args* a,
@@ -130,10 +139,11 @@ int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb
     own.units_per_page = 1;
     own.num_units = own.num_pages;
     own.rows_per_head = shared;
-    const int64_t parts = most_parts(a->batch, a->q_heads, cache->kv_heads, cache->head_dim);
+    char* const ws = (char*)a->ws + kCounters;
+    const int64_t sums = most_parts(a->batch * shared, cache->kv_heads, cache->head_dim) * rows;
     own.part_rows = rows;
-    own.part_tops = (float2*)((char*)a->ws + need - part_bytes(rows, cache->head_dim, parts));
-    own.part_sums = (float*)((char*)own.part_tops + round_up(parts * rows * 8, 256));
+    own.part_tops = (float2*)(ws + workspace_bytes(shared, cache->head_dim));
+    own.part_sums = (float*)((char*)own.part_tops + round_up(sums * 8, 256));
     own.parts = 1;
     if (a->batch * shared <= few_rows(cache->head_dim)) {
         // the prefix as one sequence, whose key heads are asked by the rows of all
@@ -145,7 +155,8 @@ int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb
         first.tokens_in_table = prefix->num_pages * cache->page_size;
         first.parts = 0;
         first.keep_parts = true;
-        lay_out(first, a->ws, a->batch * shared);
+        lay_out(first, (char*)own.part_tops + part_bytes(sums, cache->head_dim), a->batch * shared);
+        first.arrived = (uint64_t*)a->ws;
         const int32_t done = launch_general((cudaStream_t)stream, first);
         if (done != RC_SUCCESS) return done;
     } else {
@@ -163,9 +174,9 @@ int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb
         const int32_t done = launch_prefix((cudaStream_t)stream, p);
         if (done != RC_SUCCESS) return done;
         own.parts = p.splits;
-        own.late_wait = true;
     }
-    lay_out(own, a->ws, shared);
+    own.late_wait = true;
+    lay_out(own, ws, shared);
     return launch_general((cudaStream_t)stream, own);
 }
 

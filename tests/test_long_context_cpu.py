@@ -148,6 +148,14 @@ def test_attention_refusals(bad, rc):
     assert c["prefix"](_cache(), **bad) == c["sparse"](_cache(), **bad) == rc and pplb200.last_error()
 
 
+@pytest.mark.parametrize("hq,hk", [(1, 1), (8, 1), (32, 8), (64, 8), (20, 20), (256, 1), (300, 300)])
+@pytest.mark.parametrize("d", [64, 256])
+def test_a_workspace_fits_every_smaller_batch(hq, hk, d):
+    from pplb200 import lib
+    sizes = [lib.pplb200_shared_prefix_attention_workspace_bytes(b, hq, hk, d) for b in list(range(1100)) + list(range(1100, 40000, 997))]
+    assert all(s > 0 and s % 256 == 0 for s in sizes) and sizes == sorted(sizes)
+
+
 @pytest.mark.parametrize("bad,rc", [(dict(pages=0), 4), (dict(length=0), 4), (dict(pages=AT + 2), 4), (dict(length=AT + 1), 4), (dict(num_pages=-1), 4), (dict(num_pages=1 << 40), 2)])
 def test_prefix_refusals(bad, rc):
     import pplb200

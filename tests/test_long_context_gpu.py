@@ -563,6 +563,17 @@ def test_prefix_strided_and_in_place(cuda, pplb200, group):
     assert bool(((few - out[:3]).abs() <= out[:3].abs() * 4 * HALF + 1e-3).all())
 
 
+@pytest.mark.parametrize("hq,hk,d,group", [(8, 2, 128, 0), (8, 1, 64, 64), (32, 1, 256, 8)])
+def test_prefix_batches_of_all_sizes_on_one_workspace(cuda, pplb200, hq, hk, d, group):
+    """One object for them all, in turn: what a large batch leaves in the workspace is nothing to a small one, whose kernels are others."""
+    lengths = [4000, 3, 0, 777, 1200] * 13
+    _, _, _, (att, call, cache) = _run_prefix(cuda, pplb200, 3000, lengths, hq, hk, d, 16, group)
+    for n in (65, 1, 64, 2, 33, 1, 65, 16, 3, 9):
+        mine = pplb200.SharedPrefixDecodeAttention(cache, hq, n, att.max_pages * 16, 3000)
+        part = (call[0][:n], call[1], call[2], call[3][:n], call[4][:n])
+        assert cuda.equal(att(*part), mine(*part)), n
+
+
 # ---- streams, graphs, runs together --------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("group", [0, 8, 128])
