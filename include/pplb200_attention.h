@@ -175,9 +175,9 @@ int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb2
  * above over the prefix's tokens and sequence b's own, of which `lengths` counts and `pages` lists only the latter.  The prefix is read once for the
  * batch.  prefix->pages int32 [prefix->num_pages], prefix->length int32 [1], both on the device: how many tokens (at most num_pages * page_size are
  * looked at); pages that are not in the cache are holes.  A sequence with a length of 0 sees the prefix alone; a negative length stands for a row that is
- * no sequence: zeros and -inf, whatever its q.  As above otherwise, but window has to be 0, at most 2^24 rows of q (batch * q_heads), and where batch * q_heads / kv_heads
- * passes 16 (8 for heads of 256): over the prefix the softmax's weights enter their product with v with 11 bits, and v of int8 rows is rounded to fp16 as that of groups is.
- * ws: pplb200_shared_prefix_attention_workspace_bytes(), with the rules above.
+ * no sequence: zeros and -inf, whatever its q.  As above otherwise, but window has to be 0, at most 2^24 rows of q (batch * q_heads), and over the prefix
+ * the softmax's weights enter their product with v with 11 bits, and v of int8 rows may be rounded to fp16 as that of groups is.
+ * ws: pplb200_shared_prefix_attention_workspace_bytes(), which holds for smaller batches too, with the rules above.
  */
 typedef struct pplb200_shared_prefix {
     const int32_t *pages, *length;
@@ -186,6 +186,12 @@ typedef struct pplb200_shared_prefix {
 int64_t pplb200_shared_prefix_attention_workspace_bytes(int64_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim);
 int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb200_kv_cache* cache,
                                              const pplb200_paged_attention_args* args, const pplb200_shared_prefix* prefix);
+/*
+ * Health word of the kernel that takes a prefix through tensor memory, as pplb200_i8i8_gemm_status is the GEMM's: a wait in it that gives up leaves NaN in
+ * the rows that it was for and a code here.  0 if none has on the current device since the last call with reset != 0; -1 where it cannot be read.  Not to be called
+ * while a stream is being captured; synchronise the streams you launched on first.
+ */
+int32_t pplb200_shared_prefix_attention_status(int32_t reset);
 
 /*
  * Bounds of the keys of blocks of tokens, for choosing among them.  A page has page_size / block blocks, block a multiple of 16; block x of page p is block

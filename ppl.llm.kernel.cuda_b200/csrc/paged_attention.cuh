@@ -125,6 +125,8 @@ void lay_out(AttentionParams& p, void* ws, int64_t shared);
 
 // GENERAL: p with its tables of units and its rows set.
 int32_t launch_general(cudaStream_t stream, AttentionParams& p);
+// How many SMs all its CTAs fill.
+int32_t sms_of_general(AttentionParams& p);
 
 } // namespace paged
 
@@ -966,42 +968,47 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
 }
 
 template <class S>
-int32_t launch(cudaStream_t stream, AttentionParams& p, int64_t tokens) {
+int32_t launch(cudaStream_t stream, AttentionParams& p, int64_t tokens, int32_t* sms) {
     // No more CTAs than there can be work for: the lengths are known on the device only.
     const int64_t steps = std::max<int64_t>(1, (tokens + S::TOKENS - 1) / S::TOKENS), items = p.batch * p.cache.kv_heads * p.tiles;
     const int64_t most = S::CTAS * kSms, ctas = items >= most ? most : std::min(most, std::max(items, items * (steps + kBeginning<S>) / S::WARPS));
     // Items that are short whatever their lengths, and no more than there are CTAs: a CTA each, without looking through the lengths first (64 sequences of 8 heads
-    // behind a prefix: 2 us less).
-    p.whole_items = S::GENERAL && items <= most && 4 * items >= most && steps <= 8 * S::WARPS;
-    launch_ex(paged_attention_kernel<S>, dim3((unsigned)(p.whole_items ? items : ctas)), dim3(S::THREADS), stream, true, p);
+    // behind a prefix: 2 us less); so short that the kernel would find the same.
+    p.whole_items = S::GENERAL && items <= most && (steps + kBeginning<S> <= 4 * S::WARPS || (4 * items >= most && steps <= 8 * S::WARPS));
+    const int64_t grid = p.whole_items ? items : ctas;
+    if (sms) {
+        *sms = (int32_t)((grid + S::CTAS - 1) / S::CTAS);
+        return RC_SUCCESS;
+    }
+    launch_ex(paged_attention_kernel<S>, dim3((unsigned)grid), dim3(S::THREADS), stream, true, p);
     return check_launch("paged attention");
 }
 
 template <int D, int NT, bool PACKED, bool GENERAL>
-int32_t launch_kind(cudaStream_t stream, AttentionParams& p, int64_t tokens) {
-    if (p.cache.quant_group == 0) return launch<Shape<D, CACHE_F16, NT, PACKED, GENERAL>>(stream, p, tokens);
-    if (p.cache.quant_group == 8) return launch<Shape<D, CACHE_I8_GROUPS, NT, PACKED, GENERAL>>(stream, p, tokens);
-    return launch<Shape<D, CACHE_I8_ROWS, NT, PACKED, GENERAL>>(stream, p, tokens);
+int32_t launch_kind(cudaStream_t stream, AttentionParams& p, int64_t tokens, int32_t* sms) {
+    if (p.cache.quant_group == 0) return launch<Shape<D, CACHE_F16, NT, PACKED, GENERAL>>(stream, p, tokens, sms);
+    if (p.cache.quant_group == 8) return launch<Shape<D, CACHE_I8_GROUPS, NT, PACKED, GENERAL>>(stream, p, tokens, sms);
+    return launch<Shape<D, CACHE_I8_ROWS, NT, PACKED, GENERAL>>(stream, p, tokens, sms);
 }
 template <int D, bool PACKED, bool GENERAL>
-int32_t launch_heads(cudaStream_t stream, AttentionParams& p, int64_t tokens) {
+int32_t launch_heads(cudaStream_t stream, AttentionParams& p, int64_t tokens, int32_t* sms) {
     if constexpr (D <= 128)
-        if (heads_at_once(D, p.shared) == 16) return launch_kind<D, 2, PACKED, GENERAL>(stream, p, tokens);
-    return launch_kind<D, 1, PACKED, GENERAL>(stream, p, tokens);
+        if (heads_at_once(D, p.shared) == 16) return launch_kind<D, 2, PACKED, GENERAL>(stream, p, tokens, sms);
+    return launch_kind<D, 1, PACKED, GENERAL>(stream, p, tokens, sms);
 }
 template <int D, bool GENERAL>
-int32_t launch_dim(cudaStream_t stream, AttentionParams& p, int64_t tokens, bool packed) {
-    return packed ? launch_heads<D, true, GENERAL>(stream, p, tokens) : launch_heads<D, false, GENERAL>(stream, p, tokens);
+int32_t launch_dim(cudaStream_t stream, AttentionParams& p, int64_t tokens, bool packed, int32_t* sms) {
+    return packed ? launch_heads<D, true, GENERAL>(stream, p, tokens, sms) : launch_heads<D, false, GENERAL>(stream, p, tokens, sms);
 }
 
 template <bool GENERAL>
-int32_t launch_attention(cudaStream_t s, AttentionParams& p) {
+int32_t launch_attention(cudaStream_t s, AttentionParams& p, int32_t* sms = nullptr) {
     const int32_t D = p.cache.head_dim;
     const bool packed = p.cache.page_size % 16 == 0 && p.cache.token_stride == D && (p.cache.quant_group != 8 || p.cache.scale_token_stride == D / 8);
-    if (D == 64) return launch_dim<64, GENERAL>(s, p, p.tokens_in_table, packed);
-    if (D == 96) return launch_dim<96, GENERAL>(s, p, p.tokens_in_table, packed);
-    if (D == 128) return launch_dim<128, GENERAL>(s, p, p.tokens_in_table, packed);
-    return launch_dim<256, GENERAL>(s, p, p.tokens_in_table, packed);
+    if (D == 64) return launch_dim<64, GENERAL>(s, p, p.tokens_in_table, packed, sms);
+    if (D == 96) return launch_dim<96, GENERAL>(s, p, p.tokens_in_table, packed, sms);
+    if (D == 128) return launch_dim<128, GENERAL>(s, p, p.tokens_in_table, packed, sms);
+    return launch_dim<256, GENERAL>(s, p, p.tokens_in_table, packed, sms);
 }
 
 } // namespace

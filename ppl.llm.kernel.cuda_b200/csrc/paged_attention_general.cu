@@ -4,6 +4,12 @@
 namespace pplb200 {
 namespace paged {
 
+int32_t sms_of_general(AttentionParams& p) {
+    int32_t sms = 0;
+    launch_attention<true>(nullptr, p, &sms);
+    return sms;
+}
+
 int32_t launch_general(cudaStream_t stream, AttentionParams& p) {
     small_division(p.unit_tokens, p.page_magic, p.page_shift);
     small_division(p.units_per_page, p.unit_magic, p.unit_shift);

@@ -2,6 +2,7 @@
 // own tokens, whose sums are joined with the prefix's where the output is written.
 #include "shared_prefix.cuh"
 
+#include <cmath>
 #include <cuda.h>
 
 namespace pplb200 {
@@ -11,9 +12,6 @@ using namespace prefix;
 
 constexpr int64_t kMaxRows = 1 << 24;
 
-// Rows of a key head up to which the decode kernel, whose matrix instructions take 8 or 16 of them at once, goes through the prefix.
-int32_t few_rows(int32_t head_dim) { return head_dim <= 128 ? 16 : 8; }
-
 // Tiles of rows that a CTA takes at once.  Two share what is loaded, but leave twice as many sums to be joined: one, unless a CTA then had many blocks of a prefix to go
 // through that is not to be had from L2 (256 rows of 8 heads over 1, 4096 and 32768 tokens: 19 and 47 us with one, 22 and 49 with two; 512 rows of 64 over 8, 4096, 12345 and
 // 32768 tokens: 28, 47, 89 and 32, 47, 84).
@@ -21,21 +19,36 @@ int32_t tiles_at_once(const PrefixParams& p, int32_t most, int64_t blocks, int64
     const int64_t tiles = (p.rows + 127) / 128, ctas = std::max<int64_t>(1, kSms / (p.cache.kv_heads * tiles));
     return most == 2 && tiles > 1 && (tiles % 2 == 0 || tiles >= 7) && blocks > 24 * ctas && bytes > (64LL << 20) ? 2 : 1;
 }
-// Parts that the prefix is cut into, so that there is a CTA for every SM.
-int32_t splits_of(int64_t items) { return (int32_t)std::max<int64_t>(1, kSms / items); }
+// Parts that the prefix is cut into: at most so many that there is a CTA for every SM.
+int32_t most_splits(int64_t items) { return (int32_t)std::max<int64_t>(1, kSms / items); }
+// Joining the parts costs about an eighth of a block each, which the square root balances (64 rows of one head, 32768 tokens: 22 us with 46 parts, 41 with 148).  The
+// kernel for the own tokens fills `own_sms` SMs, and where these are left to it, it runs beside this one: up to four blocks a CTA more are worth it
+// (16 rows of 8 heads, 4096 tokens: 13.2 us with 14 parts, 17.8 with 17; 128 rows of 8, 4096 tokens and 700 of int8 each: 23 with 8, 37 with 18).
+int32_t splits_of(int64_t items, int64_t own_sms, int64_t blocks) {
+    const int64_t all = std::min<int64_t>({most_splits(items), blocks, std::max<int64_t>(8, (int64_t)std::sqrt(8.0 * (double)blocks) + 1)});
+    const int64_t spared = std::min(all, (kSms - own_sms) / items);
+    return (int32_t)(spared > 0 && (blocks + spared - 1) / spared <= (blocks + all - 1) / all + 4 ? spared : all);
+}
+
+// Few rows of an int8 cache: the decode kernel, whose matrix instructions take 8 or 16 at once, widens with all of its warps, and is faster where there are
+// several blocks for a CTA (8 rows of 8 heads over 4096, 8000 and 32768 tokens of int8 rows: 15.8, 18.0, 28.5 us and 15.5, 19.2, 43; 16 rows of groups of 8 over
+// 8000 and 32768: 22, 38 and 20, 51.  In fp16 8 rows 18.0, 32.4 and 16.2, 31.2).
+constexpr int32_t kFewRows = 16;
+bool by_decode(int64_t rows, const pplb200_kv_cache& c, int64_t tokens, int64_t own_sms) {
+    const int64_t nb = c.head_dim == 256 ? 64 : 128, blocks = std::max<int64_t>(1, (tokens + nb - 1) / nb);
+    return c.quant_group && rows <= kFewRows && blocks > splits_of(c.kv_heads, own_sms, blocks) * (rows <= 8 ? 3LL : 6LL);
+}
 
 // Workspace: counters of the decode kernel where it goes through the prefix, which have to be zero between calls of whatever sizes; what it needs for the own
 // tokens, which it begins to go through before the other ends; sums over the parts of the prefix, and what the decode kernel needs for few rows' prefix.
 constexpr int64_t kCounters = (3 * kCtas * 8 + 255) / 256 * 256;
 // Reference exponents and sums of weights, then sums of values.
 int64_t part_bytes(int64_t sums, int32_t head_dim) { return round_up(sums * 8, 256) + round_up(sums * head_dim * 4, 256); }
-// Parts as many as any kind of cache asks for.
-int64_t most_parts(int64_t rows, int32_t kv_heads, int32_t head_dim) { return rows <= few_rows(head_dim) ? 1 : splits_of(kv_heads * ((rows + 255) / 256)); }
 // Sums for up to `rows` of a key head: fewer rows can need more, in more parts.
 int64_t most_sums(int64_t rows, int32_t kv_heads) {
     int64_t most = 0;
     for (int64_t r = std::min<int64_t>(rows, 256); r > 0; r = std::min(rows, r + 256)) {
-        most = std::max(most, kv_heads * r * splits_of(kv_heads * ((r + 255) / 256)));
+        most = std::max(most, kv_heads * r * most_splits(kv_heads * ((r + 255) / 256)));
         if (r == rows || r >= 256 * kSms) break; // (one part from there on)
     }
     return std::max(most, kv_heads * rows);
@@ -69,7 +82,7 @@ int32_t launch_tiles(cudaStream_t stream, PrefixParams& p) {
     const int64_t blocks = std::max<int64_t>(1, (p.tokens_in_table + T::NB - 1) / T::NB);
     p.tiles = tiles_at_once(p, T::TILES, blocks, p.tokens_in_table * p.cache.kv_heads * D * 2 * T::ES);
     p.items = p.cache.kv_heads * (int32_t)((p.rows + p.tiles * 128 - 1) / (p.tiles * 128));
-    p.splits = (int32_t)std::min<int64_t>(splits_of(p.items), blocks);
+    p.splits = splits_of(p.items, p.own_sms, blocks);
     p.box_rows = 0;
     if (KIND == CACHE_F16 && p.cache.page_size % 16 == 0 && p.cache.num_pages > 0) {
         const int32_t rows = std::min(p.cache.page_size & -p.cache.page_size, T::NB);
@@ -113,7 +126,7 @@ extern "C" {
 int64_t pplb200_shared_prefix_attention_workspace_bytes(int64_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
     if (batch < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0 || batch > kMaxRows / q_heads) return -1;
     const int32_t shared = q_heads / kv_heads;
-    const int64_t rows = batch * shared, few = std::min<int64_t>(rows, few_rows(head_dim));
+    const int64_t rows = batch * shared, few = std::min<int64_t>(rows, kFewRows);
     return kCounters + workspace_bytes(shared, head_dim) +
            std::max(part_bytes(most_sums(rows, kv_heads), head_dim), part_bytes(kv_heads * few, head_dim) + workspace_bytes(few, head_dim));
 }
@@ -134,26 +147,31 @@ int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb
     if (!a->ws || a->ws_bytes < need || ((uintptr_t)a->ws & 255))
         return fail(RC_INVALID_VALUE, "workspace of %lld bytes (256-byte aligned) needed, got %lld", (long long)need, (long long)a->ws_bytes);
     const int32_t shared = a->q_heads / cache->kv_heads;
-    const int64_t rows = a->batch * a->q_heads;
+    const int64_t rows = a->batch * a->q_heads, tokens = prefix->num_pages * cache->page_size;
+    char* const ws = (char*)a->ws + kCounters;
     own.unit_tokens = cache->page_size;
     own.units_per_page = 1;
     own.num_units = own.num_pages;
     own.rows_per_head = shared;
-    char* const ws = (char*)a->ws + kCounters;
-    const int64_t sums = most_parts(a->batch * shared, cache->kv_heads, cache->head_dim) * rows;
     own.part_rows = rows;
+    own.parts = 1;
+    own.late_wait = true;
+    lay_out(own, ws, shared);
+    const int32_t own_sms = sms_of_general(own);
+    const bool decode = by_decode(a->batch * shared, *cache, tokens, own_sms);
+    const int64_t sums = decode ? rows : rows * most_splits(cache->kv_heads * ((a->batch * shared + 255) / 256));
     own.part_tops = (float2*)(ws + workspace_bytes(shared, cache->head_dim));
     own.part_sums = (float*)((char*)own.part_tops + round_up(sums * 8, 256));
-    own.parts = 1;
-    if (a->batch * shared <= few_rows(cache->head_dim)) {
+    if (decode) {
         // the prefix as one sequence, whose key heads are asked by the rows of all
         AttentionParams first = own;
         first.batch = 1;
         first.pages = prefix->pages;
         first.lengths = prefix->length;
         first.pages_stride = prefix->num_pages;
-        first.tokens_in_table = prefix->num_pages * cache->page_size;
+        first.tokens_in_table = tokens;
         first.parts = 0;
+        first.late_wait = false;
         first.keep_parts = true;
         lay_out(first, (char*)own.part_tops + part_bytes(sums, cache->head_dim), a->batch * shared);
         first.arrived = (uint64_t*)a->ws;
@@ -163,21 +181,34 @@ int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb
         PrefixParams p = {};
         p.q = own.q; p.q_stride = own.q_stride;
         p.pages = prefix->pages; p.length = prefix->length;
-        p.tokens_in_table = prefix->num_pages * cache->page_size;
+        p.tokens_in_table = tokens;
         p.num_pages = own.num_pages; p.rows = (int32_t)(a->batch * shared);
         p.rows_per_head = shared; p.q_heads = a->q_heads;
         small_division(shared, p.rows_magic, p.rows_shift);
         small_division(cache->page_size, p.page_magic, p.page_shift);
         p.scale_log2 = own.scale_log2;
+        p.own_sms = own_sms;
         p.cache = *cache;
         p.part_rows = rows; p.part_tops = own.part_tops; p.part_sums = own.part_sums;
         const int32_t done = launch_prefix((cudaStream_t)stream, p);
         if (done != RC_SUCCESS) return done;
         own.parts = p.splits;
     }
-    own.late_wait = true;
-    lay_out(own, ws, shared);
     return launch_general((cudaStream_t)stream, own);
+}
+
+int32_t pplb200_shared_prefix_attention_status(int32_t reset) {
+    void* word = nullptr;
+    cudaStream_t mine; // no other stream of the device is waited for
+    if (cudaGetSymbolAddress(&word, g_status) != cudaSuccess || cudaStreamCreateWithFlags(&mine, cudaStreamNonBlocking) != cudaSuccess) {
+        cudaGetLastError();
+        return -1;
+    }
+    unsigned int v = 0;
+    bool ok = cudaMemcpyAsync(&v, word, sizeof(v), cudaMemcpyDeviceToHost, mine) == cudaSuccess && cudaStreamSynchronize(mine) == cudaSuccess;
+    if (ok && reset && v) ok = cudaMemsetAsync(word, 0, sizeof(v), mine) == cudaSuccess && cudaStreamSynchronize(mine) == cudaSuccess;
+    cudaStreamDestroy(mine);
+    return ok ? (int32_t)v : -1;
 }
 
 } // extern "C"

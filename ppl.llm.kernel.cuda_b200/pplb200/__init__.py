@@ -679,7 +679,8 @@ def stream_read_probe(sizes=(16 << 20, 48 << 20, 384 << 20), pool_bytes=1536 << 
 
 
 _ATTENTION = ("BlockSparseDecodeAttention", "KeyBlockBounds", "PagedDecodeAttention", "PagedKVCache", "RotaryTable", "SharedPrefixDecodeAttention",
-              "key_bounds_read", "key_bounds_update", "kv_cache_read", "kv_cache_write", "rotary_fp16", "rotary_kv_cache_write")
+              "key_bounds_read", "key_bounds_update", "kv_cache_read", "kv_cache_write", "rotary_fp16", "rotary_kv_cache_write",
+              "shared_prefix_status")
 
 
 def __getattr__(name):

@@ -20,6 +20,7 @@ EXPORTS = [
     "pplb200_paged_attention_offset",
     "pplb200_rotary_axes_frequencies", "pplb200_rotary_axes_fp16", "pplb200_kv_cache_write_axes_fp16",
     "pplb200_shared_prefix_attention_workspace_bytes", "pplb200_shared_prefix_attention_fp16",
+    "pplb200_shared_prefix_attention_status",
     "pplb200_key_bounds_update", "pplb200_key_bounds_read",
     "pplb200_block_sparse_attention_workspace_bytes", "pplb200_block_sparse_attention_fp16",
 ]
@@ -46,6 +47,7 @@ lib.pplb200_key_bounds_read.argtypes = [_vp, _blk, _blk, _vp, _i64, _vp, _vp]
 lib.pplb200_block_sparse_attention_workspace_bytes.argtypes = [_i64, _i32, _i32, _i32, _i32]
 lib.pplb200_block_sparse_attention_workspace_bytes.restype = _i64
 lib.pplb200_block_sparse_attention_fp16.argtypes = [_vp, _blk, _blk, _blk, _blk]
+lib.pplb200_shared_prefix_attention_status.argtypes = [_i32]
 
 _pack_cache = struct.Struct("=4Q7q4i").pack
 
@@ -274,6 +276,11 @@ class SharedPrefixDecodeAttention(_LaidOutOnce):
         if rc:
             raise PplError(rc)
         return out
+
+
+def shared_prefix_status(reset=True):
+    """0, unless a wait inside a kernel of SharedPrefixDecodeAttention has given up on this device, leaving NaN; synchronise first."""
+    return lib.pplb200_shared_prefix_attention_status(1 if reset else 0)
 
 
 class KeyBlockBounds(_LaidOutOnce):

@@ -219,6 +219,13 @@ def test_null_blocks():
     assert lib.pplb200_key_bounds_update(None, _cache(), None, AT, 4) == lib.pplb200_key_bounds_read(None, _cache(), None, AT, 4, AT, AT) == 4
 
 
+def test_status_without_a_device():
+    import pplb200
+    import torch
+    if not torch.cuda.is_available():
+        assert pplb200.shared_prefix_status() == -1
+
+
 # ---- the binding: types, shapes and devices (the tensors are on the CPU, which is never the current device) ---------
 
 @pytest.fixture

@@ -574,6 +574,12 @@ def test_prefix_batches_of_all_sizes_on_one_workspace(cuda, pplb200, hq, hk, d, 
         assert cuda.equal(att(*part), mine(*part)), n
 
 
+def test_no_wait_has_given_up(cuda, pplb200):
+    _run_prefix(cuda, pplb200, 400, [5] * 20, 4, 1, 64, 16, 0)
+    cuda.cuda.synchronize()
+    assert pplb200.shared_prefix_status(reset=False) == 0 == pplb200.shared_prefix_status()
+
+
 # ---- streams, graphs, runs together --------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("group", [0, 8, 128])
