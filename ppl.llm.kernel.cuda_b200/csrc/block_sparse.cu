@@ -21,9 +21,12 @@ __device__ __forceinline__ half outer_scale(float amax) {
 __device__ __forceinline__ bool is_finite(half s) { return (__half_as_ushort(s) & 0x7c00u) != 0x7c00u; }
 
 // ---- bounds ------------------------------------------------------------------------------------------------------------
-// A CTA looks through a few slots for those that end a block; its warps then take these blocks, a head each: head_dim / 8 lanes have a token's row, eight
-// dimensions a lane, and as many rows are on their way as eight loads a lane bring.  Nothing is shared but the warp's last few shuffles.
-// Bound by HBM in a long prompt, the keys once (16384 tokens of 8 heads of 128 in fp16, blocks of 64: FIGURE); by look-ups in a decode step.
+// A CTA looks through a few slots for those that end a block; its warps then take these blocks, a head each: a lane has 16 bytes of a token's row, and eight loads are on
+// their way.  The lanes that have the same dimensions of different rows halve them between each other at the end, so that all divide and write.  Nothing is
+// shared but these shuffles.
+// In fp16 bound by HBM in a long prompt, the keys once (131072 tokens of 8 heads of 128, blocks of 64: 48 us, 5.6 TB/s), int8 by the minima and maxima, which are
+// in fp32 as the products are, of three numbers at a time (45 us, groups of 8 48; of two numbers 51 and 58; with eight bytes a lane 53 and 59).  16384 tokens: 8.2, 9.0 and
+// 8.9 us; in a decode step look-ups and the launch, 3 us.
 constexpr int BWARPS = 4, BTPB = 32 * BWARPS;
 struct BoundsParams {
     pplb200_kv_cache cache;
@@ -35,9 +38,30 @@ struct BoundsParams {
     uint32_t block_magic, block_shift;
 };
 
+__device__ __forceinline__ float least(float a, float b, float c) {
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float greatest(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// Bytes `at` and at + 1 of four int8 values, times a scale.  A byte without its sign in the last bits of 2^23 is that number more, exactly; conversions have a
+// quarter of the rate.
+__device__ __forceinline__ float2 products(uint32_t values, int at, float scale) {
+    const uint32_t u = values ^ 0x80808080u;
+    const float2 whole = ptx::add2(make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 + at)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7541 + at))),
+                                   make_float2(-8388736.0f, -8388736.0f));
+    return ptx::mul2(whole, make_float2(scale, scale));
+}
+
 template <int D, int KIND>
 __global__ void __launch_bounds__(BTPB) key_bounds_kernel(const __grid_constant__ BoundsParams p) {
-    constexpr int LANES = D / 8, ROWS = 32 / LANES, BATCH = 8; // of a row; rows at once; loads on their way
+    constexpr int PER = KIND == CACHE_F16 ? 8 : 16, LANES = D / PER;   // dimensions of a lane, and lanes of a row
+    constexpr int ROWS = D == 96 ? 24 / LANES : 32 / LANES, BATCH = 8; // rows at once (a power of two); loads on their way
+    constexpr int LEFT = PER / ROWS, GROUPS = KIND == CACHE_I8_GROUPS ? PER / 8 : 1;
     struct Block {
         int64_t page;
         int32_t x;
@@ -66,9 +90,9 @@ __global__ void __launch_bounds__(BTPB) key_bounds_kernel(const __grid_constant_
     for (int i = 0; i < found; ++i) {
         const int64_t page = block_of[i].page;
         const int32_t x = block_of[i].x, token0 = x * p.block + (active ? row : 0);
-        const int64_t at = kv_row(page, token0, head, c.page_stride, c.head_stride, c.token_stride) + part * 8;
-        const int64_t scale_at = kv_row(page, token0, head, c.scale_page_stride, c.scale_head_stride, c.scale_token_stride) + (KIND == CACHE_I8_GROUPS ? part : 0);
-        float lo[8], hi[8];
+        const int64_t at = kv_row(page, token0, head, c.page_stride, c.head_stride, c.token_stride) + part * PER;
+        const int64_t scale_at = kv_row(page, token0, head, c.scale_page_stride, c.scale_head_stride, c.scale_token_stride) + (KIND == CACHE_I8_GROUPS ? part * GROUPS : 0);
+        float lo[PER], hi[PER];
         bool bad = false; // a scale that is infinite or NaN; of fp16 keys, these come through in the bounds
         if constexpr (KIND == CACHE_F16) {
             __half2 l[4], h[4];
@@ -97,58 +121,78 @@ __global__ void __launch_bounds__(BTPB) key_bounds_kernel(const __grid_constant_
             for (int d = 0; d < 8; ++d) bad |= !(fabsf(lo[d]) < INFINITY) || !(fabsf(hi[d]) < INFINITY);
         } else {
 #pragma unroll
-            for (int d = 0; d < 8; ++d) lo[d] = INFINITY, hi[d] = -INFINITY;
+            for (int d = 0; d < PER; ++d) lo[d] = INFINITY, hi[d] = -INFINITY;
             for (int32_t t = 0; t < p.block; t += BATCH * ROWS) {
-                uint2 w[BATCH];
-                half s[BATCH];
+                uint4 w[BATCH];
+                half s[BATCH][GROUPS];
 #pragma unroll
                 for (int k = 0; k < BATCH; ++k)
                     if (t + k * ROWS < p.block) {
-                        asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(w[k].x), "=r"(w[k].y) : "l"((const int8_t*)c.k + at + (t + k * ROWS) * c.token_stride));
-                        s[k] = ld_global_half((const half*)c.k_scale + scale_at + (t + k * ROWS) * c.scale_token_stride);
+                        w[k] = ld_global_16((const int8_t*)c.k + at + (t + k * ROWS) * c.token_stride);
+#pragma unroll
+                        for (int x = 0; x < GROUPS; ++x) s[k][x] = ld_global_half((const half*)c.k_scale + scale_at + (t + k * ROWS) * c.scale_token_stride + x);
                     }
 #pragma unroll
-                for (int k = 0; k < BATCH; ++k)
-                    if (t + k * ROWS < p.block) {
-                        bad |= !is_finite(s[k]);
-                        const float f = __half2float(s[k]);
+                for (int k = 0; k < BATCH; k += 2)
+                    if (t + k * ROWS < p.block) { // both rows, or (16 tokens at eight rows at once: one load) the same one twice
+                        const bool both = t + (k + 1) * ROWS < p.block;
+                        const uint4 second = both ? w[k + 1] : w[k];
+                        const uint32_t words[2][4] = {{w[k].x, w[k].y, w[k].z, w[k].w}, {second.x, second.y, second.z, second.w}};
+                        half scales[2][GROUPS];
 #pragma unroll
-                        for (int d = 0; d < 8; ++d) {
-                            const float v = (float)(int8_t)((d < 4 ? w[k].x : w[k].y) >> (8 * (d & 3))) * f;
-                            lo[d] = fminf(lo[d], v);
-                            hi[d] = fmaxf(hi[d], v);
+                        for (int x = 0; x < GROUPS; ++x) {
+                            scales[0][x] = s[k][x];
+                            scales[1][x] = both ? s[k + 1][x] : s[k][x];
+                            bad |= !is_finite(scales[0][x]) || !is_finite(scales[1][x]);
+                        }
+#pragma unroll
+                        for (int d = 0; d < PER; d += 2) {
+                            const float2 a = products(words[0][d >> 2], d & 2, __half2float(scales[0][GROUPS == 1 ? 0 : d / 8]));
+                            const float2 b = products(words[1][d >> 2], d & 2, __half2float(scales[1][GROUPS == 1 ? 0 : d / 8]));
+                            lo[d] = least(lo[d], a.x, b.x);
+                            hi[d] = greatest(hi[d], a.x, b.x);
+                            lo[d + 1] = least(lo[d + 1], a.y, b.y);
+                            hi[d + 1] = greatest(hi[d + 1], a.y, b.y);
                         }
                     }
             }
         }
-        // the other rows' bounds of these dimensions
+        // Two rows exchange halves of their dimensions, until each is left with LEFT of them.
+        int mine = part * PER;
 #pragma unroll
-        for (int r = 1; r < ROWS; r <<= 1)
+        for (int r = 1, half_of = PER / 2; r < ROWS; r <<= 1, half_of >>= 1) {
+            const bool upper = row & r;
+            const int other = active ? part + (row ^ r) * LANES : lane;
+            mine += upper ? half_of : 0;
 #pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                lo[d] = fminf(lo[d], __shfl_down_sync(0xffffffffu, lo[d], r * LANES));
-                hi[d] = fmaxf(hi[d], __shfl_down_sync(0xffffffffu, hi[d], r * LANES));
+            for (int d = 0; d < half_of; ++d) {
+                const float l = __shfl_sync(0xffffffffu, upper ? lo[d] : lo[d + half_of], other), h = __shfl_sync(0xffffffffu, upper ? hi[d] : hi[d + half_of], other);
+                lo[d] = fminf(upper ? lo[d + half_of] : lo[d], l);
+                hi[d] = fmaxf(upper ? hi[d + half_of] : hi[d], h);
             }
+        }
         const bool lost_key = __any_sync(0xffffffffu, bad && active);
         float amax = 0.0f;
 #pragma unroll
-        for (int d = 0; d < 8; ++d) amax = fmaxf(amax, fmaxf(fabsf(lo[d]), fabsf(hi[d])));
-        amax = __uint_as_float(__reduce_max_sync(0xffffffffu, row == 0 ? __float_as_uint(amax) : 0u));
+        for (int d = 0; d < LEFT; ++d) amax = fmaxf(amax, fmaxf(fabsf(lo[d]), fabsf(hi[d])));
+        amax = __uint_as_float(__reduce_max_sync(0xffffffffu, active ? __float_as_uint(amax) : 0u));
         half s = outer_scale(amax);
         const bool lost = lost_key || !is_finite(s);
         if (lost) s = __ushort_as_half(0x7c00);
         const float step = __half2float(s);
-        uint32_t l[2] = {}, h[2] = {};
+        uint64_t l = 0, h = 0;
 #pragma unroll
-        for (int d = 0; d < 8; ++d) {
+        for (int d = 0; d < LEFT; ++d) {
             const int a = lost ? 0 : (int)floorf(__fdiv_rn(lo[d], step)), b = lost ? 0 : (int)ceilf(__fdiv_rn(hi[d], step));
-            l[d >> 2] |= (uint32_t)(a & 0xff) << (8 * (d & 3));
-            h[d >> 2] |= (uint32_t)(b & 0xff) << (8 * (d & 3));
+            l |= (uint64_t)(a & 0xff) << (8 * d);
+            h |= (uint64_t)(b & 0xff) << (8 * d);
         }
-        if (row == 0) {
+        if (active) {
+            using Piece = std::conditional_t<LEFT == 2, uint16_t, std::conditional_t<LEFT == 4, uint32_t, uint64_t>>;
+            static_assert(sizeof(Piece) == LEFT);
             const int64_t of = (page * c.kv_heads + head) * p.per_page + x;
-            *reinterpret_cast<uint2*>(p.bounds + of * 2 * D + part * 8) = make_uint2(l[0], l[1]);
-            *reinterpret_cast<uint2*>(p.bounds + (of * 2 + 1) * D + part * 8) = make_uint2(h[0], h[1]);
+            *reinterpret_cast<Piece*>(p.bounds + of * 2 * D + mine) = (Piece)l;
+            *reinterpret_cast<Piece*>(p.bounds + (of * 2 + 1) * D + mine) = (Piece)h;
             if (lane == 0) p.scale[of] = s;
         }
     }
