@@ -972,9 +972,11 @@ int32_t launch(cudaStream_t stream, AttentionParams& p, int64_t tokens, int32_t*
     // No more CTAs than there can be work for: the lengths are known on the device only.
     const int64_t steps = std::max<int64_t>(1, (tokens + S::TOKENS - 1) / S::TOKENS), items = p.batch * p.cache.kv_heads * p.tiles;
     const int64_t most = S::CTAS * kSms, ctas = items >= most ? most : std::min(most, std::max(items, items * (steps + kBeginning<S>) / S::WARPS));
-    // Items that are short whatever their lengths, and no more than there are CTAs: a CTA each, without looking through the lengths first (64 sequences of 8 heads
-    // behind a prefix: 2 us less); so short that the kernel would find the same.
-    p.whole_items = S::GENERAL && items <= most && (steps + kBeginning<S> <= 4 * S::WARPS || (4 * items >= most && steps <= 8 * S::WARPS));
+    // Items that are short whatever their lengths: a CTA each, of which there may be more than the device holds at once, without looking through the lengths first; so short
+    // that the kernel would find the same, or so many that the longest of them cannot hold up the others by more than joining them would take.  In fp16, heads of 128, behind
+    // 1000 tokens: 64 sequences of 8 heads with 100 tokens each 25.7 us, 31.2 if shared out; 600 of one head with 500 49, 59; 256 of 8 with up to 1500 217, 223; but 64 of 8
+    // with up to 1500 78, 67.
+    p.whole_items = S::GENERAL && (steps + kBeginning<S> <= 4 * S::WARPS || (4 * items >= most && steps * most <= 8 * S::WARPS * std::max(items, most)));
     const int64_t grid = p.whole_items ? items : ctas;
     if (sms) {
         *sms = (int32_t)((grid + S::CTAS - 1) / S::CTAS);
