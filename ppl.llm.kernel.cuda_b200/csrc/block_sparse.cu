@@ -750,11 +750,13 @@ int32_t pplb200_block_sparse_attention_fp16(pplb200_stream_t stream, const pplb2
     p.first = choice->first; p.last = choice->last; p.top = choice->top; p.total = (int32_t)total;
     small_division(p.block, p.block_magic, p.block_shift);
     small_division(p.per_page, p.page_magic, p.page_shift);
-    // Sixteen warps a CTA where there are few choices, which then take 512 blocks in one round of loads; four for many or short ones, so that several share
-    // an SM.  Clusters, whose barriers cost a microsecond each, only where a CTA would have more rounds to go, and for room for the scores (128 KB).
+    // Sixteen warps a CTA where there are few choices, which then take 512 blocks in one round of loads (whole calls, one sequence, 8 key heads: 1024 blocks 26 us, with four
+    // warps 33; 16 sequences, 375 blocks 36, 40); four for many or short ones, so that several share an SM (64 sequences, 250 blocks 91, with sixteen 96; 16 of 63
+    // 29, 35).  Clusters, whose barriers cost a microsecond each, only where a CTA would have more rounds to go (32 choices of 257 blocks 17 us, by four CTAs each 21; 8 of 2048
+    // by one CTA each 34, by eight 27), and for room for the scores (128 KB).
     const bool wide = p.items <= kSms && in_table > 128;
     int32_t cluster = 1;
-    while (cluster < MAX_CLUSTER && ((p.items * cluster * 2 <= kSms && in_table > cluster * 512) || in_table > cluster * 32768LL)) cluster *= 2;
+    while (cluster < MAX_CLUSTER && ((p.items * cluster * 2 <= kSms && in_table > 512 && in_table > cluster * 128) || in_table > cluster * 32768LL)) cluster *= 2;
     p.share = (int32_t)std::max<int64_t>(16, (in_table + cluster * 16 - 1) / (cluster * 16) * 16);
     p.gathered = cluster > 1 && (int64_t)p.share * cluster <= 16384;
     p.kept_keys = p.gathered ? p.share * cluster : p.share;

@@ -12,12 +12,13 @@ using namespace prefix;
 
 constexpr int64_t kMaxRows = 1 << 24;
 
-// Tiles of rows that a CTA takes at once.  Two share what is loaded, but leave twice as many sums to be joined: one, unless a CTA then had many blocks of a prefix to go
-// through that is not to be had from L2 (256 rows of 8 heads over 1, 4096 and 32768 tokens: 19 and 47 us with one, 22 and 49 with two; 512 rows of 64 over 8, 4096, 12345 and
-// 32768 tokens: 28, 47, 89 and 32, 47, 84).
-int32_t tiles_at_once(const PrefixParams& p, int32_t most, int64_t blocks, int64_t bytes) {
+// Tiles of rows that a CTA takes at once.  Two share what is loaded, and widened, but leave twice as many sums to be joined: where a CTA with one would have many blocks to go
+// through, fewer where a block's products take less than its loads.  64 heads over 8; one and two tiles, us: fp16 heads of 128, 64 sequences, 24 and 64 blocks a CTA, 51, 92 and
+// 54, 88; 128 sequences, 48 blocks, 86 and 86; int8 rows, 24 and 64 blocks, 67, 136 and 63, 118; 11 blocks 40.2 and 40.6; fp16 heads of 64, 8 and 24 blocks, 21, 38 and 22, 36.
+int32_t tiles_at_once(const PrefixParams& p, int32_t most, int64_t blocks) {
     const int64_t tiles = (p.rows + 127) / 128, ctas = std::max<int64_t>(1, kSms / (p.cache.kv_heads * tiles));
-    return most == 2 && tiles > 1 && (tiles % 2 == 0 || tiles >= 7) && blocks > 24 * ctas && bytes > (64LL << 20) ? 2 : 1;
+    const int64_t enough = p.cache.quant_group == 0 && p.cache.head_dim > 64 ? 40 : 16;
+    return most == 2 && tiles > 1 && (tiles % 2 == 0 || tiles >= 7) && blocks > enough * ctas ? 2 : 1;
 }
 // Parts that the prefix is cut into: at most so many that there is a CTA for every SM.
 int32_t most_splits(int64_t items) { return (int32_t)std::max<int64_t>(1, kSms / items); }
@@ -80,7 +81,7 @@ int32_t launch_tiles(cudaStream_t stream, PrefixParams& p) {
     using T = Tile<D, KIND>;
     static_assert(T::SMEM + 18 * 1024 <= 232448);
     const int64_t blocks = std::max<int64_t>(1, (p.tokens_in_table + T::NB - 1) / T::NB);
-    p.tiles = tiles_at_once(p, T::TILES, blocks, p.tokens_in_table * p.cache.kv_heads * D * 2 * T::ES);
+    p.tiles = tiles_at_once(p, T::TILES, blocks);
     p.items = p.cache.kv_heads * (int32_t)((p.rows + p.tiles * 128 - 1) / (p.tiles * 128));
     p.splits = splits_of(p.items, p.own_sms, blocks);
     p.box_rows = 0;
