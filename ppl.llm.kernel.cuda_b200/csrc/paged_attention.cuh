@@ -97,7 +97,8 @@ struct AttentionParams {
     int32_t parts;                             // sums of earlier calls that are joined
     bool keep_parts;                           // leave the sums, as part 0
     bool late_wait;
-    bool whole_items; // as many CTAs as items, one each
+    bool whole_items;     // as many CTAs as items, one each
+    int64_t whole_tokens; // for items of no more
     int64_t part_rows;                         // rows of a part: query heads of all sequences
     float2* part_tops;                         // [parts][part_rows]
     float* part_sums;                          // [parts][part_rows][D]
@@ -973,10 +974,11 @@ int32_t launch(cudaStream_t stream, AttentionParams& p, int64_t tokens, int32_t*
     const int64_t steps = std::max<int64_t>(1, (tokens + S::TOKENS - 1) / S::TOKENS), items = p.batch * p.cache.kv_heads * p.tiles;
     const int64_t most = S::CTAS * kSms, ctas = items >= most ? most : std::min(most, std::max(items, items * (steps + kBeginning<S>) / S::WARPS));
     // Items that are short whatever their lengths: a CTA each, of which there may be more than the device holds at once, without looking through the lengths first; so short
-    // that the kernel would find the same, or so many that the longest of them cannot hold up the others by more than joining them would take.  In fp16, heads of 128, behind
-    // 1000 tokens: 64 sequences of 8 heads with 100 tokens each 25.7 us, 31.2 if shared out; 600 of one head with 500 49, 59; 256 of 8 with up to 1500 217, 223; but 64 of 8
-    // with up to 1500 78, 67.
-    p.whole_items = S::GENERAL && (steps + kBeginning<S> <= 4 * S::WARPS || (4 * items >= most && steps * most <= 8 * S::WARPS * std::max(items, most)));
+    // that the kernel would find the same, or up to 512 tokens where they fill a quarter of the device (16 sequences of 8 heads, 512 chosen tokens 20.4 us, 22.8 if shared
+    // out; with 1024 29.3 and 26.4), or more of them where they are many.  In fp16, heads of 128, behind 1000 tokens: 64 sequences of 8 heads with 100 tokens each 25.7
+    // and 31.2; 600 of one head with 500 49 and 59; 256 of 8 with up to 1500 217 and 223; but 64 of 8 with up to 1500 78 and 67.  whole_tokens: what pays beside another kernel.
+    const int64_t worth = std::max(items, 4 * items >= most ? most : 0);
+    p.whole_items = S::GENERAL && (steps + kBeginning<S> <= 4 * S::WARPS || steps * S::SUBS * most <= 8 * S::WARPS * worth || tokens <= p.whole_tokens);
     const int64_t grid = p.whole_items ? items : ctas;
     if (sms) {
         *sms = (int32_t)((grid + S::CTAS - 1) / S::CTAS);

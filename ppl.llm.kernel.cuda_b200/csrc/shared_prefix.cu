@@ -12,32 +12,35 @@ using namespace prefix;
 
 constexpr int64_t kMaxRows = 1 << 24;
 
+constexpr int32_t block_tokens(int32_t head_dim) { return head_dim == 256 ? 64 : 128; }
+constexpr int32_t most_tiles(int32_t head_dim, bool groups) { return head_dim < 256 && (!groups || head_dim == 64) ? 2 : 1; } // that tensor and shared memory have room for
+
 // Tiles of rows that a CTA takes at once.  Two share what is loaded, and widened, but leave twice as many sums to be joined: where a CTA with one would have many blocks to go
 // through, fewer where a block's products take less than its loads.  64 heads over 8; one and two tiles, us: fp16 heads of 128, 64 sequences, 24 and 64 blocks a CTA, 51, 92 and
 // 54, 88; 128 sequences, 48 blocks, 86 and 86; int8 rows, 24 and 64 blocks, 67, 136 and 63, 118; 11 blocks 40.2 and 40.6; fp16 heads of 64, 8 and 24 blocks, 21, 38 and 22, 36.
-int32_t tiles_at_once(const PrefixParams& p, int32_t most, int64_t blocks) {
-    const int64_t tiles = (p.rows + 127) / 128, ctas = std::max<int64_t>(1, kSms / (p.cache.kv_heads * tiles));
-    const int64_t enough = p.cache.quant_group == 0 && p.cache.head_dim > 64 ? 40 : 16;
-    return most == 2 && tiles > 1 && (tiles % 2 == 0 || tiles >= 7) && blocks > enough * ctas ? 2 : 1;
+int32_t tiles_at_once(int64_t rows, const pplb200_kv_cache& c, int64_t blocks) {
+    const int64_t tiles = (rows + 127) / 128, ctas = std::max<int64_t>(1, kSms / (c.kv_heads * tiles));
+    return most_tiles(c.head_dim, c.quant_group == 8) == 2 && tiles > 1 && (tiles % 2 == 0 || tiles >= 7) && blocks > (c.quant_group == 0 && c.head_dim > 64 ? 40 : 16) * ctas ? 2 : 1;
 }
 // Parts that the prefix is cut into: at most so many that there is a CTA for every SM.
 int32_t most_splits(int64_t items) { return (int32_t)std::max<int64_t>(1, kSms / items); }
 // Joining the parts costs about an eighth of a block each, which the square root balances (64 rows of one head, 32768 tokens: 22 us with 46 parts, 41 with 148).  The
 // kernel for the own tokens fills `own_sms` SMs, and where these are left to it, it runs beside this one: up to four blocks a CTA more are worth it
 // (16 rows of 8 heads, 4096 tokens: 13.2 us with 14 parts, 17.8 with 17; 128 rows of 8, 4096 tokens and 700 of int8 each: 23 with 8, 37 with 18).
-int32_t splits_of(int64_t items, int64_t own_sms, int64_t blocks) {
+int32_t splits_of(int64_t items, int64_t own_sms, int64_t blocks, bool* beside = nullptr) {
     const int64_t all = std::min<int64_t>({most_splits(items), blocks, std::max<int64_t>(8, (int64_t)std::sqrt(8.0 * (double)blocks) + 1)});
     const int64_t spared = std::min(all, (kSms - own_sms) / items);
-    return (int32_t)(spared > 0 && (blocks + spared - 1) / spared <= (blocks + all - 1) / all + 4 ? spared : all);
+    const bool spare = spared > 0 && (blocks + spared - 1) / spared <= (blocks + all - 1) / all + 4;
+    if (beside) *beside = spare;
+    return (int32_t)(spare ? spared : all);
 }
 
 // Few rows of an int8 cache: the decode kernel, whose matrix instructions take 8 or 16 at once, widens with all of its warps, and is faster where there are
 // several blocks for a CTA (8 rows of 8 heads over 4096, 8000 and 32768 tokens of int8 rows: 15.8, 18.0, 28.5 us and 15.5, 19.2, 43; 16 rows of groups of 8 over
 // 8000 and 32768: 22, 38 and 20, 51.  In fp16 8 rows 18.0, 32.4 and 16.2, 31.2).
 constexpr int32_t kFewRows = 16;
-bool by_decode(int64_t rows, const pplb200_kv_cache& c, int64_t tokens, int64_t own_sms) {
-    const int64_t nb = c.head_dim == 256 ? 64 : 128, blocks = std::max<int64_t>(1, (tokens + nb - 1) / nb);
-    return c.quant_group && rows <= kFewRows && blocks > splits_of(c.kv_heads, own_sms, blocks) * (rows <= 8 ? 3LL : 6LL);
+bool by_decode(int64_t rows, const pplb200_kv_cache& c, int64_t blocks, int32_t splits) {
+    return c.quant_group && rows <= kFewRows && blocks > splits * (rows <= 8 ? 3LL : 6LL);
 }
 
 // Workspace: counters of the decode kernel where it goes through the prefix, which have to be zero between calls of whatever sizes; what it needs for the own
@@ -80,10 +83,7 @@ template <int D, int KIND>
 int32_t launch_tiles(cudaStream_t stream, PrefixParams& p) {
     using T = Tile<D, KIND>;
     static_assert(T::SMEM + 18 * 1024 <= 232448);
-    const int64_t blocks = std::max<int64_t>(1, (p.tokens_in_table + T::NB - 1) / T::NB);
-    p.tiles = tiles_at_once(p, T::TILES, blocks);
-    p.items = p.cache.kv_heads * (int32_t)((p.rows + p.tiles * 128 - 1) / (p.tiles * 128));
-    p.splits = splits_of(p.items, p.own_sms, blocks);
+    static_assert(T::NB == block_tokens(D) && T::TILES == most_tiles(D, KIND == CACHE_I8_GROUPS));
     p.box_rows = 0;
     if (KIND == CACHE_F16 && p.cache.page_size % 16 == 0 && p.cache.num_pages > 0) {
         const int32_t rows = std::min(p.cache.page_size & -p.cache.page_size, T::NB);
@@ -158,8 +158,19 @@ int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb
     own.parts = 1;
     own.late_wait = true;
     lay_out(own, ws, shared);
-    const int32_t own_sms = sms_of_general(own);
-    const bool decode = by_decode(a->batch * shared, *cache, tokens, own_sms);
+    const int64_t nb = block_tokens(cache->head_dim), blocks = std::max<int64_t>(1, (tokens + nb - 1) / nb);
+    const int32_t tiles = tiles_at_once(a->batch * shared, *cache, blocks), items = (int32_t)(cache->kv_heads * ((a->batch * shared + 128 * tiles - 1) / (128 * tiles)));
+    // Own tokens by a CTA for each sequence and key head, on SMs that are left to them, up to 1024 tokens (fp16, 32 sequences of 8 heads, 1000 tokens each behind 1000 31 us, 51 if
+    // shared out; but 8 of one 18 and 15.4, and behind 12345 tokens, without SMs for them, 71 and 68); up to 512 in any case (64 of one head with 300 11.7, 20.4).
+    bool beside;
+    own.whole_tokens = a->batch * cache->kv_heads >= 32 ? 1024 : 512;
+    int32_t splits = splits_of(items, sms_of_general(own), blocks, &beside);
+    if (!beside && own.whole_tokens > 512) {
+        own.whole_tokens = 512;
+        splits = splits_of(items, sms_of_general(own), blocks);
+    }
+    const bool decode = by_decode(a->batch * shared, *cache, blocks, splits);
+    if (decode) own.whole_tokens = 512;
     const int64_t sums = decode ? rows : rows * most_splits(cache->kv_heads * ((a->batch * shared + 255) / 256));
     own.part_tops = (float2*)(ws + workspace_bytes(shared, cache->head_dim));
     own.part_sums = (float*)((char*)own.part_tops + round_up(sums * 8, 256));
@@ -173,6 +184,7 @@ int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb
         first.tokens_in_table = tokens;
         first.parts = 0;
         first.late_wait = false;
+        first.whole_tokens = 0;
         first.keep_parts = true;
         lay_out(first, (char*)own.part_tops + part_bytes(sums, cache->head_dim), a->batch * shared);
         first.arrived = (uint64_t*)a->ws;
@@ -188,7 +200,7 @@ int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb
         small_division(shared, p.rows_magic, p.rows_shift);
         small_division(cache->page_size, p.page_magic, p.page_shift);
         p.scale_log2 = own.scale_log2;
-        p.own_sms = own_sms;
+        p.tiles = tiles; p.items = items; p.splits = splits;
         p.cache = *cache;
         p.part_rows = rows; p.part_tops = own.part_tops; p.part_sums = own.part_sums;
         const int32_t done = launch_prefix((cudaStream_t)stream, p);

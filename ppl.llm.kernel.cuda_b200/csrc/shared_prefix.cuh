@@ -67,7 +67,6 @@ struct PrefixParams {
     int64_t tokens_in_table;
     int32_t num_pages, rows, tiles; // rows of a key head, and tiles of rows that a CTA takes at once (1 or 2)
     int32_t items, splits;          // items: groups of rows of a key head
-    int32_t own_sms;                // that the own tokens' kernel fills
     int32_t rows_per_head, q_heads;
     uint32_t rows_magic, rows_shift, page_magic, page_shift;
     float scale_log2;
