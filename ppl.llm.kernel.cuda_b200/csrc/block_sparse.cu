@@ -621,6 +621,7 @@ int32_t check_bounds(const pplb200_kv_cache* c, const pplb200_key_bounds* k) {
         return fail(RC_UNSUPPORTED, "key bounds: head_dim must be 64, 96, 128 or 256, got %d", c->head_dim);
     if (k->block <= 0 || k->block % 16 || c->page_size % k->block)
         return fail(RC_INVALID_VALUE, "a block must be a multiple of 16 tokens that divides a page (%d), got %d", c->page_size, k->block);
+    if (k->block > 1 << 30) return fail(RC_UNSUPPORTED, "a block of more than 2^30 tokens");
     if (c->num_pages == 0) return RC_SUCCESS;
     if (!k->bounds || !k->scale || !aligned16(k->bounds) || ((uintptr_t)k->scale & 1)) return fail(RC_INVALID_VALUE, "bounds must be 16-byte, their scales 2-byte aligned pointers");
     if ((__int128)c->num_pages * c->kv_heads * (c->page_size / k->block) * 2 * c->head_dim >> 61) return fail(RC_INVALID_VALUE, "bounds of too many blocks");

@@ -247,6 +247,7 @@ __global__ void __launch_bounds__(RTPB, LAYOUT == AS_IS ? 8 : 7) rotary_kv_kerne
     if (STORE) r.template fetch<V>(group, v);
     __shared__ uint64_t axis_positions[AXES ? RTPB / LANES : 1][PPLB200_ROTARY_MAX_AXES];
     if constexpr (AXES) { // the LANES threads of a row, which lie in one warp, bring a position each
+        static_assert(LANES >= PPLB200_ROTARY_MAX_AXES);
         if (r.u < PPLB200_ROTARY_MAX_AXES) axis_positions[threadIdx.x / LANES][r.u] = (uint64_t)p.positions[min(r.u, p.axes - 1) * p.axis_stride + r.token];
         __syncwarp();
     }

@@ -17,7 +17,7 @@ constexpr int32_t most_tiles(int32_t head_dim, bool groups) { return head_dim < 
 
 // Tiles of rows that a CTA takes at once.  Two share what is loaded, and widened, but leave twice as many sums to be joined: where a CTA with one would have many blocks to go
 // through, fewer where a block's products take less than its loads.  64 heads over 8; one and two tiles, us: fp16 heads of 128, 64 sequences, 24 and 64 blocks a CTA, 51, 92 and
-// 54, 88; 128 sequences, 48 blocks, 86 and 86; int8 rows, 24 and 64 blocks, 67, 136 and 63, 118; 11 blocks 40.2 and 40.6; fp16 heads of 64, 8 and 24 blocks, 21, 38 and 22, 36.
+// 54, 88; 128 sequences, 48 blocks, 86 and 86; int8 rows, 24 and 64 blocks, 75, 155 and 71, 138; 16 blocks 57 and 57; fp16 heads of 64, 8 and 24 blocks, 21, 38 and 22, 36.
 int32_t tiles_at_once(int64_t rows, const pplb200_kv_cache& c, int64_t blocks) {
     const int64_t tiles = (rows + 127) / 128, ctas = std::max<int64_t>(1, kSms / (c.kv_heads * tiles));
     return most_tiles(c.head_dim, c.quant_group == 8) == 2 && tiles > 1 && (tiles % 2 == 0 || tiles >= 7) && blocks > (c.quant_group == 0 && c.head_dim > 64 ? 40 : 16) * ctas ? 2 : 1;
@@ -26,7 +26,7 @@ int32_t tiles_at_once(int64_t rows, const pplb200_kv_cache& c, int64_t blocks) {
 int32_t most_splits(int64_t items) { return (int32_t)std::max<int64_t>(1, kSms / items); }
 // Joining the parts costs about an eighth of a block each, which the square root balances (64 rows of one head, 32768 tokens: 22 us with 46 parts, 41 with 148).  The
 // kernel for the own tokens fills `own_sms` SMs, and where these are left to it, it runs beside this one: up to four blocks a CTA more are worth it
-// (16 rows of 8 heads, 4096 tokens: 13.2 us with 14 parts, 17.8 with 17; 128 rows of 8, 4096 tokens and 700 of int8 each: 23 with 8, 37 with 18).
+// (16 rows of 8 heads, 4096 tokens: 13.2 us with 13 parts, 17.8 with 17; 4096 of int8 rows and 700 of their own each: 22.5, 33).
 int32_t splits_of(int64_t items, int64_t own_sms, int64_t blocks, bool* beside = nullptr) {
     const int64_t all = std::min<int64_t>({most_splits(items), blocks, std::max<int64_t>(8, (int64_t)std::sqrt(8.0 * (double)blocks) + 1)});
     const int64_t spared = std::min(all, (kSms - own_sms) / items);
@@ -35,12 +35,12 @@ int32_t splits_of(int64_t items, int64_t own_sms, int64_t blocks, bool* beside =
     return (int32_t)(spare ? spared : all);
 }
 
-// Few rows of an int8 cache: the decode kernel, whose matrix instructions take 8 or 16 at once, widens with all of its warps, and is faster where there are
-// several blocks for a CTA (8 rows of 8 heads over 4096, 8000 and 32768 tokens of int8 rows: 15.8, 18.0, 28.5 us and 15.5, 19.2, 43; 16 rows of groups of 8 over
-// 8000 and 32768: 22, 38 and 20, 51.  In fp16 8 rows 18.0, 32.4 and 16.2, 31.2).
+// Few rows of an int8 cache: the decode kernel, whose matrix instructions take 8 or 16 at once, widens with all of its warps, and is faster where a CTA would have several
+// blocks (int8 rows, 8 rows of 8 heads over 1000, 4096 and 32768 tokens: 11.8, 15.7, 28 us, by tiles 12.5, 17.3, 48; 4 of 32 over 1000 13.3 and 17.1; 16 of 8 over 4096, 12345
+// and 32768 19.6, 25, 36 and 17.7, 27, 47; groups of 8 19, 25, 38 and 17, 27, 55.  In fp16 8 rows of 8 heads over 8000 and 32768 18.0, 32.4 and 16.2, 31.2).
 constexpr int32_t kFewRows = 16;
 bool by_decode(int64_t rows, const pplb200_kv_cache& c, int64_t blocks, int32_t splits) {
-    return c.quant_group && rows <= kFewRows && blocks > splits * (rows <= 8 ? 3LL : 6LL);
+    return c.quant_group && rows <= kFewRows && blocks > splits * (rows <= 8 ? 1LL : 6LL);
 }
 
 // Workspace: counters of the decode kernel where it goes through the prefix, which have to be zero between calls of whatever sizes; what it needs for the own

@@ -4,7 +4,7 @@
 // never whole in one place, and a product with the values.  A CTA has up to 256 rows of a key head in two tiles of 128 and goes through a part of the
 // prefix in blocks of NB tokens; its sums and reference exponents are left as one of `splits` parts, which are joined where the output is written.
 //
-//   warps 0 - 3, 4 - 7   softmax of one tile each, a thread a row (tensor memory's lanes): scores in, weights of 11 bits out, in place
+//   warps 0 - 3, 4 - 7   softmax of one tile each, a thread a row (tensor memory's lanes): scores in, weights out, in place
 //   warps 8 - 11         keys from the pages into shared memory; int8 ones are widened on the way
 //   warps 12 - 15        values
 //   warp 16              issues all products, and owns the tensor memory
@@ -12,7 +12,16 @@
 // The two tiles' products and softmaxes alternate, so that the tensor cores work on one while the exponentials of the other are computed.  Where a CTA has one
 // tile only, the two softmax groups take turns at the blocks of it, each with a sum of its own (heads of 256: one group, whose sum alone fills
 // half of the tensor memory, over two buffers of scores).
-// Bound by both: a block of 128 tokens of two tiles of heads of 128 is 2048 clocks of the tensor cores and 2048 of the exponentials.
+//
+// Bound by the tensor cores and the exponentials: a block of 128 tokens of two tiles of heads of 128 is 2048 clocks of either.  64 sequences of 64 heads over 8 with 100
+// tokens each behind 32768: fp16 88 us, 780 TFLOP/s (1270 for the 20000 tokens from 12345 on; with the products alone the call took 71 us, then of 93), int8 rows 138
+// and groups of 8 160: there the loading warps widen every element, for each tile or pair of tiles, and groups' keys are two operands.  What a call takes besides,
+// 10 to 30 us, is the start, q, the parts' sums (64 KB a tile and part) and their joining, and own tokens that do not fit beside it.
+// Tried on fp16 and left, since none changed a block's time: two softmax groups a tile, half of the exponentials as polynomials of degree 3 to 5, looking whether the reference
+// exponent has to move after the weights instead of before them.
+// Weights are fp16 of 2^-24 to 2^14, over an fp16 cache 11 bits, off by at most 2^-11 of themselves, as much as the output's own rounding; their sum is of what they were.  v of int8 caches is
+// rounded to fp16 itself, and the two errors came to half as much again as the output's: there the weights are two operands, 22 bits (48 sequences of 64 heads over
+// 8 behind 4000 tokens of int8 rows: 53 us instead of 50, relative error 0.00028 instead of 0.00031; the output's rounding alone 0.00021).
 #pragma once
 
 #include "paged_attention.cuh"
@@ -25,9 +34,9 @@ namespace prefix {
 
 using namespace paged;
 
-__device__ unsigned int g_status = 0;
+__device__ unsigned int g_status = 0; // codes of waits that gave up
 __device__ uint4 g_nothing[32]; // zeros: what a token that is not there reads
-constexpr float kAbove = 4.0f;
+constexpr float kAbove = 4.0f; // where a reference exponent goes above the score that moved it
 constexpr unsigned ST_LOAD = 1u, ST_MMA = 2u, ST_SOFTMAX = 4u;
 
 template <int D_, int KIND_>
@@ -35,6 +44,7 @@ struct Tile {
     static constexpr int D = D_, KIND = KIND_, ES = KIND == CACHE_F16 ? 2 : 1;
     static constexpr int DP = (D + 63) / 64 * 64, ATOMS = DP / 64; // a row of shared memory is 128 bytes, 64 dimensions
     static constexpr bool LOW = KIND == CACHE_I8_GROUPS;           // keys: value x scale rounded to fp16, and what that left
+    static constexpr bool FINE = KIND != CACHE_F16;                // weights: likewise two operands, 22 bits, each 32 tokens' where their scores were
     static constexpr int NB = D == 256 ? 64 : 128;                 // tokens of a block
     static constexpr int STREAMS = D == 256 ? 1 : 2;
     static constexpr int TILES = D == 256 || (LOW && D > 64) ? 1 : 2; // of rows, at most
@@ -175,8 +185,11 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                     if (!(ok = __all_sync(0xffffffffu, ptx::mbar_wait(bar(half ? weight_full[i & 1] : weight_half[i & 1]), (i >> 1) & 1, &g_status, ST_MMA)))) break;
                     ptx::tc_fence_after();
 #pragma unroll
-                    for (int s = half * T::NB / 32; s < (half + 1) * T::NB / 32; ++s)
-                        ptx::mma_f16_tmem(d, w + s * 8, ptx::desc_from_lo(v + s * (2048 / 16)), PV, (T::STREAMS == 2 ? i > 1 : i > 0) || s > 0, leads);
+                    for (int s = half * T::NB / 32; s < (half + 1) * T::NB / 32; ++s) {
+                        const uint32_t a = T::FINE ? w + (s >> 1) * 32 + (s & 1) * 8 : w + s * 8;
+                        ptx::mma_f16_tmem(d, a, ptx::desc_from_lo(v + s * (2048 / 16)), PV, (T::STREAMS == 2 ? i > 1 : i > 0) || s > 0, leads);
+                        if constexpr (T::FINE) ptx::mma_f16_tmem(d, a + 16, ptx::desc_from_lo(v + s * (2048 / 16)), PV, 1, leads);
+                    }
                 }
                 ptx::mma_commit_by(bar(sum_done[i & 1]), leads);
                 if (tiles == 1 || (i & 1)) ptx::mma_commit_by(bar(empty_v[stage]), leads);
@@ -529,7 +542,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                 const float2 reference = make_float2(8.0f - top, 8.0f - top), factors = make_float2(factor, factor);
                 float2 sums[2] = {};
                 auto weigh = [&](const float (&x)[32], int c) { // weights of tokens c to c + 31 into their place
-                    uint32_t w[16];
+                    uint32_t w[16], low[T::FINE ? 16 : 1];
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) {
                         float2 e = ptx::fma2(make_float2(x[k], x[k + 1]), factors, reference);
@@ -537,8 +550,13 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                         e.y = exp2_fast(e.y);
                         sums[k >> 1 & 1] = ptx::add2(sums[k >> 1 & 1], e);
                         w[k / 2] = h2(__floats2half2_rn(e.x, e.y));
+                        if constexpr (T::FINE) {
+                            const float2 high = __half22float2(as_h2(w[k / 2]));
+                            low[k / 2] = h2(__floats2half2_rn(e.x - high.x, e.y - high.y));
+                        }
                     }
-                    ptx::tmem_st_32x16(at + c / 2, w);
+                    ptx::tmem_st_32x16(T::FINE ? at + c : at + c / 2, w);
+                    if constexpr (T::FINE) ptx::tmem_st_32x16(at + c + 16, low);
                 };
 #pragma unroll
                 for (int c = 0; c < KEPT; c += 32) {

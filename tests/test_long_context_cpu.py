@@ -179,6 +179,12 @@ def test_bounds_refusals(k, rc):
     assert c["sparse"](_cache(), k) == c["update"](_cache(), **k) == c["read"](_cache(), **k) == rc and pplb200.last_error()
 
 
+def test_bounds_of_blocks_beyond_all_measure():
+    c, page = _calls(), (1 << 31) - 16
+    cache = _cache(page=page, token_stride=0, head_stride=0, page_stride=0, stoken=0, shead=0, spage=0)
+    assert c["update"](cache, block=page) == c["read"](cache, block=page) == 2
+
+
 def test_bounds_refusals_of_calls():
     c = _calls()
     assert c["update"](_cache(), tokens=-1) == c["update"](_cache(), slots=0) == c["update"](_cache(), slots=AT + 4) == 4 and c["update"](_cache(), tokens=1 << 31) == 2

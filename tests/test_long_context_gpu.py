@@ -574,6 +574,28 @@ def test_prefix_batches_of_all_sizes_on_one_workspace(cuda, pplb200, hq, hk, d, 
         assert cuda.equal(att(*part), mine(*part)), n
 
 
+@pytest.mark.parametrize("prefix,batch,hq,hk,d,group,own", [
+    (900, 32, 16, 4, 128, 0, 1000),     # own tokens by a CTA each, on SMs that are left to them
+    (900, 40, 8, 8, 64, 64, 513),       # the same, where they fill them all
+    (9000, 32, 32, 8, 128, 0, 900),     # no SMs left: shared out
+    (300, 5, 4, 1, 96, 8, 511),         # few items, a CTA each
+    (300, 5, 4, 1, 256, 0, 2100),       # few and long: shared out
+    (40, 300, 4, 4, 128, 128, 130),     # more CTAs than the device holds
+    (9000, 4, 4, 4, 128, 8, 600),       # few rows of an int8 cache, which the decode kernel takes
+])
+def test_prefix_own_tokens_dealt_out(cuda, pplb200, prefix, batch, hq, hk, d, group, own):
+    lengths = [own, 0, -1, 1, own - 1, own // 2, 17] * (batch // 7) + [own] * (batch % 7)
+    _check_attention(*_run_prefix(cuda, pplb200, prefix, lengths, hq, hk, d, 16, group)[:3])
+
+
+def test_prefix_without_own_pages(cuda, pplb200):
+    """A table of no pages: the lengths are not looked at, but for their sign."""
+    out, lse, _, (att, call, cache) = _run_prefix(cuda, pplb200, 500, [0, 0, -1] * 4, 8, 2, 128, 16, 128)
+    none = pplb200.SharedPrefixDecodeAttention(cache, 8, 12, 0, 500)
+    table, lengths = cuda.empty((12, 0), dtype=cuda.int32, device="cuda"), cuda.tensor([0, 99, -1] * 4, dtype=cuda.int32, device="cuda")
+    assert cuda.equal(none(call[0], call[1], call[2], table, lengths), out) and not bool(out[2::3].any())
+
+
 def test_no_wait_has_given_up(cuda, pplb200):
     _run_prefix(cuda, pplb200, 400, [5] * 20, 4, 1, 64, 16, 0)
     cuda.cuda.synchronize()
