@@ -976,9 +976,10 @@ int32_t launch(cudaStream_t stream, AttentionParams& p, int64_t tokens, int32_t*
     // Items that are short whatever their lengths: a CTA each, of which there may be more than the device holds at once, without looking through the lengths first; so short
     // that the kernel would find the same, or up to 512 tokens where they fill a quarter of the device (16 sequences of 8 heads, 512 chosen tokens 20.4 us, 22.8 if shared
     // out; with 1024 29.3 and 26.4), or more of them where they are many.  In fp16, heads of 128, behind 1000 tokens: 64 sequences of 8 heads with 100 tokens each 25.7
-    // and 31.2; 600 of one head with 500 49 and 59; 256 of 8 with up to 1500 217 and 223; but 64 of 8 with up to 1500 78 and 67.  whole_tokens: what pays beside another kernel.
+    // and 31.2; 600 of one head with 500 49 and 59; 256 of 8 with up to 1500 217 and 223; but 64 of 8 with up to 1500 78 and 67.  (int8 rows,
+    // 1024 tokens: 32 of 8 behind 12345 62 and 64.)  whole_tokens: what pays beside another kernel.
     const int64_t worth = std::max(items, 4 * items >= most ? most : 0);
-    p.whole_items = S::GENERAL && (steps + kBeginning<S> <= 4 * S::WARPS || steps * S::SUBS * most <= 8 * S::WARPS * worth || tokens <= p.whole_tokens);
+    p.whole_items = S::GENERAL && (steps + kBeginning<S> <= 4 * S::WARPS || steps * (p.late_wait ? 1 : S::SUBS) * most <= 8 * S::WARPS * worth || tokens <= p.whole_tokens);
     const int64_t grid = p.whole_items ? items : ctas;
     if (sms) {
         *sms = (int32_t)((grid + S::CTAS - 1) / S::CTAS);
