@@ -238,57 +238,54 @@ __device__ __forceinline__ void write_out(const AttentionParams& p, int64_t b, i
 // Row `row` (GENERAL: of those that the item's key head is asked by) of key head kvh.
 template <class S>
 __device__ __forceinline__ void finish(const AttentionParams& p, int64_t b, int32_t kvh, int32_t row, int32_t d, float4 v, float top, float sum) {
-    if constexpr (!S::GENERAL) {
-        write_out(p, b, kvh * p.shared + row, S::D, d, v, top, sum);
-    } else {
-        const int32_t beyond = (uint32_t)((uint64_t)(uint32_t)row * p.rows_magic >> p.rows_shift);
-        const int64_t sequence = b + beyond;
-        const int32_t head = kvh * p.rows_per_head + (row - beyond * p.rows_per_head);
-        const int64_t at = sequence * p.q_heads + head;
-        if (p.keep_parts) {
-            __stcg(reinterpret_cast<float4*>(p.part_sums + at * S::D + d), v);
-            if (d == 0) __stcg(&p.part_tops[at], make_float2(top, sum));
-            return;
-        }
-        if (p.parts > 0) {
-            if (p.lengths[sequence] < 0) { // not a sequence
-                v = make_float4(0, 0, 0, 0);
-                top = kNothingSeen;
-                sum = 0.0f;
-            } else {
-                // eight parts at once, sixteen loads on their way
-                constexpr int BATCH = 8;
-                for (int32_t i = 0; i < p.parts; i += BATCH) {
-                    float2 s[BATCH];
-                    float4 a[BATCH];
-                    float up = top;
+    static_assert(S::GENERAL);
+    const int32_t beyond = (uint32_t)((uint64_t)(uint32_t)row * p.rows_magic >> p.rows_shift);
+    const int64_t sequence = b + beyond;
+    const int32_t head = kvh * p.rows_per_head + (row - beyond * p.rows_per_head);
+    const int64_t at = sequence * p.q_heads + head;
+    if (p.keep_parts) {
+        __stcg(reinterpret_cast<float4*>(p.part_sums + at * S::D + d), v);
+        if (d == 0) __stcg(&p.part_tops[at], make_float2(top, sum));
+        return;
+    }
+    if (p.parts > 0) {
+        if (p.lengths[sequence] < 0) { // not a sequence
+            v = make_float4(0, 0, 0, 0);
+            top = kNothingSeen;
+            sum = 0.0f;
+        } else {
+            // eight parts at once, sixteen loads on their way
+            constexpr int BATCH = 8;
+            for (int32_t i = 0; i < p.parts; i += BATCH) {
+                float2 s[BATCH];
+                float4 a[BATCH];
+                float up = top;
 #pragma unroll
-                    for (int j = 0; j < BATCH; ++j) {
-                        const int64_t from = min(i + j, p.parts - 1) * p.part_rows + at;
-                        s[j] = __ldcg(&p.part_tops[from]);
-                        a[j] = __ldcg(reinterpret_cast<const float4*>(p.part_sums + from * S::D + d));
-                    }
-#pragma unroll
-                    for (int j = 0; j < BATCH; ++j) {
-                        if (i + j >= p.parts) s[j] = make_float2(kNothingSeen, 0.0f);
-                        up = fmaxf(up, s[j].x);
-                    }
-                    const float keep = exp2_fast(top - up);
-                    top = up;
-                    sum *= keep;
-                    v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
-#pragma unroll
-                    for (int j = 0; j < BATCH; ++j)
-                        if (s[j].x != kNothingSeen) { // else its sums need not have been written
-                            const float f = exp2_fast(s[j].x - up);
-                            sum += s[j].y * f;
-                            v.x += a[j].x * f; v.y += a[j].y * f; v.z += a[j].z * f; v.w += a[j].w * f;
-                        }
+                for (int j = 0; j < BATCH; ++j) {
+                    const int64_t from = min(i + j, p.parts - 1) * p.part_rows + at;
+                    s[j] = __ldcg(&p.part_tops[from]);
+                    a[j] = __ldcg(reinterpret_cast<const float4*>(p.part_sums + from * S::D + d));
                 }
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j) {
+                    if (i + j >= p.parts) s[j] = make_float2(kNothingSeen, 0.0f);
+                    up = fmaxf(up, s[j].x);
+                }
+                const float keep = exp2_fast(top - up);
+                top = up;
+                sum *= keep;
+                v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j)
+                    if (s[j].x != kNothingSeen) { // else its sums need not have been written
+                        const float f = exp2_fast(s[j].x - up);
+                        sum += s[j].y * f;
+                        v.x += a[j].x * f; v.y += a[j].y * f; v.z += a[j].z * f; v.w += a[j].w * f;
+                    }
             }
         }
-        write_out(p, sequence, head, S::D, d, v, top, sum);
     }
+    write_out(p, sequence, head, S::D, d, v, top, sum);
 }
 
 template <class S>
@@ -424,8 +421,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                                    (S::KIND == CACHE_I8_GROUPS ? t * S::KG * 2 + (S::PACKED ? g * (S::D / 4) : 0) : 0);
         const char* const vsbase = (const char*)p.cache.v_scale + (int64_t)kvh * p.cache.scale_head_stride * 2 + scale_bytes +
                                    (S::KIND == CACHE_I8_GROUPS ? g * (S::VP / S::ES) / 8 * 2 + (S::PACKED ? 2 * t * (S::D / 4) : 0) : 0);
-        const int32_t* row_pages = p.pages + b * p.pages_stride;
-        if constexpr (S::GENERAL) row_pages += kvh * p.pages_head_stride;
+        const int32_t* const row_pages = p.pages + b * p.pages_stride + (S::GENERAL ? kvh * p.pages_head_stride : 0);
 
         // ---- tokens on their way -----------------------------------------------------------------------------------------
         // Of the step that is loaded next: which tokens there are, and where their rows lie.  Lane l looks after token l of a step (of l %
@@ -453,15 +449,16 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
             if constexpr (S::PACKED) coming = 0;
 #pragma unroll
             for (int i = 0; i < PLACES; ++i) {
-                uint32_t page = at.page[i], in_page = at.in_page[i];
-                const bool ok = page < (uint32_t)(S::GENERAL ? p.num_units : p.num_pages);
+                const bool ok = (uint32_t)at.page[i] < (uint32_t)(S::GENERAL ? p.num_units : p.num_pages);
                 if constexpr (S::GENERAL) { // (a number of 31 bits, or not taken)
-                    const uint32_t unit = page;
-                    page = (uint32_t)((uint64_t)unit * p.unit_magic >> p.unit_shift);
-                    in_page += (unit - page * p.units_per_page) * p.unit_tokens;
+                    const uint32_t unit = at.page[i], page = (uint32_t)((uint64_t)unit * p.unit_magic >> p.unit_shift);
+                    const uint32_t in_page = at.in_page[i] + (unit - page * p.units_per_page) * p.unit_tokens;
+                    row[i] = ok ? page * p.page_units + in_page * p.token_units : 0u;
+                    if constexpr (S::KIND != CACHE_F16) scale_row[i] = ok ? page * p.scale_page_units + in_page * p.scale_token_units : 0u;
+                } else {
+                    row[i] = ok ? at.page[i] * p.page_units + at.in_page[i] * p.token_units : 0u;
+                    if constexpr (S::KIND != CACHE_F16) scale_row[i] = ok ? at.page[i] * p.scale_page_units + at.in_page[i] * p.scale_token_units : 0u;
                 }
-                row[i] = ok ? page * p.page_units + in_page * p.token_units : 0u;
-                if constexpr (S::KIND != CACHE_F16) scale_row[i] = ok ? page * p.scale_page_units + in_page * p.scale_token_units : 0u;
                 if constexpr (S::PACKED) {
                     off[i] = (uint64_t)row[i] * p.unit;
                     scale_off[i] = (uint64_t)scale_row[i] * p.scale_unit;
@@ -838,6 +835,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
         if (late) pdl_wait_prior_grid();
         const bool whole = step0 == 0 && step1 == steps;
         const int64_t slot = 2 * (int64_t)blockIdx.x + (step0 == 0 ? 1 : 0);
+        const int head0 = kvh * p.shared + q_first;
         for (int x = threadIdx.x; x < q_count * (S::D / 4); x += S::THREADS) {
             const int h = x / (S::D / 4), d = (x - h * (S::D / 4)) * 4;
             float m = kNothingSeen, l = 0.0f;
@@ -853,7 +851,8 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                 v.x += f * a.x; v.y += f * a.y; v.z += f * a.z; v.w += f * a.w;
             }
             if (whole) {
-                finish<S>(p, b, kvh, q_first + h, d, v, m, l);
+                if constexpr (S::GENERAL) finish<S>(p, b, kvh, q_first + h, d, v, m, l);
+                else write_out(p, b, head0 + h, S::D, d, v, m, l);
             } else {
                 __stcg(reinterpret_cast<float4*>(p.sums + (slot * S::HEADS + h) * S::D + d), v);
                 if (d == 0) __stcg(&p.tops[slot * S::HEADS + h], make_float2(m, l));
@@ -959,7 +958,10 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
             if (ends && last_of(p.arrived + c0, groups)) {
                 join(0, groups, per_group);
 #pragma unroll
-                for (int x = 0; x < ITEMS; ++x) finish<S>(p, b, kvh, q_first + h[x], d[x], v[x], m[x], l[x]);
+                for (int x = 0; x < ITEMS; ++x) {
+                    if constexpr (S::GENERAL) finish<S>(p, b, kvh, q_first + h[x], d[x], v[x], m[x], l[x]);
+                    else write_out(p, b, head0 + h[x], S::D, d[x], v[x], m[x], l[x]);
+                }
             }
         }
         __syncthreads();
