@@ -582,6 +582,10 @@ def test_prefix_batches_of_all_sizes_on_one_workspace(cuda, pplb200, hq, hk, d, 
     (300, 5, 4, 1, 256, 0, 2100),       # few and long: shared out
     (40, 300, 4, 4, 128, 128, 130),     # more CTAs than the device holds
     (9000, 4, 4, 4, 128, 8, 600),       # few rows of an int8 cache, which the decode kernel takes
+    (9000, 2, 4, 1, 256, 8, 40),
+    (9000, 4, 32, 8, 256, 256, 50),
+    (17000, 4, 32, 8, 96, 96, 50),
+    (17000, 16, 8, 8, 64, 8, 50),
 ])
 def test_prefix_own_tokens_dealt_out(cuda, pplb200, prefix, batch, hq, hk, d, group, own):
     lengths = [own, 0, -1, 1, own - 1, own // 2, 17] * (batch // 7) + [own] * (batch % 7)
@@ -630,6 +634,34 @@ def test_same_run_after_run_and_in_a_graph(cuda, pplb200, group):
         graph.replay()
         cuda.cuda.synchronize()
         assert cuda.equal(a, att(q, table, lens)) and cuda.equal(b, prefix(*call))
+
+
+@pytest.mark.parametrize("group", [0, 128])
+def test_two_graphs_at_once(cuda, pplb200, group):
+    """Calls on two streams, each with workspaces of its own, over one cache each."""
+    graphs = []
+    for seed in (1, 2):
+        _, _, _, (att, q, table, lens, _, _, _) = _run_sparse(cuda, pplb200, [3000, 40, 999], 8, 2, 128, 16, 16, group, 1, 2, 9, seed=seed)
+        _, _, _, (prefix, call, _) = _run_prefix(cuda, pplb200, 2500, [30, 600, 7] * 9, 8, 2, 128, 16, group, seed=seed)
+        want = att(q, table, lens), prefix(*call)
+        out = tuple(cuda.zeros_like(t) for t in want)
+        graph, stream = cuda.cuda.CUDAGraph(), cuda.cuda.Stream()
+        stream.wait_stream(cuda.cuda.current_stream())
+        with cuda.cuda.graph(graph, stream=stream):
+            for _ in range(3):
+                prefix(*call, out=out[1])
+                att(q, table, lens, out=out[0])
+        graphs.append((graph, stream, want, out, (att, prefix, q, table, lens, call)))
+    for _ in range(5):
+        cuda.cuda.synchronize()
+        for _, _, _, out, _ in graphs:
+            [t.zero_() for t in out]
+        cuda.cuda.synchronize()
+        for graph, stream, _, _, _ in graphs:
+            with cuda.cuda.stream(stream):
+                graph.replay()
+        cuda.cuda.synchronize()
+        assert all(cuda.equal(a, b) for _, _, want, out, _ in graphs for a, b in zip(want, out))
 
 
 def test_a_decode_step_behind_a_shared_image(cuda, pplb200):
