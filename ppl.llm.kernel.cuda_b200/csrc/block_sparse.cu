@@ -25,8 +25,8 @@ __device__ __forceinline__ bool is_finite(half s) { return (__half_as_ushort(s) 
 // their way.  The lanes that have the same dimensions of different rows halve them between each other at the end, so that all divide and write.  Nothing is
 // shared but these shuffles.
 // In fp16 bound by HBM in a long prompt, the keys once (131072 tokens of 8 heads of 128, blocks of 64: 48 us, 5.6 TB/s), int8 by the minima and maxima, which are
-// in fp32 as the products are, of three numbers at a time (45 us, groups of 8 48; of two numbers 51 and 58; with eight bytes a lane 53 and 59).  16384 tokens: 8.2, 9.0 and
-// 8.9 us; in a decode step look-ups and the launch, 3 us.
+// in fp32 as the products are, of three numbers at a time (45 us, groups of 8 48; of two numbers 51 and 58; with eight bytes a lane 53 and 59).  16384 tokens: 7.7, 7.1 and
+// 7.8 us; in a decode step look-ups and the launch, 3 us.
 constexpr int BWARPS = 4, BTPB = 32 * BWARPS;
 struct BoundsParams {
     pplb200_kv_cache cache;
@@ -682,9 +682,11 @@ int32_t pplb200_key_bounds_update(pplb200_stream_t stream, const pplb200_kv_cach
     p.slots = slots; p.tokens = tokens;
     p.block = bounds->block; p.per_page = cache->page_size / bounds->block;
     small_division(p.block, p.block_magic, p.block_shift);
-    // one slot a CTA while that makes no more than eight CTAs an SM, then up to as many as a block has, so that a prompt's CTA has one block
+    // one slot a CTA while that makes no more than eight CTAs an SM, then more of them, and in a long prompt as many as a block has, so that each CTA has one block (16384
+    // tokens of 8 heads, blocks of 64, int8 rows: 7.1 us; with 27 slots, which makes eight CTAs an SM, most of them idle, 9.0; with 8 12.5)
     const int64_t heads = (cache->kv_heads + BWARPS - 1) / BWARPS;
-    p.slots_here = (int32_t)std::min<int64_t>(std::min(p.block, BTPB), std::max<int64_t>(1, tokens * heads / (8 * kSms)));
+    const int64_t share = tokens * heads / (8 * kSms), whole = std::min(p.block, BTPB);
+    p.slots_here = (int32_t)(share >= 16 ? whole : std::min(whole, std::max<int64_t>(1, share)));
     const dim3 grid((unsigned)((tokens + p.slots_here - 1) / p.slots_here), (unsigned)heads);
     if (cache->head_dim == 64) launch_bounds_of<64>((cudaStream_t)stream, p, grid);
     else if (cache->head_dim == 96) launch_bounds_of<96>((cudaStream_t)stream, p, grid);
