@@ -448,12 +448,13 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                 const uint32_t at = tmem + lanes + (i & 1) * 128;
                 // Where registers hold half of the scores (KEPT), the others are looked at for the largest and loaded again when the first half's weights are on their way.
                 constexpr int HALF = T::NB / 2, KEPT = T::KEPT;
-                const bool straight = p.scale_log2 > 0.0f; // the largest product stays the largest score
-                const float factor = straight ? p.scale_log2 : 1.0f; // of what score() gives
+                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
                 const uint4 mask4 = *reinterpret_cast<const uint4*>(masks[slot]);
                 met |= (mask4.x | mask4.y | (T::NB == 128 ? mask4.z | mask4.w : 0u)) != 0;
                 const bool whole = (mask4.x & mask4.y & mask4.z & mask4.w) == 0xffffffffu;
-                auto score = [&](const uint32_t (&bits)[32], float (&x)[32], int c) { // of tokens c to c + 31
+                // Of tokens c to c + 31, rounded to 32 bits here: fused with the reference exponent's subtraction below, which takes half an instruction less, scores from 2^27 on
+                // would differ from the largest, which is rounded, by more than a weight has room for.
+                auto score = [&](const uint32_t (&bits)[32], float (&x)[32], int c) {
                     if constexpr (T::KIND == CACHE_I8_ROWS) { // the scales of 32 keys, read as they are: in 32 bits they would take half of the shared memory's time
                         const uint4* const ks = reinterpret_cast<const uint4*>(raw_smem + (smem - ptx::smem_addr(raw_smem)) + T::INFO) + (slot * T::NB + c) / 8;
 #pragma unroll
@@ -462,17 +463,17 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                             const uint32_t f4[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
                             for (int y = 0; y < 4; ++y) {
-                                const float2 u = ptx::mul2(make_float2(__uint_as_float(bits[k + 2 * y]), __uint_as_float(bits[k + 2 * y + 1])), __half22float2(as_h2(f4[y])));
+                                const float2 u = ptx::mul2(make_float2(__uint_as_float(bits[k + 2 * y]), __uint_as_float(bits[k + 2 * y + 1])), ptx::mul2(__half22float2(as_h2(f4[y])), scale2));
                                 x[k + 2 * y] = u.x; x[k + 2 * y + 1] = u.y;
                             }
                         }
                     } else {
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) x[k] = __uint_as_float(bits[k]);
+                        for (int k = 0; k < 32; k += 2) {
+                            const float2 u = ptx::mul2(make_float2(__uint_as_float(bits[k]), __uint_as_float(bits[k + 1])), scale2);
+                            x[k] = u.x; x[k + 1] = u.y;
+                        }
                     }
-                    if (!straight)
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) x[k] *= p.scale_log2;
                     if (!whole) {
                         const uint32_t mask = c == 0 ? mask4.x : c == 32 ? mask4.y : c == 64 ? mask4.z : mask4.w;
 #pragma unroll
@@ -514,7 +515,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                 for (int y = 4; y > 0; y >>= 1)
 #pragma unroll
                     for (int k = 0; k < y; ++k) high[k] = fmaxf(high[k], high[k + y]);
-                const float m = high[0] * factor;
+                const float m = high[0];
                 // The reference exponent moves when a weight would pass 2^14, each row's for itself, and then to kAbove above the largest score: some row of 32 meets a score
                 // 2^6 times as heavy again and again where keys have a few large dimensions.  The largest weight is 2^4 at least; those below 2^-18 of it lose bits.
                 const bool higher = m > top + 6.0f;
@@ -539,13 +540,14 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                         }
                     }
                 }
-                const float2 reference = make_float2(8.0f - top, 8.0f - top), factors = make_float2(factor, factor);
+                const float less = __fadd_rd(8.0f, -top); // down: of numbers 16 apart the next one would make a weight 2^16
+                const float2 reference = make_float2(less, less);
                 float2 sums[2] = {};
                 auto weigh = [&](const float (&x)[32], int c) { // weights of tokens c to c + 31 into their place
                     uint32_t w[16], low[T::FINE ? 16 : 1];
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) {
-                        float2 e = ptx::fma2(make_float2(x[k], x[k + 1]), factors, reference);
+                        float2 e = ptx::add2(make_float2(x[k], x[k + 1]), reference);
                         e.x = exp2_fast(e.x);
                         e.y = exp2_fast(e.y);
                         sums[k >> 1 & 1] = ptx::add2(sums[k >> 1 & 1], e);
