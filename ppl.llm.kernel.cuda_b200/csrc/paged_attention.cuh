@@ -697,7 +697,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                     for (int k = 0; k < 2; ++k) {
                         high[nt][k] = fmaxf(c[0][nt][k] + e0[0], c[0][nt][2 + k] + e1[0]);
                         if constexpr (S::SUBS == 2) high[nt][k] = fmaxf(high[nt][k], fmaxf(c[S::SUBS - 1][nt][k] + e0[S::SUBS - 1], c[S::SUBS - 1][nt][2 + k] + e1[S::SUBS - 1]));
-                        higher |= high[nt][k] > top[nt][k] + 6.0f;
+                        higher |= high[nt][k] - top[nt][k] > 6.0f; // (top + 6 may be rounded to top + 8)
                     }
                 // The reference exponent need not be the maximum: it moves when a weight would pass 2^14, which after the first steps is rare.
                 if (__any_sync(0xffffffffu, higher)) {
@@ -710,7 +710,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                             for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
                             m = fmaxf(m, top[nt][k]);
                             if constexpr (S::GENERAL) // rows of other sequences: what one needs leaves the others' bits alone
-                                if (!(m > top[nt][k] + 6.0f)) m = top[nt][k];
+                                if (!(m - top[nt][k] > 6.0f)) m = top[nt][k];
                             const float keep = exp2_fast(top[nt][k] - m);
                             top[nt][k] = m;
                             sum[nt][k] *= keep;
@@ -730,7 +730,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
                     for (int nt = 0; nt < S::NT; ++nt) {
                         float w[4];
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) w[x] = exp2_fast(c[sub][nt][x] - (top[nt][x & 1] - 8.0f));
+                        for (int x = 0; x < 4; ++x) w[x] = exp2_fast(c[sub][nt][x] - __fadd_ru(top[nt][x & 1], -8.0f)); // up: of scores 16 apart the one below would make a weight 2^16
                         sum[nt][0] += w[0] + w[2];
                         sum[nt][1] += w[1] + w[3];
                         if constexpr (S::KIND == CACHE_I8_ROWS) {

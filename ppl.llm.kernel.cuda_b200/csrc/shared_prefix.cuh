@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                 const float m = high[0];
                 // The reference exponent moves when a weight would pass 2^14, each row's for itself, and then to kAbove above the largest score: some row of 32 meets a score
                 // 2^6 times as heavy again and again where keys have a few large dimensions.  The largest weight is 2^4 at least; those below 2^-18 of it lose bits.
-                const bool higher = m > top + 6.0f;
+                const bool higher = m - top > 6.0f; // (top + 6 may be rounded to top + 8)
                 if (__any_sync(0xffffffffu, higher)) {
                     const float to = higher ? m + kAbove : top, keep = exp2_fast(top - to);
                     top = to;

@@ -1,5 +1,6 @@
 """Attention behind a shared prefix, over chosen blocks and over all tokens, on the GPU, where the usual cases do not go.  Tolerances as in test_attention_gpu.py: sums of half
 steps."""
+import numpy as np
 import pytest
 
 from test_attention_gpu import HALF, TINY, _cache, _gen, _randn, _stored
@@ -9,8 +10,8 @@ pytestmark = pytest.mark.gpu
 
 # ---- scores beyond 2^24 ------------------------------------------------------------------------------------------------
 
-# base-2 scores near 2^30, and at the largest scale that is taken
-@pytest.mark.parametrize("scale", [2.0 ** 15, 2.0 ** 50, -(2.0 ** 50)])
+# base-2 scores of up to 2^27 to 2^28, where 8 lies half way between two numbers of 32 bits; near 2^30; the largest scale that is taken
+@pytest.mark.parametrize("scale", [2.0 ** 12, -(2.0 ** 12), 2.0 ** 15, 2.0 ** 50, -(2.0 ** 50)])
 @pytest.mark.parametrize("group", [0, 8, 128])
 @pytest.mark.parametrize("kind", ["decode", "sparse", "prefix few", "prefix many"])
 def test_scores_far_beyond_what_their_steps_resolve(cuda, pplb200, kind, group, scale):
@@ -36,3 +37,44 @@ def test_scores_far_beyond_what_their_steps_resolve(cuda, pplb200, kind, group, 
     score = cuda.einsum("bhd,td->bht", q.double(), kr[:, 0]) * scale
     want = vr[score.argmax(-1), 0]
     assert bool(((out.double() - want).abs() <= want.abs() * (2 * HALF + 2.0 ** -20) + 2 * TINY).all())
+
+
+@pytest.mark.parametrize("step", [1, 2, 4, 8, 16, 32])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("group", [0, 8, 128])
+@pytest.mark.parametrize("kind", ["decode", "sparse", "prefix few", "prefix many"])
+def test_scores_that_rise_by_what_32_bits_resolve(cuda, pplb200, kind, group, sign, step):
+    """Base-2 scores of +-2^23 step and a multiple of `step` more: every number on the way is exact in 32 bits, every weight a power of two.  So the outputs are off by their own rounding, by
+    the sums' of 300 tokens in 32 bits, and by that of values which are rounded when they are read."""
+    d, n, rows = 128, 300, 16
+    cache = _cache(cuda, pplb200, 20, 16, 1, d, group, "heads", 0)
+    at = cuda.arange(n, device="cuda")
+    k = cuda.zeros((n, 1, d), dtype=cuda.float16, device="cuda")
+    k[:, 0, 0], k[:, 0, 8] = 4.0 * sign, (at // 3 * 2.0 ** -4).to(cuda.float16)
+    pplb200.kv_cache_write(cache, k, _randn(cuda, _gen(cuda, 4), n, 1, d), at)
+    if group:  # whole numbers times 2^-4
+        cache.k.view(20, 16, d)[at // 16, at % 16] = (k[:, 0] * 16).to(cuda.int8)
+        cache.k_scale.fill_(2.0 ** -4)
+    kr, vr = _stored(cuda, cache, at)
+    assert cuda.equal(kr, k.double())
+    batch = 12 if kind == "prefix many" else 1
+    q = cuda.zeros((batch, rows, d), dtype=cuda.float16, device="cuda")
+    q[..., 0], q[..., 8] = 8192.0, 2.0 ** -4
+    scale = np.float32(step * 256.0 / 1.4426950408889634)
+    while scale * np.float32(1.4426950408889634) < step * 256:
+        scale = np.nextafter(scale, np.float32(np.inf))
+    while scale * np.float32(1.4426950408889634) > step * 256:
+        scale = np.nextafter(scale, np.float32(0))
+    assert scale * np.float32(1.4426950408889634) == step * 256  # so that a score is 2^15 times step 2^8, and 2^-8 times that for a third of the token's number
+    table, i32 = cuda.arange(20, dtype=cuda.int32, device="cuda"), dict(dtype=cuda.int32, device="cuda")
+    if kind == "decode":
+        out = pplb200.PagedDecodeAttention(cache, rows, 1, 320, scale=float(scale))(q, table[None], cuda.tensor([n], **i32))
+    elif kind == "sparse":
+        out = pplb200.BlockSparseDecodeAttention(pplb200.KeyBlockBounds(cache, 16), rows, 1, 320, 1, 1, 30, scale=float(scale))(q, table[None], cuda.tensor([n], **i32))
+    else:
+        att = pplb200.SharedPrefixDecodeAttention(cache, rows, batch, 112, 208, scale=float(scale))
+        out = att(q, table[:13].contiguous(), cuda.tensor([208], **i32), table[13:].expand(batch, -1).contiguous(), cuda.full((batch,), n - 208, **i32))
+    weight = 2.0 ** (step * (at // 3 - (n - 1) // 3).double())
+    weight /= weight.sum()
+    want, size = weight @ vr[:, 0], weight @ vr[:, 0].abs()
+    assert bool(((out.double() - want).abs() <= want.abs() * HALF + size * (HALF * (group > 0) + 2.0 ** -14) + 2 * TINY).all())
