@@ -176,7 +176,7 @@ int32_t pplb200_paged_decode_attention_fp16(pplb200_stream_t stream, const pplb2
  * batch.  prefix->pages int32 [prefix->num_pages], prefix->length int32 [1], both on the device: how many tokens (at most num_pages * page_size are
  * looked at); pages that are not in the cache are holes.  A sequence with a length of 0 sees the prefix alone; a negative length stands for a row that is
  * no sequence: zeros and -inf, whatever its q.  As above otherwise, but window has to be 0, at most 2^24 rows of q (batch * q_heads), and over the prefix
- * the softmax's weights enter their product with v with 11 bits over an fp16 cache (22 over int8 ones), and v of int8 rows may be rounded to fp16 as that of groups is.
+ * the softmax's weights enter their product with v with 11 bits over an fp16 cache (22 over int8 ones).
  * ws: pplb200_shared_prefix_attention_workspace_bytes(), which holds for smaller batches too, with the rules above.
  */
 typedef struct pplb200_shared_prefix {

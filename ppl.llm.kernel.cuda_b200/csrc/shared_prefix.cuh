@@ -14,14 +14,15 @@
 // half of the tensor memory, over two buffers of scores).
 //
 // Bound by the tensor cores and the exponentials: a block of 128 tokens of two tiles of heads of 128 is 2048 clocks of either.  64 sequences of 64 heads over 8 with 100
-// tokens each behind 32768: fp16 88 us, 780 TFLOP/s (1270 for the 20000 tokens from 12345 on; with the products alone the call took 71 us, then of 93), int8 rows 138
-// and groups of 8 160: there the loading warps widen every element, for each tile or pair of tiles, and groups' keys are two operands.  What a call takes besides,
+// tokens each behind 32768: fp16 88 us, 780 TFLOP/s (1270 for the 20000 tokens from 12345 on; with the products alone the call took 71 us, then of 93), int8 rows 128
+// and groups of 8 160: there the loading warps widen every element, for each tile or pair of tiles, the weights are two operands, and groups' keys too.  What a call takes besides,
 // 10 to 30 us, is the start, q, the parts' sums (64 KB a tile and part) and their joining, and own tokens that do not fit beside it.
 // Tried on fp16 and left, since none changed a block's time: two softmax groups a tile, half of the exponentials as polynomials of degree 3 to 5, looking whether the reference
 // exponent has to move after the weights instead of before them.
-// Weights are fp16 of 2^-24 to 2^14, over an fp16 cache 11 bits, off by at most 2^-11 of themselves, as much as the output's own rounding; their sum is of what they were.  v of int8 caches is
-// rounded to fp16 itself, and the two errors came to half as much again as the output's: there the weights are two operands, 22 bits (48 sequences of 64 heads over
-// 8 behind 4000 tokens of int8 rows: 53 us instead of 50, relative error 0.00028 instead of 0.00031; the output's rounding alone 0.00021).
+// Weights are fp16 of 2^-24 to 2^14, over an fp16 cache 11 bits, off by at most 2^-11 of themselves, as much as the output's own rounding; their sum is of what they were.  v of groups of 8 is
+// rounded to fp16 itself, and the two errors came to half as much again as the output's: over int8 caches the weights are two operands, 22 bits.  v of rows is whole numbers, and
+// its scales are in the weights, so that any finite scale is taken, as by decode attention, and nothing but the output is rounded to fp16 (relative error 0.00021, 2-norm).
+// The code of the softmax is long: where a form of it is only there for rare blocks, it is a loop (unrolled four times, the whole call took 2.7 us longer, in fetching instructions).
 #pragma once
 
 #include "paged_attention.cuh"
@@ -52,7 +53,7 @@ struct Tile {
     static constexpr int Q_BYTES = 128 * DP * 2, V_BYTES = NB * DP * 2, K_BYTES = V_BYTES * (LOW ? 2 : 1);
     static constexpr int RING = TILES * Q_BYTES, V_RING = RING + KS * K_BYTES, INFO = V_RING + VS * V_BYTES;
     static constexpr int INFOS = 8; // blocks whose masks and scales are kept: more than stages of values
-    static constexpr int SCALES = KIND == CACHE_I8_ROWS ? INFOS * NB * 2 : 0; // of keys
+    static constexpr int SCALES = KIND == CACHE_I8_ROWS ? INFOS * NB * 6 : 0; // of keys, in 32 bits, and of values
     // What is read back of the sums lies over the rings and q, behind the sums that the two groups of one tile exchange (tiles' sums and these are not there at
     // the same time, and one tile's are half as long).
     static constexpr int STAGED_BYTES = STREAMS * 128 * (D + 4) * 4, EXCHANGE = STREAMS == 2 ? D * 512 : 0, ONE_TILE = EXCHANGE + 128 * (D + 4) * 4;
@@ -61,8 +62,10 @@ struct Tile {
     static constexpr int CH = D * ES / 16, LOADS = CH * NB / 128; // pieces of 16 bytes: of a row, and of a block for a thread
     static_assert(CH * NB % 128 == 0 && VS < INFOS);
     static constexpr int THREADS = 640;
-    // Registers of softmax, loading and issuing threads: what 640 threads are launched with, 96 each.
-    static constexpr int R_SOFTMAX = KIND == CACHE_F16 ? 176 : 152, R_LOAD = KIND == CACHE_F16 ? 48 : 72, R_ISSUE = 32;
+    // Registers of softmax, loading and issuing threads: what 640 threads are launched with, 96 each.  (int8 rows of 256: with 152 and 72 its loading warps spill, 64 sequences of 32 heads over 8
+    // behind 32768 tokens 139 us, 125 with 160 and 64; of 128 the other way round, 105 and 109.)
+    static constexpr bool LEAN = KIND == CACHE_I8_ROWS && D == 256;
+    static constexpr int R_SOFTMAX = KIND == CACHE_F16 ? 176 : LEAN ? 160 : 152, R_LOAD = KIND == CACHE_F16 ? 48 : LEAN ? 64 : 72, R_ISSUE = 32;
     static constexpr int KEPT = KIND == CACHE_F16 ? NB : NB / 2; // scores of a row that a softmax thread keeps
     static_assert(2 * R_SOFTMAX + 2 * R_LOAD + R_ISSUE <= 5 * 96);
     static constexpr uint32_t O_COLUMN = 256; // scores: columns 0 and 128
@@ -89,6 +92,8 @@ struct PrefixParams {
 // Descriptors of rows of 128 bytes with the 128-byte swizzle: K-major (ptx::desc_lo_sw128), or MN-major, 64 dimensions wide, the next 64 `apart` bytes on.
 __device__ __forceinline__ uint32_t mn_desc_lo(uint32_t addr, uint32_t apart) { return ((addr & 0x3ffffu) >> 4) | (apart >> 4 << 16); }
 
+// How large a scale is: less than 2^size, -24 to 16.  (An infinite one: as large as a finite one can be.)
+__device__ __forceinline__ int32_t size_of(float scale) { return max(-24, min(16, (int32_t)(__float_as_uint(scale) >> 23 & 0xffu) - 126)); }
 // 16 bytes of int8 as fp16, whole numbers, in order
 __device__ __forceinline__ void whole_numbers(const uint4& raw, uint32_t (&o)[8]) {
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -111,6 +116,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
     };
     __shared__ Row row_at[2][4][T::NB]; // keys and values, of four blocks
     __shared__ float2 joint[128];
+    __shared__ __align__(16) int2 sizes[T::KIND == CACHE_I8_ROWS ? T::INFOS : 1][T::NB / 32]; // of the scales of 32 values: the largest and the least
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t smem = (ptx::smem_addr(raw_smem) + 1023u) & ~1023u;
     auto bar = [](uint64_t& b) { return ptx::smem_addr(&b); };
@@ -212,7 +218,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
         // two, and what the softmax has to know is published one ahead.
         int32_t page = -1;
         bool there = false;
-        uint32_t scale = 0; // fp16
+        uint32_t scale = 0, value_scale = 0; // fp16
         auto request = [&](int32_t j) {
             const int32_t token = (block0 + j) * T::NB + id;
             page = -1;
@@ -229,7 +235,10 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
             }
             if (id < T::NB) row_at[values][j & 3][id] = to;
             if constexpr (T::KIND == CACHE_I8_ROWS)
-                if (!values) scale = load_scales<1>(to.scale);
+                if (!values) {
+                    scale = load_scales<1>(to.scale);
+                    value_scale = load_scales<1>(there ? to.scale + ((const char*)p.cache.v_scale - (const char*)p.cache.k_scale) : to.scale); // (strides are those of the keys')
+                }
         };
         auto publish = [&](int32_t j) { // to the softmax: by the keys' threads
             const int slot = j % T::INFOS;
@@ -237,7 +246,14 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
             if (values) return;
             if (lane == 0) masks[slot][id >> 5] = id < T::NB ? mask : 0xffffffffu;
             if constexpr (T::KIND == CACHE_I8_ROWS)
-                if (id < T::NB) reinterpret_cast<uint16_t*>(raw_smem + (smem - ptx::smem_addr(raw_smem)) + T::INFO)[slot * T::NB + id] = (uint16_t)scale;
+                if (id < T::NB) {
+                    uint8_t* const to = raw_smem + (smem - ptx::smem_addr(raw_smem)) + T::INFO + slot * 6 * T::NB;
+                    reinterpret_cast<float*>(to)[id] = __half2float(__ushort_as_half((unsigned short)scale)) * p.scale_log2;
+                    reinterpret_cast<uint16_t*>(to + 4 * T::NB)[id] = (uint16_t)value_scale;
+                    const int32_t size = size_of(__half2float(__ushort_as_half((unsigned short)value_scale)));
+                    const int32_t most = __reduce_max_sync(0xffffffffu, there ? size : -24), least = __reduce_min_sync(0xffffffffu, there ? size : 16);
+                    if (lane == 0) sizes[slot][id >> 5] = make_int2(most, least);
+                }
             report(bar(info_full[slot]));
         };
         const int barrier_id = values ? 3 : 1;
@@ -356,12 +372,11 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
             }
         } else {
             uint4 w[T::LOADS];
-            uint32_t scales[T::LOADS];
+            uint32_t scales[T::LOADS]; // CACHE_I8_GROUPS
             auto fetch = [&](int32_t j, int i) {
                 const Row row = row_at[values][j & 3][token_of(i)];
                 w[i] = ld_global_16(row.at + piece_of(i) * 16);
                 if constexpr (T::KIND == CACHE_I8_GROUPS) scales[i] = load_scales<2>(row.scale + piece_of(i) * 4);
-                else if (values) scales[i] = load_scales<1>(row.scale);
             };
             // into its place, and each piece's successor of the next block is requested
             auto put = [&](uint32_t dst, int32_t next) {
@@ -378,11 +393,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                             r[x] = h2(__hfma2(as_h2(o[x]), f, __hneg2(h)));
                             o[x] = h2(h);
                         }
-                    } else if (values) { // (keys' scales go into the scores)
-                        const __half2 f = as_h2(__byte_perm(scales[i], 0, 0x1010));
-#pragma unroll
-                        for (int x = 0; x < 8; ++x) o[x] = h2(__hmul2(as_h2(o[x]), f));
-                    }
+                    } // (rows' scales go into the scores and the weights)
                     // (eight threads meet the banks twice; a store the other way round for every second 64 dimensions costs more instructions than that time)
                     const uint32_t c = 2 * piece_of(i), a = dst + place(token_of(i), c), b = dst + place(token_of(i), c + 1);
                     ptx::st_shared_v4(a, make_uint4(o[0], o[1], o[2], o[3]));
@@ -447,25 +458,34 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                 ptx::tc_fence_after();
                 const uint32_t at = tmem + lanes + (i & 1) * 128;
                 // Where registers hold half of the scores (KEPT), the others are looked at for the largest and loaded again when the first half's weights are on their way.
-                constexpr int HALF = T::NB / 2, KEPT = T::KEPT;
+                constexpr int HALF = T::NB / 2, KEPT = T::KEPT, ROLL = T::KIND == CACHE_I8_ROWS ? 1 : 2;
                 const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+                // CACHE_I8_ROWS: keys' scales times scale_log2 in 32 bits, values' as they are (with both as they are, 64 x 32768 tokens took 137 us; 128 so).
+                const uint8_t* const scales_at = raw_smem + (smem - ptx::smem_addr(raw_smem)) + T::INFO + slot * 6 * T::NB;
+                auto scales_of = [&](int c, auto use) { // of values c to c + 31
+                    const uint4* const from = reinterpret_cast<const uint4*>(scales_at + 4 * T::NB + c * 2);
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8) {
+                        const uint4 f = from[k / 8];
+                        const uint32_t f4[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) use(k + 2 * y, __half22float2(as_h2(f4[y])));
+                    }
+                };
                 const uint4 mask4 = *reinterpret_cast<const uint4*>(masks[slot]);
                 met |= (mask4.x | mask4.y | (T::NB == 128 ? mask4.z | mask4.w : 0u)) != 0;
                 const bool whole = (mask4.x & mask4.y & mask4.z & mask4.w) == 0xffffffffu;
                 // Of tokens c to c + 31, rounded to 32 bits here: fused with the reference exponent's subtraction below, which takes half an instruction less, scores from 2^27 on
                 // would differ from the largest, which is rounded, by more than a weight has room for.
                 auto score = [&](const uint32_t (&bits)[32], float (&x)[32], int c) {
-                    if constexpr (T::KIND == CACHE_I8_ROWS) { // the scales of 32 keys, read as they are: in 32 bits they would take half of the shared memory's time
-                        const uint4* const ks = reinterpret_cast<const uint4*>(raw_smem + (smem - ptx::smem_addr(raw_smem)) + T::INFO) + (slot * T::NB + c) / 8;
+                    if constexpr (T::KIND == CACHE_I8_ROWS) {
+                        const float4* const from = reinterpret_cast<const float4*>(scales_at + c * 4);
 #pragma unroll
-                        for (int k = 0; k < 32; k += 8) {
-                            const uint4 f = ks[k / 8];
-                            const uint32_t f4[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-                            for (int y = 0; y < 4; ++y) {
-                                const float2 u = ptx::mul2(make_float2(__uint_as_float(bits[k + 2 * y]), __uint_as_float(bits[k + 2 * y + 1])), ptx::mul2(__half22float2(as_h2(f4[y])), scale2));
-                                x[k + 2 * y] = u.x; x[k + 2 * y + 1] = u.y;
-                            }
+                        for (int k = 0; k < 32; k += 4) {
+                            const float4 f = from[k / 4];
+                            const float2 u = ptx::mul2(make_float2(__uint_as_float(bits[k]), __uint_as_float(bits[k + 1])), make_float2(f.x, f.y));
+                            const float2 v = ptx::mul2(make_float2(__uint_as_float(bits[k + 2]), __uint_as_float(bits[k + 3])), make_float2(f.z, f.w));
+                            x[k] = u.x; x[k + 1] = u.y; x[k + 2] = v.x; x[k + 3] = v.y;
                         }
                     } else {
 #pragma unroll
@@ -484,13 +504,28 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                 float high[8];
 #pragma unroll
                 for (int y = 0; y < 8; ++y) high[y] = -INFINITY;
+                // CACHE_I8_ROWS: a value's scale goes into its weight (the sum of the weights is without it), and its size into what decides about the reference exponent.  Where the block's
+                // scales are much alike, the largest size stands for all; else each counts for itself, so that a large scale takes no bits from what weighs more.
+                int32_t most = 0;
+                bool alike = true;
+                if constexpr (T::KIND == CACHE_I8_ROWS) {
+                    int32_t least = 16;
+                    most = -24;
+#pragma unroll
+                    for (int w = 0; w < T::NB / 32; ++w) {
+                        const int2 of = sizes[slot][w];
+                        most = max(most, of.x);
+                        least = min(least, of.y);
+                    }
+                    alike = most - least <= 4;
+                }
                 auto look = [&](const float (&x)[32]) {
 #pragma unroll
                     for (int k = 0; k < 32; k += 16)
 #pragma unroll
                         for (int y = 0; y < 8; ++y) high[y] = fmaxf(high[y], fmaxf(x[k + y], x[k + 8 + y]));
                 };
-#pragma unroll
+#pragma unroll ROLL
                 for (int c = KEPT; c < T::NB; c += 32) {
                     uint32_t bits[32];
                     float x[32];
@@ -511,11 +546,25 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                         look(s[c / 32]);
                     }
                 }
+                if (T::KIND == CACHE_I8_ROWS && !alike) {
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) high[y] = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < T::NB; c += 32) {
+                        uint32_t bits[32];
+                        float x[32];
+                        ptx::tmem_ld_32x32(at + c, bits);
+                        ptx::tmem_ld_wait();
+                        score(bits, x, c);
+                        scales_of(c, [&](int k, float2 f) { x[k] += (float)size_of(f.x), x[k + 1] += (float)size_of(f.y); });
+                        look(x);
+                    }
+                }
 #pragma unroll
                 for (int y = 4; y > 0; y >>= 1)
 #pragma unroll
                     for (int k = 0; k < y; ++k) high[k] = fmaxf(high[k], high[k + y]);
-                const float m = high[0];
+                const float m = high[0] + (T::KIND == CACHE_I8_ROWS && alike ? (float)most : 0.0f);
                 // The reference exponent moves when a weight would pass 2^14, each row's for itself, and then to kAbove above the largest score: some row of 32 meets a score
                 // 2^6 times as heavy again and again where keys have a few large dimensions.  The largest weight is 2^4 at least; those below 2^-18 of it lose bits.
                 const bool higher = m - top > 6.0f; // (top + 6 may be rounded to top + 8)
@@ -545,17 +594,23 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                 float2 sums[2] = {};
                 auto weigh = [&](const float (&x)[32], int c) { // weights of tokens c to c + 31 into their place
                     uint32_t w[16], low[T::FINE ? 16 : 1];
-#pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
+                    auto pair = [&](int k, float2 f) {
                         float2 e = ptx::add2(make_float2(x[k], x[k + 1]), reference);
                         e.x = exp2_fast(e.x);
                         e.y = exp2_fast(e.y);
                         sums[k >> 1 & 1] = ptx::add2(sums[k >> 1 & 1], e);
+                        if constexpr (T::KIND == CACHE_I8_ROWS) e = ptx::mul2(e, f);
                         w[k / 2] = h2(__floats2half2_rn(e.x, e.y));
                         if constexpr (T::FINE) {
                             const float2 high = __half22float2(as_h2(w[k / 2]));
                             low[k / 2] = h2(__floats2half2_rn(e.x - high.x, e.y - high.y));
                         }
+                    };
+                    if constexpr (T::KIND == CACHE_I8_ROWS) {
+                        scales_of(c, pair);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2) pair(k, float2());
                     }
                     ptx::tmem_st_32x16(T::FINE ? at + c : at + c / 2, w);
                     if constexpr (T::FINE) ptx::tmem_st_32x16(at + c + 16, low);
@@ -569,7 +624,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                         report(bar(weight_half[i & 1]));
                     }
                 }
-#pragma unroll
+#pragma unroll ROLL
                 for (int c = KEPT; c < T::NB; c += 32) {
                     uint32_t bits[32];
                     float x[32];

@@ -3,7 +3,8 @@ steps."""
 import numpy as np
 import pytest
 
-from test_attention_gpu import HALF, TINY, _cache, _gen, _randn, _stored
+from test_attention_gpu import HALF, TINY, _attention, _cache, _gen, _randn, _rows, _stored
+from test_long_context_gpu import _run_prefix
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +79,60 @@ def test_scores_that_rise_by_what_32_bits_resolve(cuda, pplb200, kind, group, si
     weight /= weight.sum()
     want, size = weight @ vr[:, 0], weight @ vr[:, 0].abs()
     assert bool(((out.double() - want).abs() <= want.abs() * HALF + size * (HALF * (group > 0) + 2.0 ** -14) + 2 * TINY).all())
+
+
+# ---- scales of an int8 cache ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("prefix,batch", [(500, 24), (500, 1), (9000, 2), (9000, 40)])
+@pytest.mark.parametrize("q_scale", [0.5, 20.0])
+def test_prefix_of_rows_of_any_finite_scale(cuda, pplb200, prefix, batch, d, q_scale):
+    """Values whose product with their scale fp16 does not hold, on the way from 2^-24 to 65504, of either sign: by tiles and by the decode kernel, whatever the number of rows."""
+    g, page, own, hq, hk = _gen(cuda, 7), 16, 32, 8, 2
+    n, pages = prefix + batch * own, -(-prefix // page) + batch * own // page
+    cache = _cache(cuda, pplb200, pages, page, hk, d, d, "heads", 0)
+    pplb200.kv_cache_write(cache, _randn(cuda, g, pages * page, hk, d), _randn(cuda, g, pages * page, hk, d), cuda.arange(pages * page, device="cuda"))
+    size = cuda.exp2(cuda.rand(cache.v_scale.shape, generator=g, device="cuda") * 31 - 24)
+    big = cuda.rand(size.shape, generator=g, device="cuda") < 8 / n  # 127 times 520 and more is beyond fp16; eight of them or so, so that a mean of all stays below
+    size = cuda.where(big, 520.0 + cuda.rand(size.shape, generator=g, device="cuda") * (2000 if q_scale < 1 else 64984), size)
+    cache.v_scale.copy_(size * ((cuda.rand(size.shape, generator=g, device="cuda") < 0.5) * 2 - 1))
+    table = cuda.randperm(pages, generator=g, device="cuda").to(cuda.int32)
+    shared, mine = table[:-(-prefix // page)].contiguous(), table[-(-prefix // page):].view(batch, -1).contiguous()
+    att = pplb200.SharedPrefixDecodeAttention(cache, hq, batch, own, len(shared) * page)
+    q, i32 = _randn(cuda, g, batch, hq, d, scale=q_scale), dict(dtype=cuda.int32, device="cuda")
+    lse = cuda.empty((batch, hq), device="cuda")
+    out = att(q, shared, cuda.tensor([prefix], **i32), mine, cuda.full((batch,), own, **i32), lse=lse)
+    want = []
+    for b in range(batch):
+        token = cuda.arange(prefix, device="cuda")
+        slots = cuda.cat([shared.long()[token // page] * page + token % page, (mine[b].long()[:, None] * page + cuda.arange(page, device="cuda")).flatten()])
+        k, v = _stored(cuda, cache, slots)
+        o, l, bound, lse_bound = _attention(cuda, q[b], k, v, cuda.ones(len(slots), dtype=cuda.bool, device="cuda"), att.scale)
+        # A weight times its scale is the sum of two fp16, the second of which is off by half a step, 2^-25 at least.  The reference exponent is up to 4 above a score and the size of
+        # the scales beside it, of which the least may be 5 below: the largest product is 2^(8 - 4 - 5) or more, so that a token loses 2^-24 of it.
+        s = _rows(cache.v_scale, slots, page).double().abs()[..., 0].repeat_interleave(hq // hk, 1).T
+        p = cuda.softmax(cuda.einsum("hd,thd->ht", q[b].double(), k.repeat_interleave(hq // hk, 1)) * att.scale, -1)
+        bound += 2.0 ** -24 * (p * s).amax(-1, keepdim=True) * (v.abs().repeat_interleave(hq // hk, 1) / s.T[..., None]).sum(0)
+        want.append((o, l, bound, lse_bound))
+    inside = cuda.stack([w[0] for w in want]).abs() < 65000.0
+    assert float(inside.double().mean()) > 0.9
+    for b, (o, l, bound, lse_bound) in enumerate(want):
+        assert bool(((out[b].double() - o).abs() <= bound)[inside[b]].all()), b
+        assert bool(((lse[b].double() - l).abs() <= lse_bound).all()), b
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prefix_of_rows_is_as_exact_as_decode_attention(cuda, pplb200, d):
+    """Whole numbers times weights of 22 bits: no value is rounded.  48 rows of 1000 tokens behind a shared prefix, and by the decode kernel over all."""
+    out, lse, _, (att, call, cache) = _run_prefix(cuda, pplb200, 968, [32] * 24, 8, 2, d, 16, d)
+    rows = lambda table, n: _stored(cuda, cache, (table.long()[:, None] * 16 + cuda.arange(16, device="cuda")).flatten()[:n])  # noqa: E731
+    k, v = rows(call[1], 968)
+    error = []
+    for b in range(24):
+        own = rows(call[3][b], 32)
+        want = _attention(cuda, call[0][b], cuda.cat([k, own[0]]), cuda.cat([v, own[1]]), cuda.ones(1000, dtype=cuda.bool, device="cuda"), att.scale)[0]
+        error.append(((out[b].double() - want), want))
+    # the output's rounding, evenly spread over a step of 2^-11 to 2^-10 of the value: the 2-norm of the errors is 2^-11 / sqrt(3) of the values' at most, 0.00028, and over a whole octave 0.00021
+    # in the mean; a tenth more for the weights' and the sums' roundings
+    off, size = (cuda.stack([e[i] for e in error]).norm() for i in (0, 1))
+    assert float(off / size) < 0.00023
