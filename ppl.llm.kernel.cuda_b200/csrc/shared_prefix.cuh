@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                         const int32_t token = (block0 + j) * T::NB + lane * p.box_rows;
                         return j < blocks && lane < groups && token < n ? p.pages[(uint32_t)((uint64_t)(uint32_t)token * p.page_magic >> p.page_shift)] : -1;
                     };
-                    int32_t next = page_of(0);
+                    int32_t next = page_of(0), issued = 0; // blocks whose barrier `full` tells when they are there
                     for (int32_t j = 0; j < blocks; ++j) {
                         const int32_t now = next, first = (block0 + j) * T::NB, token = first + lane * p.box_rows;
                         next = page_of(j + 1);
@@ -334,7 +334,11 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                             __syncwarp();
                             if (lane == 0) ptx::mbar_arrive(full(stage));
                         }
+                        issued = j + 1;
                     }
+                    // no copy is under way when the CTA leaves, although nobody may have waited for it
+                    for (int32_t j = max(0, issued - stages); j < issued; ++j)
+                        if (!__all_sync(0xffffffffu, ptx::mbar_wait(full(j % stages), (j / stages) & 1, &g_status, ST_LOAD))) break;
                 }
             } else {
                 // one block's pieces on their way while the next one's are issued
@@ -369,6 +373,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                     }
                 }
                 if (ok) settle(blocks);
+                ptx::cp_async_wait<0>();
             }
         } else {
             uint4 w[T::LOADS];
