@@ -1,5 +1,6 @@
 """Builds the sm_100a shared library in-tree, lib/libpplb200_i8i8.so, and (where torch is installed, whose tensors it reads) the
 compiled part of the Python binding, lib/pplb200_attention_binding.<python>.torch-<version>.so: another torch or Python needs another.
+For tests, lib/libpplb200_impatient_prefix.so is built beside them.
 
     python build.py [--force] [--verbose]
 
@@ -20,6 +21,9 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libpplb200_i8i8.so")
 SOURCES = ["capi.cu", "quantize.cu", "rmsnorm_quantize.cu", "activation_requant.cu", "gemm_i8_tcgen05.cu", "gemm_i8_decode.cu", "gemm_i8_token_pair.cu", "tensor_parallel.cu", "p2p_row_parallel.cu", "no_alloc.cu", "rotary_kv.cu", "paged_attention.cu", "paged_attention_general.cu", "shared_prefix.cu", "block_sparse.cu", "probes.cu"]
+# For tests alone: the library with a kernel for shared prefixes in which the warp that issues the products has no patience for the last two tasks' values.
+TEST_LIB = os.path.join(LIBDIR, "libpplb200_impatient_prefix.so")
+TEST_FLAGS = ["-DPPLB200_IMPATIENT_PREFIX"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 BINDING_SOURCE = os.path.join(CSRC, "attention_binding.cpp")
 FLAGS = [
@@ -65,6 +69,9 @@ def build(force=False, verbose=False):
             cmds.append([NVCC] + FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-c", s, "-o", o])
             if verbose:
                 print(" ".join(cmds[-1]))
+    impatient, prefix = os.path.join(LIBDIR, "shared_prefix_impatient.o"), os.path.join(CSRC, "shared_prefix.cu")
+    if force or _stale(impatient, [prefix] + headers):
+        cmds.append([NVCC] + FLAGS + TEST_FLAGS + ["-c", prefix, "-o", impatient])
     with concurrent.futures.ThreadPoolExecutor(os.cpu_count()) as pool:  # files compile side by side
         list(pool.map(lambda cmd: subprocess.run(cmd, check=True), cmds))
     if force or _stale(LIB, objs):
@@ -72,6 +79,9 @@ def build(force=False, verbose=False):
         if verbose:
             print(" ".join(cmd))
         subprocess.run(cmd, check=True)
+    parts = [impatient if os.path.basename(o) == "shared_prefix.o" else o for o in objs]
+    if force or _stale(TEST_LIB, parts):
+        subprocess.run([NVCC, "-shared", "-o", TEST_LIB] + parts + ["-ldl"], check=True)
     home = torch_home()
     if home is None:
         print("torch is not installed: the compiled part of the Python binding (rotary positions, cache, attention) is not built")

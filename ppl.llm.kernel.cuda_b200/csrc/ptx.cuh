@@ -40,14 +40,18 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 // something upstream is broken.
 constexpr long long kWaitCycleLimit = 4000000000LL;
 
-// Waits for the barrier phase with the given parity.  Gives up after the cycle budget:
+// Waits for the barrier phase with the given parity.  Gives up after the cycle budget (a negative one: at once):
 // ORs `code` into *status and returns false, so the caller can unwind instead of hanging.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, unsigned int* status, unsigned int code) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, unsigned int* status, unsigned int code, long long limit = kWaitCycleLimit) {
+    if (limit < 0) {
+        atomicOr(status, code);
+        return false;
+    }
     if (mbar_try_wait(bar, parity)) return true;
     const long long t0 = clock64();
     for (uint32_t spin = 1;; ++spin) {
         if (mbar_try_wait(bar, parity)) return true;
-        if ((spin & 0x3ffu) == 0 && clock64() - t0 > kWaitCycleLimit) {
+        if ((spin & 0x3ffu) == 0 && clock64() - t0 > limit) {
             atomicOr(status, code);
             return false;
         }

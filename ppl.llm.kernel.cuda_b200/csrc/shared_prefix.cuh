@@ -35,6 +35,15 @@ namespace prefix {
 
 using namespace paged;
 
+// How long the warp that issues the products waits for the values of task i.  (Tests of what is left behind a wait that gives up build the kernel with another limit.)
+__device__ __forceinline__ long long value_wait(int32_t i, int32_t tasks) {
+#ifdef PPLB200_IMPATIENT_PREFIX
+    return i >= tasks - 2 ? -1 : ptx::kWaitCycleLimit;
+#else
+    return ptx::kWaitCycleLimit;
+#endif
+}
+
 __device__ unsigned int g_status = 0; // codes of waits that gave up
 __device__ uint4 g_nothing[32]; // zeros: what a token that is not there reads
 constexpr float kAbove = 4.0f; // where a reference exponent goes above the score that moved it
@@ -110,6 +119,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
     extern __shared__ uint8_t raw_smem[];
     __shared__ __align__(8) uint64_t full_k[T::KS], empty_k[T::KS], full_v[T::VS], empty_v[T::VS], info_full[T::INFOS], score_full[2], weight_half[2], weight_full[2], sum_done[2], q_full, all_done, tail_full;
     __shared__ uint32_t tmem_slot;
+    __shared__ volatile uint32_t products_lost; // a wait of the warp that issues them has given up
     __shared__ __align__(16) uint32_t masks[T::INFOS][4]; // (blocks of 64 tokens: two, and two that say that all is there)
     struct __align__(16) Row { // where a token's row and its scales begin
         const char *at, *scale;
@@ -132,7 +142,8 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
         ptx::mbar_init(bar(tail_full), 1);
         for (int i = 0; i < 2; ++i) ptx::mbar_init(bar(score_full[i]), 1), ptx::mbar_init(bar(weight_half[i]), 4), ptx::mbar_init(bar(weight_full[i]), 4), ptx::mbar_init(bar(sum_done[i]), 1);
         ptx::mbar_init(bar(q_full), 8);
-        ptx::mbar_init(bar(all_done), 1);
+        ptx::mbar_init(bar(all_done), 2);
+        products_lost = 0;
         ptx::fence_mbar_init();
     }
     if (warp == 16) {
@@ -182,7 +193,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
             if (tasks > 1) scores(1);
             for (int32_t i = 0; i < tasks && ok; ++i) {
                 const int32_t j = i >> shift, stage = j % T::VS;
-                if (!(ok = __all_sync(0xffffffffu, ptx::mbar_wait(bar(full_v[stage]), (j / T::VS) & 1, &g_status, ST_MMA)))) break;
+                if (!(ok = __all_sync(0xffffffffu, ptx::mbar_wait(bar(full_v[stage]), (j / T::VS) & 1, &g_status, ST_MMA, value_wait(i, tasks))))) break;
                 const uint32_t v = mn_desc_lo(smem + T::V_RING + stage * T::V_BYTES, T::NB * 128);
                 const uint32_t d = tmem + T::O_COLUMN + (T::STREAMS == 2 ? (i & 1) * T::DP : 0), w = tmem + (i & 1) * 128;
                 // the weights of the block's first half are worked with while the others are computed
@@ -201,7 +212,13 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
                 if (tiles == 1 || (i & 1)) ptx::mma_commit_by(bar(empty_v[stage]), leads);
                 if (i + 2 < tasks) scores(i + 2);
             }
-            ptx::mma_commit_by(bar(all_done), leads); // all that was issued
+            // All that was issued, and whether that is all there is: the softmax has scores, and no more to wait for, where only the last tasks' values are missing.
+            if (leads) {
+                if (!ok) products_lost = 1;
+                ptx::mbar_arrive(bar(all_done));
+            }
+            __syncwarp();
+            ptx::mma_commit_by(bar(all_done), leads);
         }
     } else if (warp >= 8) {
         ptx::registers_down<T::R_LOAD>();
@@ -645,7 +662,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
             }
         }
         // ---- the sums ---------------------------------------------------------------------------------------------------------------
-        if (tasks > 0) ok = __all_sync(0xffffffffu, ptx::mbar_wait(bar(all_done), 0, &g_status, ST_SOFTMAX)) && ok;
+        if (tasks > 0) ok = __all_sync(0xffffffffu, ptx::mbar_wait(bar(all_done), 0, &g_status, ST_SOFTMAX)) && ok && !products_lost;
         ptx::tc_fence_after();
         if (met) top = fmaxf(top, kLowest);
         if (!ok) top = sum = __int_as_float(0x7fffffff); // a wait ran out: not a number rather than a wrong one

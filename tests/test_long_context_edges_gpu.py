@@ -1,5 +1,9 @@
 """Attention behind a shared prefix, over chosen blocks and over all tokens, on the GPU, where the usual cases do not go.  Tolerances as in test_attention_gpu.py: sums of half
 steps."""
+import ctypes
+import os
+import struct
+
 import numpy as np
 import pytest
 
@@ -136,3 +140,37 @@ def test_prefix_of_rows_is_as_exact_as_decode_attention(cuda, pplb200, d):
     # in the mean; a tenth more for the weights' and the sums' roundings
     off, size = (cuda.stack([e[i] for e in error]).norm() for i in (0, 1))
     assert float(off / size) < 0.00023
+
+
+# ---- waits that give up ----------------------------------------------------------------------------------------------------
+
+@pytest.fixture(scope="module")
+def impatient(pplb200):
+    """The library in which the warp that issues a prefix's products does not wait for the values of its last two tasks.  Everybody else arrives and waits as ever: the scores of these
+    tasks are there, so that no other wait runs out."""
+    lib = ctypes.CDLL(os.path.join(os.path.dirname(pplb200.LIB_PATH), "libpplb200_impatient_prefix.so"))
+    lib.pplb200_shared_prefix_attention_fp16.argtypes = [ctypes.c_void_p] + [ctypes.c_char_p] * 3
+    lib.pplb200_shared_prefix_attention_status.argtypes = [ctypes.c_int32]
+    return lib
+
+
+@pytest.mark.parametrize("group,d", [(0, 64), (0, 128), (128, 128), (64, 64)])
+@pytest.mark.parametrize("prefix,batch,page", [(100, 24, 16), (3, 40, 16), (2100, 64, 64), (2100, 64, 24), (300, 1, 16)])
+def test_products_that_are_not_all_there_leave_nan(cuda, pplb200, impatient, prefix, batch, page, group, d):
+    """One task of a CTA, two, and several: no finite sum without all of its values."""
+    hq, hk = 64, 8
+    out, lse, _, (att, call, cache) = _run_prefix(cuda, pplb200, prefix, ([5, 0, -1, 40] * batch)[:batch], hq, hk, d, page, group)
+    cuda.cuda.synchronize()
+    lost, lost_lse = cuda.full_like(out, 7.0), cuda.full_like(lse, 7.0)
+    q, shared, length, pages, lengths = call
+    args = struct.pack("=6Q6q2ifi", q.data_ptr(), lost.data_ptr(), lost_lse.data_ptr(), pages.data_ptr(), lengths.data_ptr(), att.ws.data_ptr(), att.ws.numel(), batch, pages.shape[1], pages.stride(0),
+                       q.stride(0), lost.stride(0), hq, 0, att.scale, 0)
+    stream = cuda.cuda.current_stream().cuda_stream
+    impatient.pplb200_shared_prefix_attention_status(1)
+    assert impatient.pplb200_shared_prefix_attention_fp16(stream, cache._args[0], args, struct.pack("=2Qq", shared.data_ptr(), length.data_ptr(), shared.shape[0])) == 0
+    cuda.cuda.synchronize()
+    assert impatient.pplb200_shared_prefix_attention_status(1) == 2 and impatient.pplb200_shared_prefix_attention_status(0) == 0  # the code of the products' warp
+    there = lengths >= 0
+    assert bool(lost[there].isnan().all()) and bool(lost_lse[there].isnan().all())
+    assert not lost[~there].any() and bool((lost_lse[~there] == -float("inf")).all())
+    assert cuda.equal(att(*call), out) and pplb200.shared_prefix_status() == 0  # the workspace is fit for the next call
