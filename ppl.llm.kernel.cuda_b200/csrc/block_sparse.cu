@@ -239,6 +239,7 @@ __global__ void __launch_bounds__(BTPB) key_bounds_read_kernel(const __grid_cons
 // every CTA writes those of its blocks that are above the threshold, and as many of those at it, from the lowest on, as there is room for.
 constexpr int MAX_CLUSTER = 8, BINS = 2048;
 constexpr int64_t MAX_BLOCKS = 1 << 18, MAX_TOTAL = 65536, MAX_ITEMS = 1 << 24;
+constexpr int MOST_SCORES = MAX_BLOCKS / MAX_CLUSTER; // of a CTA: of its share; gathered, or with the blocks' numbers beside them, half as many and as many again
 struct ChoiceParams {
     const half* q;
     int64_t q_stride, pages_stride;
@@ -653,8 +654,8 @@ int32_t launch_choice(cudaStream_t stream, const ChoiceParams& p, int32_t cluste
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    if (cfg.dynamicSmemBytes > 32768) { // beyond what a kernel has without being asked for, its static 11 KB included
-        const cudaError_t e = cudaFuncSetAttribute(choose_blocks_kernel<D, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+    if (cfg.dynamicSmemBytes > 32768) { // beyond what a kernel has without being asked for, its static 11 KB included: always the same, since another thread may be about to launch
+        const cudaError_t e = cudaFuncSetAttribute(choose_blocks_kernel<D, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_SCORES * 4);
         if (e != cudaSuccess) return fail(RC_DEVICE_RUNTIME_ERROR, "choice of blocks: %s", cudaGetErrorString(e));
     }
     cudaLaunchKernelEx(&cfg, choose_blocks_kernel<D, WARPS>, p);
@@ -761,9 +762,9 @@ int32_t pplb200_block_sparse_attention_fp16(pplb200_stream_t stream, const pplb2
     int32_t cluster = 1;
     while (cluster < MAX_CLUSTER && ((p.items * cluster * 2 <= kSms && in_table > 512 && in_table > cluster * 128) || in_table > cluster * 32768LL)) cluster *= 2;
     p.share = (int32_t)std::max<int64_t>(16, (in_table + cluster * 16 - 1) / (cluster * 16) * 16);
-    p.gathered = cluster > 1 && (int64_t)p.share * cluster <= 16384;
+    p.gathered = cluster > 1 && (int64_t)p.share * cluster <= MOST_SCORES / 2;
     p.kept_keys = p.gathered ? p.share * cluster : p.share;
-    p.units_kept = p.share <= 16384;
+    p.units_kept = p.share <= MOST_SCORES / 2;
     const cudaStream_t s = (cudaStream_t)stream;
     const auto launch_dims = [&](auto warps) {
         constexpr int W = decltype(warps)::value;

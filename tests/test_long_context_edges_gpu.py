@@ -3,6 +3,7 @@ steps."""
 import ctypes
 import os
 import struct
+import threading
 
 import numpy as np
 import pytest
@@ -174,3 +175,39 @@ def test_products_that_are_not_all_there_leave_nan(cuda, pplb200, impatient, pre
     assert bool(lost[there].isnan().all()) and bool(lost_lse[there].isnan().all())
     assert not lost[~there].any() and bool((lost_lse[~there] == -float("inf")).all())
     assert cuda.equal(att(*call), out) and pplb200.shared_prefix_status() == 0  # the workspace is fit for the next call
+
+
+# ---- calls of several threads ----------------------------------------------------------------------------------------------
+
+def test_choices_of_several_threads(cuda, pplb200):
+    """Tables that need different amounts of shared memory, on a stream and a workspace each: no thread's launch depends on what another is doing."""
+    cache = _cache(cuda, pplb200, 200, 16, 1, 128, 0, "heads", 0)
+    pplb200.kv_cache_write(cache, _randn(cuda, _gen(cuda, 1), 3200, 1, 128), _randn(cuda, _gen(cuda, 2), 3200, 1, 128), cuda.arange(3200, device="cuda"))
+    bounds = pplb200.KeyBlockBounds(cache, 16)
+    pplb200.key_bounds_update(bounds, cuda.arange(3200, device="cuda"))
+    q, lengths = _randn(cuda, _gen(cuda, 3), 1, 4, 128), cuda.tensor([3200], dtype=cuda.int32, device="cuda")
+    jobs = []
+    for blocks in (9000, 16000, 11000, 200):
+        table = cuda.full((1, blocks), -1, dtype=cuda.int32, device="cuda")
+        table[0, :200] = cuda.arange(200, dtype=cuda.int32, device="cuda")
+        att = pplb200.BlockSparseDecodeAttention(bounds, 4, 1, blocks * 16, 1, 1, 30)
+        jobs.append((att, table, cuda.cuda.Stream(), cuda.empty_like(q)))
+    want = jobs[0][0](q, jobs[0][1], lengths)
+    cuda.cuda.synchronize()
+    failed = []
+
+    def work(att, table, stream, out):
+        try:
+            with cuda.cuda.stream(stream):
+                for _ in range(3000):
+                    att(q, table, lengths, out=out)
+        except Exception as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=job) for job in jobs]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    cuda.cuda.synchronize()
+    assert not failed, failed
+    for _, _, _, out in jobs:
+        assert bool(((out - want).abs().float() <= want.abs().float() * 2 * HALF + 2.0 ** -14).all())  # the order in which parts are joined may differ
