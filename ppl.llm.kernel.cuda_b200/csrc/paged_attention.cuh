@@ -97,6 +97,7 @@ struct AttentionParams {
     int32_t parts;                             // sums of earlier calls that are joined
     bool keep_parts;                           // leave the sums, as part 0
     bool late_wait;
+    uint32_t* ahead;      // word of the workspace: 1 while the kernel that sets it has begun behind its wait and the one behind it has not ended, else 0
     bool whole_items;     // as many CTAs as items, one each
     int64_t whole_tokens; // for items of no more
     int64_t part_rows;                         // rows of a part: query heads of all sequences
@@ -134,6 +135,16 @@ int32_t sms_of_general(AttentionParams& p);
 namespace {
 
 using namespace paged;
+
+// Going ahead of a wait.  What a grid may read behind its wait for the grid before it (lengths, pages, q, the cache) is not promised to be visible to the one after it, which has not
+// waited yet, although that one starts only when all CTAs of the grid between are behind their waits.  So that grid says that it is, with a release, and the one after it looks,
+// with an acquire: what it then finds ordered before that, all that the grid between had waited for, is visible to it too.  Where it does not find the word set, it waits as any other.
+__device__ __forceinline__ void let_go_ahead(uint32_t* word) { asm volatile("st.release.gpu.global.u32 [%0], 1;" ::"l"(word) : "memory"); }
+__device__ __forceinline__ bool may_go_ahead(const uint32_t* word) {
+    uint32_t v;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(word) : "memory");
+    return v == 1;
+}
 
 // A piece of a row, read once: kept out of L1.  volatile: loads stay where they are put, ahead of the work on the tile before.
 template <int BYTES>
@@ -296,13 +307,23 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
     __shared__ int64_t scan[WARPS], ends[2][2];
     __shared__ volatile struct { int64_t all, last_item; int32_t ctas, to_step; } share; // kept out of the registers
     __shared__ int32_t longest[WARPS], is_last;
+    __shared__ bool begun;
     // the warp's number from a shuffle, so that the compiler knows that it is the same in all lanes
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, t = lane & 3;
     const int heads_per_sequence = p.cache.kv_heads * p.tiles;
-    // late_wait: the grid before this one belongs to the same call, all of it had started behind its own wait when this one could, and only the sums that
-    // it leaves are needed from it: where an item's output is written.
-    const bool late = S::GENERAL && p.late_wait;
+    // late_wait: the grid before this one belongs to the same call, and only the sums that it leaves are needed from it: where an item's output is written.
+    bool late = false;
+    if constexpr (S::GENERAL) {
+        if (p.late_wait) {
+            if (threadIdx.x == 0) begun = may_go_ahead(p.ahead);
+            __syncthreads();
+            late = begun;
+        }
+    }
     if (!late) pdl_wait_prior_grid();
+    if constexpr (S::GENERAL) {
+        if (p.ahead && !p.late_wait && blockIdx.x == 0 && threadIdx.x == 0) let_go_ahead(p.ahead);
+    }
     pdl_launch_dependents();
 
     // ---- this CTA's share -----------------------------------------------------------------------------------------------
@@ -352,7 +373,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
         if (whole_items) ctas = (int32_t)items;
         if (blockIdx.x >= ctas) {
             if (late) pdl_wait_prior_grid();
-            return;
+            return; // (not CTA 0)
         }
         if (whole_items) {
             from.b = blockIdx.x / heads_per_sequence;
@@ -968,6 +989,9 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) paged_attention_kernel(co
         if (++hh == heads_per_sequence) hh = 0, ++b;
     }
     if (late) pdl_wait_prior_grid();
+    if constexpr (S::GENERAL) {
+        if (p.late_wait && blockIdx.x == 0 && threadIdx.x == 0) *(volatile uint32_t*)p.ahead = 0; // CTAs that begin from here on wait first, which takes them no time any more
+    }
 }
 
 template <class S>

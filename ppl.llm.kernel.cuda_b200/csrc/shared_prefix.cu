@@ -43,9 +43,10 @@ bool by_decode(int64_t rows, const pplb200_kv_cache& c, int64_t blocks, int32_t 
     return c.quant_group && rows <= kFewRows && blocks > splits * (rows <= 8 ? 1LL : 6LL);
 }
 
-// Workspace: counters of the decode kernel where it goes through the prefix, which have to be zero between calls of whatever sizes; what it needs for the own
+// Workspace: counters of the decode kernel where it goes through the prefix, and behind them the word by which the own tokens' kernel goes ahead of its wait, which have to be zero between calls of
+// whatever sizes; what it needs for the own
 // tokens, which it begins to go through before the other ends; sums over the parts of the prefix, and what the decode kernel needs for few rows' prefix.
-constexpr int64_t kCounters = (3 * kCtas * 8 + 255) / 256 * 256;
+constexpr int64_t kAhead = 3 * kCtas * 8, kCounters = (kAhead + 4 + 255) / 256 * 256;
 // Reference exponents and sums of weights, then sums of values.
 int64_t part_bytes(int64_t sums, int32_t head_dim) { return round_up(sums * 8, 256) + round_up(sums * head_dim * 4, 256); }
 // Sums for up to `rows` of a key head: fewer rows can need more, in more parts.
@@ -157,6 +158,7 @@ int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb
     own.part_rows = rows;
     own.parts = 1;
     own.late_wait = true;
+    own.ahead = (uint32_t*)((char*)a->ws + kAhead);
     lay_out(own, ws, shared);
     const int64_t nb = block_tokens(cache->head_dim), blocks = std::max<int64_t>(1, (tokens + nb - 1) / nb);
     const int32_t tiles = tiles_at_once(a->batch * shared, *cache, blocks), items = (int32_t)(cache->kv_heads * ((a->batch * shared + 128 * tiles - 1) / (128 * tiles)));
@@ -203,6 +205,7 @@ int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb
         p.tiles = tiles; p.items = items; p.splits = splits;
         p.cache = *cache;
         p.part_rows = rows; p.part_tops = own.part_tops; p.part_sums = own.part_sums;
+        p.ahead = own.ahead;
         const int32_t done = launch_prefix((cudaStream_t)stream, p);
         if (done != RC_SUCCESS) return done;
         own.parts = p.splits;

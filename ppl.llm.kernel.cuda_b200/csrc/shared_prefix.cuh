@@ -93,6 +93,7 @@ struct PrefixParams {
     uint32_t rows_magic, rows_shift, page_magic, page_shift;
     float scale_log2;
     pplb200_kv_cache cache;
+    uint32_t* ahead; // what is said to the kernel for the own tokens
     int64_t part_rows;
     float2* part_tops;
     float* part_sums;
@@ -155,6 +156,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) prefix_tile_kernel(const __grid
     ptx::tc_fence_after();
     const uint32_t tmem = tmem_slot;
     pdl_wait_prior_grid();
+    if (blockIdx.x == 0 && threadIdx.x == 0) let_go_ahead(p.ahead);
     pdl_launch_dependents(); // behind the allocation, so that no later kernel has this SM's tensor memory
 
     const int32_t item = blockIdx.x / p.splits, split = blockIdx.x - item * p.splits;

@@ -211,3 +211,63 @@ def test_choices_of_several_threads(cuda, pplb200):
     assert not failed, failed
     for _, _, _, out in jobs:
         assert bool(((out - want).abs().float() <= want.abs().float() * 2 * HALF + 2.0 ** -14).all())  # the order in which parts are joined may differ
+
+
+# ---- chains of steps --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("batch,hq,hk,d,group,prefix", [(16, 8, 8, 128, 0, 2000), (4, 32, 8, 128, 128, 9000), (40, 16, 2, 64, 8, 700), (100, 8, 1, 256, 256, 3000), (2, 4, 4, 96, 0, 200)])
+def test_steps_in_one_captured_chain(cuda, pplb200, batch, hq, hk, d, group, prefix):
+    """Lengths, page tables, positions and the cache are advanced by kernels between the calls of one graph, each call's own tokens' kernel beginning beside its prefix's: what a step gives is what it
+    gives with the device waited for in front of every kernel."""
+    g, page, steps, most = _gen(cuda, 21), 16, 24, 64
+    own = most // page
+    pages = -(-prefix // page) + batch * own
+    table = pplb200.RotaryTable(d)
+    shared = cuda.arange(pages - batch * own, dtype=cuda.int32, device="cuda")
+    every = len(shared) + cuda.randperm(batch * own, generator=g, device="cuda").to(cuda.int32).view(batch, own)
+    rows = _randn(cuda, g, steps, batch, hq + 2 * hk, d)
+    at = cuda.arange(len(shared) * page, device="cuda")
+    k, v = (_randn(cuda, g, len(at), hk, d) for _ in range(2))
+
+    def run(settled):
+        cache = pplb200.PagedKVCache.allocate(pages, page, hk, d, group)
+        cache.v.fill_(1)
+        for t in (cache.k_scale, cache.v_scale) if group else (cache.k, cache.v):
+            t.fill_(float("nan"))  # what is read too early is lost
+        att = pplb200.SharedPrefixDecodeAttention(cache, hq, batch, most, prefix)
+        pages_now, lengths, length = cuda.full_like(every, -1), cuda.zeros(batch, dtype=cuda.int32, device="cuda"), cuda.zeros(1, dtype=cuda.int32, device="cuda")
+        slots, positions = cuda.zeros(batch, dtype=cuda.int64, device="cuda"), cuda.zeros(batch, dtype=cuda.int64, device="cuda")
+        outs, lses = cuda.zeros((steps, batch, hq, d), dtype=cuda.float16, device="cuda"), cuda.zeros((steps, batch, hq), device="cuda")
+        number = cuda.arange(batch, device="cuda")
+
+        def chain():
+            wait = cuda.cuda.synchronize if settled else (lambda: None)
+            lengths.zero_(), pages_now.fill_(-1), length.fill_(prefix - steps)
+            pplb200.kv_cache_write(cache, k, v, at)
+            for i in range(steps):
+                positions.copy_(lengths)
+                pages_now[:, i // page] = every[:, i // page]
+                slots.copy_(every[number, i // page].long() * page + i % page)
+                wait()
+                q = pplb200.rotary_kv_cache_write(cache, rows[i, :, :hq], rows[i, :, hq:hq + hk], rows[i, :, hq + hk:], positions, slots, table)
+                wait()
+                lengths.add_(1), length.add_(1)
+                wait()
+                att(q, shared, length, pages_now, lengths, out=outs[i], lse=lses[i])
+                wait()
+        if settled:
+            chain()
+        else:
+            graph, stream = cuda.cuda.CUDAGraph(), cuda.cuda.Stream()
+            stream.wait_stream(cuda.cuda.current_stream())
+            with cuda.cuda.graph(graph, stream=stream):
+                chain()
+            for _ in range(3):
+                outs.zero_(), lses.zero_()
+                graph.replay()
+        cuda.cuda.synchronize()
+        assert int(att.ws[3 * 592 * 8:3 * 592 * 8 + 4].view(cuda.int32)) == 0  # the word by which the next call's kernel goes ahead
+        return outs, lses
+
+    want, got = run(True), run(False)
+    assert bool(cuda.isfinite(want[0]).all()) and cuda.equal(got[0], want[0]) and cuda.equal(got[1], want[1])
