@@ -148,7 +148,7 @@ int32_t pplb200_kv_cache_read_fp16(pplb200_stream_t stream, const pplb200_kv_cac
  * sequences and 65535 query heads; rows of one head of the cache, and their scales, less than 2^32 times the largest power of two (up to
  * 2^30 bytes) that divides their distances apart.
  * ws: pplb200_paged_decode_attention_workspace_bytes(), 256-byte aligned, zeroed before its first use (every call leaves it fit for the
- * next, of whatever sizes), not shared by calls that may run at the same time (two captured graphs that are replayed at once need
+ * next, of whatever sizes, over a shared prefix or chosen blocks (below) too), not shared by calls that may run at the same time (two captured graphs that are replayed at once need
  * one each).  Where calls have overlapped all the same, their results are void, and the workspace is to be zeroed before a captured call is
  * replayed on it again.
  * The result does not depend on what else is in the batch's other rows beyond the order in which a sequence's parts are summed,

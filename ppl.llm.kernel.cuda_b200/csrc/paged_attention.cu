@@ -72,7 +72,7 @@ void lay_out(AttentionParams& p, void* ws, int64_t shared) {
     p.tiles = (int32_t)((shared + heads - 1) / heads);
     p.call = ++calls;
     p.arrived = (uint64_t*)ws;
-    p.tops = (float2*)((char*)ws + round_up(3 * kCtas * 8, 256));
+    p.tops = (float2*)((char*)ws + kZeros);
     p.sums = (float*)((char*)p.tops + round_up(2 * kCtas * heads * 8, 256));
 }
 

@@ -114,10 +114,13 @@ namespace paged {
 // 96 43 (59).
 inline int heads_at_once(int32_t head_dim, int64_t shared) { return shared > 8 && head_dim <= 128 ? 16 : 8; }
 
-// Bytes of the attention kernel's workspace: three counters and two pieces a CTA at most.
+// A workspace begins with what has to be zero between calls, in one place for all forms of attention and all sizes, so that one workspace serves them in turn: three counters a CTA and (kAhead) the
+// word by which a kernel goes ahead of its wait; then counters once more, of the decode kernel where it goes through a shared prefix while another goes through own tokens.
+constexpr int64_t kAhead = 3 * kCtas * 8, kCounters = (kAhead + 4 + 255) / 256 * 256, kZeros = 2 * kCounters;
+// Bytes of the attention kernel's workspace: behind the zeros, two pieces a CTA at most.
 inline int64_t workspace_bytes(int64_t shared, int32_t head_dim) {
     const int heads = heads_at_once(head_dim, shared);
-    return round_up(3 * kCtas * 8, 256) + round_up(2 * kCtas * heads * 8, 256) + 2LL * kCtas * heads * head_dim * 4;
+    return kZeros + round_up(2 * kCtas * heads * 8, 256) + 2LL * kCtas * heads * head_dim * 4;
 }
 
 // What is wrong with a call's cache and block (the workspace aside), or RC_SUCCESS with the parameters that all forms have in common.

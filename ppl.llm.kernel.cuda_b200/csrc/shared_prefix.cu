@@ -43,10 +43,8 @@ bool by_decode(int64_t rows, const pplb200_kv_cache& c, int64_t blocks, int32_t 
     return c.quant_group && rows <= kFewRows && blocks > splits * (rows <= 8 ? 1LL : 6LL);
 }
 
-// Workspace: counters of the decode kernel where it goes through the prefix, and behind them the word by which the own tokens' kernel goes ahead of its wait, which have to be zero between calls of
-// whatever sizes; what it needs for the own
-// tokens, which it begins to go through before the other ends; sums over the parts of the prefix, and what the decode kernel needs for few rows' prefix.
-constexpr int64_t kAhead = 3 * kCtas * 8, kCounters = (kAhead + 4 + 255) / 256 * 256;
+// Workspace: what the decode kernel needs for the own tokens, which it begins to go through before the prefix's kernel ends; sums over the parts of the prefix, and what the decode
+// kernel needs for few rows' prefix.
 // Reference exponents and sums of weights, then sums of values.
 int64_t part_bytes(int64_t sums, int32_t head_dim) { return round_up(sums * 8, 256) + round_up(sums * head_dim * 4, 256); }
 // Sums for up to `rows` of a key head: fewer rows can need more, in more parts.
@@ -129,7 +127,7 @@ int64_t pplb200_shared_prefix_attention_workspace_bytes(int64_t batch, int32_t q
     if (batch < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0 || batch > kMaxRows / q_heads) return -1;
     const int32_t shared = q_heads / kv_heads;
     const int64_t rows = batch * shared, few = std::min<int64_t>(rows, kFewRows);
-    return kCounters + workspace_bytes(shared, head_dim) +
+    return workspace_bytes(shared, head_dim) +
            std::max(part_bytes(most_sums(rows, kv_heads), head_dim), part_bytes(kv_heads * few, head_dim) + workspace_bytes(few, head_dim));
 }
 
@@ -150,7 +148,7 @@ int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb
         return fail(RC_INVALID_VALUE, "workspace of %lld bytes (256-byte aligned) needed, got %lld", (long long)need, (long long)a->ws_bytes);
     const int32_t shared = a->q_heads / cache->kv_heads;
     const int64_t rows = a->batch * a->q_heads, tokens = prefix->num_pages * cache->page_size;
-    char* const ws = (char*)a->ws + kCounters;
+    char* const ws = (char*)a->ws;
     own.unit_tokens = cache->page_size;
     own.units_per_page = 1;
     own.num_units = own.num_pages;
@@ -158,7 +156,7 @@ int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb
     own.part_rows = rows;
     own.parts = 1;
     own.late_wait = true;
-    own.ahead = (uint32_t*)((char*)a->ws + kAhead);
+    own.ahead = (uint32_t*)(ws + kAhead);
     lay_out(own, ws, shared);
     const int64_t nb = block_tokens(cache->head_dim), blocks = std::max<int64_t>(1, (tokens + nb - 1) / nb);
     const int32_t tiles = tiles_at_once(a->batch * shared, *cache, blocks), items = (int32_t)(cache->kv_heads * ((a->batch * shared + 128 * tiles - 1) / (128 * tiles)));
@@ -189,7 +187,7 @@ int32_t pplb200_shared_prefix_attention_fp16(pplb200_stream_t stream, const pplb
         first.whole_tokens = 0;
         first.keep_parts = true;
         lay_out(first, (char*)own.part_tops + part_bytes(sums, cache->head_dim), a->batch * shared);
-        first.arrived = (uint64_t*)a->ws;
+        first.arrived = (uint64_t*)(ws + kCounters);
         const int32_t done = launch_general((cudaStream_t)stream, first);
         if (done != RC_SUCCESS) return done;
     } else {

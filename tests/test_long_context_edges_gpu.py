@@ -8,8 +8,8 @@ import threading
 import numpy as np
 import pytest
 
-from test_attention_gpu import HALF, TINY, _attention, _cache, _gen, _randn, _rows, _stored
-from test_long_context_gpu import _run_prefix
+from test_attention_gpu import HALF, TINY, _attention, _cache, _gen, _randn, _rows, _run_attention, _stored
+from test_long_context_gpu import _run_prefix, _run_sparse
 
 pytestmark = pytest.mark.gpu
 
@@ -211,6 +211,32 @@ def test_choices_of_several_threads(cuda, pplb200):
     assert not failed, failed
     for _, _, _, out in jobs:
         assert bool(((out - want).abs().float() <= want.abs().float() * 2 * HALF + 2.0 ** -14).all())  # the order in which parts are joined may differ
+
+
+# ---- one workspace ------------------------------------------------------------------------------------------------------------
+
+def test_one_workspace_for_all_forms_of_attention(cuda, pplb200):
+    """As large as the largest of them needs, zeroed once: what a call leaves in it is nothing to the next, whatever that is."""
+    calls = []
+    for d, group in ((128, 128), (64, 0)):
+        for lengths, hq, hk in (([9000, 3, 500], 16, 2), ([20000], 4, 1)):
+            _, _, _, (att, q, table, lens, cache) = _run_attention(cuda, pplb200, lengths, hq, hk, d, 16, group)
+            calls.append((att, (q, table, lens), cache))
+        for prefix, lengths, hq, hk in ((300, [2100] * 5, 4, 1), (9000, [40] * 4, 4, 4), (9000, [3000, 0, 5], 32, 2), (700, [900] * 40, 8, 2)):
+            _, _, _, (att, call, cache) = _run_prefix(cuda, pplb200, prefix, lengths, hq, hk, d, 16, group)
+            calls.append((att, call, cache))
+        _, _, _, (att, q, table, lens, cache, bounds, _) = _run_sparse(cuda, pplb200, [9000, 40, 3000], 8, 2, d, 16, 16, group, 1, 2, 400)
+        calls.append((att, (q, table, lens), cache))
+    want = [att(*call) for att, call, _ in calls]
+    ws = cuda.zeros(max(att.ws.numel() for att, _, _ in calls), dtype=cuda.uint8, device="cuda")
+    for att, _, _ in calls:  # (an object's workspace is its own: a caller of the C functions brings one)
+        args = att._args
+        object.__setattr__(att, "_args", args[:3] + (ws.data_ptr(), ws.numel()) + args[5:])
+    order = list(range(len(calls))) * 3
+    np.random.default_rng(1).shuffle(order)
+    for i in order + order[::-1]:
+        att, call, _ = calls[i]
+        assert cuda.equal(att(*call, out=cuda.full_like(want[i], 7.0)), want[i]), i
 
 
 # ---- chains of steps --------------------------------------------------------------------------------------------------------
