@@ -70,7 +70,7 @@ int32_t pplb200_rotary_fp16(pplb200_stream_t stream, const pplb200_rotary_args* 
  * other, or, with `alternating`, dealt out in turn (axis 0, 1, ..., 0, 1, ...), an axis that has all its planes being passed over.  The planes' frequencies are those of
  * pplb200_rotary_frequencies; with `restart` the n planes of each axis have those of a rotary_dim of 2 n, in order, instead.  axis_of_plane_host (HOST,
  * rotary_dim / 2 bytes) receives the axes; the caller keeps a copy on the device, as of turns_host.
- * The calls: as those with one axis, but positions int64 [axes, tokens], axis_stride elements between axes.  axis_of_plane (device, 4-byte aligned): the
+ * The calls: as those with one axis, but positions int64 [axes, tokens], axis_stride elements between axes: `tokens` or more, or 0 where all axes have the same positions.  axis_of_plane (device, 4-byte aligned): the
  * two lowest bits are looked at, and a number beyond the axes stands for the last one.
  */
 enum { PPLB200_ROTARY_MAX_AXES = 4 };

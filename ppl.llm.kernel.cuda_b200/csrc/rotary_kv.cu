@@ -453,7 +453,8 @@ int32_t take_axes(const pplb200_rotary_axes* axes, int64_t tokens, RotaryKvParam
     if (!axes) return fail(RC_INVALID_VALUE, "null axes");
     if (axes->axes < 1 || axes->axes > PPLB200_ROTARY_MAX_AXES) return fail(RC_UNSUPPORTED, "1 to %d axes, got %d", PPLB200_ROTARY_MAX_AXES, axes->axes);
     if (!axes->axis_of_plane || ((uintptr_t)axes->axis_of_plane & 3)) return fail(RC_INVALID_VALUE, "axis_of_plane must be a 4-byte aligned pointer");
-    if (axes->axis_stride < 0 || (axes->axes > 1 && axes->axis_stride < tokens)) return fail(RC_INVALID_VALUE, "the positions of the axes overlap");
+    if (axes->axis_stride < 0 || (axes->axes > 1 && axes->axis_stride > 0 && axes->axis_stride < tokens)) // 0: all axes have the same, as text among images has
+        return fail(RC_INVALID_VALUE, "the positions of the axes overlap in part");
     p.axis_of_plane = axes->axis_of_plane;
     p.axis_stride = axes->axis_stride;
     p.axes = axes->axes;

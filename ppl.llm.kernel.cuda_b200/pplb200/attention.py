@@ -139,7 +139,7 @@ class RotaryTable(_LaidOutOnce):
 
 def rotary_fp16(q, k, positions, table, interleaved=False, q_out=None, k_out=None):
     """q [tokens, q_heads, head_dim], k [tokens, k_heads, head_dim] fp16 (either may be None) -> both rotated by `positions` (int64
-    [tokens]; [axes, tokens] where the table has several).  q_out=q and k_out=k rotate in place."""
+    [tokens]; [axes, tokens] where the table has several, of text expand(axes, -1) of one row will do).  q_out=q and k_out=k rotate in place."""
     dev, stream = _here()
     if q is not None and q_out is None:
         q_out = torch.empty(q.shape, dtype=_F16, device=q.device)

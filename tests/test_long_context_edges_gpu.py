@@ -297,3 +297,22 @@ def test_steps_in_one_captured_chain(cuda, pplb200, batch, hq, hk, d, group, pre
 
     want, got = run(True), run(False)
     assert bool(cuda.isfinite(want[0]).all()) and cuda.equal(got[0], want[0]) and cuda.equal(got[1], want[1])
+
+
+# ---- positions ----------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens", [1, 5, 3001])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_positions_expanded_over_the_axes(cuda, pplb200, tokens, interleaved):
+    """A token of text has the same position on every axis: one row stands for all, in both calls, bit for bit as the rows written out and as one axis."""
+    g = _gen(cuda, 5)
+    q, k, v = _randn(cuda, g, tokens, 8, 64), _randn(cuda, g, tokens, 2, 64), _randn(cuda, g, tokens, 2, 64)
+    pos, slots = cuda.randint(0, 100000, (tokens,), generator=g, device="cuda"), cuda.arange(tokens, device="cuda")
+    one, table = pplb200.RotaryTable(64), pplb200.RotaryTable(64, axes=(12, 10, 10), alternating=True)
+    caches = [pplb200.PagedKVCache.allocate(-(-tokens // 16), 16, 2, 64, 8) for _ in range(3)]
+    got = [(pplb200.rotary_fp16(q, k, p, t, interleaved), pplb200.rotary_kv_cache_write(c, q, k, v, p, slots, t, interleaved))
+           for c, p, t in zip(caches, (pos.expand(3, -1), pos.expand(3, -1).contiguous(), pos), (table, table, one))]
+    for (qo, ko), qc in got:
+        assert cuda.equal(qo, got[2][0][0]) and cuda.equal(ko, got[2][0][1]) and cuda.equal(qc, qo)
+    for c in caches[:2]:
+        assert cuda.equal(c.k, caches[2].k) and cuda.equal(c.k_scale, caches[2].k_scale)
