@@ -25,8 +25,9 @@ __device__ __forceinline__ bool is_finite(half s) { return (__half_as_ushort(s) 
 // their way.  The lanes that have the same dimensions of different rows halve them between each other at the end, so that all divide and write.  Nothing is
 // shared but these shuffles.
 // In fp16 bound by HBM in a long prompt, the keys once (131072 tokens of 8 heads of 128, blocks of 64: 48 us, 5.6 TB/s), int8 by the minima and maxima, which are
-// in fp32 as the products are, of three numbers at a time (45 us, groups of 8 48; of two numbers 51 and 58; with eight bytes a lane 53 and 59).  16384 tokens: 7.7, 7.1 and
-// 7.8 us; in a decode step look-ups and the launch, 3 us.
+// in fp32 as the products are, of three numbers at a time (45 us, groups of 8 49; of two numbers 51 and 58; with eight bytes a lane 53 and 59).  16384 tokens: 7.7, 7.1 and
+// 7.9 us; in a decode step look-ups and the launch, 3 us.  Four CTAs share an SM over int8: left to itself the compiler takes up to 164 registers, and heads of 256 in groups of 8 98 us
+// instead of 81, of 96 56 instead of 47 (131072 tokens); in fp16, where it takes 80, a bound costs 2 %.
 constexpr int BWARPS = 4, BTPB = 32 * BWARPS;
 struct BoundsParams {
     pplb200_kv_cache cache;
@@ -58,7 +59,7 @@ __device__ __forceinline__ float2 products(uint32_t values, int at, float scale)
 }
 
 template <int D, int KIND>
-__global__ void __launch_bounds__(BTPB) key_bounds_kernel(const __grid_constant__ BoundsParams p) {
+__global__ void __launch_bounds__(BTPB, KIND == CACHE_F16 ? 0 : 4) key_bounds_kernel(const __grid_constant__ BoundsParams p) {
     constexpr int PER = KIND == CACHE_F16 ? 8 : 16, LANES = D / PER;   // dimensions of a lane, and lanes of a row
     constexpr int ROWS = D == 96 ? 24 / LANES : 32 / LANES, BATCH = 8; // rows at once (a power of two); loads on their way
     constexpr int LEFT = PER / ROWS, GROUPS = KIND == CACHE_I8_GROUPS ? PER / 8 : 1;
@@ -122,6 +123,7 @@ __global__ void __launch_bounds__(BTPB) key_bounds_kernel(const __grid_constant_
         } else {
 #pragma unroll
             for (int d = 0; d < PER; ++d) lo[d] = INFINITY, hi[d] = -INFINITY;
+            static_assert(16 % (2 * ROWS) == 0); // two rows at a time
             for (int32_t t = 0; t < p.block; t += BATCH * ROWS) {
                 uint4 w[BATCH];
                 half s[BATCH][GROUPS];
@@ -134,21 +136,14 @@ __global__ void __launch_bounds__(BTPB) key_bounds_kernel(const __grid_constant_
                     }
 #pragma unroll
                 for (int k = 0; k < BATCH; k += 2)
-                    if (t + k * ROWS < p.block) { // both rows, or (16 tokens at eight rows at once: one load) the same one twice
-                        const bool both = t + (k + 1) * ROWS < p.block;
-                        const uint4 second = both ? w[k + 1] : w[k];
-                        const uint32_t words[2][4] = {{w[k].x, w[k].y, w[k].z, w[k].w}, {second.x, second.y, second.z, second.w}};
-                        half scales[2][GROUPS];
+                    if (t + k * ROWS < p.block) { // and the next one with it
+                        const uint32_t words[2][4] = {{w[k].x, w[k].y, w[k].z, w[k].w}, {w[k + 1].x, w[k + 1].y, w[k + 1].z, w[k + 1].w}};
 #pragma unroll
-                        for (int x = 0; x < GROUPS; ++x) {
-                            scales[0][x] = s[k][x];
-                            scales[1][x] = both ? s[k + 1][x] : s[k][x];
-                            bad |= !is_finite(scales[0][x]) || !is_finite(scales[1][x]);
-                        }
+                        for (int x = 0; x < GROUPS; ++x) bad |= !is_finite(s[k][x]) || !is_finite(s[k + 1][x]);
 #pragma unroll
                         for (int d = 0; d < PER; d += 2) {
-                            const float2 a = products(words[0][d >> 2], d & 2, __half2float(scales[0][GROUPS == 1 ? 0 : d / 8]));
-                            const float2 b = products(words[1][d >> 2], d & 2, __half2float(scales[1][GROUPS == 1 ? 0 : d / 8]));
+                            const float2 a = products(words[0][d >> 2], d & 2, __half2float(s[k][GROUPS == 1 ? 0 : d / 8]));
+                            const float2 b = products(words[1][d >> 2], d & 2, __half2float(s[k + 1][GROUPS == 1 ? 0 : d / 8]));
                             lo[d] = least(lo[d], a.x, b.x);
                             hi[d] = greatest(hi[d], a.x, b.x);
                             lo[d + 1] = least(lo[d + 1], a.y, b.y);
