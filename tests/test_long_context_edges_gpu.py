@@ -8,7 +8,7 @@ import threading
 import numpy as np
 import pytest
 
-from test_attention_gpu import HALF, TINY, _attention, _cache, _gen, _randn, _rows, _run_attention, _stored
+from test_attention_gpu import HALF, TINY, _attention, _cache, _check_attention, _gen, _randn, _rows, _run_attention, _stored
 from test_long_context_gpu import _run_prefix, _run_sparse
 
 pytestmark = pytest.mark.gpu
@@ -316,3 +316,28 @@ def test_positions_expanded_over_the_axes(cuda, pplb200, tokens, interleaved):
         assert cuda.equal(qo, got[2][0][0]) and cuda.equal(ko, got[2][0][1]) and cuda.equal(qc, qo)
     for c in caches[:2]:
         assert cuda.equal(c.k, caches[2].k) and cuda.equal(c.k_scale, caches[2].k_scale)
+
+
+# ---- choices among more blocks than the CTAs of a cluster tell each other -----------------------------------------------------
+
+@pytest.mark.parametrize("lengths,hk,first,last,top", [([300000], 1, 1, 2, 40), ([270001, 290000], 1, 0, 1, 3000), ([280000], 2, 5, 3, 17000), ([400000, 7, 262145], 1, 3, 1, 1), ([300000], 1, 0, 1, 18000)])
+def test_sparse_scores_across_a_cluster(cuda, pplb200, lengths, hk, first, last, top):
+    """Over 16384 blocks: every CTA keeps the scores of its own share, and the threshold is found by all together.  Among so many keys some are infinite; their blocks are chosen first, and a
+    head that has one attends to it has NaN by the definition too."""
+    out, lse, want, _ = _run_sparse(cuda, pplb200, lengths, 2 * hk, hk, 64, 16, 16, 0, first, last, top)
+    for b, (o, l, bound, lse_bound) in enumerate(want):
+        lost = o.isnan().any(-1)
+        assert bool(out[b][lost].isnan().all()) and bool(lse[b][lost].isnan().all())
+        _check_attention(out[b:b + 1][:, ~lost], lse[b:b + 1][:, ~lost], [(o[~lost], l[~lost], bound[~lost], lse_bound[~lost])])
+
+
+@pytest.mark.parametrize("top", [1, 300, 5000, 18747])
+def test_sparse_ties_across_a_cluster(cuda, pplb200, top):
+    """Equal scores in all shares but for a few blocks, holes among them: what is at the threshold is taken from the first share on."""
+    def spoil(q, table, cache, bounds):
+        bounds.bounds[:] = bounds.bounds[0, 0, 0]
+        bounds.scales.fill_(1.0)
+        for number, scale in ((40, 0.5), (5000, 2.0), (9999, 0.0), (18000, 2.0), (18001, float("inf"))):
+            bounds.scales[table[0, number].long()] = scale
+        table[0, 7000:7010] = -1
+    _check_attention(*_run_sparse(cuda, pplb200, [300000], 2, 1, 64, 16, 16, 0, 1, 1, top, spoil=spoil)[:3])
