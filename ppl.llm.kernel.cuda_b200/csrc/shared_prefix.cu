@@ -15,20 +15,30 @@ constexpr int64_t kMaxRows = 1 << 24;
 constexpr int32_t block_tokens(int32_t head_dim) { return head_dim == 256 ? 64 : 128; }
 constexpr int32_t most_tiles(int32_t head_dim, bool groups) { return head_dim < 256 && (!groups || head_dim == 64) ? 2 : 1; } // that tensor and shared memory have room for
 
-// Tiles of rows that a CTA takes at once.  Two share what is loaded, and widened, but leave twice as many sums to be joined: where a CTA with one would have many blocks to go
-// through, fewer where a block's products take less than its loads.  64 heads over 8; one and two tiles, us: fp16 heads of 128, 64 sequences, 24 and 64 blocks a CTA, 51, 92 and
-// 54, 88; 128 sequences, 48 blocks, 86 and 86; int8 rows, 24 and 64 blocks, 75, 155 and 71, 138; 16 blocks 57 and 57; fp16 heads of 64, 8 and 24 blocks, 21, 38 and 22, 36.
-int32_t tiles_at_once(int64_t rows, const pplb200_kv_cache& c, int64_t blocks) {
-    const int64_t tiles = (rows + 127) / 128, ctas = std::max<int64_t>(1, kSms / (c.kv_heads * tiles));
-    return most_tiles(c.head_dim, c.quant_group == 8) == 2 && tiles > 1 && (tiles % 2 == 0 || tiles >= 7) && blocks > (c.quant_group == 0 && c.head_dim > 64 ? 40 : 16) * ctas ? 2 : 1;
-}
 // Parts that the prefix is cut into: at most so many that there is a CTA for every SM.
 int32_t most_splits(int64_t items) { return (int32_t)std::max<int64_t>(1, kSms / items); }
+// More are not worth their joining (splits_of).
+int64_t worthwhile_splits(int64_t blocks) { return std::max<int64_t>(8, (int64_t)std::sqrt(8.0 * (double)blocks) + 1); }
+
+// Tiles of rows that a CTA takes at once.  Two share what is loaded, and widened: a block of 128 tokens for both takes 2.04 us where it takes 1.09 for one in fp16 (heads of 64: 1.85 and 0.99),
+// 3.7 and 2.13 over int8, and 2 to 5 of the latter more at the ends, for twice as many sums to be joined.  How many blocks a CTA goes through, and so which is less, depends on how either divides
+// the SMs.  64 heads over 8, 32768 tokens, one tile and two, us: fp16 48 sequences (3 tiles) 62 and 73, 80 (5) 104 and 103, 112 (7) 147 and 144, 144 (9) 160 and 185; int8 rows 104 and 120, 193 and
+// 174, 285 and 254, 287 and 332; 8 heads over one, fp16, 24, 40 and 56 tiles 58, 103, 148 and 61, 92, 122; over 4096 tokens 21, 31, 38 and 24, 31, 38.
+int32_t tiles_at_once(int64_t rows, const pplb200_kv_cache& c, int64_t blocks) {
+    const int64_t tiles = (rows + 127) / 128;
+    if (most_tiles(c.head_dim, c.quant_group == 8) == 1 || tiles == 1) return 1;
+    const auto through = [&](int64_t items) { // blocks of a CTA
+        const int64_t splits = std::min<int64_t>({most_splits(c.kv_heads * items), blocks, worthwhile_splits(blocks)});
+        return (double)((blocks + splits - 1) / splits);
+    };
+    const bool f16 = c.quant_group == 0;
+    return (f16 ? 1.88 : 1.74) * through((tiles + 1) / 2) + (f16 && c.head_dim > 64 ? 5 : 2) < through(tiles) ? 2 : 1;
+}
 // Joining the parts costs about an eighth of a block each, which the square root balances (64 rows of one head, 32768 tokens: 22 us with 46 parts, 41 with 148).  The
 // kernel for the own tokens fills `own_sms` SMs, and where these are left to it, it runs beside this one: up to four blocks a CTA more are worth it
 // (16 rows of 8 heads, 4096 tokens: 13.2 us with 13 parts, 17.8 with 17; 4096 of int8 rows and 700 of their own each: 22.5, 33).
 int32_t splits_of(int64_t items, int64_t own_sms, int64_t blocks, bool* beside = nullptr) {
-    const int64_t all = std::min<int64_t>({most_splits(items), blocks, std::max<int64_t>(8, (int64_t)std::sqrt(8.0 * (double)blocks) + 1)});
+    const int64_t all = std::min<int64_t>({most_splits(items), blocks, worthwhile_splits(blocks)});
     const int64_t spared = std::min(all, (kSms - own_sms) / items);
     const bool spare = spared > 0 && (blocks + spared - 1) / spared <= (blocks + all - 1) / all + 4;
     if (beside) *beside = spare;
@@ -37,7 +47,9 @@ int32_t splits_of(int64_t items, int64_t own_sms, int64_t blocks, bool* beside =
 
 // Few rows of an int8 cache: the decode kernel, whose matrix instructions take 8 or 16 at once, widens with all of its warps, and is faster where a CTA would have several
 // blocks (int8 rows, 8 rows of 8 heads over 1000, 4096 and 32768 tokens: 11.8, 15.7, 28 us, by tiles 12.5, 17.3, 48; 4 of 32 over 1000 13.3 and 17.1; 16 of 8 over 4096, 12345
-// and 32768 19.6, 25, 36 and 17.7, 27, 47; groups of 8 19, 25, 38 and 17, 27, 55.  In fp16 8 rows of 8 heads over 8000 and 32768 18.0, 32.4 and 16.2, 31.2).
+// and 32768 19.6, 25, 36 and 17.7, 27, 47; groups of 8 19, 25, 38 and 17, 27, 55.  Other heads, rows of int8, 8 of 8 over 1000, 4096, 12345 and 32768: of 64 10.7, 12.9, 16.3, 20.4 and
+// 9.6, 11.9, 20.0, 34.8; of 96 11.9, 15.6, 20, 29 and 11.6, 14.2, 24, 40; of 256 15.6, 19.0, 26, 40 and 13.2, 18.4, 35, 63.  In fp16 8 rows of 8 heads over 8000 and 32768
+// 18.0, 32.4 and 16.2, 31.2).
 constexpr int32_t kFewRows = 16;
 bool by_decode(int64_t rows, const pplb200_kv_cache& c, int64_t blocks, int32_t splits) {
     return c.quant_group && rows <= kFewRows && blocks > splits * (rows <= 8 ? 1LL : 6LL);
