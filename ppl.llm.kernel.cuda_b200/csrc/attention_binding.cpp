@@ -375,10 +375,10 @@ PyMethodDef methods[] = {{"rotary", (PyCFunction)(void (*)(void))rotary, METH_FA
                          {"write", (PyCFunction)(void (*)(void))write, METH_FASTCALL, nullptr},
                          {"read", (PyCFunction)(void (*)(void))read, METH_FASTCALL, nullptr},
                          {"attend", (PyCFunction)(void (*)(void))attend, METH_FASTCALL, nullptr},
-                             {"attend_prefix", (PyCFunction)(void (*)(void))attend_prefix, METH_FASTCALL, nullptr},
-                             {"attend_blocks", (PyCFunction)(void (*)(void))attend_blocks, METH_FASTCALL, nullptr},
-                             {"bounds_update", (PyCFunction)(void (*)(void))bounds_update, METH_FASTCALL, nullptr},
-                             {"bounds_read", (PyCFunction)(void (*)(void))bounds_read, METH_FASTCALL, nullptr},
+                         {"attend_prefix", (PyCFunction)(void (*)(void))attend_prefix, METH_FASTCALL, nullptr},
+                         {"attend_blocks", (PyCFunction)(void (*)(void))attend_blocks, METH_FASTCALL, nullptr},
+                         {"bounds_update", (PyCFunction)(void (*)(void))bounds_update, METH_FASTCALL, nullptr},
+                         {"bounds_read", (PyCFunction)(void (*)(void))bounds_read, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "pplb200_attention_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

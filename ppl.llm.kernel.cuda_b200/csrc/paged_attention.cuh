@@ -45,7 +45,9 @@ constexpr int piece(int bytes) { return bytes % 16 == 0 ? 16 : bytes % 8 == 0 ? 
 //
 // GENERAL: what attention over a shared prefix and over chosen blocks ask for besides.  The page table may differ from key head to key
 // head, and its entries be blocks, several to a page; the query rows of an item may be those of several sequences; the sums may be left for a
-// later call in place of the output, or be joined with those that an earlier call has left.
+// later call in place of the output, or be joined with those that an earlier call has left.  Threads and CTAs an SM are those of the plain forms, for which they were measured;
+// what there is besides takes registers that these do not leave, so that 27 of the 42 forms spill 4 to 260 bytes (of the plain ones 14, up to 72): groups of 8, heads of 128, eight query heads,
+// 80, int8 rows of 64 and 96, sixteen, 244 and 260.
 template <int D_, int KIND_, int NT_, bool PACKED_, bool GENERAL_ = false>
 struct Shape {
     static constexpr int D = D_, KIND = KIND_, NT = NT_, HEADS = 8 * NT;
@@ -96,18 +98,14 @@ struct AttentionParams {
     uint32_t rows_magic, rows_shift;
     int32_t parts;                             // sums of earlier calls that are joined
     bool keep_parts;                           // leave the sums, as part 0
-    bool late_wait;
-    uint32_t* ahead;      // word of the workspace: 1 while the kernel that sets it has begun behind its wait and the one behind it has not ended, else 0
-    bool whole_items;     // as many CTAs as items, one each
-    int64_t whole_tokens; // for items of no more
+    bool late_wait;                            // go ahead of the wait for the grid before, if *ahead says so
+    uint32_t* ahead;                           // of the workspace: 1 from when the grid before is behind its own wait until this one is behind it, else 0
+    bool whole_items;                          // as many CTAs as items, one each
+    int64_t whole_tokens;                      // for items of no more
     int64_t part_rows;                         // rows of a part: query heads of all sequences
     float2* part_tops;                         // [parts][part_rows]
     float* part_sums;                          // [parts][part_rows][D]
 };
-
-} // namespace paged
-
-namespace paged {
 
 // Query heads that a CTA takes at once: two blocks of eight where that many share a key-value head and registers allow.  16 sequences of up to
 // 4096 tokens, 128 heads over 8: heads of 128 in fp16 50 us (79 if eight at a time), int8 rows 44 (52), groups of 8 52 (64); of 64 in fp16 31 (40), of
