@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 
 from test_attention_gpu import HALF, TINY, _attention, _cache, _check_attention, _gen, _randn, _rows, _run_attention, _stored
-from test_long_context_gpu import _run_prefix, _run_sparse
+from test_long_context_gpu import _choice, _run_prefix, _run_sparse
 
 pytestmark = pytest.mark.gpu
 
@@ -341,3 +341,102 @@ def test_sparse_ties_across_a_cluster(cuda, pplb200, top):
             bounds.scales[table[0, number].long()] = scale
         table[0, 7000:7010] = -1
     _check_attention(*_run_sparse(cuda, pplb200, [300000], 2, 1, 64, 16, 16, 0, 1, 1, top, spoil=spoil)[:3])
+
+
+# ---- caches of more than 2^32 bytes -------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("group,pages,page", [(0, 36000, 64), (0, 96000, 24), (8, 70000, 64), (128, 70000, 64)])
+@pytest.mark.parametrize("order", ["heads", "tokens"])
+def test_offsets_beyond_32_bits(cuda, pplb200, group, pages, page, order):
+    """A prefix and own tokens on the cache's last pages, by tiles and by the decode kernel; blocks there, their bounds and the choice among them."""
+    d, heads, n = 128, 8, 2000
+    shape = (pages, heads, page) if order == "heads" else (pages, page, heads)
+    make = lambda w, t: cuda.empty(shape + (w,), dtype=t, device="cuda")  # noqa: E731
+    tensors = [make(d, cuda.int8 if group else cuda.float16) for _ in range(2)] + ([make(d // group, cuda.float16) for _ in range(2)] if group else [])
+    assert tensors[0].numel() * tensors[0].element_size() > 1 << 32
+    cache = pplb200.PagedKVCache(*(t if order == "heads" else t.transpose(1, 2) for t in tensors))
+    g, count, i32 = _gen(cuda, 4), -(-n // page), dict(dtype=cuda.int32, device="cuda")
+    table = (pages - 1 - cuda.randperm(2 * count, generator=g, device="cuda")[:count]).to(cuda.int32)
+    table[::3] = cuda.arange(len(table[::3]), **i32)
+    at = cuda.arange(count * page, device="cuda")
+    slots = table.long()[at // page] * page + at % page
+    pplb200.kv_cache_write(cache, _randn(cuda, g, len(at), heads, d), _randn(cuda, g, len(at), heads, d), slots)
+    k, v = _stored(cuda, cache, slots[:n])
+    first = n // 2 // page * page
+    for batch in (2, 20):
+        q = _randn(cuda, g, batch, 16, d)
+        att = pplb200.SharedPrefixDecodeAttention(cache, 16, batch, (count - first // page) * page, first)
+        out = att(q, table[:first // page].contiguous(), cuda.tensor([first], **i32), table[first // page:].expand(batch, -1).contiguous(), cuda.full((batch,), n - first, **i32))
+        _check_attention(out, None, [_attention(cuda, x, k, v, at[:n] >= 0, att.scale, group == 8) for x in q])
+    if page % 16:
+        return
+    bounds = pplb200.KeyBlockBounds(cache, 16)
+    pplb200.key_bounds_update(bounds, slots)
+    q, blocks = _randn(cuda, g, 1, 16, d), cuda.empty((1, heads, 33), **i32)
+    att = pplb200.BlockSparseDecodeAttention(bounds, 16, 1, count * page, 1, 2, 30)
+    out = att(q, table[None], cuda.tensor([n], **i32), blocks=blocks)
+    chosen, parts = _choice(cuda, q[0], bounds, table, n, 1, 2, 30, pages), []
+    for h in range(heads):
+        assert blocks[0, h].tolist() == chosen[h]
+        token = (cuda.tensor(chosen[h], device="cuda")[:, None] * 16 + cuda.arange(16, device="cuda")).flatten()
+        token = token[token < n]
+        parts.append(_attention(cuda, q[0, 2 * h:2 * h + 2], k[token, h:h + 1], v[token, h:h + 1], token >= 0, att.scale, group == 8))
+    _check_attention(out, None, [tuple(cuda.cat(x) for x in zip(*parts))])
+
+
+# ---- layouts of the cache -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("group", [0, 8, 128])
+@pytest.mark.parametrize("layout", ["keys and values side by side", "one head for all", "wider rows", "a window of the pages"])
+def test_layouts_of_the_cache(cuda, pplb200, layout, group):
+    """Strides other than a dense tensor's: the same bits as over a dense copy, whichever way the tokens are brought.  (Rows further apart than long are other forms of the kernels.)"""
+    g, pages, page, heads, d = _gen(cuda, 31), 90, 16, 4, 128
+    wide = {"keys and values side by side": (pages, 2, heads, page), "one head for all": (pages, 2, 1, page), "wider rows": (pages, 2, heads, page), "a window of the pages": (pages + 9, 2, heads, page)}[layout]
+
+    def laid(width, dtype):
+        extra = 32 if layout == "wider rows" else 0
+        t = cuda.randn(wide + (width + extra,), generator=g, device="cuda")
+        t = (t * 40).clamp(-127, 127).to(cuda.int8) if dtype == cuda.int8 else (t.abs() * 0.02 if group else t).to(dtype)
+        out = [t[:, i, ..., :width] for i in (0, 1)]
+        if layout == "one head for all":
+            return [x.expand(-1, heads, -1, -1) for x in out]
+        return [x[4:4 + pages] for x in out] if layout == "a window of the pages" else out
+
+    kv = laid(d, cuda.int8 if group else cuda.float16)
+    scales = laid(d // group, cuda.float16) if group else []
+    caches = [pplb200.PagedKVCache(*kv, *scales), pplb200.PagedKVCache(*(t.contiguous() for t in kv + scales))]
+    i32 = dict(dtype=cuda.int32, device="cuda")
+    table = cuda.randperm(pages, generator=g, device="cuda").to(cuda.int32)
+    exact = layout != "wider rows"
+    for batch, prefix in ((1, 900), (30, 900), (2, 60)):
+        q, own = _randn(cuda, g, batch, 8, d), table[60:].view(1, -1).expand(batch, -1).contiguous()
+        a, b = (pplb200.SharedPrefixDecodeAttention(c, 8, batch, 480, 960)(q, table[:60].contiguous(), cuda.tensor([prefix], **i32), own, cuda.full((batch,), 333, **i32)) for c in caches)
+        assert bool(((a - b).abs().float() <= b.abs().float() * 4 * HALF + 2.0 ** -12).all()) and (cuda.equal(a, b) or not exact)
+    both = [pplb200.KeyBlockBounds(c, 16) for c in caches]
+    at = cuda.arange(pages * page, device="cuda")
+    for b in both:
+        pplb200.key_bounds_update(b, at)
+    assert cuda.equal(both[0].bounds, both[1].bounds) and cuda.equal(both[0].scales, both[1].scales)
+    q, blocks = _randn(cuda, g, 1, 8, d), [cuda.empty((1, heads, 20), **i32) for _ in caches]
+    a, b = (pplb200.BlockSparseDecodeAttention(k, 8, 1, pages * page, 1, 2, 17)(q, table[None], cuda.tensor([1400], **i32), blocks=x) for k, x in zip(both, blocks))
+    assert cuda.equal(*blocks) and bool(((a - b).abs().float() <= b.abs().float() * 4 * HALF + 2.0 ** -12).all()) and (cuda.equal(a, b) or not exact)
+
+
+@pytest.mark.parametrize("group", [0, 8, 128])
+def test_a_cache_without_pages(cuda, pplb200, group):
+    """Every page is a hole: zeros and -inf, blocks chosen from the front."""
+    cache = pplb200.PagedKVCache.allocate(0, 16, 2, 128, group)
+    bounds = pplb200.KeyBlockBounds(cache, 16)
+    i32 = dict(dtype=cuda.int32, device="cuda")
+    pplb200.key_bounds_update(bounds, cuda.arange(64, device="cuda"))
+    lo, hi = pplb200.key_bounds_read(bounds, cuda.arange(-1, 3, device="cuda"))
+    assert not lo.any() and not hi.any()
+    table = cuda.arange(100, **i32)
+    for batch in (1, 40):
+        q, out, lse = _randn(cuda, _gen(cuda, 1), batch, 8, 128), cuda.full((batch, 8, 128), 7.0, dtype=cuda.float16, device="cuda"), cuda.zeros((batch, 8), device="cuda")
+        pplb200.SharedPrefixDecodeAttention(cache, 8, batch, 160, 1600)(q, table, cuda.tensor([1500], **i32), table[:10].expand(batch, -1).contiguous(), cuda.full((batch,), 99, **i32), out=out, lse=lse)
+        assert not out.any() and bool((lse == -float("inf")).all())
+        out.fill_(7.0), lse.zero_()
+        blocks = cuda.empty((batch, 2, 9), **i32)
+        pplb200.BlockSparseDecodeAttention(bounds, 8, batch, 1600, 1, 2, 6)(q, table.expand(batch, -1).contiguous(), cuda.full((batch,), 1590, **i32), out=out, lse=lse, blocks=blocks)
+        assert not out.any() and bool((lse == -float("inf")).all()) and bool((blocks == cuda.tensor([0, 1, 2, 3, 4, 5, 6, 98, 99], **i32)).all())
